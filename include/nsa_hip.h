@@ -517,6 +517,42 @@ int nsa_decode_prep(const void* q, const int64_t* q_stride, const void* k, const
                     const int64_t* v_row_stride, void* k_run_row, const int64_t* k_run_stride, void* v_run_row,
                     const int64_t* v_run_stride, void* stream);
 
+/* Softmax cross entropy of a projection onto a vocabulary, logits = x weight^T, without the logits in memory; its gradients (no counterpart in
+ * the reference, whose Transformer makes all logits for F.cross_entropy: transformer.py:326-330).
+ *   x [rows, dim] with row stride x_stride, weight [vocab, dim] with row stride w_stride, both of `dtype`; labels [rows] contiguous; loss: fp32, one
+ *   value, or [rows] with reduction 0.  Rows whose label is ignore_index count nothing: loss 0 (reduction 0), gradient 0, and what
+ *   they hold is not read.  Any other label outside [0, vocab) makes its loss NaN, and the gradients with it.  Mean of no rows: NaN.
+ *   `state` is written by nsa_loss_fwd and read by nsa_loss_bwd (any number of times); ws is dead after either call.
+ *   dloss: fp32, as loss; dx [rows, dim], dw [vocab, dim] contiguous, of `dtype`; either may be NULL.  rows >= 1 for the backward.
+ * Sums in fp32; fp32 operands as two fp16 halves each (22 bits; what is below 2^-18 of a matrix's largest value is kept to 2^-40 of that), results
+ * rounded once.  The order of the additions depends on sizes and number of counting rows only.  Alignment: that of the type.
+ * rows <= 2^24, dim <= 2^16, vocab <= 2^24 (NSA_E_UNSUPPORTED otherwise). */
+typedef struct nsa_loss_desc {
+  int64_t rows;
+  int32_t dim, vocab;
+  int32_t dtype;        /* 0 bf16, 1 fp16, 2 fp32 */
+  int32_t reduction;    /* 0 none, 1 mean, 2 sum */
+  int32_t labels_int64; /* 1: int64, 0: int32 */
+  int64_t ignore_index, x_stride, w_stride;
+} nsa_loss_desc;
+/* `weight` decides by its alignment whether it is read in place. */
+int nsa_loss_workspace_bytes(const nsa_loss_desc* d, const void* weight, size_t* state_bytes, size_t* fwd_bytes, size_t* bwd_bytes);
+int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* weight, const void* labels, void* state, size_t state_bytes,
+                 void* ws, size_t ws_bytes, float* loss, void* stream);
+int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const void* state, size_t state_bytes, const float* dloss,
+                 void* ws, size_t ws_bytes, void* dx, void* dw, void* stream);
+
+/* Orthogonalised updates (no counterpart in the reference): of each of `many` matrices, X = in / (|in| + eps) with the Frobenius norm, then `steps`
+ * times X <- a X + (b A + c A A) X with A = X X^T (X^T X where there are more rows than columns), written to out.
+ *   rows, cols: host arrays, any sizes up to 2^20, the smaller one up to 2^15; in, out: host arrays of device addresses, rows of in[k] in_stride[k]
+ *   elements apart, out[k] contiguous (aligned to 4 elements where cols[k] % 4 == 0); all of dtype 0 bf16, 1 fp16, 2 fp32.  out[k] may be in[k] where that is
+ *   contiguous.  Products of two fp16 halves (22 bits) with fp32 sums, results rounded once: as exact as fp32 products.
+ *   Coefficients that take a singular value of [0, 1] past 4 on its way: NSA_E_UNSUPPORTED.  Zero matrices give zeros (eps > 0).
+ * The result of a matrix depends on nothing but itself and the sizes of all. */
+int nsa_newton_workspace_bytes(int32_t many, const int32_t* rows, const int32_t* cols, size_t* bytes);
+int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_t* cols, const void* const* in, const int64_t* in_stride, void* const* out,
+                      int32_t dtype, int32_t steps, float a, float b, float c, float eps, void* ws, size_t ws_bytes, void* stream);
+
 /* Same as nsa_select_fwd / nsa_select_bwd, additionally recording the caller's hipEvent_t
  * handles (created with timing enabled) between the kernels of the call, so that a benchmark
  * can time each kernel on the launch stream.  Events: fwd {start, after block walk, after

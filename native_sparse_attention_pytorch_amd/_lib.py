@@ -61,6 +61,13 @@ class QkvDesc(C.Structure):
     ]
 
 
+class LossDesc(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("dim", C.c_int32), ("vocab", C.c_int32), ("dtype", C.c_int32), ("reduction", C.c_int32), ("labels_int64", C.c_int32),
+        ("ignore_index", C.c_int64), ("x_stride", C.c_int64), ("w_stride", C.c_int64),
+    ]
+
+
 _ERR = {-1: "invalid argument", -2: "shape not supported by the compiled kernels", -3: "workspace too small"}
 
 
@@ -174,6 +181,15 @@ def lib():
         for name in ("nsa_dense_workspace_bytes", "nsa_dense_fwd", "nsa_dense_bwd", "nsa_topk", "nsa_topk_prefix", "nsa_gate_fwd", "nsa_gate_bwd"):
             getattr(L, name).restype = C.c_int
         for name in ("nsa_select_workspace_bytes", "nsa_select_build_index", "nsa_select_fwd", "nsa_select_bwd"):
+            getattr(L, name).restype = C.c_int
+        ld = C.POINTER(LossDesc)
+        L.nsa_loss_workspace_bytes.argtypes = [ld, vp, C.POINTER(sz), C.POINTER(sz), C.POINTER(sz)]
+        L.nsa_loss_fwd.argtypes = [ld, vp, vp, vp, vp, sz, vp, sz, vp, vp]
+        L.nsa_loss_bwd.argtypes = [ld, vp, vp, sz, vp, vp, sz, vp, vp, vp]
+        ints, ptrs = C.POINTER(i32), C.POINTER(vp)
+        L.nsa_newton_workspace_bytes.argtypes = [i32, ints, ints, C.POINTER(sz)]
+        L.nsa_newton_schulz.argtypes = [i32, ints, ints, ptrs, s3, ptrs, i32, i32, f32, f32, f32, f32, vp, sz, vp]
+        for name in ("nsa_loss_workspace_bytes", "nsa_loss_fwd", "nsa_loss_bwd", "nsa_newton_workspace_bytes", "nsa_newton_schulz"):
             getattr(L, name).restype = C.c_int
         _lib = L
     return _lib

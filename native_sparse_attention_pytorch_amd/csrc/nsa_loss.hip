@@ -1,0 +1,765 @@
+// Softmax cross entropy of a projection onto a vocabulary, l = x w^T, and its gradients, without the logits in memory.
+//
+//   loss_i = lse_i - l[i][t_i],  lse_i = log sum_v exp l[i][v]
+//   G[i][v] = g_i (exp(l[i][v] - lse_i) - [v == t_i]),  dx = G w,  dw = G^T x
+//
+// Rows whose label is `ignore` are left out of everything: the others are gathered first (their order kept), so work goes by their number,
+// which stays on the device, and what an ignored row holds (a NaN) reaches nothing.
+//
+// Forward: a tile of logits is made with the vocabulary along the registers of a lane and the tokens along the lanes, so a token's maximum
+// and sum over a wave's 64 or 128 logits are a lane's own and one exchange of the wave's halves; the pairs (maximum, sum) of all waves'
+// parts are merged by a second kernel.  Backward, piece by piece of the vocabulary: the logits again, G as fp16 (below), then both products.
+//
+// G in fp16: probabilities and g_i / max |g| are at most 1, so G 2^14 / max |g| has 11 bits down to 2^-28 of the largest, against bf16's 8: with
+// a bf16 G the gradients of a bf16 model were off by 1.4 times their own rounding, with this by 1.01.  The other operands of those
+// products, w and x, are scaled by powers of two into fp16's range and lose nothing that is above 2^-29 of their largest value.
+// fp32 operands are two fp16 planes each, G too (nsa_tiles.hpp).
+#include <algorithm>
+#include "nsa_tiles.hpp"
+#include "../../include/nsa_hip.h"
+
+namespace nsa {
+
+constexpr int kGradBits = 14;
+// device words of a call: rows that count; bits of the largest finite |x|, |w|, |g|
+enum { CELL_ROWS, CELL_X, CELL_W, CELL_G, CELLS = 16 };
+
+struct LossPlan {
+  int n, npad, kp, P;                     // rows and their capacity (a multiple of 64), features padded to 64, planes
+  bool in_place;                          // the forward reads the weight where it lies
+  int fwd_rows, bwd_rows;                 // vocabulary entries of a piece
+  int splits;                             // slices of the vocabulary that dx is summed from
+  bool wide;                              // 256 x 256 tiles
+  bool few;                               // tiles of 32 tokens
+  size_t state, fwd, bwd;                 // bytes
+  size_t s_map, s_place, s_label, s_lse, s_x;                          // offsets in the state
+  size_t f_part, f_target, f_loss, f_w;                                // in the forward's workspace
+  size_t b_cells, b_g, b_x, b_wf, b_wg, b_grad, b_dx;                  // in the backward's
+};
+
+static size_t up(size_t v, size_t to) { return (v + to - 1) / to * to; }
+
+static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
+  if (!d || d->rows < 0 || d->dim <= 0 || d->vocab <= 0 || d->dtype < 0 || d->dtype > 2 || d->reduction < 0 || d->reduction > 2) return NSA_E_ARG;
+  if (d->x_stride < d->dim || d->w_stride < d->dim) return NSA_E_ARG;
+  if (d->rows > (1 << 24) || d->dim > (1 << 16) || d->vocab > (1 << 24)) return NSA_E_UNSUPPORTED;
+  p.n = (int)d->rows;
+  p.npad = (int)up(std::max<size_t>(p.n, 1), 64);
+  p.kp = (int)up(d->dim, 64);
+  p.P = d->dtype == 2 ? 2 : 1;
+  p.in_place = d->dtype != 2 && d->dim % 64 == 0 && d->w_stride % 8 == 0 && d->w_stride < (1 << 20) && ((uintptr_t)weight & 15) == 0;
+  const size_t v256 = up(d->vocab, 256), v64 = up(d->vocab, 64);
+  const size_t row = (size_t)p.P * p.kp * 2;
+  p.few = p.n <= 32;
+  // 256 x 256 tiles where they fill the CUs twice; measured at 8192 rows: see loss_tile_kernel
+  p.wide = !p.few && (v256 / 256) * (((size_t)p.n + 255) / 256) >= 512;
+  p.fwd_rows = (int)std::min(v256, std::max<size_t>(256, ((size_t)256 << 20) / row / 256 * 256));
+  // a piece's G: up to 256 MB
+  p.bwd_rows = (int)std::min(v256, std::max<size_t>(1024, ((size_t)256 << 20) / ((size_t)p.P * p.npad * 2) / 1024 * 1024));
+  const size_t tile = p.wide ? 256 : 128, dx_tiles = up(p.kp, tile) / tile * (up(p.n, tile) / tile);
+  p.splits = (int)std::max<size_t>(1, std::min<size_t>({8, 512 / std::max<size_t>(1, dx_tiles), std::min<size_t>(p.bwd_rows, v64) / 512}));
+  size_t at = CELLS * 4;
+  auto take = [&](size_t bytes) { const size_t here = at; at = up(at + bytes, 256); return here; };
+  at = up(at, 256);
+  p.s_map = take((size_t)p.npad * 4);
+  p.s_place = take((size_t)p.npad * 4);
+  p.s_label = take((size_t)p.npad * 4);
+  p.s_lse = take((size_t)p.npad * 4);
+  p.s_x = take((size_t)p.npad * row);
+  p.state = at;
+  at = 0;
+  p.f_part = take(up(d->vocab, 256) / 32 * (size_t)p.npad * 8 / (p.few ? 1 : p.wide ? 4 : 2));
+  p.f_target = take((size_t)p.npad * 4);
+  p.f_loss = take((size_t)p.npad * 4);
+  p.f_w = take(p.in_place ? 0 : p.fwd_rows * row);
+  p.fwd = at;
+  at = 0;
+  p.b_cells = take(CELLS * 4);
+  p.b_g = take((size_t)p.npad * 4);
+  p.b_x = take(d->dtype == 0 ? (size_t)p.npad * row : 0);
+  p.b_wf = take(p.in_place || d->dtype != 0 ? 0 : p.bwd_rows * row);
+  p.b_wg = take(p.bwd_rows * row);
+  p.b_grad = take((size_t)p.P * p.npad * p.bwd_rows * 2);
+  p.b_dx = take((size_t)p.splits * p.npad * p.kp * 4);
+  p.bwd = at;
+  return 0;
+}
+
+// ------------------------------------------------------------------------------------ rows that count
+
+// map[c] = row of the c-th row that counts, label[c] = its label (-1: outside the vocabulary), place[row] = c or -1.  A work-group takes
+// 1024 rows; how many count before them it finds out itself (8 bytes a row from L2: 4 us at 16384 rows, and no second launch).
+__global__ __launch_bounds__(256) void loss_rows_kernel(const void* labels, int is64, int n, int vocab, long ignore, int* map, int* place, int* label,
+                                                        unsigned* cells, float* losses) {
+  __shared__ int sums[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, first = blockIdx.x * 1024;
+  auto at = [&](int i) { return is64 ? ((const long*)labels)[i] : (long)((const int*)labels)[i]; };
+  int before = 0;
+#pragma unroll 8
+  for (int i = tid; i < first; i += 256) before += at(i) != ignore;
+  long mine[4];
+  int count = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int row = first + 4 * tid + e;
+    mine[e] = row < n ? at(row) : ignore;
+    count += mine[e] != ignore;
+  }
+  int upto = count;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    before += __shfl_xor(before, o);
+    const int other = __shfl_up(upto, o);
+    if (lane >= o) upto += other;
+  }
+  if (lane == 63) { sums[wave] = before; sums[4 + wave] = upto; }
+  __syncthreads();
+  int c = sums[0] + sums[1] + sums[2] + sums[3] + upto - count, total = sums[0] + sums[1] + sums[2] + sums[3];
+  for (int w = 0; w < 4; ++w) {
+    c += w < wave ? sums[4 + w] : 0;
+    total += sums[4 + w];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int row = first + 4 * tid + e;
+    if (row >= n) break;
+    const bool counts = mine[e] != ignore;
+    place[row] = counts ? c : -1;
+    if (counts) {
+      map[c] = row;
+      label[c] = mine[e] >= 0 && mine[e] < vocab ? (int)mine[e] : -1;
+      ++c;
+    } else if (losses != nullptr) {
+      losses[row] = 0.f;
+    }
+  }
+  if (blockIdx.x == gridDim.x - 1 && tid == 0) cells[CELL_ROWS] = (unsigned)total;
+  if (blockIdx.x == 0 && tid >= 1 && tid < CELLS) cells[tid] = 0;
+}
+
+template <class S> __device__ __forceinline__ void load_values(const S* p, int have, bool vec, float (&v)[8]) {
+  if (vec && have >= 8) {
+    if constexpr (sizeof(S) == 4) {
+      const floatx4 a = *reinterpret_cast<const floatx4*>(p), b = *reinterpret_cast<const floatx4*>(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+    } else {
+      const typename PlaneVec<S>::x8 a = *reinterpret_cast<const typename PlaneVec<S>::x8*>(p);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (float)a[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < have ? (float)p[e] : 0.f;
+  }
+}
+
+// bits of the largest finite |value| of a matrix (of the rows that map names, if it is given) into *cell, which is zero or such bits
+template <class S>
+__global__ __launch_bounds__(256) void loss_largest_kernel(const S* src, long ld, int rows, int cols, int vec, const int* map, const unsigned* count, unsigned* cell) {
+  const int live = count != nullptr ? (int)*count : rows;
+  const int per = (cols + 7) / 8;
+  unsigned best = 0;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < (long)live * per; i += (long)gridDim.x * 256) {
+    const int r = (int)(i / per), c = (int)(i % per) * 8;
+    float v[8];
+    load_values(src + (map != nullptr ? map[r] : r) * ld + c, cols - c, vec, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned u = __builtin_bit_cast(unsigned, v[e]) & 0x7fffffffu;
+      best = u < 0x7f800000u ? max(best, u) : best;
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) best = max(best, (unsigned)__shfl_xor((int)best, o));
+  if ((threadIdx.x & 63) == 0 && best != 0) atomicMax(cell, best);
+}
+
+// Rows (named by map, or all) as planes of kp columns, those past `cols` zero; rows past the last one up to a multiple of 64 zero too.
+// cell: the values are scaled below 2^15 by the power of two that suits its magnitude.
+template <class S, class D, int P>
+__global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld, int rows, int cols, int kp, int vec, const int* map, const unsigned* count,
+                                                          const unsigned* cell, D* dst, long plane) {
+  const int live = count != nullptr ? (int)*count : rows, per = kp / 8;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const int r = (int)(i / per), c = (int)(i % per) * 8;
+  if (r >= (live + 63) / 64 * 64) return;
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  if (r < live && c < cols) load_values(src + (map != nullptr ? map[r] : r) * ld + c, cols - c, vec, v);
+  const int shift = cell != nullptr ? plane_shift(*cell) : 0;
+  typename PlaneVec<D>::x8 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = shift != 0 ? __builtin_ldexpf(v[e], shift) : v[e];
+    if constexpr (P == 2) {
+      const Halves s = halves_of(x);
+      hi[e] = s.hi;
+      lo[e] = s.lo;
+    } else {
+      hi[e] = (D)x;
+    }
+  }
+  const long at = (long)r * kp + c;
+  *reinterpret_cast<decltype(hi)*>(dst + at) = hi;
+  if (P == 2) *reinterpret_cast<decltype(lo)*>(dst + plane + at) = lo;
+}
+
+// ------------------------------------------------------------------------------------ tiles of logits
+
+struct LossTileArgs {
+  const void *w, *x;
+  long w_plane, w_ld, x_plane;
+  int kp, vocab, v0, vend;                 // the piece: entries v0 .. vend - 1
+  int n, tiles_m, tiles_n;
+  const unsigned *count, *x_cell, *w_cell;  // cells: null where the planes are not scaled
+  const int* label;
+  float2* part;                            // [parts][npad]
+  float* target;
+  int npad;
+  // backward
+  const float *lse, *g;
+  const unsigned* g_cell;
+  _Float16* grad;                          // [planes][npad][grad_ld]
+  long grad_plane;
+  int grad_ld;
+};
+
+// One tile: TM entries of the vocabulary (registers) by TN tokens (lanes).  GRAD: G of the tile; else its maxima, sums and the labels' logits.
+template <class Tiles, bool GRAD>
+__global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const LossTileArgs G) {
+  typedef typename Tiles::T T;
+  __shared__ __align__(1024) char shared[Tiles::LDS];
+  const TileAt tile = tile_at(blockIdx.x, G.tiles_m, G.tiles_n, 4);
+  const int m0 = G.v0 + tile.m * Tiles::TM, n0 = tile.n * Tiles::TN, live = (int)*G.count;
+  if (n0 >= live) {
+    // rows of G up to a multiple of 64 are read as the contraction index of dw
+    if (GRAD && n0 < (live + 63) / 64 * 64) {
+      const int width = min(Tiles::TM, G.grad_ld - tile.m * Tiles::TM) / 8;
+      for (int i = threadIdx.x; i < Tiles::P * Tiles::TN * width; i += Tiles::THREADS) {
+        const int row = i / width % Tiles::TN, plane = i / width / Tiles::TN;
+        *reinterpret_cast<uintx4*>(G.grad + plane * G.grad_plane + (size_t)(n0 + row) * G.grad_ld + tile.m * Tiles::TM + i % width * 8) = uintx4{0u, 0u, 0u, 0u};
+      }
+    }
+    return;
+  }
+  Tiles t;
+  t.init(shared);
+  t.operand_a((const T*)G.w, G.w_plane, G.w_ld, tile.m * Tiles::TM, G.vend - G.v0);
+  t.operand_b((const T*)G.x, G.x_plane, G.kp, n0, live);
+  t.run(G.kp / Tiles::BK);
+
+  int unscale = 0;
+  if (Tiles::P == 2) unscale = -(plane_shift(*G.x_cell) + plane_shift(*G.w_cell));
+  const bool cut = m0 + Tiles::TM > G.vend;      // entries past the last one
+  constexpr int PART = Tiles::TM / Tiles::WM;
+  const int g_shift = GRAD ? kGradBits - plane_exponent(*G.g_cell) : 0;
+#pragma unroll
+  for (int j = 0; j < Tiles::NI; ++j) {
+    const int token = n0 + t.col_of(j);
+    const bool ok = token < live;
+    const int label = ok ? G.label[token] : -1, own = label - (m0 + t.wm * PART);      // in this wave's part
+    const bool hit = label >= 0 && own >= 0 && own < PART && ((own >> 2) & 1) == (t.lane >> 5);
+    if (Tiles::P == 2) {
+#pragma unroll
+      for (int i = 0; i < Tiles::MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t.acc[i][j][e] = __builtin_ldexpf(t.acc[i][j][e], unscale);
+    }
+    if (!GRAD) {
+      if (cut) {
+#pragma unroll
+        for (int i = 0; i < Tiles::MI; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (m0 + t.row_of(i, e >> 2) + (e & 3) >= G.vend) t.acc[i][j][e] = -INFINITY;
+      }
+      if (__any(hit)) {
+        float found = 0.f;
+#pragma unroll
+        for (int i = 0; i < Tiles::MI; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) found = own == 32 * i + 8 * (e >> 2) + 4 * (t.lane >> 5) + (e & 3) ? t.acc[i][j][e] : found;
+        if (hit) G.target[token] = found;
+      }
+      float top = t.acc[0][j][0];
+#pragma unroll
+      for (int i = 0; i < Tiles::MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, t.acc[i][j][e]);
+      top = halves_max(top);
+      const float from = top > -INFINITY ? top * kLog2e : 0.f;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < Tiles::MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum += fast_exp2(__builtin_fmaf(t.acc[i][j][e], kLog2e, -from));
+      sum = halves_sum(sum);
+      if (ok && t.lane < 32) G.part[(size_t)((m0 / PART) + t.wm) * G.npad + token] = make_float2(top, sum);
+    } else {
+      const int pad = (live + 63) / 64 * 64;
+      const float lse = ok ? G.lse[token] : 0.f, g = ok ? __builtin_ldexpf(G.g[token], g_shift) : 0.f;
+#pragma unroll
+      for (int i = 0; i < Tiles::MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t.acc[i][j][e] = ok ? g * fast_exp2((t.acc[i][j][e] - lse) * kLog2e) : 0.f;
+      if (__any(hit)) {
+#pragma unroll
+        for (int i = 0; i < Tiles::MI; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (hit && own == 32 * i + 8 * (e >> 2) + 4 * (t.lane >> 5) + (e & 3)) t.acc[i][j][e] -= g;
+      }
+      if (cut) {
+#pragma unroll
+        for (int i = 0; i < Tiles::MI; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (m0 + t.row_of(i, e >> 2) + (e & 3) >= G.vend) t.acc[i][j][e] = 0.f;
+      }
+      if (token >= pad) continue;
+      constexpr int GP = Tiles::P;
+#pragma unroll
+      for (int i = 0; i < Tiles::MI; ++i) {
+        const int col = tile.m * Tiles::TM + t.wm * PART + 32 * i;
+        if (col >= G.grad_ld) break;
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          f16x4 hi[2], lo[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = t.acc[i][j][4 * (q + u) + e];
+              if (GP == 2) {
+                const Halves s = halves_of(v);
+                hi[u][e] = s.hi;
+                lo[u][e] = s.lo;
+              } else {
+                hi[u][e] = (_Float16)v;
+              }
+            }
+          _Float16* at = G.grad + (size_t)token * G.grad_ld + col + 8 * q + 8 * (t.lane >> 5);
+          *reinterpret_cast<uintx4*>(at) = join_quads(__builtin_bit_cast(uintx2, hi[0]), __builtin_bit_cast(uintx2, hi[1]));
+          if (GP == 2) *reinterpret_cast<uintx4*>(at + G.grad_plane) = join_quads(__builtin_bit_cast(uintx2, lo[0]), __builtin_bit_cast(uintx2, lo[1]));
+        }
+      }
+    }
+  }
+}
+
+// lse and loss of 8 tokens from the parts' maxima and sums: 32 threads a token
+__global__ __launch_bounds__(256) void loss_merge_kernel(const float2* part, int parts, int npad, const unsigned* count, const int* map, const int* label,
+                                                         const float* target, float* lse, float* loss, float* losses) {
+  __shared__ float top_s[32][8], sum_s[32][8];
+  const int live = (int)*count, tid = threadIdx.x, t8 = tid & 7, p0 = tid >> 3, token = blockIdx.x * 8 + t8;
+  if (blockIdx.x * 8 >= live) return;
+  float top = -INFINITY, sum = 0.f;
+  bool nan = false;
+  if (token < live) {
+#pragma unroll 8
+    for (int p = p0; p < parts; p += 32) {
+      const float2 v = part[(size_t)p * npad + token];
+      nan |= v.y != v.y;
+      const float m = fmaxf(top, v.x);
+      const float at = m > -INFINITY ? m : 0.f;
+      sum = sum * fast_exp2((top - at) * kLog2e) + v.y * fast_exp2((v.x - at) * kLog2e);
+      top = m;
+    }
+  }
+  top_s[p0][t8] = top;
+  sum_s[p0][t8] = nan ? __builtin_nanf("") : sum;
+  __syncthreads();
+  if (tid >= 8 || token >= live) return;
+  float all = -INFINITY, s = 0.f;
+  for (int p = 0; p < 32; ++p) all = fmaxf(all, top_s[p][tid]);
+  const float at = all > -INFINITY ? all : 0.f;
+  for (int p = 0; p < 32; ++p) s += sum_s[p][tid] * fast_exp2((top_s[p][tid] - at) * kLog2e);
+  float l = at + fast_log2(s) * kLn2;
+  if (label[token] < 0) l = __builtin_nanf("");      // no entry of the vocabulary: said by the loss and all gradients
+  const float value = l - (label[token] < 0 ? 0.f : target[token]);
+  lse[token] = l;
+  loss[token] = value;
+  if (losses != nullptr) losses[map[token]] = value;
+}
+
+// the sum of the losses, or their mean (of none: NaN)
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const float* loss, const unsigned* count, int mean, float* out) {
+  __shared__ double sums[16];
+  const int live = (int)*count;
+  double s = 0.0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < live; i += 1024) s += loss[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < 16; ++w) s += sums[w];
+  *out = (float)(mean ? s / live : s);
+}
+
+// ------------------------------------------------------------------------------------ gradients
+
+// g of the rows that count, the bits of their largest finite magnitude, and the other cells cleared
+__global__ __launch_bounds__(1024) void loss_weights_kernel(const float* dloss, int reduction, const unsigned* count, const int* map, float* g, unsigned* cells) {
+  __shared__ unsigned best_s[16];
+  const int live = (int)*count, tid = threadIdx.x;
+  unsigned best = 0;
+  for (int i = tid; i < live; i += 1024) {
+    const float v = reduction == 0 ? dloss[map[i]] : reduction == 1 ? dloss[0] / (float)live : dloss[0];
+    g[i] = v;
+    const unsigned u = __builtin_bit_cast(unsigned, v) & 0x7fffffffu;
+    best = u < 0x7f800000u ? max(best, u) : best;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) best = max(best, (unsigned)__shfl_xor((int)best, o));
+  if ((tid & 63) == 0) best_s[tid >> 6] = best;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < 16; ++w) best = max(best, best_s[w]);
+    cells[CELL_G] = best;
+    cells[CELL_X] = cells[CELL_W] = 0;
+  }
+}
+
+struct LossGradArgs {
+  const _Float16 *grad, *other;       // G [npad][grad_ld]; w [piece][kp] or x [npad][kp]
+  long grad_plane, other_plane;
+  int grad_ld, kp, dim, tiles_m, tiles_n, entries;
+  const unsigned *count, *other_cell, *g_cell;
+  // dx
+  float* sums;                        // [splits][npad][kp]
+  int npad, per, first;               // steps of a split; first piece
+  // dw
+  void* dw;
+  long dw_ld;
+  int vec;
+};
+
+// dx, one slice of the piece's vocabulary: features (registers) by tokens (lanes), unscaled, added to what the pieces before gave
+template <class Tiles>
+__global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dx_kernel(const LossGradArgs G) {
+  __shared__ __align__(1024) char shared[Tiles::LDS];
+  const int tiles = G.tiles_m * G.tiles_n, split = blockIdx.x / tiles;
+  const TileAt tile = tile_at(blockIdx.x % tiles, G.tiles_m, G.tiles_n, 4);
+  const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN, live = (int)*G.count;
+  if (n0 >= live) return;
+  const int from = min(split * G.per, G.grad_ld / Tiles::BK), steps = min(G.per, G.grad_ld / Tiles::BK - from);
+  if (steps <= 0 && !G.first) return;
+  Tiles t;
+  t.init(shared);
+  t.operand_a(G.other, G.other_plane, G.kp, m0, G.kp);
+  t.operand_b(G.grad, G.grad_plane, G.grad_ld, n0, live);
+  t.run(steps, from);
+  // (this piece's power of two: all pieces share it)
+  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.other_cell != nullptr ? plane_shift(*G.other_cell) : 0);
+  float* sums = G.sums + (size_t)split * G.npad * G.kp;
+#pragma unroll
+  for (int j = 0; j < Tiles::NI; ++j) {
+    const int token = n0 + t.col_of(j);
+    if (token >= live) continue;
+#pragma unroll
+    for (int i = 0; i < Tiles::MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int col = m0 + t.row_of(i, q);
+        if (col >= G.kp) continue;
+        floatx4* at = reinterpret_cast<floatx4*>(sums + (size_t)token * G.kp + col);
+        floatx4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_ldexpf(t.acc[i][j][4 * q + e], shift);
+        *at = G.first ? v : *at + v;
+      }
+  }
+}
+
+template <class O> __device__ __forceinline__ void store_quad(O* p, floatx4 v, int have, bool vec) {
+  if (vec) {
+    if constexpr (sizeof(O) == 4) {
+      *reinterpret_cast<floatx4*>(p) = v;
+    } else {
+      typedef __attribute__((__vector_size__(4 * sizeof(O)))) O ox4;
+      ox4 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = (O)v[e];
+      *reinterpret_cast<ox4*>(p) = r;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < have) p[e] = (O)v[e];
+  }
+}
+
+// dw of the piece: features (registers) by entries of the vocabulary (lanes), over all tokens
+template <class Tiles, class O>
+__global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dw_kernel(const LossGradArgs G) {
+  __shared__ __align__(1024) char shared[Tiles::LDS];
+  const TileAt tile = tile_at(blockIdx.x, G.tiles_m, G.tiles_n, 4);
+  const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN, live = (int)*G.count;
+  Tiles t;
+  t.init(shared);
+  t.operand_a(G.other, G.other_plane, G.kp, m0, G.kp);
+  t.operand_b(G.grad, G.grad_plane, G.grad_ld, n0, G.grad_ld);
+  t.run((live + Tiles::BK - 1) / Tiles::BK);
+  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.other_cell != nullptr ? plane_shift(*G.other_cell) : 0);
+#pragma unroll
+  for (int j = 0; j < Tiles::NI; ++j) {
+    const int entry = n0 + t.col_of(j);
+    if (entry >= G.entries) continue;
+    O* row = (O*)G.dw + (size_t)entry * G.dw_ld;
+#pragma unroll
+    for (int i = 0; i < Tiles::MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int col = m0 + t.row_of(i, q);
+        if (col >= G.dim) continue;
+        floatx4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_ldexpf(t.acc[i][j][4 * q + e], shift);
+        store_quad(row + col, v, G.dim - col, G.vec);
+      }
+  }
+}
+
+// dx [n][dim] from the slices; rows that do not count are zero
+template <class O>
+__global__ __launch_bounds__(256) void loss_dx_rows_kernel(const float* sums, int splits, int npad, int kp, int n, int dim, int vec, const int* place, O* dx) {
+  const int per = (dim + 3) / 4;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long)n * per) return;
+  const int row = (int)(i / per), c = (int)(i % per) * 4, at = place[row];
+  floatx4 v = {0.f, 0.f, 0.f, 0.f};
+  if (at >= 0)
+    for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const floatx4*>(sums + ((size_t)s * npad + at) * kp + c);
+  store_quad(dx + (size_t)row * dim + c, v, dim - c, vec);
+}
+
+// ------------------------------------------------------------------------------------ launches
+
+typedef __bf16 B16;
+typedef _Float16 H16;
+template <class T, int P> struct LogitTiles {
+  typedef TileProduct<T, P, ROWS, ROWS, 256, 256, 2, 4, P == 2 ? 32 : 64, 2> Wide;
+  typedef TileProduct<T, P, ROWS, ROWS, 128, 128, 2, 2, P == 2 ? 32 : 64, 2> Small;
+  typedef TileProduct<T, P, ROWS, ROWS, 128, 32, 4, 1, 64, P == 2 ? 2 : 4> Few;
+};
+template <int P> struct GradTiles {
+  typedef TileProduct<H16, P, COLUMNS, ROWS, 256, 256, 2, 4, P == 2 ? 32 : 64, 2> WideX;
+  typedef TileProduct<H16, P, COLUMNS, ROWS, 128, 128, 2, 2, P == 2 ? 32 : 64, 2> SmallX;
+  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 256, 256, 2, 4, P == 2 ? 32 : 64, 2> WideW;
+  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 128, 128, 2, 2, P == 2 ? 32 : 64, 2> SmallW;
+};
+
+template <class Tiles, bool GRAD>
+static void launch_tile(LossTileArgs a, hipStream_t st) {
+  a.tiles_m = (a.vend - a.v0 + Tiles::TM - 1) / Tiles::TM;
+  a.tiles_n = ((GRAD ? a.npad : a.n) + Tiles::TN - 1) / Tiles::TN;
+  hipLaunchKernelGGL((loss_tile_kernel<Tiles, GRAD>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(Tiles::THREADS), 0, st, a);
+}
+template <class T, int P, bool GRAD>
+static void launch_tiles(const LossPlan& p, const LossTileArgs& a, hipStream_t st) {
+  typedef LogitTiles<T, P> L;
+  if (p.few) launch_tile<typename L::Few, GRAD>(a, st);
+  else if (p.wide) launch_tile<typename L::Wide, GRAD>(a, st);
+  else launch_tile<typename L::Small, GRAD>(a, st);
+}
+template <bool GRAD>
+static void logits_tiles(const nsa_loss_desc* d, const LossPlan& p, const LossTileArgs& a, hipStream_t st) {
+  if (d->dtype == 0) launch_tiles<B16, 1, GRAD>(p, a, st);
+  else if (d->dtype == 1) launch_tiles<H16, 1, GRAD>(p, a, st);
+  else launch_tiles<H16, 2, GRAD>(p, a, st);
+}
+
+static unsigned blocks_for(long work) { return (unsigned)std::max<long>(1, (work + 255) / 256); }
+static bool vectors(const void* p, long ld, int each) { return ((uintptr_t)p & 15) == 0 && ld * each % 16 == 0; }
+
+template <class S, class D, int P>
+static void planes(const void* src, long ld, int rows, int rows_cap, int cols, int kp, const int* map, const unsigned* count, const unsigned* cell, void* dst,
+                   long plane, hipStream_t st) {
+  hipLaunchKernelGGL((loss_planes_kernel<S, D, P>), dim3(blocks_for((long)up(rows_cap, 64) * kp / 8)), dim3(256), 0, st, (const S*)src, ld, rows, cols, kp,
+                     (int)vectors(src, ld, sizeof(S)), map, count, cell, (D*)dst, plane);
+}
+template <class S>
+static void largest(const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, unsigned* cell, hipStream_t st) {
+  const long work = (long)rows * ((cols + 7) / 8);
+  hipLaunchKernelGGL((loss_largest_kernel<S>), dim3(std::min(4096u, blocks_for(work))), dim3(256), 0, st, (const S*)src, ld, rows, cols,
+                     (int)vectors(src, ld, sizeof(S)), map, count, cell);
+}
+// the weight's rows from v0 as the forward's planes
+static void forward_weight(const nsa_loss_desc* d, const LossPlan& p, const void* weight, int v0, int rows, const unsigned* cell, void* dst, hipStream_t st) {
+  const long plane = (long)p.kp * up(rows, 64);
+  if (d->dtype == 0) planes<B16, B16, 1>((const B16*)weight + (long)v0 * d->w_stride, d->w_stride, rows, rows, d->dim, p.kp, nullptr, nullptr, nullptr, dst, plane, st);
+  else if (d->dtype == 1) planes<H16, H16, 1>((const H16*)weight + (long)v0 * d->w_stride, d->w_stride, rows, rows, d->dim, p.kp, nullptr, nullptr, nullptr, dst, plane, st);
+  else planes<float, H16, 2>((const float*)weight + (long)v0 * d->w_stride, d->w_stride, rows, rows, d->dim, p.kp, nullptr, nullptr, cell, dst, plane, st);
+}
+
+}  // namespace nsa
+
+using namespace nsa;
+
+extern "C" int nsa_loss_workspace_bytes(const nsa_loss_desc* d, const void* weight, size_t* state_bytes, size_t* fwd_bytes, size_t* bwd_bytes) {
+  LossPlan p;
+  if (!state_bytes || !fwd_bytes || !bwd_bytes) return NSA_E_ARG;
+  if (int rc = loss_plan(d, weight, p)) return rc;
+  *state_bytes = p.state;
+  *fwd_bytes = p.fwd;
+  *bwd_bytes = p.bwd;
+  return 0;
+}
+
+extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* weight, const void* labels, void* state, size_t state_bytes, void* ws,
+                            size_t ws_bytes, float* loss, void* stream) {
+  LossPlan p;
+  if (int rc = loss_plan(d, weight, p)) return rc;
+  if (!weight || !state || !ws || !loss || (p.n > 0 && (!x || !labels))) return NSA_E_ARG;
+  if (state_bytes < p.state || ws_bytes < p.fwd) return NSA_E_WORKSPACE;
+  hipStream_t st = (hipStream_t)stream;
+  char *s = (char*)state, *w = (char*)ws;
+  unsigned* cells = (unsigned*)s;
+  int *map = (int*)(s + p.s_map), *place = (int*)(s + p.s_place), *label = (int*)(s + p.s_label);
+  float *lse = (float*)(s + p.s_lse), *each = (float*)(w + p.f_loss), *target = (float*)(w + p.f_target);
+  float* losses = d->reduction == 0 ? loss : nullptr;
+  hipLaunchKernelGGL(loss_rows_kernel, dim3((unsigned)std::max(1, (p.n + 1023) / 1024)), dim3(256), 0, st, labels, (int)d->labels_int64, p.n, d->vocab,
+                     (long)d->ignore_index, map, place, label, cells, losses);
+  const unsigned *count = cells + CELL_ROWS, *xc = d->dtype == 2 ? cells + CELL_X : nullptr, *wc = d->dtype == 2 ? cells + CELL_W : nullptr;
+  const long x_plane = (long)p.npad * p.kp;
+  if (p.n > 0) {
+    if (d->dtype == 2) {
+      largest<float>(x, d->x_stride, p.n, d->dim, map, count, cells + CELL_X, st);
+      largest<float>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
+      planes<float, H16, 2>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, xc, s + p.s_x, x_plane, st);
+    } else if (d->dtype == 1) {
+      planes<H16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, s + p.s_x, x_plane, st);
+    } else {
+      planes<B16, B16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, s + p.s_x, x_plane, st);
+    }
+    const int rows = p.in_place ? d->vocab : p.fwd_rows;
+    for (long v0 = 0; v0 < d->vocab; v0 += rows) {
+      LossTileArgs a{};
+      a.v0 = (int)v0;
+      a.vend = (int)std::min<long>(d->vocab, v0 + rows);
+      if (p.in_place) {
+        a.w = weight;
+        a.w_ld = d->w_stride;
+      } else {
+        forward_weight(d, p, weight, a.v0, a.vend - a.v0, wc, w + p.f_w, st);
+        a.w = w + p.f_w;
+        a.w_ld = p.kp;
+        a.w_plane = (long)p.kp * up(a.vend - a.v0, 64);
+      }
+      a.x = s + p.s_x; a.x_plane = x_plane; a.kp = p.kp; a.vocab = d->vocab; a.n = p.n; a.npad = p.npad;
+      a.count = count; a.x_cell = xc; a.w_cell = wc; a.label = label; a.part = (float2*)(w + p.f_part); a.target = target;
+      logits_tiles<false>(d, p, a, st);
+    }
+    const int part = p.few ? 32 : p.wide ? 128 : 64, tile = p.few ? 128 : p.wide ? 256 : 128;
+    const int parts = (d->vocab + tile - 1) / tile * (tile / part);
+    hipLaunchKernelGGL(loss_merge_kernel, dim3((unsigned)((p.n + 7) / 8)), dim3(256), 0, st, (const float2*)(w + p.f_part), parts, p.npad, count, (const int*)map,
+                       (const int*)label, (const float*)target, lse, each, losses);
+  }
+  if (d->reduction != 0)
+    hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, (const float*)each, count, (int)(d->reduction == 1), loss);
+  return (int)hipGetLastError();
+}
+
+extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const void* state, size_t state_bytes, const float* dloss, void* ws, size_t ws_bytes,
+                            void* dx, void* dw, void* stream) {
+  LossPlan p;
+  if (int rc = loss_plan(d, weight, p)) return rc;
+  if (!weight || !state || !dloss || !ws || (!dx && !dw)) return NSA_E_ARG;
+  if (state_bytes < p.state || ws_bytes < p.bwd) return NSA_E_WORKSPACE;
+  if (p.n == 0) return NSA_E_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  const char* s = (const char*)state;
+  char* w = (char*)ws;
+  const unsigned* kept = (const unsigned*)s;
+  unsigned* cells = (unsigned*)(w + p.b_cells);
+  const int *map = (const int*)(s + p.s_map), *place = (const int*)(s + p.s_place), *label = (const int*)(s + p.s_label);
+  const unsigned* count = kept + CELL_ROWS;
+  float* g = (float*)(w + p.b_g);
+  hipLaunchKernelGGL(loss_weights_kernel, dim3(1), dim3(1024), 0, st, dloss, (int)d->reduction, count, map, g, cells);
+  // the operands of both products in fp16: x once, w with each piece
+  const long x_plane = (long)p.npad * p.kp;
+  const void* xg = s + p.s_x;
+  const unsigned *xc = d->dtype == 2 ? kept + CELL_X : nullptr, *wc = d->dtype == 2 ? kept + CELL_W : nullptr;
+  if (d->dtype == 0) {
+    xc = cells + CELL_X;
+    wc = cells + CELL_W;
+    if (dw) {
+      largest<B16>(s + p.s_x, p.kp, p.n, p.kp, nullptr, count, cells + CELL_X, st);
+      planes<B16, H16, 1>(s + p.s_x, p.kp, p.n, p.n, p.kp, p.kp, nullptr, count, xc, w + p.b_x, x_plane, st);
+      xg = w + p.b_x;
+    }
+    if (dx) largest<B16>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
+  }
+  const int each = d->dtype == 2 ? 4 : 2;
+  for (long v0 = 0; v0 < d->vocab; v0 += p.bwd_rows) {
+    LossTileArgs a{};
+    a.v0 = (int)v0;
+    a.vend = (int)std::min<long>(d->vocab, v0 + p.bwd_rows);
+    const int entries = a.vend - a.v0, ld = (int)up(entries, 64);
+    const long w_plane = (long)p.kp * ld;
+    const char* from = (const char*)weight + v0 * d->w_stride * each;
+    if (d->dtype == 0) {
+      if (dx) planes<B16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, w + p.b_wg, w_plane, st);
+      if (!p.in_place) planes<B16, B16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, nullptr, w + p.b_wf, w_plane, st);
+    } else if (d->dtype == 1) {
+      planes<H16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, nullptr, w + p.b_wg, w_plane, st);
+    } else {
+      planes<float, H16, 2>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, w + p.b_wg, w_plane, st);
+    }
+    const bool direct = p.in_place && d->dtype == 0;
+    a.w = direct ? (const void*)from : d->dtype == 0 ? w + p.b_wf : w + p.b_wg;
+    a.w_ld = direct ? d->w_stride : p.kp;
+    a.w_plane = w_plane;
+    a.x = s + p.s_x; a.x_plane = x_plane; a.kp = p.kp; a.vocab = d->vocab; a.n = p.n; a.npad = p.npad;
+    a.count = count; a.x_cell = d->dtype == 2 ? xc : nullptr; a.w_cell = d->dtype == 2 ? wc : nullptr; a.label = label;
+    a.lse = (const float*)(s + p.s_lse); a.g = g; a.g_cell = cells + CELL_G;
+    a.grad = (H16*)(w + p.b_grad); a.grad_plane = (long)p.npad * ld; a.grad_ld = ld;
+    logits_tiles<true>(d, p, a, st);
+
+    LossGradArgs q{};
+    q.grad = a.grad; q.grad_plane = a.grad_plane; q.grad_ld = ld; q.kp = p.kp; q.dim = d->dim; q.entries = entries;
+    q.count = count; q.g_cell = cells + CELL_G; q.npad = p.npad;
+    const int tile = p.wide ? 256 : 128;
+    q.tiles_m = (p.kp + tile - 1) / tile;
+    if (dx) {
+      const int bk = p.P == 2 ? 32 : 64;
+      q.other = (const H16*)(w + p.b_wg); q.other_plane = w_plane; q.other_cell = wc;
+      q.tiles_n = (p.n + tile - 1) / tile;
+      q.sums = (float*)(w + p.b_dx); q.per = (ld / bk + p.splits - 1) / p.splits; q.first = v0 == 0;
+      const dim3 grid((unsigned)(q.tiles_m * q.tiles_n * p.splits));
+      if (p.P == 1 && p.wide) hipLaunchKernelGGL((loss_dx_kernel<GradTiles<1>::WideX>), grid, dim3(512), 0, st, q);
+      else if (p.P == 1) hipLaunchKernelGGL((loss_dx_kernel<GradTiles<1>::SmallX>), grid, dim3(256), 0, st, q);
+      else if (p.wide) hipLaunchKernelGGL((loss_dx_kernel<GradTiles<2>::WideX>), grid, dim3(512), 0, st, q);
+      else hipLaunchKernelGGL((loss_dx_kernel<GradTiles<2>::SmallX>), grid, dim3(256), 0, st, q);
+    }
+    if (dw) {
+      q.other = (const H16*)xg; q.other_plane = x_plane; q.other_cell = xc;
+      q.tiles_n = (entries + tile - 1) / tile;
+      q.dw = (char*)dw + v0 * d->dim * each; q.dw_ld = d->dim; q.vec = d->dim % 4 == 0;
+      const dim3 grid((unsigned)(q.tiles_m * q.tiles_n));
+      if (d->dtype == 2) {
+        if (p.wide) hipLaunchKernelGGL((loss_dw_kernel<GradTiles<2>::WideW, float>), grid, dim3(512), 0, st, q);
+        else hipLaunchKernelGGL((loss_dw_kernel<GradTiles<2>::SmallW, float>), grid, dim3(256), 0, st, q);
+      } else if (d->dtype == 1) {
+        if (p.wide) hipLaunchKernelGGL((loss_dw_kernel<GradTiles<1>::WideW, H16>), grid, dim3(512), 0, st, q);
+        else hipLaunchKernelGGL((loss_dw_kernel<GradTiles<1>::SmallW, H16>), grid, dim3(256), 0, st, q);
+      } else {
+        if (p.wide) hipLaunchKernelGGL((loss_dw_kernel<GradTiles<1>::WideW, B16>), grid, dim3(512), 0, st, q);
+        else hipLaunchKernelGGL((loss_dw_kernel<GradTiles<1>::SmallW, B16>), grid, dim3(256), 0, st, q);
+      }
+    }
+  }
+  if (dx) {
+    const dim3 grid(blocks_for((long)p.n * ((d->dim + 3) / 4)));
+    const float* sums = (const float*)(w + p.b_dx);
+    const int vec = d->dim % 4 == 0;
+    if (d->dtype == 0) hipLaunchKernelGGL((loss_dx_rows_kernel<B16>), grid, dim3(256), 0, st, sums, p.splits, p.npad, p.kp, p.n, d->dim, vec, place, (B16*)dx);
+    else if (d->dtype == 1) hipLaunchKernelGGL((loss_dx_rows_kernel<H16>), grid, dim3(256), 0, st, sums, p.splits, p.npad, p.kp, p.n, d->dim, vec, place, (H16*)dx);
+    else hipLaunchKernelGGL((loss_dx_rows_kernel<float>), grid, dim3(256), 0, st, sums, p.splits, p.npad, p.kp, p.n, d->dim, vec, place, (float*)dx);
+  }
+  return (int)hipGetLastError();
+}

@@ -1,0 +1,577 @@
+// Orthogonalised updates: the polar factor of a matrix by Newton-Schulz products,
+//
+//   X <- G / (|G| + eps) (turned so that it is not taller than wide), `steps` times:  A = X X^T,  B = b A + c A A,  X <- a X + B X,
+//
+// for a list of matrices of any sizes, all of them in each launch: the norms, the first planes, then three launches a step.
+//
+// X, A and B are held as two fp16 halves each (22 bits; nsa_tiles.hpp).  Directions of small singular values grow by a = 3.4 a step, and what
+// a step's rounding adds to them grows alike: against 64 bits the result is 4e-5 off with bf16 halves, 3 % with bf16 alone, and 6e-7 with
+// these, less than with fp32 products (1.6e-6 at 512 x 512).  Scales: X 2^(12 + s), A and B 2^(10 + 2 s).  s is 0 unless |G| is small beside eps:
+// then X starts so small that fp16 would lose it, and s is what brings its norm to 1; it falls by the bits of a with each step, so nothing grows out
+// of range.  The entry checks that singular values up to 1 stay below 4 for the given coefficients.
+//
+// A and B are symmetric: only tiles on and below the diagonal are made, and stored twice.
+#include <algorithm>
+#include <cmath>
+#include "nsa_tiles.hpp"
+#include "../../include/nsa_hip.h"
+
+namespace nsa {
+
+constexpr int kNewtonMany = 56, kNormChunks = 512;      // matrices of one launch (their table is a kernel argument)
+
+struct NewtonMatrix {
+  const void* in;
+  void* out;
+  long stride;                // of the rows of `in`
+  unsigned at;                // of its planes in the workspace, in units of 256 bytes
+  int rows, cols;             // as given
+};
+struct NewtonTable {
+  NewtonMatrix of[kNewtonMany];
+  int tile0[kNewtonMany + 1];      // first tile of each, in the launch at hand
+  int many, chunks;
+  char* ws;
+  double* partial;                 // [many][kNormChunks]
+  int* shift;                      // s of each
+};
+
+__host__ __device__ inline long up64(long v) { return (v + 63) / 64 * 64; }
+// X [2 buffers][2 halves][mp][np], then A and B [2 halves][mp][mp]
+struct NewtonPlanes {
+  int m, n, mp, np;
+  bool turned;
+  __host__ __device__ NewtonPlanes(int rows, int cols) {
+    turned = rows > cols;
+    m = turned ? cols : rows;
+    n = turned ? rows : cols;
+    mp = (int)up64(m);
+    np = (int)up64(n);
+  }
+  __host__ __device__ long x_plane() const { return (long)mp * np; }
+  __host__ __device__ long a_plane() const { return (long)mp * mp; }
+  __host__ __device__ long halves() const { return 4 * x_plane() + 4 * a_plane(); }
+};
+__device__ __forceinline__ _Float16* planes_of(const NewtonTable& t, int k) { return (_Float16*)(t.ws + (size_t)t.of[k].at * 256); }
+
+__device__ __forceinline__ int matrix_of(const NewtonTable& t, int tile) {
+  int k = 0, past = t.many;
+  while (past - k > 1) {
+    const int mid = (k + past) / 2;
+    if (tile >= t.tile0[mid]) k = mid;
+    else past = mid;
+  }
+  return k;
+}
+
+template <class S>
+__global__ __launch_bounds__(256) void newton_norm_kernel(const NewtonTable G) {
+  __shared__ double sums[4];
+  const int k = blockIdx.y, tid = threadIdx.x;
+  const NewtonMatrix M = G.of[k];
+  const S* in = (const S*)M.in;
+  const bool whole = M.stride == M.cols && ((uintptr_t)in & 15) == 0;      // one run of values
+  double sum = 0.0;
+  const long total = (long)M.rows * M.cols, per = ((total + G.chunks - 1) / G.chunks + 2047) / 2048 * 2048, first = blockIdx.x * per, last = min(total, first + per);
+  if (whole) {
+    constexpr int V = 16 / sizeof(S);
+    typedef __attribute__((__vector_size__(16))) S vec;
+    for (long i = first + tid * V; i < last; i += 256 * V) {
+      if (i + V <= last) {
+        const vec v = *reinterpret_cast<const vec*>(in + i);
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum += (double)(float)v[e] * (double)(float)v[e];
+      } else {
+        for (long e = i; e < last; ++e) sum += (double)(float)in[e] * (double)(float)in[e];
+      }
+    }
+  } else {
+    for (long i = first + tid; i < last; i += 256) {
+      const double v = (double)(float)in[i / M.cols * M.stride + i % M.cols];
+      sum += v * v;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if ((tid & 63) == 0) sums[tid >> 6] = sum;
+  __syncthreads();
+  if (tid == 0) G.partial[k * kNormChunks + blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
+}
+
+// A 64 x 64 tile of the first X, scaled, with zeros up to whole multiples of 64
+template <class S>
+__global__ __launch_bounds__(256) void newton_begin_kernel(const NewtonTable G, float eps) {
+  __shared__ float tile_s[64][65];
+  __shared__ double sums[4];
+  const int k = matrix_of(G, blockIdx.x), tid = threadIdx.x;
+  const NewtonMatrix M = G.of[k];
+  const NewtonPlanes L(M.rows, M.cols);
+  const int at = blockIdx.x - G.tile0[k], wide = L.np / 64, r0 = at / wide * 64, c0 = at % wide * 64;
+  double sum = 0.0;
+  for (int i = tid; i < G.chunks; i += 256) sum += G.partial[k * kNormChunks + i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if ((tid & 63) == 0) sums[tid >> 6] = sum;
+  // (turned: the tile's rows are columns of the matrix)
+  const S* in = (const S*)M.in;
+  const int first = L.turned ? c0 : r0, second = L.turned ? r0 : c0, col = second + (tid & 63);
+#pragma unroll 4
+  for (int i = tid >> 6; i < 64; i += 4) {
+    const int row = first + i;
+    tile_s[i][tid & 63] = row < M.rows && col < M.cols ? (float)in[row * M.stride + col] : 0.f;
+  }
+  __syncthreads();
+  const double norm = sqrt(sums[0] + sums[1] + sums[2] + sums[3]), part = norm / (norm + eps);
+  // (a norm of zero, and one that is no number: s = 0)
+  const int s = part > 0.0 && part < 1.0 ? min(100, -(ilogb(part) + 1)) : 0;
+  const double scale = ldexp(1.0 / (norm + eps), 12 + s);
+  if (at == 0 && tid == 0) G.shift[k] = s;
+  const int r = tid >> 2, c = (tid & 3) * 16;
+  _Float16* x = planes_of(G, k) + (long)(r0 + r) * L.np + c0 + c;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    f16x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int cc = c + 8 * u + e;
+      const Halves h = halves_of((float)((double)(L.turned ? tile_s[cc][r] : tile_s[r][cc]) * scale));
+      hi[e] = h.hi;
+      lo[e] = h.lo;
+    }
+    *reinterpret_cast<f16x8*>(x + 8 * u) = hi;
+    *reinterpret_cast<f16x8*>(x + 8 * u + L.x_plane()) = lo;
+  }
+}
+
+struct NewtonStep {
+  int step, last, growth, from;      // growth: bits that a step takes off s; from: the buffer of X that is read
+  float a, b, c;
+};
+__device__ __forceinline__ int shift_at(const NewtonTable& G, const NewtonStep& S, int k, int step) { return max(0, G.shift[k] - S.growth * step); }
+
+// four consecutive halves pairs in memory
+__device__ __forceinline__ floatx4 load_halves(const _Float16* p, long plane) {
+  const f16x4 hi = *reinterpret_cast<const f16x4*>(p), lo = *reinterpret_cast<const f16x4*>(p + plane);
+  floatx4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (float)hi[e] + (float)lo[e];
+  return v;
+}
+// Two register quads of a result's column as 16 bytes of a row of each plane (join_quads)
+__device__ __forceinline__ void store_halves(_Float16* p, long plane, const floatx4 (&v)[2]) {
+  f16x4 hi[2], lo[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const Halves h = halves_of(v[u][e]);
+      hi[u][e] = h.hi;
+      lo[u][e] = h.lo;
+    }
+  const uintx4 a = join_quads(__builtin_bit_cast(uintx2, hi[0]), __builtin_bit_cast(uintx2, hi[1]));
+  const uintx4 b = join_quads(__builtin_bit_cast(uintx2, lo[0]), __builtin_bit_cast(uintx2, lo[1]));
+  *reinterpret_cast<uintx4*>(p) = a;
+  *reinterpret_cast<uintx4*>(p + plane) = b;
+}
+
+// POLY 0: A = X X^T; 1: B = b A + c A A.  Tiles on and below the diagonal.
+template <class Tiles, bool POLY>
+__global__ __launch_bounds__(Tiles::THREADS, 2) void newton_square_kernel(const NewtonTable G, const NewtonStep S) {
+  __shared__ __align__(1024) char shared[Tiles::LDS];
+  const int k = matrix_of(G, blockIdx.x);
+  const NewtonPlanes L(G.of[k].rows, G.of[k].cols);
+  const int nth = blockIdx.x - G.tile0[k];
+  int tm = (int)((sqrtf(8.f * nth + 1.f) - 1.f) * 0.5f);
+  while ((tm + 1) * (tm + 2) / 2 <= nth) ++tm;
+  while (tm * (tm + 1) / 2 > nth) --tm;
+  const int tn = nth - tm * (tm + 1) / 2, m0 = tm * Tiles::TM, n0 = tn * Tiles::TN;
+  _Float16* base = planes_of(G, k);
+  const _Float16* x = base + (S.from ? 2 * L.x_plane() : 0);
+  _Float16* A = base + 4 * L.x_plane();
+  _Float16* out = POLY ? A + 2 * L.a_plane() : A;
+  Tiles t;
+  t.init(shared);
+  if (POLY) {
+    t.operand_a(A, L.a_plane(), L.mp, m0, L.m);
+    t.operand_b(A, L.a_plane(), L.mp, n0, L.m);
+    t.run(L.mp / Tiles::BK);
+  } else {
+    t.operand_a(x, L.x_plane(), L.np, m0, L.m);
+    t.operand_b(x, L.x_plane(), L.np, n0, L.m);
+    t.run(L.np / Tiles::BK);
+  }
+  const float unit = POLY ? __builtin_ldexpf(S.c, -10 - 2 * shift_at(G, S, k, S.step)) : 0x1p-14f;
+#pragma unroll
+  for (int j = 0; j < Tiles::NI; ++j) {
+    const int col = n0 + t.col_of(j);
+#pragma unroll
+    for (int i = 0; i < Tiles::MI; ++i) {
+#pragma unroll
+      for (int q = 0; q < 4; q += 2) {
+        floatx4 v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = m0 + t.row_of(i, q + u);
+          floatx4 old = {0.f, 0.f, 0.f, 0.f};
+          if (POLY && col < L.m && row < L.mp) old = load_halves(A + (long)col * L.mp + row, L.a_plane());
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float f = t.acc[i][j][4 * (q + u) + e] * unit;
+            v[u][e] = row + e < L.m && col < L.m ? POLY ? __builtin_fmaf(S.b, old[e], f) : f : 0.f;
+          }
+        }
+        if (tm != tn && col < L.mp) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int row = m0 + t.row_of(i, q + u) + e;
+              if (row >= L.m) continue;
+              const Halves h = halves_of(v[u][e]);
+              out[(long)row * L.mp + col] = h.hi;
+              out[(long)row * L.mp + col + L.a_plane()] = h.lo;
+            }
+        }
+        // (a lane and its partner of the exchange have the same column, and rows of the same block of 32: both store or neither)
+        const int at = m0 + t.wm * (Tiles::TM / Tiles::WM) + 32 * i + 8 * q + 8 * (t.lane >> 5);
+        if (at < L.mp && col < L.m) store_halves(out + (long)col * L.mp + at, L.a_plane(), v);
+      }
+    }
+  }
+}
+
+// X <- a X + B X (the other buffer; LAST: the result as it was given), columns of X (registers) by its rows (lanes)
+template <class Tiles, bool LAST, class O>
+__global__ __launch_bounds__(Tiles::THREADS, 2) void newton_update_kernel(const NewtonTable G, const NewtonStep S) {
+  __shared__ __align__(1024) char shared[Tiles::LDS];
+  const int k = matrix_of(G, blockIdx.x);
+  const NewtonMatrix M = G.of[k];
+  const NewtonPlanes L(M.rows, M.cols);
+  const int tiles_n = (L.mp + Tiles::TN - 1) / Tiles::TN, tiles_m = (L.np + Tiles::TM - 1) / Tiles::TM;
+  const TileAt tile = tile_at(blockIdx.x - G.tile0[k], tiles_m, tiles_n, 4);
+  const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN;
+  _Float16* base = planes_of(G, k);
+  const _Float16* x = base + (S.from ? 2 * L.x_plane() : 0);
+  _Float16* next = base + (S.from ? 0 : 2 * L.x_plane());
+  const _Float16* B = base + 4 * L.x_plane() + 2 * L.a_plane();
+  Tiles t;
+  t.init(shared);
+  t.operand_a(x, L.x_plane(), L.np, m0, L.np);
+  t.operand_b(B, L.a_plane(), L.mp, n0, L.m);
+  t.run(L.mp / Tiles::BK);
+  const int s = shift_at(G, S, k, S.step), s2 = shift_at(G, S, k, S.step + 1);
+  const float unit = __builtin_ldexpf(1.f, -10 - 2 * s), scale = __builtin_ldexpf(1.f, LAST ? -12 - s : s2 - s);
+#pragma unroll
+  for (int j = 0; j < Tiles::NI; ++j) {
+    const int row = n0 + t.col_of(j);
+#pragma unroll
+    for (int i = 0; i < Tiles::MI; ++i) {
+#pragma unroll
+      for (int q = 0; q < 4; q += 2) {
+        floatx4 v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int col = m0 + t.row_of(i, q + u);
+          floatx4 old = {0.f, 0.f, 0.f, 0.f};
+          const bool ok = row < L.m && col < L.np;
+          if (ok) old = load_halves(x + (long)row * L.np + col, L.x_plane());
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[u][e] = ok ? scale * __builtin_fmaf(S.a, old[e], t.acc[i][j][4 * (q + u) + e] * unit) : 0.f;
+          if (LAST && ok) {
+            if (L.turned) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (col + e < L.n) ((O*)M.out)[(long)(col + e) * M.cols + row] = (O)v[u][e];
+            } else {
+              O* p = (O*)M.out + (long)row * M.cols + col;
+              typedef __attribute__((__vector_size__(4 * sizeof(O)))) O ox4;
+              if (M.cols % 4 == 0 && col < L.n) {
+                ox4 o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = (O)v[u][e];
+                *reinterpret_cast<ox4*>(p) = o;
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (col + e < L.n) p[e] = (O)v[u][e];
+              }
+            }
+          }
+        }
+        if (!LAST) {
+          const int at = m0 + t.wm * (Tiles::TM / Tiles::WM) + 32 * i + 8 * q + 8 * (t.lane >> 5);
+          if (at < L.np && row < L.mp) store_halves(next + (long)row * L.np + at, L.x_plane(), v);
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------ small matrices
+
+// A matrix of up to 64 rows that fits a CU's LDS, all steps in one work-group, in fp32 throughout (32 x 32 x 2 products): the launches of the
+// other kernels would be all of its time (a 24 x 512 matrix took 99 us with them), and sums this short show that halves have a bit or two less
+// than fp32.  X lies in LDS for the whole time; a step is A (the columns of X split over the waves and summed), B, and X, 32 columns a
+// wave, in place.
+constexpr int kSmallFloats = 40960 - 4 * 8, kSmallWaves = 8, kSmallPart = kSmallWaves * 1024;
+__host__ __device__ inline int up32(int v) { return (v + 31) / 32 * 32; }
+__host__ __device__ inline bool newton_small(int m, int n) {
+  if (m > 64) return false;
+  const int M = up32(m);
+  return (long)M * (up32(n) + 4) + 2 * M * (M + 4) + kSmallPart <= kSmallFloats;
+}
+__device__ __forceinline__ floatx16 mma_f32(floatx4 a, floatx4 b, floatx16 c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+template <class S>
+__global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const NewtonTable G, const NewtonStep T, int steps, float eps) {
+  __shared__ __align__(16) float lds[kSmallFloats];
+  __shared__ double sums[kSmallWaves];
+  const NewtonMatrix K = G.of[blockIdx.x];
+  const NewtonPlanes L(K.rows, K.cols);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, l = lane & 31;
+  const int M = up32(L.m), N = up32(L.n), xp = N + 4, ap = M + 4, blocks = (M / 32) * (M / 32), splits = kSmallWaves / blocks;
+  float *x = lds, *A = x + M * xp, *B = A + M * ap, *part = B + M * ap;
+
+  for (int i = tid; i < M * xp; i += 64 * kSmallWaves) x[i] = 0.f;
+  __syncthreads();
+  double sum = 0.0;
+  for (int i = tid; i < K.rows * K.cols; i += 64 * kSmallWaves) {
+    const int r = i / K.cols, c = i % K.cols;
+    const float v = (float)((const S*)K.in)[r * K.stride + c];
+    x[L.turned ? c * xp + r : r * xp + c] = v;
+    sum += (double)v * (double)v;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (int w = 0; w < kSmallWaves; ++w) sum += sums[w];
+  const double scale = 1.0 / (sqrt(sum) + eps);
+  for (int i = tid; i < M * xp; i += 64 * kSmallWaves) x[i] = (float)((double)x[i] * scale);
+  __syncthreads();
+
+  for (int step = 0; step < steps; ++step) {
+    {
+      const int blk = wave % blocks, split = wave / blocks, bi = blk / (M / 32), bj = blk % (M / 32), groups = N / 8;
+      const int per = (groups + splits - 1) / splits;
+      const float *xi = x + (32 * bi + l) * xp + 4 * h, *xj = x + (32 * bj + l) * xp + 4 * h;
+      floatx16 acc = zero_acc();
+#pragma unroll 4
+      for (int g = split * per; g < min(groups, (split + 1) * per); ++g)
+        acc = mma_f32(*reinterpret_cast<const floatx4*>(xi + 8 * g), *reinterpret_cast<const floatx4*>(xj + 8 * g), acc);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) part[wave * 1024 + e * 64 + lane] = acc[e];
+    }
+    __syncthreads();
+    for (int i = tid; i < blocks * 1024; i += 64 * kSmallWaves) {
+      const int blk = i >> 10, e = (i >> 6) & 15, at = i & 1023;
+      float v = 0.f;
+      for (int s = 0; s < splits; ++s) v += part[(s * blocks + blk) * 1024 + at];
+      A[(blk / (M / 32) * 32 + 8 * (e >> 2) + 4 * ((i >> 5) & 1) + (e & 3)) * ap + blk % (M / 32) * 32 + (i & 31)] = v;
+    }
+    __syncthreads();
+    if (wave < blocks) {
+      const int bi = wave / (M / 32), bj = wave % (M / 32);
+      const float *ai = A + (32 * bi + l) * ap + 4 * h, *aj = A + (32 * bj + l) * ap + 4 * h;
+      floatx16 acc = zero_acc();
+#pragma unroll 4
+      for (int g = 0; g < M / 8; ++g) acc = mma_f32(*reinterpret_cast<const floatx4*>(ai + 8 * g), *reinterpret_cast<const floatx4*>(aj + 8 * g), acc);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int at = (32 * bi + 8 * (e >> 2) + 4 * h + (e & 3)) * ap + 32 * bj + l;
+        B[at] = __builtin_fmaf(T.b, A[at], T.c * acc[e]);
+      }
+    }
+    __syncthreads();
+    for (int cb = wave; cb < N / 32; cb += kSmallWaves) {
+      floatx16 acc[2] = {zero_acc(), zero_acc()};
+      float* col = x + 32 * cb + l;
+      for (int g = 0; g < M / 8; ++g) {
+        floatx4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = col[(8 * g + 4 * h + e) * xp];
+#pragma unroll
+        for (int bi = 0; bi < 2; ++bi)
+          if (bi < M / 32) acc[bi] = mma_f32(*reinterpret_cast<const floatx4*>(B + (32 * bi + l) * ap + 8 * g + 4 * h), v, acc[bi]);
+      }
+#pragma unroll
+      for (int bi = 0; bi < 2; ++bi)
+        if (bi < M / 32) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float* p = col + (32 * bi + 8 * (e >> 2) + 4 * h + (e & 3)) * xp;
+            *p = __builtin_fmaf(T.a, *p, acc[bi][e]);
+          }
+        }
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < K.rows * K.cols; i += 64 * kSmallWaves) {
+    const int r = i / K.cols, c = i % K.cols;
+    ((S*)K.out)[i] = (S)x[L.turned ? c * xp + r : r * xp + c];
+  }
+}
+
+// ------------------------------------------------------------------------------------ launches
+
+typedef _Float16 H16;
+template <int SIZE> struct NewtonTiles;
+template <> struct NewtonTiles<256> {
+  typedef TileProduct<H16, 2, ROWS, ROWS, 256, 256, 2, 4, 32, 2> Square;
+  typedef TileProduct<H16, 2, COLUMNS, ROWS, 256, 256, 2, 4, 32, 2> Update;
+};
+template <> struct NewtonTiles<128> {
+  typedef TileProduct<H16, 2, ROWS, ROWS, 128, 128, 2, 2, 32, 2> Square;
+  typedef TileProduct<H16, 2, COLUMNS, ROWS, 128, 128, 2, 2, 32, 2> Update;
+};
+template <> struct NewtonTiles<64> {
+  typedef TileProduct<H16, 2, ROWS, ROWS, 64, 64, 2, 2, 64, 2> Square;
+  typedef TileProduct<H16, 2, COLUMNS, ROWS, 64, 64, 2, 2, 64, 2> Update;
+};
+
+static long square_tiles(const NewtonPlanes& p, int size) {
+  const long t = (p.m + size - 1) / size;
+  return t * (t + 1) / 2;
+}
+static long update_tiles(const NewtonPlanes& p, int size) { return ((long)p.np + size - 1) / size * (((long)p.mp + size - 1) / size); }
+template <class Count>
+static long fill(NewtonTable& t, int size, Count count) {
+  long at = 0;
+  for (int k = 0; k < t.many; ++k) {
+    t.tile0[k] = (int)at;
+    at += count(NewtonPlanes(t.of[k].rows, t.of[k].cols), size);
+  }
+  t.tile0[t.many] = (int)at;
+  return at;
+}
+// the largest tiles that give every CU one
+template <class Count>
+static int tile_size(NewtonTable& t, Count count) {
+  for (int size = 256; size > 64; size /= 2)
+    if (fill(t, size, count) >= 256) return size;
+  return 64;
+}
+
+template <int SIZE, bool POLY>
+static void square(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
+  typedef typename NewtonTiles<SIZE>::Square Tiles;
+  const long tiles = fill(t, SIZE, square_tiles);
+  hipLaunchKernelGGL((newton_square_kernel<Tiles, POLY>), dim3((unsigned)tiles), dim3(Tiles::THREADS), 0, st, t, s);
+}
+template <int SIZE, bool LAST, class O>
+static void update(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
+  typedef typename NewtonTiles<SIZE>::Update Tiles;
+  const long tiles = fill(t, SIZE, update_tiles);
+  hipLaunchKernelGGL((newton_update_kernel<Tiles, LAST, O>), dim3((unsigned)tiles), dim3(Tiles::THREADS), 0, st, t, s);
+}
+template <int SIZE, class O>
+static void update_any(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
+  if (s.last) update<SIZE, true, O>(t, s, st);
+  else update<SIZE, false, H16>(t, s, st);
+}
+
+template <class S>
+static void newton(NewtonTable& t, NewtonStep s, int steps, float eps, hipStream_t st) {
+  hipLaunchKernelGGL((newton_norm_kernel<S>), dim3((unsigned)t.chunks, (unsigned)t.many), dim3(256), 0, st, t);
+  const long begin = fill(t, 64, update_tiles);
+  hipLaunchKernelGGL((newton_begin_kernel<S>), dim3((unsigned)begin), dim3(256), 0, st, t, eps);
+  const int sq = tile_size(t, square_tiles), un = tile_size(t, update_tiles);
+  for (s.step = 0; s.step < steps; ++s.step) {
+    s.from = s.step & 1;
+    s.last = s.step == steps - 1;
+    if (sq == 256) { square<256, false>(t, s, st); square<256, true>(t, s, st); }
+    else if (sq == 128) { square<128, false>(t, s, st); square<128, true>(t, s, st); }
+    else { square<64, false>(t, s, st); square<64, true>(t, s, st); }
+    if (un == 256) update_any<256, S>(t, s, st);
+    else if (un == 128) update_any<128, S>(t, s, st);
+    else update_any<64, S>(t, s, st);
+  }
+}
+
+// bytes before the planes: sums of squares and shifts
+static size_t newton_head() { return (size_t)kNewtonMany * kNormChunks * 8 + 256; }
+
+}  // namespace nsa
+
+using namespace nsa;
+
+static bool is_small(int rows, int cols) { return newton_small(std::min(rows, cols), std::max(rows, cols)); }
+
+extern "C" int nsa_newton_workspace_bytes(int32_t many, const int32_t* rows, const int32_t* cols, size_t* bytes) {
+  if (many < 0 || (many > 0 && (!rows || !cols)) || !bytes) return NSA_E_ARG;
+  size_t most = 0, now = 0;
+  int large = 0;
+  for (int32_t k = 0; k < many; ++k) {
+    if (rows[k] <= 0 || cols[k] <= 0) return NSA_E_ARG;
+    if (rows[k] > (1 << 20) || cols[k] > (1 << 20) || std::min(rows[k], cols[k]) > (1 << 15)) return NSA_E_UNSUPPORTED;
+    if (is_small(rows[k], cols[k])) continue;
+    if (large++ % kNewtonMany == 0) now = 0;
+    now += (NewtonPlanes(rows[k], cols[k]).halves() * 2 + 255) / 256 * 256;
+    most = std::max(most, now);
+  }
+  if (most >> 40) return NSA_E_UNSUPPORTED;
+  *bytes = newton_head() + most;
+  return 0;
+}
+
+extern "C" int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_t* cols, const void* const* in, const int64_t* in_stride, void* const* out,
+                                 int32_t dtype, int32_t steps, float a, float b, float c, float eps, void* ws, size_t ws_bytes, void* stream) {
+  size_t need = 0;
+  if (int rc = nsa_newton_workspace_bytes(many, rows, cols, &need)) return rc;
+  if (many == 0) return 0;
+  if (!in || !in_stride || !out || !ws || dtype < 0 || dtype > 2 || steps < 1 || steps > 100 || !(eps >= 0.f)) return NSA_E_ARG;
+  if (ws_bytes < need) return NSA_E_WORKSPACE;
+  // singular values start in [0, 1]: where the polynomial takes them has to stay in the planes' range
+  for (int i = 0; i <= 1024; ++i) {
+    double x = i / 1024.0;
+    for (int s = 0; s < steps; ++s) {
+      const double l = x * x, f = b * l + c * l * l;
+      if (!(std::fabs(f) <= 30.0)) return NSA_E_UNSUPPORTED;
+      x = x * (a + f);
+      if (!(std::fabs(x) <= 4.0)) return NSA_E_UNSUPPORTED;
+    }
+  }
+  const int each = dtype == 2 ? 4 : 2;
+  for (int32_t k = 0; k < many; ++k) {
+    if (!in[k] || !out[k] || in_stride[k] < cols[k] || ((uintptr_t)in[k] | (uintptr_t)out[k]) % each) return NSA_E_ARG;
+    if (cols[k] % 4 == 0 && (uintptr_t)out[k] % (4 * each)) return NSA_E_ARG;      // (rows of whole quads are stored as such)
+  }
+  NewtonStep s{};
+  s.a = a; s.b = b; s.c = c;
+  s.growth = std::max(0, (int)std::ceil(std::log2(std::max(1e-6f, std::fabs(a)))));
+  hipStream_t st = (hipStream_t)stream;
+  for (int small = 0; small < 2; ++small)
+    for (int32_t k = 0; k < many;) {
+      NewtonTable t{};
+      t.partial = (double*)ws;
+      t.shift = (int*)((char*)ws + (size_t)kNewtonMany * kNormChunks * 8);
+      t.ws = (char*)ws + newton_head();
+      size_t at = 0;
+      long largest = 0;
+      for (; k < many && t.many < kNewtonMany; ++k) {
+        if (is_small(rows[k], cols[k]) != (small == 1)) continue;
+        t.of[t.many++] = NewtonMatrix{in[k], out[k], (long)in_stride[k], (unsigned)(at / 256), rows[k], cols[k]};
+        at += (NewtonPlanes(rows[k], cols[k]).halves() * 2 + 255) / 256 * 256;
+        largest = std::max(largest, (long)rows[k] * cols[k]);
+      }
+      if (t.many == 0) break;
+      if (small) {
+        const dim3 grid((unsigned)t.many), block(64 * kSmallWaves);
+        if (dtype == 0) hipLaunchKernelGGL((newton_small_kernel<__bf16>), grid, block, 0, st, t, s, steps, eps);
+        else if (dtype == 1) hipLaunchKernelGGL((newton_small_kernel<_Float16>), grid, block, 0, st, t, s, steps, eps);
+        else hipLaunchKernelGGL((newton_small_kernel<float>), grid, block, 0, st, t, s, steps, eps);
+      } else {
+        t.chunks = (int)std::max<long>(1, std::min<long>(kNormChunks, largest / 16384));
+        if (dtype == 0) newton<__bf16>(t, s, steps, eps, st);
+        else if (dtype == 1) newton<_Float16>(t, s, steps, eps, st);
+        else newton<float>(t, s, steps, eps, st);
+      }
+      if (hipError_t e = hipGetLastError()) return (int)e;
+    }
+  return 0;
+}

@@ -8,7 +8,9 @@ missing library raise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
+import functools
 import struct
 from typing import NamedTuple, Optional
 
@@ -2596,3 +2598,195 @@ def qkv_prep_f32(qkv: Tensor, freqs: Tensor, k_positions: Tensor, v_positions: T
     if not torch.is_grad_enabled() and plain_call():
         return _qkv_prep_f32(*args)[0]                                      # (nothing to record: the node around it is 10 us of host time)
     return _QkvPrepF32.apply(*args)
+
+
+# ------------------------------------------------------------------ the two ends of a training step
+
+_LOSS_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _on(device: torch.device):
+    """The device that launches by address go to: the operands' own."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _unit_rows(t: Tensor) -> Tensor:
+    """A matrix whose rows are contiguous and do not overlap (a view where it is one already)."""
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _loss_desc(rows: int, weight: Tensor, x_stride: int, labels_int64: bool, ignore_index: int, reduction: int):
+    d = _lib.LossDesc(rows, weight.shape[1], weight.shape[0], _LOSS_TYPES[weight.dtype], reduction, labels_int64, ignore_index,
+                      max(x_stride, weight.shape[1]), max(weight.stride(0), weight.shape[1]))
+    sizes = C.c_size_t(), C.c_size_t(), C.c_size_t()
+    _lib.check(_lib.lib().nsa_loss_workspace_bytes(C.byref(d), _ptr(weight), *map(C.byref, sizes)), "nsa_loss_workspace_bytes")
+    return d, *(s.value for s in sizes)
+
+
+@torch.library.custom_op("nsa_amd::linear_cross_entropy_fwd", mutates_args=())
+def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_index: int, reduction: int) -> tuple[Tensor, Tensor]:
+    """(loss, what the gradients need): x 'n d', weight 'v d', labels 'n'; reduction 0 none, 1 mean, 2 sum."""
+    n = x.shape[0]
+    with _on(x.device):
+        x, weight, labels = _unit_rows(x), _unit_rows(weight), labels.contiguous()
+        d, state_bytes, fwd_bytes, _ = _loss_desc(n, weight, x.stride(0), labels.dtype == torch.int64, ignore_index, reduction)
+        loss = torch.empty((n,) if reduction == 0 else (), dtype=torch.float32, device=x.device)
+        state = torch.empty((state_bytes,), dtype=torch.uint8, device=x.device)
+        if loss.numel():
+            ws = torch.empty((fwd_bytes,), dtype=torch.uint8, device=x.device)
+            _lib.check(_lib.lib().nsa_loss_fwd(C.byref(d), _ptr(x), _ptr(weight), _ptr(labels), _ptr(state), state_bytes, _ptr(ws), fwd_bytes, _ptr(loss),
+                                               _stream()), "nsa_loss_fwd")
+    return loss, state
+
+
+@linear_cross_entropy_fwd.register_fake
+def _(x, weight, labels, ignore_index, reduction):
+    return x.new_empty((x.shape[0],) if reduction == 0 else (), dtype=torch.float32), x.new_empty((1,), dtype=torch.uint8)
+
+
+@torch.library.custom_op("nsa_amd::linear_cross_entropy_bwd", mutates_args=())
+def linear_cross_entropy_bwd(dloss: Tensor, x: Tensor, weight: Tensor, state: Tensor, ignore_index: int, reduction: int, want_dx: bool,
+                             want_dw: bool) -> tuple[Tensor, Tensor]:
+    """(dx 'n d', dw 'v d'), empty where not wanted.  (x itself is in the state; named here, its gradient's dependence on it is known.)"""
+    rows = x.shape[0]
+    make = torch.empty if rows else torch.zeros
+    with _on(weight.device):
+        dx = make((rows if want_dx else 0, weight.shape[1]), dtype=weight.dtype, device=weight.device)
+        dw = make(weight.shape if want_dw else (0, weight.shape[1]), dtype=weight.dtype, device=weight.device)
+        if rows and (want_dx or want_dw):
+            weight, dloss = _unit_rows(weight), dloss.to(torch.float32).contiguous()
+            d, state_bytes, _, bwd_bytes = _loss_desc(rows, weight, 0, True, ignore_index, reduction)
+            ws = torch.empty((bwd_bytes,), dtype=torch.uint8, device=weight.device)
+            _lib.check(_lib.lib().nsa_loss_bwd(C.byref(d), _ptr(weight), _ptr(state), state_bytes, _ptr(dloss), _ptr(ws), bwd_bytes,
+                                               _ptr(dx) if want_dx else 0, _ptr(dw) if want_dw else 0, _stream()), "nsa_loss_bwd")
+    return dx, dw
+
+
+@linear_cross_entropy_bwd.register_fake
+def _(dloss, x, weight, state, ignore_index, reduction, want_dx, want_dw):
+    d = weight.shape[1]
+    return weight.new_empty((x.shape[0] if want_dx else 0, d)), weight.new_empty((weight.shape[0] if want_dw else 0, d))
+
+
+def _loss_setup(ctx, inputs, output):
+    x, weight, labels, ignore_index, reduction = inputs
+    ctx.save_for_backward(x, weight, output[1])
+    ctx.args = ignore_index, reduction
+    ctx.set_materialize_grads(False)
+
+
+def _loss_backward(ctx, dloss, _):
+    if dloss is None:
+        return (None,) * 5
+    want_dx, want_dw = ctx.needs_input_grad[:2]
+    dx, dw = _direct_bwd(linear_cross_entropy_bwd)(dloss, *ctx.saved_tensors, *ctx.args, want_dx, want_dw)
+    return dx if want_dx else None, dw if want_dw else None, None, None, None
+
+
+linear_cross_entropy_fwd.register_autograd(_loss_backward, setup_context=_loss_setup)
+_linear_cross_entropy = _eager_function(linear_cross_entropy_fwd, _loss_setup, _loss_backward)
+
+
+def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, ignore_index: int = -100, reduction: str = "mean") -> Tensor:
+    """F.cross_entropy(F.linear(x, weight).float(), labels) over the last axis of x '... d' (the loss of transformer.py:326-330), without the
+    logits in memory: weight 'v d', labels '...' int64 or int32, x and weight both bf16, fp16 or fp32 on one device.  fp32, one value or
+    (reduction "none") one per row; rows labelled `ignore_index` count nothing and are not read.  Logits and sums are fp32 (F.linear would
+    round them to x's type first); gradients have x's and weight's type.  A label that is neither `ignore_index` nor in the vocabulary
+    makes its loss and the gradients NaN: it is known to the device only.  The gradients cannot be differentiated again."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction {reduction!r}, expected one of {sorted(_REDUCTIONS)}")
+    if x.is_cuda and torch.is_autocast_enabled():
+        dtype = torch.get_autocast_dtype("cuda")
+        x, weight = x.to(dtype), weight.to(dtype)
+    if not x.is_cuda or weight.device != x.device or labels.device != x.device:
+        raise RuntimeError("linear_cross_entropy: needs tensors on one GPU (HIP kernels, no CPU fallback)")
+    if x.dtype not in _LOSS_TYPES or weight.dtype != x.dtype:
+        raise RuntimeError(f"linear_cross_entropy: x {x.dtype}, weight {weight.dtype}: expected both bf16, both fp16 or both fp32")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or labels.shape != x.shape[:-1] or 0 in weight.shape:
+        raise RuntimeError(f"linear_cross_entropy: x {tuple(x.shape)}, weight {tuple(weight.shape)}, labels {tuple(labels.shape)}: expected '... d', "
+                           "'v d' and '...'")
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError(f"linear_cross_entropy: labels {labels.dtype}: expected int64 or int32")
+    loss, _ = _linear_cross_entropy(x.reshape(-1, x.shape[-1]), weight, labels.reshape(-1), int(ignore_index), _REDUCTIONS[reduction])
+    return loss.view(labels.shape) if reduction == "none" else loss
+
+
+def _newton_schulz(matrices, steps: int, a: float, b: float, c: float, eps: float):
+    """New tensors 'm n' or 'b m n' for those of `matrices` (one type, one device, none empty)."""
+    first = matrices[0]
+    with _on(first.device):
+        out, sizes, ins, strides, outs = [], [], [], [], []
+        for t in matrices:
+            rows, cols = t.shape[-2:]
+            if t.stride(-1) != 1 or t.stride(-2) < cols:
+                t = t.contiguous()
+            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            out.append(o)
+            each, at, to = t.element_size(), t.data_ptr(), o.data_ptr()
+            step = t.stride(0) * each if t.dim() == 3 else 0
+            for i in range(t.shape[0] if t.dim() == 3 else 1):
+                sizes.append((rows, cols))
+                ins.append(at + i * step)
+                outs.append(to + i * rows * cols * each)
+                strides.append(t.stride(-2))
+        many = len(sizes)
+        ints, longs, ptrs = C.c_int32 * many, C.c_int64 * many, C.c_void_p * many
+        rows, cols, ws = ints(*(r for r, _ in sizes)), ints(*(c for _, c in sizes)), C.c_size_t()
+        _lib.check(_lib.lib().nsa_newton_workspace_bytes(many, rows, cols, C.byref(ws)), "nsa_newton_workspace_bytes")
+        buf = torch.empty((ws.value,), dtype=torch.uint8, device=first.device)
+        _lib.check(_lib.lib().nsa_newton_schulz(many, rows, cols, ptrs(*ins), longs(*strides), ptrs(*outs), _LOSS_TYPES[first.dtype], steps, a, b, c, eps,
+                                                buf.data_ptr(), ws.value, _stream()), "nsa_newton_schulz")
+    return out
+
+
+@torch.library.custom_op("nsa_amd::newton_schulz", mutates_args=())
+def newton_schulz_op(matrices: list[Tensor], steps: int, a: float, b: float, c: float, eps: float) -> list[Tensor]:
+    return _newton_schulz(matrices, steps, a, b, c, eps)
+
+
+@newton_schulz_op.register_fake
+def _(matrices, steps, a, b, c, eps):
+    return [t.new_empty(t.shape) for t in matrices]
+
+
+@functools.lru_cache(maxsize=64)
+def _newton_coefficients(coefficients, steps: int) -> None:
+    """Singular values start in [0, 1]; where the polynomial takes them has to stay in the range that the kernels hold X in."""
+    a, b, c = coefficients
+    for i in range(1025):
+        x = i / 1024
+        for _ in range(steps):
+            f = b * x ** 2 + c * x ** 4
+            x *= a + f
+            if not (abs(f) <= 30 and abs(x) <= 4):
+                raise ValueError(f"newton_schulz: coefficients {coefficients} take the singular value {i / 1024:.3f} out of range in {steps} steps")
+
+
+def newton_schulz(updates, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315), eps: float = 1e-7):
+    """Orthogonalised updates, for optimizers: X = G / (|G| + eps) with the Frobenius norm, then `steps` times X <- a X + (b A + c A A) X, A = X X^T
+    (from the shorter side).  `updates`: a matrix, a batch '... m n' of them, or a list or tuple of either, bf16, fp16 or fp32; the result is laid
+    out alike, contiguous, in new tensors.  All matrices are in every launch, so a list costs little more than its largest member.  As exact
+    as fp32 products (see nsa_newton.hip), rounded once; no gradients."""
+    alone = isinstance(updates, Tensor)
+    given = [updates] if alone else list(updates)
+    coefficients = tuple(float(v) for v in coefficients)
+    if len(coefficients) != 3 or not 1 <= int(steps) <= 100 or not eps >= 0:
+        raise ValueError(f"newton_schulz: steps {steps}, coefficients {coefficients}, eps {eps}: expected 1 to 100 steps, three coefficients, eps >= 0")
+    _newton_coefficients(coefficients, int(steps))
+    for t in given:
+        if not t.is_cuda or t.device != given[0].device:
+            raise RuntimeError("newton_schulz: needs tensors on one GPU (HIP kernels, no CPU fallback)")
+        if t.dtype not in _LOSS_TYPES or t.dim() < 2:
+            raise RuntimeError(f"newton_schulz: {t.dtype} of shape {tuple(t.shape)}: expected bf16, fp16 or fp32 matrices '... m n'")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("newton_schulz has no gradient: call it under torch.no_grad()")
+    out = [None if t.numel() else torch.empty_like(t) for t in given]
+    call = newton_schulz_op if torch.compiler.is_compiling() else _newton_schulz
+    for dtype in dict.fromkeys(t.dtype for t in given):
+        at = [i for i, t in enumerate(given) if t.dtype == dtype and out[i] is None]
+        if at:
+            made = call([given[i] if given[i].dim() <= 3 else given[i].flatten(0, -3) for i in at], int(steps), *coefficients, float(eps))
+            for i, m in zip(at, made):
+                out[i] = m if given[i].dim() <= 3 else m.view(given[i].shape)
+    return out[0] if alone else type(updates)(out) if type(updates) in (list, tuple) else out

@@ -10,6 +10,9 @@ curve agrees with the fp32 oracle as closely.
 
 `GraphedStep` goes one further for fixed shapes: the forward and backward of the bf16 model are recorded once into a HIP
 graph and replayed per step (one launch instead of ~700); the optimizer stays outside the graph.
+
+`Muon` is an optimizer for the matrices among the parameters (the masters, or a model's own): momentum whose update is orthogonalised, all
+matrices of a step together (ops.newton_schulz).
 """
 from __future__ import annotations
 
@@ -107,3 +110,57 @@ class GraphedStep:
         self.ids.copy_(ids)
         self.graph.replay()
         return self.loss
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum with orthogonalised updates, for matrices (parameters of more axes are taken as first axis by the rest):
+
+        buffer <- momentum buffer + gradient;  update = gradient + momentum buffer (nesterov) or the buffer
+        p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / columns)) newton_schulz(update)
+
+    Embeddings, norm weights and biases belong to another optimizer; vectors are refused.
+
+        masters = Fp32Masters(model)
+        matrices = [m for m, (name, p) in zip(masters.masters, model.named_parameters()) if p.dim() == 2 and "emb" not in name]
+        muon = Muon(matrices, lr=0.02)
+    """
+
+    def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0., steps: int = 5,
+                 coefficients=(3.4445, -4.7750, 2.0315), eps: float = 1e-7):
+        if lr < 0 or weight_decay < 0 or not 0 <= momentum < 1:
+            raise ValueError(f"Muon: lr {lr}, momentum {momentum}, weight_decay {weight_decay}")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                                      coefficients=tuple(coefficients), eps=eps))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon takes matrices, got a parameter of shape {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        from . import ops
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            grads = [p.grad for p in params]
+            for p in params:
+                if "momentum_buffer" not in self.state[p]:
+                    self.state[p]["momentum_buffer"] = torch.zeros_like(p)
+            buffers = [self.state[p]["momentum_buffer"] for p in params]
+            torch._foreach_mul_(buffers, group["momentum"])
+            torch._foreach_add_(buffers, grads)
+            updates = torch._foreach_add(grads, buffers, alpha=group["momentum"]) if group["nesterov"] else buffers
+            updates = ops.newton_schulz([u.flatten(1) for u in updates], steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"])
+            if group["weight_decay"]:
+                torch._foreach_mul_(params, 1 - group["lr"] * group["weight_decay"])
+            torch._foreach_mul_(updates, [-group["lr"] * max(1., u.shape[0] / u.shape[1]) ** 0.5 for u in updates])
+            torch._foreach_add_(params, [u.view(p.shape) for u, p in zip(updates, params)])
+        return loss

@@ -22,7 +22,7 @@ def FeedForward(dim, expansion_factor=4.):
 class Transformer(nn.Module):
     def __init__(self, num_tokens, dim, depth, dim_head=64, heads=8, kv_heads=None, ff_expansion_factor=4.,
                  use_sparse_attn=True, causal=True, use_flex_sliding_window=False, use_flex_fine_selection=False,
-                 use_triton_fine_selection=False, sparse_attn_kwargs: dict | None = None):
+                 use_triton_fine_selection=False, sparse_attn_kwargs: dict | None = None, fused_loss=False):
         super().__init__()
         if not use_sparse_attn:
             raise NotImplementedError("only the sparse-attention model is provided (the dense baseline is not part of the hot path)")
@@ -35,6 +35,8 @@ class Transformer(nn.Module):
                                                              num_selected_blocks=4))
         self.token_emb = nn.Embedding(num_tokens, dim)
         self.causal = causal
+        # return_loss by ops.linear_cross_entropy: no logits in memory, and their values in fp32 rather than rounded to the model's type
+        self.fused_loss = fused_loss
         layers = []
         for _ in range(depth):
             attn = SparseAttention(dim=dim, dim_head=dim_head, heads=heads, kv_heads=kv_heads, causal=causal,
@@ -136,6 +138,9 @@ class Transformer(nn.Module):
             caches.append(layer_cache)
             tokens = attn_out + tokens
             tokens = self._feed_forward(ff, tokens)
+        if return_loss and self.fused_loss and SparseAttention._plain(self.to_logits, nn.Linear) and self.to_logits.bias is None:
+            from . import ops
+            return ops.linear_cross_entropy(self.norm(tokens), self.to_logits.weight, labels)
         logits = self.to_logits(self.norm(tokens))
         if not return_loss:
             return (logits, caches) if return_cache else logits
