@@ -28,13 +28,13 @@ struct LossPlan {
   int n, npad, kp, P;                     // rows and their capacity (a multiple of 64), features padded to 64, planes
   bool in_place;                          // the forward reads the weight where it lies
   int fwd_rows, bwd_rows;                 // vocabulary entries of a piece
-  int splits;                             // slices of the vocabulary that dx is summed from
+  int splits, w_splits;                   // slices of a piece's entries that dx is summed from, of the rows that dw is
   bool wide;                              // 256 x 256 tiles
   bool few;                               // tiles of 32 tokens
   size_t state, fwd, bwd;                 // bytes
   size_t s_map, s_place, s_label, s_lse, s_x;                          // offsets in the state
   size_t f_part, f_target, f_loss, f_w;                                // in the forward's workspace
-  size_t b_cells, b_g, b_x, b_wf, b_wg, b_grad, b_dx;                  // in the backward's
+  size_t b_cells, b_g, b_x, b_w, b_grad, b_dx, b_dw;                   // in the backward's
 };
 
 static size_t up(size_t v, size_t to) { return (v + to - 1) / to * to; }
@@ -42,7 +42,7 @@ static size_t up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   if (!d || d->rows < 0 || d->dim <= 0 || d->vocab <= 0 || d->dtype < 0 || d->dtype > 2 || d->reduction < 0 || d->reduction > 2) return NSA_E_ARG;
   if (d->x_stride < d->dim || d->w_stride < d->dim) return NSA_E_ARG;
-  if (d->rows > (1 << 24) || d->dim > (1 << 16) || d->vocab > (1 << 24)) return NSA_E_UNSUPPORTED;
+  if (d->rows > (1 << 24) || d->dim > (1 << 16) || d->vocab > (1 << 24) || std::max<long>(d->rows, d->vocab) * up(d->dim, 64) >> 33) return NSA_E_UNSUPPORTED;
   p.n = (int)d->rows;
   p.npad = (int)up(std::max<size_t>(p.n, 1), 64);
   p.kp = (int)up(d->dim, 64);
@@ -56,8 +56,10 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.fwd_rows = (int)std::min(v256, std::max<size_t>(256, ((size_t)256 << 20) / row / 256 * 256));
   // a piece's G: up to 256 MB
   p.bwd_rows = (int)std::min(v256, std::max<size_t>(1024, ((size_t)256 << 20) / ((size_t)p.P * p.npad * 2) / 1024 * 1024));
-  const size_t tile = p.wide ? 256 : 128, dx_tiles = up(p.kp, tile) / tile * (up(p.n, tile) / tile);
-  p.splits = (int)std::max<size_t>(1, std::min<size_t>({8, 512 / std::max<size_t>(1, dx_tiles), std::min<size_t>(p.bwd_rows, v64) / 512}));
+  const size_t tile = p.wide ? 256 : 128, dx_tiles = up(p.kp, tile) / tile * (up(p.npad, tile) / tile);
+  p.splits = (int)std::max<size_t>(1, std::min<size_t>({32, 512 / dx_tiles, std::min<size_t>(p.bwd_rows, v64) / 512}));
+  const size_t piece = std::min<size_t>(p.bwd_rows, v64), dw_tiles = up(p.kp, tile) / tile * (up(piece, tile) / tile);
+  p.w_splits = (int)std::max<size_t>(1, std::min<size_t>({64, 512 / dw_tiles, (size_t)p.npad / 256}));
   size_t at = CELLS * 4;
   auto take = [&](size_t bytes) { const size_t here = at; at = up(at + bytes, 256); return here; };
   at = up(at, 256);
@@ -77,10 +79,10 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.b_cells = take(CELLS * 4);
   p.b_g = take((size_t)p.npad * 4);
   p.b_x = take(d->dtype == 0 ? (size_t)p.npad * row : 0);
-  p.b_wf = take(p.in_place || d->dtype != 0 ? 0 : p.bwd_rows * row);
-  p.b_wg = take(p.bwd_rows * row);
+  p.b_w = take(p.bwd_rows * row);
   p.b_grad = take((size_t)p.P * p.npad * p.bwd_rows * 2);
   p.b_dx = take((size_t)p.splits * p.npad * p.kp * 4);
+  p.b_dw = take(p.w_splits > 1 ? p.w_splits * piece * p.kp * 4 : 0);
   p.bwd = at;
   return 0;
 }
@@ -154,40 +156,65 @@ template <class S> __device__ __forceinline__ void load_values(const S* p, int h
   }
 }
 
+// The largest of the work-group's values into *cell.  (Whoever finds a larger one there already has nothing to say: with an atomic a wave, 16384 of
+// them on one address, the kernel took 100 us for 8 MB.)
+__device__ __forceinline__ void largest_into(unsigned best, unsigned* cell) {
+  __shared__ unsigned best_s[4];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) best = max(best, (unsigned)__shfl_xor((int)best, o));
+  if ((threadIdx.x & 63) == 0) best_s[threadIdx.x >> 6] = best;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  best = max(max(best_s[0], best_s[1]), max(best_s[2], best_s[3]));
+  if (best > __hip_atomic_load(cell, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(cell, best);
+}
+__device__ __forceinline__ unsigned finite_bits(float v) {
+  const unsigned u = __builtin_bit_cast(unsigned, v) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;
+}
+
 // bits of the largest finite |value| of a matrix (of the rows that map names, if it is given) into *cell, which is zero or such bits
 template <class S>
 __global__ __launch_bounds__(256) void loss_largest_kernel(const S* src, long ld, int rows, int cols, int vec, const int* map, const unsigned* count, unsigned* cell) {
   const int live = count != nullptr ? (int)*count : rows;
-  const int per = (cols + 7) / 8;
+  const unsigned per = (cols + 7) / 8;
+  const bool flat = vec && map == nullptr && ld == cols && cols % 8 == 0;
   unsigned best = 0;
+#pragma unroll 4
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < (long)live * per; i += (long)gridDim.x * 256) {
-    const int r = (int)(i / per), c = (int)(i % per) * 8;
     float v[8];
-    load_values(src + (map != nullptr ? map[r] : r) * ld + c, cols - c, vec, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const unsigned u = __builtin_bit_cast(unsigned, v[e]) & 0x7fffffffu;
-      best = u < 0x7f800000u ? max(best, u) : best;
+    if (flat) {
+      load_values(src + 8 * i, 8, true, v);
+    } else {
+      const unsigned r = (unsigned)i / per, c = ((unsigned)i - r * per) * 8;
+      load_values(src + (map != nullptr ? map[r] : (int)r) * ld + c, cols - (int)c, vec, v);
     }
-  }
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) best = max(best, (unsigned)__shfl_xor((int)best, o));
-  if ((threadIdx.x & 63) == 0 && best != 0) atomicMax(cell, best);
+    for (int e = 0; e < 8; ++e) best = max(best, finite_bits(v[e]));
+  }
+  largest_into(best, cell);
 }
 
 // Rows (named by map, or all) as planes of kp columns, those past `cols` zero; rows past the last one up to a multiple of 64 zero too.
-// cell: the values are scaled below 2^15 by the power of two that suits its magnitude.
+// cell: the values are scaled below 2^15 by the power of two that suits its magnitude.  most: their largest magnitude goes there.
 template <class S, class D, int P>
 __global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld, int rows, int cols, int kp, int vec, const int* map, const unsigned* count,
-                                                          const unsigned* cell, D* dst, long plane) {
-  const int live = count != nullptr ? (int)*count : rows, per = kp / 8;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+                                                          const unsigned* cell, D* dst, long plane, unsigned* most) {
+  const int live = count != nullptr ? (int)*count : rows;
+  const unsigned per = kp / 8, i = blockIdx.x * 256 + threadIdx.x;      // (below 2^31: loss_plan)
   const int r = (int)(i / per), c = (int)(i % per) * 8;
-  if (r >= (live + 63) / 64 * 64) return;
+  if (blockIdx.x * 256 / per >= (unsigned)(live + 63) / 64 * 64) return;
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 0.f;
   if (r < live && c < cols) load_values(src + (map != nullptr ? map[r] : r) * ld + c, cols - c, vec, v);
+  if (most != nullptr) {
+    unsigned best = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) best = max(best, finite_bits(v[e]));
+    largest_into(best, most);
+  }
+  if (r >= (live + 63) / 64 * 64) return;
   const int shift = cell != nullptr ? plane_shift(*cell) : 0;
   typename PlaneVec<D>::x8 hi, lo;
 #pragma unroll
@@ -250,8 +277,8 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
   t.operand_b((const T*)G.x, G.x_plane, G.kp, n0, live);
   t.run(G.kp / Tiles::BK);
 
-  int unscale = 0;
-  if (Tiles::P == 2) unscale = -(plane_shift(*G.x_cell) + plane_shift(*G.w_cell));
+  constexpr bool SCALED = Tiles::P == 2 || GRAD;
+  const int unscale = SCALED && G.x_cell != nullptr ? -(plane_shift(*G.x_cell) + plane_shift(*G.w_cell)) : 0;
   const bool cut = m0 + Tiles::TM > G.vend;      // entries past the last one
   constexpr int PART = Tiles::TM / Tiles::WM;
   const int g_shift = GRAD ? kGradBits - plane_exponent(*G.g_cell) : 0;
@@ -261,7 +288,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
     const bool ok = token < live;
     const int label = ok ? G.label[token] : -1, own = label - (m0 + t.wm * PART);      // in this wave's part
     const bool hit = label >= 0 && own >= 0 && own < PART && ((own >> 2) & 1) == (t.lane >> 5);
-    if (Tiles::P == 2) {
+    if (SCALED) {
 #pragma unroll
       for (int i = 0; i < Tiles::MI; ++i)
 #pragma unroll
@@ -432,6 +459,7 @@ struct LossGradArgs {
   // dx
   float* sums;                        // [splits][npad][kp]
   int npad, per, first;               // steps of a split; first piece
+  int splits;                         // of dw
   // dw
   void* dw;
   long dw_ld;
@@ -453,26 +481,52 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dx_kernel(const LossGr
   t.operand_a(G.other, G.other_plane, G.kp, m0, G.kp);
   t.operand_b(G.grad, G.grad_plane, G.grad_ld, n0, live);
   t.run(steps, from);
-  // (this piece's power of two: all pieces share it)
+  // (all pieces share the power of two)
   const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.other_cell != nullptr ? plane_shift(*G.other_cell) : 0);
   float* sums = G.sums + (size_t)split * G.npad * G.kp;
 #pragma unroll
-  for (int j = 0; j < Tiles::NI; ++j) {
-    const int token = n0 + t.col_of(j);
-    if (token >= live) continue;
-#pragma unroll
-    for (int i = 0; i < Tiles::MI; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = m0 + t.row_of(i, q);
-        if (col >= G.kp) continue;
-        floatx4* at = reinterpret_cast<floatx4*>(sums + (size_t)token * G.kp + col);
-        floatx4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_ldexpf(t.acc[i][j][4 * q + e], shift);
-        *at = G.first ? v : *at + v;
-      }
+  for (int j = 0; j < Tiles::NI; ++j)
+    t.template rows_of<float>(shared, [&](int i, int e) { return __builtin_ldexpf(t.acc[i][j][e], shift); }, [&](int r, int c, floatx4 v) {
+      const int token = n0 + t.col_of(j) - (t.lane & 31) + r, col = m0 + t.wm * Tiles::W + c;
+      if (token >= live || col >= G.kp) return;
+      floatx4* at = reinterpret_cast<floatx4*>(sums + (size_t)token * G.kp + col);
+      *at = G.first ? v : *at + v;
+    });
+}
+
+// dw of the piece: features (registers) by entries of the vocabulary (lanes), over all rows or (SLICES, unscaled fp32 [splits][entries][kp]) a slice of them
+template <class Tiles, class O, bool SLICES>
+__global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dw_kernel(const LossGradArgs G) {
+  __shared__ __align__(1024) char shared[Tiles::LDS];
+  const int tiles = G.tiles_m * G.tiles_n, split = SLICES ? blockIdx.x / tiles : 0;
+  const TileAt tile = tile_at(SLICES ? blockIdx.x % tiles : blockIdx.x, G.tiles_m, G.tiles_n, 4);
+  const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN, live = (int)*G.count, steps = (live + Tiles::BK - 1) / Tiles::BK;
+  Tiles t;
+  t.init(shared);
+  t.operand_a(G.other, G.other_plane, G.kp, m0, G.kp);
+  t.operand_b(G.grad, G.grad_plane, G.grad_ld, n0, G.grad_ld);
+  if (SLICES) {
+    const int per = (steps + G.splits - 1) / G.splits, from = min(steps, split * per);
+    t.run(min(per, steps - from), from);
+  } else {
+    t.run(steps);
   }
+  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.other_cell != nullptr ? plane_shift(*G.other_cell) : 0);
+  O* dw = (O*)G.dw + (SLICES ? (size_t)split * G.entries * G.dw_ld : 0);
+#pragma unroll
+  for (int j = 0; j < Tiles::NI; ++j)
+    t.template rows_of<O>(shared, [&](int i, int e) { return __builtin_ldexpf(t.acc[i][j][e], shift); }, [&](int r, int c, auto v) {
+      const int entry = n0 + t.col_of(j) - (t.lane & 31) + r, col = m0 + t.wm * Tiles::W + c;
+      if (entry >= G.entries || col >= G.dim) return;
+      O* at = dw + (size_t)entry * G.dw_ld + col;
+      if (G.vec) {
+        *reinterpret_cast<decltype(v)*>(at) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < (int)(16 / sizeof(O)); ++e)
+          if (col + e < G.dim) at[e] = v[e];
+      }
+    });
 }
 
 template <class O> __device__ __forceinline__ void store_quad(O* p, floatx4 v, int have, bool vec) {
@@ -493,48 +547,19 @@ template <class O> __device__ __forceinline__ void store_quad(O* p, floatx4 v, i
   }
 }
 
-// dw of the piece: features (registers) by entries of the vocabulary (lanes), over all tokens
-template <class Tiles, class O>
-__global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dw_kernel(const LossGradArgs G) {
-  __shared__ __align__(1024) char shared[Tiles::LDS];
-  const TileAt tile = tile_at(blockIdx.x, G.tiles_m, G.tiles_n, 4);
-  const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN, live = (int)*G.count;
-  Tiles t;
-  t.init(shared);
-  t.operand_a(G.other, G.other_plane, G.kp, m0, G.kp);
-  t.operand_b(G.grad, G.grad_plane, G.grad_ld, n0, G.grad_ld);
-  t.run((live + Tiles::BK - 1) / Tiles::BK);
-  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.other_cell != nullptr ? plane_shift(*G.other_cell) : 0);
-#pragma unroll
-  for (int j = 0; j < Tiles::NI; ++j) {
-    const int entry = n0 + t.col_of(j);
-    if (entry >= G.entries) continue;
-    O* row = (O*)G.dw + (size_t)entry * G.dw_ld;
-#pragma unroll
-    for (int i = 0; i < Tiles::MI; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = m0 + t.row_of(i, q);
-        if (col >= G.dim) continue;
-        floatx4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_ldexpf(t.acc[i][j][4 * q + e], shift);
-        store_quad(row + col, v, G.dim - col, G.vec);
-      }
-  }
-}
-
-// dx [n][dim] from the slices; rows that do not count are zero
+// rows of dx or dw [n][dim] from `splits` slices [size][kp]; place: the slices' row of each, -1: zeros
 template <class O>
-__global__ __launch_bounds__(256) void loss_dx_rows_kernel(const float* sums, int splits, int npad, int kp, int n, int dim, int vec, const int* place, O* dx) {
-  const int per = (dim + 3) / 4;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long)n * per) return;
-  const int row = (int)(i / per), c = (int)(i % per) * 4, at = place[row];
+__global__ __launch_bounds__(256) void loss_rows_of_slices_kernel(const float* sums, int splits, int size, int kp, int n, int dim, int vec, const int* place, O* to) {
+  const unsigned per = (dim + 3) / 4, i = blockIdx.x * 256 + threadIdx.x;      // (below 2^31: loss_plan)
+  const unsigned row = i / per, c = (i - row * per) * 4;
+  if (row >= (unsigned)n) return;
+  const int at = place != nullptr ? place[row] : (int)row;
   floatx4 v = {0.f, 0.f, 0.f, 0.f};
-  if (at >= 0)
-    for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const floatx4*>(sums + ((size_t)s * npad + at) * kp + c);
-  store_quad(dx + (size_t)row * dim + c, v, dim - c, vec);
+  if (at >= 0) {
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const floatx4*>(sums + ((size_t)s * size + at) * kp + c);
+  }
+  store_quad(to + (size_t)row * dim + c, v, dim - (int)c, vec);
 }
 
 // ------------------------------------------------------------------------------------ launches
@@ -566,26 +591,20 @@ static void launch_tiles(const LossPlan& p, const LossTileArgs& a, hipStream_t s
   else if (p.wide) launch_tile<typename L::Wide, GRAD>(a, st);
   else launch_tile<typename L::Small, GRAD>(a, st);
 }
-template <bool GRAD>
-static void logits_tiles(const nsa_loss_desc* d, const LossPlan& p, const LossTileArgs& a, hipStream_t st) {
-  if (d->dtype == 0) launch_tiles<B16, 1, GRAD>(p, a, st);
-  else if (d->dtype == 1) launch_tiles<H16, 1, GRAD>(p, a, st);
-  else launch_tiles<H16, 2, GRAD>(p, a, st);
-}
 
 static unsigned blocks_for(long work) { return (unsigned)std::max<long>(1, (work + 255) / 256); }
 static bool vectors(const void* p, long ld, int each) { return ((uintptr_t)p & 15) == 0 && ld * each % 16 == 0; }
 
 template <class S, class D, int P>
 static void planes(const void* src, long ld, int rows, int rows_cap, int cols, int kp, const int* map, const unsigned* count, const unsigned* cell, void* dst,
-                   long plane, hipStream_t st) {
+                   long plane, hipStream_t st, unsigned* most = nullptr) {
   hipLaunchKernelGGL((loss_planes_kernel<S, D, P>), dim3(blocks_for((long)up(rows_cap, 64) * kp / 8)), dim3(256), 0, st, (const S*)src, ld, rows, cols, kp,
-                     (int)vectors(src, ld, sizeof(S)), map, count, cell, (D*)dst, plane);
+                     (int)vectors(src, ld, sizeof(S)), map, count, cell, (D*)dst, plane, most);
 }
 template <class S>
 static void largest(const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, unsigned* cell, hipStream_t st) {
   const long work = (long)rows * ((cols + 7) / 8);
-  hipLaunchKernelGGL((loss_largest_kernel<S>), dim3(std::min(4096u, blocks_for(work))), dim3(256), 0, st, (const S*)src, ld, rows, cols,
+  hipLaunchKernelGGL((loss_largest_kernel<S>), dim3(std::min(1024u, blocks_for(work))), dim3(256), 0, st, (const S*)src, ld, rows, cols,
                      (int)vectors(src, ld, sizeof(S)), map, count, cell);
 }
 // the weight's rows from v0 as the forward's planes
@@ -594,6 +613,19 @@ static void forward_weight(const nsa_loss_desc* d, const LossPlan& p, const void
   if (d->dtype == 0) planes<B16, B16, 1>((const B16*)weight + (long)v0 * d->w_stride, d->w_stride, rows, rows, d->dim, p.kp, nullptr, nullptr, nullptr, dst, plane, st);
   else if (d->dtype == 1) planes<H16, H16, 1>((const H16*)weight + (long)v0 * d->w_stride, d->w_stride, rows, rows, d->dim, p.kp, nullptr, nullptr, nullptr, dst, plane, st);
   else planes<float, H16, 2>((const float*)weight + (long)v0 * d->w_stride, d->w_stride, rows, rows, d->dim, p.kp, nullptr, nullptr, cell, dst, plane, st);
+}
+
+template <int P, class O, bool SLICES>
+static void dw_tiles(const LossPlan& p, const LossGradArgs& q, dim3 grid, hipStream_t st) {
+  if (p.wide) hipLaunchKernelGGL((loss_dw_kernel<typename GradTiles<P>::WideW, O, SLICES>), grid, dim3(512), 0, st, q);
+  else hipLaunchKernelGGL((loss_dw_kernel<typename GradTiles<P>::SmallW, O, SLICES>), grid, dim3(256), 0, st, q);
+}
+static void rows_of_slices(const nsa_loss_desc* d, const float* sums, int splits, int size, int kp, int n, const int* place, void* to, hipStream_t st) {
+  const dim3 grid(blocks_for((long)n * ((d->dim + 3) / 4)));
+  const int vec = d->dim % 4 == 0 && (uintptr_t)to % (d->dtype == 2 ? 16 : 8) == 0;
+  if (d->dtype == 0) hipLaunchKernelGGL((loss_rows_of_slices_kernel<B16>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, vec, place, (B16*)to);
+  else if (d->dtype == 1) hipLaunchKernelGGL((loss_rows_of_slices_kernel<H16>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, vec, place, (H16*)to);
+  else hipLaunchKernelGGL((loss_rows_of_slices_kernel<float>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, vec, place, (float*)to);
 }
 
 }  // namespace nsa
@@ -634,7 +666,7 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
     } else if (d->dtype == 1) {
       planes<H16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, s + p.s_x, x_plane, st);
     } else {
-      planes<B16, B16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, s + p.s_x, x_plane, st);
+      planes<B16, B16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, s + p.s_x, x_plane, st, cells + CELL_X);
     }
     const int rows = p.in_place ? d->vocab : p.fwd_rows;
     for (long v0 = 0; v0 < d->vocab; v0 += rows) {
@@ -652,7 +684,9 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
       }
       a.x = s + p.s_x; a.x_plane = x_plane; a.kp = p.kp; a.vocab = d->vocab; a.n = p.n; a.npad = p.npad;
       a.count = count; a.x_cell = xc; a.w_cell = wc; a.label = label; a.part = (float2*)(w + p.f_part); a.target = target;
-      logits_tiles<false>(d, p, a, st);
+      if (d->dtype == 0) launch_tiles<B16, 1, false>(p, a, st);
+      else if (d->dtype == 1) launch_tiles<H16, 1, false>(p, a, st);
+      else launch_tiles<H16, 2, false>(p, a, st);
     }
     const int part = p.few ? 32 : p.wide ? 128 : 64, tile = p.few ? 128 : p.wide ? 256 : 128;
     const int parts = (d->vocab + tile - 1) / tile * (tile / part);
@@ -680,19 +714,14 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const vo
   const unsigned* count = kept + CELL_ROWS;
   float* g = (float*)(w + p.b_g);
   hipLaunchKernelGGL(loss_weights_kernel, dim3(1), dim3(1024), 0, st, dloss, (int)d->reduction, count, map, g, cells);
-  // the operands of both products in fp16: x once, w with each piece
+  // all operands in fp16: x once, w with each piece
   const long x_plane = (long)p.npad * p.kp;
   const void* xg = s + p.s_x;
-  const unsigned *xc = d->dtype == 2 ? kept + CELL_X : nullptr, *wc = d->dtype == 2 ? kept + CELL_W : nullptr;
+  const unsigned *xc = d->dtype != 1 ? kept + CELL_X : nullptr, *wc = d->dtype == 2 ? kept + CELL_W : d->dtype == 0 ? cells + CELL_W : nullptr;
   if (d->dtype == 0) {
-    xc = cells + CELL_X;
-    wc = cells + CELL_W;
-    if (dw) {
-      largest<B16>(s + p.s_x, p.kp, p.n, p.kp, nullptr, count, cells + CELL_X, st);
-      planes<B16, H16, 1>(s + p.s_x, p.kp, p.n, p.n, p.kp, p.kp, nullptr, count, xc, w + p.b_x, x_plane, st);
-      xg = w + p.b_x;
-    }
-    if (dx) largest<B16>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
+    planes<B16, H16, 1>(s + p.s_x, p.kp, p.n, p.n, p.kp, p.kp, nullptr, count, xc, w + p.b_x, x_plane, st);
+    xg = w + p.b_x;
+    largest<B16>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
   }
   const int each = d->dtype == 2 ? 4 : 2;
   for (long v0 = 0; v0 < d->vocab; v0 += p.bwd_rows) {
@@ -702,23 +731,16 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const vo
     const int entries = a.vend - a.v0, ld = (int)up(entries, 64);
     const long w_plane = (long)p.kp * ld;
     const char* from = (const char*)weight + v0 * d->w_stride * each;
-    if (d->dtype == 0) {
-      if (dx) planes<B16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, w + p.b_wg, w_plane, st);
-      if (!p.in_place) planes<B16, B16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, nullptr, w + p.b_wf, w_plane, st);
-    } else if (d->dtype == 1) {
-      planes<H16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, nullptr, w + p.b_wg, w_plane, st);
-    } else {
-      planes<float, H16, 2>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, w + p.b_wg, w_plane, st);
-    }
-    const bool direct = p.in_place && d->dtype == 0;
-    a.w = direct ? (const void*)from : d->dtype == 0 ? w + p.b_wf : w + p.b_wg;
-    a.w_ld = direct ? d->w_stride : p.kp;
-    a.w_plane = w_plane;
-    a.x = s + p.s_x; a.x_plane = x_plane; a.kp = p.kp; a.vocab = d->vocab; a.n = p.n; a.npad = p.npad;
-    a.count = count; a.x_cell = d->dtype == 2 ? xc : nullptr; a.w_cell = d->dtype == 2 ? wc : nullptr; a.label = label;
+    if (d->dtype == 0) planes<B16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, w + p.b_w, w_plane, st);
+    else if (d->dtype == 1) planes<H16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, nullptr, w + p.b_w, w_plane, st);
+    else planes<float, H16, 2>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, w + p.b_w, w_plane, st);
+    a.w = w + p.b_w; a.w_ld = p.kp; a.w_plane = w_plane;
+    a.x = xg; a.x_plane = x_plane; a.kp = p.kp; a.vocab = d->vocab; a.n = p.n; a.npad = p.npad;
+    a.count = count; a.x_cell = xc; a.w_cell = wc; a.label = label;
     a.lse = (const float*)(s + p.s_lse); a.g = g; a.g_cell = cells + CELL_G;
     a.grad = (H16*)(w + p.b_grad); a.grad_plane = (long)p.npad * ld; a.grad_ld = ld;
-    logits_tiles<true>(d, p, a, st);
+    if (d->dtype == 2) launch_tiles<H16, 2, true>(p, a, st);
+    else launch_tiles<H16, 1, true>(p, a, st);
 
     LossGradArgs q{};
     q.grad = a.grad; q.grad_plane = a.grad_plane; q.grad_ld = ld; q.kp = p.kp; q.dim = d->dim; q.entries = entries;
@@ -727,7 +749,7 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const vo
     q.tiles_m = (p.kp + tile - 1) / tile;
     if (dx) {
       const int bk = p.P == 2 ? 32 : 64;
-      q.other = (const H16*)(w + p.b_wg); q.other_plane = w_plane; q.other_cell = wc;
+      q.other = (const H16*)(w + p.b_w); q.other_plane = w_plane; q.other_cell = wc;
       q.tiles_n = (p.n + tile - 1) / tile;
       q.sums = (float*)(w + p.b_dx); q.per = (ld / bk + p.splits - 1) / p.splits; q.first = v0 == 0;
       const dim3 grid((unsigned)(q.tiles_m * q.tiles_n * p.splits));
@@ -739,27 +761,20 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const vo
     if (dw) {
       q.other = (const H16*)xg; q.other_plane = x_plane; q.other_cell = xc;
       q.tiles_n = (entries + tile - 1) / tile;
-      q.dw = (char*)dw + v0 * d->dim * each; q.dw_ld = d->dim; q.vec = d->dim % 4 == 0;
-      const dim3 grid((unsigned)(q.tiles_m * q.tiles_n));
-      if (d->dtype == 2) {
-        if (p.wide) hipLaunchKernelGGL((loss_dw_kernel<GradTiles<2>::WideW, float>), grid, dim3(512), 0, st, q);
-        else hipLaunchKernelGGL((loss_dw_kernel<GradTiles<2>::SmallW, float>), grid, dim3(256), 0, st, q);
-      } else if (d->dtype == 1) {
-        if (p.wide) hipLaunchKernelGGL((loss_dw_kernel<GradTiles<1>::WideW, H16>), grid, dim3(512), 0, st, q);
-        else hipLaunchKernelGGL((loss_dw_kernel<GradTiles<1>::SmallW, H16>), grid, dim3(256), 0, st, q);
-      } else {
-        if (p.wide) hipLaunchKernelGGL((loss_dw_kernel<GradTiles<1>::WideW, B16>), grid, dim3(512), 0, st, q);
-        else hipLaunchKernelGGL((loss_dw_kernel<GradTiles<1>::SmallW, B16>), grid, dim3(256), 0, st, q);
-      }
+      const bool slices = p.w_splits > 1;
+      char* to = (char*)dw + v0 * d->dim * each;
+      q.splits = p.w_splits;
+      q.dw = slices ? w + p.b_dw : to; q.dw_ld = slices ? p.kp : d->dim; q.dim = slices ? p.kp : d->dim;
+      q.vec = slices || ((long)d->dim * each % 16 == 0 && (uintptr_t)dw % 16 == 0);
+      const dim3 grid((unsigned)(q.tiles_m * q.tiles_n * p.w_splits));
+      if (slices && p.P == 1) dw_tiles<1, float, true>(p, q, grid, st);
+      else if (slices) dw_tiles<2, float, true>(p, q, grid, st);
+      else if (d->dtype == 0) dw_tiles<1, B16, false>(p, q, grid, st);
+      else if (d->dtype == 1) dw_tiles<1, H16, false>(p, q, grid, st);
+      else dw_tiles<2, float, false>(p, q, grid, st);
+      if (slices) rows_of_slices(d, (const float*)(w + p.b_dw), p.w_splits, entries, p.kp, entries, nullptr, to, st);
     }
   }
-  if (dx) {
-    const dim3 grid(blocks_for((long)p.n * ((d->dim + 3) / 4)));
-    const float* sums = (const float*)(w + p.b_dx);
-    const int vec = d->dim % 4 == 0;
-    if (d->dtype == 0) hipLaunchKernelGGL((loss_dx_rows_kernel<B16>), grid, dim3(256), 0, st, sums, p.splits, p.npad, p.kp, p.n, d->dim, vec, place, (B16*)dx);
-    else if (d->dtype == 1) hipLaunchKernelGGL((loss_dx_rows_kernel<H16>), grid, dim3(256), 0, st, sums, p.splits, p.npad, p.kp, p.n, d->dim, vec, place, (H16*)dx);
-    else hipLaunchKernelGGL((loss_dx_rows_kernel<float>), grid, dim3(256), 0, st, sums, p.splits, p.npad, p.kp, p.n, d->dim, vec, place, (float*)dx);
-  }
+  if (dx) rows_of_slices(d, (const float*)(w + p.b_dx), p.splits, p.npad, p.kp, p.n, place, dx, st);
   return (int)hipGetLastError();
 }

@@ -339,11 +339,20 @@ __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const Ne
   for (int i = tid; i < M * xp; i += 64 * kSmallWaves) x[i] = 0.f;
   __syncthreads();
   double sum = 0.0;
-  for (int i = tid; i < K.rows * K.cols; i += 64 * kSmallWaves) {
-    const int r = i / K.cols, c = i % K.cols;
-    const float v = (float)((const S*)K.in)[r * K.stride + c];
-    x[L.turned ? c * xp + r : r * xp + c] = v;
-    sum += (double)v * (double)v;
+  const unsigned total = K.rows * K.cols, cols = K.cols;
+  for (unsigned first = 0; first < total; first += 8 * 64 * kSmallWaves) {
+    float v[8];      // (eight loads in flight: one by one, 24 rounds of them were a third of the kernel's time)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned i = first + e * 64 * kSmallWaves + tid, r = i / cols;
+      v[e] = i < total ? (float)((const S*)K.in)[r * K.stride + (i - r * cols)] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned i = first + e * 64 * kSmallWaves + tid, r = i / cols, c = i - r * cols;
+      if (i < total) x[L.turned ? c * xp + r : r * xp + c] = v[e];
+      sum += (double)v[e] * (double)v[e];
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
@@ -391,6 +400,7 @@ __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const Ne
     for (int cb = wave; cb < N / 32; cb += kSmallWaves) {
       floatx16 acc[2] = {zero_acc(), zero_acc()};
       float* col = x + 32 * cb + l;
+#pragma unroll 4
       for (int g = 0; g < M / 8; ++g) {
         floatx4 v;
 #pragma unroll
@@ -411,8 +421,9 @@ __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const Ne
     }
     __syncthreads();
   }
-  for (int i = tid; i < K.rows * K.cols; i += 64 * kSmallWaves) {
-    const int r = i / K.cols, c = i % K.cols;
+#pragma unroll 4
+  for (unsigned i = tid; i < total; i += 64 * kSmallWaves) {
+    const unsigned r = i / cols, c = i - r * cols;
     ((S*)K.out)[i] = (S)x[L.turned ? c * xp + r : r * xp + c];
   }
 }
@@ -449,12 +460,32 @@ static long fill(NewtonTable& t, int size, Count count) {
   t.tile0[t.many] = (int)at;
   return at;
 }
-// the largest tiles that give every CU one
-template <class Count>
-static int tile_size(NewtonTable& t, Count count) {
-  for (int size = 256; size > 64; size /= 2)
-    if (fill(t, size, count) >= 256) return size;
-  return 64;
+// The tile size whose launch should end first.  256 x 256 tiles use the matrix instructions best, but a CU has one at a time, and what is left
+// over of a last round waits for whole tiles; of the smaller ones it has two, and a round is shorter.  Time of a launch: its tiles'
+// steps over all places, in rounds of the shortest tile, not less than the longest; a step of a tile of 256, 128, 64 costs a CU's place
+// 100, 58, 29 (measured; two places a CU for the latter).
+template <class Count, class Steps>
+static int tile_size(const NewtonTable& t, Count count, Steps steps) {
+  int best = 0;
+  double least = 0.;
+  for (int size = 256, cost = 0; size >= 64; size /= 2) {
+    cost = size == 256 ? 100 : size == 128 ? 58 : 29;
+    const double places = size == 256 ? 256. : 512.;
+    double sum = 0., longest = 0., shortest = 1e30;
+    for (int k = 0; k < t.many; ++k) {
+      const NewtonPlanes p(t.of[k].rows, t.of[k].cols);
+      const double s = steps(p);
+      sum += s * count(p, size);
+      longest = std::max(longest, s);
+      shortest = std::min(shortest, s);
+    }
+    const double time = cost * std::max(longest, std::ceil(sum / places / shortest) * shortest);
+    if (best == 0 || time < least) {
+      best = size;
+      least = time;
+    }
+  }
+  return best;
 }
 
 template <int SIZE, bool POLY>
@@ -480,13 +511,18 @@ static void newton(NewtonTable& t, NewtonStep s, int steps, float eps, hipStream
   hipLaunchKernelGGL((newton_norm_kernel<S>), dim3((unsigned)t.chunks, (unsigned)t.many), dim3(256), 0, st, t);
   const long begin = fill(t, 64, update_tiles);
   hipLaunchKernelGGL((newton_begin_kernel<S>), dim3((unsigned)begin), dim3(256), 0, st, t, eps);
-  const int sq = tile_size(t, square_tiles), un = tile_size(t, update_tiles);
+  const auto long_side = [](const NewtonPlanes& p) { return (double)p.np; };
+  const auto short_side = [](const NewtonPlanes& p) { return (double)p.mp; };
+  const int gram = tile_size(t, square_tiles, long_side), poly = tile_size(t, square_tiles, short_side), un = tile_size(t, update_tiles, short_side);
   for (s.step = 0; s.step < steps; ++s.step) {
     s.from = s.step & 1;
     s.last = s.step == steps - 1;
-    if (sq == 256) { square<256, false>(t, s, st); square<256, true>(t, s, st); }
-    else if (sq == 128) { square<128, false>(t, s, st); square<128, true>(t, s, st); }
-    else { square<64, false>(t, s, st); square<64, true>(t, s, st); }
+    if (gram == 256) square<256, false>(t, s, st);
+    else if (gram == 128) square<128, false>(t, s, st);
+    else square<64, false>(t, s, st);
+    if (poly == 256) square<256, true>(t, s, st);
+    else if (poly == 128) square<128, true>(t, s, st);
+    else square<64, true>(t, s, st);
     if (un == 256) update_any<256, S>(t, s, st);
     else if (un == 128) update_any<128, S>(t, s, st);
     else update_any<64, S>(t, s, st);
@@ -560,6 +596,8 @@ extern "C" int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_
         largest = std::max(largest, (long)rows[k] * cols[k]);
       }
       if (t.many == 0) break;
+      // (long contractions first: what is left at the end of a launch is short)
+      std::stable_sort(t.of, t.of + t.many, [](const NewtonMatrix& u, const NewtonMatrix& v) { return std::max(u.rows, u.cols) > std::max(v.rows, v.cols); });
       if (small) {
         const dim3 grid((unsigned)t.many), block(64 * kSmallWaves);
         if (dtype == 0) hipLaunchKernelGGL((newton_small_kernel<__bf16>), grid, block, 0, st, t, s, steps, eps);

@@ -139,6 +139,37 @@ struct TileProduct {
     fence();
   }
 
+  // Columns col_of(j) of the result, each W = TM / WM consecutive values of a row in memory from row_of(0, 0) on: value(i, e) is that of register
+  // e of acc[i][j], store(r, c, v) takes the 16 bytes from value c on of column r of this wave's 32 - consecutive lanes consecutive
+  // bytes, W of a row together, where lanes as they are would write 16 bytes of 32 rows at a time.  Through this wave's own part of LDS.
+  static constexpr int W = TM / WM;
+  template <class O, class Value, class Store>
+  __device__ __forceinline__ void rows_of(char* shared, Value value, Store store) const {
+    constexpr int PER = 16 / sizeof(O), CHUNKS = W / PER, MASK = (CHUNKS < 16 ? CHUNKS : 16) - 1;
+    static_assert(WAVES * 32 * W * sizeof(O) <= LDS, "");
+    typedef __attribute__((__vector_size__(16))) O ox;
+    typedef __attribute__((__vector_size__(4 * sizeof(O)))) O o4;
+    char* own = shared + (wm * WN + wn) * 32 * W * sizeof(O);
+    const int l = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        o4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (O)value(i, 4 * q + e);
+        const int first = 32 * i + 8 * q + 4 * h;
+        *reinterpret_cast<o4*>(own + l * W * sizeof(O) + 16 * ((first / PER) ^ (l & MASK)) + first % PER * sizeof(O)) = v;
+      }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int n = 0; n < 32 * CHUNKS / 64; ++n) {
+      const int r = (64 * n + lane) / CHUNKS, c = (64 * n + lane) % CHUNKS;
+      store(r, c * PER, *reinterpret_cast<const ox*>(own + r * W * sizeof(O) + 16 * (c ^ (r & MASK))));
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+
   // two planes: the small products are summed by themselves, where there are registers for it, so that a leading sum is rounded once a
   // product of 16 and not three times
   static constexpr bool APART = P == 2 && MI * NI <= 4;
