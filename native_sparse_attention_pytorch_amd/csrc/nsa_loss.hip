@@ -567,14 +567,14 @@ __global__ __launch_bounds__(256) void loss_rows_of_slices_kernel(const float* s
 typedef __bf16 B16;
 typedef _Float16 H16;
 template <class T, int P> struct LogitTiles {
-  typedef TileProduct<T, P, ROWS, ROWS, 256, 256, 2, 4, P == 2 ? 32 : 64, 2> Wide;
+  typedef TileProduct<T, P, ROWS, ROWS, 256, 256, 2, 4, 32, P == 2 ? 2 : 4> Wide;
   typedef TileProduct<T, P, ROWS, ROWS, 128, 128, 2, 2, P == 2 ? 32 : 64, 2> Small;
   typedef TileProduct<T, P, ROWS, ROWS, 128, 32, 4, 1, 64, P == 2 ? 2 : 4> Few;
 };
 template <int P> struct GradTiles {
-  typedef TileProduct<H16, P, COLUMNS, ROWS, 256, 256, 2, 4, P == 2 ? 32 : 64, 2> WideX;
+  typedef TileProduct<H16, P, COLUMNS, ROWS, 256, 256, 2, 4, 32, P == 2 ? 2 : 4> WideX;
   typedef TileProduct<H16, P, COLUMNS, ROWS, 128, 128, 2, 2, P == 2 ? 32 : 64, 2> SmallX;
-  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 256, 256, 2, 4, P == 2 ? 32 : 64, 2> WideW;
+  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 256, 256, 2, 4, 32, P == 2 ? 2 : 4> WideW;
   typedef TileProduct<H16, P, COLUMNS, COLUMNS, 128, 128, 2, 2, P == 2 ? 32 : 64, 2> SmallW;
 };
 
@@ -748,7 +748,7 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const vo
     const int tile = p.wide ? 256 : 128;
     q.tiles_m = (p.kp + tile - 1) / tile;
     if (dx) {
-      const int bk = p.P == 2 ? 32 : 64;
+      const int bk = p.P == 2 || p.wide ? 32 : 64;
       q.other = (const H16*)(w + p.b_w); q.other_plane = w_plane; q.other_cell = wc;
       q.tiles_n = (p.n + tile - 1) / tile;
       q.sums = (float*)(w + p.b_dx); q.per = (ld / bk + p.splits - 1) / p.splits; q.first = v0 == 0;

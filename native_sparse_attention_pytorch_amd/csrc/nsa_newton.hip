@@ -1,12 +1,13 @@
 // Orthogonalised updates: the polar factor of a matrix by Newton-Schulz products,
 //
-//   X <- G / (|G| + eps) (turned so that it is not taller than wide), `steps` times:  A = X X^T,  B = b A + c A A,  X <- a X + B X,
+//   X <- G / (|G| + eps) (turned so that it is not taller than wide), `steps` times:  A = X X^T,  B = a + b A + c A A,  X <- B X,
 //
 // for a list of matrices of any sizes, all of them in each launch: the norms, the first planes, then three launches a step.
 //
 // X, A and B are held as two fp16 halves each (22 bits; nsa_tiles.hpp).  Directions of small singular values grow by a = 3.4 a step, and what
 // a step's rounding adds to them grows alike: against 64 bits the result is 4e-5 off with bf16 halves, 3 % with bf16 alone, and 6e-7 with
-// these, less than with fp32 products (1.6e-6 at 512 x 512).  Scales: X 2^(12 + s), A and B 2^(10 + 2 s).  s is 0 unless |G| is small beside eps:
+// these, less than with fp32 products (1.6e-6 at 512 x 512).  a stands on the diagonal of B and not beside the product: one pass over X less, and
+// a rounding of what is left of a + b A + c A A, not of its parts.  Scales: X 2^(12 + s), A 2^(10 + 2 s), B 2^10.  s is 0 unless |G| is small beside eps:
 // then X starts so small that fp16 would lose it, and s is what brings its norm to 1; it falls by the bits of a with each step, so nothing grows out
 // of range.  The entry checks that singular values up to 1 stay below 4 for the given coefficients.
 //
@@ -149,7 +150,7 @@ struct NewtonStep {
 };
 __device__ __forceinline__ int shift_at(const NewtonTable& G, const NewtonStep& S, int k, int step) { return max(0, G.shift[k] - S.growth * step); }
 
-// four consecutive halves pairs in memory
+// four consecutive values of both planes
 __device__ __forceinline__ floatx4 load_halves(const _Float16* p, long plane) {
   const f16x4 hi = *reinterpret_cast<const f16x4*>(p), lo = *reinterpret_cast<const f16x4*>(p + plane);
   floatx4 v;
@@ -157,34 +158,27 @@ __device__ __forceinline__ floatx4 load_halves(const _Float16* p, long plane) {
   for (int e = 0; e < 4; ++e) v[e] = (float)hi[e] + (float)lo[e];
   return v;
 }
-// Two register quads of a result's column as 16 bytes of a row of each plane (join_quads)
-__device__ __forceinline__ void store_halves(_Float16* p, long plane, const floatx4 (&v)[2]) {
-  f16x4 hi[2], lo[2];
+__device__ __forceinline__ void store_halves(_Float16* p, long plane, floatx4 v) {
+  f16x4 hi, lo;
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const Halves h = halves_of(v[u][e]);
-      hi[u][e] = h.hi;
-      lo[u][e] = h.lo;
-    }
-  const uintx4 a = join_quads(__builtin_bit_cast(uintx2, hi[0]), __builtin_bit_cast(uintx2, hi[1]));
-  const uintx4 b = join_quads(__builtin_bit_cast(uintx2, lo[0]), __builtin_bit_cast(uintx2, lo[1]));
-  *reinterpret_cast<uintx4*>(p) = a;
-  *reinterpret_cast<uintx4*>(p + plane) = b;
+  for (int e = 0; e < 4; ++e) {
+    const Halves h = halves_of(v[e]);
+    hi[e] = h.hi;
+    lo[e] = h.lo;
+  }
+  *reinterpret_cast<f16x4*>(p) = hi;
+  *reinterpret_cast<f16x4*>(p + plane) = lo;
 }
 
-// POLY 0: A = X X^T; 1: B = b A + c A A.  Tiles on and below the diagonal.
+// POLY 0: A = X X^T; 1: B = a + b A + c A A.  Tiles on and below the diagonal.
 template <class Tiles, bool POLY>
 __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_square_kernel(const NewtonTable G, const NewtonStep S) {
   __shared__ __align__(1024) char shared[Tiles::LDS];
   const int k = matrix_of(G, blockIdx.x);
   const NewtonPlanes L(G.of[k].rows, G.of[k].cols);
-  const int nth = blockIdx.x - G.tile0[k];
-  int tm = (int)((sqrtf(8.f * nth + 1.f) - 1.f) * 0.5f);
-  while ((tm + 1) * (tm + 2) / 2 <= nth) ++tm;
-  while (tm * (tm + 1) / 2 > nth) --tm;
-  const int tn = nth - tm * (tm + 1) / 2, m0 = tm * Tiles::TM, n0 = tn * Tiles::TN;
+  const int rows = (L.m + Tiles::TM - 1) / Tiles::TM;
+  const TileAt tile = triangle_in(xcd_run(blockIdx.x - G.tile0[k], rows * (rows + 1) / 2), rows);
+  const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN;
   _Float16* base = planes_of(G, k);
   const _Float16* x = base + (S.from ? 2 * L.x_plane() : 0);
   _Float16* A = base + 4 * L.x_plane();
@@ -200,47 +194,45 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_square_kernel(const 
     t.operand_b(x, L.x_plane(), L.np, n0, L.m);
     t.run(L.np / Tiles::BK);
   }
-  const float unit = POLY ? __builtin_ldexpf(S.c, -10 - 2 * shift_at(G, S, k, S.step)) : 0x1p-14f;
+  const int s = POLY ? shift_at(G, S, k, S.step) : 0;
+  const float unit = POLY ? __builtin_ldexpf(S.c, -10 - 4 * s) : 0x1p-14f, linear = __builtin_ldexpf(S.b, -2 * s), diagonal = S.a * 0x1p10f;
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j) {
-    const int col = n0 + t.col_of(j);
+    if (tile.m != tile.n) {
+      // above the diagonal: a register's value of 32 lanes is a run of a row
+      const int col = n0 + t.col_of(j);
 #pragma unroll
-    for (int i = 0; i < Tiles::MI; ++i) {
+      for (int i = 0; i < Tiles::MI; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; q += 2) {
-        floatx4 v[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int row = m0 + t.row_of(i, q + u);
-          floatx4 old = {0.f, 0.f, 0.f, 0.f};
-          if (POLY && col < L.m && row < L.mp) old = load_halves(A + (long)col * L.mp + row, L.a_plane());
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float f = t.acc[i][j][4 * (q + u) + e] * unit;
-            v[u][e] = row + e < L.m && col < L.m ? POLY ? __builtin_fmaf(S.b, old[e], f) : f : 0.f;
-          }
+        for (int e = 0; e < 16; ++e) {
+          const int row = m0 + t.row_of(i, e >> 2) + (e & 3);
+          if (row >= L.m || col >= L.mp) continue;
+          const long at = (long)row * L.mp + col;
+          float v = t.acc[i][j][e] * unit;
+          if (POLY) v = __builtin_fmaf(linear, (float)A[at] + (float)A[at + L.a_plane()], v);
+          const Halves h = halves_of(col < L.m ? v : 0.f);
+          out[at] = h.hi;
+          out[at + L.a_plane()] = h.lo;
         }
-        if (tm != tn && col < L.mp) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int row = m0 + t.row_of(i, q + u) + e;
-              if (row >= L.m) continue;
-              const Halves h = halves_of(v[u][e]);
-              out[(long)row * L.mp + col] = h.hi;
-              out[(long)row * L.mp + col + L.a_plane()] = h.lo;
-            }
-        }
-        // (a lane and its partner of the exchange have the same column, and rows of the same block of 32: both store or neither)
-        const int at = m0 + t.wm * (Tiles::TM / Tiles::WM) + 32 * i + 8 * q + 8 * (t.lane >> 5);
-        if (at < L.mp && col < L.m) store_halves(out + (long)col * L.mp + at, L.a_plane(), v);
-      }
     }
+    t.template rows_of<float>(shared, [&](int i, int e) { return t.acc[i][j][e]; }, [&](int r, int c, floatx4 v) {
+      const int col = n0 + t.col_of(j) - (t.lane & 31) + r, row = m0 + t.wm * Tiles::W + c;
+      if (col >= L.m || row >= L.mp) return;
+      const long at = (long)col * L.mp + row;
+      floatx4 old = {0.f, 0.f, 0.f, 0.f};
+      if (POLY) old = load_halves(A + at, L.a_plane());
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] *= unit;
+        if (POLY) v[e] = __builtin_fmaf(linear, old[e], v[e]) + (row + e == col ? diagonal : 0.f);
+        if (row + e >= L.m) v[e] = 0.f;
+      }
+      store_halves(out + at, L.a_plane(), v);
+    });
   }
 }
 
-// X <- a X + B X (the other buffer; LAST: the result as it was given), columns of X (registers) by its rows (lanes)
+// X <- B X (the other buffer; LAST: the result as it was given), columns of X (registers) by its rows (lanes)
 template <class Tiles, bool LAST, class O>
 __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_update_kernel(const NewtonTable G, const NewtonStep S) {
   __shared__ __align__(1024) char shared[Tiles::LDS];
@@ -260,50 +252,47 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_update_kernel(const 
   t.operand_b(B, L.a_plane(), L.mp, n0, L.m);
   t.run(L.mp / Tiles::BK);
   const int s = shift_at(G, S, k, S.step), s2 = shift_at(G, S, k, S.step + 1);
-  const float unit = __builtin_ldexpf(1.f, -10 - 2 * s), scale = __builtin_ldexpf(1.f, LAST ? -12 - s : s2 - s);
+  const float unit = __builtin_ldexpf(1.f, -10 + (LAST ? -12 - s : s2 - s));
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j) {
-    const int row = n0 + t.col_of(j);
+    if (LAST && L.turned) {
+      // a register's value of 32 lanes is a run of a row of the result
+      const int row = n0 + t.col_of(j);
+      if (row >= L.m) continue;
 #pragma unroll
-    for (int i = 0; i < Tiles::MI; ++i) {
+      for (int i = 0; i < Tiles::MI; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; q += 2) {
-        floatx4 v[2];
+        for (int q = 0; q < 4; ++q) {
+          const int col = m0 + t.row_of(i, q);
+          if (col >= L.n) continue;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int col = m0 + t.row_of(i, q + u);
-          floatx4 old = {0.f, 0.f, 0.f, 0.f};
-          const bool ok = row < L.m && col < L.np;
-          if (ok) old = load_halves(x + (long)row * L.np + col, L.x_plane());
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[u][e] = ok ? scale * __builtin_fmaf(S.a, old[e], t.acc[i][j][4 * (q + u) + e] * unit) : 0.f;
-          if (LAST && ok) {
-            if (L.turned) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (col + e < L.n) ((O*)M.out)[(long)(col + e) * M.cols + row] = (O)v[u][e];
-            } else {
-              O* p = (O*)M.out + (long)row * M.cols + col;
-              typedef __attribute__((__vector_size__(4 * sizeof(O)))) O ox4;
-              if (M.cols % 4 == 0 && col < L.n) {
-                ox4 o;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = (O)v[u][e];
-                *reinterpret_cast<ox4*>(p) = o;
-              } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (col + e < L.n) p[e] = (O)v[u][e];
-              }
-            }
-          }
+          for (int e = 0; e < 4; ++e)
+            if (col + e < L.n) ((O*)M.out)[(long)(col + e) * M.cols + row] = (O)(t.acc[i][j][4 * q + e] * unit);
         }
-        if (!LAST) {
-          const int at = m0 + t.wm * (Tiles::TM / Tiles::WM) + 32 * i + 8 * q + 8 * (t.lane >> 5);
-          if (at < L.np && row < L.mp) store_halves(next + (long)row * L.np + at, L.x_plane(), v);
-        }
-      }
+      continue;
     }
+    t.template rows_of<float>(shared, [&](int i, int e) { return t.acc[i][j][e]; }, [&](int r, int c, floatx4 v) {
+      const int row = n0 + t.col_of(j) - (t.lane & 31) + r, col = m0 + t.wm * Tiles::W + c;
+      if (row >= (LAST ? L.m : L.mp) || col >= (LAST ? L.n : L.np)) return;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = row < L.m ? v[e] * unit : 0.f;      // (rows past the last one are zeros)
+      if (!LAST) {
+        store_halves(next + (long)row * L.np + col, L.x_plane(), v);
+        return;
+      }
+      O* p = (O*)M.out + (long)row * M.cols + col;
+      typedef __attribute__((__vector_size__(4 * sizeof(O)))) O ox4;
+      ox4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = (O)v[e];
+      if (M.cols % 4 == 0) {
+        *reinterpret_cast<ox4*>(p) = o;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < L.n) p[e] = o[e];
+      }
+    });
   }
 }
 
@@ -431,18 +420,28 @@ __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const Ne
 // ------------------------------------------------------------------------------------ launches
 
 typedef _Float16 H16;
+// Tiles of a launch.  Time of a round of them on all places, in us for each of the contraction index and beside that (measured from 512 to 4096).
+// 128: eight waves and four stages in one work-group a CU, as fast as two work-groups of four and two (1.05 PFLOP/s) with half the time to a
+// round; 64: two work-groups a CU, or (DEEP) one of four stages where there are no more tiles than CUs (31 us instead of 52 at 4096).
+enum NewtonSize { WIDE, MIDDLE, SMALL, DEEP, SIZES };
+struct SizeCost { int tile, places; double each, beside; };
+static constexpr SizeCost kSizes[SIZES] = {{256, 256, 0.0785, 7.0}, {128, 256, 0.0238, 3.5}, {64, 512, 0.0136, 2.7}, {64, 256, 0.0069, 3.4}};
 template <int SIZE> struct NewtonTiles;
-template <> struct NewtonTiles<256> {
+template <> struct NewtonTiles<WIDE> {
   typedef TileProduct<H16, 2, ROWS, ROWS, 256, 256, 2, 4, 32, 2> Square;
   typedef TileProduct<H16, 2, COLUMNS, ROWS, 256, 256, 2, 4, 32, 2> Update;
 };
-template <> struct NewtonTiles<128> {
-  typedef TileProduct<H16, 2, ROWS, ROWS, 128, 128, 2, 2, 32, 2> Square;
-  typedef TileProduct<H16, 2, COLUMNS, ROWS, 128, 128, 2, 2, 32, 2> Update;
+template <> struct NewtonTiles<MIDDLE> {
+  typedef TileProduct<H16, 2, ROWS, ROWS, 128, 128, 4, 2, 32, 4> Square;
+  typedef TileProduct<H16, 2, COLUMNS, ROWS, 128, 128, 4, 2, 32, 4> Update;
 };
-template <> struct NewtonTiles<64> {
+template <> struct NewtonTiles<SMALL> {
   typedef TileProduct<H16, 2, ROWS, ROWS, 64, 64, 2, 2, 64, 2> Square;
   typedef TileProduct<H16, 2, COLUMNS, ROWS, 64, 64, 2, 2, 64, 2> Update;
+};
+template <> struct NewtonTiles<DEEP> {
+  typedef TileProduct<H16, 2, ROWS, ROWS, 64, 64, 2, 2, 64, 4> Square;
+  typedef TileProduct<H16, 2, COLUMNS, ROWS, 64, 64, 2, 2, 64, 4> Update;
 };
 
 static long square_tiles(const NewtonPlanes& p, int size) {
@@ -460,27 +459,23 @@ static long fill(NewtonTable& t, int size, Count count) {
   t.tile0[t.many] = (int)at;
   return at;
 }
-// The tile size whose launch should end first.  256 x 256 tiles use the matrix instructions best, but a CU has one at a time, and what is left
-// over of a last round waits for whole tiles; of the smaller ones it has two, and a round is shorter.  Time of a launch: its tiles'
-// steps over all places, in rounds of the shortest tile, not less than the longest; a step of a tile of 256, 128, 64 costs a CU's place
-// 100, 58, 29 (measured; two places a CU for the latter).
+// The tiles whose launch should end first: all tiles' time over the places, in rounds of the shortest, not less than the longest.
 template <class Count, class Steps>
 static int tile_size(const NewtonTable& t, Count count, Steps steps) {
   int best = 0;
   double least = 0.;
-  for (int size = 256, cost = 0; size >= 64; size /= 2) {
-    cost = size == 256 ? 100 : size == 128 ? 58 : 29;
-    const double places = size == 256 ? 256. : 512.;
+  for (int size = 0; size < SIZES; ++size) {
+    const SizeCost& c = kSizes[size];
     double sum = 0., longest = 0., shortest = 1e30;
     for (int k = 0; k < t.many; ++k) {
       const NewtonPlanes p(t.of[k].rows, t.of[k].cols);
-      const double s = steps(p);
-      sum += s * count(p, size);
-      longest = std::max(longest, s);
-      shortest = std::min(shortest, s);
+      const double one = steps(p) * c.each + c.beside;
+      sum += one * count(p, c.tile);
+      longest = std::max(longest, one);
+      shortest = std::min(shortest, one);
     }
-    const double time = cost * std::max(longest, std::ceil(sum / places / shortest) * shortest);
-    if (best == 0 || time < least) {
+    const double time = std::max(longest, std::ceil(sum / c.places / shortest) * shortest);
+    if (size == 0 || time < least) {
       best = size;
       least = time;
     }
@@ -491,13 +486,20 @@ static int tile_size(const NewtonTable& t, Count count, Steps steps) {
 template <int SIZE, bool POLY>
 static void square(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
   typedef typename NewtonTiles<SIZE>::Square Tiles;
-  const long tiles = fill(t, SIZE, square_tiles);
+  const long tiles = fill(t, Tiles::TM, square_tiles);
   hipLaunchKernelGGL((newton_square_kernel<Tiles, POLY>), dim3((unsigned)tiles), dim3(Tiles::THREADS), 0, st, t, s);
+}
+template <bool POLY>
+static void square_any(int size, NewtonTable& t, const NewtonStep& s, hipStream_t st) {
+  if (size == WIDE) square<WIDE, POLY>(t, s, st);
+  else if (size == MIDDLE) square<MIDDLE, POLY>(t, s, st);
+  else if (size == SMALL) square<SMALL, POLY>(t, s, st);
+  else square<DEEP, POLY>(t, s, st);
 }
 template <int SIZE, bool LAST, class O>
 static void update(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
   typedef typename NewtonTiles<SIZE>::Update Tiles;
-  const long tiles = fill(t, SIZE, update_tiles);
+  const long tiles = fill(t, Tiles::TM, update_tiles);
   hipLaunchKernelGGL((newton_update_kernel<Tiles, LAST, O>), dim3((unsigned)tiles), dim3(Tiles::THREADS), 0, st, t, s);
 }
 template <int SIZE, class O>
@@ -517,15 +519,12 @@ static void newton(NewtonTable& t, NewtonStep s, int steps, float eps, hipStream
   for (s.step = 0; s.step < steps; ++s.step) {
     s.from = s.step & 1;
     s.last = s.step == steps - 1;
-    if (gram == 256) square<256, false>(t, s, st);
-    else if (gram == 128) square<128, false>(t, s, st);
-    else square<64, false>(t, s, st);
-    if (poly == 256) square<256, true>(t, s, st);
-    else if (poly == 128) square<128, true>(t, s, st);
-    else square<64, true>(t, s, st);
-    if (un == 256) update_any<256, S>(t, s, st);
-    else if (un == 128) update_any<128, S>(t, s, st);
-    else update_any<64, S>(t, s, st);
+    square_any<false>(gram, t, s, st);
+    square_any<true>(poly, t, s, st);
+    if (un == WIDE) update_any<WIDE, S>(t, s, st);
+    else if (un == MIDDLE) update_any<MIDDLE, S>(t, s, st);
+    else if (un == SMALL) update_any<SMALL, S>(t, s, st);
+    else update_any<DEEP, S>(t, s, st);
   }
 }
 

@@ -199,13 +199,21 @@ struct TileProduct {
       b += B.step;
     }
     x8 fa[2][P][MI], fb[2][P][NI];
+    // the operand with fewer parts first, and with all of it each part of the other: products begin as soon as their operands arrive
+    constexpr bool A_FIRST = MI <= NI;
     auto read = [&](unsigned stage, int ks, int into) {
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i) fa[into][p][i] = A.read(stage + p * OpA::PLANE, i, ks);
+        for (int p = 0; p < P; ++p) {
+          if (A_FIRST == (u == 0)) {
 #pragma unroll
-        for (int j = 0; j < NI; ++j) fb[into][p][j] = B.read(stage + A_BYTES + p * OpB::PLANE, j, ks);
+            for (int i = 0; i < MI; ++i) fa[into][p][i] = A.read(stage + p * OpA::PLANE, i, ks);
+          } else {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) fb[into][p][j] = B.read(stage + A_BYTES + p * OpB::PLANE, j, ks);
+          }
+        }
       }
     };
     if (AHEAD) {
@@ -227,15 +235,13 @@ struct TileProduct {
 #pragma unroll
         for (int q = 0; q < PRODUCTS; ++q)
 #pragma unroll
-          for (int i = 0; i < MI; ++i)
+          for (int v = 0; v < MI * NI; ++v) {
+            const int i = A_FIRST ? v % MI : v / NI, j = A_FIRST ? v / MI : v % NI, n = (ks * PRODUCTS + q) * MI * NI + v;
+            floatx16& sum = APART && q > 0 ? small[APART ? i : 0][APART ? j : 0] : acc[i][j];
+            sum = mma(fa[ks & 1][q == 2 ? P - 1 : 0][i], fb[ks & 1][q == 1 ? P - 1 : 0][j], sum);
 #pragma unroll
-            for (int j = 0; j < NI; ++j) {
-              floatx16& sum = APART && q > 0 ? small[APART ? i : 0][APART ? j : 0] : acc[i][j];
-              sum = mma(fa[ks & 1][q == 2 ? P - 1 : 0][i], fb[ks & 1][q == 1 ? P - 1 : 0][j], sum);
-              const int n = ((ks * PRODUCTS + q) * MI + i) * NI + j;
-#pragma unroll
-              for (int c = n * LOADS / MFMAS; c < (n + 1) * LOADS / MFMAS; ++c) copy(c, a, b, to, lanes);
-            }
+            for (int c = n * LOADS / MFMAS; c < (n + 1) * LOADS / MFMAS; ++c) copy(c, a, b, to, lanes);
+          }
       }
       a += A.step;
       b += B.step;
@@ -250,14 +256,29 @@ struct TileProduct {
   }
 };
 
-// Tile `id` of a grid of tiles_m x tiles_n: one run of tiles to each XCD (work-groups go to the 8 XCDs in turn, each with an L2 of its own),
-// in bands of `band` columns, along the rows of the band first: the CUs of an XCD share the operands of a few rows and columns of tiles.
+// Of `total` tiles, work-group id's: one run of them to each XCD (work-groups go to the 8 XCDs in turn, each with an L2 of its own).
+__device__ __forceinline__ int xcd_run(int id, int total) {
+  const int per = total / 8, rest = total % 8, x = id & 7;
+  return x * per + min(x, rest) + (id >> 3);
+}
+// Tile `id` of a grid of tiles_m x tiles_n, in bands of `band` columns, along the rows of the band first: the CUs of an XCD share the operands of
+// a few rows and columns of tiles.
 struct TileAt { int m, n; };
-__device__ __forceinline__ TileAt tile_at(int id, int tiles_m, int tiles_n, int band) {
-  const int total = tiles_m * tiles_n, per = total / 8, rest = total % 8, x = id & 7;
-  const int nth = x * per + min(x, rest) + (id >> 3);
+__device__ __forceinline__ TileAt tile_in(int nth, int tiles_m, int tiles_n, int band) {
   const int g = nth / (band * tiles_m), in = nth - g * band * tiles_m, width = min(band, tiles_n - g * band);
   return TileAt{in / width, g * band + in % width};
+}
+__device__ __forceinline__ TileAt tile_at(int id, int tiles_m, int tiles_n, int band) { return tile_in(xcd_run(id, tiles_m * tiles_n), tiles_m, tiles_n, band); }
+// The same of the tiles on and below the diagonal of `tiles` rows: bands of 8 rows, column by column, then the triangle at the band's end.
+__device__ __forceinline__ TileAt triangle_in(int nth, int tiles) {
+  int g = (int)(sqrtf((float)nth) * 0.176776695f);      // 32 g^2 + 4 g tiles lie before band g
+  while (32 * (g + 1) * (g + 1) + 4 * (g + 1) <= nth) ++g;
+  while (32 * g * g + 4 * g > nth) --g;
+  const int in = nth - 32 * g * g - 4 * g, rows = min(8, tiles - 8 * g);
+  if (in < rows * 8 * g) return TileAt{8 * g + in % rows, in / rows};
+  int left = in - rows * 8 * g, c = 0;
+  while (left >= rows - c) left -= rows - c++;
+  return TileAt{8 * g + c + left, 8 * g + c};
 }
 
 // The power of two (its exponent) that scales values below the given magnitude (bits of an fp32, finite) to below 2^15
