@@ -30,8 +30,11 @@ struct NewtonMatrix {
 };
 struct NewtonTable {
   NewtonMatrix of[kNewtonMany];
-  int tile0[kNewtonMany + 1];      // first tile of each, in the launch at hand
-  int many, chunks;
+  // The launch at hand: every XCD (work-groups go to them in turn) has a queue of places; entry e has those from first[e] on, and begins
+  // with matrix base[e].  One matrix, spread over all XCDs, or eight of them, one to an XCD (its operands are then read by that one alone).
+  int first[kNewtonMany + 1];
+  uint8_t base[kNewtonMany], kind[kNewtonMany];      // kind: spread, eight, eight in reverse
+  int entries, many, chunks;
   char* ws;
   double* partial;                 // [many][kNormChunks]
   int* shift;                      // s of each
@@ -55,15 +58,30 @@ struct NewtonPlanes {
 };
 __device__ __forceinline__ _Float16* planes_of(const NewtonTable& t, int k) { return (_Float16*)(t.ws + (size_t)t.of[k].at * 256); }
 
-__device__ __forceinline__ int matrix_of(const NewtonTable& t, int tile) {
-  int k = 0, past = t.many;
-  while (past - k > 1) {
-    const int mid = (k + past) / 2;
-    if (tile >= t.tile0[mid]) k = mid;
+enum { SPREAD, EIGHT, REVERSED };
+// The matrix (-1: none) and its tile that a work-group makes; count(planes): tiles of a matrix
+struct NewtonPlace { int k, nth; };
+template <class Count>
+__device__ __forceinline__ NewtonPlace place_of(const NewtonTable& t, Count count) {
+  const int i = blockIdx.x >> 3, x = blockIdx.x & 7;
+  int e = 0, past = t.entries;
+  while (past - e > 1) {
+    const int mid = (e + past) / 2;
+    if (i >= t.first[mid]) e = mid;
     else past = mid;
   }
-  return k;
+  const int at = i - t.first[e], base = t.base[e], kind = t.kind[e], k = kind == SPREAD ? base : base + (kind == EIGHT ? x : 7 - x);
+  const int total = count(NewtonPlanes(t.of[k].rows, t.of[k].cols));
+  if (kind != SPREAD) return NewtonPlace{at < total ? k : -1, at};
+  // (turned by the entry: small ones do not all begin on the same XCD)
+  const int turn = (x + e) & 7, per = total / 8, rest = total % 8;
+  return NewtonPlace{at < per + (turn < rest) ? k : -1, turn * per + min(turn, rest) + at};
 }
+__host__ __device__ inline int square_tiles(const NewtonPlanes& p, int size) {
+  const int t = (p.m + size - 1) / size;
+  return t * (t + 1) / 2;
+}
+__host__ __device__ inline int update_tiles(const NewtonPlanes& p, int size) { return (p.np + size - 1) / size * ((p.mp + size - 1) / size); }
 
 template <class S>
 __global__ __launch_bounds__(256) void newton_norm_kernel(const NewtonTable G) {
@@ -104,10 +122,12 @@ template <class S>
 __global__ __launch_bounds__(256) void newton_begin_kernel(const NewtonTable G, float eps) {
   __shared__ float tile_s[64][65];
   __shared__ double sums[4];
-  const int k = matrix_of(G, blockIdx.x), tid = threadIdx.x;
+  const NewtonPlace place = place_of(G, [](const NewtonPlanes& p) { return update_tiles(p, 64); });
+  if (place.k < 0) return;
+  const int k = place.k, at = place.nth, tid = threadIdx.x;
   const NewtonMatrix M = G.of[k];
   const NewtonPlanes L(M.rows, M.cols);
-  const int at = blockIdx.x - G.tile0[k], wide = L.np / 64, r0 = at / wide * 64, c0 = at % wide * 64;
+  const int wide = L.np / 64, r0 = at / wide * 64, c0 = at % wide * 64;
   double sum = 0.0;
   for (int i = tid; i < G.chunks; i += 256) sum += G.partial[k * kNormChunks + i];
 #pragma unroll
@@ -174,10 +194,11 @@ __device__ __forceinline__ void store_halves(_Float16* p, long plane, floatx4 v)
 template <class Tiles, bool POLY>
 __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_square_kernel(const NewtonTable G, const NewtonStep S) {
   __shared__ __align__(1024) char shared[Tiles::LDS];
-  const int k = matrix_of(G, blockIdx.x);
+  const NewtonPlace place = place_of(G, [](const NewtonPlanes& p) { return square_tiles(p, Tiles::TM); });
+  if (place.k < 0) return;
+  const int k = place.k;
   const NewtonPlanes L(G.of[k].rows, G.of[k].cols);
-  const int rows = (L.m + Tiles::TM - 1) / Tiles::TM;
-  const TileAt tile = triangle_in(xcd_run(blockIdx.x - G.tile0[k], rows * (rows + 1) / 2), rows);
+  const TileAt tile = triangle_in(place.nth, (L.m + Tiles::TM - 1) / Tiles::TM);
   const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN;
   _Float16* base = planes_of(G, k);
   const _Float16* x = base + (S.from ? 2 * L.x_plane() : 0);
@@ -236,11 +257,13 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_square_kernel(const 
 template <class Tiles, bool LAST, class O>
 __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_update_kernel(const NewtonTable G, const NewtonStep S) {
   __shared__ __align__(1024) char shared[Tiles::LDS];
-  const int k = matrix_of(G, blockIdx.x);
+  const NewtonPlace place = place_of(G, [](const NewtonPlanes& p) { return update_tiles(p, Tiles::TM); });
+  if (place.k < 0) return;
+  const int k = place.k;
   const NewtonMatrix M = G.of[k];
   const NewtonPlanes L(M.rows, M.cols);
   const int tiles_n = (L.mp + Tiles::TN - 1) / Tiles::TN, tiles_m = (L.np + Tiles::TM - 1) / Tiles::TM;
-  const TileAt tile = tile_at(blockIdx.x - G.tile0[k], tiles_m, tiles_n, 4);
+  const TileAt tile = tile_in(place.nth, tiles_m, tiles_n, 4);
   const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN;
   _Float16* base = planes_of(G, k);
   const _Float16* x = base + (S.from ? 2 * L.x_plane() : 0);
@@ -444,19 +467,36 @@ template <> struct NewtonTiles<DEEP> {
   typedef TileProduct<H16, 2, COLUMNS, ROWS, 64, 64, 2, 2, 64, 4> Update;
 };
 
-static long square_tiles(const NewtonPlanes& p, int size) {
-  const long t = (p.m + size - 1) / size;
-  return t * (t + 1) / 2;
-}
-static long update_tiles(const NewtonPlanes& p, int size) { return ((long)p.np + size - 1) / size * (((long)p.mp + size - 1) / size); }
-template <class Count>
-static long fill(NewtonTable& t, int size, Count count) {
-  long at = 0;
-  for (int k = 0; k < t.many; ++k) {
-    t.tile0[k] = (int)at;
-    at += count(NewtonPlanes(t.of[k].rows, t.of[k].cols), size);
+// The queues of a launch with tiles of kSizes[size], and their length.  Matrices go to the XCDs by eights, back and forth, where that leaves no XCD with
+// more than an eighth above the mean; what is over, and large ones, are spread.  (The byte-level model's 24: A = X X^T 60 -> us.)
+template <class Count, class Steps>
+static int fill(NewtonTable& t, int size, Count count, Steps steps) {
+  const SizeCost& c = kSizes[size];
+  double load[8] = {}, sum = 0.;
+  const int eights = t.many / 8;
+  for (int k = 0; k < 8 * eights; ++k) {
+    const NewtonPlanes p(t.of[k].rows, t.of[k].cols);
+    const double time = (steps(p) * c.each + c.beside) * count(p, c.tile);
+    load[k / 8 % 2 ? 7 - k % 8 : k % 8] += time;
+    sum += time;
   }
-  t.tile0[t.many] = (int)at;
+  const bool by_eights = eights > 0 && *std::max_element(load, load + 8) <= sum / 8 * 1.125;
+  int at = 0;
+  t.entries = 0;
+  for (int k = 0; k < t.many;) {
+    const bool eight = by_eights && k < 8 * eights;
+    int places = 0;
+    for (int i = k; i < k + (eight ? 8 : 1); ++i) {
+      const int tiles = count(NewtonPlanes(t.of[i].rows, t.of[i].cols), c.tile);
+      places = std::max(places, eight ? tiles : (tiles + 7) / 8);
+    }
+    t.first[t.entries] = at;
+    t.base[t.entries] = (uint8_t)k;
+    t.kind[t.entries++] = !eight ? SPREAD : k / 8 % 2 ? REVERSED : EIGHT;
+    at += places;
+    k += eight ? 8 : 1;
+  }
+  t.first[t.entries] = at;
   return at;
 }
 // The tiles whose launch should end first: all tiles' time over the places, in rounds of the shortest, not less than the longest.
@@ -483,11 +523,13 @@ static int tile_size(const NewtonTable& t, Count count, Steps steps) {
   return best;
 }
 
+static double long_side(const NewtonPlanes& p) { return p.np; }
+static double short_side(const NewtonPlanes& p) { return p.mp; }
 template <int SIZE, bool POLY>
 static void square(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
   typedef typename NewtonTiles<SIZE>::Square Tiles;
-  const long tiles = fill(t, Tiles::TM, square_tiles);
-  hipLaunchKernelGGL((newton_square_kernel<Tiles, POLY>), dim3((unsigned)tiles), dim3(Tiles::THREADS), 0, st, t, s);
+  const int places = fill(t, SIZE, square_tiles, POLY ? short_side : long_side);
+  hipLaunchKernelGGL((newton_square_kernel<Tiles, POLY>), dim3(8u * places), dim3(Tiles::THREADS), 0, st, t, s);
 }
 template <bool POLY>
 static void square_any(int size, NewtonTable& t, const NewtonStep& s, hipStream_t st) {
@@ -499,8 +541,8 @@ static void square_any(int size, NewtonTable& t, const NewtonStep& s, hipStream_
 template <int SIZE, bool LAST, class O>
 static void update(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
   typedef typename NewtonTiles<SIZE>::Update Tiles;
-  const long tiles = fill(t, Tiles::TM, update_tiles);
-  hipLaunchKernelGGL((newton_update_kernel<Tiles, LAST, O>), dim3((unsigned)tiles), dim3(Tiles::THREADS), 0, st, t, s);
+  const int places = fill(t, SIZE, update_tiles, short_side);
+  hipLaunchKernelGGL((newton_update_kernel<Tiles, LAST, O>), dim3(8u * places), dim3(Tiles::THREADS), 0, st, t, s);
 }
 template <int SIZE, class O>
 static void update_any(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
@@ -511,10 +553,8 @@ static void update_any(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
 template <class S>
 static void newton(NewtonTable& t, NewtonStep s, int steps, float eps, hipStream_t st) {
   hipLaunchKernelGGL((newton_norm_kernel<S>), dim3((unsigned)t.chunks, (unsigned)t.many), dim3(256), 0, st, t);
-  const long begin = fill(t, 64, update_tiles);
-  hipLaunchKernelGGL((newton_begin_kernel<S>), dim3((unsigned)begin), dim3(256), 0, st, t, eps);
-  const auto long_side = [](const NewtonPlanes& p) { return (double)p.np; };
-  const auto short_side = [](const NewtonPlanes& p) { return (double)p.mp; };
+  const int begin = fill(t, SMALL, update_tiles, short_side);
+  hipLaunchKernelGGL((newton_begin_kernel<S>), dim3(8u * begin), dim3(256), 0, st, t, eps);
   const int gram = tile_size(t, square_tiles, long_side), poly = tile_size(t, square_tiles, short_side), un = tile_size(t, update_tiles, short_side);
   for (s.step = 0; s.step < steps; ++s.step) {
     s.from = s.step & 1;
