@@ -51,15 +51,18 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   const size_t v256 = up(d->vocab, 256), v64 = up(d->vocab, 64);
   const size_t row = (size_t)p.P * p.kp * 2;
   p.few = p.n <= 32;
-  // 256 x 256 tiles where they fill the CUs twice; measured at 8192 rows: see loss_tile_kernel
-  p.wide = !p.few && (v256 / 256) * (((size_t)p.n + 255) / 256) >= 512;
+  // Tiles of 256 x 256, one a CU, or of 128 x 128, two a CU: whose rounds end first.  A round of the former takes 27 ns for each of the contraction
+  // index (two planes: 79), of the latter 17 (46), measured at 8192 x 8192 x 8192 (two planes: 4096 x 4096 x 8192).
+  const auto rounds = [&](size_t tile, size_t places) { return (up(d->vocab, tile) / tile * (up(p.npad, tile) / tile) + places - 1) / places; };
+  p.wide = !p.few && rounds(256, 256) * 100 <= rounds(128, 512) * 60;
   p.fwd_rows = (int)std::min(v256, std::max<size_t>(256, ((size_t)256 << 20) / row / 256 * 256));
   // a piece's G: up to 256 MB
   p.bwd_rows = (int)std::min(v256, std::max<size_t>(1024, ((size_t)256 << 20) / ((size_t)p.P * p.npad * 2) / 1024 * 1024));
   const size_t tile = p.wide ? 256 : 128, dx_tiles = up(p.kp, tile) / tile * (up(p.npad, tile) / tile);
-  p.splits = (int)std::max<size_t>(1, std::min<size_t>({32, 512 / dx_tiles, std::min<size_t>(p.bwd_rows, v64) / 512}));
+  const size_t places = p.wide ? 256 : 512;
+  p.splits = (int)std::max<size_t>(1, std::min<size_t>({32, places / dx_tiles, std::min<size_t>(p.bwd_rows, v64) / 512}));
   const size_t piece = std::min<size_t>(p.bwd_rows, v64), dw_tiles = up(p.kp, tile) / tile * (up(piece, tile) / tile);
-  p.w_splits = (int)std::max<size_t>(1, std::min<size_t>({64, 512 / dw_tiles, (size_t)p.npad / 256}));
+  p.w_splits = (int)std::max<size_t>(1, std::min<size_t>({64, places / dw_tiles, (size_t)p.npad / 256}));
   size_t at = CELLS * 4;
   auto take = [&](size_t bytes) { const size_t here = at; at = up(at + bytes, 256); return here; };
   at = up(at, 256);
@@ -376,34 +379,40 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
   }
 }
 
-// lse and loss of 8 tokens from the parts' maxima and sums: 32 threads a token
+// lse and loss of TOKENS tokens from the parts' maxima and sums: 256 / TOKENS threads a token.  (8 of them read whole 64 bytes; 2 end a long
+// vocabulary's parts sooner where there are not many: 24 tokens, 4096 parts 16 -> 6 us.)
+template <int TOKENS>
 __global__ __launch_bounds__(256) void loss_merge_kernel(const float2* part, int parts, int npad, const unsigned* count, const int* map, const int* label,
                                                          const float* target, float* lse, float* loss, float* losses) {
-  __shared__ float top_s[32][8], sum_s[32][8];
-  const int live = (int)*count, tid = threadIdx.x, t8 = tid & 7, p0 = tid >> 3, token = blockIdx.x * 8 + t8;
-  if (blockIdx.x * 8 >= live) return;
+  constexpr int LANES = 256 / TOKENS;
+  __shared__ float top_s[LANES][TOKENS], sum_s[LANES][TOKENS];
+  const int live = (int)*count, tid = threadIdx.x, at = tid % TOKENS, lane = tid / TOKENS, token = blockIdx.x * TOKENS + at;
+  if (blockIdx.x * TOKENS >= (unsigned)live) return;
   float top = -INFINITY, sum = 0.f;
-  bool nan = false;
+  auto add = [&](float m, float s) {
+    const float most = fmaxf(top, m), from = most > -INFINITY ? most : 0.f;
+    sum = sum * fast_exp2((top - from) * kLog2e) + s * fast_exp2((m - from) * kLog2e);
+    top = most;
+  };
   if (token < live) {
 #pragma unroll 8
-    for (int p = p0; p < parts; p += 32) {
+    for (int p = lane; p < parts; p += LANES) {
       const float2 v = part[(size_t)p * npad + token];
-      nan |= v.y != v.y;
-      const float m = fmaxf(top, v.x);
-      const float at = m > -INFINITY ? m : 0.f;
-      sum = sum * fast_exp2((top - at) * kLog2e) + v.y * fast_exp2((v.x - at) * kLog2e);
-      top = m;
+      add(v.x, v.y);
     }
   }
-  top_s[p0][t8] = top;
-  sum_s[p0][t8] = nan ? __builtin_nanf("") : sum;
-  __syncthreads();
-  if (tid >= 8 || token >= live) return;
-  float all = -INFINITY, s = 0.f;
-  for (int p = 0; p < 32; ++p) all = fmaxf(all, top_s[p][tid]);
-  const float at = all > -INFINITY ? all : 0.f;
-  for (int p = 0; p < 32; ++p) s += sum_s[p][tid] * fast_exp2((top_s[p][tid] - at) * kLog2e);
-  float l = at + fast_log2(s) * kLn2;
+  top_s[lane][at] = top;
+  sum_s[lane][at] = sum;
+  for (int half = LANES / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (lane < half) {
+      add(top_s[lane + half][at], sum_s[lane + half][at]);
+      top_s[lane][at] = top;
+      sum_s[lane][at] = sum;
+    }
+  }
+  if (lane != 0 || token >= live) return;
+  float l = (top > -INFINITY ? top : 0.f) + fast_log2(sum) * kLn2;
   if (label[token] < 0) l = __builtin_nanf("");      // no entry of the vocabulary: said by the loss and all gradients
   const float value = l - (label[token] < 0 ? 0.f : target[token]);
   lse[token] = l;
@@ -690,8 +699,9 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
     }
     const int part = p.few ? 32 : p.wide ? 128 : 64, tile = p.few ? 128 : p.wide ? 256 : 128;
     const int parts = (d->vocab + tile - 1) / tile * (tile / part);
-    hipLaunchKernelGGL(loss_merge_kernel, dim3((unsigned)((p.n + 7) / 8)), dim3(256), 0, st, (const float2*)(w + p.f_part), parts, p.npad, count, (const int*)map,
-                       (const int*)label, (const float*)target, lse, each, losses);
+    const auto merge = p.n <= 2048 ? loss_merge_kernel<2> : loss_merge_kernel<8>;
+    hipLaunchKernelGGL(merge, dim3((unsigned)(p.n <= 2048 ? (p.n + 1) / 2 : (p.n + 7) / 8)), dim3(256), 0, st, (const float2*)(w + p.f_part), parts, p.npad, count,
+                       (const int*)map, (const int*)label, (const float*)target, lse, each, losses);
   }
   if (d->reduction != 0)
     hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, (const float*)each, count, (int)(d->reduction == 1), loss);

@@ -117,50 +117,61 @@ __global__ __launch_bounds__(256) void newton_norm_kernel(const NewtonTable G) {
   if (tid == 0) G.partial[k * kNormChunks + blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
-// A 64 x 64 tile of the first X, scaled, with zeros up to whole multiples of 64
+// kBeginTiles tiles of 64 x 64 of the first X, scaled, with zeros up to whole multiples of 64
+constexpr int kBeginTiles = 2;
+__host__ __device__ inline int begin_parts(const NewtonPlanes& p, int size) { return (update_tiles(p, size) + kBeginTiles - 1) / kBeginTiles; }
 template <class S>
 __global__ __launch_bounds__(256) void newton_begin_kernel(const NewtonTable G, float eps) {
   __shared__ float tile_s[64][65];
-  __shared__ double sums[4];
-  const NewtonPlace place = place_of(G, [](const NewtonPlanes& p) { return update_tiles(p, 64); });
+  __shared__ double sums[4], scale_s;
+  const NewtonPlace place = place_of(G, [](const NewtonPlanes& p) { return begin_parts(p, 64); });
   if (place.k < 0) return;
-  const int k = place.k, at = place.nth, tid = threadIdx.x;
+  const int k = place.k, tid = threadIdx.x;
   const NewtonMatrix M = G.of[k];
   const NewtonPlanes L(M.rows, M.cols);
-  const int wide = L.np / 64, r0 = at / wide * 64, c0 = at % wide * 64;
   double sum = 0.0;
   for (int i = tid; i < G.chunks; i += 256) sum += G.partial[k * kNormChunks + i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
   if ((tid & 63) == 0) sums[tid >> 6] = sum;
-  // (turned: the tile's rows are columns of the matrix)
-  const S* in = (const S*)M.in;
-  const int first = L.turned ? c0 : r0, second = L.turned ? r0 : c0, col = second + (tid & 63);
-#pragma unroll 4
-  for (int i = tid >> 6; i < 64; i += 4) {
-    const int row = first + i;
-    tile_s[i][tid & 63] = row < M.rows && col < M.cols ? (float)in[row * M.stride + col] : 0.f;
-  }
   __syncthreads();
-  const double norm = sqrt(sums[0] + sums[1] + sums[2] + sums[3]), part = norm / (norm + eps);
-  // (a norm of zero, and one that is no number: s = 0)
-  const int s = part > 0.0 && part < 1.0 ? min(100, -(ilogb(part) + 1)) : 0;
-  const double scale = ldexp(1.0 / (norm + eps), 12 + s);
-  if (at == 0 && tid == 0) G.shift[k] = s;
-  const int r = tid >> 2, c = (tid & 3) * 16;
-  _Float16* x = planes_of(G, k) + (long)(r0 + r) * L.np + c0 + c;
+  if (tid == 0) {
+    const double norm = sqrt(sums[0] + sums[1] + sums[2] + sums[3]), part = norm / (norm + eps);
+    // (a norm of zero, and one that is no number: s = 0)
+    const int s = part > 0.0 && part < 1.0 ? min(100, -(ilogb(part) + 1)) : 0;
+    scale_s = ldexp(1.0 / (norm + eps), 12 + s);
+    if (place.nth == 0) G.shift[k] = s;
+  }
+  const S* in = (const S*)M.in;
+  const int wide = L.np / 64, r = tid >> 2, c = (tid & 3) * 16;
+  for (int at = place.nth * kBeginTiles; at < min((place.nth + 1) * kBeginTiles, wide * (L.mp / 64)); ++at) {
+    // (turned: the tile's rows are columns of the matrix)
+    const int r0 = at / wide * 64, c0 = at % wide * 64, first = L.turned ? c0 : r0, col = (L.turned ? r0 : c0) + (tid & 63);
+    float v[16];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    f16x8 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int cc = c + 8 * u + e;
-      const Halves h = halves_of((float)((double)(L.turned ? tile_s[cc][r] : tile_s[r][cc]) * scale));
-      hi[e] = h.hi;
-      lo[e] = h.lo;
+    for (int i = 0; i < 16; ++i) {
+      const int row = first + 4 * i + (tid >> 6);
+      v[i] = row < M.rows && col < M.cols ? (float)in[row * M.stride + col] : 0.f;
     }
-    *reinterpret_cast<f16x8*>(x + 8 * u) = hi;
-    *reinterpret_cast<f16x8*>(x + 8 * u + L.x_plane()) = lo;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) tile_s[4 * i + (tid >> 6)][tid & 63] = v[i];
+    __syncthreads();
+    const double scale = scale_s;
+    _Float16* x = planes_of(G, k) + (long)(r0 + r) * L.np + c0 + c;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f16x8 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int cc = c + 8 * u + e;
+        const Halves h = halves_of((float)((double)(L.turned ? tile_s[cc][r] : tile_s[r][cc]) * scale));
+        hi[e] = h.hi;
+        lo[e] = h.lo;
+      }
+      *reinterpret_cast<f16x8*>(x + 8 * u) = hi;
+      *reinterpret_cast<f16x8*>(x + 8 * u + L.x_plane()) = lo;
+    }
   }
 }
 
@@ -219,37 +230,25 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_square_kernel(const 
   const float unit = POLY ? __builtin_ldexpf(S.c, -10 - 4 * s) : 0x1p-14f, linear = __builtin_ldexpf(S.b, -2 * s), diagonal = S.a * 0x1p10f;
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j) {
-    if (tile.m != tile.n) {
-      // above the diagonal: a register's value of 32 lanes is a run of a row
-      const int col = n0 + t.col_of(j);
-#pragma unroll
-      for (int i = 0; i < Tiles::MI; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int row = m0 + t.row_of(i, e >> 2) + (e & 3);
-          if (row >= L.m || col >= L.mp) continue;
-          const long at = (long)row * L.mp + col;
-          float v = t.acc[i][j][e] * unit;
-          if (POLY) v = __builtin_fmaf(linear, (float)A[at] + (float)A[at + L.a_plane()], v);
-          const Halves h = halves_of(col < L.m ? v : 0.f);
-          out[at] = h.hi;
-          out[at + L.a_plane()] = h.lo;
-        }
-    }
-    t.template rows_of<float>(shared, [&](int i, int e) { return t.acc[i][j][e]; }, [&](int r, int c, floatx4 v) {
-      const int col = n0 + t.col_of(j) - (t.lane & 31) + r, row = m0 + t.wm * Tiles::W + c;
-      if (col >= L.m || row >= L.mp) return;
+    const int col0 = n0 + t.col_of(j) - (t.lane & 31), row0 = m0 + t.wm * Tiles::W;
+    t.template rows_of<float>(shared, [&](int i, int e) { return t.acc[i][j][e]; }, [&](int r, int c, floatx4& v) {
+      const int col = col0 + r, row = row0 + c;
+      const bool ok = col < L.m && row < L.mp;
       const long at = (long)col * L.mp + row;
       floatx4 old = {0.f, 0.f, 0.f, 0.f};
-      if (POLY) old = load_halves(A + at, L.a_plane());
+      if (POLY && ok) old = load_halves(A + at, L.a_plane());
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v[e] *= unit;
         if (POLY) v[e] = __builtin_fmaf(linear, old[e], v[e]) + (row + e == col ? diagonal : 0.f);
-        if (row + e >= L.m) v[e] = 0.f;
+        if (row + e >= L.m || col >= L.m) v[e] = 0.f;
       }
-      store_halves(out + at, L.a_plane(), v);
+      if (ok) store_halves(out + at, L.a_plane(), v);
     });
+    if (tile.m != tile.n)      // the other side of the diagonal
+      t.turned_of(shared, [&](int r, int c, floatx4 v) {
+        if (row0 + c < L.m && col0 + r < L.mp) store_halves(out + (long)(row0 + c) * L.mp + col0 + r, L.a_plane(), v);
+      });
   }
 }
 
@@ -445,10 +444,11 @@ __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const Ne
 typedef _Float16 H16;
 // Tiles of a launch.  Time of a round of them on all places, in us for each of the contraction index and beside that (measured from 512 to 4096).
 // 128: eight waves and four stages in one work-group a CU, as fast as two work-groups of four and two (1.05 PFLOP/s) with half the time to a
-// round; 64: two work-groups a CU, or (DEEP) one of four stages where there are no more tiles than CUs (31 us instead of 52 at 4096).
+// round; 64: two work-groups a CU, or (DEEP) one of four stages where there are no more tiles than CUs (31 us instead of 52 at 4096); what they read is
+// near what an L2 gives (64 bytes a clock to each CU), so theirs is the time with operands that do not all lie there.
 enum NewtonSize { WIDE, MIDDLE, SMALL, DEEP, SIZES };
 struct SizeCost { int tile, places; double each, beside; };
-static constexpr SizeCost kSizes[SIZES] = {{256, 256, 0.0785, 7.0}, {128, 256, 0.0238, 3.5}, {64, 512, 0.0136, 2.7}, {64, 256, 0.0069, 3.4}};
+static constexpr SizeCost kSizes[SIZES] = {{256, 256, 0.0785, 7.0}, {128, 256, 0.0238, 3.5}, {64, 512, 0.021, 2.7}, {64, 256, 0.0089, 3.4}};
 template <int SIZE> struct NewtonTiles;
 template <> struct NewtonTiles<WIDE> {
   typedef TileProduct<H16, 2, ROWS, ROWS, 256, 256, 2, 4, 32, 2> Square;
@@ -553,7 +553,7 @@ static void update_any(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
 template <class S>
 static void newton(NewtonTable& t, NewtonStep s, int steps, float eps, hipStream_t st) {
   hipLaunchKernelGGL((newton_norm_kernel<S>), dim3((unsigned)t.chunks, (unsigned)t.many), dim3(256), 0, st, t);
-  const int begin = fill(t, SMALL, update_tiles, short_side);
+  const int begin = fill(t, SMALL, begin_parts, short_side);
   hipLaunchKernelGGL((newton_begin_kernel<S>), dim3(8u * begin), dim3(256), 0, st, t, eps);
   const int gram = tile_size(t, square_tiles, long_side), poly = tile_size(t, square_tiles, short_side), un = tile_size(t, update_tiles, short_side);
   for (s.step = 0; s.step < steps; ++s.step) {

@@ -141,16 +141,21 @@ struct TileProduct {
 
   // Columns col_of(j) of the result, each W = TM / WM consecutive values of a row in memory from row_of(0, 0) on: value(i, e) is that of register
   // e of acc[i][j], store(r, c, v) takes the 16 bytes from value c on of column r of this wave's 32 - consecutive lanes consecutive
-  // bytes, W of a row together, where lanes as they are would write 16 bytes of 32 rows at a time.  Through this wave's own part of LDS.
+  // bytes, W of a row together, where lanes as they are would write 16 bytes of 32 rows at a time.  Through this wave's own part of LDS, where
+  // what `store` makes of v stays for turned_of.
   static constexpr int W = TM / WM;
+  template <class O> static constexpr int PER = 16 / sizeof(O);
+  template <class O>
+  __device__ __forceinline__ char* own_at(char* shared, int r, int c) const {
+    constexpr int CHUNKS = W / PER<O>, MASK = (CHUNKS < 16 ? CHUNKS : 16) - 1;
+    return shared + ((wm * WN + wn) * 32 + r) * W * sizeof(O) + 16 * ((c / PER<O>) ^ (r & MASK)) + c % PER<O> * sizeof(O);
+  }
   template <class O, class Value, class Store>
   __device__ __forceinline__ void rows_of(char* shared, Value value, Store store) const {
-    constexpr int PER = 16 / sizeof(O), CHUNKS = W / PER, MASK = (CHUNKS < 16 ? CHUNKS : 16) - 1;
+    constexpr int CHUNKS = W / PER<O>;
     static_assert(WAVES * 32 * W * sizeof(O) <= LDS, "");
     typedef __attribute__((__vector_size__(16))) O ox;
     typedef __attribute__((__vector_size__(4 * sizeof(O)))) O o4;
-    char* own = shared + (wm * WN + wn) * 32 * W * sizeof(O);
-    const int l = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -158,14 +163,29 @@ struct TileProduct {
         o4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = (O)value(i, 4 * q + e);
-        const int first = 32 * i + 8 * q + 4 * h;
-        *reinterpret_cast<o4*>(own + l * W * sizeof(O) + 16 * ((first / PER) ^ (l & MASK)) + first % PER * sizeof(O)) = v;
+        *reinterpret_cast<o4*>(own_at<O>(shared, lane & 31, 32 * i + 8 * q + 4 * (lane >> 5))) = v;
       }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int n = 0; n < 32 * CHUNKS / 64; ++n) {
-      const int r = (64 * n + lane) / CHUNKS, c = (64 * n + lane) % CHUNKS;
-      store(r, c * PER, *reinterpret_cast<const ox*>(own + r * W * sizeof(O) + 16 * (c ^ (r & MASK))));
+      const int r = (64 * n + lane) / CHUNKS, c = (64 * n + lane) % CHUNKS * PER<O>;
+      ox* at = reinterpret_cast<ox*>(own_at<O>(shared, r, c));
+      ox v = *at;
+      store(r, c, v);
+      *at = v;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  // The same values (of floats) the other way: store(r, c, v) takes those of row c of this wave's W in columns r .. r + 3 of its 32.
+  template <class Store>
+  __device__ __forceinline__ void turned_of(char* shared, Store store) const {
+#pragma unroll
+    for (int n = 0; n < W / 8; ++n) {
+      const int c = 8 * n + (lane >> 3), r = 4 * (lane & 7);
+      floatx4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float*>(own_at<float>(shared, r + e, c));
+      store(r, c, v);
     }
     __builtin_amdgcn_wave_barrier();
   }
