@@ -261,11 +261,14 @@ template <class Tiles, bool GRAD>
 __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const LossTileArgs G) {
   typedef typename Tiles::T T;
   __shared__ __align__(1024) char shared[Tiles::LDS];
-  const TileAt tile = tile_at(blockIdx.x, G.tiles_m, G.tiles_n, 4);
-  const int m0 = G.v0 + tile.m * Tiles::TM, n0 = tile.n * Tiles::TN, live = (int)*G.count;
+  // (the grid is for all rows; of the tiles that have any, each XCD gets its share)
+  const int live = (int)*G.count, tiles_n = ((GRAD ? (live + 63) / 64 * 64 : live) + Tiles::TN - 1) / Tiles::TN;
+  if ((int)blockIdx.x >= G.tiles_m * tiles_n) return;
+  const TileAt tile = tile_at(blockIdx.x, G.tiles_m, tiles_n, 4);
+  const int m0 = G.v0 + tile.m * Tiles::TM, n0 = tile.n * Tiles::TN;
   if (n0 >= live) {
     // rows of G up to a multiple of 64 are read as the contraction index of dw
-    if (GRAD && n0 < (live + 63) / 64 * 64) {
+    if (GRAD) {
       const int width = min(Tiles::TM, G.grad_ld - tile.m * Tiles::TM) / 8;
       for (int i = threadIdx.x; i < Tiles::P * Tiles::TN * width; i += Tiles::THREADS) {
         const int row = i / width % Tiles::TN, plane = i / width / Tiles::TN;
@@ -468,7 +471,7 @@ struct LossGradArgs {
   // dx
   float* sums;                        // [splits][npad][kp]
   int npad, per, first;               // steps of a split; first piece
-  int splits;                         // of dw
+  int splits;
   // dw
   void* dw;
   long dw_ld;
@@ -479,10 +482,11 @@ struct LossGradArgs {
 template <class Tiles>
 __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dx_kernel(const LossGradArgs G) {
   __shared__ __align__(1024) char shared[Tiles::LDS];
-  const int tiles = G.tiles_m * G.tiles_n, split = blockIdx.x / tiles;
-  const TileAt tile = tile_at(blockIdx.x % tiles, G.tiles_m, G.tiles_n, 4);
-  const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN, live = (int)*G.count;
-  if (n0 >= live) return;
+  const int live = (int)*G.count, tiles_n = (live + Tiles::TN - 1) / Tiles::TN, tiles = G.tiles_m * tiles_n;
+  if ((int)blockIdx.x >= tiles * G.splits) return;
+  const int nth = xcd_run(blockIdx.x, tiles * G.splits), split = nth / tiles;
+  const TileAt tile = tile_in(nth % tiles, G.tiles_m, tiles_n, 4);
+  const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN;
   const int from = min(split * G.per, G.grad_ld / Tiles::BK), steps = min(G.per, G.grad_ld / Tiles::BK - from);
   if (steps <= 0 && !G.first) return;
   Tiles t;
@@ -507,8 +511,8 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dx_kernel(const LossGr
 template <class Tiles, class O, bool SLICES>
 __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dw_kernel(const LossGradArgs G) {
   __shared__ __align__(1024) char shared[Tiles::LDS];
-  const int tiles = G.tiles_m * G.tiles_n, split = SLICES ? blockIdx.x / tiles : 0;
-  const TileAt tile = tile_at(SLICES ? blockIdx.x % tiles : blockIdx.x, G.tiles_m, G.tiles_n, 4);
+  const int tiles = G.tiles_m * G.tiles_n, nth = xcd_run(blockIdx.x, gridDim.x), split = SLICES ? nth / tiles : 0;
+  const TileAt tile = tile_in(SLICES ? nth % tiles : nth, G.tiles_m, G.tiles_n, 4);
   const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN, live = (int)*G.count, steps = (live + Tiles::BK - 1) / Tiles::BK;
   Tiles t;
   t.init(shared);
@@ -760,9 +764,8 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const vo
     if (dx) {
       const int bk = p.P == 2 || p.wide ? 32 : 64;
       q.other = (const H16*)(w + p.b_w); q.other_plane = w_plane; q.other_cell = wc;
-      q.tiles_n = (p.n + tile - 1) / tile;
-      q.sums = (float*)(w + p.b_dx); q.per = (ld / bk + p.splits - 1) / p.splits; q.first = v0 == 0;
-      const dim3 grid((unsigned)(q.tiles_m * q.tiles_n * p.splits));
+      q.sums = (float*)(w + p.b_dx); q.splits = p.splits; q.per = (ld / bk + p.splits - 1) / p.splits; q.first = v0 == 0;
+      const dim3 grid((unsigned)(q.tiles_m * ((p.n + tile - 1) / tile) * p.splits));
       if (p.P == 1 && p.wide) hipLaunchKernelGGL((loss_dx_kernel<GradTiles<1>::WideX>), grid, dim3(512), 0, st, q);
       else if (p.P == 1) hipLaunchKernelGGL((loss_dx_kernel<GradTiles<1>::SmallX>), grid, dim3(256), 0, st, q);
       else if (p.wide) hipLaunchKernelGGL((loss_dx_kernel<GradTiles<2>::WideX>), grid, dim3(512), 0, st, q);
