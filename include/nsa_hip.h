@@ -545,7 +545,7 @@ int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const void* state, 
 /* Orthogonalised updates (no counterpart in the reference): of each of `many` matrices, X = in / (|in| + eps) with the Frobenius norm, then `steps`
  * times X <- a X + (b A + c A A) X with A = X X^T (X^T X where there are more rows than columns), written to out.
  *   rows, cols: host arrays, any sizes up to 2^20, the smaller one up to 2^15; in, out: host arrays of device addresses, rows of in[k] in_stride[k]
- *   elements apart, out[k] contiguous (aligned to 4 elements where cols[k] % 4 == 0); all of dtype 0 bf16, 1 fp16, 2 fp32.  out[k] may be in[k] where that is
+ *   elements apart, out[k] contiguous, alignment that of the type; all of dtype 0 bf16, 1 fp16, 2 fp32.  out[k] may be in[k] where that is
  *   contiguous.  Products of two fp16 halves (22 bits) with fp32 sums, results rounded once: as exact as fp32 products.
  *   Coefficients that take a singular value of [0, 1] past 4 on its way: NSA_E_UNSUPPORTED.  Zero matrices give zeros (eps > 0).
  * The result of a matrix depends on nothing but itself and the sizes of all. */

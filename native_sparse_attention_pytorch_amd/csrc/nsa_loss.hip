@@ -142,17 +142,12 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(const void* labels, int 
   if (blockIdx.x == 0 && tid >= 1 && tid < CELLS) cells[tid] = 0;
 }
 
-template <class S> __device__ __forceinline__ void load_values(const S* p, int have, bool vec, float (&v)[8]) {
-  if (vec && have >= 8) {
-    if constexpr (sizeof(S) == 4) {
-      const floatx4 a = *reinterpret_cast<const floatx4*>(p), b = *reinterpret_cast<const floatx4*>(p + 4);
+// up to 8 values of a row, zeros past its end
+template <class S> __device__ __forceinline__ void load_values(const S* p, int have, float (&v)[8]) {
+  if (have >= 8) {
+    const auto a = load_any<16 / sizeof(S)>(p), b = load_any<16 / sizeof(S)>(p + 8 - 16 / sizeof(S));      // (of 16 bits: the same)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
-    } else {
-      const typename PlaneVec<S>::x8 a = *reinterpret_cast<const typename PlaneVec<S>::x8*>(p);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (float)a[e];
-    }
+    for (int e = 0; e < 8; ++e) v[e] = (float)(e < (int)(16 / sizeof(S)) ? a[e] : b[e - (8 - 16 / (int)sizeof(S))]);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = e < have ? (float)p[e] : 0.f;
@@ -178,19 +173,20 @@ __device__ __forceinline__ unsigned finite_bits(float v) {
 
 // bits of the largest finite |value| of a matrix (of the rows that map names, if it is given) into *cell, which is zero or such bits
 template <class S>
-__global__ __launch_bounds__(256) void loss_largest_kernel(const S* src, long ld, int rows, int cols, int vec, const int* map, const unsigned* count, unsigned* cell) {
+__global__ __launch_bounds__(256) void loss_largest_kernel(const S* src, long ld, int rows, int cols, const int* map, const unsigned* count, unsigned* cell) {
   const int live = count != nullptr ? (int)*count : rows;
+  const bool flat = map == nullptr && ld == cols;      // one run of values
   const unsigned per = (cols + 7) / 8;
-  const bool flat = vec && map == nullptr && ld == cols && cols % 8 == 0;
+  const long total = (long)live * cols, pieces = flat ? (total + 7) / 8 : (long)live * per;
   unsigned best = 0;
 #pragma unroll 4
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < (long)live * per; i += (long)gridDim.x * 256) {
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (long)gridDim.x * 256) {
     float v[8];
     if (flat) {
-      load_values(src + 8 * i, 8, true, v);
+      load_values(src + 8 * i, (int)min(8L, total - 8 * i), v);
     } else {
       const unsigned r = (unsigned)i / per, c = ((unsigned)i - r * per) * 8;
-      load_values(src + (map != nullptr ? map[r] : (int)r) * ld + c, cols - (int)c, vec, v);
+      load_values(src + (map != nullptr ? map[r] : (int)r) * ld + c, cols - (int)c, v);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) best = max(best, finite_bits(v[e]));
@@ -201,7 +197,7 @@ __global__ __launch_bounds__(256) void loss_largest_kernel(const S* src, long ld
 // Rows (named by map, or all) as planes of kp columns, those past `cols` zero; rows past the last one up to a multiple of 64 zero too.
 // cell: the values are scaled below 2^15 by the power of two that suits its magnitude.  most: their largest magnitude goes there.
 template <class S, class D, int P>
-__global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld, int rows, int cols, int kp, int vec, const int* map, const unsigned* count,
+__global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld, int rows, int cols, int kp, const int* map, const unsigned* count,
                                                           const unsigned* cell, D* dst, long plane, unsigned* most) {
   const int live = count != nullptr ? (int)*count : rows;
   const unsigned per = kp / 8, i = blockIdx.x * 256 + threadIdx.x;      // (below 2^31: loss_plan)
@@ -210,7 +206,7 @@ __global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld,
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 0.f;
-  if (r < live && c < cols) load_values(src + (map != nullptr ? map[r] : r) * ld + c, cols - c, vec, v);
+  if (r < live && c < cols) load_values(src + (map != nullptr ? map[r] : r) * ld + c, cols - c, v);
   if (most != nullptr) {
     unsigned best = 0;
 #pragma unroll
@@ -475,7 +471,6 @@ struct LossGradArgs {
   // dw
   void* dw;
   long dw_ld;
-  int vec;
 };
 
 // dx, one slice of the piece's vocabulary: features (registers) by tokens (lanes), unscaled, added to what the pieces before gave
@@ -532,8 +527,8 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dw_kernel(const LossGr
       const int entry = n0 + t.col_of(j) - (t.lane & 31) + r, col = m0 + t.wm * Tiles::W + c;
       if (entry >= G.entries || col >= G.dim) return;
       O* at = dw + (size_t)entry * G.dw_ld + col;
-      if (G.vec) {
-        *reinterpret_cast<decltype(v)*>(at) = v;
+      if (col + (int)(16 / sizeof(O)) <= G.dim) {
+        store_any(at, v);
       } else {
 #pragma unroll
         for (int e = 0; e < (int)(16 / sizeof(O)); ++e)
@@ -542,27 +537,9 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dw_kernel(const LossGr
     });
 }
 
-template <class O> __device__ __forceinline__ void store_quad(O* p, floatx4 v, int have, bool vec) {
-  if (vec) {
-    if constexpr (sizeof(O) == 4) {
-      *reinterpret_cast<floatx4*>(p) = v;
-    } else {
-      typedef __attribute__((__vector_size__(4 * sizeof(O)))) O ox4;
-      ox4 r;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = (O)v[e];
-      *reinterpret_cast<ox4*>(p) = r;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < have) p[e] = (O)v[e];
-  }
-}
-
 // rows of dx or dw [n][dim] from `splits` slices [size][kp]; place: the slices' row of each, -1: zeros
 template <class O>
-__global__ __launch_bounds__(256) void loss_rows_of_slices_kernel(const float* sums, int splits, int size, int kp, int n, int dim, int vec, const int* place, O* to) {
+__global__ __launch_bounds__(256) void loss_rows_of_slices_kernel(const float* sums, int splits, int size, int kp, int n, int dim, const int* place, O* to) {
   const unsigned per = (dim + 3) / 4, i = blockIdx.x * 256 + threadIdx.x;      // (below 2^31: loss_plan)
   const unsigned row = i / per, c = (i - row * per) * 4;
   if (row >= (unsigned)n) return;
@@ -572,7 +549,18 @@ __global__ __launch_bounds__(256) void loss_rows_of_slices_kernel(const float* s
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const floatx4*>(sums + ((size_t)s * size + at) * kp + c);
   }
-  store_quad(to + (size_t)row * dim + c, v, dim - (int)c, vec);
+  O* p = to + (size_t)row * dim + c;
+  typedef __attribute__((__vector_size__(4 * sizeof(O)))) O o4;
+  o4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = (O)v[e];
+  if ((int)c + 4 <= dim) {
+    store_any(p, o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if ((int)c + e < dim) p[e] = o[e];
+  }
 }
 
 // ------------------------------------------------------------------------------------ launches
@@ -606,19 +594,18 @@ static void launch_tiles(const LossPlan& p, const LossTileArgs& a, hipStream_t s
 }
 
 static unsigned blocks_for(long work) { return (unsigned)std::max<long>(1, (work + 255) / 256); }
-static bool vectors(const void* p, long ld, int each) { return ((uintptr_t)p & 15) == 0 && ld * each % 16 == 0; }
 
 template <class S, class D, int P>
 static void planes(const void* src, long ld, int rows, int rows_cap, int cols, int kp, const int* map, const unsigned* count, const unsigned* cell, void* dst,
                    long plane, hipStream_t st, unsigned* most = nullptr) {
   hipLaunchKernelGGL((loss_planes_kernel<S, D, P>), dim3(blocks_for((long)up(rows_cap, 64) * kp / 8)), dim3(256), 0, st, (const S*)src, ld, rows, cols, kp,
-                     (int)vectors(src, ld, sizeof(S)), map, count, cell, (D*)dst, plane, most);
+                     map, count, cell, (D*)dst, plane, most);
 }
 template <class S>
 static void largest(const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, unsigned* cell, hipStream_t st) {
   const long work = (long)rows * ((cols + 7) / 8);
-  hipLaunchKernelGGL((loss_largest_kernel<S>), dim3(std::min(1024u, blocks_for(work))), dim3(256), 0, st, (const S*)src, ld, rows, cols,
-                     (int)vectors(src, ld, sizeof(S)), map, count, cell);
+  hipLaunchKernelGGL((loss_largest_kernel<S>), dim3(std::min(1024u, blocks_for(work))), dim3(256), 0, st, (const S*)src, ld, rows, cols, map, count,
+                     cell);
 }
 // the weight's rows from v0 as the forward's planes
 static void forward_weight(const nsa_loss_desc* d, const LossPlan& p, const void* weight, int v0, int rows, const unsigned* cell, void* dst, hipStream_t st) {
@@ -635,10 +622,9 @@ static void dw_tiles(const LossPlan& p, const LossGradArgs& q, dim3 grid, hipStr
 }
 static void rows_of_slices(const nsa_loss_desc* d, const float* sums, int splits, int size, int kp, int n, const int* place, void* to, hipStream_t st) {
   const dim3 grid(blocks_for((long)n * ((d->dim + 3) / 4)));
-  const int vec = d->dim % 4 == 0 && (uintptr_t)to % (d->dtype == 2 ? 16 : 8) == 0;
-  if (d->dtype == 0) hipLaunchKernelGGL((loss_rows_of_slices_kernel<B16>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, vec, place, (B16*)to);
-  else if (d->dtype == 1) hipLaunchKernelGGL((loss_rows_of_slices_kernel<H16>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, vec, place, (H16*)to);
-  else hipLaunchKernelGGL((loss_rows_of_slices_kernel<float>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, vec, place, (float*)to);
+  if (d->dtype == 0) hipLaunchKernelGGL((loss_rows_of_slices_kernel<B16>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, place, (B16*)to);
+  else if (d->dtype == 1) hipLaunchKernelGGL((loss_rows_of_slices_kernel<H16>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, place, (H16*)to);
+  else hipLaunchKernelGGL((loss_rows_of_slices_kernel<float>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, place, (float*)to);
 }
 
 }  // namespace nsa
@@ -778,7 +764,6 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const vo
       char* to = (char*)dw + v0 * d->dim * each;
       q.splits = p.w_splits;
       q.dw = slices ? w + p.b_dw : to; q.dw_ld = slices ? p.kp : d->dim; q.dim = slices ? p.kp : d->dim;
-      q.vec = slices || ((long)d->dim * each % 16 == 0 && (uintptr_t)dw % 16 == 0);
       const dim3 grid((unsigned)(q.tiles_m * q.tiles_n * p.w_splits));
       if (slices && p.P == 1) dw_tiles<1, float, true>(p, q, grid, st);
       else if (slices) dw_tiles<2, float, true>(p, q, grid, st);

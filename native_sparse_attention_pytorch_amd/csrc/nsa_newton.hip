@@ -89,15 +89,14 @@ __global__ __launch_bounds__(256) void newton_norm_kernel(const NewtonTable G) {
   const int k = blockIdx.y, tid = threadIdx.x;
   const NewtonMatrix M = G.of[k];
   const S* in = (const S*)M.in;
-  const bool whole = M.stride == M.cols && ((uintptr_t)in & 15) == 0;      // one run of values
+  const bool whole = M.stride == M.cols;      // one run of values
   double sum = 0.0;
   const long total = (long)M.rows * M.cols, per = ((total + G.chunks - 1) / G.chunks + 2047) / 2048 * 2048, first = blockIdx.x * per, last = min(total, first + per);
   if (whole) {
     constexpr int V = 16 / sizeof(S);
-    typedef __attribute__((__vector_size__(16))) S vec;
     for (long i = first + tid * V; i < last; i += 256 * V) {
       if (i + V <= last) {
-        const vec v = *reinterpret_cast<const vec*>(in + i);
+        const auto v = load_any<V>(in + i);
 #pragma unroll
         for (int e = 0; e < V; ++e) sum += (double)(float)v[e] * (double)(float)v[e];
       } else {
@@ -307,8 +306,8 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_update_kernel(const 
       ox4 o;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = (O)v[e];
-      if (M.cols % 4 == 0) {
-        *reinterpret_cast<ox4*>(p) = o;
+      if (col + 4 <= L.n) {
+        store_any(p, o);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -614,7 +613,6 @@ extern "C" int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_
   const int each = dtype == 2 ? 4 : 2;
   for (int32_t k = 0; k < many; ++k) {
     if (!in[k] || !out[k] || in_stride[k] < cols[k] || ((uintptr_t)in[k] | (uintptr_t)out[k]) % each) return NSA_E_ARG;
-    if (cols[k] % 4 == 0 && (uintptr_t)out[k] % (4 * each)) return NSA_E_ARG;      // (rows of whole quads are stored as such)
   }
   NewtonStep s{};
   s.a = a; s.b = b; s.c = c;

@@ -26,6 +26,15 @@ template <> struct PlaneVec<_Float16> { typedef f16x8 x8; };
 __device__ __forceinline__ floatx16 mma(bf16x8 a, bf16x8 b, floatx16 c) { return mfma32(a, b, c); }
 __device__ __forceinline__ floatx16 mma(f16x8 a, f16x8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
+// N values from or to an address that is aligned to one of them only: global memory takes wide accesses there as well, and rows of any length
+// are read and written as others are
+template <class S, int N> struct AnyVec { typedef __attribute__((__vector_size__(N * sizeof(S)), aligned(sizeof(S)))) S type; };
+template <int N, class S> __device__ __forceinline__ auto load_any(const S* p) {
+  typedef __attribute__((__vector_size__(N * sizeof(S)))) S vec;
+  return (vec)*reinterpret_cast<const typename AnyVec<S, N>::type*>(p);
+}
+template <class S, class V> __device__ __forceinline__ void store_any(S* p, V v) { *reinterpret_cast<typename AnyVec<S, sizeof(V) / sizeof(S)>::type*>(p) = v; }
+
 enum { ROWS = 0, COLUMNS = 1 };
 
 // One operand's tile: R result rows by BK of k.  ROWS: `limit` rows exist (those past it are read as the last one: callers drop their

@@ -82,7 +82,7 @@ def test_entries_check_pointers_and_workspaces():
         1, ints(rows), ints(cols), ptrs(at), longs(stride), ptrs(to), dtype, steps, a, b, c, eps, one, ws, 0)
     assert call(rows=0) == -1 and call(stride=49) == -1 and call(at=0) == -1 and call(to=0) == -1 and call(dtype=3) == -1
     assert call(steps=0) == -1 and call(steps=101) == -1 and call(eps=-1.) == -1 and call(at=258) == -1
-    assert call(cols=48, to=260) == -1                    # rows of whole quads: aligned to one
+    assert call(to=258) == -1 and call(dtype=0, at=257) == -1
     assert call(a=5., b=0., c=0.) == -2 and call(ws=need.value - 1) == -3
     assert L.nsa_newton_workspace_bytes(1, ints((1 << 20) + 1), ints(4), C.byref(need)) == -2
     assert L.nsa_newton_workspace_bytes(1, ints(1 << 16), ints(1 << 16), C.byref(need)) == -2
