@@ -7,7 +7,9 @@
 // X, A and B are held as two fp16 halves each (22 bits; nsa_tiles.hpp).  Directions of small singular values grow by a = 3.4 a step, and what
 // a step's rounding adds to them grows alike: against 64 bits the result is 4e-5 off with bf16 halves, 3 % with bf16 alone, and 6e-7 with
 // these, less than with fp32 products (1.6e-6 at 512 x 512).  a stands on the diagonal of B and not beside the product: one pass over X less, and
-// a rounding of what is left of a + b A + c A A, not of its parts.  Scales: X 2^(12 + s), A 2^(10 + 2 s), B 2^10.  s is 0 unless |G| is small beside eps:
+// a rounding of what is left of a + b A + c A A, not of its parts.  A bf16 result is itself rounded to 2^-9, so its last two steps, after which little grows,
+// take the first halves alone, at a third of the matrix instructions: that adds at most a tenth to the result's error (1.66e-3 of its norm
+// from rounding, 1.83e-3 with two such steps, 2.0e-3 with three, 2.1e-3 with all five).  Scales: X 2^(12 + s), A 2^(10 + 2 s), B 2^10.  s is 0 unless |G| is small beside eps:
 // then X starts so small that fp16 would lose it, and s is what brings its norm to 1; it falls by the bits of a with each step, so nothing grows out
 // of range.  The entry checks that singular values up to 1 stay below 4 for the given coefficients.
 //
@@ -175,20 +177,20 @@ __global__ __launch_bounds__(256) void newton_begin_kernel(const NewtonTable G, 
 }
 
 struct NewtonStep {
-  int step, last, growth, from;      // growth: bits that a step takes off s; from: the buffer of X that is read
+  int step, last, growth, from, both;      // growth: bits that a step takes off s; from: the buffer of X that is read; both: halves of X are wanted
   float a, b, c;
 };
 __device__ __forceinline__ int shift_at(const NewtonTable& G, const NewtonStep& S, int k, int step) { return max(0, G.shift[k] - S.growth * step); }
 
-// four consecutive values of both planes
-__device__ __forceinline__ floatx4 load_halves(const _Float16* p, long plane) {
-  const f16x4 hi = *reinterpret_cast<const f16x4*>(p), lo = *reinterpret_cast<const f16x4*>(p + plane);
+// four consecutive values of P planes
+template <int P> __device__ __forceinline__ floatx4 load_halves(const _Float16* p, long plane) {
+  const f16x4 hi = *reinterpret_cast<const f16x4*>(p), lo = *reinterpret_cast<const f16x4*>(p + (P == 2 ? plane : 0));
   floatx4 v;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = (float)hi[e] + (float)lo[e];
+  for (int e = 0; e < 4; ++e) v[e] = P == 2 ? (float)hi[e] + (float)lo[e] : (float)hi[e];
   return v;
 }
-__device__ __forceinline__ void store_halves(_Float16* p, long plane, floatx4 v) {
+__device__ __forceinline__ void store_halves(_Float16* p, long plane, floatx4 v, bool both) {
   f16x4 hi, lo;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -197,7 +199,7 @@ __device__ __forceinline__ void store_halves(_Float16* p, long plane, floatx4 v)
     lo[e] = h.lo;
   }
   *reinterpret_cast<f16x4*>(p) = hi;
-  *reinterpret_cast<f16x4*>(p + plane) = lo;
+  if (both) *reinterpret_cast<f16x4*>(p + plane) = lo;
 }
 
 // POLY 0: A = X X^T; 1: B = a + b A + c A A.  Tiles on and below the diagonal.
@@ -235,18 +237,18 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_square_kernel(const 
       const bool ok = col < L.m && row < L.mp;
       const long at = (long)col * L.mp + row;
       floatx4 old = {0.f, 0.f, 0.f, 0.f};
-      if (POLY && ok) old = load_halves(A + at, L.a_plane());
+      if (POLY && ok) old = load_halves<Tiles::P>(A + at, L.a_plane());
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v[e] *= unit;
         if (POLY) v[e] = __builtin_fmaf(linear, old[e], v[e]) + (row + e == col ? diagonal : 0.f);
         if (row + e >= L.m || col >= L.m) v[e] = 0.f;
       }
-      if (ok) store_halves(out + at, L.a_plane(), v);
+      if (ok) store_halves(out + at, L.a_plane(), v, Tiles::P == 2);
     });
     if (tile.m != tile.n)      // the other side of the diagonal
       t.turned_of(shared, [&](int r, int c, floatx4 v) {
-        if (row0 + c < L.m && col0 + r < L.mp) store_halves(out + (long)(row0 + c) * L.mp + col0 + r, L.a_plane(), v);
+        if (row0 + c < L.m && col0 + r < L.mp) store_halves(out + (long)(row0 + c) * L.mp + col0 + r, L.a_plane(), v, Tiles::P == 2);
       });
   }
 }
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_update_kernel(const 
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = row < L.m ? v[e] * unit : 0.f;      // (rows past the last one are zeros)
       if (!LAST) {
-        store_halves(next + (long)row * L.np + col, L.x_plane(), v);
+        store_halves(next + (long)row * L.np + col, L.x_plane(), v, S.both);
         return;
       }
       O* p = (O*)M.out + (long)row * M.cols + col;
@@ -448,22 +450,18 @@ typedef _Float16 H16;
 enum NewtonSize { WIDE, MIDDLE, SMALL, DEEP, SIZES };
 struct SizeCost { int tile, places; double each, beside; };
 static constexpr SizeCost kSizes[SIZES] = {{256, 256, 0.0785, 7.0}, {128, 256, 0.0238, 3.5}, {64, 512, 0.021, 2.7}, {64, 256, 0.0089, 3.4}};
-template <int SIZE> struct NewtonTiles;
-template <> struct NewtonTiles<WIDE> {
-  typedef TileProduct<H16, 2, ROWS, ROWS, 256, 256, 2, 4, 32, 2> Square;
-  typedef TileProduct<H16, 2, COLUMNS, ROWS, 256, 256, 2, 4, 32, 2> Update;
+template <int SIZE, int P> struct NewtonTiles;
+template <int P> struct NewtonTiles<WIDE, P> {
+  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 256, 256, 2, 4, 32, P == 2 ? 2 : 4>;
 };
-template <> struct NewtonTiles<MIDDLE> {
-  typedef TileProduct<H16, 2, ROWS, ROWS, 128, 128, 4, 2, 32, 4> Square;
-  typedef TileProduct<H16, 2, COLUMNS, ROWS, 128, 128, 4, 2, 32, 4> Update;
+template <int P> struct NewtonTiles<MIDDLE, P> {
+  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 128, 128, 4, 2, P == 2 ? 32 : 64, 4>;
 };
-template <> struct NewtonTiles<SMALL> {
-  typedef TileProduct<H16, 2, ROWS, ROWS, 64, 64, 2, 2, 64, 2> Square;
-  typedef TileProduct<H16, 2, COLUMNS, ROWS, 64, 64, 2, 2, 64, 2> Update;
+template <int P> struct NewtonTiles<SMALL, P> {
+  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 64, 64, 2, 2, 64, P == 2 ? 2 : 4>;
 };
-template <> struct NewtonTiles<DEEP> {
-  typedef TileProduct<H16, 2, ROWS, ROWS, 64, 64, 2, 2, 64, 4> Square;
-  typedef TileProduct<H16, 2, COLUMNS, ROWS, 64, 64, 2, 2, 64, 4> Update;
+template <int P> struct NewtonTiles<DEEP, P> {
+  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 64, 64, 2, 2, 64, P == 2 ? 4 : 8>;
 };
 
 // The queues of a launch with tiles of kSizes[size], and their length.  Matrices go to the XCDs by eights, back and forth, where that leaves no XCD with
@@ -524,29 +522,31 @@ static int tile_size(const NewtonTable& t, Count count, Steps steps) {
 
 static double long_side(const NewtonPlanes& p) { return p.np; }
 static double short_side(const NewtonPlanes& p) { return p.mp; }
-template <int SIZE, bool POLY>
+template <int SIZE, int P, bool POLY>
 static void square(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
-  typedef typename NewtonTiles<SIZE>::Square Tiles;
+  typedef typename NewtonTiles<SIZE, P>::template Of<ROWS> Tiles;
   const int places = fill(t, SIZE, square_tiles, POLY ? short_side : long_side);
   hipLaunchKernelGGL((newton_square_kernel<Tiles, POLY>), dim3(8u * places), dim3(Tiles::THREADS), 0, st, t, s);
 }
-template <bool POLY>
+template <int P, bool POLY>
 static void square_any(int size, NewtonTable& t, const NewtonStep& s, hipStream_t st) {
-  if (size == WIDE) square<WIDE, POLY>(t, s, st);
-  else if (size == MIDDLE) square<MIDDLE, POLY>(t, s, st);
-  else if (size == SMALL) square<SMALL, POLY>(t, s, st);
-  else square<DEEP, POLY>(t, s, st);
+  if (size == WIDE) square<WIDE, P, POLY>(t, s, st);
+  else if (size == MIDDLE) square<MIDDLE, P, POLY>(t, s, st);
+  else if (size == SMALL) square<SMALL, P, POLY>(t, s, st);
+  else square<DEEP, P, POLY>(t, s, st);
 }
-template <int SIZE, bool LAST, class O>
+template <int SIZE, int P, bool LAST, class O>
 static void update(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
-  typedef typename NewtonTiles<SIZE>::Update Tiles;
+  typedef typename NewtonTiles<SIZE, P>::template Of<COLUMNS> Tiles;
   const int places = fill(t, SIZE, update_tiles, short_side);
   hipLaunchKernelGGL((newton_update_kernel<Tiles, LAST, O>), dim3(8u * places), dim3(Tiles::THREADS), 0, st, t, s);
 }
-template <int SIZE, class O>
-static void update_any(NewtonTable& t, const NewtonStep& s, hipStream_t st) {
-  if (s.last) update<SIZE, true, O>(t, s, st);
-  else update<SIZE, false, H16>(t, s, st);
+template <int P, bool LAST, class O>
+static void update_any(int size, NewtonTable& t, const NewtonStep& s, hipStream_t st) {
+  if (size == WIDE) update<WIDE, P, LAST, O>(t, s, st);
+  else if (size == MIDDLE) update<MIDDLE, P, LAST, O>(t, s, st);
+  else if (size == SMALL) update<SMALL, P, LAST, O>(t, s, st);
+  else update<DEEP, P, LAST, O>(t, s, st);
 }
 
 template <class S>
@@ -554,16 +554,22 @@ static void newton(NewtonTable& t, NewtonStep s, int steps, float eps, hipStream
   hipLaunchKernelGGL((newton_norm_kernel<S>), dim3((unsigned)t.chunks, (unsigned)t.many), dim3(256), 0, st, t);
   const int begin = fill(t, SMALL, begin_parts, short_side);
   hipLaunchKernelGGL((newton_begin_kernel<S>), dim3(8u * begin), dim3(256), 0, st, t, eps);
+  constexpr int LAST_P = std::is_same<S, __bf16>::value ? 1 : 2;      // planes of the last two steps
   const int gram = tile_size(t, square_tiles, long_side), poly = tile_size(t, square_tiles, short_side), un = tile_size(t, update_tiles, short_side);
   for (s.step = 0; s.step < steps; ++s.step) {
     s.from = s.step & 1;
     s.last = s.step == steps - 1;
-    square_any<false>(gram, t, s, st);
-    square_any<true>(poly, t, s, st);
-    if (un == WIDE) update_any<WIDE, S>(t, s, st);
-    else if (un == MIDDLE) update_any<MIDDLE, S>(t, s, st);
-    else if (un == SMALL) update_any<SMALL, S>(t, s, st);
-    else update_any<DEEP, S>(t, s, st);
+    s.both = LAST_P == 2 || s.step + 3 < steps;
+    if (LAST_P == 2 || s.step + 2 < steps) {
+      square_any<2, false>(gram, t, s, st);
+      square_any<2, true>(poly, t, s, st);
+    } else {
+      square_any<LAST_P, false>(gram, t, s, st);
+      square_any<LAST_P, true>(poly, t, s, st);
+    }
+    if (s.last) update_any<LAST_P, true, S>(un, t, s, st);
+    else if (LAST_P == 2 || s.step + 2 < steps) update_any<2, false, H16>(un, t, s, st);
+    else update_any<LAST_P, false, H16>(un, t, s, st);
   }
 }
 

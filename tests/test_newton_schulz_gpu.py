@@ -211,3 +211,15 @@ def test_muon_steps(nesterov, decay):
     again = Muon(params, lr=lr)
     again.load_state_dict(opt.state_dict())
     assert torch.equal(again.state[params[0]]["momentum_buffer"], opt.state[params[0]]["momentum_buffer"])
+
+
+@pytest.mark.parametrize("m,n", [(70, 80), (130, 70), (128, 1000), (512, 512), (1024, 600)])
+def test_bf16_results_are_off_by_their_rounding(m, n):
+    """The last two steps of a bf16 result are made of fp16 values, 2^-12 off each: together at most half of what rounding the result to bf16
+    adds (2^-9 on average over a binade's values 2^-9.2), so at most sqrt(1 + 1/4) of it."""
+    from native_sparse_attention_pytorch_amd import ops
+    for seed in range(3):
+        g = _g(m, n, dtype=BF16, seed=seed)
+        want = _exact(g)
+        off = lambda x: float((x.double() - want).norm())
+        assert off(ops.newton_schulz(g)) <= 1.25 ** 0.5 * off(want.to(BF16)), seed
