@@ -539,7 +539,7 @@ typedef struct nsa_loss_desc {
 int nsa_loss_workspace_bytes(const nsa_loss_desc* d, const void* weight, size_t* state_bytes, size_t* fwd_bytes, size_t* bwd_bytes);
 int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* weight, const void* labels, void* state, size_t state_bytes,
                  void* ws, size_t ws_bytes, float* loss, void* stream);
-int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const void* state, size_t state_bytes, const float* dloss,
+int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* weight, const void* state, size_t state_bytes, const float* dloss,
                  void* ws, size_t ws_bytes, void* dx, void* dw, void* stream);
 
 /* Orthogonalised updates (no counterpart in the reference): of each of `many` matrices, X = in / (|in| + eps) with the Frobenius norm, then `steps`

@@ -185,7 +185,7 @@ def lib():
         ld = C.POINTER(LossDesc)
         L.nsa_loss_workspace_bytes.argtypes = [ld, vp, C.POINTER(sz), C.POINTER(sz), C.POINTER(sz)]
         L.nsa_loss_fwd.argtypes = [ld, vp, vp, vp, vp, sz, vp, sz, vp, vp]
-        L.nsa_loss_bwd.argtypes = [ld, vp, vp, sz, vp, vp, sz, vp, vp, vp]
+        L.nsa_loss_bwd.argtypes = [ld, vp, vp, vp, sz, vp, vp, sz, vp, vp, vp]
         ints, ptrs = C.POINTER(i32), C.POINTER(vp)
         L.nsa_newton_workspace_bytes.argtypes = [i32, ints, ints, C.POINTER(sz)]
         L.nsa_newton_schulz.argtypes = [i32, ints, ints, ptrs, s3, ptrs, i32, i32, f32, f32, f32, f32, vp, sz, vp]

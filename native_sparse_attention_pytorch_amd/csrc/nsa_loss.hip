@@ -1,10 +1,14 @@
 // Softmax cross entropy of a projection onto a vocabulary, l = x w^T, and its gradients, without the logits in memory.
 //
-//   loss_i = lse_i - l[i][t_i],  lse_i = log sum_v exp l[i][v]
-//   G[i][v] = g_i (exp(l[i][v] - lse_i) - [v == t_i]),  dx = G w,  dw = G^T x
+//   loss_i = m_i - l[i][t_i] + log s_i,  m_i = max_v l[i][v],  s_i = sum_v exp(l[i][v] - m_i)
+//   G[i][v] = g_i (exp(l[i][v] - m_i - log s_i) - [v == t_i]),  dx = G w,  dw = G^T x
 //
 // Rows whose label is `ignore` are left out of everything: the others are gathered first (their order kept), so work goes by their number,
 // which stays on the device, and what an ignored row holds (a NaN) reaches nothing.
+// Where the label is the likely entry, the loss and its G are differences of about equal numbers.  So the maximum and the logarithm of the sum
+// stay two numbers, the maximum is taken off before the product with log2 e, and the label's G / g_i = exp(-loss_i) - 1 comes from the forward's
+// logit, not from one that the backward has rounded otherwise.  (With m + log s in one, and the product first, a loss below 1e-6 was noise and
+// fp32 gradients were 1.8e-6 off instead of 2.5e-7; a subtraction a logit is 1 % of the time at 512 features.)
 //
 // Forward: a tile of logits is made with the vocabulary along the registers of a lane and the tokens along the lanes, so a token's maximum
 // and sum over a wave's 64 or 128 logits are a lane's own and one exchange of the wave's halves; the pairs (maximum, sum) of all waves'
@@ -15,6 +19,7 @@
 // products, w and x, are scaled by powers of two into fp16's range and lose nothing that is above 2^-29 of their largest value.
 // fp32 operands are two fp16 planes each, G too (nsa_tiles.hpp).
 #include <algorithm>
+#include <cmath>
 #include "nsa_tiles.hpp"
 #include "../../include/nsa_hip.h"
 
@@ -24,16 +29,20 @@ constexpr int kGradBits = 14;
 // device words of a call: rows that count; bits of the largest finite |x|, |w|, |g|
 enum { CELL_ROWS, CELL_X, CELL_W, CELL_G, CELLS = 16 };
 
+// How logits are made: FEW rows as loss_few_kernel has them, the others by tiles of 64, 128 or 256 (loss_plan)
+enum LossSize { FEW, TINY, MIDDLE, WIDE };
+
 struct LossPlan {
-  int n, npad, kp, P;                     // rows and their capacity (a multiple of 64), features padded to 64, planes
+  int n, npad, kp;                        // rows and their capacity (a multiple of 64), features padded to 64
+  int P, grad_P;                          // planes of the operands of the forward, of the backward
+  LossSize size;
   bool in_place;                          // the forward reads the weight where it lies
-  int fwd_rows, bwd_rows;                 // vocabulary entries of a piece
+  int tile, part;                         // entries of the vocabulary of a tile, of a pair (maximum, sum)
+  int fwd_rows, bwd_rows;                 // entries of a piece
   int splits, w_splits;                   // slices of a piece's entries that dx is summed from, of the rows that dw is
-  bool wide;                              // 256 x 256 tiles
-  bool few;                               // tiles of 32 tokens
   size_t state, fwd, bwd;                 // bytes
-  size_t s_map, s_place, s_label, s_lse, s_x;                          // offsets in the state
-  size_t f_part, f_target, f_loss, f_w;                                // in the forward's workspace
+  size_t s_map, s_place, s_label, s_norm, s_own;                            // offsets in the state
+  size_t f_part, f_target, f_loss, f_x, f_w;                           // in the forward's workspace
   size_t b_cells, b_g, b_x, b_w, b_grad, b_dx, b_dw;                   // in the backward's
 };
 
@@ -47,43 +56,58 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.npad = (int)up(std::max<size_t>(p.n, 1), 64);
   p.kp = (int)up(d->dim, 64);
   p.P = d->dtype == 2 ? 2 : 1;
-  p.in_place = d->dtype != 2 && d->dim % 64 == 0 && d->w_stride % 8 == 0 && d->w_stride < (1 << 20) && ((uintptr_t)weight & 15) == 0;
-  const size_t v256 = up(d->vocab, 256), v64 = up(d->vocab, 64);
-  const size_t row = (size_t)p.P * p.kp * 2;
-  p.few = p.n <= 32;
-  // Tiles of 256 x 256, one a CU, or of 128 x 128, two a CU: whose rounds end first.  A round of the former takes 27 ns for each of the contraction
-  // index (two planes: 79), of the latter 17 (46), measured at 8192 x 8192 x 8192 (two planes: 4096 x 4096 x 8192).
-  const auto rounds = [&](size_t tile, size_t places) { return (up(d->vocab, tile) / tile * (up(p.npad, tile) / tile) + places - 1) / places; };
-  p.wide = !p.few && rounds(256, 256) * 100 <= rounds(128, 512) * 60;
-  p.fwd_rows = (int)std::min(v256, std::max<size_t>(256, ((size_t)256 << 20) / row / 256 * 256));
+  // (fp16 results have as many bits as an fp16 G: over many rows its rounding adds as much as theirs, but a few rows' gradients hang on single
+  // entries of G, and their second halves cost nothing beside the weight's one pass)
+  p.grad_P = d->dtype == 2 || (d->dtype == 1 && p.n <= 32) ? 2 : 1;
+  // The tiles whose rounds end first: time of a round on all places, in us for each feature and beside that (products measured from 512 to 4096
+  // features, the maxima and sums of a tile beside them).  256 x 256 tiles have no registers for sums in pieces (TileProduct::PIECES), so long
+  // fp32 rows do without them: at 2066 features the gradients were 2.8e-6 off, 7 times as much as fp32 products by the library.
+  struct Cost { LossSize size; int tile, places; double each, beside; };
+  static constexpr Cost one[3] = {{WIDE, 256, 256, 0.0272, 13.0}, {MIDDLE, 128, 256, 0.0085, 5.0}, {TINY, 64, 512, 0.0060, 3.5}};
+  static constexpr Cost two[3] = {{WIDE, 256, 256, 0.0785, 13.0}, {MIDDLE, 128, 256, 0.0238, 5.0}, {TINY, 64, 512, 0.0210, 3.5}};
+  double least = 0.;
+  p.size = FEW;
+  for (const Cost& c : p.P == 2 ? two : one) {
+    if (p.n <= 32 || (c.size == WIDE && p.P == 2 && p.kp > 1024)) continue;
+    const double tiles = (double)(up(d->vocab, c.tile) / c.tile) * (up(p.npad, c.tile) / c.tile), time = std::ceil(tiles / c.places) * (p.kp * c.each + c.beside);
+    if (p.size == FEW || time < least) {
+      p.size = c.size;
+      least = time;
+    }
+  }
+  p.tile = p.size == WIDE ? 256 : p.size == TINY ? 64 : 128;
+  p.part = p.size == WIDE || p.size == FEW ? 128 : p.size == MIDDLE ? 64 : 32;
+  p.in_place = d->dtype != 2 && d->dim % 8 == 0 && d->dim >= 64 && d->w_stride % 8 == 0 && d->w_stride < (1 << 20) && ((uintptr_t)weight & 15) == 0;
+  const size_t v256 = up(d->vocab, 256), v64 = up(d->vocab, 64), row = (size_t)p.kp * 2;
+  p.fwd_rows = (int)std::min(v256, std::max<size_t>(256, ((size_t)256 << 20) / (row * p.P) / 256 * 256));
   // a piece's G: up to 256 MB
-  p.bwd_rows = (int)std::min(v256, std::max<size_t>(1024, ((size_t)256 << 20) / ((size_t)p.P * p.npad * 2) / 1024 * 1024));
-  const size_t tile = p.wide ? 256 : 128, dx_tiles = up(p.kp, tile) / tile * (up(p.npad, tile) / tile);
-  const size_t places = p.wide ? 256 : 512;
-  p.splits = (int)std::max<size_t>(1, std::min<size_t>({32, places / dx_tiles, std::min<size_t>(p.bwd_rows, v64) / 512}));
-  const size_t piece = std::min<size_t>(p.bwd_rows, v64), dw_tiles = up(p.kp, tile) / tile * (up(piece, tile) / tile);
-  p.w_splits = (int)std::max<size_t>(1, std::min<size_t>({64, places / dw_tiles, (size_t)p.npad / 256}));
-  size_t at = CELLS * 4;
+  p.bwd_rows = (int)std::min(v256, std::max<size_t>(1024, ((size_t)256 << 20) / ((size_t)p.grad_P * p.npad * 2) / 1024 * 1024));
+  // gradients: tiles of 256 where the logits have them, else 128; as many slices as give every CU a tile
+  const size_t tile = p.size == WIDE ? 256 : 128, piece = std::min<size_t>(p.bwd_rows, v64);
+  const size_t dx_tiles = up(p.kp, tile) / tile * (up(p.npad, tile) / tile), dw_tiles = up(p.kp, tile) / tile * (up(piece, tile) / tile);
+  p.splits = (int)std::max<size_t>(1, std::min<size_t>({32, 256 / dx_tiles, piece / 512}));
+  p.w_splits = (int)std::max<size_t>(1, std::min<size_t>({32, 256 / dw_tiles, (size_t)p.npad / 256}));
+  size_t at = up(CELLS * 4, 256);
   auto take = [&](size_t bytes) { const size_t here = at; at = up(at + bytes, 256); return here; };
-  at = up(at, 256);
   p.s_map = take((size_t)p.npad * 4);
   p.s_place = take((size_t)p.npad * 4);
   p.s_label = take((size_t)p.npad * 4);
-  p.s_lse = take((size_t)p.npad * 4);
-  p.s_x = take((size_t)p.npad * row);
+  p.s_norm = take((size_t)p.npad * 8);
+  p.s_own = take((size_t)p.npad * 4);
   p.state = at;
   at = 0;
-  p.f_part = take(up(d->vocab, 256) / 32 * (size_t)p.npad * 8 / (p.few ? 1 : p.wide ? 4 : 2));
+  p.f_part = take(up(d->vocab, p.tile) / p.part * (size_t)p.npad * 8);
   p.f_target = take((size_t)p.npad * 4);
   p.f_loss = take((size_t)p.npad * 4);
-  p.f_w = take(p.in_place ? 0 : p.fwd_rows * row);
+  p.f_x = take(p.size == FEW ? 0 : p.npad * row * p.P);
+  p.f_w = take(p.size == FEW || p.in_place ? 0 : p.fwd_rows * row * p.P);
   p.fwd = at;
   at = 0;
   p.b_cells = take(CELLS * 4);
   p.b_g = take((size_t)p.npad * 4);
-  p.b_x = take(d->dtype == 0 ? (size_t)p.npad * row : 0);
-  p.b_w = take(p.bwd_rows * row);
-  p.b_grad = take((size_t)p.P * p.npad * p.bwd_rows * 2);
+  p.b_x = take(p.npad * row * p.grad_P);
+  p.b_w = take(p.bwd_rows * row * p.grad_P);
+  p.b_grad = take((size_t)p.grad_P * p.npad * p.bwd_rows * 2);
   p.b_dx = take((size_t)p.splits * p.npad * p.kp * 4);
   p.b_dw = take(p.w_splits > 1 ? p.w_splits * piece * p.kp * 4 : 0);
   p.bwd = at;
@@ -195,10 +219,11 @@ __global__ __launch_bounds__(256) void loss_largest_kernel(const S* src, long ld
 }
 
 // Rows (named by map, or all) as planes of kp columns, those past `cols` zero; rows past the last one up to a multiple of 64 zero too.
-// cell: the values are scaled below 2^15 by the power of two that suits its magnitude.  most: their largest magnitude goes there.
+// cell: the values are scaled below 2^15 by the power of two that suits its magnitude.  most: their largest magnitude goes there.  back: the last
+// 64 columns end with the row's last value, `back` zeros before what is left (TileProduct::run).
 template <class S, class D, int P>
 __global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld, int rows, int cols, int kp, const int* map, const unsigned* count,
-                                                          const unsigned* cell, D* dst, long plane, unsigned* most) {
+                                                          const unsigned* cell, D* dst, long plane, unsigned* most, int back) {
   const int live = count != nullptr ? (int)*count : rows;
   const unsigned per = kp / 8, i = blockIdx.x * 256 + threadIdx.x;      // (below 2^31: loss_plan)
   const int r = (int)(i / per), c = (int)(i % per) * 8;
@@ -206,7 +231,8 @@ __global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld,
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 0.f;
-  if (r < live && c < cols) load_values(src + (map != nullptr ? map[r] : r) * ld + c, cols - c, v);
+  const int from = back > 0 && c >= kp - 64 ? c - back : c;
+  if (r < live && from < cols && (from == c || from >= kp - 64)) load_values(src + (map != nullptr ? map[r] : r) * ld + from, cols - from, v);
   if (most != nullptr) {
     unsigned best = 0;
 #pragma unroll
@@ -237,15 +263,17 @@ __global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld,
 struct LossTileArgs {
   const void *w, *x;
   long w_plane, w_ld, x_plane;
-  int kp, vocab, v0, vend;                 // the piece: entries v0 .. vend - 1
-  int n, tiles_m, tiles_n;
+  int kp, v0, vend;                        // the piece: entries v0 .. vend - 1
+  int tail, back;                          // see TileProduct::run; tail in features
+  int n, tiles_m;
   const unsigned *count, *x_cell, *w_cell;  // cells: null where the planes are not scaled
   const int* label;
   float2* part;                            // [parts][npad]
   float* target;
   int npad;
   // backward
-  const float *lse, *g;
+  const float2* norm;                      // maximum, log2 of the sum
+  const float *own, *g;                    // the label's G / g
   const unsigned* g_cell;
   _Float16* grad;                          // [planes][npad][grad_ld]
   long grad_plane;
@@ -277,7 +305,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
   t.init(shared);
   t.operand_a((const T*)G.w, G.w_plane, G.w_ld, tile.m * Tiles::TM, G.vend - G.v0);
   t.operand_b((const T*)G.x, G.x_plane, G.kp, n0, live);
-  t.run(G.kp / Tiles::BK);
+  t.run(G.kp / Tiles::BK, 0, G.back > 0 ? G.tail / Tiles::BK : -1, G.back);
 
   constexpr bool SCALED = Tiles::P == 2 || GRAD;
   const int unscale = SCALED && G.x_cell != nullptr ? -(plane_shift(*G.x_cell) + plane_shift(*G.w_cell)) : 0;
@@ -318,27 +346,29 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, t.acc[i][j][e]);
       top = halves_max(top);
-      const float from = top > -INFINITY ? top * kLog2e : 0.f;
+      const float from = top > -INFINITY ? top : 0.f;
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < Tiles::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sum += fast_exp2(__builtin_fmaf(t.acc[i][j][e], kLog2e, -from));
+        for (int e = 0; e < 16; ++e) sum += fast_exp2((t.acc[i][j][e] - from) * kLog2e);
       sum = halves_sum(sum);
       if (ok && t.lane < 32) G.part[(size_t)((m0 / PART) + t.wm) * G.npad + token] = make_float2(top, sum);
     } else {
       const int pad = (live + 63) / 64 * 64;
-      const float lse = ok ? G.lse[token] : 0.f, g = ok ? __builtin_ldexpf(G.g[token], g_shift) : 0.f;
+      const float2 norm = ok ? G.norm[token] : make_float2(0.f, 0.f);
+      const float g = ok ? __builtin_ldexpf(G.g[token], g_shift) : 0.f;
 #pragma unroll
       for (int i = 0; i < Tiles::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) t.acc[i][j][e] = ok ? g * fast_exp2((t.acc[i][j][e] - lse) * kLog2e) : 0.f;
+        for (int e = 0; e < 16; ++e) t.acc[i][j][e] = ok ? g * fast_exp2(__builtin_fmaf(t.acc[i][j][e] - norm.x, kLog2e, -norm.y)) : 0.f;
       if (__any(hit)) {
+        const float at_label = hit ? g * G.own[token] : 0.f;
 #pragma unroll
         for (int i = 0; i < Tiles::MI; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (hit && own == 32 * i + 8 * (e >> 2) + 4 * (t.lane >> 5) + (e & 3)) t.acc[i][j][e] -= g;
+            if (hit && own == 32 * i + 8 * (e >> 2) + 4 * (t.lane >> 5) + (e & 3)) t.acc[i][j][e] = at_label;
       }
       if (cut) {
 #pragma unroll
@@ -378,11 +408,192 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
   }
 }
 
-// lse and loss of TOKENS tokens from the parts' maxima and sums: 256 / TOKENS threads a token.  (8 of them read whole 64 bytes; 2 end a long
+// ------------------------------------------------------------------------------------ few rows
+
+// Up to 32 rows (scoring, decoding): one pass over the weight where it lies, of any type and alignment, is all their time.  Tiles of 128 entries by
+// 32 rows, 128 bytes of each at a time in LDS (swizzled as TileOperand's).  Rows that begin at multiples of 16 bytes are copied there three
+// stages ahead of their use (24 rows of 4096 features, 131072 entries in bf16, 1.07 GB: 5.8 TB/s); others go through registers, a stage ahead
+// (4.7 TB/s).  fp32 takes fp32 products (32 x 32 x 2: half the time that the weight takes from memory), so there are no planes.  Every
+// work-group finds out the rows that count by itself.
+struct LossFewArgs {
+  const void *x, *w, *labels;
+  long x_ld, w_ld, ignore;
+  int is64, n, dim, vocab, npad;
+  int *map, *place, *label;
+  unsigned* cells;
+  float2* part;
+  float *target, *losses;
+};
+template <class S, bool ALIGNED>
+__global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
+  // (all of LDS is the stages: two work-groups fit into a CU)
+  constexpr int STAGES = ALIGNED ? 4 : 2, STAGE = 160 * 128;
+  __shared__ __align__(1024) char stage_s[STAGES][STAGE];      // rows of 128 bytes: entries, then rows of x
+  int* map_s = reinterpret_cast<int*>(stage_s[0]);
+  float(*top_s)[32] = reinterpret_cast<float(*)[32]>(stage_s[0]), (*sum_s)[32] = top_s + 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, token = lane & 31;
+  const long given = lane < G.n ? (G.is64 ? ((const long*)G.labels)[lane] : (long)((const int*)G.labels)[lane]) : G.ignore;
+  const bool counts = given != G.ignore;
+  const unsigned long mask = __ballot(counts);
+  const int live = __popcll(mask), c = __popcll(mask & ((1ul << lane) - 1)), label = given >= 0 && given < G.vocab ? (int)given : -1;
+  if (wave == 0 && counts) {
+    map_s[c] = lane;
+    map_s[32 + c] = label;
+  }
+  if (blockIdx.x == 0 && wave == 0) {
+    if (lane < G.n) G.place[lane] = counts ? c : -1;
+    if (counts) {
+      G.map[c] = lane;
+      G.label[c] = label;
+    } else if (G.losses != nullptr && lane < G.n) {
+      G.losses[lane] = 0.f;
+    }
+    if (lane < CELLS) G.cells[lane] = lane == CELL_ROWS ? (unsigned)live : 0;
+  }
+  if (live == 0) return;
+  __syncthreads();
+
+  // (an XCD takes neighbouring tiles: 4.8 TB/s with every eighth of them)
+  const int tile = xcd_run(blockIdx.x, gridDim.x), m0 = tile * 128 + 32 * wave, dim = G.dim;
+  constexpr int V = 16 / sizeof(S), BK = 8 * V;      // values of 16 bytes, of a stage
+  typedef decltype(load_any<V>((const S*)nullptr)) vec;
+  // this thread's 16 bytes of five rows: every 32nd entry, one row of x
+  const int r0 = tid >> 3, swz = (r0 >> 1) & 7, chunk = ALIGNED ? (tid & 7) ^ swz : tid & 7, first = tile * 128;
+  const S* src[5];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) src[u] = (const S*)G.w + (long)min(first + r0 + 32 * u, G.vocab - 1) * G.w_ld + chunk * V;
+  src[4] = (const S*)G.x + (long)map_s[min(r0, live - 1)] * G.x_ld + chunk * V;
+  const int own = token < live ? map_s[32 + token] - m0 : -1;
+  __syncthreads();
+  char* to = &stage_s[0][0] + r0 * 128 + 16 * (chunk ^ swz);
+  vec held[2][5];
+  floatx16 part[4], acc = zero_acc();      // sums in parts: each of 64 products, then theirs
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) part[ks] = zero_acc();
+  auto store = [&](const vec (&v)[5], int buf) {
+#pragma unroll
+    for (int u = 0; u < 5; ++u) *reinterpret_cast<vec*>(to + buf * STAGE + u * 32 * 128) = v[u];
+  };
+  auto products = [&](int buf) {
+    const char* row = stage_s[buf] + token * 128;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const int at = 16 * ((2 * ks + h) ^ ((token >> 1) & 7));
+      const vec a = *reinterpret_cast<const vec*>(row + wave * 32 * 128 + at), b = *reinterpret_cast<const vec*>(row + 128 * 128 + at);
+      if constexpr (sizeof(S) == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[ks] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], part[ks], 0, 0, 0);
+      } else {
+        part[ks] = mma(a, b, part[ks]);
+      }
+    }
+  };
+  auto piece = [&](int k) {      // (sums in pieces: see TileProduct::PIECES)
+    if (k % 256 == 0) {
+      acc += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) part[ks] = zero_acc();
+    }
+  };
+  int k = 0;
+  if constexpr (ALIGNED) {
+    typedef __attribute__((address_space(3))) void* lds_p;
+    const unsigned mine = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long)(lds_p)stage_s + wave * 1024);
+    const int stages = dim / BK;
+    // (a stage past the last one: no lane takes part)
+    auto copy = [&](int t) {
+      const unsigned lanes = __builtin_amdgcn_readfirstlane(t < stages ? ~0u : 0u);
+#pragma unroll
+      for (int u = 0; u < 5; ++u)
+        asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 vcc, exec\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\ts_nop 0\n\t"
+                     "global_load_lds_dwordx4 %1, off\n\ts_mov_b64 exec, vcc"
+                     :: "s"(mine + (t & 3) * STAGE + u * 32 * 128), "v"(src[u] + t * BK), "s"(lanes) : "memory", "m0", "vcc");
+    };
+#pragma unroll
+    for (int t = 0; t < 3; ++t) copy(t);
+    for (int t = 0; t < stages; ++t, k += BK) {
+      fence();
+      asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      fence();
+      copy(t + 3);
+      products(t & 3);
+      piece(k + BK);
+    }
+    fence();
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    fence();
+  } else {
+    // (No branch around a load - behind the last one it is read again - or every use of one waits for all of them.  A buffer is written again
+    // when all have passed the barrier behind its reading.)
+    const int pairs = dim / (2 * BK) * (2 * BK);
+    auto load = [&](int at, vec (&into)[5]) {
+#pragma unroll
+      for (int u = 0; u < 5; ++u) into[u] = load_any<V>(src[u] + at);
+    };
+    if (pairs > 0) {
+      load(0, held[0]);
+      load(BK, held[1]);
+      for (; k < pairs; k += 2 * BK) {
+        const int next = min(k + 2 * BK, pairs - 2 * BK);
+        store(held[0], 0);
+        load(next, held[0]);
+        __syncthreads();
+        products(0);
+        store(held[1], 1);
+        load(next + BK, held[1]);
+        __syncthreads();
+        products(1);
+        piece(k + 2 * BK);
+      }
+    }
+  }
+  for (; k < dim; k += BK) {      // what is left of the rows
+    const int have = dim - k - chunk * V;
+#pragma unroll
+    for (int u = 0; u < 5; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) held[0][u][e] = e < have ? src[u][k + e] : (S)0.f;
+    __syncthreads();
+    store(held[0], 0);
+    __syncthreads();
+    products(0);
+  }
+  acc += (part[0] + part[1]) + (part[2] + part[3]);
+
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int row = 8 * (e >> 2) + 4 * h + (e & 3);
+    if (token < live && row == own) G.target[token] = acc[e];
+    if (m0 + row >= G.vocab) acc[e] = -INFINITY;
+    top = fmaxf(top, acc[e]);
+  }
+  top = halves_max(top);
+  const float from = top > -INFINITY ? top : 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum += fast_exp2((acc[e] - from) * kLog2e);
+  sum = halves_sum(sum);
+  __syncthreads();
+  if (h == 0) {
+    top_s[wave][token] = top;
+    sum_s[wave][token] = sum;
+  }
+  __syncthreads();
+  if (tid >= live) return;
+  float most = -INFINITY, s = 0.f;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) most = fmaxf(most, top_s[v][tid]);
+  const float at = most > -INFINITY ? most : 0.f;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) s += sum_s[v][tid] * fast_exp2((top_s[v][tid] - at) * kLog2e);
+  G.part[(size_t)blockIdx.x * G.npad + tid] = make_float2(most, s);
+}
+
+// norm and loss of TOKENS tokens from the parts' maxima and sums: 256 / TOKENS threads a token.  (8 of them read whole 64 bytes; 2 end a long
 // vocabulary's parts sooner where there are not many: 24 tokens, 4096 parts 16 -> 6 us.)
 template <int TOKENS>
 __global__ __launch_bounds__(256) void loss_merge_kernel(const float2* part, int parts, int npad, const unsigned* count, const int* map, const int* label,
-                                                         const float* target, float* lse, float* loss, float* losses) {
+                                                         const float* target, float2* norm, float* own, float* loss, float* losses) {
   constexpr int LANES = 256 / TOKENS;
   __shared__ float top_s[LANES][TOKENS], sum_s[LANES][TOKENS];
   const int live = (int)*count, tid = threadIdx.x, at = tid % TOKENS, lane = tid / TOKENS, token = blockIdx.x * TOKENS + at;
@@ -411,10 +622,10 @@ __global__ __launch_bounds__(256) void loss_merge_kernel(const float2* part, int
     }
   }
   if (lane != 0 || token >= live) return;
-  float l = (top > -INFINITY ? top : 0.f) + fast_log2(sum) * kLn2;
-  if (label[token] < 0) l = __builtin_nanf("");      // no entry of the vocabulary: said by the loss and all gradients
-  const float value = l - (label[token] < 0 ? 0.f : target[token]);
-  lse[token] = l;
+  const float from = label[token] < 0 ? __builtin_nanf("") : top > -INFINITY ? top : 0.f;      // no entry of the vocabulary: said by the loss and all gradients
+  const float value = from - (label[token] < 0 ? 0.f : target[token]) + logf(sum);
+  norm[token] = make_float2(from, log2f(sum));
+  own[token] = expm1f(-value);
   loss[token] = value;
   if (losses != nullptr) losses[map[token]] = value;
 }
@@ -466,7 +677,7 @@ struct LossGradArgs {
   const unsigned *count, *other_cell, *g_cell;
   // dx
   float* sums;                        // [splits][npad][kp]
-  int npad, per, first;               // steps of a split; first piece
+  int npad, first;                    // first piece
   int splits;
   // dw
   void* dw;
@@ -482,7 +693,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dx_kernel(const LossGr
   const int nth = xcd_run(blockIdx.x, tiles * G.splits), split = nth / tiles;
   const TileAt tile = tile_in(nth % tiles, G.tiles_m, tiles_n, 4);
   const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN;
-  const int from = min(split * G.per, G.grad_ld / Tiles::BK), steps = min(G.per, G.grad_ld / Tiles::BK - from);
+  const int all = G.grad_ld / Tiles::BK, per = (all + G.splits - 1) / G.splits, from = min(split * per, all), steps = min(per, all - from);
   if (steps <= 0 && !G.first) return;
   Tiles t;
   t.init(shared);
@@ -569,37 +780,40 @@ typedef __bf16 B16;
 typedef _Float16 H16;
 template <class T, int P> struct LogitTiles {
   typedef TileProduct<T, P, ROWS, ROWS, 256, 256, 2, 4, 32, P == 2 ? 2 : 4> Wide;
-  typedef TileProduct<T, P, ROWS, ROWS, 128, 128, 2, 2, P == 2 ? 32 : 64, 2> Small;
+  typedef TileProduct<T, P, ROWS, ROWS, 128, 128, 2, 4, P == 2 ? 32 : 64, 4> Middle;
+  typedef TileProduct<T, P, ROWS, ROWS, 64, 64, 2, 2, 64, P == 2 ? 2 : 4> Tiny;
   typedef TileProduct<T, P, ROWS, ROWS, 128, 32, 4, 1, 64, P == 2 ? 2 : 4> Few;
 };
 template <int P> struct GradTiles {
   typedef TileProduct<H16, P, COLUMNS, ROWS, 256, 256, 2, 4, 32, P == 2 ? 2 : 4> WideX;
-  typedef TileProduct<H16, P, COLUMNS, ROWS, 128, 128, 2, 2, P == 2 ? 32 : 64, 2> SmallX;
+  typedef TileProduct<H16, P, COLUMNS, ROWS, 128, 128, 2, 4, P == 2 ? 32 : 64, 4> MiddleX;
   typedef TileProduct<H16, P, COLUMNS, COLUMNS, 256, 256, 2, 4, 32, P == 2 ? 2 : 4> WideW;
-  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 128, 128, 2, 2, P == 2 ? 32 : 64, 2> SmallW;
+  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 128, 128, 2, 4, P == 2 ? 32 : 64, 4> MiddleW;
+  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 128, 128, 2, 4, P == 2 ? 32 : 64, 2> FewW;
 };
 
 template <class Tiles, bool GRAD>
 static void launch_tile(LossTileArgs a, hipStream_t st) {
   a.tiles_m = (a.vend - a.v0 + Tiles::TM - 1) / Tiles::TM;
-  a.tiles_n = ((GRAD ? a.npad : a.n) + Tiles::TN - 1) / Tiles::TN;
-  hipLaunchKernelGGL((loss_tile_kernel<Tiles, GRAD>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(Tiles::THREADS), 0, st, a);
+  const int tiles_n = ((GRAD ? a.npad : a.n) + Tiles::TN - 1) / Tiles::TN;
+  hipLaunchKernelGGL((loss_tile_kernel<Tiles, GRAD>), dim3((unsigned)(a.tiles_m * tiles_n)), dim3(Tiles::THREADS), 0, st, a);
 }
 template <class T, int P, bool GRAD>
 static void launch_tiles(const LossPlan& p, const LossTileArgs& a, hipStream_t st) {
   typedef LogitTiles<T, P> L;
-  if (p.few) launch_tile<typename L::Few, GRAD>(a, st);
-  else if (p.wide) launch_tile<typename L::Wide, GRAD>(a, st);
-  else launch_tile<typename L::Small, GRAD>(a, st);
+  if (p.size == WIDE) launch_tile<typename L::Wide, GRAD>(a, st);
+  else if (p.size == MIDDLE) launch_tile<typename L::Middle, GRAD>(a, st);
+  else if (p.size == TINY) launch_tile<typename L::Tiny, GRAD>(a, st);
+  else if constexpr (GRAD) launch_tile<typename L::Few, GRAD>(a, st);      // (the forward of few rows: loss_few_kernel)
 }
 
 static unsigned blocks_for(long work) { return (unsigned)std::max<long>(1, (work + 255) / 256); }
 
 template <class S, class D, int P>
 static void planes(const void* src, long ld, int rows, int rows_cap, int cols, int kp, const int* map, const unsigned* count, const unsigned* cell, void* dst,
-                   long plane, hipStream_t st, unsigned* most = nullptr) {
+                   long plane, hipStream_t st, unsigned* most = nullptr, int back = 0) {
   hipLaunchKernelGGL((loss_planes_kernel<S, D, P>), dim3(blocks_for((long)up(rows_cap, 64) * kp / 8)), dim3(256), 0, st, (const S*)src, ld, rows, cols, kp,
-                     map, count, cell, (D*)dst, plane, most);
+                     map, count, cell, (D*)dst, plane, most, back);
 }
 template <class S>
 static void largest(const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, unsigned* cell, hipStream_t st) {
@@ -615,10 +829,27 @@ static void forward_weight(const nsa_loss_desc* d, const LossPlan& p, const void
   else planes<float, H16, 2>((const float*)weight + (long)v0 * d->w_stride, d->w_stride, rows, rows, d->dim, p.kp, nullptr, nullptr, cell, dst, plane, st);
 }
 
+template <int P>
+static void dx_tiles(const LossPlan& p, const LossGradArgs& q, hipStream_t st) {
+  const int tile = p.size == WIDE ? 256 : 128;
+  const dim3 grid((unsigned)(q.tiles_m * ((p.n + tile - 1) / tile) * p.splits));
+  if (p.size == WIDE) hipLaunchKernelGGL((loss_dx_kernel<typename GradTiles<P>::WideX>), grid, dim3(512), 0, st, q);
+  else hipLaunchKernelGGL((loss_dx_kernel<typename GradTiles<P>::MiddleX>), grid, dim3(512), 0, st, q);
+}
 template <int P, class O, bool SLICES>
-static void dw_tiles(const LossPlan& p, const LossGradArgs& q, dim3 grid, hipStream_t st) {
-  if (p.wide) hipLaunchKernelGGL((loss_dw_kernel<typename GradTiles<P>::WideW, O, SLICES>), grid, dim3(512), 0, st, q);
-  else hipLaunchKernelGGL((loss_dw_kernel<typename GradTiles<P>::SmallW, O, SLICES>), grid, dim3(256), 0, st, q);
+static void dw_tiles(const LossPlan& p, const LossGradArgs& q, hipStream_t st) {
+  const dim3 grid((unsigned)(q.tiles_m * q.tiles_n * p.w_splits));
+  // few rows: nothing to read ahead, so two work-groups a CU that write in turn (25 rows, 1917 features, 21120 entries in bf16: 36 -> 24 us)
+  if constexpr (!SLICES)
+    if (p.size == FEW) {
+      hipLaunchKernelGGL((loss_dw_kernel<typename GradTiles<P>::FewW, O, SLICES>), grid, dim3(512), 0, st, q);
+      return;
+    }
+  // (fp16 operands of two planes: few rows only)
+  if constexpr (P == 1 || sizeof(O) == 4) {
+    if (p.size == WIDE) hipLaunchKernelGGL((loss_dw_kernel<typename GradTiles<P>::WideW, O, SLICES>), grid, dim3(512), 0, st, q);
+    else hipLaunchKernelGGL((loss_dw_kernel<typename GradTiles<P>::MiddleW, O, SLICES>), grid, dim3(512), 0, st, q);
+  }
 }
 static void rows_of_slices(const nsa_loss_desc* d, const float* sums, int splits, int size, int kp, int n, const int* place, void* to, hipStream_t st) {
   const dim3 grid(blocks_for((long)n * ((d->dim + 3) / 4)));
@@ -651,21 +882,34 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
   char *s = (char*)state, *w = (char*)ws;
   unsigned* cells = (unsigned*)s;
   int *map = (int*)(s + p.s_map), *place = (int*)(s + p.s_place), *label = (int*)(s + p.s_label);
-  float *lse = (float*)(s + p.s_lse), *each = (float*)(w + p.f_loss), *target = (float*)(w + p.f_target);
+  float2* norm = (float2*)(s + p.s_norm);
+  float *own = (float*)(s + p.s_own), *each = (float*)(w + p.f_loss), *target = (float*)(w + p.f_target);
   float* losses = d->reduction == 0 ? loss : nullptr;
-  hipLaunchKernelGGL(loss_rows_kernel, dim3((unsigned)std::max(1, (p.n + 1023) / 1024)), dim3(256), 0, st, labels, (int)d->labels_int64, p.n, d->vocab,
-                     (long)d->ignore_index, map, place, label, cells, losses);
+  float2* part = (float2*)(w + p.f_part);
   const unsigned *count = cells + CELL_ROWS, *xc = d->dtype == 2 ? cells + CELL_X : nullptr, *wc = d->dtype == 2 ? cells + CELL_W : nullptr;
-  const long x_plane = (long)p.npad * p.kp;
-  if (p.n > 0) {
+  if (p.size == FEW) {
+    LossFewArgs a{x, weight, labels, (long)d->x_stride, (long)d->w_stride, (long)d->ignore_index, (int)d->labels_int64, p.n, d->dim, d->vocab, p.npad,
+                  map, place, label, cells, part, target, losses};
+    const dim3 grid((unsigned)((d->vocab + 127) / 128));
+    const int each = d->dtype == 2 ? 4 : 2;
+    const bool aligned = (((uintptr_t)x | (uintptr_t)weight) & 15) == 0 && d->x_stride * each % 16 == 0 && d->w_stride * each % 16 == 0;
+    const auto kernel = d->dtype == 0 ? aligned ? loss_few_kernel<B16, true> : loss_few_kernel<B16, false>
+                        : d->dtype == 1 ? aligned ? loss_few_kernel<H16, true> : loss_few_kernel<H16, false>
+                                        : aligned ? loss_few_kernel<float, true> : loss_few_kernel<float, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(loss_rows_kernel, dim3((unsigned)((p.n + 1023) / 1024)), dim3(256), 0, st, labels, (int)d->labels_int64, p.n, d->vocab,
+                       (long)d->ignore_index, map, place, label, cells, losses);
+    const long x_plane = (long)p.npad * p.kp;
+    const int back = p.in_place ? p.kp - d->dim : 0;
     if (d->dtype == 2) {
       largest<float>(x, d->x_stride, p.n, d->dim, map, count, cells + CELL_X, st);
       largest<float>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
-      planes<float, H16, 2>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, xc, s + p.s_x, x_plane, st);
+      planes<float, H16, 2>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, xc, w + p.f_x, x_plane, st);
     } else if (d->dtype == 1) {
-      planes<H16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, s + p.s_x, x_plane, st);
+      planes<H16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, w + p.f_x, x_plane, st, nullptr, back);
     } else {
-      planes<B16, B16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, s + p.s_x, x_plane, st, cells + CELL_X);
+      planes<B16, B16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, w + p.f_x, x_plane, st, cells + CELL_X, back);
     }
     const int rows = p.in_place ? d->vocab : p.fwd_rows;
     for (long v0 = 0; v0 < d->vocab; v0 += rows) {
@@ -675,36 +919,38 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
       if (p.in_place) {
         a.w = weight;
         a.w_ld = d->w_stride;
+        a.tail = p.kp - 64;
+        a.back = back;
       } else {
         forward_weight(d, p, weight, a.v0, a.vend - a.v0, wc, w + p.f_w, st);
         a.w = w + p.f_w;
         a.w_ld = p.kp;
         a.w_plane = (long)p.kp * up(a.vend - a.v0, 64);
       }
-      a.x = s + p.s_x; a.x_plane = x_plane; a.kp = p.kp; a.vocab = d->vocab; a.n = p.n; a.npad = p.npad;
-      a.count = count; a.x_cell = xc; a.w_cell = wc; a.label = label; a.part = (float2*)(w + p.f_part); a.target = target;
+      a.x = w + p.f_x; a.x_plane = x_plane; a.kp = p.kp; a.n = p.n; a.npad = p.npad;
+      a.count = count; a.x_cell = xc; a.w_cell = wc; a.label = label; a.part = part; a.target = target;
       if (d->dtype == 0) launch_tiles<B16, 1, false>(p, a, st);
       else if (d->dtype == 1) launch_tiles<H16, 1, false>(p, a, st);
       else launch_tiles<H16, 2, false>(p, a, st);
     }
-    const int part = p.few ? 32 : p.wide ? 128 : 64, tile = p.few ? 128 : p.wide ? 256 : 128;
-    const int parts = (d->vocab + tile - 1) / tile * (tile / part);
+  }
+  if (p.n > 0) {
+    const int parts = (int)(up(d->vocab, p.tile) / p.part);
     const auto merge = p.n <= 2048 ? loss_merge_kernel<2> : loss_merge_kernel<8>;
-    hipLaunchKernelGGL(merge, dim3((unsigned)(p.n <= 2048 ? (p.n + 1) / 2 : (p.n + 7) / 8)), dim3(256), 0, st, (const float2*)(w + p.f_part), parts, p.npad, count,
-                       (const int*)map, (const int*)label, (const float*)target, lse, each, losses);
+    hipLaunchKernelGGL(merge, dim3((unsigned)(p.n <= 2048 ? (p.n + 1) / 2 : (p.n + 7) / 8)), dim3(256), 0, st, (const float2*)part, parts, p.npad, count,
+                       (const int*)map, (const int*)label, (const float*)target, norm, own, each, losses);
   }
   if (d->reduction != 0)
     hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, (const float*)each, count, (int)(d->reduction == 1), loss);
   return (int)hipGetLastError();
 }
 
-extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const void* state, size_t state_bytes, const float* dloss, void* ws, size_t ws_bytes,
-                            void* dx, void* dw, void* stream) {
+extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* weight, const void* state, size_t state_bytes, const float* dloss, void* ws,
+                            size_t ws_bytes, void* dx, void* dw, void* stream) {
   LossPlan p;
   if (int rc = loss_plan(d, weight, p)) return rc;
-  if (!weight || !state || !dloss || !ws || (!dx && !dw)) return NSA_E_ARG;
+  if (!x || !weight || !state || !dloss || !ws || (!dx && !dw) || p.n == 0) return NSA_E_ARG;
   if (state_bytes < p.state || ws_bytes < p.bwd) return NSA_E_WORKSPACE;
-  if (p.n == 0) return NSA_E_ARG;
   hipStream_t st = (hipStream_t)stream;
   const char* s = (const char*)state;
   char* w = (char*)ws;
@@ -714,15 +960,22 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const vo
   const unsigned* count = kept + CELL_ROWS;
   float* g = (float*)(w + p.b_g);
   hipLaunchKernelGGL(loss_weights_kernel, dim3(1), dim3(1024), 0, st, dloss, (int)d->reduction, count, map, g, cells);
-  // all operands in fp16: x once, w with each piece
-  const long x_plane = (long)p.npad * p.kp;
-  const void* xg = s + p.s_x;
-  const unsigned *xc = d->dtype != 1 ? kept + CELL_X : nullptr, *wc = d->dtype == 2 ? kept + CELL_W : d->dtype == 0 ? cells + CELL_W : nullptr;
+  // All operands in fp16: x once, w with each piece.  Magnitudes: those the forward has found, else here.
+  const bool have_x = p.size != FEW, have_w = p.size != FEW && d->dtype == 2;
+  const unsigned *xc = d->dtype == 1 ? nullptr : have_x ? kept + CELL_X : cells + CELL_X, *wc = d->dtype == 1 ? nullptr : have_w ? kept + CELL_W : cells + CELL_W;
   if (d->dtype == 0) {
-    planes<B16, H16, 1>(s + p.s_x, p.kp, p.n, p.n, p.kp, p.kp, nullptr, count, xc, w + p.b_x, x_plane, st);
-    xg = w + p.b_x;
+    if (!have_x) largest<B16>(x, d->x_stride, p.n, d->dim, map, count, cells + CELL_X, st);
     largest<B16>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
+  } else if (d->dtype == 2 && !have_x) {
+    largest<float>(x, d->x_stride, p.n, d->dim, map, count, cells + CELL_X, st);
+    largest<float>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
   }
+  const long x_plane = (long)p.npad * p.kp;
+  void* xg = w + p.b_x;
+  if (d->dtype == 0) planes<B16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, xc, xg, x_plane, st);
+  else if (d->dtype == 2) planes<float, H16, 2>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, xc, xg, x_plane, st);
+  else if (p.grad_P == 2) planes<H16, H16, 2>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, xg, x_plane, st);
+  else planes<H16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, xg, x_plane, st);
   const int each = d->dtype == 2 ? 4 : 2;
   for (long v0 = 0; v0 < d->vocab; v0 += p.bwd_rows) {
     LossTileArgs a{};
@@ -731,31 +984,29 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const vo
     const int entries = a.vend - a.v0, ld = (int)up(entries, 64);
     const long w_plane = (long)p.kp * ld;
     const char* from = (const char*)weight + v0 * d->w_stride * each;
-    if (d->dtype == 0) planes<B16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, w + p.b_w, w_plane, st);
-    else if (d->dtype == 1) planes<H16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, nullptr, w + p.b_w, w_plane, st);
-    else planes<float, H16, 2>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, w + p.b_w, w_plane, st);
-    a.w = w + p.b_w; a.w_ld = p.kp; a.w_plane = w_plane;
-    a.x = xg; a.x_plane = x_plane; a.kp = p.kp; a.vocab = d->vocab; a.n = p.n; a.npad = p.npad;
+    void* wg = w + p.b_w;
+    if (d->dtype == 0) planes<B16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, wg, w_plane, st);
+    else if (d->dtype == 2) planes<float, H16, 2>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, wg, w_plane, st);
+    else if (p.grad_P == 2) planes<H16, H16, 2>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, nullptr, wg, w_plane, st);
+    else planes<H16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, nullptr, wg, w_plane, st);
+    a.w = wg; a.w_ld = p.kp; a.w_plane = w_plane;
+    a.x = xg; a.x_plane = x_plane; a.kp = p.kp; a.n = p.n; a.npad = p.npad;
     a.count = count; a.x_cell = xc; a.w_cell = wc; a.label = label;
-    a.lse = (const float*)(s + p.s_lse); a.g = g; a.g_cell = cells + CELL_G;
+    a.norm = (const float2*)(s + p.s_norm); a.own = (const float*)(s + p.s_own); a.g = g; a.g_cell = cells + CELL_G;
     a.grad = (H16*)(w + p.b_grad); a.grad_plane = (long)p.npad * ld; a.grad_ld = ld;
-    if (d->dtype == 2) launch_tiles<H16, 2, true>(p, a, st);
+    if (p.grad_P == 2) launch_tiles<H16, 2, true>(p, a, st);
     else launch_tiles<H16, 1, true>(p, a, st);
 
     LossGradArgs q{};
     q.grad = a.grad; q.grad_plane = a.grad_plane; q.grad_ld = ld; q.kp = p.kp; q.dim = d->dim; q.entries = entries;
     q.count = count; q.g_cell = cells + CELL_G; q.npad = p.npad;
-    const int tile = p.wide ? 256 : 128;
+    const int tile = p.size == WIDE ? 256 : 128;
     q.tiles_m = (p.kp + tile - 1) / tile;
     if (dx) {
-      const int bk = p.P == 2 || p.wide ? 32 : 64;
-      q.other = (const H16*)(w + p.b_w); q.other_plane = w_plane; q.other_cell = wc;
-      q.sums = (float*)(w + p.b_dx); q.splits = p.splits; q.per = (ld / bk + p.splits - 1) / p.splits; q.first = v0 == 0;
-      const dim3 grid((unsigned)(q.tiles_m * ((p.n + tile - 1) / tile) * p.splits));
-      if (p.P == 1 && p.wide) hipLaunchKernelGGL((loss_dx_kernel<GradTiles<1>::WideX>), grid, dim3(512), 0, st, q);
-      else if (p.P == 1) hipLaunchKernelGGL((loss_dx_kernel<GradTiles<1>::SmallX>), grid, dim3(256), 0, st, q);
-      else if (p.wide) hipLaunchKernelGGL((loss_dx_kernel<GradTiles<2>::WideX>), grid, dim3(512), 0, st, q);
-      else hipLaunchKernelGGL((loss_dx_kernel<GradTiles<2>::SmallX>), grid, dim3(256), 0, st, q);
+      q.other = (const H16*)wg; q.other_plane = w_plane; q.other_cell = wc;
+      q.sums = (float*)(w + p.b_dx); q.splits = p.splits; q.first = v0 == 0;
+      if (p.grad_P == 2) dx_tiles<2>(p, q, st);
+      else dx_tiles<1>(p, q, st);
     }
     if (dw) {
       q.other = (const H16*)xg; q.other_plane = x_plane; q.other_cell = xc;
@@ -764,12 +1015,12 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* weight, const vo
       char* to = (char*)dw + v0 * d->dim * each;
       q.splits = p.w_splits;
       q.dw = slices ? w + p.b_dw : to; q.dw_ld = slices ? p.kp : d->dim; q.dim = slices ? p.kp : d->dim;
-      const dim3 grid((unsigned)(q.tiles_m * q.tiles_n * p.w_splits));
-      if (slices && p.P == 1) dw_tiles<1, float, true>(p, q, grid, st);
-      else if (slices) dw_tiles<2, float, true>(p, q, grid, st);
-      else if (d->dtype == 0) dw_tiles<1, B16, false>(p, q, grid, st);
-      else if (d->dtype == 1) dw_tiles<1, H16, false>(p, q, grid, st);
-      else dw_tiles<2, float, false>(p, q, grid, st);
+      if (slices && p.grad_P == 1) dw_tiles<1, float, true>(p, q, st);
+      else if (slices) dw_tiles<2, float, true>(p, q, st);
+      else if (d->dtype == 0) dw_tiles<1, B16, false>(p, q, st);
+      else if (d->dtype == 2) dw_tiles<2, float, false>(p, q, st);
+      else if (p.grad_P == 2) dw_tiles<2, H16, false>(p, q, st);
+      else dw_tiles<1, H16, false>(p, q, st);
       if (slices) rows_of_slices(d, (const float*)(w + p.b_dw), p.w_splits, entries, p.kp, entries, nullptr, to, st);
     }
   }

@@ -200,21 +200,24 @@ struct TileProduct {
   }
 
   // two planes: the small products are summed by themselves, where there are registers for it, so that a leading sum is rounded once a
-  // product of 16 and not three times
-  static constexpr bool APART = P == 2 && MI * NI <= 4;
+  // product of 16 and not three times; and where there are more, every 256 of the contraction index are a sum of their own (sums of 2048 and
+  // 4096 are then off by 1.2e-7 and 1.6e-7 of their size instead of 3e-7 and 4e-7)
+  static constexpr bool APART = P == 2 && MI * NI <= 4, PIECES = P == 2 && MI * NI <= 2;
 
   // `steps` times BK of the contraction index from k0 * BK on.  All waves of the work-group; LDS is free again behind it.
-  __device__ __forceinline__ void run(int steps, int k0 = 0) {
+  // From stage `tail` on, operand a is read `back` elements before its place: rows that end `back` short of a whole number of stages (the other
+  // operand holds zeros in the place of what comes twice).
+  __device__ __forceinline__ void run(int steps, int k0 = 0, int tail = -1, int back = 0) {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[i][j] = zero_acc();
-    floatx16 small[APART ? MI : 1][APART ? NI : 1];
+    floatx16 small[APART ? MI : 1][APART ? NI : 1], whole[PIECES ? MI : 1][PIECES ? NI : 1];
     if (APART) {
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j) small[APART ? i : 0][APART ? j : 0] = zero_acc();
+        for (int j = 0; j < NI; ++j) small[APART ? i : 0][APART ? j : 0] = whole[PIECES ? i : 0][PIECES ? j : 0] = zero_acc();
     }
     const T* a = A.base + k0 * A.step;
     const T* b = B.base + k0 * B.step;
@@ -226,6 +229,7 @@ struct TileProduct {
       for (int i = 0; i < LOADS; ++i) copy(i, a, b, mine + s * STAGE, s < steps ? ~0u : 0u);
       a += A.step;
       b += B.step;
+      if (s + 1 == tail) a -= back;
     }
     x8 fa[2][P][MI], fb[2][P][NI];
     // the operand with fewer parts first, and with all of it each part of the other: products begin as soon as their operands arrive
@@ -274,12 +278,25 @@ struct TileProduct {
       }
       a += A.step;
       b += B.step;
+      if (t + FIRST + 1 == tail) a -= back;
+      if (PIECES && t % (256 / BK) == 256 / BK - 1) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j) {
+            whole[PIECES ? i : 0][PIECES ? j : 0] += acc[i][j] + small[APART ? i : 0][APART ? j : 0];
+            acc[i][j] = small[APART ? i : 0][APART ? j : 0] = zero_acc();
+          }
+      }
     }
     if (APART) {
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] += small[APART ? i : 0][APART ? j : 0];
+        for (int j = 0; j < NI; ++j) {
+          acc[i][j] += small[APART ? i : 0][APART ? j : 0];
+          if (PIECES) acc[i][j] += whole[PIECES ? i : 0][PIECES ? j : 0];
+        }
     }
     meet<0>();      // (copies without lanes too; LDS is free)
   }

@@ -2648,17 +2648,17 @@ def _(x, weight, labels, ignore_index, reduction):
 @torch.library.custom_op("nsa_amd::linear_cross_entropy_bwd", mutates_args=())
 def linear_cross_entropy_bwd(dloss: Tensor, x: Tensor, weight: Tensor, state: Tensor, ignore_index: int, reduction: int, want_dx: bool,
                              want_dw: bool) -> tuple[Tensor, Tensor]:
-    """(dx 'n d', dw 'v d'), empty where not wanted.  (x itself is in the state; named here, its gradient's dependence on it is known.)"""
+    """(dx 'n d', dw 'v d'), empty where not wanted."""
     rows = x.shape[0]
     make = torch.empty if rows else torch.zeros
     with _on(weight.device):
         dx = make((rows if want_dx else 0, weight.shape[1]), dtype=weight.dtype, device=weight.device)
         dw = make(weight.shape if want_dw else (0, weight.shape[1]), dtype=weight.dtype, device=weight.device)
         if rows and (want_dx or want_dw):
-            weight, dloss = _unit_rows(weight), dloss.to(torch.float32).contiguous()
-            d, state_bytes, _, bwd_bytes = _loss_desc(rows, weight, 0, True, ignore_index, reduction)
+            x, weight, dloss = _unit_rows(x), _unit_rows(weight), dloss.to(torch.float32).contiguous()
+            d, state_bytes, _, bwd_bytes = _loss_desc(rows, weight, x.stride(0), True, ignore_index, reduction)
             ws = torch.empty((bwd_bytes,), dtype=torch.uint8, device=weight.device)
-            _lib.check(_lib.lib().nsa_loss_bwd(C.byref(d), _ptr(weight), _ptr(state), state_bytes, _ptr(dloss), _ptr(ws), bwd_bytes,
+            _lib.check(_lib.lib().nsa_loss_bwd(C.byref(d), _ptr(x), _ptr(weight), _ptr(state), state_bytes, _ptr(dloss), _ptr(ws), bwd_bytes,
                                                _ptr(dx) if want_dx else 0, _ptr(dw) if want_dw else 0, _stream()), "nsa_loss_bwd")
     return dx, dw
 

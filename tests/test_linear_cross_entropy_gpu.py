@@ -118,6 +118,76 @@ def test_large_tiles_and_pieces(n, d, v, dtype):
     _check(x, w, labels, "none", weights)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n,d,v", [
+    (1, 8, 129),                   # features short of one copy of 128 bytes
+    (2, 63, 128),
+    (4, 65, 300),
+    (16, 128, 31),
+    (17, 256, 500),                # whole sums of 256
+    (31, 264, 127),                # and one step more
+    (32, 1000, 385),
+    (32, 520, 1),
+])
+def test_few_rows(n, d, v, dtype):
+    """Up to 32 rows, from rows at multiples of 16 bytes and from others: the same sums in the same order."""
+    from native_sparse_attention_pytorch_amd import ops
+    x, w, labels, weights = _inputs(n, d, v, dtype, seed=d, ignored=0.3 if n > 2 else 0.)
+    _check(x, w, labels, "none", weights)
+    wide = max(8, (d + 7) // 8 * 8) + 8
+    at = [torch.randn(r, wide, device=DEV).to(dtype) for r in (n, v, n, v)]
+    at[0][:, :d], at[1][:, :d], at[2][:, 1:d + 1], at[3][:, 3:d + 3] = x, w, x, w
+    want = ops.linear_cross_entropy(at[0][:, :d], at[1][:, :d], labels, reduction="none")
+    got = ops.linear_cross_entropy(at[2][:, 1:d + 1], at[3][:, 3:d + 3], labels.int(), reduction="none")
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n,d,v", [
+    (70, 72, 700),                 # rows in place, their last 64 features read with what is left of them
+    (200, 200, 2500),
+    (1500, 120, 5000),
+    (600, 1096, 1100),
+    (1100, 520, 40001),            # tiles of 256
+    (33, 2056, 1500),              # tiles of 64, long sums
+])
+def test_features_short_of_whole_steps(n, d, v, dtype):
+    x, w, labels, weights = _inputs(n, d, v, dtype, seed=5)
+    _check(x, w, labels, "none", weights)
+    wide = torch.randn(v, d + 24, device=DEV).to(dtype)
+    wide[:, 8:d + 8] = w
+    _check(x, wide[:, 8:d + 8], labels, "mean", weights)
+
+
+@pytest.mark.parametrize("n", [20, 100])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_likely_labels(n, dtype):
+    """Losses down to 1e-12.  Where the label has the row's largest logit by far, its own logit's error drops out: the loss, and its G but for the
+    weight, are a sum of the others' exponentials, each off by two logits' dL and 2^-16 of itself, beside the label's own 1.  That 1 goes
+    through at most 16 additions in its lane, one of the wave's halves, 4 of waves and 7 of parts, each off by 2^-24 (sums below 2): 28 2^-24."""
+    from native_sparse_attention_pytorch_amd import ops
+    d, v = 96, 300
+    _, w, labels, weights = _inputs(n, d, v, dtype, seed=7, ignored=0.)
+    x = (w.float()[labels] * torch.linspace(8, 40, n, device=DEV)[:, None]).to(dtype)
+    x.requires_grad_(), w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, labels, reduction="none")
+    dx, = torch.autograd.grad(loss, x, weights)
+    x6, w6, at = x.detach().double(), w.detach().double(), labels[:, None]
+    logits, size = x6 @ w6.t().contiguous(), x6.abs() @ w6.abs().t().contiguous()
+    h, u = (2 ** -22, 2 ** -24) if dtype == F32 else (0., torch.finfo(dtype).eps / 2)
+    dl = 2 * (((d / 4 + 8) * 2 ** -24 + 2 * h) * size).amax(-1, keepdim=True) + 2 ** -16
+    assert (logits.argmax(-1) == labels).all()
+    others = torch.exp(logits - logits.gather(1, at)).scatter(1, at, 0.)
+    want = torch.log1p(others.sum(-1, keepdim=True))
+    assert want.min() < 1e-10
+    _within(loss.detach(), (want[:, 0], (dl * want)[:, 0] + 28 * 2 ** -24), "loss")
+    G = weights.double()[:, None] * (others / (1 + others.sum(-1, keepdim=True))).scatter(1, at, torch.expm1(-want))
+    dG = G.abs() * (2 * dl + (2 ** -11 if dtype != F32 else h)) + 2 ** -38 * float(weights.max())
+    dG.scatter_add_(1, at, weights.double()[:, None] * 28 * 2 ** -24)
+    tol = dG @ w6.abs() + G.abs() @ ((h + v / 4 * 2 ** -24) * w6.abs() + 2 ** -38 * float(w6.abs().max()))
+    _within(dx, (G @ w6, 1.01 * tol + u * (G @ w6).abs() + torch.finfo(dtype).tiny * 2 * u), "dx")
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_rows_that_do_not_count_are_not_read(dtype):
     """Whole runs of ignored rows, NaN and infinities in them; their gradients are zeros."""
