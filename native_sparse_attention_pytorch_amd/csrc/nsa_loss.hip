@@ -26,8 +26,8 @@
 namespace nsa {
 
 constexpr int kGradBits = 14;
-// device words of a call: rows that count; bits of the largest finite |x|, |w|, |g|
-enum { CELL_ROWS, CELL_X, CELL_W, CELL_G, CELLS = 16 };
+// device words of a call: rows that count; bits of the largest finite |x|, |w|, |g|; slices of dx
+enum { CELL_ROWS, CELL_X, CELL_W, CELL_G, CELL_SLICES, CELLS = 16 };
 
 // How logits are made: FEW rows as loss_few_kernel has them, the others by tiles of 64, 128 or 256 (loss_plan)
 enum LossSize { FEW, TINY, MIDDLE, WIDE };
@@ -39,7 +39,7 @@ struct LossPlan {
   bool in_place;                          // the forward reads the weight where it lies
   int tile, part;                         // entries of the vocabulary of a tile, of a pair (maximum, sum)
   int fwd_rows, bwd_rows;                 // entries of a piece
-  int splits, w_splits;                   // slices of a piece's entries that dx is summed from, of the rows that dw is
+  int w_splits, last_splits;              // slices of the rows that dw of a piece, of the last one, is summed from
   size_t state, fwd, bwd;                 // bytes
   size_t s_map, s_place, s_label, s_norm, s_own;                            // offsets in the state
   size_t f_part, f_target, f_loss, f_x, f_w;                           // in the forward's workspace
@@ -47,6 +47,8 @@ struct LossPlan {
 };
 
 static size_t up(size_t v, size_t to) { return (v + to - 1) / to * to; }
+
+constexpr int kMaxSlices = 32, kSliceTiles = 512;      // of dx
 
 static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   if (!d || d->rows < 0 || d->dim <= 0 || d->vocab <= 0 || d->dtype < 0 || d->dtype > 2 || d->reduction < 0 || d->reduction > 2) return NSA_E_ARG;
@@ -83,10 +85,12 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   // a piece's G: up to 256 MB
   p.bwd_rows = (int)std::min(v256, std::max<size_t>(1024, ((size_t)256 << 20) / ((size_t)p.grad_P * p.npad * 2) / 1024 * 1024));
   // gradients: tiles of 256 where the logits have them, else 128; as many slices as give every CU a tile
-  const size_t tile = p.size == WIDE ? 256 : 128, piece = std::min<size_t>(p.bwd_rows, v64);
-  const size_t dx_tiles = up(p.kp, tile) / tile * (up(p.npad, tile) / tile), dw_tiles = up(p.kp, tile) / tile * (up(piece, tile) / tile);
-  p.splits = (int)std::max<size_t>(1, std::min<size_t>({32, 256 / dx_tiles, piece / 512}));
-  p.w_splits = (int)std::max<size_t>(1, std::min<size_t>({32, 256 / dw_tiles, (size_t)p.npad / 256}));
+  const size_t tile = p.size == WIDE ? 256 : 128, piece = std::min<size_t>(p.bwd_rows, v64), last = (v64 - 1) % p.bwd_rows + 1;
+  auto w_slices = [&](size_t entries) {
+    return (int)std::max<size_t>(1, std::min<size_t>({kMaxSlices, 256 / (up(p.kp, tile) / tile * (up(entries, tile) / tile)), (size_t)p.npad / 256}));
+  };
+  p.w_splits = w_slices(piece);
+  p.last_splits = w_slices(last);
   size_t at = up(CELLS * 4, 256);
   auto take = [&](size_t bytes) { const size_t here = at; at = up(at + bytes, 256); return here; };
   p.s_map = take((size_t)p.npad * 4);
@@ -108,8 +112,9 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.b_x = take(p.npad * row * p.grad_P);
   p.b_w = take(p.bwd_rows * row * p.grad_P);
   p.b_grad = take((size_t)p.grad_P * p.npad * p.bwd_rows * 2);
-  p.b_dx = take((size_t)p.splits * p.npad * p.kp * 4);
-  p.b_dw = take(p.w_splits > 1 ? p.w_splits * piece * p.kp * 4 : 0);
+  // (rows of the slices: no more than kSliceTiles tiles of them where there are two or more)
+  p.b_dx = take(std::max<size_t>((size_t)p.npad * p.kp, std::min<size_t>((size_t)kMaxSlices * p.npad * p.kp, kSliceTiles * tile * tile)) * 4);
+  p.b_dw = take(std::max<size_t>(p.w_splits > 1 ? p.w_splits * piece : 0, p.last_splits > 1 ? p.last_splits * last : 0) * p.kp * 4);
   p.bwd = at;
   return 0;
 }
@@ -648,10 +653,22 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const float* loss, const
 
 // ------------------------------------------------------------------------------------ gradients
 
-// g of the rows that count, the bits of their largest finite magnitude, and the other cells cleared
-__global__ __launch_bounds__(1024) void loss_weights_kernel(const float* dloss, int reduction, const unsigned* count, const int* map, float* g, unsigned* cells) {
+// g of the rows that count, the bits of their largest finite magnitude, the other cells cleared, and the slices of a piece's entries that dx is
+// summed from: those whose rounds on 256 CUs end first, where a tile's beginning and end, and its share of the sum of slices, cost as much as 512
+// entries.  The rows that count decide, so they are chosen here.  (8192 rows, 40 % of them ignored, 1024 features, 50021 entries: 80 tiles in 2 slices
+// as for all rows 695 us, in 3 of them 600.)
+__global__ __launch_bounds__(1024) void loss_weights_kernel(const float* dloss, int reduction, const unsigned* count, const int* map, float* g, unsigned* cells,
+                                                            int tiles_m, int tile, int piece) {
   __shared__ unsigned best_s[16];
   const int live = (int)*count, tid = threadIdx.x;
+  if (tid < kMaxSlices) {
+    const int n = tid + 1, tiles = tiles_m * ((live + tile - 1) / tile), rounds = (tiles * n + 255) / 256;
+    long time = n > 1 && (tiles * n > kSliceTiles || piece / n < 512) ? 1L << 50 : (long)rounds * (piece / n + 512);
+    time = time * 64 + n;
+#pragma unroll
+    for (int o = 1; o < kMaxSlices; o <<= 1) time = min(time, (long)__shfl_xor(time, o));
+    if (tid == 0) cells[CELL_SLICES] = (unsigned)(time & 63);
+  }
   unsigned best = 0;
   for (int i = tid; i < live; i += 1024) {
     const float v = reduction == 0 ? dloss[map[i]] : reduction == 1 ? dloss[0] / (float)live : dloss[0];
@@ -676,10 +693,11 @@ struct LossGradArgs {
   int grad_ld, kp, dim, tiles_m, tiles_n, entries;
   const unsigned *count, *other_cell, *g_cell;
   // dx
-  float* sums;                        // [splits][npad][kp]
-  int npad, first;                    // first piece
-  int splits;
+  float* sums;                        // [slices][live rows up to a multiple of 64][kp]
+  int first;                          // first piece
+  const unsigned* slices;
   // dw
+  int splits;
   void* dw;
   long dw_ld;
 };
@@ -688,12 +706,12 @@ struct LossGradArgs {
 template <class Tiles>
 __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dx_kernel(const LossGradArgs G) {
   __shared__ __align__(1024) char shared[Tiles::LDS];
-  const int live = (int)*G.count, tiles_n = (live + Tiles::TN - 1) / Tiles::TN, tiles = G.tiles_m * tiles_n;
-  if ((int)blockIdx.x >= tiles * G.splits) return;
-  const int nth = xcd_run(blockIdx.x, tiles * G.splits), split = nth / tiles;
+  const int live = (int)*G.count, tiles_n = (live + Tiles::TN - 1) / Tiles::TN, tiles = G.tiles_m * tiles_n, splits = (int)*G.slices;
+  if ((int)blockIdx.x >= tiles * splits) return;
+  const int nth = xcd_run(blockIdx.x, tiles * splits), split = nth / tiles;
   const TileAt tile = tile_in(nth % tiles, G.tiles_m, tiles_n, 4);
   const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN;
-  const int all = G.grad_ld / Tiles::BK, per = (all + G.splits - 1) / G.splits, from = min(split * per, all), steps = min(per, all - from);
+  const int all = G.grad_ld / Tiles::BK, per = (all + splits - 1) / splits, from = min(split * per, all), steps = min(per, all - from);
   if (steps <= 0 && !G.first) return;
   Tiles t;
   t.init(shared);
@@ -702,7 +720,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dx_kernel(const LossGr
   t.run(steps, from);
   // (all pieces share the power of two)
   const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.other_cell != nullptr ? plane_shift(*G.other_cell) : 0);
-  float* sums = G.sums + (size_t)split * G.npad * G.kp;
+  float* sums = G.sums + (size_t)split * ((live + 63) / 64 * 64) * G.kp;
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j)
     t.template rows_of<float>(shared, [&](int i, int e) { return __builtin_ldexpf(t.acc[i][j][e], shift); }, [&](int r, int c, floatx4 v) {
@@ -748,14 +766,20 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dw_kernel(const LossGr
     });
 }
 
-// rows of dx or dw [n][dim] from `splits` slices [size][kp]; place: the slices' row of each, -1: zeros
+// rows of dx or dw [n][dim] from `splits` slices [size][kp].  dx: place is the slices' row of each, -1: zeros, and
+// `slices` of them have the rows that count up to a multiple of 64.
 template <class O>
-__global__ __launch_bounds__(256) void loss_rows_of_slices_kernel(const float* sums, int splits, int size, int kp, int n, int dim, const int* place, O* to) {
+__global__ __launch_bounds__(256) void loss_rows_of_slices_kernel(const float* sums, int splits, int size, int kp, int n, int dim, const int* place, const unsigned* count,
+                                                                  const unsigned* slices, O* to) {
   const unsigned per = (dim + 3) / 4, i = blockIdx.x * 256 + threadIdx.x;      // (below 2^31: loss_plan)
   const unsigned row = i / per, c = (i - row * per) * 4;
   if (row >= (unsigned)n) return;
   const int at = place != nullptr ? place[row] : (int)row;
   floatx4 v = {0.f, 0.f, 0.f, 0.f};
+  if (place != nullptr) {
+    splits = (int)*slices;
+    size = ((int)*count + 63) / 64 * 64;
+  }
   if (at >= 0) {
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const floatx4*>(sums + ((size_t)s * size + at) * kp + c);
@@ -831,14 +855,14 @@ static void forward_weight(const nsa_loss_desc* d, const LossPlan& p, const void
 
 template <int P>
 static void dx_tiles(const LossPlan& p, const LossGradArgs& q, hipStream_t st) {
-  const int tile = p.size == WIDE ? 256 : 128;
-  const dim3 grid((unsigned)(q.tiles_m * ((p.n + tile - 1) / tile) * p.splits));
+  const int tile = p.size == WIDE ? 256 : 128, all = q.tiles_m * ((p.n + tile - 1) / tile);
+  const dim3 grid((unsigned)std::max(all, std::min(kMaxSlices * all, kSliceTiles)));
   if (p.size == WIDE) hipLaunchKernelGGL((loss_dx_kernel<typename GradTiles<P>::WideX>), grid, dim3(512), 0, st, q);
   else hipLaunchKernelGGL((loss_dx_kernel<typename GradTiles<P>::MiddleX>), grid, dim3(512), 0, st, q);
 }
 template <int P, class O, bool SLICES>
 static void dw_tiles(const LossPlan& p, const LossGradArgs& q, hipStream_t st) {
-  const dim3 grid((unsigned)(q.tiles_m * q.tiles_n * p.w_splits));
+  const dim3 grid((unsigned)(q.tiles_m * q.tiles_n * q.splits));
   // few rows: nothing to read ahead, so two work-groups a CU that write in turn (25 rows, 1917 features, 21120 entries in bf16: 36 -> 24 us)
   if constexpr (!SLICES)
     if (p.size == FEW) {
@@ -851,11 +875,14 @@ static void dw_tiles(const LossPlan& p, const LossGradArgs& q, hipStream_t st) {
     else hipLaunchKernelGGL((loss_dw_kernel<typename GradTiles<P>::MiddleW, O, SLICES>), grid, dim3(512), 0, st, q);
   }
 }
-static void rows_of_slices(const nsa_loss_desc* d, const float* sums, int splits, int size, int kp, int n, const int* place, void* to, hipStream_t st) {
+static void rows_of_slices(const nsa_loss_desc* d, const LossGradArgs& q, const float* sums, int size, int n, const int* place, void* to, hipStream_t st) {
   const dim3 grid(blocks_for((long)n * ((d->dim + 3) / 4)));
-  if (d->dtype == 0) hipLaunchKernelGGL((loss_rows_of_slices_kernel<B16>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, place, (B16*)to);
-  else if (d->dtype == 1) hipLaunchKernelGGL((loss_rows_of_slices_kernel<H16>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, place, (H16*)to);
-  else hipLaunchKernelGGL((loss_rows_of_slices_kernel<float>), grid, dim3(256), 0, st, sums, splits, size, kp, n, d->dim, place, (float*)to);
+  auto go = [&](auto kernel, auto* out) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, sums, q.splits, size, q.kp, n, d->dim, place, q.count, q.slices, out);
+  };
+  if (d->dtype == 0) go(loss_rows_of_slices_kernel<B16>, (B16*)to);
+  else if (d->dtype == 1) go(loss_rows_of_slices_kernel<H16>, (H16*)to);
+  else go(loss_rows_of_slices_kernel<float>, (float*)to);
 }
 
 }  // namespace nsa
@@ -959,7 +986,9 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
   const int *map = (const int*)(s + p.s_map), *place = (const int*)(s + p.s_place), *label = (const int*)(s + p.s_label);
   const unsigned* count = kept + CELL_ROWS;
   float* g = (float*)(w + p.b_g);
-  hipLaunchKernelGGL(loss_weights_kernel, dim3(1), dim3(1024), 0, st, dloss, (int)d->reduction, count, map, g, cells);
+  const int each = d->dtype == 2 ? 4 : 2, tile = p.size == WIDE ? 256 : 128, tiles_m = (p.kp + tile - 1) / tile;
+  hipLaunchKernelGGL(loss_weights_kernel, dim3(1), dim3(1024), 0, st, dloss, (int)d->reduction, count, map, g, cells, tiles_m, tile,
+                     std::min(p.bwd_rows, (int)up(d->vocab, 64)));
   // All operands in fp16: x once, w with each piece.  Magnitudes: those the forward has found, else here.
   const bool have_x = p.size != FEW, have_w = p.size != FEW && d->dtype == 2;
   const unsigned *xc = d->dtype == 1 ? nullptr : have_x ? kept + CELL_X : cells + CELL_X, *wc = d->dtype == 1 ? nullptr : have_w ? kept + CELL_W : cells + CELL_W;
@@ -976,7 +1005,8 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
   else if (d->dtype == 2) planes<float, H16, 2>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, xc, xg, x_plane, st);
   else if (p.grad_P == 2) planes<H16, H16, 2>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, xg, x_plane, st);
   else planes<H16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, xg, x_plane, st);
-  const int each = d->dtype == 2 ? 4 : 2;
+  LossGradArgs q{};
+  q.kp = p.kp; q.count = count; q.g_cell = cells + CELL_G; q.tiles_m = tiles_m; q.slices = cells + CELL_SLICES;
   for (long v0 = 0; v0 < d->vocab; v0 += p.bwd_rows) {
     LossTileArgs a{};
     a.v0 = (int)v0;
@@ -997,23 +1027,19 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
     if (p.grad_P == 2) launch_tiles<H16, 2, true>(p, a, st);
     else launch_tiles<H16, 1, true>(p, a, st);
 
-    LossGradArgs q{};
-    q.grad = a.grad; q.grad_plane = a.grad_plane; q.grad_ld = ld; q.kp = p.kp; q.dim = d->dim; q.entries = entries;
-    q.count = count; q.g_cell = cells + CELL_G; q.npad = p.npad;
-    const int tile = p.size == WIDE ? 256 : 128;
-    q.tiles_m = (p.kp + tile - 1) / tile;
+    q.grad = a.grad; q.grad_plane = a.grad_plane; q.grad_ld = ld; q.entries = entries;
     if (dx) {
-      q.other = (const H16*)wg; q.other_plane = w_plane; q.other_cell = wc;
-      q.sums = (float*)(w + p.b_dx); q.splits = p.splits; q.first = v0 == 0;
+      q.other = (const H16*)wg; q.other_plane = w_plane; q.other_cell = wc; q.dim = d->dim;
+      q.sums = (float*)(w + p.b_dx); q.first = v0 == 0;
       if (p.grad_P == 2) dx_tiles<2>(p, q, st);
       else dx_tiles<1>(p, q, st);
     }
     if (dw) {
       q.other = (const H16*)xg; q.other_plane = x_plane; q.other_cell = xc;
       q.tiles_n = (entries + tile - 1) / tile;
-      const bool slices = p.w_splits > 1;
+      q.splits = a.vend == d->vocab ? p.last_splits : p.w_splits;
+      const bool slices = q.splits > 1;
       char* to = (char*)dw + v0 * d->dim * each;
-      q.splits = p.w_splits;
       q.dw = slices ? w + p.b_dw : to; q.dw_ld = slices ? p.kp : d->dim; q.dim = slices ? p.kp : d->dim;
       if (slices && p.grad_P == 1) dw_tiles<1, float, true>(p, q, st);
       else if (slices) dw_tiles<2, float, true>(p, q, st);
@@ -1021,9 +1047,9 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
       else if (d->dtype == 2) dw_tiles<2, float, false>(p, q, st);
       else if (p.grad_P == 2) dw_tiles<2, H16, false>(p, q, st);
       else dw_tiles<1, H16, false>(p, q, st);
-      if (slices) rows_of_slices(d, (const float*)(w + p.b_dw), p.w_splits, entries, p.kp, entries, nullptr, to, st);
+      if (slices) rows_of_slices(d, q, (const float*)(w + p.b_dw), entries, entries, nullptr, to, st);
     }
   }
-  if (dx) rows_of_slices(d, (const float*)(w + p.b_dx), p.splits, p.npad, p.kp, p.n, place, dx, st);
+  if (dx) rows_of_slices(d, q, (const float*)(w + p.b_dx), 0, p.n, place, dx, st);
   return (int)hipGetLastError();
 }

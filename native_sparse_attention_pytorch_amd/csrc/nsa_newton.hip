@@ -465,7 +465,7 @@ template <int P> struct NewtonTiles<DEEP, P> {
 };
 
 // The queues of a launch with tiles of kSizes[size], and their length.  Matrices go to the XCDs by eights, back and forth, where that leaves no XCD with
-// more than an eighth above the mean; what is over, and large ones, are spread.  (The byte-level model's 24: A = X X^T 60 -> us.)
+// more than an eighth above the mean; what is over, and large ones, are spread.  (The byte-level model's 24: 1.04 -> 1.00 ms for all five steps.)
 template <class Count, class Steps>
 static int fill(NewtonTable& t, int size, Count count, Steps steps) {
   const SizeCost& c = kSizes[size];

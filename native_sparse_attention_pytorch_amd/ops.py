@@ -2642,7 +2642,9 @@ def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_i
 
 @linear_cross_entropy_fwd.register_fake
 def _(x, weight, labels, ignore_index, reduction):
-    return x.new_empty((x.shape[0],) if reduction == 0 else (), dtype=torch.float32), x.new_empty((1,), dtype=torch.uint8)
+    n = x.shape[0]
+    state = 256 + 24 * 64 * ((n + 63) // 64 if n > 0 else 1)      # (nsa_loss_workspace_bytes)
+    return x.new_empty((n,) if reduction == 0 else (), dtype=torch.float32), x.new_empty((state,), dtype=torch.uint8)
 
 
 @torch.library.custom_op("nsa_amd::linear_cross_entropy_bwd", mutates_args=())
@@ -2680,7 +2682,10 @@ def _loss_backward(ctx, dloss, _):
     if dloss is None:
         return (None,) * 5
     want_dx, want_dw = ctx.needs_input_grad[:2]
-    dx, dw = _direct_bwd(linear_cross_entropy_bwd)(dloss, *ctx.saved_tensors, *ctx.args, want_dx, want_dw)
+    tensors = dloss, *ctx.saved_tensors
+    # (a backward pass that is traced has tensors without memory)
+    launched = all(type(t) in (Tensor, torch.nn.Parameter) for t in tensors)
+    dx, dw = (_direct_bwd(linear_cross_entropy_bwd) if launched else linear_cross_entropy_bwd)(*tensors, *ctx.args, want_dx, want_dw)
     return dx if want_dx else None, dw if want_dw else None, None, None, None
 
 

@@ -405,3 +405,39 @@ def test_captured_forward_and_backward_replay():
         torch.cuda.synchronize()
         for got, w in zip(out, want):
             assert torch.equal(got, w)
+
+
+def test_traced():
+    """The traced call and its gradients are the launched ones."""
+    from native_sparse_attention_pytorch_amd import ops
+    run = torch.compile(lambda x, w, labels: ops.linear_cross_entropy(x, w, labels, reduction="none"), backend="aot_eager", fullgraph=True)
+    for n in (20, 100):
+        x, w, labels, weights = _inputs(n, 64, 300, BF16)
+        want = _check(x, w, labels, "none", weights)
+        x.requires_grad_(), w.requires_grad_()
+        loss = run(x, w, labels)
+        for got, exact in zip((loss, *torch.autograd.grad(loss, (x, w), weights)), want):
+            assert torch.equal(got, exact)
+
+
+def test_few_rows_replay():
+    """A captured forward of up to 32 rows takes other labels, and other numbers of rows that count, at each replay."""
+    from native_sparse_attention_pytorch_amd import ops
+    sets = [_inputs(24, 200, 900, F16, seed=s, ignored=i) for s, i in enumerate((0., 0.5, 1.1, 0.2))]
+    held = [t.clone() for t in sets[0][:3]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.linear_cross_entropy(*held, reduction="none")
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        each, mean = ops.linear_cross_entropy(*held, reduction="none"), ops.linear_cross_entropy(*held)
+    for inputs in sets + sets[:1]:
+        for a, b in zip(held, inputs):
+            a.copy_(b)
+        graph.replay()
+        want = ops.linear_cross_entropy(*inputs[:3], reduction="none"), ops.linear_cross_entropy(*inputs[:3])
+        torch.cuda.synchronize()
+        assert torch.equal(each, want[0]) and torch.equal(mean.nan_to_num(nan=-1.), want[1].nan_to_num(nan=-1.))

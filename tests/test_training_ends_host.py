@@ -56,6 +56,21 @@ def test_loss_entry_checks_its_descriptor():
         assert _sizes(_desc(**bad))[0] == -2, bad
 
 
+@pytest.mark.parametrize("rows", [0, 1, 32, 33, 64, 65, 1000])
+@pytest.mark.parametrize("dtype", [0, 2])
+def test_traced_shapes_are_the_real_ones(rows, dtype):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x, w = (torch.empty(n, 64, dtype=(torch.bfloat16, None, torch.float32)[dtype]) for n in (rows, 300))
+        labels = torch.empty(rows, dtype=torch.int64)
+        for reduction in (0, 1):
+            loss, state = ops.linear_cross_entropy_fwd(x, w, labels, -100, reduction)
+            assert loss.shape == ((rows,) if reduction == 0 else ()) and state.numel() == _sizes(_desc(rows=rows, dtype=dtype))[1][0]
+        for wanted in ((True, True), (True, False), (False, True)):
+            dx, dw = ops.linear_cross_entropy_bwd(loss, x, w, state, -100, 1, *wanted)
+            assert dx.shape == (rows if wanted[0] else 0, 64) and dw.shape == (300 if wanted[1] else 0, 64) and dw.dtype == w.dtype
+
+
 def test_loss_workspaces_hold_pieces_not_logits():
     for rows, dim, vocab, dtype in ((16384, 4096, 131072, 0), (16384, 4096, 131072, 2), (1 << 20, 512, 50021, 0), (8, 512, 256, 1)):
         rc, (state, fwd, bwd) = _sizes(_desc(rows=rows, dim=dim, vocab=vocab, dtype=dtype, x_stride=dim, w_stride=dim))
