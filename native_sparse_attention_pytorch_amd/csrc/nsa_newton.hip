@@ -9,7 +9,8 @@
 // these, less than with fp32 products (1.6e-6 at 512 x 512).  a stands on the diagonal of B and not beside the product: one pass over X less, and
 // a rounding of what is left of a + b A + c A A, not of its parts.  A bf16 result is itself rounded to 2^-9, so its last two steps, after which little grows,
 // take the first halves alone, at a third of the matrix instructions: that adds at most a tenth to the result's error (1.66e-3 of its norm
-// from rounding, 1.83e-3 with two such steps, 2.0e-3 with three, 2.1e-3 with all five).  Scales: X 2^(12 + s), A 2^(10 + 2 s), B 2^10.  s is 0 unless |G| is small beside eps:
+// from rounding, 1.83e-3 with two such steps, 2.0e-3 with three, 2.1e-3 with all five).  And a matrix of 16 bits begins as itself times a power of
+// two, one half and exact; what it is short of G / (|G| + eps) is a factor of the first A and B X.  Scales: X 2^(12 + s), A 2^(10 + 2 s), B 2^10.  s is 0 unless |G| is small beside eps:
 // then X starts so small that fp16 would lose it, and s is what brings its norm to 1; it falls by the bits of a with each step, so nothing grows out
 // of range.  The entry checks that singular values up to 1 stay below 4 for the given coefficients.
 //
@@ -40,6 +41,7 @@ struct NewtonTable {
   char* ws;
   double* partial;                 // [many][kNormChunks]
   int* shift;                      // s of each
+  float* factor;                   // what the first X is short of
 };
 
 __host__ __device__ inline long up64(long v) { return (v + 63) / 64 * 64; }
@@ -122,7 +124,7 @@ __global__ __launch_bounds__(256) void newton_norm_kernel(const NewtonTable G) {
 constexpr int kBeginTiles = 2;
 __host__ __device__ inline int begin_parts(const NewtonPlanes& p, int size) { return (update_tiles(p, size) + kBeginTiles - 1) / kBeginTiles; }
 template <class S>
-__global__ __launch_bounds__(256) void newton_begin_kernel(const NewtonTable G, float eps) {
+__global__ __launch_bounds__(256) void newton_begin_kernel(const NewtonTable G, float eps, int exact) {
   __shared__ float tile_s[64][65];
   __shared__ double sums[4], scale_s;
   const NewtonPlace place = place_of(G, [](const NewtonPlanes& p) { return begin_parts(p, 64); });
@@ -140,8 +142,17 @@ __global__ __launch_bounds__(256) void newton_begin_kernel(const NewtonTable G, 
     const double norm = sqrt(sums[0] + sums[1] + sums[2] + sums[3]), part = norm / (norm + eps);
     // (a norm of zero, and one that is no number: s = 0)
     const int s = part > 0.0 && part < 1.0 ? min(100, -(ilogb(part) + 1)) : 0;
-    scale_s = ldexp(1.0 / (norm + eps), 12 + s);
-    if (place.nth == 0) G.shift[k] = s;
+    double scale = ldexp(1.0 / (norm + eps), 12 + s), factor = 1.0;
+    if (exact && scale > 0.0 && scale < INFINITY) {
+      int bits;
+      factor = 2.0 * frexp(scale, &bits);
+      scale = ldexp(1.0, bits - 1);
+    }
+    scale_s = scale;
+    if (place.nth == 0) {
+      G.shift[k] = s;
+      G.factor[k] = (float)factor;
+    }
   }
   const S* in = (const S*)M.in;
   const int wide = L.np / 64, r = tid >> 2, c = (tid & 3) * 16;
@@ -171,13 +182,14 @@ __global__ __launch_bounds__(256) void newton_begin_kernel(const NewtonTable G, 
         lo[e] = h.lo;
       }
       *reinterpret_cast<f16x8*>(x + 8 * u) = hi;
-      *reinterpret_cast<f16x8*>(x + 8 * u + L.x_plane()) = lo;
+      if (!exact) *reinterpret_cast<f16x8*>(x + 8 * u + L.x_plane()) = lo;
     }
   }
 }
 
 struct NewtonStep {
-  int step, last, growth, from, both;      // growth: bits that a step takes off s; from: the buffer of X that is read; both: halves of X are wanted
+  int step, growth, from;      // growth: bits that a step takes off s; from: the buffer of X that is read
+  int both_x, both_a;          // second halves are wanted of the next X, of A and B
   float a, b, c;
 };
 __device__ __forceinline__ int shift_at(const NewtonTable& G, const NewtonStep& S, int k, int step) { return max(0, G.shift[k] - S.growth * step); }
@@ -228,7 +240,8 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_square_kernel(const 
     t.run(L.np / Tiles::BK);
   }
   const int s = POLY ? shift_at(G, S, k, S.step) : 0;
-  const float unit = POLY ? __builtin_ldexpf(S.c, -10 - 4 * s) : 0x1p-14f, linear = __builtin_ldexpf(S.b, -2 * s), diagonal = S.a * 0x1p10f;
+  const float factor = !POLY && S.step == 0 ? G.factor[k] : 1.f;
+  const float unit = POLY ? __builtin_ldexpf(S.c, -10 - 4 * s) : 0x1p-14f * factor * factor, linear = __builtin_ldexpf(S.b, -2 * s), diagonal = S.a * 0x1p10f;
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j) {
     const int col0 = n0 + t.col_of(j) - (t.lane & 31), row0 = m0 + t.wm * Tiles::W;
@@ -244,11 +257,11 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_square_kernel(const 
         if (POLY) v[e] = __builtin_fmaf(linear, old[e], v[e]) + (row + e == col ? diagonal : 0.f);
         if (row + e >= L.m || col >= L.m) v[e] = 0.f;
       }
-      if (ok) store_halves(out + at, L.a_plane(), v, Tiles::P == 2);
+      if (ok) store_halves(out + at, L.a_plane(), v, S.both_a);
     });
     if (tile.m != tile.n)      // the other side of the diagonal
       t.turned_of(shared, [&](int r, int c, floatx4 v) {
-        if (row0 + c < L.m && col0 + r < L.mp) store_halves(out + (long)(row0 + c) * L.mp + col0 + r, L.a_plane(), v, Tiles::P == 2);
+        if (row0 + c < L.m && col0 + r < L.mp) store_halves(out + (long)(row0 + c) * L.mp + col0 + r, L.a_plane(), v, S.both_a);
       });
   }
 }
@@ -275,7 +288,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_update_kernel(const 
   t.operand_b(B, L.a_plane(), L.mp, n0, L.m);
   t.run(L.mp / Tiles::BK);
   const int s = shift_at(G, S, k, S.step), s2 = shift_at(G, S, k, S.step + 1);
-  const float unit = __builtin_ldexpf(1.f, -10 + (LAST ? -12 - s : s2 - s));
+  const float unit = __builtin_ldexpf(S.step == 0 ? G.factor[k] : 1.f, -10 + (LAST ? -12 - s : s2 - s));
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j) {
     if (LAST && L.turned) {
@@ -300,7 +313,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_update_kernel(const 
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = row < L.m ? v[e] * unit : 0.f;      // (rows past the last one are zeros)
       if (!LAST) {
-        store_halves(next + (long)row * L.np + col, L.x_plane(), v, S.both);
+        store_halves(next + (long)row * L.np + col, L.x_plane(), v, S.both_x);
         return;
       }
       O* p = (O*)M.out + (long)row * M.cols + col;
@@ -452,16 +465,16 @@ struct SizeCost { int tile, places; double each, beside; };
 static constexpr SizeCost kSizes[SIZES] = {{256, 256, 0.0785, 7.0}, {128, 256, 0.0238, 3.5}, {64, 512, 0.021, 2.7}, {64, 256, 0.0089, 3.4}};
 template <int SIZE, int P> struct NewtonTiles;
 template <int P> struct NewtonTiles<WIDE, P> {
-  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 256, 256, 2, 4, 32, P == 2 ? 2 : 4>;
+  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 256, 256, 2, 4, 32, P == 2 ? 2 : P == 1 ? 4 : 3>;
 };
 template <int P> struct NewtonTiles<MIDDLE, P> {
-  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 128, 128, 4, 2, P == 2 ? 32 : 64, 4>;
+  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 128, 128, 4, 2, P == 1 ? 64 : 32, 4>;
 };
 template <int P> struct NewtonTiles<SMALL, P> {
-  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 64, 64, 2, 2, 64, P == 2 ? 2 : 4>;
+  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 64, 64, 2, 2, 64, P == 1 ? 4 : 2>;
 };
 template <int P> struct NewtonTiles<DEEP, P> {
-  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 64, 64, 2, 2, 64, P == 2 ? 4 : 8>;
+  template <int FORM_A> using Of = TileProduct<H16, P, FORM_A, ROWS, 64, 64, 2, 2, 64, P == 1 ? 8 : 4>;
 };
 
 // The queues of a launch with tiles of kSizes[size], and their length.  Matrices go to the XCDs by eights, back and forth, where that leaves no XCD with
@@ -553,28 +566,29 @@ template <class S>
 static void newton(NewtonTable& t, NewtonStep s, int steps, float eps, hipStream_t st) {
   hipLaunchKernelGGL((newton_norm_kernel<S>), dim3((unsigned)t.chunks, (unsigned)t.many), dim3(256), 0, st, t);
   const int begin = fill(t, SMALL, begin_parts, short_side);
-  hipLaunchKernelGGL((newton_begin_kernel<S>), dim3(8u * begin), dim3(256), 0, st, t, eps);
+  // (steps >= 3: the first is none of the last two)
+  const int exact = sizeof(S) == 2 && steps >= 3;
+  hipLaunchKernelGGL((newton_begin_kernel<S>), dim3(8u * begin), dim3(256), 0, st, t, eps, exact);
   constexpr int LAST_P = std::is_same<S, __bf16>::value ? 1 : 2;      // planes of the last two steps
   const int gram = tile_size(t, square_tiles, long_side), poly = tile_size(t, square_tiles, short_side), un = tile_size(t, update_tiles, short_side);
   for (s.step = 0; s.step < steps; ++s.step) {
+    const bool last = s.step == steps - 1;
     s.from = s.step & 1;
-    s.last = s.step == steps - 1;
-    s.both = LAST_P == 2 || s.step + 3 < steps;
-    if (LAST_P == 2 || s.step + 2 < steps) {
-      square_any<2, false>(gram, t, s, st);
-      square_any<2, true>(poly, t, s, st);
-    } else {
-      square_any<LAST_P, false>(gram, t, s, st);
-      square_any<LAST_P, true>(poly, t, s, st);
-    }
-    if (s.last) update_any<LAST_P, true, S>(un, t, s, st);
-    else if (LAST_P == 2 || s.step + 2 < steps) update_any<2, false, H16>(un, t, s, st);
-    else update_any<LAST_P, false, H16>(un, t, s, st);
+    s.both_a = LAST_P == 2 || s.step + 2 < steps;
+    s.both_x = LAST_P == 2 || s.step + 3 < steps;
+    if (s.both_a && !(s.step == 0 && exact)) square_any<2, false>(gram, t, s, st);
+    else square_any<1, false>(gram, t, s, st);
+    if (s.both_a) square_any<2, true>(poly, t, s, st);
+    else square_any<1, true>(poly, t, s, st);
+    if (last) update_any<LAST_P, true, S>(un, t, s, st);
+    else if (!s.both_a) update_any<1, false, H16>(un, t, s, st);
+    else if (s.step == 0 && exact) update_any<ONE_BY_TWO, false, H16>(un, t, s, st);
+    else update_any<2, false, H16>(un, t, s, st);
   }
 }
 
-// bytes before the planes: sums of squares and shifts
-static size_t newton_head() { return (size_t)kNewtonMany * kNormChunks * 8 + 256; }
+// bytes before the planes: sums of squares, shifts and factors
+static size_t newton_head() { return (size_t)kNewtonMany * kNormChunks * 8 + 512; }
 
 }  // namespace nsa
 
@@ -629,6 +643,7 @@ extern "C" int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_
       NewtonTable t{};
       t.partial = (double*)ws;
       t.shift = (int*)((char*)ws + (size_t)kNewtonMany * kNormChunks * 8);
+      t.factor = (float*)(t.shift + 64);
       t.ws = (char*)ws + newton_head();
       size_t at = 0;
       long largest = 0;

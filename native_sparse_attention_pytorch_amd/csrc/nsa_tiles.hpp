@@ -104,16 +104,18 @@ struct TileOperand {
   }
 };
 
+// P: planes of both operands, 1 or 2 (three products then), or ONE_BY_TWO: one of a, two of b, and two products
+enum { ONE_BY_TWO = 3 };
 template <class T_, int P_, int FORM_A, int FORM_B, int TM_, int TN_, int WM_, int WN_, int BK_, int STAGES_>
 struct TileProduct {
   typedef T_ T;
   typedef typename PlaneVec<T>::x8 x8;
-  static constexpr int P = P_, TM = TM_, TN = TN_, WM = WM_, WN = WN_, BK = BK_, STAGES = STAGES_, WAVES = WM * WN, THREADS = 64 * WAVES;
-  static constexpr int MI = TM / WM / 32, NI = TN / WN / 32, KS = BK / 16, PRODUCTS = P == 1 ? 1 : 3;
+  static constexpr int P = P_, PA = P == 2 ? 2 : 1, PB = P == 1 ? 1 : 2, TM = TM_, TN = TN_, WM = WM_, WN = WN_, BK = BK_, STAGES = STAGES_, WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int MI = TM / WM / 32, NI = TN / WN / 32, KS = BK / 16, PRODUCTS = PA + PB - 1;
   typedef TileOperand<T, FORM_A, TM, BK, WAVES> OpA;
   typedef TileOperand<T, FORM_B, TN, BK, WAVES> OpB;
-  static constexpr unsigned A_BYTES = P * OpA::PLANE, STAGE = A_BYTES + P * OpB::PLANE, LDS = STAGES * STAGE;
-  static constexpr int LOADS = P * (OpA::ROUNDS + OpB::ROUNDS), MFMAS = KS * PRODUCTS * MI * NI;
+  static constexpr unsigned A_BYTES = PA * OpA::PLANE, STAGE = A_BYTES + PB * OpB::PLANE, LDS = STAGES * STAGE;
+  static constexpr int LOADS = PA * OpA::ROUNDS + PB * OpB::ROUNDS, MFMAS = KS * PRODUCTS * MI * NI;
   static_assert((MI == 1 || MI % 2 == 0) && (NI == 1 || NI % 2 == 0) && STAGES >= 2 && (STAGES == 2 || (STAGES - 2) * LOADS < 64), "");
 
   OpA A;
@@ -138,8 +140,8 @@ struct TileProduct {
   __device__ __forceinline__ int col_of(int j) const { return wn * (TN / WN) + 32 * j + (lane & 31); }
 
   __device__ __forceinline__ void copy(int i, const T* a, const T* b, unsigned to, unsigned lanes) const {
-    if (i < P * OpA::ROUNDS) A.copy(a, i / OpA::ROUNDS, i % OpA::ROUNDS, to, lanes);
-    else B.copy(b, (i - P * OpA::ROUNDS) / OpB::ROUNDS, (i - P * OpA::ROUNDS) % OpB::ROUNDS, to + A_BYTES, lanes);
+    if (i < PA * OpA::ROUNDS) A.copy(a, i / OpA::ROUNDS, i % OpA::ROUNDS, to, lanes);
+    else B.copy(b, (i - PA * OpA::ROUNDS) / OpB::ROUNDS, (i - PA * OpA::ROUNDS) % OpB::ROUNDS, to + A_BYTES, lanes);
   }
   template <int OUTSTANDING>
   __device__ __forceinline__ static void meet() {
@@ -202,7 +204,7 @@ struct TileProduct {
   // two planes: the small products are summed by themselves, where there are registers for it, so that a leading sum is rounded once a
   // product of 16 and not three times; and where there are more, every 256 of the contraction index are a sum of their own (sums of 2048 and
   // 4096 are then off by 1.2e-7 and 1.6e-7 of their size instead of 3e-7 and 4e-7)
-  static constexpr bool APART = P == 2 && MI * NI <= 4, PIECES = P == 2 && MI * NI <= 2;
+  static constexpr bool APART = PB == 2 && MI * NI <= 4, PIECES = PB == 2 && MI * NI <= 2;
 
   // `steps` times BK of the contraction index from k0 * BK on.  All waves of the work-group; LDS is free again behind it.
   // From stage `tail` on, operand a is read `back` elements before its place: rows that end `back` short of a whole number of stages (the other
@@ -231,14 +233,14 @@ struct TileProduct {
       b += B.step;
       if (s + 1 == tail) a -= back;
     }
-    x8 fa[2][P][MI], fb[2][P][NI];
+    x8 fa[2][PA][MI], fb[2][PB][NI];
     // the operand with fewer parts first, and with all of it each part of the other: products begin as soon as their operands arrive
     constexpr bool A_FIRST = MI <= NI;
     auto read = [&](unsigned stage, int ks, int into) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
+        for (int p = 0; p < (A_FIRST == (u == 0) ? PA : PB); ++p) {
           if (A_FIRST == (u == 0)) {
 #pragma unroll
             for (int i = 0; i < MI; ++i) fa[into][p][i] = A.read(stage + p * OpA::PLANE, i, ks);
@@ -271,7 +273,7 @@ struct TileProduct {
           for (int v = 0; v < MI * NI; ++v) {
             const int i = A_FIRST ? v % MI : v / NI, j = A_FIRST ? v / MI : v % NI, n = (ks * PRODUCTS + q) * MI * NI + v;
             floatx16& sum = APART && q > 0 ? small[APART ? i : 0][APART ? j : 0] : acc[i][j];
-            sum = mma(fa[ks & 1][q == 2 ? P - 1 : 0][i], fb[ks & 1][q == 1 ? P - 1 : 0][j], sum);
+            sum = mma(fa[ks & 1][q == 2 ? PA - 1 : 0][i], fb[ks & 1][q == 1 ? PB - 1 : 0][j], sum);
 #pragma unroll
             for (int c = n * LOADS / MFMAS; c < (n + 1) * LOADS / MFMAS; ++c) copy(c, a, b, to, lanes);
           }

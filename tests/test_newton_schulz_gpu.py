@@ -223,3 +223,41 @@ def test_bf16_results_are_off_by_their_rounding(m, n):
         want = _exact(g)
         off = lambda x: float((x.double() - want).norm())
         assert off(ops.newton_schulz(g)) <= 1.25 ** 0.5 * off(want.to(BF16)), seed
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("m,n", [(70, 130), (300, 200)])
+@pytest.mark.parametrize("eps", [1e-7, 1., 30., 1e3])
+def test_16_bit_matrices_begin_exactly(m, n, dtype, eps):
+    """They are held as they are, times a power of two, whatever the norm: fp16 results are fp32's and a rounding (2^-14: a few units of 2^-22 a
+    step, as for fp32); bf16's last two steps add at most half of the rounding."""
+    from native_sparse_attention_pytorch_amd import ops
+    for scale in (1., 3.7, 2 ** -9):
+        g = _g(m, n, dtype=dtype, scale=scale)
+        got, want = ops.newton_schulz(g, eps=eps), _exact(g, eps=eps)
+        off = lambda x: float((x.double() - want).norm())
+        assert off(got) <= (1.25 ** 0.5 if dtype == BF16 else 1.) * off(want.to(dtype)) + 2 ** -14 * float(want.norm()), scale
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("steps", [1, 2, 3, 4])
+def test_few_steps_of_16_bits(dtype, steps):
+    """One and two steps of a bf16 result are made of fp16 values from the beginning: 8 roundings of 2^-12 a step, each growing at most 4 times in a
+    step that follows or makes it."""
+    from native_sparse_attention_pytorch_amd import ops
+    for m, n in ((130, 70), (90, 3000)):
+        g = _g(m, n, dtype=dtype)
+        got, want = ops.newton_schulz(g, steps=steps), _exact(g, steps=steps)
+        off = float((got.double() - want).norm())
+        tol = 8 * 2 ** -12 * (4, 20)[steps - 1] if dtype == BF16 and steps < 3 else 2 ** -8
+        assert off <= tol + torch.finfo(dtype).eps / 2 * float(want.norm())
+
+
+def test_a_parameter_without_elements_is_left_alone():
+    from native_sparse_attention_pytorch_amd.training import Muon
+    params = [torch.nn.Parameter(torch.zeros(5, 0, device=DEV)), torch.nn.Parameter(_g(6, 4))]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    before = params[1].detach().clone()
+    Muon(params).step()
+    assert not torch.equal(params[1], before) and params[0].shape == (5, 0)
