@@ -688,38 +688,38 @@ __global__ __launch_bounds__(1024) void loss_weights_kernel(const float* dloss, 
 }
 
 struct LossGradArgs {
-  const _Float16 *grad, *other;       // G [npad][grad_ld]; w [piece][kp] or x [npad][kp]
-  long grad_plane, other_plane;
-  int grad_ld, kp, dim, tiles_m, tiles_n, entries;
-  const unsigned *count, *other_cell, *g_cell;
+  const _Float16 *grad, *w, *x;       // G [npad][grad_ld]; w [piece][kp]; x [npad][kp]
+  long grad_plane, w_plane, x_plane;
+  int grad_ld, kp, tiles_m, entries;
+  const unsigned *count, *w_cell, *x_cell, *g_cell;
   // dx
   float* sums;                        // [slices][live rows up to a multiple of 64][kp]
   int first;                          // first piece
   const unsigned* slices;
-  // dw
-  int splits;
+  // dw: the first dw_tiles work-groups
+  int dw_tiles, tiles_n, splits, dim;
   void* dw;
   long dw_ld;
 };
 
 // dx, one slice of the piece's vocabulary: features (registers) by tokens (lanes), unscaled, added to what the pieces before gave
 template <class Tiles>
-__global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dx_kernel(const LossGradArgs G) {
-  __shared__ __align__(1024) char shared[Tiles::LDS];
+__device__ __forceinline__ void loss_dx(const LossGradArgs& G, char* shared) {
   const int live = (int)*G.count, tiles_n = (live + Tiles::TN - 1) / Tiles::TN, tiles = G.tiles_m * tiles_n, splits = (int)*G.slices;
-  if ((int)blockIdx.x >= tiles * splits) return;
-  const int nth = xcd_run(blockIdx.x, tiles * splits), split = nth / tiles;
+  const int id = (int)blockIdx.x - G.dw_tiles;
+  if (id >= tiles * splits) return;
+  const int nth = xcd_run(id, tiles * splits), split = nth / tiles;
   const TileAt tile = tile_in(nth % tiles, G.tiles_m, tiles_n, 4);
   const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN;
   const int all = G.grad_ld / Tiles::BK, per = (all + splits - 1) / splits, from = min(split * per, all), steps = min(per, all - from);
   if (steps <= 0 && !G.first) return;
   Tiles t;
   t.init(shared);
-  t.operand_a(G.other, G.other_plane, G.kp, m0, G.kp);
+  t.operand_a(G.w, G.w_plane, G.kp, m0, G.kp);
   t.operand_b(G.grad, G.grad_plane, G.grad_ld, n0, live);
   t.run(steps, from);
   // (all pieces share the power of two)
-  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.other_cell != nullptr ? plane_shift(*G.other_cell) : 0);
+  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.w_cell != nullptr ? plane_shift(*G.w_cell) : 0);
   float* sums = G.sums + (size_t)split * ((live + 63) / 64 * 64) * G.kp;
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j)
@@ -733,14 +733,13 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dx_kernel(const LossGr
 
 // dw of the piece: features (registers) by entries of the vocabulary (lanes), over all rows or (SLICES, unscaled fp32 [splits][entries][kp]) a slice of them
 template <class Tiles, class O, bool SLICES>
-__global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dw_kernel(const LossGradArgs G) {
-  __shared__ __align__(1024) char shared[Tiles::LDS];
-  const int tiles = G.tiles_m * G.tiles_n, nth = xcd_run(blockIdx.x, gridDim.x), split = SLICES ? nth / tiles : 0;
+__device__ __forceinline__ void loss_dw(const LossGradArgs& G, char* shared) {
+  const int tiles = G.tiles_m * G.tiles_n, nth = xcd_run(blockIdx.x, G.dw_tiles), split = SLICES ? nth / tiles : 0;
   const TileAt tile = tile_in(SLICES ? nth % tiles : nth, G.tiles_m, G.tiles_n, 4);
   const int m0 = tile.m * Tiles::TM, n0 = tile.n * Tiles::TN, live = (int)*G.count, steps = (live + Tiles::BK - 1) / Tiles::BK;
   Tiles t;
   t.init(shared);
-  t.operand_a(G.other, G.other_plane, G.kp, m0, G.kp);
+  t.operand_a(G.x, G.x_plane, G.kp, m0, G.kp);
   t.operand_b(G.grad, G.grad_plane, G.grad_ld, n0, G.grad_ld);
   if (SLICES) {
     const int per = (steps + G.splits - 1) / G.splits, from = min(steps, split * per);
@@ -748,7 +747,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dw_kernel(const LossGr
   } else {
     t.run(steps);
   }
-  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.other_cell != nullptr ? plane_shift(*G.other_cell) : 0);
+  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.x_cell != nullptr ? plane_shift(*G.x_cell) : 0);
   O* dw = (O*)G.dw + (SLICES ? (size_t)split * G.entries * G.dw_ld : 0);
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j)
@@ -764,6 +763,15 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_dw_kernel(const LossGr
           if (col + e < G.dim) at[e] = v[e];
       }
     });
+}
+
+// Both products of a piece's G in one launch: neither waits for the other's last tiles.
+template <class TilesX, class TilesW, class O, bool SLICES>
+__global__ __launch_bounds__(TilesX::THREADS, 2) void loss_products_kernel(const LossGradArgs G) {
+  static_assert(TilesX::THREADS == TilesW::THREADS, "");
+  __shared__ __align__(1024) char shared[TilesX::LDS > TilesW::LDS ? TilesX::LDS : TilesW::LDS];
+  if ((int)blockIdx.x < G.dw_tiles) loss_dw<TilesW, O, SLICES>(G, shared);
+  else loss_dx<TilesX>(G, shared);
 }
 
 // rows of dx or dw [n][dim] from `splits` slices [size][kp].  dx: place is the slices' row of each, -1: zeros, and
@@ -813,6 +821,7 @@ template <int P> struct GradTiles {
   typedef TileProduct<H16, P, COLUMNS, ROWS, 128, 128, 2, 4, P == 2 ? 32 : 64, 4> MiddleX;
   typedef TileProduct<H16, P, COLUMNS, COLUMNS, 256, 256, 2, 4, 32, P == 2 ? 2 : 4> WideW;
   typedef TileProduct<H16, P, COLUMNS, COLUMNS, 128, 128, 2, 4, P == 2 ? 32 : 64, 4> MiddleW;
+  typedef TileProduct<H16, P, COLUMNS, ROWS, 128, 128, 2, 4, P == 2 ? 32 : 64, 2> FewX;
   typedef TileProduct<H16, P, COLUMNS, COLUMNS, 128, 128, 2, 4, P == 2 ? 32 : 64, 2> FewW;
 };
 
@@ -853,26 +862,21 @@ static void forward_weight(const nsa_loss_desc* d, const LossPlan& p, const void
   else planes<float, H16, 2>((const float*)weight + (long)v0 * d->w_stride, d->w_stride, rows, rows, d->dim, p.kp, nullptr, nullptr, cell, dst, plane, st);
 }
 
-template <int P>
-static void dx_tiles(const LossPlan& p, const LossGradArgs& q, hipStream_t st) {
-  const int tile = p.size == WIDE ? 256 : 128, all = q.tiles_m * ((p.n + tile - 1) / tile);
-  const dim3 grid((unsigned)std::max(all, std::min(kMaxSlices * all, kSliceTiles)));
-  if (p.size == WIDE) hipLaunchKernelGGL((loss_dx_kernel<typename GradTiles<P>::WideX>), grid, dim3(512), 0, st, q);
-  else hipLaunchKernelGGL((loss_dx_kernel<typename GradTiles<P>::MiddleX>), grid, dim3(512), 0, st, q);
-}
 template <int P, class O, bool SLICES>
-static void dw_tiles(const LossPlan& p, const LossGradArgs& q, hipStream_t st) {
-  const dim3 grid((unsigned)(q.tiles_m * q.tiles_n * q.splits));
+static void products(const LossPlan& p, const LossGradArgs& q, bool dx, hipStream_t st) {
+  typedef GradTiles<P> T;
+  const int tile = p.size == WIDE ? 256 : 128, all = q.tiles_m * ((p.n + tile - 1) / tile);
+  const dim3 grid((unsigned)(q.dw_tiles + (dx ? std::max(all, std::min(kMaxSlices * all, kSliceTiles)) : 0))), block(512);
   // few rows: nothing to read ahead, so two work-groups a CU that write in turn (25 rows, 1917 features, 21120 entries in bf16: 36 -> 24 us)
-  if constexpr (!SLICES)
+  if constexpr (!SLICES && !(P == 1 && std::is_same<O, H16>::value))      // (few rows of fp16 have two planes)
     if (p.size == FEW) {
-      hipLaunchKernelGGL((loss_dw_kernel<typename GradTiles<P>::FewW, O, SLICES>), grid, dim3(512), 0, st, q);
+      hipLaunchKernelGGL((loss_products_kernel<typename T::FewX, typename T::FewW, O, SLICES>), grid, block, 0, st, q);
       return;
     }
   // (fp16 operands of two planes: few rows only)
   if constexpr (P == 1 || sizeof(O) == 4) {
-    if (p.size == WIDE) hipLaunchKernelGGL((loss_dw_kernel<typename GradTiles<P>::WideW, O, SLICES>), grid, dim3(512), 0, st, q);
-    else hipLaunchKernelGGL((loss_dw_kernel<typename GradTiles<P>::MiddleW, O, SLICES>), grid, dim3(512), 0, st, q);
+    if (p.size == WIDE) hipLaunchKernelGGL((loss_products_kernel<typename T::WideX, typename T::WideW, O, SLICES>), grid, block, 0, st, q);
+    else hipLaunchKernelGGL((loss_products_kernel<typename T::MiddleX, typename T::MiddleW, O, SLICES>), grid, block, 0, st, q);
   }
 }
 static void rows_of_slices(const nsa_loss_desc* d, const LossGradArgs& q, const float* sums, int size, int n, const int* place, void* to, hipStream_t st) {
@@ -1007,6 +1011,7 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
   else planes<H16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, xg, x_plane, st);
   LossGradArgs q{};
   q.kp = p.kp; q.count = count; q.g_cell = cells + CELL_G; q.tiles_m = tiles_m; q.slices = cells + CELL_SLICES;
+  q.x = (const H16*)xg; q.x_plane = x_plane; q.x_cell = xc; q.w = (const H16*)(w + p.b_w); q.w_cell = wc; q.sums = (float*)(w + p.b_dx);
   for (long v0 = 0; v0 < d->vocab; v0 += p.bwd_rows) {
     LossTileArgs a{};
     a.v0 = (int)v0;
@@ -1027,28 +1032,20 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
     if (p.grad_P == 2) launch_tiles<H16, 2, true>(p, a, st);
     else launch_tiles<H16, 1, true>(p, a, st);
 
-    q.grad = a.grad; q.grad_plane = a.grad_plane; q.grad_ld = ld; q.entries = entries;
-    if (dx) {
-      q.other = (const H16*)wg; q.other_plane = w_plane; q.other_cell = wc; q.dim = d->dim;
-      q.sums = (float*)(w + p.b_dx); q.first = v0 == 0;
-      if (p.grad_P == 2) dx_tiles<2>(p, q, st);
-      else dx_tiles<1>(p, q, st);
-    }
-    if (dw) {
-      q.other = (const H16*)xg; q.other_plane = x_plane; q.other_cell = xc;
-      q.tiles_n = (entries + tile - 1) / tile;
-      q.splits = a.vend == d->vocab ? p.last_splits : p.w_splits;
-      const bool slices = q.splits > 1;
-      char* to = (char*)dw + v0 * d->dim * each;
-      q.dw = slices ? w + p.b_dw : to; q.dw_ld = slices ? p.kp : d->dim; q.dim = slices ? p.kp : d->dim;
-      if (slices && p.grad_P == 1) dw_tiles<1, float, true>(p, q, st);
-      else if (slices) dw_tiles<2, float, true>(p, q, st);
-      else if (d->dtype == 0) dw_tiles<1, B16, false>(p, q, st);
-      else if (d->dtype == 2) dw_tiles<2, float, false>(p, q, st);
-      else if (p.grad_P == 2) dw_tiles<2, H16, false>(p, q, st);
-      else dw_tiles<1, H16, false>(p, q, st);
-      if (slices) rows_of_slices(d, q, (const float*)(w + p.b_dw), entries, entries, nullptr, to, st);
-    }
+    q.grad = a.grad; q.grad_plane = a.grad_plane; q.grad_ld = ld; q.w_plane = w_plane; q.entries = entries; q.first = v0 == 0;
+    q.tiles_n = (entries + tile - 1) / tile;
+    q.splits = !dw ? 1 : a.vend == d->vocab ? p.last_splits : p.w_splits;
+    q.dw_tiles = dw ? tiles_m * q.tiles_n * q.splits : 0;
+    const bool slices = q.splits > 1;
+    char* to = (char*)dw + v0 * d->dim * each;
+    q.dw = slices ? w + p.b_dw : to; q.dw_ld = q.dim = slices ? p.kp : d->dim;
+    if (slices && p.grad_P == 1) products<1, float, true>(p, q, dx, st);
+    else if (slices) products<2, float, true>(p, q, dx, st);
+    else if (d->dtype == 0) products<1, B16, false>(p, q, dx, st);
+    else if (d->dtype == 2) products<2, float, false>(p, q, dx, st);
+    else if (p.grad_P == 2) products<2, H16, false>(p, q, dx, st);
+    else products<1, H16, false>(p, q, dx, st);
+    if (slices) rows_of_slices(d, q, (const float*)(w + p.b_dw), entries, entries, nullptr, to, st);
   }
   if (dx) rows_of_slices(d, q, (const float*)(w + p.b_dx), 0, p.n, place, dx, st);
   return (int)hipGetLastError();

@@ -2616,12 +2616,19 @@ def _unit_rows(t: Tensor) -> Tensor:
     return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
+@functools.lru_cache(maxsize=256)
+def _loss_sizes(*desc, aligned: bool):
+    """(descriptor, bytes of state, of the forward's workspace, of the backward's); the host's part of a small call is most of its time, so what
+    depends on sizes only is looked up."""
+    d, sizes = _lib.LossDesc(*desc), [C.c_size_t() for _ in range(3)]
+    _lib.check(_lib.lib().nsa_loss_workspace_bytes(C.byref(d), 0 if aligned else 8, *map(C.byref, sizes)), "nsa_loss_workspace_bytes")
+    return C.byref(d), *(s.value for s in sizes)
+
+
 def _loss_desc(rows: int, weight: Tensor, x_stride: int, labels_int64: bool, ignore_index: int, reduction: int):
-    d = _lib.LossDesc(rows, weight.shape[1], weight.shape[0], _LOSS_TYPES[weight.dtype], reduction, labels_int64, ignore_index,
-                      max(x_stride, weight.shape[1]), max(weight.stride(0), weight.shape[1]))
-    sizes = C.c_size_t(), C.c_size_t(), C.c_size_t()
-    _lib.check(_lib.lib().nsa_loss_workspace_bytes(C.byref(d), _ptr(weight), *map(C.byref, sizes)), "nsa_loss_workspace_bytes")
-    return d, *(s.value for s in sizes)
+    vocab, dim = weight.shape
+    return _loss_sizes(rows, dim, vocab, _LOSS_TYPES[weight.dtype], reduction, labels_int64, ignore_index, max(x_stride, dim), max(weight.stride(0), dim),
+                       aligned=weight.data_ptr() % 16 == 0)
 
 
 @torch.library.custom_op("nsa_amd::linear_cross_entropy_fwd", mutates_args=())
@@ -2635,7 +2642,7 @@ def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_i
         state = torch.empty((state_bytes,), dtype=torch.uint8, device=x.device)
         if loss.numel():
             ws = torch.empty((fwd_bytes,), dtype=torch.uint8, device=x.device)
-            _lib.check(_lib.lib().nsa_loss_fwd(C.byref(d), _ptr(x), _ptr(weight), _ptr(labels), _ptr(state), state_bytes, _ptr(ws), fwd_bytes, _ptr(loss),
+            _lib.check(_lib.lib().nsa_loss_fwd(d, _ptr(x), _ptr(weight), _ptr(labels), _ptr(state), state_bytes, _ptr(ws), fwd_bytes, _ptr(loss),
                                                _stream()), "nsa_loss_fwd")
     return loss, state
 
@@ -2660,7 +2667,7 @@ def linear_cross_entropy_bwd(dloss: Tensor, x: Tensor, weight: Tensor, state: Te
             x, weight, dloss = _unit_rows(x), _unit_rows(weight), dloss.to(torch.float32).contiguous()
             d, state_bytes, _, bwd_bytes = _loss_desc(rows, weight, x.stride(0), True, ignore_index, reduction)
             ws = torch.empty((bwd_bytes,), dtype=torch.uint8, device=weight.device)
-            _lib.check(_lib.lib().nsa_loss_bwd(C.byref(d), _ptr(x), _ptr(weight), _ptr(state), state_bytes, _ptr(dloss), _ptr(ws), bwd_bytes,
+            _lib.check(_lib.lib().nsa_loss_bwd(d, _ptr(x), _ptr(weight), _ptr(state), state_bytes, _ptr(dloss), _ptr(ws), bwd_bytes,
                                                _ptr(dx) if want_dx else 0, _ptr(dw) if want_dw else 0, _stream()), "nsa_loss_bwd")
     return dx, dw
 
@@ -2698,7 +2705,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, ignore_index
     logits in memory: weight 'v d', labels '...' int64 or int32, x and weight both bf16, fp16 or fp32 on one device.  fp32, one value or
     (reduction "none") one per row; rows labelled `ignore_index` count nothing and are not read.  Logits and sums are fp32 (F.linear would
     round them to x's type first); gradients have x's and weight's type.  A label that is neither `ignore_index` nor in the vocabulary
-    makes its loss and the gradients NaN: it is known to the device only.  The gradients cannot be differentiated again."""
+    makes its loss and the gradients NaN: it is known to the device only.  Weights are finite.  The gradients cannot be differentiated again."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction {reduction!r}, expected one of {sorted(_REDUCTIONS)}")
     if x.is_cuda and torch.is_autocast_enabled():
@@ -2713,8 +2720,10 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, ignore_index
                            "'v d' and '...'")
     if labels.dtype not in (torch.int64, torch.int32):
         raise RuntimeError(f"linear_cross_entropy: labels {labels.dtype}: expected int64 or int32")
-    loss, _ = _linear_cross_entropy(x.reshape(-1, x.shape[-1]), weight, labels.reshape(-1), int(ignore_index), _REDUCTIONS[reduction])
-    return loss.view(labels.shape) if reduction == "none" else loss
+    flat = x.dim() == 2
+    loss, _ = _linear_cross_entropy(x if flat else x.reshape(-1, x.shape[-1]), weight, labels if flat else labels.reshape(-1), int(ignore_index),
+                                    _REDUCTIONS[reduction])
+    return loss if flat or reduction != "none" else loss.view(labels.shape)
 
 
 def _newton_schulz(matrices, steps: int, a: float, b: float, c: float, eps: float):

@@ -441,3 +441,41 @@ def test_few_rows_replay():
         want = ops.linear_cross_entropy(*inputs[:3], reduction="none"), ops.linear_cross_entropy(*inputs[:3])
         torch.cuda.synchronize()
         assert torch.equal(each, want[0]) and torch.equal(mean.nan_to_num(nan=-1.), want[1].nan_to_num(nan=-1.))
+
+
+@pytest.mark.parametrize("n", [20, 40])
+def test_weights_past_4_gigabytes(n):
+    """Offsets of weights and gradients past 32 bits: the last entries' logits and gradients (in float64, piece by piece of the vocabulary)."""
+    from native_sparse_attention_pytorch_amd import ops
+    d, v = 4096, 600011
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(n, d, device=DEV, dtype=BF16, generator=g)
+    w = torch.randn(v, d, device=DEV, dtype=BF16, generator=g) * d ** -0.5
+    labels = torch.randint(v - 1000, v, (n,), device=DEV, generator=g)
+    weights = torch.rand(n, device=DEV, generator=g) + 0.1
+    x.requires_grad_(), w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, labels, reduction="none")
+    dx, dw = torch.autograd.grad(loss, (x, w), weights)
+    x6, size = x.detach().double(), x.detach().double().abs()
+    pieces = [w.detach()[i:i + 60000].double() for i in range(0, v, 60000)]
+    lse = torch.logsumexp(torch.cat([x6 @ p.t().contiguous() for p in pieces], 1), 1)
+    # logits as in _exact, where |x| |w| is at most 4096 times a product's mean of 0.64 d^-1/2, twice that with room
+    dl = (d / 4 + 8) * 2 ** -24 * 2 * 0.64 * d ** 0.5
+    own = (x6 * w.detach()[labels].double()).sum(1)
+    _within(loss.detach(), (lse - own, torch.full_like(own, 2 * dl + 2 ** -16 + 2 ** -20)), "loss")
+    want, tol = torch.zeros_like(x6), torch.zeros_like(x6)
+    for i, p in enumerate(pieces):
+        G = torch.exp(x6 @ p.t().contiguous() - lse[:, None])
+        off = G * (2 * dl + 2 ** -15 + 2 ** -11) + 2 ** -38
+        at = (labels - 60000 * i)
+        here = (at >= 0) & (at < len(p))
+        rows = here.nonzero()[:, 0]
+        off[rows, at[here]] += 2 ** -11 + 2 * dl + 2 ** -15
+        G[rows, at[here]] -= 1
+        G, off = G * weights.double()[:, None], off * weights.double()[:, None]
+        want += G @ p
+        tol += off @ p.abs() + 2 ** -14 * (G.abs() @ p.abs())
+        if i in (0, len(pieces) - 1):
+            exact = G.t().contiguous() @ x6
+            _within(dw[60000 * i:60000 * i + len(p)], (exact, off.t().contiguous() @ size + 2 ** -20 * (G.t().contiguous().abs() @ size) + 2 ** -8 * exact.abs()), "dw")
+    _within(dx, (want, tol + 2 ** -8 * want.abs()), "dx")

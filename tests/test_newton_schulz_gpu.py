@@ -261,3 +261,54 @@ def test_a_parameter_without_elements_is_left_alone():
     before = params[1].detach().clone()
     Muon(params).step()
     assert not torch.equal(params[1], before) and params[0].shape == (5, 0)
+
+
+@pytest.mark.parametrize("m,n,dtype", [(24, 512, F32), (130, 70, F16), (70, 130, BF16)])
+def test_in_place(m, n, dtype):
+    """The C entry writes a contiguous matrix over itself; the operator never writes its arguments."""
+    import ctypes as C
+
+    from native_sparse_attention_pytorch_amd import _lib, ops
+    g = _g(m, n, dtype=dtype)
+    kept = g.clone()
+    want = ops.newton_schulz(g)
+    assert torch.equal(g, kept)
+    ints, longs, ptrs, need = C.c_int32 * 1, C.c_int64 * 1, C.c_void_p * 1, C.c_size_t()
+    _lib.check(_lib.lib().nsa_newton_workspace_bytes(1, ints(m), ints(n), C.byref(need)), "nsa_newton_workspace_bytes")
+    ws = torch.empty(need.value, dtype=torch.uint8, device=DEV)
+    code = {BF16: 0, F16: 1, F32: 2}[dtype]
+    _lib.check(_lib.lib().nsa_newton_schulz(1, ints(m), ints(n), ptrs(g.data_ptr()), longs(n), ptrs(g.data_ptr()), code, 5, *ABC, 1e-7, ws.data_ptr(),
+                                            need.value, torch.cuda.current_stream().cuda_stream), "nsa_newton_schulz")
+    assert torch.equal(g, want)
+
+
+def test_two_graphs_and_launches_between_them():
+    """Two captured calls keep their own workspaces: replayed in turn, with launched calls between them, each gives its own result."""
+    from native_sparse_attention_pytorch_amd import ops
+    held = [[_g(130, 70, seed=1), _g(40, 600, seed=2)], [_g(90, 300, seed=3)]]
+    for h in held:
+        ops.newton_schulz(h)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for h in held:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.newton_schulz(h))
+        graphs.append(graph)
+    for seed in range(3):
+        for h in held:
+            for i, t in enumerate(h):
+                t.copy_(_g(*t.shape, seed=10 * seed + i))
+        for graph in graphs:
+            graph.replay()
+        want = [ops.newton_schulz(h) for h in held]
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for out, ws in zip(outs, want) for o, w in zip(out, ws))
+
+
+def test_traced():
+    from native_sparse_attention_pytorch_amd import ops
+    gs = [_g(70, 130), _g(24, 100, seed=1)]
+    want = ops.newton_schulz(gs)
+    got = torch.compile(lambda a, b: ops.newton_schulz([a, b]), backend="aot_eager")(*gs)
+    assert all(torch.equal(o, w) for o, w in zip(got, want))
