@@ -526,7 +526,7 @@ int nsa_decode_prep(const void* q, const int64_t* q_stride, const void* k, const
  *   dloss: fp32, as loss; dx [rows, dim], dw [vocab, dim] contiguous, of `dtype`; either may be NULL.  rows >= 1 for the backward.
  * Sums in fp32; fp32 operands as two fp16 halves each (22 bits; what is below 2^-18 of a matrix's largest value is kept to 2^-40 of that), results
  * rounded once.  Infinities and NaN among the weights may make NaN of any logit of their entry.  The order of the additions depends on sizes, the
- * weight's stride and alignment, and the number of counting rows only.  Alignment: that of the type.
+ * weight's stride and alignment, and the number of counting rows only.  Alignment: that of the type; state and ws: 256 bytes.
  * rows <= 2^24, dim <= 2^16, vocab <= 2^24, either of rows and vocab times dim (rounded up to 64) below 2^33 (NSA_E_UNSUPPORTED otherwise). */
 typedef struct nsa_loss_desc {
   int64_t rows;
@@ -549,7 +549,7 @@ int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* weight, cons
  *   elements apart, out[k] contiguous, alignment that of the type; all of dtype 0 bf16, 1 fp16, 2 fp32.  out[k] may be in[k] where that is
  *   contiguous.  Products of two fp16 halves (22 bits) with fp32 sums, results rounded once: as exact as fp32 products.
  *   Coefficients that take a singular value of [0, 1] past 4 on its way: NSA_E_UNSUPPORTED.  Zero matrices give zeros (eps > 0).
- * The result of a matrix depends on nothing but itself and the sizes of all. */
+ * The result of a matrix depends on nothing but itself and the sizes of all.  ws: aligned to 256 bytes. */
 int nsa_newton_workspace_bytes(int32_t many, const int32_t* rows, const int32_t* cols, size_t* bytes);
 int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_t* cols, const void* const* in, const int64_t* in_stride, void* const* out,
                       int32_t dtype, int32_t steps, float a, float b, float c, float eps, void* ws, size_t ws_bytes, void* stream);

@@ -27,7 +27,10 @@ namespace nsa {
 
 constexpr int kGradBits = 14;
 // device words of a call: rows that count; bits of the largest finite |x|, |w|, |g|; slices of dx
-enum { CELL_ROWS, CELL_X, CELL_W, CELL_G, CELL_SLICES, CELLS = 16 };
+enum { CELL_ROWS, CELL_X, CELL_W, CELL_G, CELL_SLICES, CELLS = 64 };
+// the largest bf16 |x| is found while its rows are copied, by this many work-groups' atomics in turn to words of their own, 64 bytes apart (8184 rows of
+// 512: 24 us with one word for all, 13 so); the backward takes the largest of them
+constexpr int kMost = 16;
 
 // How logits are made: FEW rows as loss_few_kernel has them, the others by tiles of 64, 128 or 256 (loss_plan)
 enum LossSize { FEW, TINY, MIDDLE, WIDE };
@@ -91,7 +94,7 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   };
   p.w_splits = w_slices(piece);
   p.last_splits = w_slices(last);
-  size_t at = up(CELLS * 4, 256);
+  size_t at = CELLS * 4 + kMost * 64;
   auto take = [&](size_t bytes) { const size_t here = at; at = up(at + bytes, 256); return here; };
   p.s_map = take((size_t)p.npad * 4);
   p.s_place = take((size_t)p.npad * 4);
@@ -169,6 +172,7 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(const void* labels, int 
   }
   if (blockIdx.x == gridDim.x - 1 && tid == 0) cells[CELL_ROWS] = (unsigned)total;
   if (blockIdx.x == 0 && tid >= 1 && tid < CELLS) cells[tid] = 0;
+  if (blockIdx.x == 0 && tid < kMost) cells[CELLS + 16 * tid] = 0;
 }
 
 // up to 8 values of a row, zeros past its end
@@ -224,7 +228,7 @@ __global__ __launch_bounds__(256) void loss_largest_kernel(const S* src, long ld
 }
 
 // Rows (named by map, or all) as planes of kp columns, those past `cols` zero; rows past the last one up to a multiple of 64 zero too.
-// cell: the values are scaled below 2^15 by the power of two that suits its magnitude.  most: their largest magnitude goes there.  back: the last
+// cell: the values are scaled below 2^15 by the power of two that suits its magnitude.  most: their largest magnitude goes to one of those words.  back: the last
 // 64 columns end with the row's last value, `back` zeros before what is left (TileProduct::run).
 template <class S, class D, int P>
 __global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld, int rows, int cols, int kp, const int* map, const unsigned* count,
@@ -242,7 +246,7 @@ __global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld,
     unsigned best = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) best = max(best, finite_bits(v[e]));
-    largest_into(best, most);
+    largest_into(best, most + 16 * (blockIdx.x % kMost));
   }
   if (r >= (live + 63) / 64 * 64) return;
   const int shift = cell != nullptr ? plane_shift(*cell) : 0;
@@ -658,7 +662,7 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const float* loss, const
 // entries.  The rows that count decide, so they are chosen here.  (8192 rows, 40 % of them ignored, 1024 features, 50021 entries: 80 tiles in 2 slices
 // as for all rows 695 us, in 3 of them 600.)
 __global__ __launch_bounds__(1024) void loss_weights_kernel(const float* dloss, int reduction, const unsigned* count, const int* map, float* g, unsigned* cells,
-                                                            int tiles_m, int tile, int piece) {
+                                                            int tiles_m, int tile, int piece, const unsigned* most) {
   __shared__ unsigned best_s[16];
   const int live = (int)*count, tid = threadIdx.x;
   if (tid < kMaxSlices) {
@@ -669,7 +673,9 @@ __global__ __launch_bounds__(1024) void loss_weights_kernel(const float* dloss, 
     for (int o = 1; o < kMaxSlices; o <<= 1) time = min(time, (long)__shfl_xor(time, o));
     if (tid == 0) cells[CELL_SLICES] = (unsigned)(time & 63);
   }
-  unsigned best = 0;
+  unsigned best = 0, most_x = tid < kMost && most != nullptr ? most[16 * tid] : 0;
+#pragma unroll
+  for (int o = 1; o < kMost; o <<= 1) most_x = max(most_x, (unsigned)__shfl_xor((int)most_x, o));
   for (int i = tid; i < live; i += 1024) {
     const float v = reduction == 0 ? dloss[map[i]] : reduction == 1 ? dloss[0] / (float)live : dloss[0];
     g[i] = v;
@@ -683,7 +689,8 @@ __global__ __launch_bounds__(1024) void loss_weights_kernel(const float* dloss, 
   if (tid == 0) {
     for (int w = 1; w < 16; ++w) best = max(best, best_s[w]);
     cells[CELL_G] = best;
-    cells[CELL_X] = cells[CELL_W] = 0;
+    cells[CELL_W] = 0;
+    cells[CELL_X] = most_x;
   }
 }
 
@@ -840,6 +847,11 @@ static void launch_tiles(const LossPlan& p, const LossTileArgs& a, hipStream_t s
   else if constexpr (GRAD) launch_tile<typename L::Few, GRAD>(a, st);      // (the forward of few rows: loss_few_kernel)
 }
 
+static bool misaligned(std::initializer_list<const void*> all, size_t to) {
+  for (const void* p : all)
+    if ((uintptr_t)p % to) return true;
+  return false;
+}
 static unsigned blocks_for(long work) { return (unsigned)std::max<long>(1, (work + 255) / 256); }
 
 template <class S, class D, int P>
@@ -908,6 +920,8 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
   LossPlan p;
   if (int rc = loss_plan(d, weight, p)) return rc;
   if (!weight || !state || !ws || !loss || (p.n > 0 && (!x || !labels))) return NSA_E_ARG;
+  if (misaligned({x, weight}, d->dtype == 2 ? 4 : 2) || misaligned({state, ws}, 256) || misaligned({loss}, 4) || misaligned({labels}, d->labels_int64 ? 8 : 4))
+    return NSA_E_ARG;
   if (state_bytes < p.state || ws_bytes < p.fwd) return NSA_E_WORKSPACE;
   hipStream_t st = (hipStream_t)stream;
   char *s = (char*)state, *w = (char*)ws;
@@ -940,7 +954,7 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
     } else if (d->dtype == 1) {
       planes<H16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, w + p.f_x, x_plane, st, nullptr, back);
     } else {
-      planes<B16, B16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, w + p.f_x, x_plane, st, cells + CELL_X, back);
+      planes<B16, B16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, w + p.f_x, x_plane, st, cells + CELLS, back);
     }
     const int rows = p.in_place ? d->vocab : p.fwd_rows;
     for (long v0 = 0; v0 < d->vocab; v0 += rows) {
@@ -981,6 +995,7 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
   LossPlan p;
   if (int rc = loss_plan(d, weight, p)) return rc;
   if (!x || !weight || !state || !dloss || !ws || (!dx && !dw) || p.n == 0) return NSA_E_ARG;
+  if (misaligned({x, weight, dx, dw}, d->dtype == 2 ? 4 : 2) || misaligned({state, ws}, 256) || misaligned({dloss}, 4)) return NSA_E_ARG;
   if (state_bytes < p.state || ws_bytes < p.bwd) return NSA_E_WORKSPACE;
   hipStream_t st = (hipStream_t)stream;
   const char* s = (const char*)state;
@@ -992,14 +1007,14 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
   float* g = (float*)(w + p.b_g);
   const int each = d->dtype == 2 ? 4 : 2, tile = p.size == WIDE ? 256 : 128, tiles_m = (p.kp + tile - 1) / tile;
   hipLaunchKernelGGL(loss_weights_kernel, dim3(1), dim3(1024), 0, st, dloss, (int)d->reduction, count, map, g, cells, tiles_m, tile,
-                     std::min(p.bwd_rows, (int)up(d->vocab, 64)));
+                     std::min(p.bwd_rows, (int)up(d->vocab, 64)), d->dtype == 0 && p.size != FEW ? kept + CELLS : nullptr);
   // All operands in fp16: x once, w with each piece.  Magnitudes: those the forward has found, else here.
-  const bool have_x = p.size != FEW, have_w = p.size != FEW && d->dtype == 2;
-  const unsigned *xc = d->dtype == 1 ? nullptr : have_x ? kept + CELL_X : cells + CELL_X, *wc = d->dtype == 1 ? nullptr : have_w ? kept + CELL_W : cells + CELL_W;
+  const bool have = p.size != FEW, both = have && d->dtype == 2;
+  const unsigned *xc = d->dtype == 1 ? nullptr : both ? kept + CELL_X : cells + CELL_X, *wc = d->dtype == 1 ? nullptr : both ? kept + CELL_W : cells + CELL_W;
   if (d->dtype == 0) {
-    if (!have_x) largest<B16>(x, d->x_stride, p.n, d->dim, map, count, cells + CELL_X, st);
+    if (!have) largest<B16>(x, d->x_stride, p.n, d->dim, map, count, cells + CELL_X, st);
     largest<B16>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
-  } else if (d->dtype == 2 && !have_x) {
+  } else if (d->dtype == 2 && !have) {
     largest<float>(x, d->x_stride, p.n, d->dim, map, count, cells + CELL_X, st);
     largest<float>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
   }

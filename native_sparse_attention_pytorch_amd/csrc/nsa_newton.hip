@@ -618,7 +618,7 @@ extern "C" int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_
   size_t need = 0;
   if (int rc = nsa_newton_workspace_bytes(many, rows, cols, &need)) return rc;
   if (many == 0) return 0;
-  if (!in || !in_stride || !out || !ws || dtype < 0 || dtype > 2 || steps < 1 || steps > 100 || !(eps >= 0.f)) return NSA_E_ARG;
+  if (!in || !in_stride || !out || !ws || (uintptr_t)ws % 256 || dtype < 0 || dtype > 2 || steps < 1 || steps > 100 || !(eps >= 0.f)) return NSA_E_ARG;
   if (ws_bytes < need) return NSA_E_WORKSPACE;
   // singular values start in [0, 1]: where the polynomial takes them has to stay in the planes' range
   for (int i = 0; i <= 1024; ++i) {

@@ -20,6 +20,9 @@ def FeedForward(dim, expansion_factor=4.):
 
 
 class Transformer(nn.Module):
+    # return_loss by ops.linear_cross_entropy: no logits in memory, and their values in fp32 rather than rounded to the model's type
+    fused_loss = False
+
     def __init__(self, num_tokens, dim, depth, dim_head=64, heads=8, kv_heads=None, ff_expansion_factor=4.,
                  use_sparse_attn=True, causal=True, use_flex_sliding_window=False, use_flex_fine_selection=False,
                  use_triton_fine_selection=False, sparse_attn_kwargs: dict | None = None, fused_loss=False):
@@ -35,7 +38,6 @@ class Transformer(nn.Module):
                                                              num_selected_blocks=4))
         self.token_emb = nn.Embedding(num_tokens, dim)
         self.causal = causal
-        # return_loss by ops.linear_cross_entropy: no logits in memory, and their values in fp32 rather than rounded to the model's type
         self.fused_loss = fused_loss
         layers = []
         for _ in range(depth):

@@ -103,3 +103,27 @@ def test_entries_check_pointers_and_workspaces():
     assert L.nsa_newton_workspace_bytes(1, ints((1 << 20) + 1), ints(4), C.byref(need)) == -2
     assert L.nsa_newton_workspace_bytes(1, ints(1 << 16), ints(1 << 16), C.byref(need)) == -2
     assert L.nsa_newton_schulz(0, None, None, None, None, None, 0, 5, 1., 0., 0., 0., None, 0, 0) == 0
+
+
+def test_entries_check_alignment():
+    L, d = _lib.lib(), _desc(dtype=2)
+    _, (state, fwd, bwd) = _sizes(d, 256)
+    good = dict(x=256, w=256, labels=256, state=256, ws=256, loss=256)
+    for bad in (dict(x=258), dict(w=257), dict(labels=260), dict(state=272), dict(ws=384), dict(loss=258)):
+        p = {**good, **bad}
+        assert L.nsa_loss_fwd(C.byref(d), p["x"], p["w"], p["labels"], p["state"], state, p["ws"], fwd, p["loss"], 0) == -1, bad
+    good = dict(x=256, w=256, state=256, dloss=256, ws=256, dx=256, dw=256)
+    for bad in (dict(x=258), dict(w=257), dict(state=272), dict(dloss=258), dict(ws=384), dict(dx=258), dict(dw=257)):
+        p = {**good, **bad}
+        assert L.nsa_loss_bwd(C.byref(d), p["x"], p["w"], p["state"], state, p["dloss"], p["ws"], bwd, p["dx"], p["dw"], 0) == -1, bad
+    ints, longs, ptrs, need = C.c_int32 * 1, C.c_int64 * 1, C.c_void_p * 1, C.c_size_t()
+    assert L.nsa_newton_workspace_bytes(1, ints(40), ints(50), C.byref(need)) == 0
+    assert L.nsa_newton_schulz(1, ints(40), ints(50), ptrs(256), longs(50), ptrs(256), 2, 5, 1.5, -0.5, 0., 1e-7, 272, need.value, 0) == -1
+
+
+def test_a_model_made_before_the_option_has_it_off():
+    from native_sparse_attention_pytorch_amd.transformer import Transformer
+    model = Transformer(num_tokens=11, dim=64, depth=1, heads=1, fused_loss=True)
+    assert model.fused_loss
+    del model.__dict__["fused_loss"]
+    assert model.fused_loss is False
