@@ -2787,7 +2787,8 @@ def newton_schulz(updates, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315
     coefficients = tuple(float(v) for v in coefficients)
     if len(coefficients) != 3 or not 1 <= int(steps) <= 100 or not eps >= 0:
         raise ValueError(f"newton_schulz: steps {steps}, coefficients {coefficients}, eps {eps}: expected 1 to 100 steps, three coefficients, eps >= 0")
-    _newton_coefficients(coefficients, int(steps))
+    if not torch.compiler.is_compiling():      # (traced calls: the entry checks them)
+        _newton_coefficients(coefficients, int(steps))
     for t in given:
         if not t.is_cuda or t.device != given[0].device:
             raise RuntimeError("newton_schulz: needs tensors on one GPU (HIP kernels, no CPU fallback)")

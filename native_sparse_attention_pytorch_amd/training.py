@@ -118,7 +118,8 @@ class Muon(torch.optim.Optimizer):
         buffer <- momentum buffer + gradient;  update = gradient + momentum buffer (nesterov) or the buffer
         p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / columns)) newton_schulz(update)
 
-    Embeddings, norm weights and biases belong to another optimizer; vectors are refused.
+    Embeddings, norm weights and biases belong to another optimizer; vectors are refused.  The momentum buffer and the update are fp32, of 16-bit
+    parameters too: gradients below 2^-8 of the buffer would be lost in bf16.
 
         masters = Fp32Masters(model)
         matrices = [m for m, (name, p) in zip(masters.masters, model.named_parameters()) if p.dim() == 2 and "emb" not in name]
@@ -138,6 +139,18 @@ class Muon(torch.optim.Optimizer):
             if p.dim() < 2:
                 self.param_groups.pop()
                 raise ValueError(f"Muon takes matrices, got a parameter of shape {tuple(p.shape)}")
+            if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                self.param_groups.pop()
+                raise ValueError(f"Muon takes fp32, bf16 or fp16 parameters, got {p.dtype}")
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # (the base class rounds a state to its parameter's type)
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(ids, (p for group in self.param_groups for p in group["params"])):
+            kept = state_dict["state"].get(i, {}).get("momentum_buffer")
+            if kept is not None:
+                self.state[p]["momentum_buffer"] = kept.to(device=p.device, dtype=torch.float32, copy=True)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -153,7 +166,7 @@ class Muon(torch.optim.Optimizer):
             grads = [p.grad for p in params]
             for p in params:
                 if "momentum_buffer" not in self.state[p]:
-                    self.state[p]["momentum_buffer"] = torch.zeros_like(p)
+                    self.state[p]["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
             buffers = [self.state[p]["momentum_buffer"] for p in params]
             torch._foreach_mul_(buffers, group["momentum"])
             torch._foreach_add_(buffers, grads)

@@ -310,5 +310,29 @@ def test_traced():
     from native_sparse_attention_pytorch_amd import ops
     gs = [_g(70, 130), _g(24, 100, seed=1)]
     want = ops.newton_schulz(gs)
-    got = torch.compile(lambda a, b: ops.newton_schulz([a, b]), backend="aot_eager")(*gs)
+    got = torch.compile(lambda a, b: ops.newton_schulz([a, b]), backend="aot_eager", fullgraph=True)(*gs)
     assert all(torch.equal(o, w) for o, w in zip(got, want))
+    with pytest.raises(RuntimeError, match="nsa_newton_schulz"):
+        torch.compile(lambda a, b: ops.newton_schulz([a, b], coefficients=(5., 0., 0.)), backend="aot_eager", fullgraph=True)(*gs)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_muon_of_16_bit_parameters(dtype):
+    """The momentum is held in fp32, through a saved state too; the parameter is rounded at each of a step's two operations on it."""
+    from native_sparse_attention_pytorch_amd.training import Muon
+    p = torch.nn.Parameter(_g(70, 40, dtype=dtype))
+    opt = Muon([p], lr=0.05, momentum=0.9, weight_decay=0.1)
+    buffer = torch.zeros(70, 40, dtype=torch.float64, device=DEV)
+    for step in range(3):
+        p.grad = _g(70, 40, dtype=dtype, seed=20 + step, scale=2. ** -12 if step else 1.)      # (2^-12 of the buffer: gone in 16 bits)
+        buffer = 0.9 * buffer + p.grad.double()
+        want = (1 - 0.05 * 0.1) * p.detach().double() - 0.05 * (70 / 40) ** 0.5 * _exact(p.grad.double() + 0.9 * buffer)
+        opt.step()
+        u = torch.finfo(dtype).eps / 2
+        assert float((p.detach().double() - want).norm()) <= 2 * 1.01 * u * float(want.norm()) + 0.05 * (70 / 40) ** 0.5 * 2 ** -8
+        kept = opt.state[p]["momentum_buffer"]
+        assert kept.dtype == F32 and float((kept.double() - buffer).abs().max()) <= 2 ** -22 * float(buffer.abs().max())
+    again = Muon([p], lr=0.05)
+    again.load_state_dict(opt.state_dict())
+    assert torch.equal(again.state[p]["momentum_buffer"], kept) and again.state[p]["momentum_buffer"].dtype == F32
+    assert again.state[p]["momentum_buffer"].data_ptr() != kept.data_ptr() and again.param_groups[0]["momentum"] == 0.9

@@ -35,6 +35,8 @@ def test_muon_arguments():
             Muon([p], **bad)
     with pytest.raises(ValueError, match="matrices"):
         Muon([p, torch.nn.Parameter(torch.randn(4))])
+    with pytest.raises(ValueError, match="float64"):
+        Muon([p, torch.nn.Parameter(torch.randn(4, 4).double())])
     assert Muon([p]).step(lambda: 3.) == 3.      # no gradients: nothing to do
 
 
