@@ -26,11 +26,17 @@
 namespace nsa {
 
 constexpr int kGradBits = 14;
-// device words of a call: rows that count; bits of the largest finite |x|, |w|, |g|; slices of dx
-enum { CELL_ROWS, CELL_X, CELL_W, CELL_G, CELL_SLICES, CELLS = 64 };
-// the largest bf16 |x| is found while its rows are copied, by this many work-groups' atomics in turn to words of their own, 64 bytes apart (8184 rows of
-// 512: 24 us with one word for all, 13 so); the backward takes the largest of them
+// device words: of the state, the rows that count; of a backward pass, bits of the largest finite |g| and the slices of dx
+enum { CELL_ROWS, CELL_G = 0, CELL_SLICES, CELLS = 64 };
+// Behind those of the state, the bits of the largest finite |x| and |w| that work-groups have found, each in one of 16 words 64 bytes apart: a word
+// for all held up the copy of 8184 rows of 512 by 11 us.
 constexpr int kMost = 16;
+__device__ __forceinline__ unsigned most_of(const unsigned* words) {
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) m = max(m, words[16 * i]);
+  return m;
+}
 
 // How logits are made: FEW rows as loss_few_kernel has them, the others by tiles of 64, 128 or 256 (loss_plan)
 enum LossSize { FEW, TINY, MIDDLE, WIDE };
@@ -46,7 +52,7 @@ struct LossPlan {
   size_t state, fwd, bwd;                 // bytes
   size_t s_map, s_place, s_label, s_norm, s_own;                            // offsets in the state
   size_t f_part, f_target, f_loss, f_x, f_w;                           // in the forward's workspace
-  size_t b_cells, b_g, b_x, b_w, b_grad, b_dx, b_dw;                   // in the backward's
+  size_t b_cells, b_most, b_g, b_x, b_w, b_grad, b_dx, b_dw;                   // in the backward's
 };
 
 static size_t up(size_t v, size_t to) { return (v + to - 1) / to * to; }
@@ -94,7 +100,7 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   };
   p.w_splits = w_slices(piece);
   p.last_splits = w_slices(last);
-  size_t at = CELLS * 4 + kMost * 64;
+  size_t at = CELLS * 4 + 2 * kMost * 64;
   auto take = [&](size_t bytes) { const size_t here = at; at = up(at + bytes, 256); return here; };
   p.s_map = take((size_t)p.npad * 4);
   p.s_place = take((size_t)p.npad * 4);
@@ -111,6 +117,7 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.fwd = at;
   at = 0;
   p.b_cells = take(CELLS * 4);
+  p.b_most = take((size_t)(p.npad + 1023) / 1024 * 4);
   p.b_g = take((size_t)p.npad * 4);
   p.b_x = take(p.npad * row * p.grad_P);
   p.b_w = take(p.bwd_rows * row * p.grad_P);
@@ -171,8 +178,7 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(const void* labels, int 
     }
   }
   if (blockIdx.x == gridDim.x - 1 && tid == 0) cells[CELL_ROWS] = (unsigned)total;
-  if (blockIdx.x == 0 && tid >= 1 && tid < CELLS) cells[tid] = 0;
-  if (blockIdx.x == 0 && tid < kMost) cells[CELLS + 16 * tid] = 0;
+  if (blockIdx.x == 0 && tid < 2 * kMost) cells[CELLS + 16 * tid] = 0;
 }
 
 // up to 8 values of a row, zeros past its end
@@ -187,69 +193,153 @@ template <class S> __device__ __forceinline__ void load_values(const S* p, int h
   }
 }
 
-// The largest of the work-group's values into *cell.  (Whoever finds a larger one there already has nothing to say: with an atomic a wave, 16384 of
-// them on one address, the kernel took 100 us for 8 MB.)
-__device__ __forceinline__ void largest_into(unsigned best, unsigned* cell) {
+__device__ __forceinline__ unsigned finite_bits(float v) {
+  const unsigned u = __builtin_bit_cast(unsigned, v) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;
+}
+// the largest of the work-group's values, in thread 0
+__device__ __forceinline__ unsigned largest_of(unsigned best) {
   __shared__ unsigned best_s[4];
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) best = max(best, (unsigned)__shfl_xor((int)best, o));
   if ((threadIdx.x & 63) == 0) best_s[threadIdx.x >> 6] = best;
   __syncthreads();
-  if (threadIdx.x != 0) return;
-  best = max(max(best_s[0], best_s[1]), max(best_s[2], best_s[3]));
-  if (best > __hip_atomic_load(cell, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(cell, best);
+  return max(max(best_s[0], best_s[1]), max(best_s[2], best_s[3]));
 }
-__device__ __forceinline__ unsigned finite_bits(float v) {
-  const unsigned u = __builtin_bit_cast(unsigned, v) & 0x7fffffffu;
-  return u < 0x7f800000u ? u : 0u;
+// Into one of `words`.  (Whoever finds a larger one there already has nothing to say: with an atomic a wave, 16384 of them on one address, the
+// kernel took 100 us for 8 MB.)
+__device__ __forceinline__ void largest_into(unsigned best, unsigned* words, int block) {
+  best = largest_of(best);
+  unsigned* word = words + 16 * (block % kMost);
+  if (threadIdx.x == 0 && best > __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(word, best);
 }
 
-// bits of the largest finite |value| of a matrix (of the rows that map names, if it is given) into *cell, which is zero or such bits
+// A matrix, or the rows of it that map names, whose largest finite |value| is to be known: `words` are zero, or hold such values of it
+struct LossMost {
+  const void* src;
+  long ld;
+  int rows, cols;
+  const int* map;
+  const unsigned* count;
+  unsigned* words;
+  int blocks;
+};
+struct LossBegin {
+  LossMost of[2];
+  // the backward's weights (work-groups behind those): g of the rows that count, and of each 1024 of them the bits of the largest finite |g|
+  const float* dloss;
+  int reduction;
+  const int* map;
+  const unsigned* count;
+  float* g;
+  unsigned* most;
+};
+// What has to be known of the operands before they are copied
 template <class S>
-__global__ __launch_bounds__(256) void loss_largest_kernel(const S* src, long ld, int rows, int cols, const int* map, const unsigned* count, unsigned* cell) {
-  const int live = count != nullptr ? (int)*count : rows;
-  const bool flat = map == nullptr && ld == cols;      // one run of values
-  const unsigned per = (cols + 7) / 8;
-  const long total = (long)live * cols, pieces = flat ? (total + 7) / 8 : (long)live * per;
+__global__ __launch_bounds__(256) void loss_begin_kernel(const LossBegin G) {
+  const int second = (int)blockIdx.x - G.of[0].blocks, third = second - G.of[1].blocks;
   unsigned best = 0;
+  if (third >= 0) {
+    const int live = (int)*G.count;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = third * 1024 + e * 256 + threadIdx.x;
+      if (i >= live) break;
+      const float v = G.reduction == 0 ? G.dloss[G.map[i]] : G.reduction == 1 ? G.dloss[0] / (float)live : G.dloss[0];
+      G.g[i] = v;
+      best = max(best, finite_bits(v));
+    }
+    best = largest_of(best);
+    if (threadIdx.x == 0) G.most[third] = best;
+    return;
+  }
+  const LossMost& M = G.of[second >= 0];
+  const int block = second >= 0 ? second : (int)blockIdx.x;
+  const S* src = (const S*)M.src;
+  const int live = M.count != nullptr ? (int)*M.count : M.rows;
+  const bool flat = M.map == nullptr && M.ld == M.cols;      // one run of values
+  const unsigned per = (M.cols + 7) / 8;
+  const long total = (long)live * M.cols, pieces = flat ? (total + 7) / 8 : (long)live * per;
 #pragma unroll 4
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (long)gridDim.x * 256) {
+  for (long i = (long)block * 256 + threadIdx.x; i < pieces; i += (long)M.blocks * 256) {
     float v[8];
     if (flat) {
       load_values(src + 8 * i, (int)min(8L, total - 8 * i), v);
     } else {
       const unsigned r = (unsigned)i / per, c = ((unsigned)i - r * per) * 8;
-      load_values(src + (map != nullptr ? map[r] : (int)r) * ld + c, cols - (int)c, v);
+      load_values(src + (M.map != nullptr ? M.map[r] : (int)r) * M.ld + c, M.cols - (int)c, v);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) best = max(best, finite_bits(v[e]));
   }
-  largest_into(best, cell);
+  largest_into(best, M.words, block);
 }
 
 // Rows (named by map, or all) as planes of kp columns, those past `cols` zero; rows past the last one up to a multiple of 64 zero too.
-// cell: the values are scaled below 2^15 by the power of two that suits its magnitude.  most: their largest magnitude goes to one of those words.  back: the last
-// 64 columns end with the row's last value, `back` zeros before what is left (TileProduct::run).
+// words: the values are scaled below 2^15 by the power of two that suits the largest of those.  most: their own largest goes there.  back: the
+// last 64 columns end with the row's last value, `back` zeros before what is left (TileProduct::run).
+struct LossRows {
+  const void* src;
+  long ld;
+  int rows, cols;
+  const int* map;
+  const unsigned *count, *words;
+  void* dst;
+  long plane;
+  unsigned* most;
+  int back, blocks;
+};
+struct LossCopy {
+  LossRows of[2];
+  int kp;
+  // the first of a backward pass: the largest of the weights, and the slices of a piece's entries that dx is summed from
+  const unsigned *most, *count;
+  unsigned* cells;
+  int tiles_m, tile, piece;
+};
+// Slices of dx: those whose rounds on 256 CUs end first, where a tile's beginning and end, and its share of the sum of slices, cost as much as 512
+// entries.  The rows that count decide, so they are chosen here.  (8192 rows, 40 % of them ignored, 1024 features, 50021 entries: 80 tiles in 2 slices
+// as for all rows 695 us, in 3 of them 600.)
+__device__ __forceinline__ void loss_cells(const LossCopy& G) {
+  const int live = (int)*G.count, tid = threadIdx.x;
+  unsigned best = 0;
+  for (int i = tid; i < (live + 1023) / 1024; i += 256) best = max(best, G.most[i]);
+  best = largest_of(best);
+  if (tid == 0) G.cells[CELL_G] = best;
+  if (tid < kMaxSlices) {
+    const int n = tid + 1, tiles = G.tiles_m * ((live + G.tile - 1) / G.tile), rounds = (tiles * n + 255) / 256;
+    long time = n > 1 && (tiles * n > kSliceTiles || G.piece / n < 512) ? 1L << 50 : (long)rounds * (G.piece / n + 512);
+    time = time * 64 + n;
+#pragma unroll
+    for (int o = 1; o < kMaxSlices; o <<= 1) time = min(time, (long)__shfl_xor(time, o));
+    if (tid == 0) G.cells[CELL_SLICES] = (unsigned)(time & 63);
+  }
+}
 template <class S, class D, int P>
-__global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld, int rows, int cols, int kp, const int* map, const unsigned* count,
-                                                          const unsigned* cell, D* dst, long plane, unsigned* most, int back) {
-  const int live = count != nullptr ? (int)*count : rows;
-  const unsigned per = kp / 8, i = blockIdx.x * 256 + threadIdx.x;      // (below 2^31: loss_plan)
+__global__ __launch_bounds__(256) void loss_planes_kernel(const LossCopy G) {
+  if (G.cells != nullptr && (int)blockIdx.x == G.of[0].blocks + G.of[1].blocks) {
+    loss_cells(G);
+    return;
+  }
+  const bool second = (int)blockIdx.x >= G.of[0].blocks;
+  const LossRows& M = G.of[second];
+  const unsigned block = blockIdx.x - (second ? G.of[0].blocks : 0), per = G.kp / 8, i = block * 256 + threadIdx.x;      // (below 2^31: loss_plan)
+  const int live = M.count != nullptr ? (int)*M.count : M.rows;
   const int r = (int)(i / per), c = (int)(i % per) * 8;
-  if (blockIdx.x * 256 / per >= (unsigned)(live + 63) / 64 * 64) return;
+  if (block * 256 / per >= (unsigned)(live + 63) / 64 * 64) return;
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 0.f;
-  const int from = back > 0 && c >= kp - 64 ? c - back : c;
-  if (r < live && from < cols && (from == c || from >= kp - 64)) load_values(src + (map != nullptr ? map[r] : r) * ld + from, cols - from, v);
-  if (most != nullptr) {
+  const int from = M.back > 0 && c >= G.kp - 64 ? c - M.back : c;
+  if (r < live && from < M.cols && (from == c || from >= G.kp - 64)) load_values((const S*)M.src + (M.map != nullptr ? M.map[r] : r) * M.ld + from, M.cols - from, v);
+  if (M.most != nullptr) {
     unsigned best = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) best = max(best, finite_bits(v[e]));
-    largest_into(best, most + 16 * (blockIdx.x % kMost));
+    largest_into(best, M.most, block);
   }
   if (r >= (live + 63) / 64 * 64) return;
-  const int shift = cell != nullptr ? plane_shift(*cell) : 0;
+  const int shift = M.words != nullptr ? plane_shift(most_of(M.words)) : 0;
   typename PlaneVec<D>::x8 hi, lo;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -262,9 +352,9 @@ __global__ __launch_bounds__(256) void loss_planes_kernel(const S* src, long ld,
       hi[e] = (D)x;
     }
   }
-  const long at = (long)r * kp + c;
-  *reinterpret_cast<decltype(hi)*>(dst + at) = hi;
-  if (P == 2) *reinterpret_cast<decltype(lo)*>(dst + plane + at) = lo;
+  D* to = (D*)M.dst + (long)r * G.kp + c;
+  *reinterpret_cast<decltype(hi)*>(to) = hi;
+  if (P == 2) *reinterpret_cast<decltype(lo)*>(to + M.plane) = lo;
 }
 
 // ------------------------------------------------------------------------------------ tiles of logits
@@ -275,7 +365,7 @@ struct LossTileArgs {
   int kp, v0, vend;                        // the piece: entries v0 .. vend - 1
   int tail, back;                          // see TileProduct::run; tail in features
   int n, tiles_m;
-  const unsigned *count, *x_cell, *w_cell;  // cells: null where the planes are not scaled
+  const unsigned *count, *x_most, *w_most;  // null where the planes are not scaled
   const int* label;
   float2* part;                            // [parts][npad]
   float* target;
@@ -317,7 +407,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
   t.run(G.kp / Tiles::BK, 0, G.back > 0 ? G.tail / Tiles::BK : -1, G.back);
 
   constexpr bool SCALED = Tiles::P == 2 || GRAD;
-  const int unscale = SCALED && G.x_cell != nullptr ? -(plane_shift(*G.x_cell) + plane_shift(*G.w_cell)) : 0;
+  const int unscale = SCALED && G.x_most != nullptr ? -(plane_shift(most_of(G.x_most)) + plane_shift(most_of(G.w_most))) : 0;
   const bool cut = m0 + Tiles::TM > G.vend;      // entries past the last one
   constexpr int PART = Tiles::TM / Tiles::WM;
   const int g_shift = GRAD ? kGradBits - plane_exponent(*G.g_cell) : 0;
@@ -457,7 +547,8 @@ __global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
     } else if (G.losses != nullptr && lane < G.n) {
       G.losses[lane] = 0.f;
     }
-    if (lane < CELLS) G.cells[lane] = lane == CELL_ROWS ? (unsigned)live : 0;
+    if (lane == 0) G.cells[CELL_ROWS] = (unsigned)live;
+    if (lane < 2 * kMost) G.cells[CELLS + 16 * lane] = 0;
   }
   if (live == 0) return;
   __syncthreads();
@@ -657,48 +748,11 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const float* loss, const
 
 // ------------------------------------------------------------------------------------ gradients
 
-// g of the rows that count, the bits of their largest finite magnitude, the other cells cleared, and the slices of a piece's entries that dx is
-// summed from: those whose rounds on 256 CUs end first, where a tile's beginning and end, and its share of the sum of slices, cost as much as 512
-// entries.  The rows that count decide, so they are chosen here.  (8192 rows, 40 % of them ignored, 1024 features, 50021 entries: 80 tiles in 2 slices
-// as for all rows 695 us, in 3 of them 600.)
-__global__ __launch_bounds__(1024) void loss_weights_kernel(const float* dloss, int reduction, const unsigned* count, const int* map, float* g, unsigned* cells,
-                                                            int tiles_m, int tile, int piece, const unsigned* most) {
-  __shared__ unsigned best_s[16];
-  const int live = (int)*count, tid = threadIdx.x;
-  if (tid < kMaxSlices) {
-    const int n = tid + 1, tiles = tiles_m * ((live + tile - 1) / tile), rounds = (tiles * n + 255) / 256;
-    long time = n > 1 && (tiles * n > kSliceTiles || piece / n < 512) ? 1L << 50 : (long)rounds * (piece / n + 512);
-    time = time * 64 + n;
-#pragma unroll
-    for (int o = 1; o < kMaxSlices; o <<= 1) time = min(time, (long)__shfl_xor(time, o));
-    if (tid == 0) cells[CELL_SLICES] = (unsigned)(time & 63);
-  }
-  unsigned best = 0, most_x = tid < kMost && most != nullptr ? most[16 * tid] : 0;
-#pragma unroll
-  for (int o = 1; o < kMost; o <<= 1) most_x = max(most_x, (unsigned)__shfl_xor((int)most_x, o));
-  for (int i = tid; i < live; i += 1024) {
-    const float v = reduction == 0 ? dloss[map[i]] : reduction == 1 ? dloss[0] / (float)live : dloss[0];
-    g[i] = v;
-    const unsigned u = __builtin_bit_cast(unsigned, v) & 0x7fffffffu;
-    best = u < 0x7f800000u ? max(best, u) : best;
-  }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) best = max(best, (unsigned)__shfl_xor((int)best, o));
-  if ((tid & 63) == 0) best_s[tid >> 6] = best;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < 16; ++w) best = max(best, best_s[w]);
-    cells[CELL_G] = best;
-    cells[CELL_W] = 0;
-    cells[CELL_X] = most_x;
-  }
-}
-
 struct LossGradArgs {
   const _Float16 *grad, *w, *x;       // G [npad][grad_ld]; w [piece][kp]; x [npad][kp]
   long grad_plane, w_plane, x_plane;
   int grad_ld, kp, tiles_m, entries;
-  const unsigned *count, *w_cell, *x_cell, *g_cell;
+  const unsigned *count, *w_most, *x_most, *g_cell;
   // dx
   float* sums;                        // [slices][live rows up to a multiple of 64][kp]
   int first;                          // first piece
@@ -726,7 +780,7 @@ __device__ __forceinline__ void loss_dx(const LossGradArgs& G, char* shared) {
   t.operand_b(G.grad, G.grad_plane, G.grad_ld, n0, live);
   t.run(steps, from);
   // (all pieces share the power of two)
-  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.w_cell != nullptr ? plane_shift(*G.w_cell) : 0);
+  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.w_most != nullptr ? plane_shift(most_of(G.w_most)) : 0);
   float* sums = G.sums + (size_t)split * ((live + 63) / 64 * 64) * G.kp;
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j)
@@ -754,7 +808,7 @@ __device__ __forceinline__ void loss_dw(const LossGradArgs& G, char* shared) {
   } else {
     t.run(steps);
   }
-  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.x_cell != nullptr ? plane_shift(*G.x_cell) : 0);
+  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.x_most != nullptr ? plane_shift(most_of(G.x_most)) : 0);
   O* dw = (O*)G.dw + (SLICES ? (size_t)split * G.entries * G.dw_ld : 0);
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j)
@@ -854,24 +908,23 @@ static bool misaligned(std::initializer_list<const void*> all, size_t to) {
 }
 static unsigned blocks_for(long work) { return (unsigned)std::max<long>(1, (work + 255) / 256); }
 
+static LossMost most_to(const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, unsigned* words) {
+  return LossMost{src, ld, rows, cols, map, count, words, (int)std::min(1024u, blocks_for((long)rows * ((cols + 7) / 8)))};
+}
+static void begin(const nsa_loss_desc* d, const LossBegin& a, int blocks, hipStream_t st) {
+  const dim3 grid((unsigned)(a.of[0].blocks + a.of[1].blocks + blocks)), block(256);
+  if (d->dtype == 0) hipLaunchKernelGGL((loss_begin_kernel<B16>), grid, block, 0, st, a);
+  else if (d->dtype == 1) hipLaunchKernelGGL((loss_begin_kernel<H16>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((loss_begin_kernel<float>), grid, block, 0, st, a);
+}
+static LossRows rows_to(const LossPlan& p, const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, const unsigned* words, void* dst,
+                        long plane, unsigned* most = nullptr, int back = 0) {
+  return LossRows{src, ld, rows, cols, map, count, words, dst, plane, most, back, (int)blocks_for((long)up(rows, 64) * p.kp / 8)};
+}
 template <class S, class D, int P>
-static void planes(const void* src, long ld, int rows, int rows_cap, int cols, int kp, const int* map, const unsigned* count, const unsigned* cell, void* dst,
-                   long plane, hipStream_t st, unsigned* most = nullptr, int back = 0) {
-  hipLaunchKernelGGL((loss_planes_kernel<S, D, P>), dim3(blocks_for((long)up(rows_cap, 64) * kp / 8)), dim3(256), 0, st, (const S*)src, ld, rows, cols, kp,
-                     map, count, cell, (D*)dst, plane, most, back);
-}
-template <class S>
-static void largest(const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, unsigned* cell, hipStream_t st) {
-  const long work = (long)rows * ((cols + 7) / 8);
-  hipLaunchKernelGGL((loss_largest_kernel<S>), dim3(std::min(1024u, blocks_for(work))), dim3(256), 0, st, (const S*)src, ld, rows, cols, map, count,
-                     cell);
-}
-// the weight's rows from v0 as the forward's planes
-static void forward_weight(const nsa_loss_desc* d, const LossPlan& p, const void* weight, int v0, int rows, const unsigned* cell, void* dst, hipStream_t st) {
-  const long plane = (long)p.kp * up(rows, 64);
-  if (d->dtype == 0) planes<B16, B16, 1>((const B16*)weight + (long)v0 * d->w_stride, d->w_stride, rows, rows, d->dim, p.kp, nullptr, nullptr, nullptr, dst, plane, st);
-  else if (d->dtype == 1) planes<H16, H16, 1>((const H16*)weight + (long)v0 * d->w_stride, d->w_stride, rows, rows, d->dim, p.kp, nullptr, nullptr, nullptr, dst, plane, st);
-  else planes<float, H16, 2>((const float*)weight + (long)v0 * d->w_stride, d->w_stride, rows, rows, d->dim, p.kp, nullptr, nullptr, cell, dst, plane, st);
+static void copy(const LossCopy& a, hipStream_t st) {
+  const unsigned blocks = (unsigned)(a.of[0].blocks + a.of[1].blocks + (a.cells != nullptr));
+  if (blocks > 0) hipLaunchKernelGGL((loss_planes_kernel<S, D, P>), dim3(blocks), dim3(256), 0, st, a);
 }
 
 template <int P, class O, bool SLICES>
@@ -931,13 +984,14 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
   float *own = (float*)(s + p.s_own), *each = (float*)(w + p.f_loss), *target = (float*)(w + p.f_target);
   float* losses = d->reduction == 0 ? loss : nullptr;
   float2* part = (float2*)(w + p.f_part);
-  const unsigned *count = cells + CELL_ROWS, *xc = d->dtype == 2 ? cells + CELL_X : nullptr, *wc = d->dtype == 2 ? cells + CELL_W : nullptr;
+  const unsigned* count = cells + CELL_ROWS;
+  unsigned *x_most = cells + CELLS, *w_most = x_most + 16 * kMost;
+  const int each_bytes = d->dtype == 2 ? 4 : 2;
   if (p.size == FEW) {
     LossFewArgs a{x, weight, labels, (long)d->x_stride, (long)d->w_stride, (long)d->ignore_index, (int)d->labels_int64, p.n, d->dim, d->vocab, p.npad,
                   map, place, label, cells, part, target, losses};
     const dim3 grid((unsigned)((d->vocab + 127) / 128));
-    const int each = d->dtype == 2 ? 4 : 2;
-    const bool aligned = (((uintptr_t)x | (uintptr_t)weight) & 15) == 0 && d->x_stride * each % 16 == 0 && d->w_stride * each % 16 == 0;
+    const bool aligned = (((uintptr_t)x | (uintptr_t)weight) & 15) == 0 && d->x_stride * each_bytes % 16 == 0 && d->w_stride * each_bytes % 16 == 0;
     const auto kernel = d->dtype == 0 ? aligned ? loss_few_kernel<B16, true> : loss_few_kernel<B16, false>
                         : d->dtype == 1 ? aligned ? loss_few_kernel<H16, true> : loss_few_kernel<H16, false>
                                         : aligned ? loss_few_kernel<float, true> : loss_few_kernel<float, false>;
@@ -947,33 +1001,39 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
                        (long)d->ignore_index, map, place, label, cells, losses);
     const long x_plane = (long)p.npad * p.kp;
     const int back = p.in_place ? p.kp - d->dim : 0;
-    if (d->dtype == 2) {
-      largest<float>(x, d->x_stride, p.n, d->dim, map, count, cells + CELL_X, st);
-      largest<float>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
-      planes<float, H16, 2>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, xc, w + p.f_x, x_plane, st);
-    } else if (d->dtype == 1) {
-      planes<H16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, w + p.f_x, x_plane, st, nullptr, back);
-    } else {
-      planes<B16, B16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, w + p.f_x, x_plane, st, cells + CELLS, back);
+    const bool scaled = d->dtype == 2;
+    if (scaled) {
+      LossBegin a{};
+      a.of[0] = most_to(x, d->x_stride, p.n, d->dim, map, count, x_most);
+      a.of[1] = most_to(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, w_most);
+      begin(d, a, 0, st);
     }
     const int rows = p.in_place ? d->vocab : p.fwd_rows;
     for (long v0 = 0; v0 < d->vocab; v0 += rows) {
       LossTileArgs a{};
       a.v0 = (int)v0;
       a.vend = (int)std::min<long>(d->vocab, v0 + rows);
+      LossCopy c{};
+      c.kp = p.kp;
+      // (a bf16 backward pass wants to know the largest |x|)
+      if (v0 == 0) c.of[0] = rows_to(p, x, d->x_stride, p.n, d->dim, map, count, scaled ? x_most : nullptr, w + p.f_x, x_plane, d->dtype == 0 ? x_most : nullptr, back);
       if (p.in_place) {
         a.w = weight;
         a.w_ld = d->w_stride;
         a.tail = p.kp - 64;
         a.back = back;
       } else {
-        forward_weight(d, p, weight, a.v0, a.vend - a.v0, wc, w + p.f_w, st);
         a.w = w + p.f_w;
         a.w_ld = p.kp;
         a.w_plane = (long)p.kp * up(a.vend - a.v0, 64);
+        c.of[1] = rows_to(p, (const char*)weight + v0 * d->w_stride * each_bytes, d->w_stride, a.vend - a.v0, d->dim, nullptr, nullptr, scaled ? w_most : nullptr,
+                          w + p.f_w, a.w_plane);
       }
+      if (d->dtype == 0) copy<B16, B16, 1>(c, st);
+      else if (d->dtype == 1) copy<H16, H16, 1>(c, st);
+      else copy<float, H16, 2>(c, st);
       a.x = w + p.f_x; a.x_plane = x_plane; a.kp = p.kp; a.n = p.n; a.npad = p.npad;
-      a.count = count; a.x_cell = xc; a.w_cell = wc; a.label = label; a.part = part; a.target = target;
+      a.count = count; a.x_most = scaled ? x_most : nullptr; a.w_most = w_most; a.label = label; a.part = part; a.target = target;
       if (d->dtype == 0) launch_tiles<B16, 1, false>(p, a, st);
       else if (d->dtype == 1) launch_tiles<H16, 1, false>(p, a, st);
       else launch_tiles<H16, 2, false>(p, a, st);
@@ -990,7 +1050,7 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
   return (int)hipGetLastError();
 }
 
-extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* weight, const void* state, size_t state_bytes, const float* dloss, void* ws,
+extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* weight, void* state, size_t state_bytes, const float* dloss, void* ws,
                             size_t ws_bytes, void* dx, void* dw, void* stream) {
   LossPlan p;
   if (int rc = loss_plan(d, weight, p)) return rc;
@@ -998,50 +1058,47 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
   if (misaligned({x, weight, dx, dw}, d->dtype == 2 ? 4 : 2) || misaligned({state, ws}, 256) || misaligned({dloss}, 4)) return NSA_E_ARG;
   if (state_bytes < p.state || ws_bytes < p.bwd) return NSA_E_WORKSPACE;
   hipStream_t st = (hipStream_t)stream;
-  const char* s = (const char*)state;
-  char* w = (char*)ws;
-  const unsigned* kept = (const unsigned*)s;
-  unsigned* cells = (unsigned*)(w + p.b_cells);
+  char *s = (char*)state, *w = (char*)ws;
+  unsigned *kept = (unsigned*)s, *cells = (unsigned*)(w + p.b_cells), *g_most = (unsigned*)(w + p.b_most);
   const int *map = (const int*)(s + p.s_map), *place = (const int*)(s + p.s_place), *label = (const int*)(s + p.s_label);
   const unsigned* count = kept + CELL_ROWS;
   float* g = (float*)(w + p.b_g);
   const int each = d->dtype == 2 ? 4 : 2, tile = p.size == WIDE ? 256 : 128, tiles_m = (p.kp + tile - 1) / tile;
-  hipLaunchKernelGGL(loss_weights_kernel, dim3(1), dim3(1024), 0, st, dloss, (int)d->reduction, count, map, g, cells, tiles_m, tile,
-                     std::min(p.bwd_rows, (int)up(d->vocab, 64)), d->dtype == 0 && p.size != FEW ? kept + CELLS : nullptr);
-  // All operands in fp16: x once, w with each piece.  Magnitudes: those the forward has found, else here.
-  const bool have = p.size != FEW, both = have && d->dtype == 2;
-  const unsigned *xc = d->dtype == 1 ? nullptr : both ? kept + CELL_X : cells + CELL_X, *wc = d->dtype == 1 ? nullptr : both ? kept + CELL_W : cells + CELL_W;
-  if (d->dtype == 0) {
-    if (!have) largest<B16>(x, d->x_stride, p.n, d->dim, map, count, cells + CELL_X, st);
-    largest<B16>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
-  } else if (d->dtype == 2 && !have) {
-    largest<float>(x, d->x_stride, p.n, d->dim, map, count, cells + CELL_X, st);
-    largest<float>(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, cells + CELL_W, st);
-  }
+  // All operands in fp16: x once, w with each piece.  Magnitudes: those the forward has found, else here (into the state as well: the same each time).
+  const bool have = p.size != FEW, scaled = d->dtype != 1;
+  unsigned *x_found = kept + CELLS, *w_found = x_found + 16 * kMost;
+  const unsigned *x_most = scaled ? x_found : nullptr, *w_most = scaled ? w_found : nullptr;
+  LossBegin b{};
+  if (scaled && !have) b.of[0] = most_to(x, d->x_stride, p.n, d->dim, map, count, x_found);
+  if (scaled && !(have && d->dtype == 2)) b.of[1] = most_to(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, w_found);
+  b.dloss = dloss; b.reduction = d->reduction; b.map = map; b.count = count; b.g = g; b.most = g_most;
+  begin(d, b, (p.n + 1023) / 1024, st);
   const long x_plane = (long)p.npad * p.kp;
   void* xg = w + p.b_x;
-  if (d->dtype == 0) planes<B16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, xc, xg, x_plane, st);
-  else if (d->dtype == 2) planes<float, H16, 2>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, xc, xg, x_plane, st);
-  else if (p.grad_P == 2) planes<H16, H16, 2>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, xg, x_plane, st);
-  else planes<H16, H16, 1>(x, d->x_stride, p.n, p.n, d->dim, p.kp, map, count, nullptr, xg, x_plane, st);
   LossGradArgs q{};
   q.kp = p.kp; q.count = count; q.g_cell = cells + CELL_G; q.tiles_m = tiles_m; q.slices = cells + CELL_SLICES;
-  q.x = (const H16*)xg; q.x_plane = x_plane; q.x_cell = xc; q.w = (const H16*)(w + p.b_w); q.w_cell = wc; q.sums = (float*)(w + p.b_dx);
+  q.x = (const H16*)xg; q.x_plane = x_plane; q.x_most = x_most; q.w = (const H16*)(w + p.b_w); q.w_most = w_most; q.sums = (float*)(w + p.b_dx);
   for (long v0 = 0; v0 < d->vocab; v0 += p.bwd_rows) {
     LossTileArgs a{};
     a.v0 = (int)v0;
     a.vend = (int)std::min<long>(d->vocab, v0 + p.bwd_rows);
     const int entries = a.vend - a.v0, ld = (int)up(entries, 64);
     const long w_plane = (long)p.kp * ld;
-    const char* from = (const char*)weight + v0 * d->w_stride * each;
     void* wg = w + p.b_w;
-    if (d->dtype == 0) planes<B16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, wg, w_plane, st);
-    else if (d->dtype == 2) planes<float, H16, 2>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, wc, wg, w_plane, st);
-    else if (p.grad_P == 2) planes<H16, H16, 2>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, nullptr, wg, w_plane, st);
-    else planes<H16, H16, 1>(from, d->w_stride, entries, entries, d->dim, p.kp, nullptr, nullptr, nullptr, wg, w_plane, st);
+    LossCopy c{};
+    c.kp = p.kp;
+    if (v0 == 0) {
+      c.of[0] = rows_to(p, x, d->x_stride, p.n, d->dim, map, count, x_most, xg, x_plane);
+      c.most = g_most; c.count = count; c.cells = cells; c.tiles_m = tiles_m; c.tile = tile; c.piece = std::min(p.bwd_rows, (int)up(d->vocab, 64));
+    }
+    c.of[1] = rows_to(p, (const char*)weight + v0 * d->w_stride * each, d->w_stride, entries, d->dim, nullptr, nullptr, w_most, wg, w_plane);
+    if (d->dtype == 0) copy<B16, H16, 1>(c, st);
+    else if (d->dtype == 2) copy<float, H16, 2>(c, st);
+    else if (p.grad_P == 2) copy<H16, H16, 2>(c, st);
+    else copy<H16, H16, 1>(c, st);
     a.w = wg; a.w_ld = p.kp; a.w_plane = w_plane;
     a.x = xg; a.x_plane = x_plane; a.kp = p.kp; a.n = p.n; a.npad = p.npad;
-    a.count = count; a.x_cell = xc; a.w_cell = wc; a.label = label;
+    a.count = count; a.x_most = x_most; a.w_most = w_most; a.label = label;
     a.norm = (const float2*)(s + p.s_norm); a.own = (const float*)(s + p.s_own); a.g = g; a.g_cell = cells + CELL_G;
     a.grad = (H16*)(w + p.b_grad); a.grad_plane = (long)p.npad * ld; a.grad_ld = ld;
     if (p.grad_P == 2) launch_tiles<H16, 2, true>(p, a, st);

@@ -2650,7 +2650,7 @@ def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_i
 @linear_cross_entropy_fwd.register_fake
 def _(x, weight, labels, ignore_index, reduction):
     n = x.shape[0]
-    state = 1280 + 24 * 64 * ((n + 63) // 64 if n > 0 else 1)      # (nsa_loss_workspace_bytes)
+    state = 2304 + 24 * 64 * ((n + 63) // 64 if n > 0 else 1)      # (nsa_loss_workspace_bytes)
     return x.new_empty((n,) if reduction == 0 else (), dtype=torch.float32), x.new_empty((state,), dtype=torch.uint8)
 
 
