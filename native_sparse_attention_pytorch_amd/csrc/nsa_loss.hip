@@ -17,7 +17,7 @@
 // G in fp16: probabilities and g_i / max |g| are at most 1, so G 2^14 / max |g| has 11 bits down to 2^-28 of the largest, against bf16's 8: with
 // a bf16 G the gradients of a bf16 model were off by 1.4 times their own rounding, with this by 1.01.  The other operands of those
 // products, w and x, are scaled by powers of two into fp16's range and lose nothing that is above 2^-29 of their largest value.
-// fp32 operands are two fp16 planes each, G too (nsa_tiles.hpp).
+// fp32 operands are two fp16 planes each, G too (nsa_tiles.hpp); fp16 ones are exact in one, and G two where that is cheap (loss_plan).
 #include <algorithm>
 #include <cmath>
 #include "nsa_tiles.hpp"
@@ -43,7 +43,7 @@ enum LossSize { FEW, TINY, MIDDLE, WIDE };
 
 struct LossPlan {
   int n, npad, kp;                        // rows and their capacity (a multiple of 64), features padded to 64
-  int P, grad_P;                          // planes of the operands of the forward, of the backward
+  int P, grad_P;                          // planes of the operands of the forward, of the backward (ONE_BY_TWO: one of w and x, two of G)
   LossSize size;
   bool in_place;                          // the forward reads the weight where it lies
   int tile, part;                         // entries of the vocabulary of a tile, of a pair (maximum, sum)
@@ -67,9 +67,10 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.npad = (int)up(std::max<size_t>(p.n, 1), 64);
   p.kp = (int)up(d->dim, 64);
   p.P = d->dtype == 2 ? 2 : 1;
-  // (fp16 results have as many bits as an fp16 G: over many rows its rounding adds as much as theirs, but a few rows' gradients hang on single
-  // entries of G, and their second halves cost nothing beside the weight's one pass)
-  p.grad_P = d->dtype == 2 || (d->dtype == 1 && p.n <= 32) ? 2 : 1;
+  // fp16 results have as many bits as an fp16 G, and hang on single entries of it, the labels': its rounding makes them 1.41 times as far off as
+  // their own alone.  Two halves of G cost a product more for dx and dw each; they are taken where that is little (2^33: 35 us of products) or
+  // where few rows make 1.41 as likely to be 1.6.  (2047 rows, 768 features, 32000 entries: 483 us and dw 1.2 times its own rounding off, 750 with two halves.)
+  p.grad_P = d->dtype == 2 ? 2 : d->dtype == 1 && (p.n <= 256 || (double)p.n * d->vocab * d->dim < 8589934592.0) ? ONE_BY_TWO : 1;
   // The tiles whose rounds end first: time of a round on all places, in us for each feature and beside that (products measured from 512 to 4096
   // features, the maxima and sums of a tile beside them).  256 x 256 tiles have no registers for sums in pieces (TileProduct::PIECES), so long
   // fp32 rows do without them: at 2066 features the gradients were 2.8e-6 off, 7 times as much as fp32 products by the library.
@@ -91,8 +92,9 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.in_place = d->dtype != 2 && d->dim % 8 == 0 && d->dim >= 64 && d->w_stride % 8 == 0 && d->w_stride < (1 << 20) && ((uintptr_t)weight & 15) == 0;
   const size_t v256 = up(d->vocab, 256), v64 = up(d->vocab, 64), row = (size_t)p.kp * 2;
   p.fwd_rows = (int)std::min(v256, std::max<size_t>(256, ((size_t)256 << 20) / (row * p.P) / 256 * 256));
+  const int planes = p.grad_P == 2 ? 2 : 1, g_planes = p.grad_P == 1 ? 1 : 2;
   // a piece's G: up to 256 MB
-  p.bwd_rows = (int)std::min(v256, std::max<size_t>(1024, ((size_t)256 << 20) / ((size_t)p.grad_P * p.npad * 2) / 1024 * 1024));
+  p.bwd_rows = (int)std::min(v256, std::max<size_t>(1024, ((size_t)256 << 20) / ((size_t)g_planes * p.npad * 2) / 1024 * 1024));
   // gradients: tiles of 256 where the logits have them, else 128; as many slices as give every CU a tile
   const size_t tile = p.size == WIDE ? 256 : 128, piece = std::min<size_t>(p.bwd_rows, v64), last = (v64 - 1) % p.bwd_rows + 1;
   auto w_slices = [&](size_t entries) {
@@ -119,9 +121,9 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.b_cells = take(CELLS * 4);
   p.b_most = take((size_t)(p.npad + 1023) / 1024 * 4);
   p.b_g = take((size_t)p.npad * 4);
-  p.b_x = take(p.npad * row * p.grad_P);
-  p.b_w = take(p.bwd_rows * row * p.grad_P);
-  p.b_grad = take((size_t)p.grad_P * p.npad * p.bwd_rows * 2);
+  p.b_x = take(p.npad * row * planes);
+  p.b_w = take(p.bwd_rows * row * planes);
+  p.b_grad = take((size_t)g_planes * p.npad * p.bwd_rows * 2);
   // (rows of the slices: no more than kSliceTiles tiles of them where there are two or more)
   p.b_dx = take(std::max<size_t>((size_t)p.npad * p.kp, std::min<size_t>((size_t)kMaxSlices * p.npad * p.kp, kSliceTiles * tile * tile)) * 4);
   p.b_dw = take(std::max<size_t>(p.w_splits > 1 ? p.w_splits * piece : 0, p.last_splits > 1 ? p.last_splits * last : 0) * p.kp * 4);
@@ -374,9 +376,9 @@ struct LossTileArgs {
   const float2* norm;                      // maximum, log2 of the sum
   const float *own, *g;                    // the label's G / g
   const unsigned* g_cell;
-  _Float16* grad;                          // [planes][npad][grad_ld]
+  _Float16* grad;                          // [grad_planes][npad][grad_ld]
   long grad_plane;
-  int grad_ld;
+  int grad_ld, grad_planes;
 };
 
 // One tile: TM entries of the vocabulary (registers) by TN tokens (lanes).  GRAD: G of the tile; else its maxima, sums and the labels' logits.
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
     // rows of G up to a multiple of 64 are read as the contraction index of dw
     if (GRAD) {
       const int width = min(Tiles::TM, G.grad_ld - tile.m * Tiles::TM) / 8;
-      for (int i = threadIdx.x; i < Tiles::P * Tiles::TN * width; i += Tiles::THREADS) {
+      for (int i = threadIdx.x; i < G.grad_planes * Tiles::TN * width; i += Tiles::THREADS) {
         const int row = i / width % Tiles::TN, plane = i / width / Tiles::TN;
         *reinterpret_cast<uintx4*>(G.grad + plane * G.grad_plane + (size_t)(n0 + row) * G.grad_ld + tile.m * Tiles::TM + i % width * 8) = uintx4{0u, 0u, 0u, 0u};
       }
@@ -477,7 +479,6 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
             if (m0 + t.row_of(i, e >> 2) + (e & 3) >= G.vend) t.acc[i][j][e] = 0.f;
       }
       if (token >= pad) continue;
-      constexpr int GP = Tiles::P;
 #pragma unroll
       for (int i = 0; i < Tiles::MI; ++i) {
         const int col = tile.m * Tiles::TM + t.wm * PART + 32 * i;
@@ -490,17 +491,13 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float v = t.acc[i][j][4 * (q + u) + e];
-              if (GP == 2) {
-                const Halves s = halves_of(v);
-                hi[u][e] = s.hi;
-                lo[u][e] = s.lo;
-              } else {
-                hi[u][e] = (_Float16)v;
-              }
+              const Halves s = halves_of(v);
+              hi[u][e] = s.hi;
+              lo[u][e] = s.lo;
             }
           _Float16* at = G.grad + (size_t)token * G.grad_ld + col + 8 * q + 8 * (t.lane >> 5);
           *reinterpret_cast<uintx4*>(at) = join_quads(__builtin_bit_cast(uintx2, hi[0]), __builtin_bit_cast(uintx2, hi[1]));
-          if (GP == 2) *reinterpret_cast<uintx4*>(at + G.grad_plane) = join_quads(__builtin_bit_cast(uintx2, lo[0]), __builtin_bit_cast(uintx2, lo[1]));
+          if (G.grad_planes == 2) *reinterpret_cast<uintx4*>(at + G.grad_plane) = join_quads(__builtin_bit_cast(uintx2, lo[0]), __builtin_bit_cast(uintx2, lo[1]));
         }
       }
     }
@@ -878,12 +875,13 @@ template <class T, int P> struct LogitTiles {
   typedef TileProduct<T, P, ROWS, ROWS, 128, 32, 4, 1, 64, P == 2 ? 2 : 4> Few;
 };
 template <int P> struct GradTiles {
-  typedef TileProduct<H16, P, COLUMNS, ROWS, 256, 256, 2, 4, 32, P == 2 ? 2 : 4> WideX;
-  typedef TileProduct<H16, P, COLUMNS, ROWS, 128, 128, 2, 4, P == 2 ? 32 : 64, 4> MiddleX;
-  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 256, 256, 2, 4, 32, P == 2 ? 2 : 4> WideW;
-  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 128, 128, 2, 4, P == 2 ? 32 : 64, 4> MiddleW;
-  typedef TileProduct<H16, P, COLUMNS, ROWS, 128, 128, 2, 4, P == 2 ? 32 : 64, 2> FewX;
-  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 128, 128, 2, 4, P == 2 ? 32 : 64, 2> FewW;
+  static constexpr int WIDE_STAGES = P == 1 ? 4 : P == 2 ? 2 : 3, BK = P == 1 ? 64 : 32, FEW_STAGES = P == ONE_BY_TWO ? 3 : 2;
+  typedef TileProduct<H16, P, COLUMNS, ROWS, 256, 256, 2, 4, 32, WIDE_STAGES> WideX;
+  typedef TileProduct<H16, P, COLUMNS, ROWS, 128, 128, 2, 4, BK, 4> MiddleX;
+  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 256, 256, 2, 4, 32, WIDE_STAGES> WideW;
+  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 128, 128, 2, 4, BK, 4> MiddleW;
+  typedef TileProduct<H16, P, COLUMNS, ROWS, 128, 128, 2, 4, BK, FEW_STAGES> FewX;
+  typedef TileProduct<H16, P, COLUMNS, COLUMNS, 128, 128, 2, 4, BK, FEW_STAGES> FewW;
 };
 
 template <class Tiles, bool GRAD>
@@ -933,16 +931,13 @@ static void products(const LossPlan& p, const LossGradArgs& q, bool dx, hipStrea
   const int tile = p.size == WIDE ? 256 : 128, all = q.tiles_m * ((p.n + tile - 1) / tile);
   const dim3 grid((unsigned)(q.dw_tiles + (dx ? std::max(all, std::min(kMaxSlices * all, kSliceTiles)) : 0))), block(512);
   // few rows: nothing to read ahead, so two work-groups a CU that write in turn (25 rows, 1917 features, 21120 entries in bf16: 36 -> 24 us)
-  if constexpr (!SLICES && !(P == 1 && std::is_same<O, H16>::value))      // (few rows of fp16 have two planes)
+  if constexpr (!SLICES && !(P == 1 && std::is_same<O, H16>::value))      // (few rows of fp16 have two planes of G)
     if (p.size == FEW) {
       hipLaunchKernelGGL((loss_products_kernel<typename T::FewX, typename T::FewW, O, SLICES>), grid, block, 0, st, q);
       return;
     }
-  // (fp16 operands of two planes: few rows only)
-  if constexpr (P == 1 || sizeof(O) == 4) {
-    if (p.size == WIDE) hipLaunchKernelGGL((loss_products_kernel<typename T::WideX, typename T::WideW, O, SLICES>), grid, block, 0, st, q);
-    else hipLaunchKernelGGL((loss_products_kernel<typename T::MiddleX, typename T::MiddleW, O, SLICES>), grid, block, 0, st, q);
-  }
+  if (p.size == WIDE) hipLaunchKernelGGL((loss_products_kernel<typename T::WideX, typename T::WideW, O, SLICES>), grid, block, 0, st, q);
+  else hipLaunchKernelGGL((loss_products_kernel<typename T::MiddleX, typename T::MiddleW, O, SLICES>), grid, block, 0, st, q);
 }
 static void rows_of_slices(const nsa_loss_desc* d, const LossGradArgs& q, const float* sums, int size, int n, const int* place, void* to, hipStream_t st) {
   const dim3 grid(blocks_for((long)n * ((d->dim + 3) / 4)));
@@ -1094,13 +1089,12 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
     c.of[1] = rows_to(p, (const char*)weight + v0 * d->w_stride * each, d->w_stride, entries, d->dim, nullptr, nullptr, w_most, wg, w_plane);
     if (d->dtype == 0) copy<B16, H16, 1>(c, st);
     else if (d->dtype == 2) copy<float, H16, 2>(c, st);
-    else if (p.grad_P == 2) copy<H16, H16, 2>(c, st);
     else copy<H16, H16, 1>(c, st);
     a.w = wg; a.w_ld = p.kp; a.w_plane = w_plane;
     a.x = xg; a.x_plane = x_plane; a.kp = p.kp; a.n = p.n; a.npad = p.npad;
     a.count = count; a.x_most = x_most; a.w_most = w_most; a.label = label;
     a.norm = (const float2*)(s + p.s_norm); a.own = (const float*)(s + p.s_own); a.g = g; a.g_cell = cells + CELL_G;
-    a.grad = (H16*)(w + p.b_grad); a.grad_plane = (long)p.npad * ld; a.grad_ld = ld;
+    a.grad = (H16*)(w + p.b_grad); a.grad_plane = (long)p.npad * ld; a.grad_ld = ld; a.grad_planes = p.grad_P == 1 ? 1 : 2;
     if (p.grad_P == 2) launch_tiles<H16, 2, true>(p, a, st);
     else launch_tiles<H16, 1, true>(p, a, st);
 
@@ -1112,11 +1106,12 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
     char* to = (char*)dw + v0 * d->dim * each;
     q.dw = slices ? w + p.b_dw : to; q.dw_ld = q.dim = slices ? p.kp : d->dim;
     if (slices && p.grad_P == 1) products<1, float, true>(p, q, dx, st);
-    else if (slices) products<2, float, true>(p, q, dx, st);
+    else if (slices && p.grad_P == 2) products<2, float, true>(p, q, dx, st);
+    else if (slices) products<ONE_BY_TWO, float, true>(p, q, dx, st);
     else if (d->dtype == 0) products<1, B16, false>(p, q, dx, st);
     else if (d->dtype == 2) products<2, float, false>(p, q, dx, st);
-    else if (p.grad_P == 2) products<2, H16, false>(p, q, dx, st);
-    else products<1, H16, false>(p, q, dx, st);
+    else if (p.grad_P == 1) products<1, H16, false>(p, q, dx, st);
+    else products<ONE_BY_TWO, H16, false>(p, q, dx, st);
     if (slices) rows_of_slices(d, q, (const float*)(w + p.b_dw), entries, entries, nullptr, to, st);
   }
   if (dx) rows_of_slices(d, q, (const float*)(w + p.b_dx), 0, p.n, place, dx, st);

@@ -337,19 +337,22 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_update_kernel(const 
 // A matrix of up to 64 rows that fits a CU's LDS, all steps in one work-group, in fp32 throughout (32 x 32 x 2 products): the launches of the
 // other kernels would be all of its time (a 24 x 512 matrix took 99 us with them), and sums this short show that halves have a bit or two less
 // than fp32.  X lies in LDS for the whole time; a step is A (the columns of X split over the waves and summed), B, and X, 32 columns a
-// wave, in place.
-constexpr int kSmallFloats = 40960 - 4 * 8, kSmallWaves = 8, kSmallPart = kSmallWaves * 1024;
+// wave, in place.  A and B lie there in blocks of 32 x 32 as the matrix instructions leave them, four values of a lane together: what is a
+// result's element of row 8 g + 4 h + e in column l is the operand's of column 8 g + 4 h + e in row l, and both are symmetric.
+constexpr int kSmallFloats = 40960 - 4 * 8, kSmallWaves = 8, kSmallPart = kSmallWaves * 1024;      // (floats)
 __host__ __device__ inline int up32(int v) { return (v + 31) / 32 * 32; }
 __host__ __device__ inline bool newton_small(int m, int n) {
   if (m > 64) return false;
   const int M = up32(m);
-  return (long)M * (up32(n) + 4) + 2 * M * (M + 4) + kSmallPart <= kSmallFloats;
+  return (long)M * (up32(n) + 4) + 2 * M * M + kSmallPart <= kSmallFloats;
 }
 __device__ __forceinline__ floatx16 mma_f32(floatx4 a, floatx4 b, floatx16 c) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
   return c;
 }
+
+__device__ __forceinline__ floatx4 quad(const floatx16& v, int g) { return floatx4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]}; }
 
 template <class S>
 __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const NewtonTable G, const NewtonStep T, int steps, float eps) {
@@ -358,8 +361,9 @@ __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const Ne
   const NewtonMatrix K = G.of[blockIdx.x];
   const NewtonPlanes L(K.rows, K.cols);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, l = lane & 31;
-  const int M = up32(L.m), N = up32(L.n), xp = N + 4, ap = M + 4, blocks = (M / 32) * (M / 32), splits = kSmallWaves / blocks;
-  float *x = lds, *A = x + M * xp, *B = A + M * ap, *part = B + M * ap;
+  const int M = up32(L.m), N = up32(L.n), xp = N + 4, side = M / 32, blocks = side * side, splits = kSmallWaves / blocks;
+  float* x = lds;
+  floatx4 *A = reinterpret_cast<floatx4*>(x + M * xp), *B = A + blocks * 256, *part = B + blocks * 256;      // [block][g][lane]
 
   for (int i = tid; i < M * xp; i += 64 * kSmallWaves) x[i] = 0.f;
   __syncthreads();
@@ -391,7 +395,7 @@ __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const Ne
 
   for (int step = 0; step < steps; ++step) {
     {
-      const int blk = wave % blocks, split = wave / blocks, bi = blk / (M / 32), bj = blk % (M / 32), groups = N / 8;
+      const int blk = wave % blocks, split = wave / blocks, bi = blk / side, bj = blk % side, groups = N / 8;
       const int per = (groups + splits - 1) / splits;
       const float *xi = x + (32 * bi + l) * xp + 4 * h, *xj = x + (32 * bj + l) * xp + 4 * h;
       floatx16 acc = zero_acc();
@@ -399,26 +403,25 @@ __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const Ne
       for (int g = split * per; g < min(groups, (split + 1) * per); ++g)
         acc = mma_f32(*reinterpret_cast<const floatx4*>(xi + 8 * g), *reinterpret_cast<const floatx4*>(xj + 8 * g), acc);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) part[wave * 1024 + e * 64 + lane] = acc[e];
+      for (int g = 0; g < 4; ++g) part[wave * 256 + g * 64 + lane] = quad(acc, g);
     }
     __syncthreads();
-    for (int i = tid; i < blocks * 1024; i += 64 * kSmallWaves) {
-      const int blk = i >> 10, e = (i >> 6) & 15, at = i & 1023;
-      float v = 0.f;
-      for (int s = 0; s < splits; ++s) v += part[(s * blocks + blk) * 1024 + at];
-      A[(blk / (M / 32) * 32 + 8 * (e >> 2) + 4 * ((i >> 5) & 1) + (e & 3)) * ap + blk % (M / 32) * 32 + (i & 31)] = v;
+    for (int i = tid; i < blocks * 256; i += 64 * kSmallWaves) {
+      floatx4 v = part[i];
+      for (int s = 1; s < splits; ++s) v += part[s * blocks * 256 + i];
+      A[i] = v;
     }
     __syncthreads();
     if (wave < blocks) {
-      const int bi = wave / (M / 32), bj = wave % (M / 32);
-      const float *ai = A + (32 * bi + l) * ap + 4 * h, *aj = A + (32 * bj + l) * ap + 4 * h;
+      const int bi = wave / side, bj = wave % side;
       floatx16 acc = zero_acc();
-#pragma unroll 4
-      for (int g = 0; g < M / 8; ++g) acc = mma_f32(*reinterpret_cast<const floatx4*>(ai + 8 * g), *reinterpret_cast<const floatx4*>(aj + 8 * g), acc);
+      for (int bk = 0; bk < side; ++bk)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int at = (32 * bi + 8 * (e >> 2) + 4 * h + (e & 3)) * ap + 32 * bj + l;
-        B[at] = __builtin_fmaf(T.b, A[at], T.c * acc[e]);
+        for (int g = 0; g < 4; ++g) acc = mma_f32(A[(bk * side + bi) * 256 + g * 64 + lane], A[(bk * side + bj) * 256 + g * 64 + lane], acc);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int at = wave * 256 + g * 64 + lane;
+        B[at] = T.b * A[at] + T.c * quad(acc, g);
       }
     }
     __syncthreads();
@@ -432,11 +435,11 @@ __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const Ne
         for (int e = 0; e < 4; ++e) v[e] = col[(8 * g + 4 * h + e) * xp];
 #pragma unroll
         for (int bi = 0; bi < 2; ++bi)
-          if (bi < M / 32) acc[bi] = mma_f32(*reinterpret_cast<const floatx4*>(B + (32 * bi + l) * ap + 8 * g + 4 * h), v, acc[bi]);
+          if (bi < side) acc[bi] = mma_f32(B[((g >> 2) * side + bi) * 256 + (g & 3) * 64 + lane], v, acc[bi]);
       }
 #pragma unroll
       for (int bi = 0; bi < 2; ++bi)
-        if (bi < M / 32) {
+        if (bi < side) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float* p = col + (32 * bi + 8 * (e >> 2) + 4 * h + (e & 3)) * xp;

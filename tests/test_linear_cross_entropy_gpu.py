@@ -479,3 +479,15 @@ def test_weights_past_4_gigabytes(n):
             exact = G.t().contiguous() @ x6
             _within(dw[60000 * i:60000 * i + len(p)], (exact, off.t().contiguous() @ size + 2 ** -20 * (G.t().contiguous().abs() @ size) + 2 ** -8 * exact.abs()), "dw")
     _within(dx, (want, tol + 2 ** -8 * want.abs()), "dx")
+
+
+@pytest.mark.parametrize("n,d,v", [(20, 130, 400), (90, 200, 1000), (257, 64, 2000)])
+def test_fp16_gradients_are_off_by_their_rounding(n, d, v):
+    """G's two halves hold 22 bits, so what is left beside the rounding of the result are fp32 sums: a tenth of it with room."""
+    from native_sparse_attention_pytorch_amd import ops
+    x, w, labels, weights = _inputs(n, d, v, F16, seed=11)
+    x.requires_grad_(), w.requires_grad_()
+    got = torch.autograd.grad(ops.linear_cross_entropy(x, w, labels, reduction="none"), (x, w), weights)
+    _, (dx, _), (dw, _) = _exact(x.detach(), w.detach(), labels, "none", weights)
+    for g, e in zip(got, (dx, dw)):
+        assert float((g.double() - e).norm()) <= 1.1 * float((e.to(F16).double() - e).norm())
