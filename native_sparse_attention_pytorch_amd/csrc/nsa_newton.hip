@@ -335,7 +335,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void newton_update_kernel(const 
 // ------------------------------------------------------------------------------------ small matrices
 
 // A matrix of up to 64 rows that fits a CU's LDS, all steps in one work-group, in fp32 throughout (32 x 32 x 2 products): the launches of the
-// other kernels would be all of its time (a 24 x 512 matrix took 99 us with them), and sums this short show that halves have a bit or two less
+// other kernels would be all of its time (a 24 x 512 matrix took 99 us with them, 39 so), and sums this short show that halves have a bit or two less
 // than fp32.  X lies in LDS for the whole time; a step is A (the columns of X split over the waves and summed), B, and X, 32 columns a
 // wave, in place.  A and B lie there in blocks of 32 x 32 as the matrix instructions leave them, four values of a lane together: what is a
 // result's element of row 8 g + 4 h + e in column l is the operand's of column 8 g + 4 h + e in row l, and both are symmetric.
@@ -353,6 +353,26 @@ __device__ __forceinline__ floatx16 mma_f32(floatx4 a, floatx4 b, floatx16 c) {
 }
 
 __device__ __forceinline__ floatx4 quad(const floatx16& v, int g) { return floatx4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]}; }
+// X <- a X + B X of 32 columns, from this lane's on.  (An operand's values are those that the result's registers stand for.)
+template <int SIDE>
+__device__ __forceinline__ void small_update(float* col, int xp, const floatx4* B, float a) {
+  floatx16 acc[SIDE];
+  floatx4 v[4 * SIDE];
+#pragma unroll
+  for (int bi = 0; bi < SIDE; ++bi) acc[bi] = zero_acc();
+#pragma unroll
+  for (int g = 0; g < 4 * SIDE; ++g)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[g][e] = col[(8 * g + e) * xp];
+#pragma unroll
+  for (int g = 0; g < 4 * SIDE; ++g)
+#pragma unroll
+    for (int bi = 0; bi < SIDE; ++bi) acc[bi] = mma_f32(B[((g >> 2) * SIDE + bi) * 256 + (g & 3) * 64], v[g], acc[bi]);
+#pragma unroll
+  for (int g = 0; g < 4 * SIDE; ++g)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) col[(8 * g + e) * xp] = __builtin_fmaf(a, v[g][e], acc[g >> 2][4 * (g & 3) + e]);
+}
 
 template <class S>
 __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const NewtonTable G, const NewtonStep T, int steps, float eps) {
@@ -368,19 +388,34 @@ __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const Ne
   for (int i = tid; i < M * xp; i += 64 * kSmallWaves) x[i] = 0.f;
   __syncthreads();
   double sum = 0.0;
-  const unsigned total = K.rows * K.cols, cols = K.cols;
-  for (unsigned first = 0; first < total; first += 8 * 64 * kSmallWaves) {
+  constexpr int THREADS = 64 * kSmallWaves;
+  const int total = K.rows * K.cols;
+  // row and column of every THREADS-th value, one after the other (a division for each was a tenth of the kernel's time)
+  struct Place {
+    int cols, rows_on, cols_on, r, c;
+    __device__ __forceinline__ Place(int at, int cols_) : cols(cols_), rows_on(THREADS / cols_), cols_on(THREADS % cols_), r(at / cols_), c(at % cols_) {}
+    __device__ __forceinline__ void next() {
+      r += rows_on;
+      c += cols_on;
+      if (c >= cols) {
+        c -= cols;
+        ++r;
+      }
+    }
+  };
+  Place from(tid, K.cols), to = from;
+  for (int first = tid; first < total; first += 8 * THREADS) {
     float v[8];      // (eight loads in flight: one by one, 24 rounds of them were a third of the kernel's time)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const unsigned i = first + e * 64 * kSmallWaves + tid, r = i / cols;
-      v[e] = i < total ? (float)((const S*)K.in)[r * K.stride + (i - r * cols)] : 0.f;
+      v[e] = first + e * THREADS < total ? (float)((const S*)K.in)[from.r * K.stride + from.c] : 0.f;
+      from.next();
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const unsigned i = first + e * 64 * kSmallWaves + tid, r = i / cols, c = i - r * cols;
-      if (i < total) x[L.turned ? c * xp + r : r * xp + c] = v[e];
+      if (first + e * THREADS < total) x[L.turned ? to.c * xp + to.r : to.r * xp + to.c] = v[e];
       sum += (double)v[e] * (double)v[e];
+      to.next();
     }
   }
 #pragma unroll
@@ -426,33 +461,17 @@ __global__ __launch_bounds__(64 * kSmallWaves) void newton_small_kernel(const Ne
     }
     __syncthreads();
     for (int cb = wave; cb < N / 32; cb += kSmallWaves) {
-      floatx16 acc[2] = {zero_acc(), zero_acc()};
-      float* col = x + 32 * cb + l;
-#pragma unroll 4
-      for (int g = 0; g < M / 8; ++g) {
-        floatx4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = col[(8 * g + 4 * h + e) * xp];
-#pragma unroll
-        for (int bi = 0; bi < 2; ++bi)
-          if (bi < side) acc[bi] = mma_f32(B[((g >> 2) * side + bi) * 256 + (g & 3) * 64 + lane], v, acc[bi]);
-      }
-#pragma unroll
-      for (int bi = 0; bi < 2; ++bi)
-        if (bi < side) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float* p = col + (32 * bi + 8 * (e >> 2) + 4 * h + (e & 3)) * xp;
-            *p = __builtin_fmaf(T.a, *p, acc[bi][e]);
-          }
-        }
+      float* col = x + 32 * cb + l + 4 * h * xp;
+      if (side == 1) small_update<1>(col, xp, B + lane, T.a);
+      else small_update<2>(col, xp, B + lane, T.a);
     }
     __syncthreads();
   }
+  Place out(tid, K.cols);
 #pragma unroll 4
-  for (unsigned i = tid; i < total; i += 64 * kSmallWaves) {
-    const unsigned r = i / cols, c = i - r * cols;
-    ((S*)K.out)[i] = (S)x[L.turned ? c * xp + r : r * xp + c];
+  for (int i = tid; i < total; i += THREADS) {
+    ((S*)K.out)[i] = (S)x[L.turned ? out.c * xp + out.r : out.r * xp + out.c];
+    out.next();
   }
 }
 
