@@ -522,8 +522,7 @@ int nsa_decode_prep(const void* q, const int64_t* q_stride, const void* k, const
  *   x [rows, dim] with row stride x_stride, weight [vocab, dim] with row stride w_stride, both of `dtype`; labels [rows] contiguous; loss: fp32, one
  *   value, or [rows] with reduction 0.  Rows whose label is ignore_index count nothing: loss 0 (reduction 0), gradient 0, and what
  *   they hold is not read.  Any other label outside [0, vocab) makes its loss NaN, and the gradients with it.  Mean of no rows: NaN.
- *   `state` is written by nsa_loss_fwd and read by nsa_loss_bwd (any number of times, at once too: what that adds to it is the same each time); ws is
- *   dead after either call.
+ *   `state` is written by nsa_loss_fwd and read by nsa_loss_bwd (any number of times); ws is dead after either call.
  *   dloss: fp32, as loss; dx [rows, dim], dw [vocab, dim] contiguous, of `dtype`; either may be NULL.  rows >= 1 for the backward.
  * Sums in fp32; fp32 operands as two fp16 halves each (22 bits; what is below 2^-18 of a matrix's largest value is kept to 2^-40 of that), results
  * rounded once.  Infinities and NaN among the weights may make NaN of any logit of their entry.  The order of the additions depends on sizes, the
@@ -541,14 +540,15 @@ typedef struct nsa_loss_desc {
 int nsa_loss_workspace_bytes(const nsa_loss_desc* d, const void* weight, size_t* state_bytes, size_t* fwd_bytes, size_t* bwd_bytes);
 int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* weight, const void* labels, void* state, size_t state_bytes,
                  void* ws, size_t ws_bytes, float* loss, void* stream);
-int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* weight, void* state, size_t state_bytes, const float* dloss,
+int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* weight, const void* state, size_t state_bytes, const float* dloss,
                  void* ws, size_t ws_bytes, void* dx, void* dw, void* stream);
 
 /* Orthogonalised updates (no counterpart in the reference): of each of `many` matrices, X = in / (|in| + eps) with the Frobenius norm, then `steps`
  * times X <- a X + (b A + c A A) X with A = X X^T (X^T X where there are more rows than columns), written to out.
  *   rows, cols: host arrays, any sizes up to 2^20, the smaller one up to 2^15; in, out: host arrays of device addresses, rows of in[k] in_stride[k]
  *   elements apart, out[k] contiguous, alignment that of the type; all of dtype 0 bf16, 1 fp16, 2 fp32.  out[k] may be in[k] where that is
- *   contiguous.  Products of two fp16 halves (22 bits) with fp32 sums, results rounded once: as exact as fp32 products.
+ *   contiguous.  Products of two fp16 halves (22 bits) with fp32 sums, results rounded once: as exact as fp32 products.  The last two steps
+ *   of bf16 results take one half: they are off by up to 1.12 times their own rounding.
  *   Coefficients that take a singular value of [0, 1] past 4 on its way: NSA_E_UNSUPPORTED.  Zero matrices give zeros (eps > 0).
  * The result of a matrix depends on nothing but itself and the sizes of all.  ws: aligned to 256 bytes. */
 int nsa_newton_workspace_bytes(int32_t many, const int32_t* rows, const int32_t* cols, size_t* bytes);

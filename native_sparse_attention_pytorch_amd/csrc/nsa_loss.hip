@@ -26,17 +26,16 @@
 namespace nsa {
 
 constexpr int kGradBits = 14;
-// device words: of the state, the rows that count; of a backward pass, bits of the largest finite |g| and the slices of dx
-enum { CELL_ROWS, CELL_G = 0, CELL_SLICES, CELLS = 64 };
-// Behind those of the state, the bits of the largest finite |x| and |w| that work-groups have found, each in one of 16 words 64 bytes apart: a word
+// device words, of the state and of a backward pass: rows that count; bits of the largest finite |x|, |w| and |g|; slices of dx
+enum { CELL_ROWS, CELL_X, CELL_W, CELL_G, CELL_SLICES, CELLS = 64 };
+// Behind those of the state, for bf16, the bits of the largest finite |x| that work-groups have found, each in one of 16 words 64 bytes apart: one word
 // for all held up the copy of 8184 rows of 512 by 11 us.
-constexpr int kMost = 16;
-__device__ __forceinline__ unsigned most_of(const unsigned* words) {
-  unsigned m = 0;
-#pragma unroll
-  for (int i = 0; i < kMost; ++i) m = max(m, words[16 * i]);
-  return m;
-}
+constexpr int kMost = 16, kParts = 1024;
+// the largest of `count` words is that of a matrix
+struct LossFound {
+  const unsigned* words;
+  int count, stride;
+};
 
 // How logits are made: FEW rows as loss_few_kernel has them, the others by tiles of 64, 128 or 256 (loss_plan)
 enum LossSize { FEW, TINY, MIDDLE, WIDE };
@@ -51,7 +50,7 @@ struct LossPlan {
   int w_splits, last_splits;              // slices of the rows that dw of a piece, of the last one, is summed from
   size_t state, fwd, bwd;                 // bytes
   size_t s_map, s_place, s_label, s_norm, s_own;                            // offsets in the state
-  size_t f_part, f_target, f_loss, f_x, f_w;                           // in the forward's workspace
+  size_t f_part, f_target, f_loss, f_x, f_w, f_most;                         // in the forward's workspace
   size_t b_cells, b_most, b_g, b_x, b_w, b_grad, b_dx, b_dw;                   // in the backward's
 };
 
@@ -102,7 +101,7 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   };
   p.w_splits = w_slices(piece);
   p.last_splits = w_slices(last);
-  size_t at = CELLS * 4 + 2 * kMost * 64;
+  size_t at = CELLS * 4 + kMost * 64;
   auto take = [&](size_t bytes) { const size_t here = at; at = up(at + bytes, 256); return here; };
   p.s_map = take((size_t)p.npad * 4);
   p.s_place = take((size_t)p.npad * 4);
@@ -116,10 +115,11 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.f_loss = take((size_t)p.npad * 4);
   p.f_x = take(p.size == FEW ? 0 : p.npad * row * p.P);
   p.f_w = take(p.size == FEW || p.in_place ? 0 : p.fwd_rows * row * p.P);
+  p.f_most = take(d->dtype == 2 ? 2 * kParts * 4 : 0);
   p.fwd = at;
   at = 0;
   p.b_cells = take(CELLS * 4);
-  p.b_most = take((size_t)(p.npad + 1023) / 1024 * 4);
+  p.b_most = take((2 * kParts + (size_t)(p.npad + 1023) / 1024) * 4);
   p.b_g = take((size_t)p.npad * 4);
   p.b_x = take(p.npad * row * planes);
   p.b_w = take(p.bwd_rows * row * planes);
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(const void* labels, int 
     }
   }
   if (blockIdx.x == gridDim.x - 1 && tid == 0) cells[CELL_ROWS] = (unsigned)total;
-  if (blockIdx.x == 0 && tid < 2 * kMost) cells[CELLS + 16 * tid] = 0;
+  if (blockIdx.x == 0 && tid < kMost) cells[CELLS + 16 * tid] = 0;
 }
 
 // up to 8 values of a row, zeros past its end
@@ -199,14 +199,21 @@ __device__ __forceinline__ unsigned finite_bits(float v) {
   const unsigned u = __builtin_bit_cast(unsigned, v) & 0x7fffffffu;
   return u < 0x7f800000u ? u : 0u;
 }
-// the largest of the work-group's values, in thread 0
+// the largest of the work-group's values
 __device__ __forceinline__ unsigned largest_of(unsigned best) {
   __shared__ unsigned best_s[4];
+  __syncthreads();
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) best = max(best, (unsigned)__shfl_xor((int)best, o));
   if ((threadIdx.x & 63) == 0) best_s[threadIdx.x >> 6] = best;
   __syncthreads();
   return max(max(best_s[0], best_s[1]), max(best_s[2], best_s[3]));
+}
+__device__ __forceinline__ unsigned largest_of(const LossFound& f) {
+  if (f.count == 1) return *f.words;
+  unsigned best = 0;
+  for (int i = threadIdx.x; i < f.count; i += 256) best = max(best, f.words[i * f.stride]);
+  return largest_of(best);
 }
 // Into one of `words`.  (Whoever finds a larger one there already has nothing to say: with an atomic a wave, 16384 of them on one address, the
 // kernel took 100 us for 8 MB.)
@@ -216,14 +223,14 @@ __device__ __forceinline__ void largest_into(unsigned best, unsigned* words, int
   if (threadIdx.x == 0 && best > __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(word, best);
 }
 
-// A matrix, or the rows of it that map names, whose largest finite |value| is to be known: `words` are zero, or hold such values of it
+// A matrix, or the rows of it that map names, whose largest finite |value| is to be known: that of each work-group's part
 struct LossMost {
   const void* src;
   long ld;
   int rows, cols;
   const int* map;
   const unsigned* count;
-  unsigned* words;
+  unsigned* parts;
   int blocks;
 };
 struct LossBegin {
@@ -274,18 +281,20 @@ __global__ __launch_bounds__(256) void loss_begin_kernel(const LossBegin G) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) best = max(best, finite_bits(v[e]));
   }
-  largest_into(best, M.words, block);
+  best = largest_of(best);
+  if (threadIdx.x == 0) M.parts[block] = best;
 }
 
 // Rows (named by map, or all) as planes of kp columns, those past `cols` zero; rows past the last one up to a multiple of 64 zero too.
-// words: the values are scaled below 2^15 by the power of two that suits the largest of those.  most: their own largest goes there.  back: the
-// last 64 columns end with the row's last value, `back` zeros before what is left (TileProduct::run).
+// found: the values are scaled below 2^15 by the power of two that suits the largest (none: they are not).  most: their own largest goes there.
+// back: the last 64 columns end with the row's last value, `back` zeros before what is left (TileProduct::run).
 struct LossRows {
   const void* src;
   long ld;
   int rows, cols;
   const int* map;
-  const unsigned *count, *words;
+  const unsigned* count;
+  LossFound found;
   void* dst;
   long plane;
   unsigned* most;
@@ -294,16 +303,24 @@ struct LossRows {
 struct LossCopy {
   LossRows of[2];
   int kp;
-  // the first of a backward pass: the largest of the weights, and the slices of a piece's entries that dx is summed from
-  const unsigned *most, *count;
+  // The first copy of a pass: one more work-group leaves the largest of both matrices here, and in a backward pass that of the weights (`most`: of
+  // each 1024) and the slices of a piece's entries that dx is summed from
   unsigned* cells;
+  const unsigned *most, *count;
   int tiles_m, tile, piece;
 };
 // Slices of dx: those whose rounds on 256 CUs end first, where a tile's beginning and end, and its share of the sum of slices, cost as much as 512
 // entries.  The rows that count decide, so they are chosen here.  (8192 rows, 40 % of them ignored, 1024 features, 50021 entries: 80 tiles in 2 slices
 // as for all rows 695 us, in 3 of them 600.)
 __device__ __forceinline__ void loss_cells(const LossCopy& G) {
-  const int live = (int)*G.count, tid = threadIdx.x;
+  const int tid = threadIdx.x;
+  for (int i = 0; i < 2; ++i)
+    if (G.of[i].found.words != nullptr) {
+      const unsigned best = largest_of(G.of[i].found);
+      if (tid == 0) G.cells[i == 0 ? CELL_X : CELL_W] = best;
+    }
+  if (G.most == nullptr) return;
+  const int live = (int)*G.count;
   unsigned best = 0;
   for (int i = tid; i < (live + 1023) / 1024; i += 256) best = max(best, G.most[i]);
   best = largest_of(best);
@@ -317,6 +334,8 @@ __device__ __forceinline__ void loss_cells(const LossCopy& G) {
     if (tid == 0) G.cells[CELL_SLICES] = (unsigned)(time & 63);
   }
 }
+// (four times 8 values a thread: with one, finding the scale was a fifth of the time)
+constexpr int kCopies = 4;
 template <class S, class D, int P>
 __global__ __launch_bounds__(256) void loss_planes_kernel(const LossCopy G) {
   if (G.cells != nullptr && (int)blockIdx.x == G.of[0].blocks + G.of[1].blocks) {
@@ -325,38 +344,49 @@ __global__ __launch_bounds__(256) void loss_planes_kernel(const LossCopy G) {
   }
   const bool second = (int)blockIdx.x >= G.of[0].blocks;
   const LossRows& M = G.of[second];
-  const unsigned block = blockIdx.x - (second ? G.of[0].blocks : 0), per = G.kp / 8, i = block * 256 + threadIdx.x;      // (below 2^31: loss_plan)
-  const int live = M.count != nullptr ? (int)*M.count : M.rows;
-  const int r = (int)(i / per), c = (int)(i % per) * 8;
-  if (block * 256 / per >= (unsigned)(live + 63) / 64 * 64) return;
-  float v[8];
+  const unsigned block = blockIdx.x - (second ? G.of[0].blocks : 0), per = G.kp / 8, first = block * kCopies * 256 + threadIdx.x;      // (below 2^31: loss_plan)
+  const int live = M.count != nullptr ? (int)*M.count : M.rows, pad = (live + 63) / 64 * 64;
+  if (block * kCopies * 256 / per >= (unsigned)pad) return;
+  float v[kCopies][8];
+  unsigned best = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = 0.f;
-  const int from = M.back > 0 && c >= G.kp - 64 ? c - M.back : c;
-  if (r < live && from < M.cols && (from == c || from >= G.kp - 64)) load_values((const S*)M.src + (M.map != nullptr ? M.map[r] : r) * M.ld + from, M.cols - from, v);
+  for (int u = 0; u < kCopies; ++u) {
+    const unsigned i = first + u * 256;
+    const int r = (int)(i / per), c = (int)(i - r * per) * 8, from = M.back > 0 && c >= G.kp - 64 ? c - M.back : c;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
+    if (r < live && from < M.cols && (from == c || from >= G.kp - 64))
+      load_values((const S*)M.src + (M.map != nullptr ? M.map[r] : r) * M.ld + from, M.cols - from, v[u]);
+  }
   if (M.most != nullptr) {
-    unsigned best = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) best = max(best, finite_bits(v[e]));
+    for (int u = 0; u < kCopies; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) best = max(best, finite_bits(v[u][e]));
     largest_into(best, M.most, block);
   }
-  if (r >= (live + 63) / 64 * 64) return;
-  const int shift = M.words != nullptr ? plane_shift(most_of(M.words)) : 0;
-  typename PlaneVec<D>::x8 hi, lo;
+  const int shift = M.found.words != nullptr ? plane_shift(largest_of(M.found)) : 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x = shift != 0 ? __builtin_ldexpf(v[e], shift) : v[e];
-    if constexpr (P == 2) {
-      const Halves s = halves_of(x);
-      hi[e] = s.hi;
-      lo[e] = s.lo;
-    } else {
-      hi[e] = (D)x;
+  for (int u = 0; u < kCopies; ++u) {
+    const unsigned i = first + u * 256;
+    const int r = (int)(i / per), c = (int)(i - r * per) * 8;
+    if (r >= pad) break;
+    typename PlaneVec<D>::x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = shift != 0 ? __builtin_ldexpf(v[u][e], shift) : v[u][e];
+      if constexpr (P == 2) {
+        const Halves s = halves_of(x);
+        hi[e] = s.hi;
+        lo[e] = s.lo;
+      } else {
+        hi[e] = (D)x;
+      }
     }
+    D* to = (D*)M.dst + (long)r * G.kp + c;
+    *reinterpret_cast<decltype(hi)*>(to) = hi;
+    if (P == 2) *reinterpret_cast<decltype(lo)*>(to + M.plane) = lo;
   }
-  D* to = (D*)M.dst + (long)r * G.kp + c;
-  *reinterpret_cast<decltype(hi)*>(to) = hi;
-  if (P == 2) *reinterpret_cast<decltype(lo)*>(to + M.plane) = lo;
 }
 
 // ------------------------------------------------------------------------------------ tiles of logits
@@ -367,7 +397,7 @@ struct LossTileArgs {
   int kp, v0, vend;                        // the piece: entries v0 .. vend - 1
   int tail, back;                          // see TileProduct::run; tail in features
   int n, tiles_m;
-  const unsigned *count, *x_most, *w_most;  // null where the planes are not scaled
+  const unsigned *count, *x_cell, *w_cell;  // cells: null where the planes are not scaled
   const int* label;
   float2* part;                            // [parts][npad]
   float* target;
@@ -409,7 +439,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
   t.run(G.kp / Tiles::BK, 0, G.back > 0 ? G.tail / Tiles::BK : -1, G.back);
 
   constexpr bool SCALED = Tiles::P == 2 || GRAD;
-  const int unscale = SCALED && G.x_most != nullptr ? -(plane_shift(most_of(G.x_most)) + plane_shift(most_of(G.w_most))) : 0;
+  const int unscale = SCALED && G.x_cell != nullptr ? -(plane_shift(*G.x_cell) + plane_shift(*G.w_cell)) : 0;
   const bool cut = m0 + Tiles::TM > G.vend;      // entries past the last one
   constexpr int PART = Tiles::TM / Tiles::WM;
   const int g_shift = GRAD ? kGradBits - plane_exponent(*G.g_cell) : 0;
@@ -545,7 +575,6 @@ __global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
       G.losses[lane] = 0.f;
     }
     if (lane == 0) G.cells[CELL_ROWS] = (unsigned)live;
-    if (lane < 2 * kMost) G.cells[CELLS + 16 * lane] = 0;
   }
   if (live == 0) return;
   __syncthreads();
@@ -749,7 +778,7 @@ struct LossGradArgs {
   const _Float16 *grad, *w, *x;       // G [npad][grad_ld]; w [piece][kp]; x [npad][kp]
   long grad_plane, w_plane, x_plane;
   int grad_ld, kp, tiles_m, entries;
-  const unsigned *count, *w_most, *x_most, *g_cell;
+  const unsigned *count, *w_cell, *x_cell, *g_cell;
   // dx
   float* sums;                        // [slices][live rows up to a multiple of 64][kp]
   int first;                          // first piece
@@ -777,7 +806,7 @@ __device__ __forceinline__ void loss_dx(const LossGradArgs& G, char* shared) {
   t.operand_b(G.grad, G.grad_plane, G.grad_ld, n0, live);
   t.run(steps, from);
   // (all pieces share the power of two)
-  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.w_most != nullptr ? plane_shift(most_of(G.w_most)) : 0);
+  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.w_cell != nullptr ? plane_shift(*G.w_cell) : 0);
   float* sums = G.sums + (size_t)split * ((live + 63) / 64 * 64) * G.kp;
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j)
@@ -805,7 +834,7 @@ __device__ __forceinline__ void loss_dw(const LossGradArgs& G, char* shared) {
   } else {
     t.run(steps);
   }
-  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.x_most != nullptr ? plane_shift(most_of(G.x_most)) : 0);
+  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.x_cell != nullptr ? plane_shift(*G.x_cell) : 0);
   O* dw = (O*)G.dw + (SLICES ? (size_t)split * G.entries * G.dw_ld : 0);
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j)
@@ -906,18 +935,20 @@ static bool misaligned(std::initializer_list<const void*> all, size_t to) {
 }
 static unsigned blocks_for(long work) { return (unsigned)std::max<long>(1, (work + 255) / 256); }
 
-static LossMost most_to(const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, unsigned* words) {
-  return LossMost{src, ld, rows, cols, map, count, words, (int)std::min(1024u, blocks_for((long)rows * ((cols + 7) / 8)))};
+static LossMost most_to(const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, unsigned* parts) {
+  return LossMost{src, ld, rows, cols, map, count, parts, (int)std::min<unsigned>(kParts, blocks_for((long)rows * ((cols + 7) / 8)))};
 }
+static LossFound found(const LossMost& m) { return LossFound{m.parts, m.blocks, 1}; }
+static LossFound found(const unsigned* cell) { return LossFound{cell, 1, 0}; }
 static void begin(const nsa_loss_desc* d, const LossBegin& a, int blocks, hipStream_t st) {
   const dim3 grid((unsigned)(a.of[0].blocks + a.of[1].blocks + blocks)), block(256);
   if (d->dtype == 0) hipLaunchKernelGGL((loss_begin_kernel<B16>), grid, block, 0, st, a);
   else if (d->dtype == 1) hipLaunchKernelGGL((loss_begin_kernel<H16>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((loss_begin_kernel<float>), grid, block, 0, st, a);
 }
-static LossRows rows_to(const LossPlan& p, const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, const unsigned* words, void* dst,
+static LossRows rows_to(const LossPlan& p, const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, const LossFound& found, void* dst,
                         long plane, unsigned* most = nullptr, int back = 0) {
-  return LossRows{src, ld, rows, cols, map, count, words, dst, plane, most, back, (int)blocks_for((long)up(rows, 64) * p.kp / 8)};
+  return LossRows{src, ld, rows, cols, map, count, found, dst, plane, most, back, (int)blocks_for(((long)up(rows, 64) * p.kp / 8 + kCopies - 1) / kCopies)};
 }
 template <class S, class D, int P>
 static void copy(const LossCopy& a, hipStream_t st) {
@@ -980,7 +1011,6 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
   float* losses = d->reduction == 0 ? loss : nullptr;
   float2* part = (float2*)(w + p.f_part);
   const unsigned* count = cells + CELL_ROWS;
-  unsigned *x_most = cells + CELLS, *w_most = x_most + 16 * kMost;
   const int each_bytes = d->dtype == 2 ? 4 : 2;
   if (p.size == FEW) {
     LossFewArgs a{x, weight, labels, (long)d->x_stride, (long)d->w_stride, (long)d->ignore_index, (int)d->labels_int64, p.n, d->dim, d->vocab, p.npad,
@@ -997,11 +1027,15 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
     const long x_plane = (long)p.npad * p.kp;
     const int back = p.in_place ? p.kp - d->dim : 0;
     const bool scaled = d->dtype == 2;
+    LossFound of_x{}, of_w{};
     if (scaled) {
+      unsigned* parts = (unsigned*)(w + p.f_most);
       LossBegin a{};
-      a.of[0] = most_to(x, d->x_stride, p.n, d->dim, map, count, x_most);
-      a.of[1] = most_to(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, w_most);
+      a.of[0] = most_to(x, d->x_stride, p.n, d->dim, map, count, parts);
+      a.of[1] = most_to(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, parts + kParts);
       begin(d, a, 0, st);
+      of_x = found(a.of[0]);
+      of_w = found(a.of[1]);
     }
     const int rows = p.in_place ? d->vocab : p.fwd_rows;
     for (long v0 = 0; v0 < d->vocab; v0 += rows) {
@@ -1010,8 +1044,11 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
       a.vend = (int)std::min<long>(d->vocab, v0 + rows);
       LossCopy c{};
       c.kp = p.kp;
-      // (a bf16 backward pass wants to know the largest |x|)
-      if (v0 == 0) c.of[0] = rows_to(p, x, d->x_stride, p.n, d->dim, map, count, scaled ? x_most : nullptr, w + p.f_x, x_plane, d->dtype == 0 ? x_most : nullptr, back);
+      if (v0 == 0) {
+        // (a bf16 backward pass wants to know the largest |x|)
+        c.of[0] = rows_to(p, x, d->x_stride, p.n, d->dim, map, count, of_x, w + p.f_x, x_plane, d->dtype == 0 ? cells + CELLS : nullptr, back);
+        c.cells = scaled ? cells : nullptr;
+      }
       if (p.in_place) {
         a.w = weight;
         a.w_ld = d->w_stride;
@@ -1021,14 +1058,15 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
         a.w = w + p.f_w;
         a.w_ld = p.kp;
         a.w_plane = (long)p.kp * up(a.vend - a.v0, 64);
-        c.of[1] = rows_to(p, (const char*)weight + v0 * d->w_stride * each_bytes, d->w_stride, a.vend - a.v0, d->dim, nullptr, nullptr, scaled ? w_most : nullptr,
+        c.of[1] = rows_to(p, (const char*)weight + v0 * d->w_stride * each_bytes, d->w_stride, a.vend - a.v0, d->dim, nullptr, nullptr, of_w,
                           w + p.f_w, a.w_plane);
       }
       if (d->dtype == 0) copy<B16, B16, 1>(c, st);
       else if (d->dtype == 1) copy<H16, H16, 1>(c, st);
       else copy<float, H16, 2>(c, st);
+      if (scaled) of_w = found(cells + CELL_W);
       a.x = w + p.f_x; a.x_plane = x_plane; a.kp = p.kp; a.n = p.n; a.npad = p.npad;
-      a.count = count; a.x_most = scaled ? x_most : nullptr; a.w_most = w_most; a.label = label; a.part = part; a.target = target;
+      a.count = count; a.x_cell = scaled ? cells + CELL_X : nullptr; a.w_cell = cells + CELL_W; a.label = label; a.part = part; a.target = target;
       if (d->dtype == 0) launch_tiles<B16, 1, false>(p, a, st);
       else if (d->dtype == 1) launch_tiles<H16, 1, false>(p, a, st);
       else launch_tiles<H16, 2, false>(p, a, st);
@@ -1045,7 +1083,7 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
   return (int)hipGetLastError();
 }
 
-extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* weight, void* state, size_t state_bytes, const float* dloss, void* ws,
+extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* weight, const void* state, size_t state_bytes, const float* dloss, void* ws,
                             size_t ws_bytes, void* dx, void* dw, void* stream) {
   LossPlan p;
   if (int rc = loss_plan(d, weight, p)) return rc;
@@ -1053,26 +1091,37 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
   if (misaligned({x, weight, dx, dw}, d->dtype == 2 ? 4 : 2) || misaligned({state, ws}, 256) || misaligned({dloss}, 4)) return NSA_E_ARG;
   if (state_bytes < p.state || ws_bytes < p.bwd) return NSA_E_WORKSPACE;
   hipStream_t st = (hipStream_t)stream;
-  char *s = (char*)state, *w = (char*)ws;
-  unsigned *kept = (unsigned*)s, *cells = (unsigned*)(w + p.b_cells), *g_most = (unsigned*)(w + p.b_most);
+  const char* s = (const char*)state;
+  char* w = (char*)ws;
+  const unsigned* kept = (const unsigned*)s;
+  unsigned *cells = (unsigned*)(w + p.b_cells), *parts = (unsigned*)(w + p.b_most), *g_most = parts + 2 * kParts;
   const int *map = (const int*)(s + p.s_map), *place = (const int*)(s + p.s_place), *label = (const int*)(s + p.s_label);
   const unsigned* count = kept + CELL_ROWS;
   float* g = (float*)(w + p.b_g);
   const int each = d->dtype == 2 ? 4 : 2, tile = p.size == WIDE ? 256 : 128, tiles_m = (p.kp + tile - 1) / tile;
-  // All operands in fp16: x once, w with each piece.  Magnitudes: those the forward has found, else here (into the state as well: the same each time).
-  const bool have = p.size != FEW, scaled = d->dtype != 1;
-  unsigned *x_found = kept + CELLS, *w_found = x_found + 16 * kMost;
-  const unsigned *x_most = scaled ? x_found : nullptr, *w_most = scaled ? w_found : nullptr;
+  // All operands in fp16: x once, w with each piece.  Magnitudes: those the forward has found, else here.
+  const bool scaled = d->dtype != 1;
   LossBegin b{};
-  if (scaled && !have) b.of[0] = most_to(x, d->x_stride, p.n, d->dim, map, count, x_found);
-  if (scaled && !(have && d->dtype == 2)) b.of[1] = most_to(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, w_found);
+  LossFound of_x{}, of_w{};
+  if (scaled && p.size != FEW) {
+    of_x = d->dtype == 2 ? found(kept + CELL_X) : LossFound{kept + CELLS, kMost, 16};
+  } else if (scaled) {
+    b.of[0] = most_to(x, d->x_stride, p.n, d->dim, map, count, parts);
+    of_x = found(b.of[0]);
+  }
+  if (d->dtype == 2 && p.size != FEW) {
+    of_w = found(kept + CELL_W);
+  } else if (scaled) {
+    b.of[1] = most_to(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, parts + kParts);
+    of_w = found(b.of[1]);
+  }
   b.dloss = dloss; b.reduction = d->reduction; b.map = map; b.count = count; b.g = g; b.most = g_most;
   begin(d, b, (p.n + 1023) / 1024, st);
   const long x_plane = (long)p.npad * p.kp;
   void* xg = w + p.b_x;
   LossGradArgs q{};
   q.kp = p.kp; q.count = count; q.g_cell = cells + CELL_G; q.tiles_m = tiles_m; q.slices = cells + CELL_SLICES;
-  q.x = (const H16*)xg; q.x_plane = x_plane; q.x_most = x_most; q.w = (const H16*)(w + p.b_w); q.w_most = w_most; q.sums = (float*)(w + p.b_dx);
+  q.x = (const H16*)xg; q.x_plane = x_plane; q.x_cell = scaled ? cells + CELL_X : nullptr; q.w = (const H16*)(w + p.b_w); q.w_cell = scaled ? cells + CELL_W : nullptr; q.sums = (float*)(w + p.b_dx);
   for (long v0 = 0; v0 < d->vocab; v0 += p.bwd_rows) {
     LossTileArgs a{};
     a.v0 = (int)v0;
@@ -1083,16 +1132,17 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
     LossCopy c{};
     c.kp = p.kp;
     if (v0 == 0) {
-      c.of[0] = rows_to(p, x, d->x_stride, p.n, d->dim, map, count, x_most, xg, x_plane);
+      c.of[0] = rows_to(p, x, d->x_stride, p.n, d->dim, map, count, of_x, xg, x_plane);
       c.most = g_most; c.count = count; c.cells = cells; c.tiles_m = tiles_m; c.tile = tile; c.piece = std::min(p.bwd_rows, (int)up(d->vocab, 64));
     }
-    c.of[1] = rows_to(p, (const char*)weight + v0 * d->w_stride * each, d->w_stride, entries, d->dim, nullptr, nullptr, w_most, wg, w_plane);
+    c.of[1] = rows_to(p, (const char*)weight + v0 * d->w_stride * each, d->w_stride, entries, d->dim, nullptr, nullptr, of_w, wg, w_plane);
     if (d->dtype == 0) copy<B16, H16, 1>(c, st);
     else if (d->dtype == 2) copy<float, H16, 2>(c, st);
     else copy<H16, H16, 1>(c, st);
+    if (scaled) of_w = found(cells + CELL_W);
     a.w = wg; a.w_ld = p.kp; a.w_plane = w_plane;
     a.x = xg; a.x_plane = x_plane; a.kp = p.kp; a.n = p.n; a.npad = p.npad;
-    a.count = count; a.x_most = x_most; a.w_most = w_most; a.label = label;
+    a.count = count; a.x_cell = q.x_cell; a.w_cell = q.w_cell; a.label = label;
     a.norm = (const float2*)(s + p.s_norm); a.own = (const float*)(s + p.s_own); a.g = g; a.g_cell = cells + CELL_G;
     a.grad = (H16*)(w + p.b_grad); a.grad_plane = (long)p.npad * ld; a.grad_ld = ld; a.grad_planes = p.grad_P == 1 ? 1 : 2;
     if (p.grad_P == 2) launch_tiles<H16, 2, true>(p, a, st);

@@ -2650,7 +2650,7 @@ def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_i
 @linear_cross_entropy_fwd.register_fake
 def _(x, weight, labels, ignore_index, reduction):
     n = x.shape[0]
-    state = 2304 + 24 * 64 * ((n + 63) // 64 if n > 0 else 1)      # (nsa_loss_workspace_bytes)
+    state = 1280 + 24 * 64 * ((n + 63) // 64 if n > 0 else 1)      # (nsa_loss_workspace_bytes)
     return x.new_empty((n,) if reduction == 0 else (), dtype=torch.float32), x.new_empty((state,), dtype=torch.uint8)
 
 
@@ -2781,7 +2781,7 @@ def newton_schulz(updates, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315
     """Orthogonalised updates, for optimizers: X = G / (|G| + eps) with the Frobenius norm, then `steps` times X <- a X + (b A + c A A) X, A = X X^T
     (from the shorter side).  `updates`: a matrix, a batch '... m n' of them, or a list or tuple of either, bf16, fp16 or fp32; the result is laid
     out alike, contiguous, in new tensors.  All matrices are in every launch, so a list costs little more than its largest member.  As exact
-    as fp32 products (see nsa_newton.hip), rounded once; no gradients."""
+    as fp32 products (see nsa_newton.hip), rounded once (bf16 results: off by up to 1.12 times their rounding); no gradients."""
     alone = isinstance(updates, Tensor)
     given = [updates] if alone else list(updates)
     coefficients = tuple(float(v) for v in coefficients)

@@ -491,3 +491,14 @@ def test_fp16_gradients_are_off_by_their_rounding(n, d, v):
     _, (dx, _), (dw, _) = _exact(x.detach(), w.detach(), labels, "none", weights)
     for g, e in zip(got, (dx, dw)):
         assert float((g.double() - e).norm()) <= 1.1 * float((e.to(F16).double() - e).norm())
+
+
+@pytest.mark.parametrize("n,dtype", [(20, BF16), (100, BF16), (100, F16), (20, F32), (100, F32)])
+def test_the_operators_are_what_they_are_registered_as(n, dtype):
+    """Arguments are left as they are, traced results are shaped like the real ones."""
+    from native_sparse_attention_pytorch_amd import ops
+    x, w, labels, _ = _inputs(n, 64, 300, dtype)
+    loss, state = ops.linear_cross_entropy_fwd(x, w, labels, -100, 1)
+    for op, args in ((torch.ops.nsa_amd.linear_cross_entropy_fwd, (x.clone().requires_grad_(), w.clone().requires_grad_(), labels, -100, 1)),
+                     (torch.ops.nsa_amd.linear_cross_entropy_bwd, (torch.ones((), device=DEV), x, w, state, -100, 1, True, True))):
+        torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
