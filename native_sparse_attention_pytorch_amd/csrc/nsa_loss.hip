@@ -1,20 +1,20 @@
 // Softmax cross entropy of a projection onto a vocabulary, l = x w^T, and its gradients, without the logits in memory.
 //
-//   loss_i = m_i - l[i][t_i] + log s_i,  m_i = max_v l[i][v],  s_i = sum_v exp(l[i][v] - m_i)
-//   G[i][v] = g_i (exp(l[i][v] - m_i - log s_i) - [v == t_i]),  dx = G w,  dw = G^T x
+//   loss_i = log sum_v exp(l[i][v] - l[i][t_i]),  G[i][v] = g_i (p[i][v] - [v == t_i]),  p[i][v] = exp(l[i][v]) / sum_u exp(l[i][u]),
+//   dx = G w,  dw = G^T x
 //
 // Rows whose label is `ignore` are left out of everything: the others are gathered first (their order kept), so work goes by their number,
 // which stays on the device, and what an ignored row holds (a NaN) reaches nothing.
-// Where the label is the likely entry, the loss and its G are differences of about equal numbers.  So the maximum and the logarithm of the sum
-// stay two numbers, the maximum is taken off before the product with log2 e, and the label's G / g_i = exp(-loss_i) - 1 comes from the forward's
-// logit, not from one that the backward has rounded otherwise.  (With m + log s in one, and the product first, a loss below 1e-6 was noise and
-// fp32 gradients were 1.8e-6 off instead of 2.5e-7; a subtraction a logit is 1 % of the time at 512 features.)
+// Where the label is the likely entry, its loss and its G are small beside what they are differences of.  So the other entries are summed by
+// themselves: with the sum r of exp(l[i][v] - l[i][t_i]) over them, loss_i = log(1 + r) and the label's G is -g_i r / (1 + r), however small (a
+// loss below 1e-6 was noise before, fp32 gradients of likely labels 1.8e-6 off instead of 2.5e-7).  That is also the largest G of its row, so
+// G is scaled by the largest of those.  The row's maximum and the logarithm of its sum stay two numbers for the others' G.
 //
 // Forward: a tile of logits is made with the vocabulary along the registers of a lane and the tokens along the lanes, so a token's maximum
 // and sum over a wave's 64 or 128 logits are a lane's own and one exchange of the wave's halves; the pairs (maximum, sum) of all waves'
 // parts are merged by a second kernel.  Backward, piece by piece of the vocabulary: the logits again, G as fp16 (below), then both products.
 //
-// G in fp16: probabilities and g_i / max |g| are at most 1, so G 2^14 / max |g| has 11 bits down to 2^-28 of the largest, against bf16's 8: with
+// G in fp16: G 2^14 / max |G| has 11 bits down to 2^-28 of the largest, against bf16's 8: with
 // a bf16 G the gradients of a bf16 model were off by 1.4 times their own rounding, with this by 1.01.  The other operands of those
 // products, w and x, are scaled by powers of two into fp16's range and lose nothing that is above 2^-29 of their largest value.
 // fp32 operands are two fp16 planes each, G too (nsa_tiles.hpp); fp16 ones are exact in one, and G two where that is cheap (loss_plan).
@@ -25,8 +25,9 @@
 
 namespace nsa {
 
-constexpr int kGradBits = 14;
-// device words, of the state and of a backward pass: rows that count; bits of the largest finite |x|, |w| and |g|; slices of dx
+// G is held times 2 to the power of this (up to 120: the exponential of a row whose g is zero stays finite)
+__device__ __forceinline__ int grad_shift(unsigned largest) { return min(120, 14 - plane_exponent(largest)); }
+// device words, of the state and of a backward pass: rows that count; bits of the largest finite |x|, |w| and |G|; slices of dx
 enum { CELL_ROWS, CELL_X, CELL_W, CELL_G, CELL_SLICES, CELLS = 64 };
 // Behind those of the state, for bf16, the bits of the largest finite |x| that work-groups have found, each in one of 16 words 64 bytes apart: one word
 // for all held up the copy of 8184 rows of 512 by 11 us.
@@ -235,11 +236,12 @@ struct LossMost {
 };
 struct LossBegin {
   LossMost of[2];
-  // the backward's weights (work-groups behind those): g of the rows that count, and of each 1024 of them the bits of the largest finite |g|
+  // the backward's weights (work-groups behind those): g of the rows that count, and of each 1024 of them the bits of the largest finite |G|
   const float* dloss;
   int reduction;
   const int* map;
   const unsigned* count;
+  const float* own;
   float* g;
   unsigned* most;
 };
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(256) void loss_begin_kernel(const LossBegin G) {
       if (i >= live) break;
       const float v = G.reduction == 0 ? G.dloss[G.map[i]] : G.reduction == 1 ? G.dloss[0] / (float)live : G.dloss[0];
       G.g[i] = v;
-      best = max(best, finite_bits(v));
+      best = max(best, finite_bits(v * G.own[i]));
     }
     best = largest_of(best);
     if (threadIdx.x == 0) G.most[third] = best;
@@ -303,7 +305,7 @@ struct LossRows {
 struct LossCopy {
   LossRows of[2];
   int kp;
-  // The first copy of a pass: one more work-group leaves the largest of both matrices here, and in a backward pass that of the weights (`most`: of
+  // The first copy of a pass: one more work-group leaves the largest of both matrices here, and in a backward pass that of G (`most`: of
   // each 1024) and the slices of a piece's entries that dx is summed from
   unsigned* cells;
   const unsigned *most, *count;
@@ -442,7 +444,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
   const int unscale = SCALED && G.x_cell != nullptr ? -(plane_shift(*G.x_cell) + plane_shift(*G.w_cell)) : 0;
   const bool cut = m0 + Tiles::TM > G.vend;      // entries past the last one
   constexpr int PART = Tiles::TM / Tiles::WM;
-  const int g_shift = GRAD ? kGradBits - plane_exponent(*G.g_cell) : 0;
+  const int g_shift = GRAD ? grad_shift(*G.g_cell) : 0;
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j) {
     const int token = n0 + t.col_of(j);
@@ -468,7 +470,11 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
 #pragma unroll
         for (int i = 0; i < Tiles::MI; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) found = own == 32 * i + 8 * (e >> 2) + 4 * (t.lane >> 5) + (e & 3) ? t.acc[i][j][e] : found;
+          for (int e = 0; e < 16; ++e) {      // (the label is none of the entries that are summed)
+            const bool it = hit && own == 32 * i + 8 * (e >> 2) + 4 * (t.lane >> 5) + (e & 3);
+            found = it ? t.acc[i][j][e] : found;
+            t.acc[i][j][e] = it ? -INFINITY : t.acc[i][j][e];
+          }
         if (hit) G.target[token] = found;
       }
       float top = t.acc[0][j][0];
@@ -488,13 +494,13 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
     } else {
       const int pad = (live + 63) / 64 * 64;
       const float2 norm = ok ? G.norm[token] : make_float2(0.f, 0.f);
-      const float g = ok ? __builtin_ldexpf(G.g[token], g_shift) : 0.f;
+      const float g = ok ? G.g[token] : 0.f, shift = (float)g_shift - norm.y;
 #pragma unroll
       for (int i = 0; i < Tiles::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) t.acc[i][j][e] = ok ? g * fast_exp2(__builtin_fmaf(t.acc[i][j][e] - norm.x, kLog2e, -norm.y)) : 0.f;
+        for (int e = 0; e < 16; ++e) t.acc[i][j][e] = ok ? g * fast_exp2(__builtin_fmaf(t.acc[i][j][e] - norm.x, kLog2e, shift)) : 0.f;
       if (__any(hit)) {
-        const float at_label = hit ? g * G.own[token] : 0.f;
+        const float at_label = hit ? __builtin_ldexpf(g * G.own[token], g_shift) : 0.f;
 #pragma unroll
         for (int i = 0; i < Tiles::MI; ++i)
 #pragma unroll
@@ -690,8 +696,8 @@ __global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const int row = 8 * (e >> 2) + 4 * h + (e & 3);
-    if (token < live && row == own) G.target[token] = acc[e];
-    if (m0 + row >= G.vocab) acc[e] = -INFINITY;
+    if (row == own) G.target[token] = acc[e];
+    if (row == own || m0 + row >= G.vocab) acc[e] = -INFINITY;      // (the label is none of the entries that are summed)
     top = fmaxf(top, acc[e]);
   }
   top = halves_max(top);
@@ -748,10 +754,13 @@ __global__ __launch_bounds__(256) void loss_merge_kernel(const float2* part, int
     }
   }
   if (lane != 0 || token >= live) return;
-  const float from = label[token] < 0 ? __builtin_nanf("") : top > -INFINITY ? top : 0.f;      // no entry of the vocabulary: said by the loss and all gradients
-  const float value = from - (label[token] < 0 ? 0.f : target[token]) + logf(sum);
-  norm[token] = make_float2(from, log2f(sum));
-  own[token] = expm1f(-value);
+  // the others' sum and the label's exponential, both from the larger maximum (no entry of the vocabulary: NaN, in the loss and all gradients; an
+  // infinite logit too)
+  const float at_label = label[token] < 0 ? __builtin_nanf("") : target[token], from = fmaxf(top, at_label) + (at_label - at_label);
+  const float others = sum > 0.f ? sum * expf(top - from) : sum, all = others + expf(at_label - from);
+  const float value = at_label >= top ? log1pf(others) + (at_label - at_label) : (top - at_label) + logf(all);
+  norm[token] = make_float2(from, log2f(all));
+  own[token] = -others / all;
   loss[token] = value;
   if (losses != nullptr) losses[map[token]] = value;
 }
@@ -806,7 +815,7 @@ __device__ __forceinline__ void loss_dx(const LossGradArgs& G, char* shared) {
   t.operand_b(G.grad, G.grad_plane, G.grad_ld, n0, live);
   t.run(steps, from);
   // (all pieces share the power of two)
-  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.w_cell != nullptr ? plane_shift(*G.w_cell) : 0);
+  const int shift = -grad_shift(*G.g_cell) - (G.w_cell != nullptr ? plane_shift(*G.w_cell) : 0);
   float* sums = G.sums + (size_t)split * ((live + 63) / 64 * 64) * G.kp;
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j)
@@ -834,7 +843,7 @@ __device__ __forceinline__ void loss_dw(const LossGradArgs& G, char* shared) {
   } else {
     t.run(steps);
   }
-  const int shift = plane_exponent(*G.g_cell) - kGradBits - (G.x_cell != nullptr ? plane_shift(*G.x_cell) : 0);
+  const int shift = -grad_shift(*G.g_cell) - (G.x_cell != nullptr ? plane_shift(*G.x_cell) : 0);
   O* dw = (O*)G.dw + (SLICES ? (size_t)split * G.entries * G.dw_ld : 0);
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j)
@@ -1115,7 +1124,7 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
     b.of[1] = most_to(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, parts + kParts);
     of_w = found(b.of[1]);
   }
-  b.dloss = dloss; b.reduction = d->reduction; b.map = map; b.count = count; b.g = g; b.most = g_most;
+  b.dloss = dloss; b.reduction = d->reduction; b.map = map; b.count = count; b.own = (const float*)(s + p.s_own); b.g = g; b.most = g_most;
   begin(d, b, (p.n + 1023) / 1024, st);
   const long x_plane = (long)p.npad * p.kp;
   void* xg = w + p.b_x;

@@ -502,3 +502,34 @@ def test_the_operators_are_what_they_are_registered_as(n, dtype):
     for op, args in ((torch.ops.nsa_amd.linear_cross_entropy_fwd, (x.clone().requires_grad_(), w.clone().requires_grad_(), labels, -100, 1)),
                      (torch.ops.nsa_amd.linear_cross_entropy_bwd, (torch.ones((), device=DEV), x, w, state, -100, 1, True, True))):
         torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("n", [1, 33])
+@pytest.mark.parametrize("gap", [5., 20., 45.])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_losses_far_below_a_rounding_of_one(n, gap, dtype):
+    """log(1 + r) with r down to 1e-17 and its gradients, to the relative error of the others' exponentials: two logits' dL, 2^-16 for the sums, and for
+    the exponents' own rounding 2^-22 of the distance in front of it."""
+    from native_sparse_attention_pytorch_amd import ops
+    d, v = 96, 300
+    _, w, labels, weights = _inputs(n, d, v, dtype, seed=8, ignored=0.)
+    x = (w.float()[labels] * gap / w.float()[labels].square().sum(-1, keepdim=True)).to(dtype)
+    x.requires_grad_(), w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, labels, reduction="none")
+    dx, dw = torch.autograd.grad(loss, (x, w), weights)
+    x6, w6, at = x.detach().double(), w.detach().double(), labels[:, None]
+    logits, size = x6 @ w6.t().contiguous(), x6.abs() @ w6.abs().t().contiguous()
+    h, u = (2 ** -22, 2 ** -24) if dtype == F32 else (0., torch.finfo(dtype).eps / 2)
+    far = logits - logits.gather(1, at)
+    rel = 2 * (((d / 4 + 8) * 2 ** -24 + 2 * h) * size).amax(-1, keepdim=True) + 2 ** -16 + 2 ** -22 * far.abs().amax(-1, keepdim=True)
+    others = torch.exp(far).scatter(1, at, 0.)
+    r = others.sum(-1, keepdim=True)
+    assert gap < 45 or r.max() < 1e-9
+    _within(loss.detach(), (torch.log1p(r)[:, 0], (rel * torch.log1p(r))[:, 0]), "loss")
+    G = weights.double()[:, None] * (others / (1 + r)).scatter(1, at, -r / (1 + r))
+    dG = G.abs() * (2 * rel + (2 ** -11 if dtype != F32 else h)) + 2 ** -38 * float(G.abs().max())
+    for got, left, off, right, k in ((dx, G, dG, w6, v), (dw, G.t().contiguous(), dG.t().contiguous(), x6, n)):
+        want = left @ right
+        tol = off @ right.abs() + left.abs() @ ((h + (k / 4 + 16) * 2 ** -24) * right.abs() + 2 ** -38 * float(right.abs().max()))
+        # (fp16 results below 2^-24 are multiples of it)
+        _within(got, (want, 1.01 * tol + u * want.abs() + (2. ** -25 if dtype == F16 else torch.finfo(dtype).tiny)), gap)
