@@ -6,9 +6,10 @@
 // Rows whose label is `ignore` are left out of everything: the others are gathered first (their order kept), so work goes by their number,
 // which stays on the device, and what an ignored row holds (a NaN) reaches nothing.
 // Where the label is the likely entry, its loss and its G are small beside what they are differences of.  So the other entries are summed by
-// themselves: with the sum r of exp(l[i][v] - l[i][t_i]) over them, loss_i = log(1 + r) and the label's G is -g_i r / (1 + r), however small (a
-// loss below 1e-6 was noise before, fp32 gradients of likely labels 1.8e-6 off instead of 2.5e-7).  That is also the largest G of its row, so
-// G is scaled by the largest of those.  The row's maximum and the logarithm of its sum stay two numbers for the others' G.
+// themselves: with the sum r of exp(l[i][v] - l[i][t_i]) over them, loss_i = log(1 + r) and the label's G is -g_i r / (1 + r) (a loss below 1e-6 was
+// noise before, fp32 gradients of likely labels 1.8e-6 off instead of 2.5e-7).  An r that 64 bits do not tell from nothing beside 1 is nothing, as
+// in a softmax computed in them: loss and the label's G are zero.  No G of a row is larger than g_i r / (1 + r), so G is scaled by the largest of
+// those.  The row's maximum and the logarithm of its sum stay two numbers for the others' G.
 //
 // Forward: a tile of logits is made with the vocabulary along the registers of a lane and the tokens along the lanes, so a token's maximum
 // and sum over a wave's 64 or 128 logits are a lane's own and one exchange of the wave's halves; the pairs (maximum, sum) of all waves'
@@ -25,6 +26,7 @@
 
 namespace nsa {
 
+constexpr float kNothing = 0x1p-53f;      // beside 1
 // G is held times 2 to the power of this (up to 120: the exponential of a row whose g is zero stays finite)
 __device__ __forceinline__ int grad_shift(unsigned largest) { return min(120, 14 - plane_exponent(largest)); }
 // device words, of the state and of a backward pass: rows that count; bits of the largest finite |x|, |w| and |G|; slices of dx
@@ -406,7 +408,7 @@ struct LossTileArgs {
   int npad;
   // backward
   const float2* norm;                      // maximum, log2 of the sum
-  const float *own, *g;                    // the label's G / g
+  const float *own, *g;                    // -r / (1 + r)
   const unsigned* g_cell;
   _Float16* grad;                          // [grad_planes][npad][grad_ld]
   long grad_plane;
@@ -500,7 +502,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
 #pragma unroll
         for (int e = 0; e < 16; ++e) t.acc[i][j][e] = ok ? g * fast_exp2(__builtin_fmaf(t.acc[i][j][e] - norm.x, kLog2e, shift)) : 0.f;
       if (__any(hit)) {
-        const float at_label = hit ? __builtin_ldexpf(g * G.own[token], g_shift) : 0.f;
+        const float of_label = hit ? G.own[token] : 0.f, at_label = __builtin_fabsf(of_label) < kNothing ? 0.f : __builtin_ldexpf(g * of_label, g_shift);
 #pragma unroll
         for (int i = 0; i < Tiles::MI; ++i)
 #pragma unroll
@@ -758,7 +760,7 @@ __global__ __launch_bounds__(256) void loss_merge_kernel(const float2* part, int
   // infinite logit too)
   const float at_label = label[token] < 0 ? __builtin_nanf("") : target[token], from = fmaxf(top, at_label) + (at_label - at_label);
   const float others = sum > 0.f ? sum * expf(top - from) : sum, all = others + expf(at_label - from);
-  const float value = at_label >= top ? log1pf(others) + (at_label - at_label) : (top - at_label) + logf(all);
+  const float value = at_label >= top ? (others < kNothing ? 0.f : log1pf(others)) + (at_label - at_label) : (top - at_label) + logf(all);
   norm[token] = make_float2(from, log2f(all));
   own[token] = -others / all;
   loss[token] = value;
