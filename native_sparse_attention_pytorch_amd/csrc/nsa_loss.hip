@@ -89,8 +89,11 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
       least = time;
     }
   }
-  p.tile = p.size == WIDE ? 256 : p.size == TINY ? 64 : 128;
-  p.part = p.size == WIDE || p.size == FEW ? 128 : p.size == MIDDLE ? 64 : 32;
+  // Few rows: tiles of 32 entries, whose waves share the features, where those of 128 leave half the CUs idle.  (7 rows, 3542 features, 3870 entries in
+  // fp32: 80 us with 128, 35 with 32; 24, 4096, 16000 in bf16: 41 and 41; 30000: 59 and 66.)
+  const bool narrow = p.size == FEW && d->vocab < 16384;
+  p.tile = p.size == WIDE ? 256 : p.size == TINY ? 64 : narrow ? 32 : 128;
+  p.part = narrow || p.size == TINY ? 32 : p.size == MIDDLE ? 64 : 128;
   p.in_place = d->dtype != 2 && d->dim % 8 == 0 && d->dim >= 64 && d->w_stride % 8 == 0 && d->w_stride < (1 << 20) && ((uintptr_t)weight & 15) == 0;
   const size_t v256 = up(d->vocab, 256), v64 = up(d->vocab, 64), row = (size_t)p.kp * 2;
   p.fwd_rows = (int)std::min(v256, std::max<size_t>(256, ((size_t)256 << 20) / (row * p.P) / 256 * 256));
@@ -545,7 +548,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
 // ------------------------------------------------------------------------------------ few rows
 
 // Up to 32 rows (scoring, decoding): one pass over the weight where it lies, of any type and alignment, is all their time.  Tiles of 128 entries by
-// 32 rows, 128 bytes of each at a time in LDS (swizzled as TileOperand's).  Rows that begin at multiples of 16 bytes are copied there three
+// 32 rows, 128 bytes of each at a time in LDS (swizzled as TileOperand's); NARROW: of 32 entries, 128 bytes for each wave at a time.  Rows that begin at multiples of 16 bytes are copied there three
 // stages ahead of their use (24 rows of 4096 features, 131072 entries in bf16, 1.07 GB: 5.8 TB/s); others go through registers, a stage ahead
 // (4.7 TB/s).  fp32 takes fp32 products (32 x 32 x 2: half the time that the weight takes from memory), so there are no planes.  Every
 // work-group finds out the rows that count by itself.
@@ -558,11 +561,11 @@ struct LossFewArgs {
   float2* part;
   float *target, *losses;
 };
-template <class S, bool ALIGNED>
+template <class S, bool ALIGNED, bool NARROW>
 __global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
-  // (all of LDS is the stages: two work-groups fit into a CU)
-  constexpr int STAGES = ALIGNED ? 4 : 2, STAGE = 160 * 128;
-  __shared__ __align__(1024) char stage_s[STAGES][STAGE];      // rows of 128 bytes: entries, then rows of x
+  // rows of 128 bytes: entries, then rows of x, of NARROW for each wave.  (All of LDS is the stages: two work-groups fit into a CU, one if NARROW)
+  constexpr int STAGES = ALIGNED ? 4 : 2, LOADS = NARROW ? 8 : 5, STAGE = LOADS * 32 * 128;
+  __shared__ __align__(1024) char stage_s[STAGES][STAGE];
   int* map_s = reinterpret_cast<int*>(stage_s[0]);
   float(*top_s)[32] = reinterpret_cast<float(*)[32]>(stage_s[0]), (*sum_s)[32] = top_s + 4;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, token = lane & 31;
@@ -588,32 +591,35 @@ __global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
   __syncthreads();
 
   // (an XCD takes neighbouring tiles: 4.8 TB/s with every eighth of them)
-  const int tile = xcd_run(blockIdx.x, gridDim.x), m0 = tile * 128 + 32 * wave, dim = G.dim;
-  constexpr int V = 16 / sizeof(S), BK = 8 * V;      // values of 16 bytes, of a stage
+  const int tile = xcd_run(blockIdx.x, gridDim.x), first = tile * (NARROW ? 32 : 128), m0 = first + (NARROW ? 0 : 32 * wave), dim = G.dim;
+  constexpr int V = 16 / sizeof(S), K = 8 * V, BK = NARROW ? 4 * K : K;      // values of 16 bytes, of 128, of a stage
   typedef decltype(load_any<V>((const S*)nullptr)) vec;
-  // this thread's 16 bytes of five rows: every 32nd entry, one row of x
-  const int r0 = tid >> 3, swz = (r0 >> 1) & 7, chunk = ALIGNED ? (tid & 7) ^ swz : tid & 7, first = tile * 128;
-  const S* src[5];
+  // this thread's 16 bytes of each load: of every 32nd entry and one row of x, or of one entry and one row of x, 128 bytes on for each wave
+  const int r0 = tid >> 3, swz = (r0 >> 1) & 7, chunk = ALIGNED ? (tid & 7) ^ swz : tid & 7;
+  const S *src[LOADS], *x_row = (const S*)G.x + (long)map_s[min(r0, live - 1)] * G.x_ld + chunk * V;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) src[u] = (const S*)G.w + (long)min(first + r0 + 32 * u, G.vocab - 1) * G.w_ld + chunk * V;
-  src[4] = (const S*)G.x + (long)map_s[min(r0, live - 1)] * G.x_ld + chunk * V;
+  for (int u = 0; u < LOADS; ++u) {
+    const bool of_x = NARROW ? u & 1 : u == 4;
+    src[u] = of_x ? x_row : (const S*)G.w + (long)min(first + r0 + (NARROW ? 0 : 32 * u), G.vocab - 1) * G.w_ld + chunk * V;
+    if (NARROW) src[u] += (u >> 1) * K;
+  }
   const int own = token < live ? map_s[32 + token] - m0 : -1;
   __syncthreads();
   char* to = &stage_s[0][0] + r0 * 128 + 16 * (chunk ^ swz);
-  vec held[2][5];
+  vec held[2][LOADS];
   floatx16 part[4], acc = zero_acc();      // sums in parts: each of 64 products, then theirs
 #pragma unroll
   for (int ks = 0; ks < 4; ++ks) part[ks] = zero_acc();
-  auto store = [&](const vec (&v)[5], int buf) {
+  auto store = [&](const vec (&v)[LOADS], int buf) {
 #pragma unroll
-    for (int u = 0; u < 5; ++u) *reinterpret_cast<vec*>(to + buf * STAGE + u * 32 * 128) = v[u];
+    for (int u = 0; u < LOADS; ++u) *reinterpret_cast<vec*>(to + buf * STAGE + u * 32 * 128) = v[u];
   };
   auto products = [&](int buf) {
-    const char* row = stage_s[buf] + token * 128;
+    const char *row = stage_s[buf] + token * 128 + (NARROW ? wave * 64 * 128 : 0), *entry = row + (NARROW ? 0 : wave * 32 * 128), *x = row + (NARROW ? 32 : 128) * 128;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       const int at = 16 * ((2 * ks + h) ^ ((token >> 1) & 7));
-      const vec a = *reinterpret_cast<const vec*>(row + wave * 32 * 128 + at), b = *reinterpret_cast<const vec*>(row + 128 * 128 + at);
+      const vec a = *reinterpret_cast<const vec*>(entry + at), b = *reinterpret_cast<const vec*>(x + at);
       if constexpr (sizeof(S) == 4) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) part[ks] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], part[ks], 0, 0, 0);
@@ -623,7 +629,7 @@ __global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
     }
   };
   auto piece = [&](int k) {      // (sums in pieces: see TileProduct::PIECES)
-    if (k % 256 == 0) {
+    if (k % (NARROW ? 1024 : 256) == 0) {
       acc += (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) part[ks] = zero_acc();
@@ -638,7 +644,7 @@ __global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
     auto copy = [&](int t) {
       const unsigned lanes = __builtin_amdgcn_readfirstlane(t < stages ? ~0u : 0u);
 #pragma unroll
-      for (int u = 0; u < 5; ++u)
+      for (int u = 0; u < LOADS; ++u)
         asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 vcc, exec\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\ts_nop 0\n\t"
                      "global_load_lds_dwordx4 %1, off\n\ts_mov_b64 exec, vcc"
                      :: "s"(mine + (t & 3) * STAGE + u * 32 * 128), "v"(src[u] + t * BK), "s"(lanes) : "memory", "m0", "vcc");
@@ -647,7 +653,7 @@ __global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
     for (int t = 0; t < 3; ++t) copy(t);
     for (int t = 0; t < stages; ++t, k += BK) {
       fence();
-      asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(2 * LOADS) : "memory");
       fence();
       copy(t + 3);
       products(t & 3);
@@ -660,9 +666,9 @@ __global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
     // (No branch around a load - behind the last one it is read again - or every use of one waits for all of them.  A buffer is written again
     // when all have passed the barrier behind its reading.)
     const int pairs = dim / (2 * BK) * (2 * BK);
-    auto load = [&](int at, vec (&into)[5]) {
+    auto load = [&](int at, vec (&into)[LOADS]) {
 #pragma unroll
-      for (int u = 0; u < 5; ++u) into[u] = load_any<V>(src[u] + at);
+      for (int u = 0; u < LOADS; ++u) into[u] = load_any<V>(src[u] + at);
     };
     if (pairs > 0) {
       load(0, held[0]);
@@ -682,23 +688,38 @@ __global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
     }
   }
   for (; k < dim; k += BK) {      // what is left of the rows
-    const int have = dim - k - chunk * V;
 #pragma unroll
-    for (int u = 0; u < 5; ++u)
+    for (int u = 0; u < LOADS; ++u) {
+      const int have = dim - (k + (NARROW ? (u >> 1) * K : 0) + chunk * V);
+      if (have >= V) {
+        held[0][u] = load_any<V>(src[u] + k);
+      } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) held[0][u][e] = e < have ? src[u][k + e] : (S)0.f;
+        for (int e = 0; e < V; ++e) held[0][u][e] = e < have ? src[u][k + e] : (S)0.f;
+      }
+    }
     __syncthreads();
     store(held[0], 0);
     __syncthreads();
     products(0);
   }
   acc += (part[0] + part[1]) + (part[2] + part[3]);
+  if (NARROW) {
+    // the waves' parts of the sums, in their order
+    float* sums = reinterpret_cast<float*>(stage_s[0]) + lane;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sums[(wave * 16 + e) * 64] = acc[e];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = (sums[e * 64] + sums[(16 + e) * 64]) + (sums[(32 + e) * 64] + sums[(48 + e) * 64]);
+  }
 
   float top = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const int row = 8 * (e >> 2) + 4 * h + (e & 3);
-    if (row == own) G.target[token] = acc[e];
+    if (row == own && (!NARROW || wave == 0)) G.target[token] = acc[e];
     if (row == own || m0 + row >= G.vocab) acc[e] = -INFINITY;      // (the label is none of the entries that are summed)
     top = fmaxf(top, acc[e]);
   }
@@ -716,10 +737,10 @@ __global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
   if (tid >= live) return;
   float most = -INFINITY, s = 0.f;
 #pragma unroll
-  for (int v = 0; v < 4; ++v) most = fmaxf(most, top_s[v][tid]);
+  for (int v = 0; v < (NARROW ? 1 : 4); ++v) most = fmaxf(most, top_s[v][tid]);
   const float at = most > -INFINITY ? most : 0.f;
 #pragma unroll
-  for (int v = 0; v < 4; ++v) s += sum_s[v][tid] * fast_exp2((top_s[v][tid] - at) * kLog2e);
+  for (int v = 0; v < (NARROW ? 1 : 4); ++v) s += sum_s[v][tid] * fast_exp2((top_s[v][tid] - at) * kLog2e);
   G.part[(size_t)blockIdx.x * G.npad + tid] = make_float2(most, s);
 }
 
@@ -939,6 +960,10 @@ static void launch_tiles(const LossPlan& p, const LossTileArgs& a, hipStream_t s
   else if constexpr (GRAD) launch_tile<typename L::Few, GRAD>(a, st);      // (the forward of few rows: loss_few_kernel)
 }
 
+template <class S>
+static auto few_kernel(bool aligned, bool narrow) {
+  return aligned ? narrow ? loss_few_kernel<S, true, true> : loss_few_kernel<S, true, false> : narrow ? loss_few_kernel<S, false, true> : loss_few_kernel<S, false, false>;
+}
 static bool misaligned(std::initializer_list<const void*> all, size_t to) {
   for (const void* p : all)
     if ((uintptr_t)p % to) return true;
@@ -1026,11 +1051,9 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
   if (p.size == FEW) {
     LossFewArgs a{x, weight, labels, (long)d->x_stride, (long)d->w_stride, (long)d->ignore_index, (int)d->labels_int64, p.n, d->dim, d->vocab, p.npad,
                   map, place, label, cells, part, target, losses};
-    const dim3 grid((unsigned)((d->vocab + 127) / 128));
+    const dim3 grid((unsigned)((d->vocab + p.tile - 1) / p.tile));
     const bool aligned = (((uintptr_t)x | (uintptr_t)weight) & 15) == 0 && d->x_stride * each_bytes % 16 == 0 && d->w_stride * each_bytes % 16 == 0;
-    const auto kernel = d->dtype == 0 ? aligned ? loss_few_kernel<B16, true> : loss_few_kernel<B16, false>
-                        : d->dtype == 1 ? aligned ? loss_few_kernel<H16, true> : loss_few_kernel<H16, false>
-                                        : aligned ? loss_few_kernel<float, true> : loss_few_kernel<float, false>;
+    const auto kernel = d->dtype == 0 ? few_kernel<B16>(aligned, p.tile == 32) : d->dtype == 1 ? few_kernel<H16>(aligned, p.tile == 32) : few_kernel<float>(aligned, p.tile == 32);
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
   } else {
     hipLaunchKernelGGL(loss_rows_kernel, dim3((unsigned)((p.n + 1023) / 1024)), dim3(256), 0, st, labels, (int)d->labels_int64, p.n, d->vocab,

@@ -128,6 +128,10 @@ def test_large_tiles_and_pieces(n, d, v, dtype):
     (31, 264, 127),                # and one step more
     (32, 1000, 385),
     (32, 520, 1),
+    (3, 7, 16383),                 # the last vocabulary of narrow tiles
+    (17, 65, 16400),               # and wide ones
+    (31, 264, 20001),
+    (5, 1000, 16385),
 ])
 def test_few_rows(n, d, v, dtype):
     """Up to 32 rows, from rows at multiples of 16 bytes and from others: the same sums in the same order."""
