@@ -550,7 +550,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
 // Up to 32 rows (scoring, decoding): one pass over the weight where it lies, of any type and alignment, is all their time.  Tiles of 128 entries by
 // 32 rows, 128 bytes of each at a time in LDS (swizzled as TileOperand's); NARROW: of 32 entries, 128 bytes for each wave at a time.  Rows that begin at multiples of 16 bytes are copied there three
 // stages ahead of their use (24 rows of 4096 features, 131072 entries in bf16, 1.07 GB: 5.8 TB/s); others go through registers, a stage ahead
-// (4.7 TB/s).  fp32 takes fp32 products (32 x 32 x 2: half the time that the weight takes from memory), so there are no planes.  Every
+// (a row of 1675, 88295 entries in fp16: 3.7 TB/s with three work-groups a CU, 3.4 with two).  fp32 takes fp32 products (32 x 32 x 2: half the time that the weight takes from memory), so there are no planes.  Every
 // work-group finds out the rows that count by itself.
 struct LossFewArgs {
   const void *x, *w, *labels;
@@ -562,7 +562,7 @@ struct LossFewArgs {
   float *target, *losses;
 };
 template <class S, bool ALIGNED, bool NARROW>
-__global__ __launch_bounds__(256) void loss_few_kernel(const LossFewArgs G) {
+__global__ __launch_bounds__(256, ALIGNED || NARROW ? 2 : 3) void loss_few_kernel(const LossFewArgs G) {
   // rows of 128 bytes: entries, then rows of x, of NARROW for each wave.  (All of LDS is the stages: two work-groups fit into a CU, one if NARROW)
   constexpr int STAGES = ALIGNED ? 4 : 2, LOADS = NARROW ? 8 : 5, STAGE = LOADS * 32 * 128;
   __shared__ __align__(1024) char stage_s[STAGES][STAGE];
