@@ -2731,10 +2731,10 @@ def _newton_schulz(matrices, steps: int, a: float, b: float, c: float, eps: floa
     first = matrices[0]
     with _on(first.device):
         out, sizes, ins, strides, outs = [], [], [], [], []
-        for t in matrices:
+        # (copies are held until the launches: the kernels are given addresses alone)
+        read = [t.contiguous() if t.stride(-1) != 1 or t.stride(-2) < t.shape[-1] else t for t in matrices]
+        for t in read:
             rows, cols = t.shape[-2:]
-            if t.stride(-1) != 1 or t.stride(-2) < cols:
-                t = t.contiguous()
             o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
             out.append(o)
             each, at, to = t.element_size(), t.data_ptr(), o.data_ptr()
