@@ -2743,7 +2743,7 @@ def _newton_schulz(matrices, steps: int, a: float, b: float, c: float, eps: floa
                 sizes.append((rows, cols))
                 ins.append(at + i * step)
                 outs.append(to + i * rows * cols * each)
-                strides.append(t.stride(-2))
+                strides.append(max(t.stride(-2), cols))      # (of one row: any)
         many = len(sizes)
         ints, longs, ptrs = C.c_int32 * many, C.c_int64 * many, C.c_void_p * many
         rows, cols, ws = ints(*(r for r, _ in sizes)), ints(*(c for _, c in sizes)), C.c_size_t()

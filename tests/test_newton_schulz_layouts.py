@@ -40,3 +40,13 @@ def test_muon_of_transposed_parameters(stand_in):
     Muon(params, lr=0.1, momentum=0.5, nesterov=False).step()
     for p, b, g in zip(params, before, grads):
         torch.testing.assert_close(p.detach(), b - 0.1 * 1.5 ** 0.5 * 2 * g)
+
+
+@pytest.mark.parametrize("make", [lambda: torch.randn(8, 1).t(), lambda: torch.randn(3, 8, 1).mT, lambda: torch.randn(8, 1), lambda: torch.randn(1)[None].expand(1, 1),
+                                  lambda: torch.randn(5, 1, 8)[:, :, :1], lambda: torch.randn(8).as_strided((1, 8), (0, 1)), lambda: torch.randn(2, 8, 1).mT.unsqueeze(0)])
+def test_matrices_of_one_row_or_column(stand_in, make):
+    """Where a matrix has one row, torch calls it contiguous whatever that row's stride."""
+    from native_sparse_attention_pytorch_amd import ops
+    given = make()
+    for o in (ops.newton_schulz(given), ops.newton_schulz([given, given])[1]):
+        assert torch.equal(o, 2 * given)

@@ -44,3 +44,11 @@ def test_muon_of_transposed_parameters():
         moved.append([p.detach() for p in params])
     for a, b in zip(*moved):
         assert torch.equal(a, b)
+
+
+def test_matrices_of_one_row():
+    """(8, 1).t() has one row and a row stride of 1."""
+    from native_sparse_attention_pytorch_amd import ops
+    for given in (torch.randn(8, 1, device=DEV).t(), torch.randn(3, 500, 1, device=DEV).mT, torch.randn(70000, 1, device=DEV).t()):
+        for o, w in zip(ops.newton_schulz([given, given]), ops.newton_schulz([given.clone(memory_format=torch.contiguous_format)] * 2)):
+            assert torch.equal(o, w) and o.isfinite().all()
