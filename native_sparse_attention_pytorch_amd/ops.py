@@ -100,11 +100,29 @@ def _ws_sizes(dsc) -> tuple[int, int, int]:
 
 # A registered operator call costs about 70 us of host time here (dispatcher, schema checks, autograd wrapper), an
 # autograd.Function call a fraction of that; at small shapes a layer's step is bound by exactly that cost.  Outside a
-# compiler trace the attention operators therefore run as plain autograd.Functions around the same Python bodies; the
-# torch.library registrations (with their fake and autograd rules) serve traced callers.
+# trace or a transform the operators therefore run as plain autograd.Functions around the same Python bodies; the
+# torch.library registrations (with their fake and autograd rules) serve the other callers.
+_is_compiling, _is_autocast, _forward_ad = torch.compiler.is_compiling, torch.is_autocast_enabled, torch.autograd.forward_ad
+_transforms, _dispatch_modes, _tracing_state = torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack, torch._C._get_tracing_state
+_dispatch_key, _PRE_DISPATCH = torch._C._dispatch_tls_is_dispatch_key_included, torch._C.DispatchKey.PreDispatch
+
+
+def _recorded() -> bool:
+    """A compiler, another tracer, a transform or a dispatch mode is at work, which sees registered operators and not what is launched by
+    address: a trace would hold the memory of a result and nothing that writes it."""
+    return bool(_is_compiling() or _transforms() is not None or _dispatch_modes() > 0 or _dispatch_key(_PRE_DISPATCH) or _tracing_state() is not None)
+
+
+def _refuse_tangents(name: str, *args) -> None:
+    """None of the operators has a rule for forward mode; a result without a tangent would say that it is constant."""
+    if not _is_compiling() and _forward_ad._current_level >= 0:
+        if any(isinstance(a, Tensor) and _forward_ad.unpack_dual(a).tangent is not None for a in args):
+            raise NotImplementedError(f"{name}: forward mode is not supported, an argument has a tangent")
+
+
 def _direct(op):
-    """The Python body of a registered operator, unless a compiler is tracing (then the operator itself)."""
-    return op if torch.compiler.is_compiling() else op._init_fn
+    """The Python body of a registered operator, unless a call is recorded (then the operator itself)."""
+    return op if _recorded() else op._init_fn
 
 
 class _NoFurther(torch.autograd.Function):
@@ -133,7 +151,7 @@ def _once(kernels):
 
 def _direct_bwd(op):
     """`_direct` of an operator that makes gradients."""
-    return op if torch.compiler.is_compiling() else _once(op._init_fn)
+    return op if _recorded() else _once(op._init_fn)
 
 
 def _eager_function(op, setup, backward):
@@ -150,10 +168,12 @@ def _eager_function(op, setup, backward):
         def backward(ctx, *grads):
             return backward(ctx, *grads)
 
-    Fn.__name__ = Fn.__qualname__ = "Eager_" + getattr(op, "_name", "op")
+    name = getattr(op, "_name", "op")
+    Fn.__name__ = Fn.__qualname__ = "Eager_" + name
 
     def call(*args):
-        if torch.compiler.is_compiling():
+        _refuse_tangents(name, *args)
+        if _recorded():
             return op(*args)
         if not torch.is_grad_enabled() or not any(isinstance(a, Tensor) and a.requires_grad for a in args):
             return raw(*args)
@@ -540,7 +560,7 @@ def _dense_backward(ctx, dout, dlse, dpooled):
         # importance term has been added
         dq, dk, dv = _direct_bwd(dense_bwd)(q, k, v, out, dout, lse, mode, causal, window, stride, num_mem, scale,
                                         mode == 1 and dpooled is not None and dpooled.numel() > 0)
-    if dq is not None and dpooled is not None and dpooled.numel() > 0 and not torch.compiler.is_compiling() and not torch.is_grad_enabled():
+    if dq is not None and dpooled is not None and dpooled.numel() > 0 and not _recorded() and not torch.is_grad_enabled():
         # both sums in one kernel each: scale, repetition over the group's heads / the block's keys, sum in fp32, one rounding
         dq2, dckb, c = _importance_products_backward(q, k, dpooled, num_mem, stride, sel_block, share, scale)
         dq = _add_repeated(dq, dq2, dq, q.shape[1] // dq2.shape[1], 0, 1, c)
@@ -1720,11 +1740,6 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float | None = None) -> Tensor:
 
 # ------------------------------------------------------------------ projections
 
-_is_compiling, _is_autocast, _forward_ad = torch.compiler.is_compiling, torch.is_autocast_enabled, torch.autograd.forward_ad
-_transforms, _dispatch_modes, _tracing_state = torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack, torch._C._get_tracing_state
-_dispatch_key, _PRE_DISPATCH = torch._C._dispatch_tls_is_dispatch_key_included, torch._C.DispatchKey.PreDispatch
-
-
 def plain_call() -> bool:
     """Nothing is at work that an operator carries and a kernel launched by address loses: autocast, a compiler or another tracer (which
     would record the result as a constant), vmap, jvp, a forward-mode level, a dispatch mode.  Asked before any address is read:
@@ -2787,7 +2802,8 @@ def newton_schulz(updates, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315
     coefficients = tuple(float(v) for v in coefficients)
     if len(coefficients) != 3 or not 1 <= int(steps) <= 100 or not eps >= 0:
         raise ValueError(f"newton_schulz: steps {steps}, coefficients {coefficients}, eps {eps}: expected 1 to 100 steps, three coefficients, eps >= 0")
-    if not torch.compiler.is_compiling():      # (traced calls: the entry checks them)
+    _refuse_tangents("newton_schulz", *given)
+    if not torch.compiler.is_compiling():      # (compiled calls: the entry checks them)
         _newton_coefficients(coefficients, int(steps))
     for t in given:
         if not t.is_cuda or t.device != given[0].device:
@@ -2797,7 +2813,7 @@ def newton_schulz(updates, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("newton_schulz has no gradient: call it under torch.no_grad()")
     out = [None if t.numel() else torch.empty_like(t) for t in given]
-    call = newton_schulz_op if torch.compiler.is_compiling() else _newton_schulz
+    call = newton_schulz_op if _recorded() else _newton_schulz
     for dtype in dict.fromkeys(t.dtype for t in given):
         at = [i for i, t in enumerate(given) if t.dtype == dtype and out[i] is None]
         if at:
