@@ -8,16 +8,19 @@
 // Where the label is the likely entry, its loss and its G are small beside what they are differences of.  So the other entries are summed by
 // themselves: with the sum r of exp(l[i][v] - l[i][t_i]) over them, loss_i = log(1 + r) and the label's G is -g_i r / (1 + r) (a loss below 1e-6 was
 // noise before, fp32 gradients of likely labels 1.8e-6 off instead of 2.5e-7).  An r that 64 bits do not tell from nothing beside 1 is nothing, as
-// in a softmax computed in them: loss and the label's G are zero.  No G of a row is larger than g_i r / (1 + r), so G is scaled by the largest of
-// those.  The row's maximum and the logarithm of its sum stay two numbers for the others' G.
+// in a softmax computed in them: loss and the label's G are zero.  No G of a row is larger than g_i r / (1 + r), and each row's G is scaled by a
+// power of two of its own, from that.  The row's maximum and the logarithm of its sum stay two numbers for the others' G.
 //
 // Forward: a tile of logits is made with the vocabulary along the registers of a lane and the tokens along the lanes, so a token's maximum
 // and sum over a wave's 64 or 128 logits are a lane's own and one exchange of the wave's halves; the pairs (maximum, sum) of all waves'
 // parts are merged by a second kernel.  Backward, piece by piece of the vocabulary: the logits again, G as fp16 (below), then both products.
 //
-// G in fp16: G 2^14 / max |G| has 11 bits down to 2^-28 of the largest, against bf16's 8: with
-// a bf16 G the gradients of a bf16 model were off by 1.4 times their own rounding, with this by 1.01.  The other operands of those
-// products, w and x, are scaled by powers of two into fp16's range and lose nothing that is above 2^-29 of their largest value.
+// G in fp16: G 2^14 / max |G| of its row has 11 bits down to 2^-28 of the row's largest, against bf16's 8: with
+// a bf16 G the gradients of a bf16 model were off by 1.4 times their own rounding, with this by 1.01.  dx, whose rows are sums along rows of G, takes
+// the row's power of two out again; for dw, a sum over rows, a second copy of x is multiplied by what it is beside the largest row's.  (With one
+// power of two for all rows, a row whose label is likely, or whose g is small, lost its others' G: a row with r = 1.2e-8 beside one with a loss
+// near 1 had a dx off by several times its norm.)  The other operands of those products, w and x, are scaled by powers of two into fp16's range and
+// lose nothing that is above 2^-29 of their largest value.
 // fp32 operands are two fp16 planes each, G too (nsa_tiles.hpp); fp16 ones are exact in one, and G two where that is cheap (loss_plan).
 #include <algorithm>
 #include <cmath>
@@ -27,11 +30,13 @@
 namespace nsa {
 
 constexpr float kNothing = 0x1p-53f;      // beside 1
-// G is held times 2 to the power of this (up to 120: the exponential of a row whose g is zero stays finite)
+// A row's G is held times 2 to the power of this (up to 120: the exponential of a row whose g is zero stays finite)
 __device__ __forceinline__ int grad_shift(unsigned largest) { return min(120, 14 - plane_exponent(largest)); }
+// and a row of x for dw times 2 to the power of this: what the row's G has more than that of the row with the largest
+__device__ __forceinline__ int weight_shift(int largest_rows, int row) { return min(0, largest_rows - row); }
 // device words, of the state and of a backward pass: rows that count; bits of the largest finite |x|, |w| and |G|; slices of dx
 enum { CELL_ROWS, CELL_X, CELL_W, CELL_G, CELL_SLICES, CELLS = 64 };
-// Behind those of the state, for bf16, the bits of the largest finite |x| that work-groups have found, each in one of 16 words 64 bytes apart: one word
+// Behind those of the state, for 16-bit types, the bits of the largest finite |x| that work-groups have found, each in one of 16 words 64 bytes apart: one word
 // for all held up the copy of 8184 rows of 512 by 11 us.
 constexpr int kMost = 16, kParts = 1024;
 // the largest of `count` words is that of a matrix
@@ -54,7 +59,7 @@ struct LossPlan {
   size_t state, fwd, bwd;                 // bytes
   size_t s_map, s_place, s_label, s_norm, s_own;                            // offsets in the state
   size_t f_part, f_target, f_loss, f_x, f_w, f_most;                         // in the forward's workspace
-  size_t b_cells, b_most, b_g, b_x, b_w, b_grad, b_dx, b_dw;                   // in the backward's
+  size_t b_cells, b_most, b_g, b_shift, b_x, b_xg, b_w, b_grad, b_dx, b_dw;    // in the backward's
 };
 
 static size_t up(size_t v, size_t to) { return (v + to - 1) / to * to; }
@@ -127,7 +132,9 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.b_cells = take(CELLS * 4);
   p.b_most = take((2 * kParts + (size_t)(p.npad + 1023) / 1024) * 4);
   p.b_g = take((size_t)p.npad * 4);
+  p.b_shift = take((size_t)p.npad * 4);
   p.b_x = take(p.npad * row * planes);
+  p.b_xg = take(p.npad * row * planes);
   p.b_w = take(p.bwd_rows * row * planes);
   p.b_grad = take((size_t)g_planes * p.npad * p.bwd_rows * 2);
   // (rows of the slices: no more than kSliceTiles tiles of them where there are two or more)
@@ -221,6 +228,12 @@ __device__ __forceinline__ unsigned largest_of(const LossFound& f) {
   for (int i = threadIdx.x; i < f.count; i += 256) best = max(best, f.words[i * f.stride]);
   return largest_of(best);
 }
+// of all rows from that of each 1024 of the `live` ones
+__device__ __forceinline__ unsigned largest_weight(const unsigned* most, int live) {
+  unsigned best = 0;
+  for (int i = threadIdx.x; i < (live + 1023) / 1024; i += 256) best = max(best, most[i]);
+  return largest_of(best);
+}
 // Into one of `words`.  (Whoever finds a larger one there already has nothing to say: with an atomic a wave, 16384 of them on one address, the
 // kernel took 100 us for 8 MB.)
 __device__ __forceinline__ void largest_into(unsigned best, unsigned* words, int block) {
@@ -241,13 +254,15 @@ struct LossMost {
 };
 struct LossBegin {
   LossMost of[2];
-  // the backward's weights (work-groups behind those): g of the rows that count, and of each 1024 of them the bits of the largest finite |G|
+  // the backward's weights (work-groups behind those): g of the rows that count, the power of two that their G is scaled by, and of each 1024 of
+  // them the bits of the largest finite |G|
   const float* dloss;
   int reduction;
   const int* map;
   const unsigned* count;
   const float* own;
   float* g;
+  int* row_shift;
   unsigned* most;
 };
 // What has to be known of the operands before they are copied
@@ -263,7 +278,10 @@ __global__ __launch_bounds__(256) void loss_begin_kernel(const LossBegin G) {
       if (i >= live) break;
       const float v = G.reduction == 0 ? G.dloss[G.map[i]] : G.reduction == 1 ? G.dloss[0] / (float)live : G.dloss[0];
       G.g[i] = v;
-      best = max(best, finite_bits(v * G.own[i]));
+      const float size = v * G.own[i];
+      const unsigned bits = finite_bits(size);
+      G.row_shift[i] = bits != 0 || size == 0.f ? grad_shift(bits) : 0;      // (what is not finite stays that)
+      best = max(best, bits);
     }
     best = largest_of(best);
     if (threadIdx.x == 0) G.most[third] = best;
@@ -293,8 +311,8 @@ __global__ __launch_bounds__(256) void loss_begin_kernel(const LossBegin G) {
 }
 
 // Rows (named by map, or all) as planes of kp columns, those past `cols` zero; rows past the last one up to a multiple of 64 zero too.
-// found: the values are scaled below 2^15 by the power of two that suits the largest (none: they are not).  most: their own largest goes there.
-// back: the last 64 columns end with the row's last value, `back` zeros before what is left (TileProduct::run).
+// found: the values are scaled below 2^15 by the power of two that suits the largest (none, or as_is: they are not).  most: their own largest
+// goes there.  weighted: a second copy, scaled, of rows times what they weigh in dw (weight_shift).  back: the last 64 columns end with the row's last value, `back` zeros before what is left (TileProduct::run).
 struct LossRows {
   const void* src;
   long ld;
@@ -306,6 +324,9 @@ struct LossRows {
   long plane;
   unsigned* most;
   int back, blocks;
+  bool as_is;
+  void* weighted;
+  const int* row_shift;
 };
 struct LossCopy {
   LossRows of[2];
@@ -328,9 +349,7 @@ __device__ __forceinline__ void loss_cells(const LossCopy& G) {
     }
   if (G.most == nullptr) return;
   const int live = (int)*G.count;
-  unsigned best = 0;
-  for (int i = tid; i < (live + 1023) / 1024; i += 256) best = max(best, G.most[i]);
-  best = largest_of(best);
+  const unsigned best = largest_weight(G.most, live);
   if (tid == 0) G.cells[CELL_G] = best;
   if (tid < kMaxSlices) {
     const int n = tid + 1, tiles = G.tiles_m * ((live + G.tile - 1) / G.tile), rounds = (tiles * n + 255) / 256;
@@ -372,16 +391,12 @@ __global__ __launch_bounds__(256) void loss_planes_kernel(const LossCopy G) {
       for (int e = 0; e < 8; ++e) best = max(best, finite_bits(v[u][e]));
     largest_into(best, M.most, block);
   }
-  const int shift = M.found.words != nullptr ? plane_shift(largest_of(M.found)) : 0;
-#pragma unroll
-  for (int u = 0; u < kCopies; ++u) {
-    const unsigned i = first + u * 256;
-    const int r = (int)(i / per), c = (int)(i - r * per) * 8;
-    if (r >= pad) break;
+  const int scale = M.found.words != nullptr ? plane_shift(largest_of(M.found)) : 0, shift = M.as_is ? 0 : scale;
+  auto store = [&](void* dst, int u, int r, int c, int by) {
     typename PlaneVec<D>::x8 hi, lo;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x = shift != 0 ? __builtin_ldexpf(v[u][e], shift) : v[u][e];
+      const float x = by != 0 ? __builtin_ldexpf(v[u][e], by) : v[u][e];
       if constexpr (P == 2) {
         const Halves s = halves_of(x);
         hi[e] = s.hi;
@@ -390,9 +405,18 @@ __global__ __launch_bounds__(256) void loss_planes_kernel(const LossCopy G) {
         hi[e] = (D)x;
       }
     }
-    D* to = (D*)M.dst + (long)r * G.kp + c;
+    D* to = (D*)dst + (long)r * G.kp + c;
     *reinterpret_cast<decltype(hi)*>(to) = hi;
     if (P == 2) *reinterpret_cast<decltype(lo)*>(to + M.plane) = lo;
+  };
+  const int largest_rows = M.weighted != nullptr ? grad_shift(largest_weight(G.most, live)) : 0;
+#pragma unroll
+  for (int u = 0; u < kCopies; ++u) {
+    const unsigned i = first + u * 256;
+    const int r = (int)(i / per), c = (int)(i - r * per) * 8;
+    if (r >= pad) break;
+    store(M.dst, u, r, c, shift);
+    if (M.weighted != nullptr) store(M.weighted, u, r, c, scale + (r < live ? weight_shift(largest_rows, M.row_shift[r]) : 0));
   }
 }
 
@@ -412,7 +436,7 @@ struct LossTileArgs {
   // backward
   const float2* norm;                      // maximum, log2 of the sum
   const float *own, *g;                    // -r / (1 + r)
-  const unsigned* g_cell;
+  const int* row_shift;
   _Float16* grad;                          // [grad_planes][npad][grad_ld]
   long grad_plane;
   int grad_ld, grad_planes;
@@ -449,7 +473,6 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
   const int unscale = SCALED && G.x_cell != nullptr ? -(plane_shift(*G.x_cell) + plane_shift(*G.w_cell)) : 0;
   const bool cut = m0 + Tiles::TM > G.vend;      // entries past the last one
   constexpr int PART = Tiles::TM / Tiles::WM;
-  const int g_shift = GRAD ? grad_shift(*G.g_cell) : 0;
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j) {
     const int token = n0 + t.col_of(j);
@@ -499,6 +522,7 @@ __global__ __launch_bounds__(Tiles::THREADS, 2) void loss_tile_kernel(const Loss
     } else {
       const int pad = (live + 63) / 64 * 64;
       const float2 norm = ok ? G.norm[token] : make_float2(0.f, 0.f);
+      const int g_shift = ok ? G.row_shift[token] : 0;
       const float g = ok ? G.g[token] : 0.f, shift = (float)g_shift - norm.y;
 #pragma unroll
       for (int i = 0; i < Tiles::MI; ++i)
@@ -807,10 +831,11 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const float* loss, const
 // ------------------------------------------------------------------------------------ gradients
 
 struct LossGradArgs {
-  const _Float16 *grad, *w, *x;       // G [npad][grad_ld]; w [piece][kp]; x [npad][kp]
+  const _Float16 *grad, *w, *x;       // G [npad][grad_ld]; w [piece][kp]; x [npad][kp], weighted
   long grad_plane, w_plane, x_plane;
   int grad_ld, kp, tiles_m, entries;
   const unsigned *count, *w_cell, *x_cell, *g_cell;
+  const int* row_shift;
   // dx
   float* sums;                        // [slices][live rows up to a multiple of 64][kp]
   int first;                          // first piece
@@ -837,17 +862,18 @@ __device__ __forceinline__ void loss_dx(const LossGradArgs& G, char* shared) {
   t.operand_a(G.w, G.w_plane, G.kp, m0, G.kp);
   t.operand_b(G.grad, G.grad_plane, G.grad_ld, n0, live);
   t.run(steps, from);
-  // (all pieces share the power of two)
-  const int shift = -grad_shift(*G.g_cell) - (G.w_cell != nullptr ? plane_shift(*G.w_cell) : 0);
+  const int of_w = G.w_cell != nullptr ? plane_shift(*G.w_cell) : 0;
   float* sums = G.sums + (size_t)split * ((live + 63) / 64 * 64) * G.kp;
 #pragma unroll
-  for (int j = 0; j < Tiles::NI; ++j)
+  for (int j = 0; j < Tiles::NI; ++j) {
+    const int shift = -G.row_shift[min(n0 + t.col_of(j), live - 1)] - of_w;
     t.template rows_of<float>(shared, [&](int i, int e) { return __builtin_ldexpf(t.acc[i][j][e], shift); }, [&](int r, int c, floatx4 v) {
       const int token = n0 + t.col_of(j) - (t.lane & 31) + r, col = m0 + t.wm * Tiles::W + c;
       if (token >= live || col >= G.kp) return;
       floatx4* at = reinterpret_cast<floatx4*>(sums + (size_t)token * G.kp + col);
       *at = G.first ? v : *at + v;
     });
+  }
 }
 
 // dw of the piece: features (registers) by entries of the vocabulary (lanes), over all rows or (SLICES, unscaled fp32 [splits][entries][kp]) a slice of them
@@ -866,7 +892,7 @@ __device__ __forceinline__ void loss_dw(const LossGradArgs& G, char* shared) {
   } else {
     t.run(steps);
   }
-  const int shift = -grad_shift(*G.g_cell) - (G.x_cell != nullptr ? plane_shift(*G.x_cell) : 0);
+  const int shift = -grad_shift(*G.g_cell) - plane_shift(*G.x_cell);
   O* dw = (O*)G.dw + (SLICES ? (size_t)split * G.entries * G.dw_ld : 0);
 #pragma unroll
   for (int j = 0; j < Tiles::NI; ++j)
@@ -984,7 +1010,7 @@ static void begin(const nsa_loss_desc* d, const LossBegin& a, int blocks, hipStr
 }
 static LossRows rows_to(const LossPlan& p, const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, const LossFound& found, void* dst,
                         long plane, unsigned* most = nullptr, int back = 0) {
-  return LossRows{src, ld, rows, cols, map, count, found, dst, plane, most, back, (int)blocks_for(((long)up(rows, 64) * p.kp / 8 + kCopies - 1) / kCopies)};
+  return LossRows{src, ld, rows, cols, map, count, found, dst, plane, most, back, (int)blocks_for(((long)up(rows, 64) * p.kp / 8 + kCopies - 1) / kCopies), false, nullptr, nullptr};
 }
 template <class S, class D, int P>
 static void copy(const LossCopy& a, hipStream_t st) {
@@ -1079,8 +1105,8 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
       LossCopy c{};
       c.kp = p.kp;
       if (v0 == 0) {
-        // (a bf16 backward pass wants to know the largest |x|)
-        c.of[0] = rows_to(p, x, d->x_stride, p.n, d->dim, map, count, of_x, w + p.f_x, x_plane, d->dtype == 0 ? cells + CELLS : nullptr, back);
+        // (a 16-bit backward pass wants to know the largest |x|)
+        c.of[0] = rows_to(p, x, d->x_stride, p.n, d->dim, map, count, of_x, w + p.f_x, x_plane, scaled ? nullptr : cells + CELLS, back);
         c.cells = scaled ? cells : nullptr;
       }
       if (p.in_place) {
@@ -1133,13 +1159,15 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
   const unsigned* count = kept + CELL_ROWS;
   float* g = (float*)(w + p.b_g);
   const int each = d->dtype == 2 ? 4 : 2, tile = p.size == WIDE ? 256 : 128, tiles_m = (p.kp + tile - 1) / tile;
-  // All operands in fp16: x once, w with each piece.  Magnitudes: those the forward has found, else here.
+  int* row_shift = (int*)(w + p.b_shift);
+  // All operands in fp16: x once (for the logits as it is where it is fp16, for dw weighted), w with each piece.  Magnitudes: those the forward has
+  // found, else here.
   const bool scaled = d->dtype != 1;
   LossBegin b{};
   LossFound of_x{}, of_w{};
-  if (scaled && p.size != FEW) {
+  if (p.size != FEW) {
     of_x = d->dtype == 2 ? found(kept + CELL_X) : LossFound{kept + CELLS, kMost, 16};
-  } else if (scaled) {
+  } else {
     b.of[0] = most_to(x, d->x_stride, p.n, d->dim, map, count, parts);
     of_x = found(b.of[0]);
   }
@@ -1149,13 +1177,12 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
     b.of[1] = most_to(weight, d->w_stride, d->vocab, d->dim, nullptr, nullptr, parts + kParts);
     of_w = found(b.of[1]);
   }
-  b.dloss = dloss; b.reduction = d->reduction; b.map = map; b.count = count; b.own = (const float*)(s + p.s_own); b.g = g; b.most = g_most;
+  b.dloss = dloss; b.reduction = d->reduction; b.map = map; b.count = count; b.own = (const float*)(s + p.s_own); b.g = g; b.row_shift = row_shift; b.most = g_most;
   begin(d, b, (p.n + 1023) / 1024, st);
   const long x_plane = (long)p.npad * p.kp;
-  void* xg = w + p.b_x;
   LossGradArgs q{};
-  q.kp = p.kp; q.count = count; q.g_cell = cells + CELL_G; q.tiles_m = tiles_m; q.slices = cells + CELL_SLICES;
-  q.x = (const H16*)xg; q.x_plane = x_plane; q.x_cell = scaled ? cells + CELL_X : nullptr; q.w = (const H16*)(w + p.b_w); q.w_cell = scaled ? cells + CELL_W : nullptr; q.sums = (float*)(w + p.b_dx);
+  q.kp = p.kp; q.count = count; q.g_cell = cells + CELL_G; q.row_shift = row_shift; q.tiles_m = tiles_m; q.slices = cells + CELL_SLICES;
+  q.x = (const H16*)(w + p.b_xg); q.x_plane = x_plane; q.x_cell = cells + CELL_X; q.w = (const H16*)(w + p.b_w); q.w_cell = scaled ? cells + CELL_W : nullptr; q.sums = (float*)(w + p.b_dx);
   for (long v0 = 0; v0 < d->vocab; v0 += p.bwd_rows) {
     LossTileArgs a{};
     a.v0 = (int)v0;
@@ -1166,7 +1193,8 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
     LossCopy c{};
     c.kp = p.kp;
     if (v0 == 0) {
-      c.of[0] = rows_to(p, x, d->x_stride, p.n, d->dim, map, count, of_x, xg, x_plane);
+      c.of[0] = rows_to(p, x, d->x_stride, p.n, d->dim, map, count, of_x, w + p.b_x, x_plane);
+      c.of[0].as_is = !scaled; c.of[0].weighted = dw ? w + p.b_xg : nullptr; c.of[0].row_shift = row_shift;
       c.most = g_most; c.count = count; c.cells = cells; c.tiles_m = tiles_m; c.tile = tile; c.piece = std::min(p.bwd_rows, (int)up(d->vocab, 64));
     }
     c.of[1] = rows_to(p, (const char*)weight + v0 * d->w_stride * each, d->w_stride, entries, d->dim, nullptr, nullptr, of_w, wg, w_plane);
@@ -1175,9 +1203,9 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
     else copy<H16, H16, 1>(c, st);
     if (scaled) of_w = found(cells + CELL_W);
     a.w = wg; a.w_ld = p.kp; a.w_plane = w_plane;
-    a.x = xg; a.x_plane = x_plane; a.kp = p.kp; a.n = p.n; a.npad = p.npad;
-    a.count = count; a.x_cell = q.x_cell; a.w_cell = q.w_cell; a.label = label;
-    a.norm = (const float2*)(s + p.s_norm); a.own = (const float*)(s + p.s_own); a.g = g; a.g_cell = cells + CELL_G;
+    a.x = w + p.b_x; a.x_plane = x_plane; a.kp = p.kp; a.n = p.n; a.npad = p.npad;
+    a.count = count; a.x_cell = scaled ? q.x_cell : nullptr; a.w_cell = q.w_cell; a.label = label;
+    a.norm = (const float2*)(s + p.s_norm); a.own = (const float*)(s + p.s_own); a.g = g; a.row_shift = row_shift;
     a.grad = (H16*)(w + p.b_grad); a.grad_plane = (long)p.npad * ld; a.grad_ld = ld; a.grad_planes = p.grad_P == 1 ? 1 : 2;
     if (p.grad_P == 2) launch_tiles<H16, 2, true>(p, a, st);
     else launch_tiles<H16, 1, true>(p, a, st);
