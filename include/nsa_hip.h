@@ -525,7 +525,7 @@ int nsa_decode_prep(const void* q, const int64_t* q_stride, const void* k, const
  *   `state` is written by nsa_loss_fwd and read by nsa_loss_bwd (any number of times); ws is dead after either call.
  *   dloss: fp32, as loss; dx [rows, dim], dw [vocab, dim] contiguous, of `dtype`; either may be NULL.  rows >= 1 for the backward.
  * Sums in fp32; fp32 operands as two fp16 halves each (22 bits; what is below 2^-18 of a matrix's largest value is kept to 2^-40 of that), results
- * rounded once.  The gradient of a row's logits is scaled by itself, whatever other rows weigh, and kept to 2^-38 of the row's largest; for dw also to
+ * rounded once; bf16 gradients, from an 11-bit gradient of the logits, are off by up to 1.05 times that rounding.  The gradient of a row's logits is scaled by itself, whatever other rows weigh, and kept to 2^-38 of the row's largest; for dw also to
  * 2^-38 of the largest row's.  Infinities and NaN among the weights may make NaN of any logit of their entry.  The order of the additions depends on sizes, the
  * weight's stride and alignment, and the number of counting rows only.  Alignment: that of the type; state and ws: 256 bytes.
  * rows <= 2^24, dim <= 2^16, vocab <= 2^24, either of rows and vocab times dim (rounded up to 64) below 2^33 (NSA_E_UNSUPPORTED otherwise). */

@@ -21,7 +21,7 @@
 // power of two for all rows, a row whose label is likely, or whose g is small, lost its others' G: a row with r = 1.2e-8 beside one with a loss
 // near 1 had a dx off by several times its norm.)  The other operands of those products, w and x, are scaled by powers of two into fp16's range and
 // lose nothing that is above 2^-29 of their largest value.
-// fp32 operands are two fp16 planes each, G too (nsa_tiles.hpp); fp16 ones are exact in one, and G two where that is cheap (loss_plan).
+// fp32 operands are two fp16 planes each, G too (nsa_tiles.hpp); fp16 ones are exact in one beside two of G.
 #include <algorithm>
 #include <cmath>
 #include "nsa_tiles.hpp"
@@ -74,10 +74,10 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.npad = (int)up(std::max<size_t>(p.n, 1), 64);
   p.kp = (int)up(d->dim, 64);
   p.P = d->dtype == 2 ? 2 : 1;
-  // fp16 results have as many bits as an fp16 G, and hang on single entries of it, the labels': its rounding makes them 1.41 times as far off as
-  // their own alone.  Two halves of G cost a product more for dx and dw each; they are taken where that is little (2^33: 35 us of products) or
-  // where few rows make 1.41 as likely to be 1.6.  (2047 rows, 768 features, 32000 entries: 483 us and dw 1.2 times its own rounding off, 750 with two halves.)
-  p.grad_P = d->dtype == 2 ? 2 : d->dtype == 1 && (p.n <= 256 || (double)p.n * d->vocab * d->dim < 8589934592.0) ? ONE_BY_TWO : 1;
+  // fp16 results have as many bits as an fp16 G, and hang on single entries of it, the labels': its rounding would make them up to 1.41 times as far
+  // off as their own alone, so fp16 takes two halves of G, a product more for dx and dw each.  (2047 rows, 768 features, 32000 entries: 720-760 us;
+  // 475 with one half, and dw off by 1.2 times its own rounding.)  bf16 results have an eighth of G's bits: 1.01 times their rounding with one half.
+  p.grad_P = d->dtype == 2 ? 2 : d->dtype == 1 ? ONE_BY_TWO : 1;
   // The tiles whose rounds end first: time of a round on all places, in us for each feature and beside that (products measured from 512 to 4096
   // features, the maxima and sums of a tile beside them).  256 x 256 tiles have no registers for sums in pieces (TileProduct::PIECES), so long
   // fp32 rows do without them: at 2066 features the gradients were 2.8e-6 off, 7 times as much as fp32 products by the library.
@@ -1024,7 +1024,7 @@ static void products(const LossPlan& p, const LossGradArgs& q, bool dx, hipStrea
   const int tile = p.size == WIDE ? 256 : 128, all = q.tiles_m * ((p.n + tile - 1) / tile);
   const dim3 grid((unsigned)(q.dw_tiles + (dx ? std::max(all, std::min(kMaxSlices * all, kSliceTiles)) : 0))), block(512);
   // few rows: nothing to read ahead, so two work-groups a CU that write in turn (25 rows, 1917 features, 21120 entries in bf16: 36 -> 24 us)
-  if constexpr (!SLICES && !(P == 1 && std::is_same<O, H16>::value))      // (few rows of fp16 have two planes of G)
+  if constexpr (!SLICES)
     if (p.size == FEW) {
       hipLaunchKernelGGL((loss_products_kernel<typename T::FewX, typename T::FewW, O, SLICES>), grid, block, 0, st, q);
       return;
@@ -1222,7 +1222,6 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
     else if (slices) products<ONE_BY_TWO, float, true>(p, q, dx, st);
     else if (d->dtype == 0) products<1, B16, false>(p, q, dx, st);
     else if (d->dtype == 2) products<2, float, false>(p, q, dx, st);
-    else if (p.grad_P == 1) products<1, H16, false>(p, q, dx, st);
     else products<ONE_BY_TWO, H16, false>(p, q, dx, st);
     if (slices) rows_of_slices(d, q, (const float*)(w + p.b_dw), entries, entries, nullptr, to, st);
   }
