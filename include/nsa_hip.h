@@ -528,7 +528,8 @@ int nsa_decode_prep(const void* q, const int64_t* q_stride, const void* k, const
  * rounded once; bf16 gradients, from an 11-bit gradient of the logits, are off by up to 1.05 times that rounding.  The gradient of a row's logits is scaled by itself, whatever other rows weigh, and kept to 2^-38 of the row's largest; for dw also to
  * 2^-38 of the largest row's.  Infinities and NaN among the weights may make NaN of any logit of their entry.  The order of the additions depends on sizes, the
  * weight's stride and alignment, and the number of counting rows only.  Alignment: that of the type; state and ws: 256 bytes.
- * rows <= 2^24, dim <= 2^16, vocab <= 2^24, either of rows and vocab times dim (rounded up to 64) below 2^33 (NSA_E_UNSUPPORTED otherwise). */
+ * rows <= 2^24, dim <= 2^16, vocab <= 2^24, either of rows and vocab times dim (rounded up to 64) below 2^33, and rows times vocab such that a launch
+ * of 2^32 threads holds their tiles: up to 2^36 always, to about 2^39 where tiles are 256 x 256 (NSA_E_UNSUPPORTED otherwise). */
 typedef struct nsa_loss_desc {
   int64_t rows;
   int32_t dim, vocab;

@@ -102,6 +102,11 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.in_place = d->dtype != 2 && d->dim % 8 == 0 && d->dim >= 64 && d->w_stride % 8 == 0 && d->w_stride < (1 << 20) && ((uintptr_t)weight & 15) == 0;
   const size_t v256 = up(d->vocab, 256), v64 = up(d->vocab, 64), row = (size_t)p.kp * 2;
   p.fwd_rows = (int)std::min(v256, std::max<size_t>(256, ((size_t)256 << 20) / (row * p.P) / 256 * 256));
+  // (a launch has fewer than 2^32 threads; backward pieces of more than 1024 entries are no larger than 2^27 values, others than 2^34)
+  if (p.size != FEW) {
+    const size_t entries = p.in_place ? d->vocab : std::min<size_t>(p.fwd_rows, d->vocab), side = p.tile;
+    if ((up(entries, side) / side) * (up(p.n, side) / side) * (p.size == TINY ? 256 : 512) >> 32) return NSA_E_UNSUPPORTED;
+  }
   const int planes = p.grad_P == 2 ? 2 : 1, g_planes = p.grad_P == 1 ? 1 : 2;
   // a piece's G: up to 256 MB
   p.bwd_rows = (int)std::min(v256, std::max<size_t>(1024, ((size_t)256 << 20) / ((size_t)g_planes * p.npad * 2) / 1024 * 1024));
