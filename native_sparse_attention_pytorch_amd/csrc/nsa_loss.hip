@@ -58,13 +58,14 @@ struct LossPlan {
   int w_splits, last_splits;              // slices of the rows that dw of a piece, of the last one, is summed from
   size_t state, fwd, bwd;                 // bytes
   size_t s_map, s_place, s_label, s_norm, s_own;                            // offsets in the state
-  size_t f_part, f_target, f_loss, f_x, f_w, f_most;                         // in the forward's workspace
+  size_t f_part, f_target, f_loss, f_x, f_w, f_most, f_count;                        // in the forward's workspace
   size_t b_cells, b_most, b_g, b_shift, b_x, b_xg, b_w, b_grad, b_dx, b_dw;    // in the backward's
 };
 
 static size_t up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
 constexpr int kMaxSlices = 32, kSliceTiles = 512;      // of dx
+constexpr int kRowsUncounted = 32768;                  // loss_rows_kernel
 
 static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   if (!d || d->rows < 0 || d->dim <= 0 || d->vocab <= 0 || d->dtype < 0 || d->dtype > 2 || d->reduction < 0 || d->reduction > 2) return NSA_E_ARG;
@@ -132,6 +133,7 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.f_x = take(p.size == FEW ? 0 : p.npad * row * p.P);
   p.f_w = take(p.size == FEW || p.in_place ? 0 : p.fwd_rows * row * p.P);
   p.f_most = take(d->dtype == 2 ? 2 * kParts * 4 : 0);
+  p.f_count = take(p.n > kRowsUncounted ? (size_t)(p.npad + 1023) / 1024 * 4 : 0);
   p.fwd = at;
   at = 0;
   p.b_cells = take(CELLS * 4);
@@ -151,16 +153,40 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
 
 // ------------------------------------------------------------------------------------ rows that count
 
+__device__ __forceinline__ long label_at(const void* labels, int is64, int i) { return is64 ? ((const long*)labels)[i] : (long)((const int*)labels)[i]; }
+// counts[b]: rows among 1024 b .. 1024 b + 1023 that count
+__global__ __launch_bounds__(256) void loss_count_kernel(const void* labels, int is64, int n, long ignore, int* counts) {
+  __shared__ int sums[4];
+  const int tid = threadIdx.x;
+  int count = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int row = blockIdx.x * 1024 + e * 256 + tid;
+    count += row < n && label_at(labels, is64, row) != ignore;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) count += __shfl_xor(count, o);
+  if ((tid & 63) == 0) sums[tid >> 6] = count;
+  __syncthreads();
+  if (tid == 0) counts[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
+}
 // map[c] = row of the c-th row that counts, label[c] = its label (-1: outside the vocabulary), place[row] = c or -1.  A work-group takes
-// 1024 rows; how many count before them it finds out itself (8 bytes a row from L2: 4 us at 16384 rows, and no second launch).
-__global__ __launch_bounds__(256) void loss_rows_kernel(const void* labels, int is64, int n, int vocab, long ignore, int* map, int* place, int* label,
-                                                        unsigned* cells, float* losses) {
+// 1024 rows; how many count before them it finds out itself, from the labels (8 bytes a row from L2, and no second launch) or, of
+// many rows, from counts of 1024 each.  (From labels 16384 rows take 7 us, 32768 10, 65536 17, 4194304 5.7 ms; from counts, with their kernel,
+// 65536 6 us and 4194304 29.)
+__global__ __launch_bounds__(256) void loss_rows_kernel(const void* labels, int is64, int n, int vocab, long ignore, const int* counts, int* map, int* place,
+                                                        int* label, unsigned* cells, float* losses) {
   __shared__ int sums[8];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, first = blockIdx.x * 1024;
-  auto at = [&](int i) { return is64 ? ((const long*)labels)[i] : (long)((const int*)labels)[i]; };
+  auto at = [&](int i) { return label_at(labels, is64, i); };
   int before = 0;
+  if (counts != nullptr) {
 #pragma unroll 8
-  for (int i = tid; i < first; i += 256) before += at(i) != ignore;
+    for (int i = tid; i < (int)blockIdx.x; i += 256) before += counts[i];
+  } else {
+#pragma unroll 8
+    for (int i = tid; i < first; i += 256) before += at(i) != ignore;
+  }
   long mine[4];
   int count = 0;
 #pragma unroll
@@ -231,12 +257,6 @@ __device__ __forceinline__ unsigned largest_of(const LossFound& f) {
   if (f.count == 1) return *f.words;
   unsigned best = 0;
   for (int i = threadIdx.x; i < f.count; i += 256) best = max(best, f.words[i * f.stride]);
-  return largest_of(best);
-}
-// of all rows from that of each 1024 of the `live` ones
-__device__ __forceinline__ unsigned largest_weight(const unsigned* most, int live) {
-  unsigned best = 0;
-  for (int i = threadIdx.x; i < (live + 1023) / 1024; i += 256) best = max(best, most[i]);
   return largest_of(best);
 }
 // Into one of `words`.  (Whoever finds a larger one there already has nothing to say: with an atomic a wave, 16384 of them on one address, the
@@ -332,6 +352,7 @@ struct LossRows {
   bool as_is;
   void* weighted;
   const int* row_shift;
+  LossFound rows_most;      // of |G|
 };
 struct LossCopy {
   LossRows of[2];
@@ -339,7 +360,8 @@ struct LossCopy {
   // The first copy of a pass: one more work-group leaves the largest of both matrices here, and in a backward pass that of G (`most`: of
   // each 1024) and the slices of a piece's entries that dx is summed from
   unsigned* cells;
-  const unsigned *most, *count;
+  LossFound most;
+  const unsigned* count;
   int tiles_m, tile, piece;
 };
 // Slices of dx: those whose rounds on 256 CUs end first, where a tile's beginning and end, and its share of the sum of slices, cost as much as 512
@@ -352,9 +374,9 @@ __device__ __forceinline__ void loss_cells(const LossCopy& G) {
       const unsigned best = largest_of(G.of[i].found);
       if (tid == 0) G.cells[i == 0 ? CELL_X : CELL_W] = best;
     }
-  if (G.most == nullptr) return;
+  if (G.most.words == nullptr) return;
   const int live = (int)*G.count;
-  const unsigned best = largest_weight(G.most, live);
+  const unsigned best = largest_of(G.most);
   if (tid == 0) G.cells[CELL_G] = best;
   if (tid < kMaxSlices) {
     const int n = tid + 1, tiles = G.tiles_m * ((live + G.tile - 1) / G.tile), rounds = (tiles * n + 255) / 256;
@@ -414,7 +436,7 @@ __global__ __launch_bounds__(256) void loss_planes_kernel(const LossCopy G) {
     *reinterpret_cast<decltype(hi)*>(to) = hi;
     if (P == 2) *reinterpret_cast<decltype(lo)*>(to + M.plane) = lo;
   };
-  const int largest_rows = M.weighted != nullptr ? grad_shift(largest_weight(G.most, live)) : 0;
+  const int largest_rows = M.weighted != nullptr ? grad_shift(largest_of(M.rows_most)) : 0;
 #pragma unroll
   for (int u = 0; u < kCopies; ++u) {
     const unsigned i = first + u * 256;
@@ -1015,7 +1037,7 @@ static void begin(const nsa_loss_desc* d, const LossBegin& a, int blocks, hipStr
 }
 static LossRows rows_to(const LossPlan& p, const void* src, long ld, int rows, int cols, const int* map, const unsigned* count, const LossFound& found, void* dst,
                         long plane, unsigned* most = nullptr, int back = 0) {
-  return LossRows{src, ld, rows, cols, map, count, found, dst, plane, most, back, (int)blocks_for(((long)up(rows, 64) * p.kp / 8 + kCopies - 1) / kCopies), false, nullptr, nullptr};
+  return LossRows{src, ld, rows, cols, map, count, found, dst, plane, most, back, (int)blocks_for(((long)up(rows, 64) * p.kp / 8 + kCopies - 1) / kCopies), false, nullptr, nullptr, LossFound{}};
 }
 template <class S, class D, int P>
 static void copy(const LossCopy& a, hipStream_t st) {
@@ -1087,8 +1109,11 @@ extern "C" int nsa_loss_fwd(const nsa_loss_desc* d, const void* x, const void* w
     const auto kernel = d->dtype == 0 ? few_kernel<B16>(aligned, p.tile == 32) : d->dtype == 1 ? few_kernel<H16>(aligned, p.tile == 32) : few_kernel<float>(aligned, p.tile == 32);
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
   } else {
-    hipLaunchKernelGGL(loss_rows_kernel, dim3((unsigned)((p.n + 1023) / 1024)), dim3(256), 0, st, labels, (int)d->labels_int64, p.n, d->vocab,
-                       (long)d->ignore_index, map, place, label, cells, losses);
+    const dim3 grid((unsigned)((p.n + 1023) / 1024));
+    int* counts = p.n > kRowsUncounted ? (int*)(w + p.f_count) : nullptr;
+    if (counts) hipLaunchKernelGGL(loss_count_kernel, grid, dim3(256), 0, st, labels, (int)d->labels_int64, p.n, (long)d->ignore_index, counts);
+    hipLaunchKernelGGL(loss_rows_kernel, grid, dim3(256), 0, st, labels, (int)d->labels_int64, p.n, d->vocab, (long)d->ignore_index, (const int*)counts, map,
+                       place, label, cells, losses);
     const long x_plane = (long)p.npad * p.kp;
     const int back = p.in_place ? p.kp - d->dim : 0;
     const bool scaled = d->dtype == 2;
@@ -1200,12 +1225,23 @@ extern "C" int nsa_loss_bwd(const nsa_loss_desc* d, const void* x, const void* w
     if (v0 == 0) {
       c.of[0] = rows_to(p, x, d->x_stride, p.n, d->dim, map, count, of_x, w + p.b_x, x_plane);
       c.of[0].as_is = !scaled; c.of[0].weighted = dw ? w + p.b_xg : nullptr; c.of[0].row_shift = row_shift;
-      c.most = g_most; c.count = count; c.cells = cells; c.tiles_m = tiles_m; c.tile = tile; c.piece = std::min(p.bwd_rows, (int)up(d->vocab, 64));
+      c.most = c.of[0].rows_most = LossFound{g_most, (p.n + 1023) / 1024, 1};
+      c.count = count; c.cells = cells; c.tiles_m = tiles_m; c.tile = tile; c.piece = std::min(p.bwd_rows, (int)up(d->vocab, 64));
     }
     c.of[1] = rows_to(p, (const char*)weight + v0 * d->w_stride * each, d->w_stride, entries, d->dim, nullptr, nullptr, of_w, wg, w_plane);
-    if (d->dtype == 0) copy<B16, H16, 1>(c, st);
-    else if (d->dtype == 2) copy<float, H16, 2>(c, st);
-    else copy<H16, H16, 1>(c, st);
+    auto make = [&](const LossCopy& a) {
+      if (d->dtype == 0) copy<B16, H16, 1>(a, st);
+      else if (d->dtype == 2) copy<float, H16, 2>(a, st);
+      else copy<H16, H16, 1>(a, st);
+    };
+    if (v0 == 0 && c.most.count > 64) {      // (many words for every work-group to read: once, in a launch before)
+      LossCopy only = c;
+      only.of[0].blocks = only.of[1].blocks = 0;
+      make(only);
+      c.cells = nullptr;
+      c.of[0].rows_most = found(cells + CELL_G);
+    }
+    make(c);
     if (scaled) of_w = found(cells + CELL_W);
     a.w = wg; a.w_ld = p.kp; a.w_plane = w_plane;
     a.x = w + p.b_x; a.x_plane = x_plane; a.kp = p.kp; a.n = p.n; a.npad = p.npad;
