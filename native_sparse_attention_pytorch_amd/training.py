@@ -122,26 +122,38 @@ class Muon(torch.optim.Optimizer):
     parameters too: gradients below 2^-8 of the buffer would be lost in bf16.
 
         masters = Fp32Masters(model)
-        matrices = [m for m, (name, p) in zip(masters.masters, model.named_parameters()) if p.dim() == 2 and "emb" not in name]
+        matrices = [m for m, (name, p) in zip(masters.masters, model.named_parameters())
+                    if p.dim() == 2 and "token_emb" not in name and "to_logits" not in name]
         muon = Muon(matrices, lr=0.02)
+
+    A step that cannot be taken (a parameter that is not on a GPU, a sparse gradient, a group's number out of range) is refused before anything of it
+    is done.  Parameters may lie on several devices.
     """
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0., steps: int = 5,
                  coefficients=(3.4445, -4.7750, 2.0315), eps: float = 1e-7):
-        if lr < 0 or weight_decay < 0 or not 0 <= momentum < 1:
-            raise ValueError(f"Muon: lr {lr}, momentum {momentum}, weight_decay {weight_decay}")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
                                       coefficients=tuple(coefficients), eps=eps))
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2:
-                self.param_groups.pop()
-                raise ValueError(f"Muon takes matrices, got a parameter of shape {tuple(p.shape)}")
-            if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-                self.param_groups.pop()
-                raise ValueError(f"Muon takes fp32, bf16 or fp16 parameters, got {p.dtype}")
+        try:
+            self._check_numbers(self.param_groups[-1])
+            for p in self.param_groups[-1]["params"]:
+                if p.dim() < 2:
+                    raise ValueError(f"Muon takes matrices, got a parameter of shape {tuple(p.shape)}")
+                if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                    raise ValueError(f"Muon takes fp32, bf16 or fp16 parameters, got {p.dtype}")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check_numbers(group) -> None:
+        from . import ops
+        if not (group["lr"] >= 0 and group["weight_decay"] >= 0 and 0 <= group["momentum"] < 1):
+            raise ValueError(f"Muon: lr {group['lr']}, momentum {group['momentum']}, weight_decay {group['weight_decay']}")
+        ops.newton_schulz([], steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"])
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
@@ -159,10 +171,19 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        todo = []
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None and p.numel()]
-            if not params:
-                continue
+            if params:
+                self._check_numbers(group)
+            for p in params:
+                if not p.is_cuda:
+                    raise RuntimeError(f"Muon: a parameter on {p.device}: needs a GPU (HIP kernels, no CPU fallback)")
+                if p.grad.is_sparse:
+                    raise RuntimeError("Muon does not take sparse gradients")
+            for device in dict.fromkeys(p.device for p in params):
+                todo.append((group, float(group["lr"]), [p for p in params if p.device == device]))
+        for group, lr, params in todo:
             grads = [p.grad for p in params]
             for p in params:
                 if "momentum_buffer" not in self.state[p]:
@@ -173,7 +194,7 @@ class Muon(torch.optim.Optimizer):
             updates = torch._foreach_add(grads, buffers, alpha=group["momentum"]) if group["nesterov"] else buffers
             updates = ops.newton_schulz([u.flatten(1) for u in updates], steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"])
             if group["weight_decay"]:
-                torch._foreach_mul_(params, 1 - group["lr"] * group["weight_decay"])
-            torch._foreach_mul_(updates, [-group["lr"] * max(1., u.shape[0] / u.shape[1]) ** 0.5 for u in updates])
+                torch._foreach_mul_(params, 1 - lr * group["weight_decay"])
+            torch._foreach_mul_(updates, [-lr * max(1., u.shape[0] / u.shape[1]) ** 0.5 for u in updates])
             torch._foreach_add_(params, [u.view(p.shape) for u, p in zip(updates, params)])
         return loss
