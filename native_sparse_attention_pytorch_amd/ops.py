@@ -2646,9 +2646,23 @@ def _loss_desc(rows: int, weight: Tensor, x_stride: int, labels_int64: bool, ign
                        aligned=weight.data_ptr() % 16 == 0)
 
 
+def _check_loss(x: Tensor, weight: Tensor, labels: Tensor, rows) -> None:
+    """What the loss kernels can be given: they read by address.  `rows`: the shape that labels have to have, x's without its last axis."""
+    if not x.is_cuda or weight.device != x.device or labels.device != x.device:
+        raise RuntimeError("linear_cross_entropy: needs tensors on one GPU (HIP kernels, no CPU fallback)")
+    if x.dtype not in _LOSS_TYPES or weight.dtype != x.dtype:
+        raise RuntimeError(f"linear_cross_entropy: x {x.dtype}, weight {weight.dtype}: expected both bf16, both fp16 or both fp32")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or labels.shape != rows or 0 in weight.shape:
+        raise RuntimeError(f"linear_cross_entropy: x {tuple(x.shape)}, weight {tuple(weight.shape)}, labels {tuple(labels.shape)}: expected '... d', "
+                           "'v d' and '...'")
+
+
 @torch.library.custom_op("nsa_amd::linear_cross_entropy_fwd", mutates_args=())
 def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_index: int, reduction: int) -> tuple[Tensor, Tensor]:
     """(loss, what the gradients need): x 'n d', weight 'v d', labels 'n'; reduction 0 none, 1 mean, 2 sum."""
+    _check_loss(x, weight, labels, x.shape[:-1])      # (a traced graph calls this with what it is run on)
+    if x.dim() != 2 or labels.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError(f"linear_cross_entropy: x {tuple(x.shape)}, labels {labels.dtype}: expected 'n d' and int64 or int32")
     n = x.shape[0]
     with _on(x.device):
         x, weight, labels = _unit_rows(x), _unit_rows(weight), labels.contiguous()
@@ -2674,15 +2688,18 @@ def linear_cross_entropy_bwd(dloss: Tensor, x: Tensor, weight: Tensor, state: Te
                              want_dw: bool) -> tuple[Tensor, Tensor]:
     """(dx 'n d', dw 'v d'), empty where not wanted."""
     rows = x.shape[0]
+    _check_loss(x, weight, dloss, x.shape[:-1] if reduction == 0 else ())
+    if x.dim() != 2 or state.device != x.device or state.dtype != torch.uint8 or not state.is_contiguous():
+        raise RuntimeError(f"linear_cross_entropy: x {tuple(x.shape)}, state {state.dtype} on {state.device}: not those of a forward call")
     make = torch.empty if rows else torch.zeros
     with _on(weight.device):
         dx = make((rows if want_dx else 0, weight.shape[1]), dtype=weight.dtype, device=weight.device)
         dw = make(weight.shape if want_dw else (0, weight.shape[1]), dtype=weight.dtype, device=weight.device)
         if rows and (want_dx or want_dw):
             x, weight, dloss = _unit_rows(x), _unit_rows(weight), dloss.to(torch.float32).contiguous()
-            d, state_bytes, _, bwd_bytes = _loss_desc(rows, weight, x.stride(0), True, ignore_index, reduction)
+            d, _, _, bwd_bytes = _loss_desc(rows, weight, x.stride(0), True, ignore_index, reduction)
             ws = torch.empty((bwd_bytes,), dtype=torch.uint8, device=weight.device)
-            _lib.check(_lib.lib().nsa_loss_bwd(d, _ptr(x), _ptr(weight), _ptr(state), state_bytes, _ptr(dloss), _ptr(ws), bwd_bytes,
+            _lib.check(_lib.lib().nsa_loss_bwd(d, _ptr(x), _ptr(weight), _ptr(state), state.numel(), _ptr(dloss), _ptr(ws), bwd_bytes,
                                                _ptr(dx) if want_dx else 0, _ptr(dw) if want_dw else 0, _stream()), "nsa_loss_bwd")
     return dx, dw
 
@@ -2719,22 +2736,15 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, ignore_index
     """F.cross_entropy(F.linear(x, weight).float(), labels) over the last axis of x '... d' (the loss of transformer.py:326-330), without the
     logits in memory: weight 'v d', labels '...' int64 or int32, x and weight both bf16, fp16 or fp32 on one device.  fp32, one value or
     (reduction "none") one per row; rows labelled `ignore_index` count nothing and are not read.  Logits and sums are fp32 (F.linear would
-    round them to x's type first); gradients have x's and weight's type and are off by little more than its rounding (bf16 up to 1.05 times, fp16 1.1).  A label that is neither `ignore_index` nor in the vocabulary
-    makes its loss and the gradients NaN: it is known to the device only.  Weights are finite.  The gradients cannot be differentiated again."""
+    round them to x's type first); gradients have x's and weight's type and are off by little more than its rounding (bf16 up to 1.05 times,
+    fp16 1.1).  A label that is neither `ignore_index` nor in the vocabulary makes its loss and the gradients NaN: it is known to the device only.
+    A loss below 2^-53 is zero, as a softmax of 64 bits has it.  Weights are finite.  The gradients cannot be differentiated again."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction {reduction!r}, expected one of {sorted(_REDUCTIONS)}")
     if x.is_cuda and torch.is_autocast_enabled():
         dtype = torch.get_autocast_dtype("cuda")
         x, weight = x.to(dtype), weight.to(dtype)
-    if not x.is_cuda or weight.device != x.device or labels.device != x.device:
-        raise RuntimeError("linear_cross_entropy: needs tensors on one GPU (HIP kernels, no CPU fallback)")
-    if x.dtype not in _LOSS_TYPES or weight.dtype != x.dtype:
-        raise RuntimeError(f"linear_cross_entropy: x {x.dtype}, weight {weight.dtype}: expected both bf16, both fp16 or both fp32")
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or labels.shape != x.shape[:-1] or 0 in weight.shape:
-        raise RuntimeError(f"linear_cross_entropy: x {tuple(x.shape)}, weight {tuple(weight.shape)}, labels {tuple(labels.shape)}: expected '... d', "
-                           "'v d' and '...'")
-    if labels.dtype not in (torch.int64, torch.int32):
-        raise RuntimeError(f"linear_cross_entropy: labels {labels.dtype}: expected int64 or int32")
+    _check_loss(x, weight, labels, x.shape[:-1])
     flat = x.dim() == 2
     loss, _ = _linear_cross_entropy(x if flat else x.reshape(-1, x.shape[-1]), weight, labels if flat else labels.reshape(-1), int(ignore_index),
                                     _REDUCTIONS[reduction])
@@ -2771,6 +2781,10 @@ def _newton_schulz(matrices, steps: int, a: float, b: float, c: float, eps: floa
 
 @torch.library.custom_op("nsa_amd::newton_schulz", mutates_args=())
 def newton_schulz_op(matrices: list[Tensor], steps: int, a: float, b: float, c: float, eps: float) -> list[Tensor]:
+    # (a traced graph calls this with what it is run on)
+    if not matrices or any(not t.is_cuda or t.device != matrices[0].device or t.dtype != matrices[0].dtype or t.dtype not in _LOSS_TYPES
+                           or t.dim() not in (2, 3) or not t.numel() for t in matrices):
+        raise RuntimeError("newton_schulz: expected matrices 'm n' or 'b m n' of one type, bf16, fp16 or fp32, on one GPU, none of them empty")
     return _newton_schulz(matrices, steps, a, b, c, eps)
 
 
