@@ -81,10 +81,14 @@ static int loss_plan(const nsa_loss_desc* d, const void* weight, LossPlan& p) {
   p.grad_P = d->dtype == 2 ? 2 : d->dtype == 1 ? ONE_BY_TWO : 1;
   // The tiles whose rounds end first: time of a round on all places, in us for each feature and beside that (products measured from 512 to 4096
   // features, the maxima and sums of a tile beside them).  256 x 256 tiles have no registers for sums in pieces (TileProduct::PIECES), so long
-  // fp32 rows do without them: at 2066 features the gradients were 2.8e-6 off, 7 times as much as fp32 products by the library.
+  // fp32 rows do without them: at 2066 features the gradients were 2.8e-6 off, 7 times as much as fp32 products by the library.  (4095 rows, 32000
+  // entries: at 1088 features 4425 us and dx 2.0e-7 off, with 256 x 256 tiles 4002 us and 6.3e-7; at 2048 7073 and 2.0e-7, 5946 and 7.7e-7.  1021 rows of
+  // 1024 features, forward: 265 us as 256 x 256 tiles, dx 4.1e-7 off; rows of 1088: 348 us without them, 304 with.)
   struct Cost { LossSize size; int tile, places; double each, beside; };
   static constexpr Cost one[3] = {{WIDE, 256, 256, 0.0272, 13.0}, {MIDDLE, 128, 256, 0.0085, 5.0}, {TINY, 64, 512, 0.0060, 3.5}};
   static constexpr Cost two[3] = {{WIDE, 256, 256, 0.0785, 13.0}, {MIDDLE, 128, 256, 0.0238, 5.0}, {TINY, 64, 512, 0.0210, 3.5}};
+  // Up to 32 rows: loss_few_kernel (32 rows, 1024 features, 32000 entries: 20 us in bf16 and 35 in fp32, as tiles of 64 rows 30 and 105; 4096 features,
+  // 131072 entries: 191 and 412 us, 196 and 1830).
   double least = 0.;
   p.size = FEW;
   for (const Cost& c : p.P == 2 ? two : one) {
