@@ -58,8 +58,8 @@ struct LossPlan {
   int w_splits, last_splits;              // slices of the rows that dw of a piece, of the last one, is summed from
   size_t state, fwd, bwd;                 // bytes
   size_t s_map, s_place, s_label, s_norm, s_own;                            // offsets in the state
-  size_t f_part, f_target, f_loss, f_x, f_w, f_most, f_count;                        // in the forward's workspace
-  size_t b_cells, b_most, b_g, b_shift, b_x, b_xg, b_w, b_grad, b_dx, b_dw;    // in the backward's
+  size_t f_part, f_target, f_loss, f_x, f_w, f_most, f_count;               // in the forward's workspace
+  size_t b_cells, b_most, b_g, b_shift, b_x, b_xg, b_w, b_grad, b_dx, b_dw;  // in the backward's
 };
 
 static size_t up(size_t v, size_t to) { return (v + to - 1) / to * to; }
@@ -341,7 +341,8 @@ __global__ __launch_bounds__(256) void loss_begin_kernel(const LossBegin G) {
 
 // Rows (named by map, or all) as planes of kp columns, those past `cols` zero; rows past the last one up to a multiple of 64 zero too.
 // found: the values are scaled below 2^15 by the power of two that suits the largest (none, or as_is: they are not).  most: their own largest
-// goes there.  weighted: a second copy, scaled, of rows times what they weigh in dw (weight_shift).  back: the last 64 columns end with the row's last value, `back` zeros before what is left (TileProduct::run).
+// goes there.  weighted: a second copy, scaled, of rows times what they weigh in dw (weight_shift).  back: the last 64 columns end with the row's
+// last value, `back` zeros before what is left (TileProduct::run).
 struct LossRows {
   const void* src;
   long ld;

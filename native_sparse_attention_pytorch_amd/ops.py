@@ -113,11 +113,10 @@ def _recorded() -> bool:
     return bool(_is_compiling() or _transforms() is not None or _dispatch_modes() > 0 or _dispatch_key(_PRE_DISPATCH) or _tracing_state() is not None)
 
 
-def _refuse_tangents(name: str, *args) -> None:
-    """None of the operators has a rule for forward mode; a result without a tangent would say that it is constant."""
-    if not _is_compiling() and _forward_ad._current_level >= 0:
-        if any(isinstance(a, Tensor) and _forward_ad.unpack_dual(a).tangent is not None for a in args):
-            raise NotImplementedError(f"{name}: forward mode is not supported, an argument has a tangent")
+def _refuse_tangents(name: str, args) -> None:
+    """In a forward-mode level: none of the operators has a rule for it, and a result without a tangent would say that it is constant."""
+    if any(isinstance(a, Tensor) and _forward_ad.unpack_dual(a).tangent is not None for a in args):
+        raise NotImplementedError(f"{name}: forward mode is not supported, an argument has a tangent")
 
 
 def _direct(op):
@@ -154,8 +153,9 @@ def _direct_bwd(op):
     return op if _recorded() else _once(op._init_fn)
 
 
-def _eager_function(op, setup, backward):
-    raw = op._init_fn
+def _eager_function(op, setup, backward, raw=None):
+    """`raw`: the body without checks of what its caller has checked."""
+    raw = raw or op._init_fn
 
     class Fn(torch.autograd.Function):
         @staticmethod
@@ -172,9 +172,12 @@ def _eager_function(op, setup, backward):
     Fn.__name__ = Fn.__qualname__ = "Eager_" + name
 
     def call(*args):
-        _refuse_tangents(name, *args)
         if _recorded():
+            if not _is_compiling() and _forward_ad._current_level >= 0:
+                _refuse_tangents(name, args)
             return op(*args)
+        if _forward_ad._current_level >= 0:
+            _refuse_tangents(name, args)
         if not torch.is_grad_enabled() or not any(isinstance(a, Tensor) and a.requires_grad for a in args):
             return raw(*args)
         return Fn.apply(*args)
@@ -2657,12 +2660,12 @@ def _check_loss(x: Tensor, weight: Tensor, labels: Tensor, rows) -> None:
                            "'v d' and '...'")
 
 
-@torch.library.custom_op("nsa_amd::linear_cross_entropy_fwd", mutates_args=())
-def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_index: int, reduction: int) -> tuple[Tensor, Tensor]:
-    """(loss, what the gradients need): x 'n d', weight 'v d', labels 'n'; reduction 0 none, 1 mean, 2 sum."""
-    _check_loss(x, weight, labels, x.shape[:-1])      # (a traced graph calls this with what it is run on)
-    if x.dim() != 2 or labels.dtype not in (torch.int64, torch.int32):
-        raise RuntimeError(f"linear_cross_entropy: x {tuple(x.shape)}, labels {labels.dtype}: expected 'n d' and int64 or int32")
+def _check_labels(labels: Tensor) -> None:
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError(f"linear_cross_entropy: labels {labels.dtype}: expected int64 or int32")
+
+
+def _loss_fwd(x, weight, labels, ignore_index, reduction):
     n = x.shape[0]
     with _on(x.device):
         x, weight, labels = _unit_rows(x), _unit_rows(weight), labels.contiguous()
@@ -2674,6 +2677,17 @@ def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_i
             _lib.check(_lib.lib().nsa_loss_fwd(d, _ptr(x), _ptr(weight), _ptr(labels), _ptr(state), state_bytes, _ptr(ws), fwd_bytes, _ptr(loss),
                                                _stream()), "nsa_loss_fwd")
     return loss, state
+
+
+@torch.library.custom_op("nsa_amd::linear_cross_entropy_fwd", mutates_args=())
+def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, labels: Tensor, ignore_index: int, reduction: int) -> tuple[Tensor, Tensor]:
+    """(loss, what the gradients need): x 'n d', weight 'v d', labels 'n'; reduction 0 none, 1 mean, 2 sum."""
+    # (a traced graph calls this with what it is run on)
+    _check_loss(x, weight, labels, x.shape[:-1])
+    _check_labels(labels)
+    if x.dim() != 2:
+        raise RuntimeError(f"linear_cross_entropy: x {tuple(x.shape)}: expected 'n d'")
+    return _loss_fwd(x, weight, labels, ignore_index, reduction)
 
 
 @linear_cross_entropy_fwd.register_fake
@@ -2729,7 +2743,7 @@ def _loss_backward(ctx, dloss, _):
 
 
 linear_cross_entropy_fwd.register_autograd(_loss_backward, setup_context=_loss_setup)
-_linear_cross_entropy = _eager_function(linear_cross_entropy_fwd, _loss_setup, _loss_backward)
+_linear_cross_entropy = _eager_function(linear_cross_entropy_fwd, _loss_setup, _loss_backward, _loss_fwd)
 
 
 def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, ignore_index: int = -100, reduction: str = "mean") -> Tensor:
@@ -2738,13 +2752,15 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, ignore_index
     (reduction "none") one per row; rows labelled `ignore_index` count nothing and are not read.  Logits and sums are fp32 (F.linear would
     round them to x's type first); gradients have x's and weight's type and are off by little more than its rounding (bf16 up to 1.05 times,
     fp16 1.1).  A label that is neither `ignore_index` nor in the vocabulary makes its loss and the gradients NaN: it is known to the device only.
-    A loss below 2^-53 is zero, as a softmax of 64 bits has it.  Weights are finite.  The gradients cannot be differentiated again."""
+    A loss below 2^-53 is zero, as a softmax of 64 bits has it.  fp32 x and weight are read to 22 bits, and to 2^-40 of their largest value.  Weights
+    are finite.  The gradients cannot be differentiated again."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction {reduction!r}, expected one of {sorted(_REDUCTIONS)}")
     if x.is_cuda and torch.is_autocast_enabled():
         dtype = torch.get_autocast_dtype("cuda")
         x, weight = x.to(dtype), weight.to(dtype)
     _check_loss(x, weight, labels, x.shape[:-1])
+    _check_labels(labels)
     flat = x.dim() == 2
     loss, _ = _linear_cross_entropy(x if flat else x.reshape(-1, x.shape[-1]), weight, labels if flat else labels.reshape(-1), int(ignore_index),
                                     _REDUCTIONS[reduction])
@@ -2816,9 +2832,10 @@ def newton_schulz(updates, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315
     coefficients = tuple(float(v) for v in coefficients)
     if len(coefficients) != 3 or not 1 <= int(steps) <= 100 or not eps >= 0:
         raise ValueError(f"newton_schulz: steps {steps}, coefficients {coefficients}, eps {eps}: expected 1 to 100 steps, three coefficients, eps >= 0")
-    _refuse_tangents("newton_schulz", *given)
     if not torch.compiler.is_compiling():      # (compiled calls: the entry checks them)
         _newton_coefficients(coefficients, int(steps))
+        if _forward_ad._current_level >= 0:
+            _refuse_tangents("newton_schulz", given)
     for t in given:
         if not t.is_cuda or t.device != given[0].device:
             raise RuntimeError("newton_schulz: needs tensors on one GPU (HIP kernels, no CPU fallback)")
