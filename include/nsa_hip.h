@@ -557,6 +557,64 @@ int nsa_newton_workspace_bytes(int32_t many, const int32_t* rows, const int32_t*
 int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_t* cols, const void* const* in, const int64_t* in_stride, void* const* out,
                       int32_t dtype, int32_t steps, float a, float b, float c, float eps, void* ws, size_t ws_bytes, void* stream);
 
+/* A key / value cache in 8 bits (no counterpart in the reference, whose caches are plain tensors: NSA.py:384-393).
+ *   keys, values: e4m3 codes [batch, kv_heads, capacity, dim_head] (finite ones up to 448, 0x7f and 0xff NaN), rows contiguous; the code c of a row stands
+ *   for c times its scale, fp32 powers of two, one for each `block` rows of a kv head: key_scales, value_scales [batch, kv_heads, capacity / block],
+ *   contiguous along the blocks.  Strides in elements: kv_stride {batch, head, row} for both of keys and values (multiples of 16), scale_stride
+ *   {batch, head} for both scales.  keys, values: 16-byte aligned.  dim_head 64 or 128, block 16, 32, 64 or 128, capacity a multiple of it below 2^31.
+ *   Sequence b holds len(b) = lengths[b * length_stride] + length rows where lengths (device int32) is not NULL, else `length`; clamped to [0, capacity].
+ *
+ * nsa_cache8_append: rows of k and v [batch, kv_heads, rows, dim_head] of `dtype` (strides {batch, head, row}, rows 16-byte aligned), the first
+ * counts[b] of them (NULL: all), become rows len(b) .. of sequence b, the ones past the capacity excepted.  A block's scale is the smallest power of two, 2^-110 at
+ * least and 2^119 at most, that takes its largest finite value to 448 or less; a block that holds rows already keeps its scale or gets a larger one, in
+ * whose units those rows are rounded again.  Values are rounded to nearest, halves to even; infinities become NaN.  All other rows stay as they are.
+ *
+ * nsa_cache8_attend: the one query of each sequence, q [batch, kv_heads * group, dim_head] of `dtype` (strides {batch, head}), attends the newest
+ * `window` of its keys (0: all), or with sel_block > 0 the blocks idx of sel_block keys (of each kv head, or of each head where per_head_sel:
+ * [batch, kv_heads or heads, num_sel] contiguous, int32 or int64) whose fmask byte is not 0, as far as the sequence has them, and the keys of the block
+ * that its newest key is in.  A block named twice counts twice.  No key: zeros.  out: [batch, heads, dim_head] contiguous, of `dtype`.  group <= 32;
+ * num_sel <= 2^20, and (num_sel + 1) * sel_block below 2^30.
+ * Sums in fp32, q and the probabilities as sums of bf16 parts (q exactly; probabilities to 16 bits, of fp32 queries to 24), results rounded once.
+ * Only rows that are attended are read, in tiles of 16 that may begin before the first and end behind the last of them, in the cache. */
+typedef struct nsa_cache8_desc {
+  int32_t batch, kv_heads, group, dim_head;
+  int32_t block, capacity;
+  int32_t dtype;                              /* 0 bf16, 1 fp16, 2 fp32 */
+  int32_t length, length_stride;
+  int32_t window;
+  int32_t sel_block, num_sel, per_head_sel, idx_is_int64;
+  float scale;
+  int32_t reserved;                           /* 0 */
+  int64_t kv_stride[3], scale_stride[2], q_stride[2];
+} nsa_cache8_desc;
+int nsa_cache8_append(const nsa_cache8_desc* d, int32_t rows, const void* k, const int64_t* k_stride, const void* v, const int64_t* v_stride,
+                      const int32_t* lengths, const int32_t* counts, void* keys, void* values, float* key_scales, float* value_scales, void* stream);
+int nsa_cache8_workspace_bytes(const nsa_cache8_desc* d, size_t* bytes);
+int nsa_cache8_attend(const nsa_cache8_desc* d, const void* q, const void* keys, const void* values, const float* key_scales,
+                      const float* value_scales, const int32_t* lengths, const void* idx, const uint8_t* fmask, void* ws, size_t ws_bytes, void* out,
+                      void* stream);
+
+/* What is done to the logits x [rows, vocab] of `dtype` (rows row_stride elements apart) before a token is drawn (transformer.py:240-247 draws from plain
+ * ones); out: fp32 [rows, vocab] contiguous.  With c = how often entry i is among the first history_lengths[r] (NULL: all) of the
+ * `history` tokens of row r ([rows, history] contiguous, int32 or int64, those outside [0, vocab) are passed over):
+ *   c > 0: x <- (x > 0 ? x / repetition[r] : x * repetition[r]) - frequency[r] c - presence[r]
+ *   x <- (x + bias[i]) / temperature[r];  entries that are not allowed: -inf.
+ * repetition, frequency, presence, temperature: fp32 values of the rows at stride 0 or 1, NULL: the descriptor's for all rows.  bias: fp32, rows bias_stride apart (0: one for all).  allowed: bytes
+ * [.., vocab] (allowed_kind 1) or int32 words of 32 entries each, lowest bit first (allowed_kind 2), rows allowed_stride elements apart (0: one
+ * for all); kind 0: none.  Every step is rounded to fp32 by itself.  rows and vocab up to 2^30, 4 rows vocab / 1024 below 2^31. */
+typedef struct nsa_logits_desc {
+  int64_t rows, row_stride;
+  int32_t vocab, dtype;
+  int64_t history;
+  int32_t history_int64, allowed_kind;
+  int64_t bias_stride, allowed_stride;
+  int32_t repetition_stride, frequency_stride, presence_stride, temperature_stride;
+  float repetition, frequency, presence, temperature;
+} nsa_logits_desc;
+int nsa_adjust_logits(const nsa_logits_desc* d, const void* x, const void* history, const int32_t* history_lengths, const float* repetition,
+                      const float* frequency, const float* presence, const float* bias, const void* allowed, const float* temperature, float* out,
+                      void* stream);
+
 /* Same as nsa_select_fwd / nsa_select_bwd, additionally recording the caller's hipEvent_t
  * handles (created with timing enabled) between the kernels of the call, so that a benchmark
  * can time each kernel on the launch stream.  Events: fwd {start, after block walk, after

@@ -189,6 +189,13 @@ def lib():
         ints, ptrs = C.POINTER(i32), C.POINTER(vp)
         L.nsa_newton_workspace_bytes.argtypes = [i32, ints, ints, C.POINTER(sz)]
         L.nsa_newton_schulz.argtypes = [i32, ints, ints, ptrs, s3, ptrs, i32, i32, f32, f32, f32, f32, vp, sz, vp]
+        # (descriptors packed by the caller)
+        L.nsa_cache8_append.argtypes = [vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+        L.nsa_cache8_workspace_bytes.argtypes = [vp, C.POINTER(sz)]
+        L.nsa_cache8_attend.argtypes = [vp] * 9 + [vp, sz, vp, vp]
+        L.nsa_adjust_logits.argtypes = [vp] * 12
+        for name in ("nsa_cache8_append", "nsa_cache8_workspace_bytes", "nsa_cache8_attend", "nsa_adjust_logits"):
+            getattr(L, name).restype = C.c_int
         for name in ("nsa_loss_workspace_bytes", "nsa_loss_fwd", "nsa_loss_bwd", "nsa_newton_workspace_bytes", "nsa_newton_schulz"):
             getattr(L, name).restype = C.c_int
         _lib = L

@@ -1,0 +1,196 @@
+// Rows that go into the 8-bit key / value cache.  The values of a block of tokens and a kv head are code x scale with e4m3 codes and a scale that is a
+// power of two: e4m3 is a floating type, so a finer scale would only move where its smallest values end, and with powers of two neither the
+// division by the scale nor a later change of it rounds anything that the codes' own rounding does not.
+//
+// HBM-bound: a row is read once (16 bits or 32 a value) and written once (8).  A block's largest value has to be known before any of its codes: the
+// block's new rows are held in registers in between, 32 values a lane, by one wave up to 2048 values and by up to eight for 128 rows of 128.  A
+// block that holds rows already is read too, and its rows are written again only where the scale grows.
+#include "nsa_cache8.hpp"
+
+namespace nsa {
+
+struct AppendArgs {
+  Cache8Args c;
+  const void *k, *v;
+  long k0, k1, k2, v0, v1, v2;
+  const int* counts;
+  int rows, touched;                   // rows handed in for each sequence, blocks that they may touch
+  long total;                          // (sequence, kv head, keys or values, block)
+};
+
+template <class T>
+__device__ __forceinline__ floatx8 load_values(const T* p) {
+  typedef __attribute__((__vector_size__(8 * sizeof(T)))) T vec;
+  return __builtin_convertvector(*reinterpret_cast<const vec*>(p), floatx8);
+}
+
+// (a bit cast of a vector's element itself takes the vector's first)
+__device__ __forceinline__ uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
+
+// Eight values times `inv`, which is a power of two, as e4m3 codes: nearest, halves to even, beyond 448 to 448, what is no finite number as NaN.
+__device__ __forceinline__ uintx2 codes_of(const floatx8& x, float inv) {
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = x[e];
+    const bool finite = (bits_of(v) & 0x7f800000u) != 0x7f800000u;
+    y[e] = finite ? fminf(fmaxf(v * inv, -448.f), 448.f) : __builtin_nanf("");
+  }
+  uintx2 r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], w, true);
+    r[h] = (uint32_t)w;
+  }
+  return r;
+}
+
+__device__ __forceinline__ floatx8 values_of(const uintx2& c) {
+  floatx8 x;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int w = (int)c[h];
+    x[4 * h] = __builtin_amdgcn_cvt_f32_fp8(w, 0);
+    x[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(w, 1);
+    x[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(w, 2);
+    x[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(w, 3);
+  }
+  return x;
+}
+
+// the exponent of the smallest power of two that takes a finite value of these bits to 448 = 1.75 x 2^8 or less
+__device__ __forceinline__ int scale_exponent(uint32_t bits) {
+  const int e = (int)(bits >> 23) - 127, k = e - 8 + ((bits & 0x7fffffu) > 0x600000u);
+  return min(max(k, -110), 119);
+}
+__device__ __forceinline__ float power_of_two(int k) { return __builtin_bit_cast(float, (uint32_t)(k + 127) << 23); }
+
+template <int D, int B>
+struct AppendShape {
+  static constexpr int CHUNKS = D * B / 8;                            // of eight values
+  static constexpr int PER = CHUNKS / 64 < 4 ? CHUNKS / 64 : 4;       // a lane
+  static constexpr int WAVES = CHUNKS / 64 / PER;                     // a block
+  static constexpr int BLOCKS = WAVES < 4 ? 4 / WAVES : 1, THREADS = 64 * WAVES * BLOCKS;
+};
+
+template <class T, int D, int B>
+__global__ __launch_bounds__((AppendShape<D, B>::THREADS)) void cache8_append_kernel(const AppendArgs A) {
+  using S = AppendShape<D, B>;
+  constexpr int LPR = D / 8;
+  __shared__ uint32_t top_s[S::BLOCKS * S::WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long id = (long)blockIdx.x * S::BLOCKS + wave / S::WAVES;
+  const bool here = id < A.total;
+  const long rest = here ? id / A.touched : 0;
+  const int t = here ? (int)(id - rest * A.touched) : 0;
+  const bool is_v = rest & 1;
+  const int unit = (int)(rest >> 1), b = unit / A.c.hk, h = unit % A.c.hk;
+  const int start = cache8_length(A.c, b);
+  const int n = A.counts != nullptr ? min(max(A.counts[b], 0), A.rows) : A.rows;
+  const long end = min((long)start + n, (long)A.c.cap), row0 = (long)(start / B + t) * B;
+  const bool any = here && row0 < end && n > 0;
+
+  const T* src = is_v ? reinterpret_cast<const T*>(A.v) + b * A.v0 + h * A.v1 : reinterpret_cast<const T*>(A.k) + b * A.k0 + h * A.k1;
+  const long s_row = is_v ? A.v2 : A.k2;
+  uint8_t* dst = (is_v ? A.c.values : A.c.keys) + b * A.c.s0 + h * A.c.s1;
+  float* scale = (is_v ? A.c.value_scales : A.c.key_scales) + b * A.c.z0 + h * A.c.z1 + row0 / B;
+
+  floatx8 x[S::PER];
+  uintx2 old[S::PER];
+  uint32_t top = 0;
+  float s_old = 0.f;
+  const bool held = row0 < start;
+  if (any) {
+    if (held) s_old = *scale;
+#pragma unroll
+    for (int c = 0; c < S::PER; ++c) {
+      const int at = (c * S::WAVES + wave % S::WAVES) * 64 + lane;
+      const long row = row0 + at / LPR;
+      const int f = at % LPR * 8;
+      if (row >= start && row < end) x[c] = load_values(src + (row - start) * s_row + f);
+      else if (row < start) old[c] = *reinterpret_cast<const uintx2*>(dst + row * A.c.s2 + f);
+    }
+#pragma unroll
+    for (int c = 0; c < S::PER; ++c) {
+      const long row = row0 + ((c * S::WAVES + wave % S::WAVES) * 64 + lane) / LPR;
+      if (row >= start && row < end)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t m = bits_of(x[c][e]) & 0x7fffffffu;
+          top = max(top, m < 0x7f800000u ? m : 0u);
+        }
+    }
+#pragma unroll
+    for (int o = 1; o <= 32; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+  }
+  if constexpr (S::WAVES > 1) {
+    if (lane == 0) top_s[wave] = top;
+    __syncthreads();
+    const int w0 = wave / S::WAVES * S::WAVES;
+#pragma unroll
+    for (int w = 0; w < S::WAVES; ++w) top = max(top, top_s[w0 + w]);
+  }
+  if (!any) return;
+  float s_new = power_of_two(scale_exponent(top));
+  if (held) s_new = fmaxf(s_new, s_old);
+  const float inv = 1.0f / s_new;      // (of a power of two: exact)
+  if (lane == 0 && wave % S::WAVES == 0) *scale = s_new;
+#pragma unroll
+  for (int c = 0; c < S::PER; ++c) {
+    const int at = (c * S::WAVES + wave % S::WAVES) * 64 + lane;
+    const long row = row0 + at / LPR;
+    uintx2* to = reinterpret_cast<uintx2*>(dst + row * A.c.s2 + at % LPR * 8);
+    if (row >= start && row < end) *to = codes_of(x[c], inv);
+    else if (row < start && s_new != s_old) *to = codes_of(values_of(old[c]), s_old * inv);
+  }
+}
+
+template <class T, int D, int B>
+static int append_launch(const AppendArgs& A, hipStream_t st) {
+  using S = AppendShape<D, B>;
+  const long groups = (A.total + S::BLOCKS - 1) / S::BLOCKS;
+  if (groups * S::THREADS > 0xffffffffL) return NSA_E_UNSUPPORTED;
+  hipLaunchKernelGGL((cache8_append_kernel<T, D, B>), dim3((unsigned)groups), dim3(S::THREADS), 0, st, A);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : (int)e;
+}
+template <class T, int D>
+static int append_block(const AppendArgs& A, hipStream_t st) {
+  switch (A.c.block) {
+    case 16: return append_launch<T, D, 16>(A, st);
+    case 32: return append_launch<T, D, 32>(A, st);
+    case 64: return append_launch<T, D, 64>(A, st);
+    default: return append_launch<T, D, 128>(A, st);
+  }
+}
+template <class T>
+static int append_dim(const AppendArgs& A, int d, hipStream_t st) { return d == 64 ? append_block<T, 64>(A, st) : append_block<T, 128>(A, st); }
+
+}  // namespace nsa
+
+extern "C" int nsa_cache8_append(const nsa_cache8_desc* d, int32_t rows, const void* k, const int64_t* k_stride, const void* v, const int64_t* v_stride,
+                                 const int32_t* lengths, const int32_t* counts, void* keys, void* values, float* key_scales, float* value_scales,
+                                 void* stream) {
+  using namespace nsa;
+  if (!cache8_check(d) || rows < 0 || !keys || !values || !key_scales || !value_scales || ((uintptr_t)keys | (uintptr_t)values) % 16) return NSA_E_ARG;
+  if (!cache8_supported(d)) return NSA_E_UNSUPPORTED;
+  if (rows == 0) return 0;
+  if (!k || !v || !k_stride || !v_stride || ((uintptr_t)k | (uintptr_t)v) % 16) return NSA_E_ARG;
+  const int per16 = d->dtype == 2 ? 4 : 8;
+  for (int i = 0; i < 3; ++i)
+    if (k_stride[i] % per16 || v_stride[i] % per16) return NSA_E_ARG;
+  AppendArgs A{};
+  A.c = cache8_args(d, keys, values, key_scales, value_scales, lengths);
+  A.k = k; A.v = v;
+  A.k0 = k_stride[0]; A.k1 = k_stride[1]; A.k2 = k_stride[2];
+  A.v0 = v_stride[0]; A.v1 = v_stride[1]; A.v2 = v_stride[2];
+  A.counts = counts; A.rows = rows;
+  // (rows that begin anywhere in a block)
+  A.touched = (int)(((long)rows + d->block - 2) / d->block + 1);
+  A.touched = A.touched < d->capacity / d->block ? A.touched : d->capacity / d->block;
+  A.total = (long)d->batch * d->kv_heads * 2 * A.touched;
+  if ((long)d->batch * d->kv_heads > 1L << 30) return NSA_E_UNSUPPORTED;
+  hipStream_t st = (hipStream_t)stream;
+  return d->dtype == 0 ? append_dim<__bf16>(A, d->dim_head, st) : d->dtype == 1 ? append_dim<_Float16>(A, d->dim_head, st) : append_dim<float>(A, d->dim_head, st);
+}

@@ -2852,3 +2852,341 @@ def newton_schulz(updates, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315
             for i, m in zip(at, made):
                 out[i] = m if given[i].dim() <= 3 else m.view(given[i].shape)
     return out[0] if alone else type(updates)(out) if type(updates) in (list, tuple) else out
+
+
+# ------------------------------------------------------------------ a serving step: the 8-bit cache and the logits
+
+_FP8 = torch.float8_e4m3fn
+_CACHE8_DESC, _LOGITS_DESC = struct.Struct("@14ifi7q"), struct.Struct("@2q2iq2i2q4i4f")      # nsa_cache8_desc, nsa_logits_desc
+
+
+class Cache8(NamedTuple):
+    """Keys and values in 8 bits: e4m3 codes 'b hk n d' (d 64 or 128) and fp32 scales 'b hk n/block', a power of two for each `block` tokens of a kv head
+    (16, 32, 64 or 128); a row stands for its codes times its block's scale.  Made by `make_cache8`, filled by `cache8_append`."""
+    keys: Tensor
+    values: Tensor
+    key_scales: Tensor
+    value_scales: Tensor
+
+    @property
+    def block(self) -> int:
+        return self.keys.shape[2] // max(self.key_scales.shape[2], 1)
+
+    def rows(self, start: int, count: int, dtype: torch.dtype = _BF16) -> tuple[Tensor, Tensor]:
+        """What rows start .. start + count - 1 stand for, (keys, values) 'b hk count d' of `dtype`."""
+        at = torch.arange(start, start + count, device=self.keys.device) // self.block
+        return tuple((codes[:, :, start:start + count].float() * scales[:, :, at, None]).to(dtype)
+                     for codes, scales in ((self.keys, self.key_scales), (self.values, self.value_scales)))
+
+
+def make_cache8(batch: int, kv_heads: int, rows: int, dim_head: int, block: int = 32, device="cuda") -> Cache8:
+    """An empty cache for at least `rows` tokens a sequence; heads of other than 64 or 128 features are kept padded to the next of the two."""
+    if block not in (16, 32, 64, 128) or min(batch, kv_heads, rows, dim_head) < 1:
+        raise ValueError(f"make_cache8: {batch} x {kv_heads} x {rows} x {dim_head}, block {block}: expected sizes of 1 or more and a block of 16, 32, 64 or 128")
+    blocks = -(-rows // block)
+    codes = lambda: torch.zeros((batch, kv_heads, blocks * block, _kernel_dim(dim_head)), dtype=torch.uint8, device=device).view(_FP8)
+    # (the least of all scales: rows of zeros hold back no scale of rows that come into their block)
+    scales = lambda: torch.full((batch, kv_heads, blocks), 2. ** -110, dtype=torch.float32, device=device)
+    return Cache8(codes(), codes(), scales(), scales())
+
+
+def _check_cache8(name: str, keys: Tensor, values: Tensor, key_scales: Tensor, value_scales: Tensor) -> int:
+    """Rows of a scale, of a cache that the kernels can be given: they read and write by address."""
+    if not keys.is_cuda or any(t.device != keys.device for t in (values, key_scales, value_scales)):
+        raise RuntimeError(f"{name}: needs a cache on one GPU (HIP kernels, no CPU fallback)")
+    if keys.dtype != _FP8 or values.dtype != _FP8 or key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32:
+        raise RuntimeError(f"{name}: cache of {keys.dtype}, {values.dtype}, {key_scales.dtype}, {value_scales.dtype}: expected float8_e4m3fn codes and fp32 scales")
+    shape, scales, stride = keys.shape, key_scales.shape, keys.stride()
+    if len(shape) != 4 or values.shape != shape or len(scales) != 3 or value_scales.shape != scales or scales[:2] != shape[:2] or 0 in shape or 0 in scales:
+        raise RuntimeError(f"{name}: cache of keys {tuple(shape)}, values {tuple(values.shape)}, scales {tuple(scales)} and {tuple(value_scales.shape)}: "
+                           "expected 'b hk n d' twice and 'b hk n/block' twice")
+    block = shape[2] // scales[2]
+    if shape[3] not in (64, 128) or block not in (16, 32, 64, 128) or shape[2] != block * scales[2]:
+        raise RuntimeError(f"{name}: cache of {shape[2]} rows of {shape[3]} features, {scales[2]} scales: expected 64 or 128 features and 16, 32, 64 or 128 rows a scale")
+    if (values.stride() != stride or value_scales.stride() != key_scales.stride() or stride[3] != 1 or stride[2] < shape[3] or (stride[0] | stride[1] | stride[2]) % 16
+            or key_scales.stride(2) != 1 or keys.data_ptr() % 16 or values.data_ptr() % 16):
+        raise RuntimeError(f"{name}: cache strides {stride}, {values.stride()}, {key_scales.stride()}, {value_scales.stride()}: keys and values, and both scales, "
+                           "are laid out alike, rows contiguous from 16-byte boundaries on")
+    return block
+
+
+def _lengths(name: str, what: str, value, batch: int, most: int, device: torch.device):
+    """(device int32 tensor or None, stride, number) of a count for all sequences or of one for each."""
+    if not isinstance(value, Tensor):
+        if not 0 <= int(value) <= most:
+            raise RuntimeError(f"{name}: {what} {value}, expected 0 to {most}")
+        return None, 0, int(value)
+    if value.device != device or value.dtype not in (torch.int32, torch.int64) or value.numel() not in (1, batch) or value.dim() > 1:
+        raise RuntimeError(f"{name}: {what} {value.dtype} {tuple(value.shape)} on {value.device}: expected int32 or int64, one or one for each of {batch} sequences, on {device}")
+    if value.dtype == torch.int64:
+        value = value.clamp(0, 2 ** 31 - 1).to(torch.int32)
+    return value, 0 if value.numel() == 1 else value.stride(0), 0
+
+
+def _aligned_rows(t: Tensor) -> Tensor:
+    """Strides and address that 16-byte accesses of rows take (a view where they are already)."""
+    return t if t.stride(-1) == 1 and not any(s % 8 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _cache8_append(keys, values, key_scales, value_scales, k, v, starts, start, counts):
+    batch, hk, rows, _ = k.shape
+    block = keys.shape[2] // key_scales.shape[2]
+    with _on(keys.device):
+        starts, stride, _ = (None, 0, 0) if starts is None else _lengths("cache8_append", "start", starts, batch, 0, keys.device)
+        k, v = _aligned_rows(_pad_dim(k, keys.shape[3])), _aligned_rows(_pad_dim(v, keys.shape[3]))
+        if counts is not None:
+            counts = counts.clamp(0, rows).to(torch.int32).contiguous() if counts.dtype == torch.int64 else counts.contiguous()
+        desc = _CACHE8_DESC.pack(batch, hk, 1, keys.shape[3], block, keys.shape[2], _LOSS_TYPES[k.dtype], start, stride, 0, 0, 0, 0, 0, 0., 0,
+                                 *keys.stride()[:3], *key_scales.stride()[:2], 0, 0)
+        strides = C.c_int64 * 3
+        _lib.check(_lib.lib().nsa_cache8_append(desc, rows, k.data_ptr(), strides(*k.stride()[:3]), v.data_ptr(), strides(*v.stride()[:3]), _ptr(starts),
+                                                _ptr(counts), keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), _stream()),
+                   "nsa_cache8_append")
+
+
+def _check_append(keys, values, key_scales, value_scales, k, v, starts, start, counts):
+    _check_cache8("cache8_append", keys, values, key_scales, value_scales)
+    batch, hk, capacity, d = keys.shape
+    if k.device != keys.device or v.device != keys.device or k.dtype not in _LOSS_TYPES or v.dtype != k.dtype:
+        raise RuntimeError(f"cache8_append: k {k.dtype}, v {v.dtype} on {k.device}, {v.device}: expected both bf16, both fp16 or both fp32, on {keys.device}")
+    if k.dim() != 4 or v.shape != k.shape or k.shape[:2] != (batch, hk) or not 0 < k.shape[3] <= d or _kernel_dim(k.shape[3]) != d:
+        raise RuntimeError(f"cache8_append: k {tuple(k.shape)}, v {tuple(v.shape)}, cache {tuple(keys.shape)}: expected 'b hk rows d' of the cache's sequences and heads")
+    if starts is None:
+        if start < 0 or start + k.shape[2] > capacity:
+            raise RuntimeError(f"cache8_append: rows {start} to {start + k.shape[2] - 1} of a cache for {capacity}")
+    else:
+        _lengths("cache8_append", "start", starts, batch, capacity, keys.device)
+    if counts is not None and (counts.device != keys.device or counts.dtype not in (torch.int32, torch.int64) or counts.shape != (batch,)):
+        raise RuntimeError(f"cache8_append: counts {counts.dtype} {tuple(counts.shape)} on {counts.device}: expected int32 or int64, one for each of {batch} sequences, on {keys.device}")
+
+
+@torch.library.custom_op("nsa_amd::cache8_append", mutates_args=("keys", "values", "key_scales", "value_scales"))
+def cache8_append_op(keys: Tensor, values: Tensor, key_scales: Tensor, value_scales: Tensor, k: Tensor, v: Tensor, starts: Optional[Tensor], start: int,
+                     counts: Optional[Tensor]) -> None:
+    # (a traced graph calls this with what it is run on)
+    _check_append(keys, values, key_scales, value_scales, k, v, starts, start, counts)
+    if k.shape[2]:
+        _cache8_append(keys, values, key_scales, value_scales, k, v, starts, start, counts)
+
+
+@cache8_append_op.register_fake
+def _(keys, values, key_scales, value_scales, k, v, starts, start, counts):
+    return None
+
+
+def _no_gradient(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(isinstance(t, Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+    if not _is_compiling() and _forward_ad._current_level >= 0:
+        _refuse_tangents(name, tensors)
+
+
+def cache8_append(cache: Cache8, k: Tensor, v: Tensor, start=0, counts: Tensor | None = None) -> None:
+    """Rows of k and v 'b hk rows d' (bf16, fp16 or fp32) become rows start .. of each sequence in `cache` (NSA.py:388-393 concatenates them).  `start`: what
+    the sequences hold already, a number for all or an int32 tensor (int64 is converted), one or 'b'; `counts`: how many of the rows each takes, all without
+    it.  Where `start` is a tensor it is known to the device only: rows past the capacity are dropped.  A block's scale is the smallest power of two that
+    takes its largest value to 448; one that grows when rows come into a block that holds some rounds those again, in units of the new.  Infinities
+    become NaN.  Nothing else of the cache is written."""
+    starts, number = (start, 0) if isinstance(start, Tensor) else (None, int(start))
+    _no_gradient("cache8_append", k, v)
+    args = *cache, k, v, starts, number, counts
+    if _recorded():
+        cache8_append_op(*args)
+        return
+    _check_append(*args)
+    if k.shape[2]:
+        _cache8_append(*args)
+
+
+def _cache8_attend(q, keys, values, key_scales, value_scales, lengths, length, window, size, idx, fmask, scale):
+    b, hq, _, d0 = q.shape
+    _, hk, capacity, d = keys.shape
+    with _on(keys.device):
+        lengths, stride, _ = (None, 0, 0) if lengths is None else _lengths("cache8_attend", "lengths", lengths, b, 0, keys.device)
+        if d != d0:
+            q = _pad_dim(q, d)
+        if q.stride(3) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+        chosen = 0
+        if size:
+            idx = idx.contiguous()
+            fmask = (fmask.view(torch.uint8) if fmask.dtype == torch.bool else fmask).contiguous()
+            chosen = idx.shape[3]
+        desc = _CACHE8_DESC.pack(b, hk, hq // hk, d, capacity // key_scales.shape[2], capacity, _LOSS_TYPES[q.dtype], length, stride, window, size, chosen,
+                                 size > 0 and idx.shape[1] != hk, size > 0 and idx.dtype == torch.int64, scale, 0, *keys.stride()[:3], *key_scales.stride()[:2],
+                                 q.stride(0), q.stride(1))
+        L = _lib.lib()
+        nbytes = C.c_size_t()
+        _lib.check(L.nsa_cache8_workspace_bytes(desc, C.byref(nbytes)), "nsa_cache8_workspace_bytes")
+        out = torch.empty((b, hq, 1, d), dtype=q.dtype, device=q.device)
+        ws = torch.empty((nbytes.value,), dtype=torch.uint8, device=q.device) if nbytes.value else None
+        _lib.check(L.nsa_cache8_attend(desc, q.data_ptr(), keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), _ptr(lengths),
+                                       _ptr(idx) if chosen else None, _ptr(fmask) if chosen else None, _ptr(ws), nbytes.value, out.data_ptr(), _stream()),
+                   "nsa_cache8_attend")
+    return out if d == d0 else out[..., :d0]
+
+
+def _check_attend8(q, keys, values, key_scales, value_scales, lengths, length, window, size, idx, fmask, scale):
+    name = "cache8_select_attend" if size else "cache8_attend"
+    _check_cache8(name, keys, values, key_scales, value_scales)
+    b, hk, capacity, d = keys.shape
+    if q.device != keys.device or q.dtype not in _LOSS_TYPES:
+        raise RuntimeError(f"{name}: q {q.dtype} on {q.device}: expected bf16, fp16 or fp32 on {keys.device}")
+    if q.dim() != 4 or q.shape[0] != b or q.shape[2] != 1 or not 0 < q.shape[3] <= d or _kernel_dim(q.shape[3]) != d or q.shape[1] % hk or not 0 < q.shape[1] <= 32 * hk:
+        raise RuntimeError(f"{name}: q {tuple(q.shape)}, cache {tuple(keys.shape)}: expected 'b hq 1 d' with hq up to 32 times the kv heads and a multiple of them")
+    if lengths is None:
+        _lengths(name, "lengths", length, b, capacity, keys.device)
+    else:
+        _lengths(name, "lengths", lengths, b, capacity, keys.device)
+    if window < 0 or size < 0 or (idx is None) != (size == 0) or (fmask is None) != (size == 0):
+        raise RuntimeError(f"{name}: window {window}, block size {size}")
+    if size:
+        if idx.device != keys.device or fmask.device != keys.device or idx.dtype not in (torch.int32, torch.int64) or fmask.dtype not in (torch.bool, torch.uint8):
+            raise RuntimeError(f"{name}: idx {idx.dtype} on {idx.device}, fmask {fmask.dtype} on {fmask.device}: expected int32 or int64, and bool, on {keys.device}")
+        if idx.dim() != 4 or idx.shape[:3] not in ((b, hk, 1), (b, q.shape[1], 1)) or fmask.shape != idx.shape:
+            raise RuntimeError(f"{name}: idx {tuple(idx.shape)}, fmask {tuple(fmask.shape)}: expected 'b hk 1 S' or 'b hq 1 S'")
+
+
+@torch.library.custom_op("nsa_amd::cache8_attend", mutates_args=())
+def cache8_attend_op(q: Tensor, keys: Tensor, values: Tensor, key_scales: Tensor, value_scales: Tensor, lengths: Optional[Tensor], length: int, window: int,
+                     size: int, idx: Optional[Tensor], fmask: Optional[Tensor], scale: float) -> Tensor:
+    _check_attend8(q, keys, values, key_scales, value_scales, lengths, length, window, size, idx, fmask, scale)
+    out = _cache8_attend(q, keys, values, key_scales, value_scales, lengths, length, window, size, idx, fmask, scale)
+    return out.contiguous()
+
+
+@cache8_attend_op.register_fake
+def _(q, keys, values, key_scales, value_scales, lengths, length, window, size, idx, fmask, scale):
+    return q.new_empty(q.shape)
+
+
+def _attend8(q, cache, lengths, window, size, idx, fmask, scale):
+    lengths, length = (lengths, 0) if isinstance(lengths, Tensor) else (None, int(lengths))
+    args = q, *cache, lengths, length, window, size, idx, fmask, float(q.shape[-1] ** -0.5 if scale is None else scale)
+    _no_gradient("cache8_select_attend" if size else "cache8_attend", q)
+    if _recorded():
+        return cache8_attend_op(*args)
+    _check_attend8(*args)
+    return _cache8_attend(*args)
+
+
+def cache8_attend(q: Tensor, cache: Cache8, lengths, window: int | None = None, scale: float | None = None) -> Tensor:
+    """`decode_range_attend` over an 8-bit cache: the newest token's query of each sequence, q 'b hq 1 d' (bf16, fp16 or fp32; hq up to 32 times the kv heads),
+    attends its keys - `lengths` of them, a number for all or an int32 tensor (int64 is converted), one or 'b', clamped to the capacity - or the newest
+    `window`.  Returns 'b hq 1 d' of q's type; zeros where there is no key.  Rows that are not attended may hold anything.  No gradients."""
+    if window is not None and int(window) < 1:
+        raise RuntimeError(f"cache8_attend: window {window}, expected 1 or more")
+    return _attend8(q, cache, lengths, 0 if window is None else int(window), 0, None, None, scale)
+
+
+def cache8_select_attend(q: Tensor, cache: Cache8, lengths, block: int, idx: Tensor, fmask: Tensor, scale: float | None = None) -> Tensor:
+    """`decode_select_attend` over an 8-bit cache (NSA.py:446-515): the newest token's query attends the blocks idx[..., slot] of `block` keys where fmask is
+    true, as far as the sequence has them, and the block that the newest token is in.  idx / fmask: 'b hk 1 S' or, for a selection of each head, 'b hq 1 S';
+    a block named twice counts twice, one that the sequence does not have not at all.  `lengths`, types and result as `cache8_attend`."""
+    if int(block) < 1:
+        raise RuntimeError(f"cache8_select_attend: blocks of {block} keys")
+    return _attend8(q, cache, lengths, 0, int(block), idx, fmask, scale)
+
+
+def _adjust_logits(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values):
+    vocab = logits.shape[-1]
+    rows = logits.numel() // vocab
+    with _on(logits.device):
+        x = logits.reshape(rows, vocab)
+        if x.stride(1) != 1:
+            x = x.contiguous()
+        per_row = lambda t, width: (t, 0) if t.dim() == 1 else (t.reshape(rows, width), None)
+        if history is not None:
+            history = history.reshape(rows, -1).contiguous()
+        if history_lengths is not None:
+            history_lengths = history_lengths.reshape(rows)
+            if history_lengths.dtype == torch.int64:
+                history_lengths = history_lengths.clamp(0, 2 ** 31 - 1).to(torch.int32)
+            history_lengths = history_lengths.contiguous()
+        strides = {}
+        if bias is not None:
+            bias, strides["bias"] = per_row(bias.float(), vocab)
+        kind = 0
+        if allowed is not None:
+            kind = 2 if allowed.dtype == torch.int32 else 1
+            allowed, strides["allowed"] = per_row(allowed, allowed.shape[-1])
+        if bias is not None and bias.stride(-1) != 1:
+            bias = bias.contiguous()
+        if allowed is not None and allowed.stride(-1) != 1:
+            allowed = allowed.contiguous()
+        step = lambda t, name: 0 if t is None or strides[name] == 0 else t.stride(0)
+        tensors = [None if t is None else t.reshape(-1).float().contiguous() for t in (repetition, frequency, presence, temperature)]
+        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+        t = 0 if history is None else history.shape[1]
+        desc = _LOGITS_DESC.pack(rows, x.stride(0), vocab, _LOSS_TYPES[x.dtype], t, history is not None and history.dtype == torch.int64, kind,
+                                 step(bias, "bias"), step(allowed, "allowed"), *(int(p is not None and p.numel() > 1) for p in tensors), *values)
+        _lib.check(_lib.lib().nsa_adjust_logits(desc, x.data_ptr(), _ptr(history) if t else None, _ptr(history_lengths), *map(_ptr, tensors[:3]), _ptr(bias),
+                                                _ptr(allowed), _ptr(tensors[3]), out.data_ptr(), _stream()), "nsa_adjust_logits")
+    return out
+
+
+def _check_adjust(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values):
+    name, device = "adjust_logits", logits.device
+    if not logits.is_cuda or any(t is not None and t.device != device for t in (history, history_lengths, bias, allowed, repetition, frequency, presence, temperature)):
+        raise RuntimeError(f"{name}: needs tensors on one GPU (HIP kernels, no CPU fallback)")
+    if logits.dtype not in _LOSS_TYPES or logits.dim() < 1 or logits.shape[-1] == 0:
+        raise RuntimeError(f"{name}: logits {logits.dtype} {tuple(logits.shape)}: expected bf16, fp16 or fp32 '... v'")
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    rows = lead.numel()
+    whole = torch.int32, torch.int64
+    if history is not None and (history.dtype not in whole or history.dim() < 1 or history.shape[:-1] != lead):
+        raise RuntimeError(f"{name}: history {history.dtype} {tuple(history.shape)}: expected int32 or int64 '... t' for logits {tuple(logits.shape)}")
+    if history_lengths is not None and (history is None or history_lengths.dtype not in whole or history_lengths.shape != lead):
+        raise RuntimeError(f"{name}: history_lengths {history_lengths.dtype} {tuple(history_lengths.shape)}: expected int32 or int64, one for each row of a history")
+    if bias is not None and (not bias.is_floating_point() or bias.shape not in ((vocab,), logits.shape)):
+        raise RuntimeError(f"{name}: bias {bias.dtype} {tuple(bias.shape)}: expected floating 'v' or '... v' for logits {tuple(logits.shape)}")
+    if allowed is not None:
+        width = {torch.bool: vocab, torch.int32: (vocab + 31) // 32}.get(allowed.dtype)
+        if width is None or allowed.shape not in ((width,), (*lead, width)):
+            raise RuntimeError(f"{name}: allowed {allowed.dtype} {tuple(allowed.shape)}: expected bool 'v' or '... v', or int32 words of 32 entries, for logits {tuple(logits.shape)}")
+    for what, t in (("repetition_penalty", repetition), ("frequency_penalty", frequency), ("presence_penalty", presence), ("temperature", temperature)):
+        if t is not None and (not t.is_floating_point() or t.numel() not in (1, rows) or t.dim() > max(len(lead), 1)):
+            raise RuntimeError(f"{name}: {what} {t.dtype} {tuple(t.shape)}: expected a number, or floating, one or one for each of {rows} rows")
+    if not (0 < values[0] < float("inf") and abs(values[1]) < float("inf") and abs(values[2]) < float("inf") and 0 < values[3] < float("inf")):
+        raise ValueError(f"{name}: repetition_penalty {values[0]}, frequency_penalty {values[1]}, presence_penalty {values[2]}, temperature {values[3]}: "
+                         "expected finite numbers, the first and the last above 0")
+
+
+@torch.library.custom_op("nsa_amd::adjust_logits", mutates_args=())
+def adjust_logits_op(logits: Tensor, history: Optional[Tensor], history_lengths: Optional[Tensor], bias: Optional[Tensor], allowed: Optional[Tensor],
+                     repetition: Optional[Tensor], frequency: Optional[Tensor], presence: Optional[Tensor], temperature: Optional[Tensor],
+                     values: list[float]) -> Tensor:
+    _check_adjust(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values)
+    if not logits.numel():
+        return logits.new_empty(logits.shape, dtype=torch.float32)
+    return _adjust_logits(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values)
+
+
+@adjust_logits_op.register_fake
+def _(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values):
+    return logits.new_empty(logits.shape, dtype=torch.float32)
+
+
+def adjust_logits(logits: Tensor, history: Tensor | None = None, history_lengths: Tensor | None = None, *, repetition_penalty=1., frequency_penalty=0.,
+                  presence_penalty=0., bias: Tensor | None = None, temperature=1., allowed: Tensor | None = None) -> Tensor:
+    """What is done to logits '... v' (bf16, fp16 or fp32) before a token is drawn from them, in one pass; fp32.  With c = how often an entry is in its row's
+    `history` '... t' (int32 or int64 tokens, the first `history_lengths` of them; what is outside [0, v), such as padding, is passed over):
+
+        c > 0:  x <- (x / repetition_penalty where x > 0, else x repetition_penalty) - frequency_penalty c - presence_penalty
+        x <- (x + bias) / temperature;   -inf where not `allowed`
+
+    The four numbers are Python's, or floating tensors of one value or one for each row (above 0 where a number has to be: not checked).  bias: 'v' or '... v';
+    allowed: bool 'v' or '... v', or int32 words of 32 entries each, the lowest bit the first, 'v/32' rounded up.  A row may have nothing allowed.
+    No gradients."""
+    numbers, tensors = [], []
+    for value in (repetition_penalty, frequency_penalty, presence_penalty, temperature):
+        given = isinstance(value, Tensor)
+        tensors.append(value if given else None)
+        numbers.append(None if given else float(value))
+    numbers = [neutral if n is None else n for n, neutral in zip(numbers, (1., 0., 0., 1.))]
+    _no_gradient("adjust_logits", logits, bias, *tensors)
+    args = logits, history, history_lengths, bias, allowed, *tensors, numbers
+    if _recorded():
+        return adjust_logits_op(*args)
+    _check_adjust(*args)
+    return _adjust_logits(*args) if logits.numel() else logits.new_empty(logits.shape, dtype=torch.float32)
