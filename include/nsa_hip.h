@@ -561,7 +561,7 @@ int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_t* cols, co
  *   keys, values: e4m3 codes [batch, kv_heads, capacity, dim_head] (finite ones up to 448, 0x7f and 0xff NaN), rows contiguous; the code c of a row stands
  *   for c times its scale, fp32 powers of two, one for each `block` rows of a kv head: key_scales, value_scales [batch, kv_heads, capacity / block],
  *   contiguous along the blocks.  Strides in elements: kv_stride {batch, head, row} for both of keys and values (multiples of 16), scale_stride
- *   {batch, head} for both scales.  keys, values: 16-byte aligned.  dim_head 64 or 128, block 16, 32, 64 or 128, capacity a multiple of it below 2^31.
+ *   {batch, head} for both scales.  keys, values: 16-byte aligned.  dim_head 64 or 128, block 16, 32, 64 or 128, capacity a multiple of it up to 2^30.
  *   Sequence b holds len(b) = lengths[b * length_stride] + length rows where lengths (device int32) is not NULL, else `length`; clamped to [0, capacity].
  *
  * nsa_cache8_append: rows of k and v [batch, kv_heads, rows, dim_head] of `dtype` (strides {batch, head, row}, rows 16-byte aligned), the first
@@ -573,7 +573,7 @@ int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_t* cols, co
  * `window` of its keys (0: all), or with sel_block > 0 the blocks idx of sel_block keys (of each kv head, or of each head where per_head_sel:
  * [batch, kv_heads or heads, num_sel] contiguous, int32 or int64) whose fmask byte is not 0, as far as the sequence has them, and the keys of the block
  * that its newest key is in.  A block named twice counts twice.  No key: zeros.  out: [batch, heads, dim_head] contiguous, of `dtype`.  group <= 32;
- * num_sel <= 2^20, and (num_sel + 1) * sel_block below 2^30.
+ * num_sel <= 2^20, (num_sel + 1) * sel_block and kv_stride below 2^30, q 16-byte aligned with strides of multiples of 8.
  * Sums in fp32, q and the probabilities as sums of bf16 parts (q exactly; probabilities to 16 bits, of fp32 queries to 24), results rounded once.
  * Only rows that are attended are read, in tiles of 16 that may begin before the first and end behind the last of them, in the cache. */
 typedef struct nsa_cache8_desc {

@@ -24,7 +24,8 @@ inline bool cache8_check(const nsa_cache8_desc* d) {
          d->reserved == 0 && !((d->kv_stride[0] | d->kv_stride[1] | d->kv_stride[2]) & 15) && d->kv_stride[2] >= d->dim_head;
 }
 inline bool cache8_supported(const nsa_cache8_desc* d) {
-  return (d->dim_head == 64 || d->dim_head == 128) && (d->block == 16 || d->block == 32 || d->block == 64 || d->block == 128);
+  return (d->dim_head == 64 || d->dim_head == 128) && (d->block == 16 || d->block == 32 || d->block == 64 || d->block == 128) &&
+         d->capacity <= 1 << 30;
 }
 
 inline Cache8Args cache8_args(const nsa_cache8_desc* d, const void* keys, const void* values, const float* key_scales, const float* value_scales,
