@@ -11,6 +11,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import functools
+import math
 import struct
 from typing import NamedTuple, Optional
 
@@ -2890,83 +2891,107 @@ def make_cache8(batch: int, kv_heads: int, rows: int, dim_head: int, block: int 
     return Cache8(codes(), codes(), scales(), scales())
 
 
-def _check_cache8(name: str, keys: Tensor, values: Tensor, key_scales: Tensor, value_scales: Tensor) -> int:
+# The host's part is most of a small call: what depends on sizes, types and layouts only - the checks and the descriptor - is looked up.
+
+def _layout(t: Tensor | None):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
+def _cache8_layout(keys: Tensor, values: Tensor, key_scales: Tensor, value_scales: Tensor):
+    return (keys.shape, keys.stride(), keys.dtype, values.shape, values.stride(), values.dtype, key_scales.shape, key_scales.stride(), key_scales.dtype,
+            value_scales.shape, value_scales.stride(), value_scales.dtype)
+
+
+def _cache8_plan(name: str, shape, stride, dtype, vshape, vstride, vdtype, scales, sstride, sdtype, zscales, zstride, zdtype) -> int:
     """Rows of a scale, of a cache that the kernels can be given: they read and write by address."""
-    if not keys.is_cuda or any(t.device != keys.device for t in (values, key_scales, value_scales)):
-        raise RuntimeError(f"{name}: needs a cache on one GPU (HIP kernels, no CPU fallback)")
-    if keys.dtype != _FP8 or values.dtype != _FP8 or key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32:
-        raise RuntimeError(f"{name}: cache of {keys.dtype}, {values.dtype}, {key_scales.dtype}, {value_scales.dtype}: expected float8_e4m3fn codes and fp32 scales")
-    shape, scales, stride = keys.shape, key_scales.shape, keys.stride()
-    if len(shape) != 4 or values.shape != shape or len(scales) != 3 or value_scales.shape != scales or scales[:2] != shape[:2] or 0 in shape or 0 in scales:
-        raise RuntimeError(f"{name}: cache of keys {tuple(shape)}, values {tuple(values.shape)}, scales {tuple(scales)} and {tuple(value_scales.shape)}: "
+    if dtype != _FP8 or vdtype != _FP8 or sdtype != torch.float32 or zdtype != torch.float32:
+        raise RuntimeError(f"{name}: cache of {dtype}, {vdtype}, {sdtype}, {zdtype}: expected float8_e4m3fn codes and fp32 scales")
+    if len(shape) != 4 or vshape != shape or len(scales) != 3 or zscales != scales or scales[:2] != shape[:2] or 0 in shape or 0 in scales:
+        raise RuntimeError(f"{name}: cache of keys {tuple(shape)}, values {tuple(vshape)}, scales {tuple(scales)} and {tuple(zscales)}: "
                            "expected 'b hk n d' twice and 'b hk n/block' twice")
     block = shape[2] // scales[2]
-    if shape[3] not in (64, 128) or block not in (16, 32, 64, 128) or shape[2] != block * scales[2]:
-        raise RuntimeError(f"{name}: cache of {shape[2]} rows of {shape[3]} features, {scales[2]} scales: expected 64 or 128 features and 16, 32, 64 or 128 rows a scale")
-    if (values.stride() != stride or value_scales.stride() != key_scales.stride() or stride[3] != 1 or stride[2] < shape[3] or (stride[0] | stride[1] | stride[2]) % 16
-            or key_scales.stride(2) != 1 or keys.data_ptr() % 16 or values.data_ptr() % 16):
-        raise RuntimeError(f"{name}: cache strides {stride}, {values.stride()}, {key_scales.stride()}, {value_scales.stride()}: keys and values, and both scales, "
-                           "are laid out alike, rows contiguous from 16-byte boundaries on")
+    if shape[3] not in (64, 128) or block not in (16, 32, 64, 128) or shape[2] != block * scales[2] or shape[2] > 1 << 30:
+        raise RuntimeError(f"{name}: cache of {shape[2]} rows of {shape[3]} features, {scales[2]} scales: expected 64 or 128 features, 16, 32, 64 or 128 rows a scale and "
+                           "up to 2^30 rows")
+    if vstride != stride or zstride != sstride or stride[3] != 1 or stride[2] < shape[3] or (stride[0] | stride[1] | stride[2]) % 16 or sstride[2] != 1:
+        raise RuntimeError(f"{name}: cache strides {stride}, {vstride}, {sstride}, {zstride}: keys and values, and both scales, are laid out alike, rows contiguous "
+                           "from 16-byte boundaries on")
     return block
 
 
-def _lengths(name: str, what: str, value, batch: int, most: int, device: torch.device):
-    """(device int32 tensor or None, stride, number) of a count for all sequences or of one for each."""
-    if not isinstance(value, Tensor):
-        if not 0 <= int(value) <= most:
-            raise RuntimeError(f"{name}: {what} {value}, expected 0 to {most}")
-        return None, 0, int(value)
-    if value.device != device or value.dtype not in (torch.int32, torch.int64) or value.numel() not in (1, batch) or value.dim() > 1:
-        raise RuntimeError(f"{name}: {what} {value.dtype} {tuple(value.shape)} on {value.device}: expected int32 or int64, one or one for each of {batch} sequences, on {device}")
-    if value.dtype == torch.int64:
-        value = value.clamp(0, 2 ** 31 - 1).to(torch.int32)
-    return value, 0 if value.numel() == 1 else value.stride(0), 0
+def _counts_ok(t, batch: int) -> bool:
+    """Layout of one count for all sequences or one for each."""
+    shape, _, dtype = t
+    return dtype in (torch.int32, torch.int64) and len(shape) <= 1 and shape.numel() in (1, batch)
 
 
-def _aligned_rows(t: Tensor) -> Tensor:
-    """Strides and address that 16-byte accesses of rows take (a view where they are already)."""
-    return t if t.stride(-1) == 1 and not any(s % 8 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+def _int32(t: Tensor) -> Tensor:
+    return t if t.dtype == torch.int32 else t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+
+
+def _step(t) -> int:
+    """Elements from one sequence's count to the next one's."""
+    return 0 if t is None or t[0].numel() == 1 else 1 if t[2] != torch.int32 else t[1][0]
+
+
+@functools.lru_cache(maxsize=256)
+def _append_plan(cache, k, v, starts, counts):
+    """(descriptor up to `length` and behind it, k's and v's strides, whether they have to be copied) of these layouts."""
+    name = "cache8_append"
+    block = _cache8_plan(name, *cache)
+    shape, stride, sstride = cache[0], cache[1], cache[7]
+    batch, hk, capacity, d = shape
+    if k[2] not in _LOSS_TYPES or v[2] != k[2]:
+        raise RuntimeError(f"{name}: k {k[2]}, v {v[2]}: expected both bf16, both fp16 or both fp32")
+    if len(k[0]) != 4 or v[0] != k[0] or k[0][:2] != (batch, hk) or not 0 < k[0][3] <= d or _kernel_dim(k[0][3]) != d:
+        raise RuntimeError(f"{name}: k {tuple(k[0])}, v {tuple(v[0])}, cache {tuple(shape)}: expected 'b hk rows d' of the cache's sequences and heads")
+    if starts is not None and not _counts_ok(starts, batch):
+        raise RuntimeError(f"{name}: start {starts[2]} {tuple(starts[0])}: expected int32 or int64, one or one for each of {batch} sequences")
+    if counts is not None and (counts[2] not in (torch.int32, torch.int64) or counts[0] != (batch,)):
+        raise RuntimeError(f"{name}: counts {counts[2]} {tuple(counts[0])}: expected int32 or int64, one for each of {batch} sequences")
+    desc = _CACHE8_DESC.pack(batch, hk, 1, d, block, capacity, _LOSS_TYPES[k[2]], 0, _step(starts), 0, 0, 0, 0, 0, 0., 0, *stride[:3], *sstride[:2], 0, 0)
+    copied = [k[0][3] != d or t[1][3] != 1 or any(x % 8 for x in t[1][:3]) for t in (k, v)]
+    strides = [(C.c_int64 * 3)(*t[1][:3]) for t in (k, v)]
+    return desc[:28], desc[32:], strides, copied, counts is not None and (counts[2] != torch.int32 or counts[1] != (1,))
 
 
 def _cache8_append(keys, values, key_scales, value_scales, k, v, starts, start, counts):
-    batch, hk, rows, _ = k.shape
-    block = keys.shape[2] // key_scales.shape[2]
-    with _on(keys.device):
-        starts, stride, _ = (None, 0, 0) if starts is None else _lengths("cache8_append", "start", starts, batch, 0, keys.device)
-        k, v = _aligned_rows(_pad_dim(k, keys.shape[3])), _aligned_rows(_pad_dim(v, keys.shape[3]))
-        if counts is not None:
-            counts = counts.clamp(0, rows).to(torch.int32).contiguous() if counts.dtype == torch.int64 else counts.contiguous()
-        desc = _CACHE8_DESC.pack(batch, hk, 1, keys.shape[3], block, keys.shape[2], _LOSS_TYPES[k.dtype], start, stride, 0, 0, 0, 0, 0, 0., 0,
-                                 *keys.stride()[:3], *key_scales.stride()[:2], 0, 0)
-        strides = C.c_int64 * 3
-        _lib.check(_lib.lib().nsa_cache8_append(desc, rows, k.data_ptr(), strides(*k.stride()[:3]), v.data_ptr(), strides(*v.stride()[:3]), _ptr(starts),
-                                                _ptr(counts), keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), _stream()),
-                   "nsa_cache8_append")
-
-
-def _check_append(keys, values, key_scales, value_scales, k, v, starts, start, counts):
-    _check_cache8("cache8_append", keys, values, key_scales, value_scales)
-    batch, hk, capacity, d = keys.shape
-    if k.device != keys.device or v.device != keys.device or k.dtype not in _LOSS_TYPES or v.dtype != k.dtype:
-        raise RuntimeError(f"cache8_append: k {k.dtype}, v {v.dtype} on {k.device}, {v.device}: expected both bf16, both fp16 or both fp32, on {keys.device}")
-    if k.dim() != 4 or v.shape != k.shape or k.shape[:2] != (batch, hk) or not 0 < k.shape[3] <= d or _kernel_dim(k.shape[3]) != d:
-        raise RuntimeError(f"cache8_append: k {tuple(k.shape)}, v {tuple(v.shape)}, cache {tuple(keys.shape)}: expected 'b hk rows d' of the cache's sequences and heads")
-    if starts is None:
-        if start < 0 or start + k.shape[2] > capacity:
-            raise RuntimeError(f"cache8_append: rows {start} to {start + k.shape[2] - 1} of a cache for {capacity}")
-    else:
-        _lengths("cache8_append", "start", starts, batch, capacity, keys.device)
-    if counts is not None and (counts.device != keys.device or counts.dtype not in (torch.int32, torch.int64) or counts.shape != (batch,)):
-        raise RuntimeError(f"cache8_append: counts {counts.dtype} {tuple(counts.shape)} on {counts.device}: expected int32 or int64, one for each of {batch} sequences, on {keys.device}")
+    device = keys.get_device()
+    if (device < 0 or values.get_device() != device or key_scales.get_device() != device or value_scales.get_device() != device or k.get_device() != device
+            or v.get_device() != device or (starts is not None and starts.get_device() != device) or (counts is not None and counts.get_device() != device)):
+        raise RuntimeError("cache8_append: needs tensors on one GPU (HIP kernels, no CPU fallback)")
+    head, tail, strides, copied, convert = _append_plan(_cache8_layout(keys, values, key_scales, value_scales), _layout(k), _layout(v), _layout(starts), _layout(counts))
+    rows = k.shape[2]
+    if starts is None and not 0 <= start <= keys.shape[2] - rows:
+        raise RuntimeError(f"cache8_append: rows {start} to {start + rows - 1} of a cache for {keys.shape[2]}")
+    kp, vp, codes, more = k.data_ptr(), v.data_ptr(), keys.data_ptr(), values.data_ptr()
+    if (codes | more) % 16:
+        raise RuntimeError("cache8_append: a cache's rows begin at 16-byte boundaries")
+    if not rows:
+        return
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return _cache8_append(keys, values, key_scales, value_scales, k, v, starts, start, counts)
+    if copied[0] or kp % 16:
+        k = _pad_dim(k, keys.shape[3]).clone(memory_format=torch.contiguous_format)
+        kp, strides = k.data_ptr(), [(C.c_int64 * 3)(*k.stride()[:3]), strides[1]]
+    if copied[1] or vp % 16:
+        v = _pad_dim(v, keys.shape[3]).clone(memory_format=torch.contiguous_format)
+        vp, strides = v.data_ptr(), [strides[0], (C.c_int64 * 3)(*v.stride()[:3])]
+    if starts is not None:
+        starts = _int32(starts)
+    if convert:
+        counts = _int32(counts).contiguous()
+    _lib.check(_lib.lib().nsa_cache8_append(head + start.to_bytes(4, "little") + tail, rows, kp, strides[0], vp, strides[1], 0 if starts is None else starts.data_ptr(),
+                                            0 if counts is None else counts.data_ptr(), codes, more, key_scales.data_ptr(), value_scales.data_ptr(), _stream()),
+               "nsa_cache8_append")
 
 
 @torch.library.custom_op("nsa_amd::cache8_append", mutates_args=("keys", "values", "key_scales", "value_scales"))
 def cache8_append_op(keys: Tensor, values: Tensor, key_scales: Tensor, value_scales: Tensor, k: Tensor, v: Tensor, starts: Optional[Tensor], start: int,
                      counts: Optional[Tensor]) -> None:
     # (a traced graph calls this with what it is run on)
-    _check_append(keys, values, key_scales, value_scales, k, v, starts, start, counts)
-    if k.shape[2]:
-        _cache8_append(keys, values, key_scales, value_scales, k, v, starts, start, counts)
+    _cache8_append(keys, values, key_scales, value_scales, k, v, starts, start, counts)
 
 
 @cache8_append_op.register_fake
@@ -2975,10 +3000,15 @@ def _(keys, values, key_scales, value_scales, k, v, starts, start, counts):
 
 
 def _no_gradient(name: str, *tensors) -> None:
+    """(called where gradients are recorded, or in a forward-mode level)"""
     if torch.is_grad_enabled() and any(isinstance(t, Tensor) and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
     if not _is_compiling() and _forward_ad._current_level >= 0:
         _refuse_tangents(name, tensors)
+
+
+def _differentiates() -> bool:
+    return torch.is_grad_enabled() or (not _is_compiling() and _forward_ad._current_level >= 0)
 
 
 def cache8_append(cache: Cache8, k: Tensor, v: Tensor, start=0, counts: Tensor | None = None) -> None:
@@ -2987,72 +3017,84 @@ def cache8_append(cache: Cache8, k: Tensor, v: Tensor, start=0, counts: Tensor |
     it.  Where `start` is a tensor it is known to the device only: rows past the capacity are dropped.  A block's scale is the smallest power of two that
     takes its largest value to 448; one that grows when rows come into a block that holds some rounds those again, in units of the new.  Infinities
     become NaN.  Nothing else of the cache is written."""
+    if _differentiates():
+        _no_gradient("cache8_append", k, v)
     starts, number = (start, 0) if isinstance(start, Tensor) else (None, int(start))
-    _no_gradient("cache8_append", k, v)
-    args = *cache, k, v, starts, number, counts
-    if _recorded():
-        cache8_append_op(*args)
-        return
-    _check_append(*args)
-    if k.shape[2]:
-        _cache8_append(*args)
+    (cache8_append_op if _recorded() else _cache8_append)(*cache, k, v, starts, number, counts)
+
+
+@functools.lru_cache(maxsize=256)
+def _attend8_plan(cache, q, lengths, window, size, idx, fmask, scale):
+    """(descriptor up to `length` and behind it, bytes of workspace, whether q and the selection have to be copied) of these layouts."""
+    name = "cache8_select_attend" if size else "cache8_attend"
+    block = _cache8_plan(name, *cache)
+    shape, stride, sstride = cache[0], cache[1], cache[7]
+    batch, hk, capacity, d = shape
+    qshape, qstride, dtype = q
+    if dtype not in _LOSS_TYPES:
+        raise RuntimeError(f"{name}: q {dtype}: expected bf16, fp16 or fp32")
+    if (len(qshape) != 4 or qshape[0] != batch or qshape[2] != 1 or not 0 < qshape[3] <= d or _kernel_dim(qshape[3]) != d or qshape[1] % hk
+            or not 0 < qshape[1] <= 32 * hk):
+        raise RuntimeError(f"{name}: q {tuple(qshape)}, cache {tuple(shape)}: expected 'b hq 1 d' with hq up to 32 times the kv heads and a multiple of them")
+    if lengths is not None and not _counts_ok(lengths, batch):
+        raise RuntimeError(f"{name}: lengths {lengths[2]} {tuple(lengths[0])}: expected int32 or int64, one or one for each of {batch} sequences")
+    if window < 0 or size < 0 or (idx is None) != (size == 0) or (fmask is None) != (size == 0):
+        raise RuntimeError(f"{name}: window {window}, block size {size}")
+    chosen, chosen_copied = 0, False
+    if size:
+        if idx[2] not in (torch.int32, torch.int64) or fmask[2] not in (torch.bool, torch.uint8):
+            raise RuntimeError(f"{name}: idx {idx[2]}, fmask {fmask[2]}: expected int32 or int64, and bool")
+        if len(idx[0]) != 4 or idx[0][:3] not in ((batch, hk, 1), (batch, qshape[1], 1)) or fmask[0] != idx[0]:
+            raise RuntimeError(f"{name}: idx {tuple(idx[0])}, fmask {tuple(fmask[0])}: expected 'b hk 1 S' or 'b hq 1 S'")
+        chosen = idx[0][3]
+        want = idx[0][1] * chosen, chosen, chosen, 1
+        chosen_copied = any(x != y for t in (idx, fmask) for x, y, n in zip(t[1], want, t[0]) if n > 1)
+    copied = qshape[3] != d or qstride[3] != 1 or qstride[0] % 8 or qstride[1] % 8
+    desc = _CACHE8_DESC.pack(batch, hk, qshape[1] // hk, d, block, capacity, _LOSS_TYPES[dtype], 0, _step(lengths), min(window, capacity), size, chosen,
+                             size > 0 and idx[0][1] != hk, size > 0 and idx[2] == torch.int64, scale, 0, *stride[:3], *sstride[:2],
+                             *((qshape[1] * d, d) if copied else qstride[:2]))
+    nbytes = C.c_size_t()
+    _lib.check(_lib.lib().nsa_cache8_workspace_bytes(desc, C.byref(nbytes)), "nsa_cache8_workspace_bytes")
+    own = _CACHE8_DESC.pack(*_CACHE8_DESC.unpack(desc)[:-2], qshape[1] * d, d)      # of a copy of q
+    return desc[:28], desc[32:], own[32:], nbytes.value, copied, chosen_copied
 
 
 def _cache8_attend(q, keys, values, key_scales, value_scales, lengths, length, window, size, idx, fmask, scale):
-    b, hq, _, d0 = q.shape
-    _, hk, capacity, d = keys.shape
-    with _on(keys.device):
-        lengths, stride, _ = (None, 0, 0) if lengths is None else _lengths("cache8_attend", "lengths", lengths, b, 0, keys.device)
-        if d != d0:
-            q = _pad_dim(q, d)
-        if q.stride(3) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-            q = q.clone(memory_format=torch.contiguous_format)
-        chosen = 0
-        if size:
-            idx = idx.contiguous()
-            fmask = (fmask.view(torch.uint8) if fmask.dtype == torch.bool else fmask).contiguous()
-            chosen = idx.shape[3]
-        desc = _CACHE8_DESC.pack(b, hk, hq // hk, d, capacity // key_scales.shape[2], capacity, _LOSS_TYPES[q.dtype], length, stride, window, size, chosen,
-                                 size > 0 and idx.shape[1] != hk, size > 0 and idx.dtype == torch.int64, scale, 0, *keys.stride()[:3], *key_scales.stride()[:2],
-                                 q.stride(0), q.stride(1))
-        L = _lib.lib()
-        nbytes = C.c_size_t()
-        _lib.check(L.nsa_cache8_workspace_bytes(desc, C.byref(nbytes)), "nsa_cache8_workspace_bytes")
-        out = torch.empty((b, hq, 1, d), dtype=q.dtype, device=q.device)
-        ws = torch.empty((nbytes.value,), dtype=torch.uint8, device=q.device) if nbytes.value else None
-        _lib.check(L.nsa_cache8_attend(desc, q.data_ptr(), keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), _ptr(lengths),
-                                       _ptr(idx) if chosen else None, _ptr(fmask) if chosen else None, _ptr(ws), nbytes.value, out.data_ptr(), _stream()),
-                   "nsa_cache8_attend")
-    return out if d == d0 else out[..., :d0]
-
-
-def _check_attend8(q, keys, values, key_scales, value_scales, lengths, length, window, size, idx, fmask, scale):
-    name = "cache8_select_attend" if size else "cache8_attend"
-    _check_cache8(name, keys, values, key_scales, value_scales)
-    b, hk, capacity, d = keys.shape
-    if q.device != keys.device or q.dtype not in _LOSS_TYPES:
-        raise RuntimeError(f"{name}: q {q.dtype} on {q.device}: expected bf16, fp16 or fp32 on {keys.device}")
-    if q.dim() != 4 or q.shape[0] != b or q.shape[2] != 1 or not 0 < q.shape[3] <= d or _kernel_dim(q.shape[3]) != d or q.shape[1] % hk or not 0 < q.shape[1] <= 32 * hk:
-        raise RuntimeError(f"{name}: q {tuple(q.shape)}, cache {tuple(keys.shape)}: expected 'b hq 1 d' with hq up to 32 times the kv heads and a multiple of them")
-    if lengths is None:
-        _lengths(name, "lengths", length, b, capacity, keys.device)
-    else:
-        _lengths(name, "lengths", lengths, b, capacity, keys.device)
-    if window < 0 or size < 0 or (idx is None) != (size == 0) or (fmask is None) != (size == 0):
-        raise RuntimeError(f"{name}: window {window}, block size {size}")
-    if size:
-        if idx.device != keys.device or fmask.device != keys.device or idx.dtype not in (torch.int32, torch.int64) or fmask.dtype not in (torch.bool, torch.uint8):
-            raise RuntimeError(f"{name}: idx {idx.dtype} on {idx.device}, fmask {fmask.dtype} on {fmask.device}: expected int32 or int64, and bool, on {keys.device}")
-        if idx.dim() != 4 or idx.shape[:3] not in ((b, hk, 1), (b, q.shape[1], 1)) or fmask.shape != idx.shape:
-            raise RuntimeError(f"{name}: idx {tuple(idx.shape)}, fmask {tuple(fmask.shape)}: expected 'b hk 1 S' or 'b hq 1 S'")
+    device = keys.get_device()
+    if (device < 0 or values.get_device() != device or key_scales.get_device() != device or value_scales.get_device() != device or q.get_device() != device
+            or (lengths is not None and lengths.get_device() != device) or (idx is not None and (idx.get_device() != device or fmask.get_device() != device))):
+        raise RuntimeError(f"cache8_{'select_' if size else ''}attend: needs tensors on one GPU (HIP kernels, no CPU fallback)")
+    head, tail, own, nbytes, copied, chosen_copied = _attend8_plan(_cache8_layout(keys, values, key_scales, value_scales), _layout(q), _layout(lengths), window, size,
+                                                                   _layout(idx), _layout(fmask), scale)
+    if lengths is None and not 0 <= length <= keys.shape[2]:
+        raise RuntimeError(f"cache8_{'select_' if size else ''}attend: lengths {length}, expected 0 to {keys.shape[2]}")
+    qp, codes, more = q.data_ptr(), keys.data_ptr(), values.data_ptr()
+    if (codes | more) % 16:
+        raise RuntimeError(f"cache8_{'select_' if size else ''}attend: a cache's rows begin at 16-byte boundaries")
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return _cache8_attend(q, keys, values, key_scales, value_scales, lengths, length, window, size, idx, fmask, scale)
+    d0 = q.shape[3]
+    if copied or qp % 16:
+        q = _pad_dim(q, keys.shape[3]).clone(memory_format=torch.contiguous_format)
+        qp, tail = q.data_ptr(), own
+    if chosen_copied:
+        idx, fmask = idx.contiguous(), fmask.contiguous()
+    if lengths is not None:
+        lengths = _int32(lengths)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ws = q.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+    _lib.check(_lib.lib().nsa_cache8_attend(head + length.to_bytes(4, "little") + tail, qp, codes, more, key_scales.data_ptr(), value_scales.data_ptr(),
+                                            0 if lengths is None else lengths.data_ptr(), 0 if idx is None else idx.data_ptr(),
+                                            0 if fmask is None else fmask.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes, out.data_ptr(), _stream()),
+               "nsa_cache8_attend")
+    return out if out.shape[3] == d0 else out[..., :d0]
 
 
 @torch.library.custom_op("nsa_amd::cache8_attend", mutates_args=())
 def cache8_attend_op(q: Tensor, keys: Tensor, values: Tensor, key_scales: Tensor, value_scales: Tensor, lengths: Optional[Tensor], length: int, window: int,
                      size: int, idx: Optional[Tensor], fmask: Optional[Tensor], scale: float) -> Tensor:
-    _check_attend8(q, keys, values, key_scales, value_scales, lengths, length, window, size, idx, fmask, scale)
-    out = _cache8_attend(q, keys, values, key_scales, value_scales, lengths, length, window, size, idx, fmask, scale)
-    return out.contiguous()
+    return _cache8_attend(q, keys, values, key_scales, value_scales, lengths, length, window, size, idx, fmask, scale).contiguous()
 
 
 @cache8_attend_op.register_fake
@@ -3060,14 +3102,12 @@ def _(q, keys, values, key_scales, value_scales, lengths, length, window, size, 
     return q.new_empty(q.shape)
 
 
-def _attend8(q, cache, lengths, window, size, idx, fmask, scale):
+def _attend8(name, q, cache, lengths, window, size, idx, fmask, scale):
+    if _differentiates():
+        _no_gradient(name, q)
     lengths, length = (lengths, 0) if isinstance(lengths, Tensor) else (None, int(lengths))
-    args = q, *cache, lengths, length, window, size, idx, fmask, float(q.shape[-1] ** -0.5 if scale is None else scale)
-    _no_gradient("cache8_select_attend" if size else "cache8_attend", q)
-    if _recorded():
-        return cache8_attend_op(*args)
-    _check_attend8(*args)
-    return _cache8_attend(*args)
+    return (cache8_attend_op if _recorded() else _cache8_attend)(q, *cache, lengths, length, window, size, idx, fmask,
+                                                                 float(q.shape[-1] ** -0.5 if scale is None else scale))
 
 
 def cache8_attend(q: Tensor, cache: Cache8, lengths, window: int | None = None, scale: float | None = None) -> Tensor:
@@ -3076,89 +3116,115 @@ def cache8_attend(q: Tensor, cache: Cache8, lengths, window: int | None = None, 
     `window`.  Returns 'b hq 1 d' of q's type; zeros where there is no key.  Rows that are not attended may hold anything.  No gradients."""
     if window is not None and int(window) < 1:
         raise RuntimeError(f"cache8_attend: window {window}, expected 1 or more")
-    return _attend8(q, cache, lengths, 0 if window is None else int(window), 0, None, None, scale)
+    return _attend8("cache8_attend", q, cache, lengths, 0 if window is None else int(window), 0, None, None, scale)
 
 
 def cache8_select_attend(q: Tensor, cache: Cache8, lengths, block: int, idx: Tensor, fmask: Tensor, scale: float | None = None) -> Tensor:
     """`decode_select_attend` over an 8-bit cache (NSA.py:446-515): the newest token's query attends the blocks idx[..., slot] of `block` keys where fmask is
     true, as far as the sequence has them, and the block that the newest token is in.  idx / fmask: 'b hk 1 S' or, for a selection of each head, 'b hq 1 S';
     a block named twice counts twice, one that the sequence does not have not at all.  `lengths`, types and result as `cache8_attend`."""
-    if int(block) < 1:
+    if not 1 <= int(block) < 1 << 30:
         raise RuntimeError(f"cache8_select_attend: blocks of {block} keys")
-    return _attend8(q, cache, lengths, 0, int(block), idx, fmask, scale)
+    return _attend8("cache8_select_attend", q, cache, lengths, 0, int(block), idx, fmask, scale)
+
+
+@functools.lru_cache(maxsize=256)
+def _logits_plan(logits, history, history_lengths, bias, allowed, numbers, values):
+    """(descriptor, which of the operands have to be laid out first) of these layouts; `numbers`: of the four tensors that may stand for values."""
+    name = "adjust_logits"
+    shape, stride, dtype = logits
+    if dtype not in _LOSS_TYPES or len(shape) < 1 or shape[-1] == 0:
+        raise RuntimeError(f"{name}: logits {dtype} {tuple(shape)}: expected bf16, fp16 or fp32 '... v'")
+    lead, vocab = shape[:-1], shape[-1]
+    rows = lead.numel()
+    whole = torch.int32, torch.int64
+    if history is not None and (history[2] not in whole or len(history[0]) < 1 or history[0][:-1] != lead):
+        raise RuntimeError(f"{name}: history {history[2]} {tuple(history[0])}: expected int32 or int64 '... t' for logits {tuple(shape)}")
+    if history_lengths is not None and (history is None or history_lengths[2] not in whole or history_lengths[0] != lead):
+        raise RuntimeError(f"{name}: history_lengths {history_lengths[2]} {tuple(history_lengths[0])}: expected int32 or int64, one for each row of a history")
+    if bias is not None and (not bias[2].is_floating_point or bias[0] not in ((vocab,), shape)):
+        raise RuntimeError(f"{name}: bias {bias[2]} {tuple(bias[0])}: expected floating 'v' or '... v' for logits {tuple(shape)}")
+    kind = 0
+    if allowed is not None:
+        width = {torch.bool: vocab, torch.int32: (vocab + 31) // 32}.get(allowed[2])
+        if width is None or allowed[0] not in ((width,), (*lead, width)):
+            raise RuntimeError(f"{name}: allowed {allowed[2]} {tuple(allowed[0])}: expected bool 'v' or '... v', or int32 words of 32 entries, for logits {tuple(shape)}")
+        kind = 2 if allowed[2] == torch.int32 else 1
+    for what, t in zip(("repetition_penalty", "frequency_penalty", "presence_penalty", "temperature"), numbers):
+        if t is not None and (not t[2].is_floating_point or t[0].numel() not in (1, rows) or len(t[0]) > max(len(lead), 1)):
+            raise RuntimeError(f"{name}: {what} {t[2]} {tuple(t[0])}: expected a number, or floating, one or one for each of {rows} rows")
+    if not (0 < values[0] < math.inf and abs(values[1]) < math.inf and abs(values[2]) < math.inf and 0 < values[3] < math.inf):
+        raise ValueError(f"{name}: repetition_penalty {values[0]}, frequency_penalty {values[1]}, presence_penalty {values[2]}, temperature {values[3]}: "
+                         "expected finite numbers, the first and the last above 0")
+
+    def row_step(t, width):
+        """Elements from a row to the next, None where rows are not laid out one after the other at equal distances."""
+        if t is None or (len(t[0]) == 1 and len(lead)):
+            return 0 if t is None or width == 1 or t[1][0] == 1 else None
+        step = width if rows == 1 else None
+        if width == 1 or t[1][-1] == 1:
+            inner = 1
+            for n, at in zip(reversed(t[0][:-1]), reversed(t[1][:-1])):
+                if n == 1:
+                    continue
+                if step is None:
+                    step = at
+                elif at != step * inner:
+                    return None
+                inner *= n
+            return step
+        return None
+
+    contiguous = lambda t: all(n == 1 or at == w for n, at, w in zip(t[0], t[1], _strides_of(t[0])))
+    x_step, bias_step, allowed_step = row_step(logits, vocab), row_step(bias, vocab), row_step(allowed, None if allowed is None else allowed[0][-1])
+    fixes = (x_step is None, history is not None and not contiguous(history), history_lengths is not None and not (history_lengths[2] == torch.int32 and contiguous(history_lengths)),
+             bias is not None and (bias[2] != torch.float32 or bias_step is None), allowed is not None and allowed_step is None,
+             tuple(t is not None and not (t[2] == torch.float32 and contiguous(t)) for t in numbers))
+    if fixes[3]:
+        bias_step = 0 if len(bias[0]) == 1 and len(lead) else vocab
+    if fixes[4]:
+        allowed_step = 0 if len(allowed[0]) == 1 and len(lead) else allowed[0][-1]
+    desc = _LOGITS_DESC.pack(rows, vocab if x_step is None else x_step, vocab, _LOSS_TYPES[dtype], 0 if history is None else history[0][-1],
+                             history is not None and history[2] == torch.int64, kind, bias_step, allowed_step,
+                             *(int(t is not None and t[0].numel() > 1) for t in numbers), *values)
+    return desc, fixes, any(fixes[:5]) or any(fixes[5])
+
+
+def _strides_of(shape):
+    steps, n = [], 1
+    for size in reversed(shape):
+        steps.append(n)
+        n *= size
+    return reversed(steps)
 
 
 def _adjust_logits(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values):
-    vocab = logits.shape[-1]
-    rows = logits.numel() // vocab
-    with _on(logits.device):
-        x = logits.reshape(rows, vocab)
-        if x.stride(1) != 1:
-            x = x.contiguous()
-        per_row = lambda t, width: (t, 0) if t.dim() == 1 else (t.reshape(rows, width), None)
-        if history is not None:
-            history = history.reshape(rows, -1).contiguous()
-        if history_lengths is not None:
-            history_lengths = history_lengths.reshape(rows)
-            if history_lengths.dtype == torch.int64:
-                history_lengths = history_lengths.clamp(0, 2 ** 31 - 1).to(torch.int32)
-            history_lengths = history_lengths.contiguous()
-        strides = {}
-        if bias is not None:
-            bias, strides["bias"] = per_row(bias.float(), vocab)
-        kind = 0
-        if allowed is not None:
-            kind = 2 if allowed.dtype == torch.int32 else 1
-            allowed, strides["allowed"] = per_row(allowed, allowed.shape[-1])
-        if bias is not None and bias.stride(-1) != 1:
-            bias = bias.contiguous()
-        if allowed is not None and allowed.stride(-1) != 1:
-            allowed = allowed.contiguous()
-        step = lambda t, name: 0 if t is None or strides[name] == 0 else t.stride(0)
-        tensors = [None if t is None else t.reshape(-1).float().contiguous() for t in (repetition, frequency, presence, temperature)]
-        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
-        t = 0 if history is None else history.shape[1]
-        desc = _LOGITS_DESC.pack(rows, x.stride(0), vocab, _LOSS_TYPES[x.dtype], t, history is not None and history.dtype == torch.int64, kind,
-                                 step(bias, "bias"), step(allowed, "allowed"), *(int(p is not None and p.numel() > 1) for p in tensors), *values)
-        _lib.check(_lib.lib().nsa_adjust_logits(desc, x.data_ptr(), _ptr(history) if t else None, _ptr(history_lengths), *map(_ptr, tensors[:3]), _ptr(bias),
-                                                _ptr(allowed), _ptr(tensors[3]), out.data_ptr(), _stream()), "nsa_adjust_logits")
+    device = logits.get_device()
+    given = history, history_lengths, bias, allowed, repetition, frequency, presence, temperature
+    if device < 0 or any([t is not None and t.get_device() != device for t in given]):
+        raise RuntimeError("adjust_logits: needs tensors on one GPU (HIP kernels, no CPU fallback)")
+    desc, fixes, any_fix = _logits_plan(_layout(logits), _layout(history), _layout(history_lengths), _layout(bias), _layout(allowed),
+                                        (_layout(repetition), _layout(frequency), _layout(presence), _layout(temperature)), tuple(values))
+    out = torch.empty_like(logits, dtype=torch.float32, memory_format=torch.contiguous_format)
+    if not out.numel():
+        return out
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return _adjust_logits(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values)
+    if any_fix:
+        logits, history = logits.contiguous() if fixes[0] else logits, history.contiguous() if fixes[1] else history
+        history_lengths = _int32(history_lengths).contiguous() if fixes[2] else history_lengths
+        bias, allowed = bias.float().contiguous() if fixes[3] else bias, allowed.contiguous() if fixes[4] else allowed
+        repetition, frequency, presence, temperature = (t.float().contiguous() if fix else t for t, fix in zip(given[4:], fixes[5]))
+    _lib.check(_lib.lib().nsa_adjust_logits(desc, logits.data_ptr(), _ptr(history), _ptr(history_lengths), _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(bias),
+                                            _ptr(allowed), _ptr(temperature), out.data_ptr(), _stream()), "nsa_adjust_logits")
     return out
-
-
-def _check_adjust(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values):
-    name, device = "adjust_logits", logits.device
-    if not logits.is_cuda or any(t is not None and t.device != device for t in (history, history_lengths, bias, allowed, repetition, frequency, presence, temperature)):
-        raise RuntimeError(f"{name}: needs tensors on one GPU (HIP kernels, no CPU fallback)")
-    if logits.dtype not in _LOSS_TYPES or logits.dim() < 1 or logits.shape[-1] == 0:
-        raise RuntimeError(f"{name}: logits {logits.dtype} {tuple(logits.shape)}: expected bf16, fp16 or fp32 '... v'")
-    lead, vocab = logits.shape[:-1], logits.shape[-1]
-    rows = lead.numel()
-    whole = torch.int32, torch.int64
-    if history is not None and (history.dtype not in whole or history.dim() < 1 or history.shape[:-1] != lead):
-        raise RuntimeError(f"{name}: history {history.dtype} {tuple(history.shape)}: expected int32 or int64 '... t' for logits {tuple(logits.shape)}")
-    if history_lengths is not None and (history is None or history_lengths.dtype not in whole or history_lengths.shape != lead):
-        raise RuntimeError(f"{name}: history_lengths {history_lengths.dtype} {tuple(history_lengths.shape)}: expected int32 or int64, one for each row of a history")
-    if bias is not None and (not bias.is_floating_point() or bias.shape not in ((vocab,), logits.shape)):
-        raise RuntimeError(f"{name}: bias {bias.dtype} {tuple(bias.shape)}: expected floating 'v' or '... v' for logits {tuple(logits.shape)}")
-    if allowed is not None:
-        width = {torch.bool: vocab, torch.int32: (vocab + 31) // 32}.get(allowed.dtype)
-        if width is None or allowed.shape not in ((width,), (*lead, width)):
-            raise RuntimeError(f"{name}: allowed {allowed.dtype} {tuple(allowed.shape)}: expected bool 'v' or '... v', or int32 words of 32 entries, for logits {tuple(logits.shape)}")
-    for what, t in (("repetition_penalty", repetition), ("frequency_penalty", frequency), ("presence_penalty", presence), ("temperature", temperature)):
-        if t is not None and (not t.is_floating_point() or t.numel() not in (1, rows) or t.dim() > max(len(lead), 1)):
-            raise RuntimeError(f"{name}: {what} {t.dtype} {tuple(t.shape)}: expected a number, or floating, one or one for each of {rows} rows")
-    if not (0 < values[0] < float("inf") and abs(values[1]) < float("inf") and abs(values[2]) < float("inf") and 0 < values[3] < float("inf")):
-        raise ValueError(f"{name}: repetition_penalty {values[0]}, frequency_penalty {values[1]}, presence_penalty {values[2]}, temperature {values[3]}: "
-                         "expected finite numbers, the first and the last above 0")
 
 
 @torch.library.custom_op("nsa_amd::adjust_logits", mutates_args=())
 def adjust_logits_op(logits: Tensor, history: Optional[Tensor], history_lengths: Optional[Tensor], bias: Optional[Tensor], allowed: Optional[Tensor],
                      repetition: Optional[Tensor], frequency: Optional[Tensor], presence: Optional[Tensor], temperature: Optional[Tensor],
                      values: list[float]) -> Tensor:
-    _check_adjust(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values)
-    if not logits.numel():
-        return logits.new_empty(logits.shape, dtype=torch.float32)
     return _adjust_logits(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values)
 
 
@@ -3179,14 +3245,10 @@ def adjust_logits(logits: Tensor, history: Tensor | None = None, history_lengths
     allowed: bool 'v' or '... v', or int32 words of 32 entries each, the lowest bit the first, 'v/32' rounded up.  A row may have nothing allowed.
     No gradients."""
     numbers, tensors = [], []
-    for value in (repetition_penalty, frequency_penalty, presence_penalty, temperature):
+    for value, neutral in zip((repetition_penalty, frequency_penalty, presence_penalty, temperature), (1., 0., 0., 1.)):
         given = isinstance(value, Tensor)
         tensors.append(value if given else None)
-        numbers.append(None if given else float(value))
-    numbers = [neutral if n is None else n for n, neutral in zip(numbers, (1., 0., 0., 1.))]
-    _no_gradient("adjust_logits", logits, bias, *tensors)
-    args = logits, history, history_lengths, bias, allowed, *tensors, numbers
-    if _recorded():
-        return adjust_logits_op(*args)
-    _check_adjust(*args)
-    return _adjust_logits(*args) if logits.numel() else logits.new_empty(logits.shape, dtype=torch.float32)
+        numbers.append(neutral if given else float(value))
+    if _differentiates():
+        _no_gradient("adjust_logits", logits, bias, *tensors)
+    return (adjust_logits_op if _recorded() else _adjust_logits)(logits, history, history_lengths, bias, allowed, *tensors, numbers)
