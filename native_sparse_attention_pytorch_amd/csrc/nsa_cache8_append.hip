@@ -15,7 +15,7 @@ struct AppendArgs {
   long k0, k1, k2, v0, v1, v2;
   const int* counts;
   int rows, touched;                   // rows handed in for each sequence, blocks that they may touch
-  long total;                          // (sequence, kv head, keys or values, block)
+  unsigned total;                      // (sequence, kv head, keys or values, block)
 };
 
 template <class T>
@@ -66,6 +66,16 @@ __device__ __forceinline__ int scale_exponent(uint32_t bits) {
 }
 __device__ __forceinline__ float power_of_two(int k) { return __builtin_bit_cast(float, (uint32_t)(k + 127) << 23); }
 
+// maximum over the wave, in all lanes; mirrors of eight and sixteen lanes reach the other half of each
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dpp_quad_xor1(v));
+  v = fmaxf(v, dpp_quad_xor2(v));
+  v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true)));
+  v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xF, 0xF, true)));
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return halves_max(v);
+}
+
 template <int D, int B>
 struct AppendShape {
   static constexpr int CHUNKS = D * B / 8;                            // of eight values
@@ -78,80 +88,79 @@ template <class T, int D, int B>
 __global__ __launch_bounds__((AppendShape<D, B>::THREADS)) void cache8_append_kernel(const AppendArgs A) {
   using S = AppendShape<D, B>;
   constexpr int LPR = D / 8;
-  __shared__ uint32_t top_s[S::BLOCKS * S::WAVES];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long id = (long)blockIdx.x * S::BLOCKS + wave / S::WAVES;
+  __shared__ float top_s[S::BLOCKS * S::WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % S::WAVES;
+  const unsigned id = blockIdx.x * S::BLOCKS + wave / S::WAVES;
   const bool here = id < A.total;
-  const long rest = here ? id / A.touched : 0;
+  const unsigned rest = here ? id / (unsigned)A.touched : 0;
   const int t = here ? (int)(id - rest * A.touched) : 0;
   const bool is_v = rest & 1;
-  const int unit = (int)(rest >> 1), b = unit / A.c.hk, h = unit % A.c.hk;
+  const int unit = (int)(rest >> 1), b = unit / A.c.hk, h = unit - b * A.c.hk;
   const int start = cache8_length(A.c, b);
   const int n = A.counts != nullptr ? min(max(A.counts[b], 0), A.rows) : A.rows;
-  const long end = min((long)start + n, (long)A.c.cap), row0 = (long)(start / B + t) * B;
-  const bool any = here && row0 < end && n > 0;
+  const int row0 = (start / B + t) * B, first = start - row0, last = (int)min((long)start + n, (long)A.c.cap) - row0;      // of the block, and its new rows
+  const bool any = here && last > 0 && last > first;
 
-  const T* src = is_v ? reinterpret_cast<const T*>(A.v) + b * A.v0 + h * A.v1 : reinterpret_cast<const T*>(A.k) + b * A.k0 + h * A.k1;
+  const T* src = (is_v ? reinterpret_cast<const T*>(A.v) + b * A.v0 + h * A.v1 : reinterpret_cast<const T*>(A.k) + b * A.k0 + h * A.k1);
   const long s_row = is_v ? A.v2 : A.k2;
-  uint8_t* dst = (is_v ? A.c.values : A.c.keys) + b * A.c.s0 + h * A.c.s1;
+  uint8_t* dst = (is_v ? A.c.values : A.c.keys) + b * A.c.s0 + h * A.c.s1 + row0 * A.c.s2;
   float* scale = (is_v ? A.c.value_scales : A.c.key_scales) + b * A.c.z0 + h * A.c.z1 + row0 / B;
+  // chunk c of a lane: row part * RPW + c * STEP + lane / LPR, values 8 (lane % LPR) ..
+  constexpr int RPW = 64 / LPR, STEP = RPW * S::WAVES;
+  const int mine = part * RPW + lane / LPR, f = lane % LPR * 8;
 
   floatx8 x[S::PER];
   uintx2 old[S::PER];
-  uint32_t top = 0;
-  float s_old = 0.f;
-  const bool held = row0 < start;
+  float top = 0.f, s_old = 0.f;
+  const bool held = first > 0;
   if (any) {
     if (held) s_old = *scale;
+    const T* from = src + (long)(mine - first) * s_row + f;
 #pragma unroll
     for (int c = 0; c < S::PER; ++c) {
-      const int at = (c * S::WAVES + wave % S::WAVES) * 64 + lane;
-      const long row = row0 + at / LPR;
-      const int f = at % LPR * 8;
-      if (row >= start && row < end) x[c] = load_values(src + (row - start) * s_row + f);
-      else if (row < start) old[c] = *reinterpret_cast<const uintx2*>(dst + row * A.c.s2 + f);
+      const int row = mine + c * STEP;
+      if (row >= first && row < last) x[c] = load_values(from + (long)(c * STEP) * s_row);
+      else if (row < first) old[c] = *reinterpret_cast<const uintx2*>(dst + row * A.c.s2 + f);
     }
 #pragma unroll
     for (int c = 0; c < S::PER; ++c) {
-      const long row = row0 + ((c * S::WAVES + wave % S::WAVES) * 64 + lane) / LPR;
-      if (row >= start && row < end)
+      const int row = mine + c * STEP;
+      if (row >= first && row < last) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const uint32_t m = bits_of(x[c][e]) & 0x7fffffffu;
-          top = max(top, m < 0x7f800000u ? m : 0u);
+          const float m = fabsf(x[c][e]);
+          top = fmaxf(top, m < INFINITY ? m : 0.f);
         }
+      }
     }
-#pragma unroll
-    for (int o = 1; o <= 32; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    top = wave_max(top);
   }
   if constexpr (S::WAVES > 1) {
     if (lane == 0) top_s[wave] = top;
     __syncthreads();
-    const int w0 = wave / S::WAVES * S::WAVES;
 #pragma unroll
-    for (int w = 0; w < S::WAVES; ++w) top = max(top, top_s[w0 + w]);
+    for (int w = 0; w < S::WAVES; ++w) top = fmaxf(top, top_s[wave - part + w]);
   }
   if (!any) return;
-  float s_new = power_of_two(scale_exponent(top));
+  float s_new = power_of_two(scale_exponent(bits_of(top)));
   if (held) s_new = fmaxf(s_new, s_old);
   const float inv = 1.0f / s_new;      // (of a power of two: exact)
-  if (lane == 0 && wave % S::WAVES == 0) *scale = s_new;
+  if (lane == 0 && part == 0) *scale = s_new;
 #pragma unroll
   for (int c = 0; c < S::PER; ++c) {
-    const int at = (c * S::WAVES + wave % S::WAVES) * 64 + lane;
-    const long row = row0 + at / LPR;
-    uintx2* to = reinterpret_cast<uintx2*>(dst + row * A.c.s2 + at % LPR * 8);
-    if (row >= start && row < end) *to = codes_of(x[c], inv);
-    else if (row < start && s_new != s_old) *to = codes_of(values_of(old[c]), s_old * inv);
+    const int row = mine + c * STEP;
+    uintx2* to = reinterpret_cast<uintx2*>(dst + row * A.c.s2 + f);
+    if (row >= first && row < last) *to = codes_of(x[c], inv);
+    else if (row < first && s_new != s_old) *to = codes_of(values_of(old[c]), s_old * inv);
   }
 }
 
 template <class T, int D, int B>
 static int append_launch(const AppendArgs& A, hipStream_t st) {
   using S = AppendShape<D, B>;
-  const long groups = (A.total + S::BLOCKS - 1) / S::BLOCKS;
-  if (groups * S::THREADS > 0xffffffffL) return NSA_E_UNSUPPORTED;
-  hipLaunchKernelGGL((cache8_append_kernel<T, D, B>), dim3((unsigned)groups), dim3(S::THREADS), 0, st, A);
+  const unsigned groups = (A.total + S::BLOCKS - 1) / S::BLOCKS;
+  if ((unsigned long)groups * S::THREADS >= 1UL << 32) return NSA_E_UNSUPPORTED;
+  hipLaunchKernelGGL((cache8_append_kernel<T, D, B>), dim3(groups), dim3(S::THREADS), 0, st, A);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : (int)e;
 }
@@ -189,8 +198,9 @@ extern "C" int nsa_cache8_append(const nsa_cache8_desc* d, int32_t rows, const v
   // (rows that begin anywhere in a block)
   A.touched = (int)(((long)rows + d->block - 2) / d->block + 1);
   A.touched = A.touched < d->capacity / d->block ? A.touched : d->capacity / d->block;
-  A.total = (long)d->batch * d->kv_heads * 2 * A.touched;
-  if ((long)d->batch * d->kv_heads > 1L << 30) return NSA_E_UNSUPPORTED;
+  const long units = (long)d->batch * d->kv_heads;
+  if (units > 1L << 24 || units * 2 * A.touched >= 1L << 31) return NSA_E_UNSUPPORTED;
+  A.total = (unsigned)(units * 2 * A.touched);
   hipStream_t st = (hipStream_t)stream;
   return d->dtype == 0 ? append_dim<__bf16>(A, d->dim_head, st) : d->dtype == 1 ? append_dim<_Float16>(A, d->dim_head, st) : append_dim<float>(A, d->dim_head, st);
 }

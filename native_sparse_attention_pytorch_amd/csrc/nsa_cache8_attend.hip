@@ -21,18 +21,24 @@ struct Attend8Args {
   const void* q;
   long q0, q1;
   int g, units, gc;                    // units: kv heads, or query heads that have blocks of their own; gc: query heads of a unit
-  int window, sel_block, num_sel, idx64;
+  int window, sel_block, num_sel, idx64, per_block;      // per_block: sel_block / 16
   const void* idx;
   const uint8_t* fmask;
   float scale;
   int block_shift;
-  int nparts, tiles;                   // a part: this many tiles of 32 keys
-  float* part;                         // records [gc][D] sums, [gc] maxima, [gc] weights, rec floats each
-  int rec;
+  int batch;
+  int shared;                          // work-groups share the tiles of all units, else each has a unit
+  int most;                            // tiles of a unit at most
+  float* part;                         // shared: two records for each work-group, [gc][D] sums, [gc] maxima, [gc] weights, rec floats each
+  int groups;                          // work-groups of the first launch
+  int rec, table;                      // table: where in LDS the sequences' first tiles are, in bytes
   void* out;
 };
 
-constexpr int kTile = 32, kWaves = 8;
+typedef __attribute__((__vector_size__(2 * sizeof(float)))) float floatx2;
+
+constexpr int kTile = 32, kTable = 2048, kListed = 64;      // kTable: sequences of a launch; kListed: tiles whose rows are in LDS
+constexpr int kUnit = 8, kShare = 16, kAlone = 40;            // see Shares; kAlone: tiles of a unit up to which it has a work-group of eight waves for itself
 
 __device__ __forceinline__ floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -55,17 +61,18 @@ __device__ __forceinline__ float quarters_sum(float v) {
 struct Keys8 {
   int len, first, base, places;
 };
-__device__ __forceinline__ Keys8 keys_of(const Attend8Args& A, int b) {
+__device__ __forceinline__ Keys8 keys_of(const Attend8Args& A, int len) {
   Keys8 K;
-  K.len = cache8_length(A.c, b);
+  K.len = len;
   K.first = A.window > 0 && A.sel_block == 0 ? max(0, K.len - A.window) : 0;
   K.base = K.first & ~15;
   K.places = A.sel_block > 0 ? (K.len > 0 ? (A.num_sel + 1) * A.sel_block : 0) : K.len - K.base;
   return K;
 }
+__device__ __forceinline__ int tiles_of(const Attend8Args& A, int b) { return (keys_of(A, cache8_length(A.c, b)).places + kTile - 1) / kTile; }
 // the row of a place of a selection; without one ~ of the newest key's, which is attended: what is there may be read in its place
 __device__ __forceinline__ int selected_row(const Attend8Args& A, const Keys8& K, long unit, int place) {
-  const int none = ~(K.len - 1);
+  const int none = ~max(K.len - 1, 0);
   if (place >= K.places) return none;
   const int slot = place / A.sel_block, own = (K.len - 1) / A.sel_block;
   long blk = own;
@@ -89,13 +96,16 @@ template <> struct Parts8<float> { static constexpr int Q = 3, P = 3; };
 template <int N>
 __device__ __forceinline__ void split_parts(const float (&x)[8], bf16x8 (&to)[N]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float r = x[e];
+  for (int e = 0; e < 8; e += 2) {
+    float r0 = x[e], r1 = x[e + 1];
 #pragma unroll
     for (int p = 0; p < N; ++p) {
-      const __bf16 h = (__bf16)r;
-      to[p][e] = h;
-      r -= (float)h;
+      const bf16x2 h = __builtin_convertvector((floatx2{r0, r1}), bf16x2);      // (as one instruction)
+      const uint32_t w = __builtin_bit_cast(uint32_t, h);
+      to[p][e] = h[0];
+      to[p][e + 1] = h[1];
+      r0 -= __builtin_bit_cast(float, w << 16);
+      r1 -= __builtin_bit_cast(float, w & 0xffff0000u);
     }
   }
 }
@@ -118,30 +128,135 @@ __device__ __forceinline__ void transpose_bytes(const uint32_t (&d)[4], uint32_t
   t[3] = __builtin_amdgcn_perm(e, b, 0x07060302u);
 }
 
+// Where a unit's keys are: a range of rows; selected blocks of a multiple of 16 keys; selected blocks of any size.
+enum { kRange = 0, kBlocks = 1, kPacked = 2 };
+
 template <int D>
 struct Tile8 {                         // what a lane holds of 32 keys
   uintx4 k[2][D / 64];                 // key n of each 16: 16 codes
   uint32_t v[2][4][D / 64];            // keys 4 q + e: D / 16 codes
-  float ks[2];
-  floatx4 vs[2];
+  float ks[2], vs[2];                  // ks: of key n.  vs: one for all 16 keys (kPacked reads them from LDS where it needs them)
 };
 
-template <class T, int D, bool SEL>
+// Shared tiles.  A sequence's tiles are as many as its length has, known to the device only.  All units lie one after the other on a line, each as long as its
+// tiles and kUnit more (what a unit costs besides them), and the line is cut into equal shares, one for each work-group, whatever the lengths are.  A unit whose
+// tiles lie in one share is finished there; of the others each share leaves a record, and the merge finds them by the same arithmetic.  (Parts of a fixed
+// size for each unit, sized for the capacity: 48 sequences of 1 to 16384 keys took 105 us where these take __; most work-groups had nothing to do,
+// and a few too much.)
+// n / d of n below 2^50: by the division of doubles, put right where that is rounded up (one of 64-bit integers takes 150 instructions)
+__device__ __forceinline__ long quotient(long n, long d) {
+  long q = (long)((double)n / (double)d);
+  q -= q * d > n;
+  return q + (n - q * d >= d);
+}
+
+struct Shares {
+  long total, share;                   // the line's length, a work-group's part of it
+  __device__ __forceinline__ void set(long all, int groups) {
+    total = all;
+    share = max(quotient(all + groups - 1, groups), (long)kShare);
+  }
+};
+
+// a value that is the same in all lanes, for the compiler too
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long uniform(long x) { return (long)((unsigned long)(unsigned)uniform((int)(x >> 32)) << 32 | (unsigned)uniform((int)x)); }
+
+__device__ __forceinline__ long length_on_line(long tiles) { return tiles > 0 ? tiles + kUnit : 0; }
+
+// where the sequences' first units begin, in units' lengths before each, into `first` (batch + 1 of them); a sequence without tiles takes none
+template <int NT>
+__device__ __forceinline__ void first_tiles(const Attend8Args& A, long* first) {
+  __shared__ long sum_s[NT / 64];
+  const int tid = threadIdx.x, each = (A.batch + NT - 1) / NT, b0 = min(A.batch, tid * each), b1 = min(A.batch, b0 + each);
+  long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += length_on_line(tiles_of(A, b));
+  long up = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long x = __shfl_up(up, o, 64);
+    if ((tid & 63) >= o) up += x;
+  }
+  if ((tid & 63) == 63) sum_s[tid >> 6] = up;
+  __syncthreads();
+  long at = up - mine;
+  for (int w = 0; w < (tid >> 6); ++w) at += sum_s[w];
+  for (int b = b0; b < b1; ++b) {
+    first[b] = at;
+    at += length_on_line(tiles_of(A, b));
+  }
+  if (b1 == A.batch && b0 < b1) first[A.batch] = at;
+  __syncthreads();
+}
+// all sequences have as many tiles
+__device__ __forceinline__ bool alike(const Attend8Args& A) { return A.sel_block > 0 || A.c.lengths == nullptr || A.c.length_stride == 0; }
+
+template <class T, int D, int MODE, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend8Args A) {
   constexpr int QP = Parts8<T>::Q, PP = Parts8<T>::P, KS = D / 32, DT = D / 16;
   extern __shared__ __align__(16) char lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, q4 = lane >> 4;
-  const long unit = blockIdx.x / A.nparts;
-  const int part = (int)(blockIdx.x - unit * A.nparts);
-  const int b = (int)(unit / A.units), u = (int)(unit - (long)b * A.units);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, q4 = lane >> 4;
+  // (the length of a sequence without keys counts for a selection: no tile of it has any)
+  long pos = 0, end = 0, each = 0;
+  Shares all;
+  const long* first = reinterpret_cast<const long*>(lds + A.table);
+  if (A.shared) {
+    if (alike(A)) {
+      each = uniform(length_on_line(A.sel_block > 0 ? A.most : tiles_of(A, 0)));
+      all.set(each * A.batch * A.units, gridDim.x);
+    } else {
+      first_tiles<64 * kWaves>(A, const_cast<long*>(first));
+      all.set(uniform(first[A.batch]) * A.units, gridDim.x);
+    }
+    pos = blockIdx.x * all.share;
+    end = min(all.total, pos + all.share);
+    if (pos >= end) return;
+  }
+  int seq = -1;
+  do {
+  int b, u, t0, t1, tiles;
+  if (A.shared) {
+    long at, length = each;            // of the unit that `pos` lies in: where it begins, how long it is
+    if (each > 0) {
+      const long unit = quotient(pos, each);
+      b = (int)unit / A.units;
+      u = (int)unit - b * A.units;
+      at = unit * each;
+    } else {
+      if (seq < 0) {                   // the last sequence that begins here or before
+        int lo = 0, hi = A.batch - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (uniform(first[mid]) * A.units <= pos) lo = mid;
+          else hi = mid - 1;
+        }
+        seq = lo;
+      } else {
+        while (uniform(first[seq + 1]) * A.units <= pos) ++seq;
+      }
+      b = seq;
+      const long before = uniform(first[b]);
+      length = uniform(first[b + 1]) - before;
+      u = (int)quotient(pos - before * A.units, length);
+      at = before * A.units + u * length;
+    }
+    tiles = (int)(length - kUnit);
+    t0 = (int)max(0L, pos - at - kUnit);
+    t1 = (int)min((long)tiles, end - at - kUnit);
+    pos = at + length;
+    if (t0 >= t1) continue;            // (its tiles are all in the next share)
+  } else {
+    b = blockIdx.x / A.units;
+    u = blockIdx.x - b * A.units;
+    t0 = 0;
+    t1 = tiles = A.most;
+  }
+  const bool whole_unit = t0 == 0 && t1 == tiles;
+  const long unit = (long)b * A.units + u;
   const int hk = A.units == A.c.hk ? u : u / A.g, head0 = A.units == A.c.hk ? u * A.g : u;
-  const Keys8 K = keys_of(A, b);
-  const int tiles = (K.places + kTile - 1) / kTile, t0 = part * A.tiles, t1 = min(tiles, t0 + A.tiles);
-  if (t0 >= t1 && part > 0) return;    // (the merge knows how many parts there are)
 
   // more than 16 query heads: half of the waves for the first 16
-  const int groups = A.gc > 16 ? 2 : 1, group = groups == 2 ? wave & 1 : 0;
-  const int w0 = groups == 2 ? wave >> 1 : wave, nw = kWaves / groups;
+  const int groups = A.gc > 16 ? 2 : 1, nw = kWaves / groups, group = wave / nw, w0 = wave - group * nw;
   const int cols = min(16, A.gc - 16 * group);
 
   bf16x8 Q[KS][QP];
@@ -157,76 +272,93 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend
       split_parts(f, Q[s]);
     }
   }
+
+  const Keys8 K = keys_of(A, uniform(cache8_length(A.c, b)));
+  const int last = K.len - 1;
+  if constexpr (MODE == kRange) t1 = min(t1, (K.places + kTile - 1) / kTile);
+
   const float sc = A.scale * kLog2e;
-  const uint8_t* kb = A.c.keys + b * A.c.s0 + hk * A.c.s1 + 16 * q4;
-  const uint8_t* vb = A.c.values + b * A.c.s0 + hk * A.c.s1 + DT * n;
+  const uint8_t* kb = A.c.keys + b * A.c.s0 + hk * A.c.s1;
+  const uint8_t* vb = A.c.values + b * A.c.s0 + hk * A.c.s1;
   const float* kz = A.c.key_scales + b * A.c.z0 + hk * A.c.z1;
   const float* vz = A.c.value_scales + b * A.c.z0 + hk * A.c.z1;
-  const uint32_t s2 = (uint32_t)A.c.s2;
+  const long s2 = A.c.s2;
+  const uint32_t k_lane = 16 * q4, v_lane = DT * n;
 
   int* row_s = reinterpret_cast<int*>(lds);
-  float* ks_s = reinterpret_cast<float*>(lds) + A.tiles * kTile;
-  float* vs_s = ks_s + A.tiles * kTile;
-  if constexpr (SEL) {
-    for (int i = tid; i < (t1 - t0) * kTile; i += 64 * kWaves) {
-      const int r = selected_row(A, K, unit, t0 * kTile + i), at = (r < 0 ? ~r : r) >> A.block_shift;
-      row_s[i] = r;
-      ks_s[i] = kz[at];
-      vs_s[i] = vz[at];
-    }
-    __syncthreads();
-  }
+  float* ks_s = reinterpret_cast<float*>(lds) + kListed * kTile;
+  float* vs_s = ks_s + kListed * kTile;
 
   float m = -INFINITY, l = 0.f;
   floatx4 O[DT];
 #pragma unroll
   for (int c = 0; c < DT; ++c) O[c] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  auto load = [&](int t, Tile8<D>& X) {
+  // tiles c0 .. c1 - 1 at a time: as many as there are lanes, or room in LDS, for where their rows are
+  const int chunk = MODE == kBlocks ? 32 * nw : MODE == kPacked ? kListed : t1 - t0;
+  int c0 = t0, lane_row = -1;
+  // the first row of the 16 keys i of the wave's tile r, -1: there is none
+  auto row0 = [&](int r, int i) {
+    if constexpr (MODE == kBlocks) return __builtin_amdgcn_readlane(lane_row, 2 * r + i);
+    const int x = K.base + (c0 + w0 + r * nw) * kTile + 16 * i;
+    return x <= last ? x : -1;
+  };
+  // the rows of 16 keys that begin with r0 where they may not all be there: without one ~ of the newest, which is attended and read instead
+  auto row = [&](int r0, int x) { return (r0 >= 0) & (x >= K.first) & (x <= last) ? x : ~last; };
+  auto whole = [&](int r0) { return r0 >= K.first && r0 + 15 <= last; };
+  auto load_k = [&](int r, Tile8<D>& X) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if constexpr (SEL) {
-        const int at = (t - t0) * kTile + 16 * i;
-        int r = row_s[at + n];
-        r = r < 0 ? ~r : r;
-        X.ks[i] = ks_s[at + n];
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) X.k[i][j] = *reinterpret_cast<const uintx4*>(kb + (uint64_t)(uint32_t)r * s2 + 64 * j);
-        const intx4 rv = *reinterpret_cast<const intx4*>(row_s + at + 4 * q4);
-        X.vs[i] = *reinterpret_cast<const floatx4*>(vs_s + at + 4 * q4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int x = rv[e] < 0 ? ~rv[e] : rv[e];
-          const uint32_t* p = reinterpret_cast<const uint32_t*>(vb + (uint64_t)(uint32_t)x * s2);
-#pragma unroll
-          for (int j = 0; j < D / 64; ++j) X.v[i][e][j] = p[j];
-        }
+      const uint8_t* p;
+      if constexpr (MODE == kPacked) {
+        const int at = (w0 + r * nw) * kTile + 16 * i + n, x = row_s[at];
+        X.ks[i] = ks_s[at];
+        p = kb + (long)(x ^ (x >> 31)) * s2 + k_lane;
       } else {
-        // (a place without a key: the newest one, which is attended, is read instead)
-        const int r0 = K.base + t * kTile + 16 * i, last = K.len - 1;
-        const int z = min(r0, last) >> A.block_shift;
-        X.ks[i] = kz[z];
-        const float s = vz[z];
-        X.vs[i] = floatx4{s, s, s, s};
-        int r = r0 + n;
-        r = r < K.first || r > last ? last : r;
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) X.k[i][j] = *reinterpret_cast<const uintx4*>(kb + (uint64_t)(uint32_t)r * s2 + 64 * j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          int x = r0 + 4 * q4 + e;
-          x = x < K.first || x > last ? last : x;
-          const uint32_t* p = reinterpret_cast<const uint32_t*>(vb + (uint64_t)(uint32_t)x * s2);
-#pragma unroll
-          for (int j = 0; j < D / 64; ++j) X.v[i][e][j] = p[j];
+        const int r0 = row0(r, i);
+        X.ks[i] = kz[(r0 < 0 ? last : r0) >> A.block_shift];
+        if (whole(r0)) {
+          p = kb + r0 * s2 + (n * s2 + k_lane);
+        } else {
+          const int x = row(r0, r0 + n);
+          p = kb + (x ^ (x >> 31)) * s2 + k_lane;
         }
       }
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) X.k[i][j] = *reinterpret_cast<const uintx4*>(p + 64 * j);
+    }
+  };
+  auto load_v = [&](int r, Tile8<D>& X) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* p[4];
+      if constexpr (MODE == kPacked) {
+        const intx4 rv = *reinterpret_cast<const intx4*>(row_s + (w0 + r * nw) * kTile + 16 * i + 4 * q4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = vb + (long)(rv[e] ^ (rv[e] >> 31)) * s2 + v_lane;
+      } else {
+        const int r0 = row0(r, i);
+        X.vs[i] = vz[(r0 < 0 ? last : r0) >> A.block_shift];
+        if (whole(r0)) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e] = vb + r0 * s2 + (4 * q4 * s2 + v_lane) + e * s2;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int x = row(r0, r0 + 4 * q4 + e);
+            p[e] = vb + (x ^ (x >> 31)) * s2 + v_lane;
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) X.v[i][e][j] = reinterpret_cast<const uint32_t*>(p[e])[j];
     }
   };
 
-  auto work = [&](int t, const Tile8<D>& X) {
-    float s[8];
-    float mx = -INFINITY;
+  float s[8];
+  auto scores = [&](int r, const Tile8<D>& X) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       floatx4 S = {0.f, 0.f, 0.f, 0.f};
@@ -239,25 +371,28 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend
           S = mfma16(k1, Q[2 * j + 1][p], S);
         }
       }
-      intx4 rows;
-      if constexpr (SEL) rows = *reinterpret_cast<const intx4*>(row_s + (t - t0) * kTile + 16 * i + 4 * q4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        bool live;
-        if constexpr (SEL) live = rows[e] >= 0;
-        else {
-          const int r = K.base + t * kTile + 16 * i + 4 * q4 + e;
-          live = r >= K.first && r < K.len;
+      for (int e = 0; e < 4; ++e) s[4 * i + e] = S[e] * sc;
+      if constexpr (MODE == kPacked) {
+        const intx4 rv = *reinterpret_cast<const intx4*>(row_s + (w0 + r * nw) * kTile + 16 * i + 4 * q4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * i + e] = rv[e] >= 0 ? s[4 * i + e] : -INFINITY;
+      } else {
+        const int r0 = row0(r, i);
+        if (!whole(r0)) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * i + e] = row(r0, r0 + 4 * q4 + e) >= 0 ? s[4 * i + e] : -INFINITY;
         }
-        const float v = live ? S[e] * sc : -INFINITY;
-        s[4 * i + e] = v;
-        mx = fmaxf(mx, v);
       }
     }
+  };
+  auto probabilities = [&](int r, const Tile8<D>& X, bf16x8 (&P)[PP]) {
+    float mx = s[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e]);
     mx = quarters_max(mx);
     if (__any(mx > m)) {                         // (a NaN raises no maximum: it reaches the sum by itself)
-      const float mn = fmaxf(m, mx), a = fast_exp2(m - mn);
-      const float by = m == -INFINITY ? 0.f : a;
+      const float mn = fmaxf(m, mx), by = m == -INFINITY ? 0.f : fast_exp2(m - mn);
       m = mn;
       l *= by;
 #pragma unroll
@@ -265,13 +400,20 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend
     }
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float p = fast_exp2(s[e] - ref);
-      l += p;
-      s[e] = p * X.vs[e >> 2][e & 3];
+    for (int i = 0; i < 2; ++i) {
+      floatx4 v;
+      if constexpr (MODE == kPacked) v = *reinterpret_cast<const floatx4*>(vs_s + (w0 + r * nw) * kTile + 16 * i + 4 * q4);
+      else v = floatx4{X.vs[i], X.vs[i], X.vs[i], X.vs[i]};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = fast_exp2(s[4 * i + e] - ref);
+        l += p;
+        s[4 * i + e] = p * v[e];
+      }
     }
-    bf16x8 P[PP];
     split_parts(s, P);
+  };
+  auto products = [&](const Tile8<D>& X, const bf16x8 (&P)[PP]) {
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
       uint32_t tr[2][4];
@@ -289,40 +431,73 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend
     }
   };
 
-  // (tiles of a selection whose blocks are not there are passed over)
-  auto next = [&](int t) {
-    for (; t < t1; t += nw) {
-      if constexpr (SEL) {
-        if (!__any(row_s[(t - t0) * kTile + (lane & 31)] >= 0)) continue;
+  // the wave's tiles; those of a selection whose blocks are not there are passed over.  The next tile's keys are asked for as soon as this one's
+  // are operands, its values likewise: one set of registers, two waves more on a SIMD than with two sets
+  for (; c0 < t1; c0 += chunk) {
+    const int c1 = min(t1, c0 + chunk), rounds = c0 + w0 < c1 ? (c1 - c0 - w0 + nw - 1) / nw : 0;
+    if constexpr (MODE == kBlocks) {
+      // lane 2 r + i: keys 16 i .. 16 i + 15 of tile c0 + w0 + r nw
+      const int at = 2 * (c0 + w0 + (lane >> 1) * nw) + (lane & 1), slot = at / A.per_block;
+      long blk = -1;
+      if (slot < A.num_sel) {
+        const long e = unit * A.num_sel + slot;
+        const uint8_t live = A.fmask[e];
+        blk = A.idx64 ? reinterpret_cast<const long*>(A.idx)[e] : (long)reinterpret_cast<const int*>(A.idx)[e];
+        blk = live != 0 && blk >= 0 && blk < 1L << 30 ? blk : -1;
+      } else if (slot == A.num_sel && last >= 0) {
+        blk = last / A.sel_block;      // the newest key's
       }
-      break;
+      const long x = blk * A.sel_block + 16 * (at - slot * A.per_block);
+      lane_row = blk < 0 || x > last ? -1 : (int)x;
+    } else if constexpr (MODE == kPacked) {
+      if (c0 > t0) __syncthreads();
+      for (int i = tid; i < (c1 - c0) * kTile; i += 64 * kWaves) {
+        const int r = selected_row(A, K, unit, c0 * kTile + i), at = (r ^ (r >> 31)) >> A.block_shift;
+        row_s[i] = r;
+        ks_s[i] = kz[at];
+        vs_s[i] = vz[at];
+      }
+      __syncthreads();
     }
-    return t;
-  };
-  Tile8<D> X, Y;
-  int t = next(t0 + w0);
-  if (t < t1) load(t, X);
-  while (t < t1) {
-    const int tn = next(t + nw);
-    if (tn < t1) load(tn, Y);
-    work(t, X);
-    X = Y;
-    t = tn;
+    auto next = [&](int r) {
+      if constexpr (MODE == kBlocks) {
+        while (r < rounds && row0(r, 0) < 0 && row0(r, 1) < 0) ++r;
+      } else if constexpr (MODE == kPacked) {
+        while (r < rounds && !__any(row_s[(w0 + r * nw) * kTile + (lane & 31)] >= 0)) ++r;
+      }
+      return r;
+    };
+    Tile8<D> X;
+    int r = next(0);
+    if (r < rounds) { load_k(r, X); load_v(r, X); }
+    while (r < rounds) {
+      const int rn = next(r + 1);
+      scores(r, X);
+      if (rn < rounds) load_k(rn, X);
+      bf16x8 P[PP];
+      probabilities(r, X, P);
+      products(X, P);
+      if (rn < rounds) load_v(rn, X);
+      r = rn;
+    }
   }
   l = quarters_sum(l);
 
   // the waves' results as one
   __syncthreads();                               // (the lists of rows are read no more)
-  constexpr int H = D / 2, RO = H + 4;           // half of the features at a time: 36 KB at 16 columns
+  constexpr int H = D / 2, RO = H + 4;           // half of the features at a time
   float* m_s = reinterpret_cast<float*>(lds);
   float* l_s = m_s + kWaves * 16;
   float* o_s = l_s + kWaves * 16;                // [wave][cols of a group][RO]
   const int most = min(16, A.gc);
-  if (q4 == 0) { m_s[wave * 16 + n] = m; l_s[wave * 16 + n] = l; }
+  if (q4 == 0) m_s[wave * 16 + n] = m;
   __syncthreads();
   float M = -INFINITY;
-  for (int w = group; w < kWaves; w += groups) M = fmaxf(M, m_s[w * 16 + n]);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    if (w < nw) M = fmaxf(M, m_s[(group * nw + w) * 16 + n]);
   const float by = m == -INFINITY ? 0.f : fast_exp2(m - M);
+  if (q4 == 0) l_s[wave * 16 + n] = m == -INFINITY ? l : by * l;      // (a NaN that raised no maximum)
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     // (place f of the half: feature DT (4 (f / 2 DT) + 2 half) + f % 2 DT)
@@ -332,73 +507,118 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int c = 0; c < DT; c += 4) {
-          const int r = 2 * half + i;
-          *reinterpret_cast<floatx4*>(o + DT * i + c) = floatx4{O[c][r] * by, O[c + 1][r] * by, O[c + 2][r] * by, O[c + 3][r] * by};
+          const int x = 2 * half + i;
+          *reinterpret_cast<floatx4*>(o + DT * i + c) = floatx4{O[c][x] * by, O[c + 1][x] * by, O[c + 2][x] * by, O[c + 3][x] * by};
         }
     }
     __syncthreads();
     for (int i = tid; i < A.gc * (H / 4); i += 64 * kWaves) {
       const int g = i / (H / 4), at = i % (H / 4) * 4, gr = g >> 4, c = g & 15, f = DT * (4 * (at / (2 * DT)) + 2 * half) + at % (2 * DT);
       floatx4 o = {0.f, 0.f, 0.f, 0.f};
-      float Mg = -INFINITY, L = 0.f;
-      for (int w = gr; w < kWaves; w += groups) Mg = fmaxf(Mg, m_s[w * 16 + c]);
-      for (int w = gr; w < kWaves; w += groups) {
-        const float mw = m_s[w * 16 + c];
-        L += (mw == -INFINITY ? 1.f : fast_exp2(mw - Mg)) * l_s[w * 16 + c];
-        o += *reinterpret_cast<const floatx4*>(o_s + (w * most + c) * RO + at);
-      }
-      if (A.nparts == 1) {
-        T* to = reinterpret_cast<T*>(A.out) + ((long)b * A.c.hk * A.g + head0 + g) * D + f;
+      float L = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) to[e] = (T)(L == 0.f ? 0.f : o[e] / L);
+      for (int w = 0; w < kWaves; ++w)
+        if (w < nw) {
+          L += l_s[(gr * nw + w) * 16 + c];
+          o += *reinterpret_cast<const floatx4*>(o_s + ((gr * nw + w) * most + c) * RO + at);
+        }
+      if (whole_unit) {
+        typedef __attribute__((__vector_size__(4 * sizeof(T)))) T vec;
+        *reinterpret_cast<vec*>(reinterpret_cast<T*>(A.out) + ((long)b * A.c.hk * A.g + head0 + g) * D + f) =
+            L == 0.f ? vec{(T)0.f, (T)0.f, (T)0.f, (T)0.f} : vec{(T)(o[0] / L), (T)(o[1] / L), (T)(o[2] / L), (T)(o[3] / L)};
       } else {
-        float* rec = A.part + blockIdx.x * (long)A.rec;
+        float* rec = A.part + (2L * blockIdx.x + (t0 == 0)) * A.rec;
         *reinterpret_cast<floatx4*>(rec + g * D + f) = o;
-        if (f == 0) { rec[A.gc * D + g] = Mg; rec[A.gc * D + A.gc + g] = L; }
+        if (f == 0) {
+          float Mg = -INFINITY;
+          for (int w = 0; w < nw; ++w) Mg = fmaxf(Mg, m_s[(gr * nw + w) * 16 + c]);
+          rec[A.gc * D + g] = Mg;
+          rec[A.gc * D + A.gc + g] = L;
+        }
       }
     }
     if (half == 0) __syncthreads();
   }
+  if (pos < end) __syncthreads();      // (LDS is used again)
+  } while (pos < end);
 }
 
 // the parts of a head, weighted by their maxima
-template <class T, int D>
-__global__ __launch_bounds__(256) void cache8_merge_kernel(const Attend8Args A) {
-  constexpr int LPP = D / 4, PPR = 256 / LPP;
-  __shared__ float red_s[4];
+template <class T, int D, int kMerge>
+__global__ __launch_bounds__(kMerge) void cache8_merge_kernel(const Attend8Args A) {
+  constexpr int LPP = D / 4, PPR = kMerge / LPP;
   __shared__ __align__(16) float acc_s[PPR][D];
-  __shared__ float l_s[PPR];
+  __shared__ float m_s[PPR], l_s[PPR];
   const int tid = threadIdx.x, heads = A.c.hk * A.g;
   const long bh = blockIdx.x;
   const int b = (int)(bh / heads), head = (int)(bh % heads);
   const int u = A.units == A.c.hk ? head / A.g : head, gi = A.units == A.c.hk ? head % A.g : 0;
-  const Keys8 K = keys_of(A, b);
-  const int parts = max(1, ((K.places + kTile - 1) / kTile + A.tiles - 1) / A.tiles);
-  const float* base = A.part + ((long)b * A.units + u) * A.nparts * A.rec;
-  const int om = A.gc * D + gi;
-  float M = -INFINITY;
-  for (int p = tid; p < parts; p += 256) M = fmaxf(M, base[(long)p * A.rec + om]);
-#pragma unroll
-  for (int o = 1; o <= 32; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-  if ((tid & 63) == 0) red_s[tid >> 6] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(red_s[0], red_s[1]), fmaxf(red_s[2], red_s[3]));
-  floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-  float L = 0.f;
-  for (int p = tid / LPP; p < parts; p += PPR) {
-    const float* rec = base + (long)p * A.rec;
-    const float mp = rec[om], w = mp == -INFINITY ? 1.f : fast_exp2(mp - M);      // (a part without a number for its maximum: NaN or nothing)
-    L += w * rec[om + A.gc];
-    acc += w * *reinterpret_cast<const floatx4*>(rec + gi * D + 4 * (tid % LPP));
+  extern __shared__ __align__(16) char lds[];
+  Shares all;
+  long at, length;
+  if (alike(A)) {
+    length = length_on_line(A.sel_block > 0 ? A.most : tiles_of(A, b));
+    all.set(length * A.batch * A.units, A.groups);
+    at = ((long)b * A.units + u) * length;
+  } else {
+    long* first = reinterpret_cast<long*>(lds);
+    first_tiles<kMerge>(A, first);
+    all.set(first[A.batch] * A.units, A.groups);
+    length = first[b + 1] - first[b];
+    at = first[b] * A.units + u * length;
   }
-  *reinterpret_cast<floatx4*>(&acc_s[tid / LPP][4 * (tid % LPP)]) = acc;
-  if (tid % LPP == 0) l_s[tid / LPP] = L;
+  T* out = reinterpret_cast<T*>(A.out) + bh * D;
+  if (length == 0) {
+    if (tid < D) out[tid] = (T)0.f;
+    return;
+  }
+  const long g0 = quotient(at + kUnit, all.share), g1 = quotient(at + length - 1, all.share);
+  if (g0 == g1) return;                // finished by its work-group
+  // a share has a record of the unit that it begins inside of and one of the unit that begins in it
+  const int parts = (int)(g1 - g0) + 1;
+  const float* base = A.part + 2 * g0 * A.rec;
+  auto record = [&](int p) { return base + (2L * p + (p == 0)) * A.rec; };
+  const int om = A.gc * D + gi, f = 4 * (tid % LPP);
+  floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+  float M = -INFINITY, L = 0.f;
+  for (int p0 = tid / LPP; p0 < parts; p0 += 4 * PPR) {
+    float mp[4], lp[4];
+    floatx4 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + i * PPR;
+      mp[i] = -INFINITY; lp[i] = 0.f; o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+      if (p < parts) {
+        const float* rec = record(p);
+        mp[i] = rec[om]; lp[i] = rec[om + A.gc];
+        o[i] = *reinterpret_cast<const floatx4*>(rec + gi * D + f);
+      }
+    }
+    const float mn = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])), M), by = M == -INFINITY ? 1.f : fast_exp2(M - mn);
+    M = mn;
+    L *= by;
+    acc *= by;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float w = mp[i] == -INFINITY ? 1.f : fast_exp2(mp[i] - mn);      // (without a maximum there is nothing, or a NaN)
+      L += w * lp[i];
+      acc += w * o[i];
+    }
+  }
+  *reinterpret_cast<floatx4*>(&acc_s[tid / LPP][f]) = acc;
+  if (tid % LPP == 0) { m_s[tid / LPP] = M; l_s[tid / LPP] = L; }
   __syncthreads();
   if (tid < D) {
-    float o = 0.f, l = 0.f;
+    float o = 0.f, l = 0.f, top = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < PPR; ++r) { o += acc_s[r][tid]; l += l_s[r]; }
-    reinterpret_cast<T*>(A.out)[bh * D + tid] = (T)(l == 0.f ? 0.f : o / l);
+    for (int r = 0; r < PPR; ++r) top = fmaxf(top, m_s[r]);
+#pragma unroll
+    for (int r = 0; r < PPR; ++r) {
+      const float w = m_s[r] == -INFINITY ? 1.f : fast_exp2(m_s[r] - top);
+      o += w * acc_s[r][tid];
+      l += w * l_s[r];
+    }
+    out[tid] = (T)(l == 0.f ? 0.f : o / l);
   }
 }
 
@@ -417,27 +637,52 @@ static int attend8_plan(const nsa_cache8_desc* d, Attend8Args& A, size_t& bytes)
   long places = d->sel_block > 0 ? ((long)d->num_sel + 1) * d->sel_block : d->capacity;
   if (d->sel_block == 0 && d->window > 0 && d->window + 15L < places) places = d->window + 15L;
   const long tiles = (places + kTile - 1) / kTile;
-  long per = (tiles * units + 511) / 512;
-  per = per < kWaves ? kWaves : (per + kWaves - 1) / kWaves * kWaves;
-  if (d->sel_block > 0 && per > 64) per = 64;    // (the lists of rows and scales in LDS)
-  if (tiles <= 5 * kWaves) per = 5 * kWaves;
-  A.tiles = (int)per;
-  A.nparts = (int)((tiles + per - 1) / per);
-  if (units * A.nparts >= 1L << 23 || (long)d->batch * d->kv_heads * d->group >= 1L << 24) return NSA_E_UNSUPPORTED;
-  bytes = A.nparts > 1 ? (size_t)units * A.nparts * A.rec * sizeof(float) : 0;
+  if ((long)d->batch * d->kv_heads * d->group >= 1L << 23) return NSA_E_UNSUPPORTED;
+  A.most = (int)tiles;
+  A.shared = tiles > kAlone;
+  const int resident = d->dtype == 2 ? (d->dim_head == 64 ? 4 : 2) : d->dim_head == 64 ? 4 : 2;
+  const long most = ((tiles + kUnit) * (units < 1L << 20 ? units : 1L << 20) + kShare - 1) / kShare;
+  A.groups = A.shared ? (int)(most < 256 * resident ? most : 256 * resident) : 0;
+  bytes = A.shared ? 2 * (size_t)A.groups * A.rec * sizeof(float) : 0;
   return 0;
 }
 
+template <class T, int D, int MODE, int W>
+static void attend8_mode(const Attend8Args& A, hipStream_t st) {
+  const int cols = A.gc < 16 ? A.gc : 16;
+  const size_t merge = (W * 32 + (size_t)W * cols * (D / 2 + 4)) * 4, lists = MODE == kPacked ? (size_t)kListed * kTile * 12 : 0;
+  Attend8Args B = A;
+  B.table = (int)((merge > lists ? merge : lists) + 15) / 16 * 16;
+  const size_t table = A.shared && A.sel_block == 0 && A.c.lengths && A.c.length_stride ? (size_t)(A.batch + 1) * 8 : 0;
+  const dim3 grid((unsigned)(A.shared ? A.groups : A.batch * A.units));
+  hipLaunchKernelGGL((cache8_attend_kernel<T, D, MODE, W>), grid, dim3(64 * W), (unsigned)(B.table + table), st, B);
+  if (!A.shared) return;
+  // few heads have many parts each; of many heads, most are finished, and a work-group finds out no more than that
+  const unsigned heads = (unsigned)(A.batch * A.c.hk * A.g);
+  if (heads <= 128) hipLaunchKernelGGL((cache8_merge_kernel<T, D, 512>), dim3(heads), dim3(512), (unsigned)table, st, B);
+  else hipLaunchKernelGGL((cache8_merge_kernel<T, D, 128>), dim3(heads), dim3(128), (unsigned)table, st, B);
+}
+
 template <class T, int D>
-static int attend8_launch(const Attend8Args& A, long units, hipStream_t st) {
-  const size_t merge = (kWaves * 32 + (size_t)kWaves * (A.gc < 16 ? A.gc : 16) * (D / 2 + 4)) * 4, lists = A.sel_block > 0 ? (size_t)A.tiles * kTile * 12 : 0;
-  const unsigned bytes = (unsigned)(merge > lists ? merge : lists);
-  const dim3 grid((unsigned)(units * A.nparts)), block(64 * kWaves);
-  if (A.sel_block > 0) hipLaunchKernelGGL((cache8_attend_kernel<T, D, true>), grid, block, bytes, st, A);
-  else hipLaunchKernelGGL((cache8_attend_kernel<T, D, false>), grid, block, bytes, st, A);
-  if (A.nparts > 1) hipLaunchKernelGGL((cache8_merge_kernel<T, D>), dim3((unsigned)(units / A.units * A.c.hk * A.g)), dim3(256), 0, st, A);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? 0 : (int)e;
+static int attend8_launch(const Attend8Args& A, hipStream_t st) {
+  // (the first tiles of a launch's sequences lie in LDS)
+  for (int b = 0; b < A.batch; b += kTable) {
+    Attend8Args B = A;
+    B.batch = A.batch - b < kTable ? A.batch - b : kTable;
+    B.q = reinterpret_cast<const T*>(A.q) + b * A.q0;
+    B.out = reinterpret_cast<T*>(A.out) + (long)b * A.c.hk * A.g * D;
+    B.c.keys += b * A.c.s0; B.c.values += b * A.c.s0; B.c.key_scales += b * A.c.z0; B.c.value_scales += b * A.c.z0;
+    if (A.c.lengths) B.c.lengths += (long)b * A.c.length_stride;
+    const long rows = (long)b * A.units * A.num_sel;
+    if (A.idx) B.idx = A.idx64 ? (const void*)(reinterpret_cast<const long*>(A.idx) + rows) : (const void*)(reinterpret_cast<const int*>(A.idx) + rows);
+    if (A.fmask) B.fmask += rows;
+    if (A.sel_block == 0) A.shared ? attend8_mode<T, D, kRange, 4>(B, st) : attend8_mode<T, D, kRange, 8>(B, st);
+    else if (A.sel_block % 16 == 0) A.shared ? attend8_mode<T, D, kBlocks, 4>(B, st) : attend8_mode<T, D, kBlocks, 8>(B, st);
+    else attend8_mode<T, D, kPacked, 8>(B, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  return 0;
 }
 
 }  // namespace nsa
@@ -462,11 +707,11 @@ extern "C" int nsa_cache8_attend(const nsa_cache8_desc* d, const void* q, const 
   if (ws_bytes < need) return NSA_E_WORKSPACE;
   A.c = cache8_args(d, keys, values, key_scales, value_scales, lengths);
   A.q = q; A.q0 = d->q_stride[0]; A.q1 = d->q_stride[1];
-  A.window = d->window; A.sel_block = d->sel_block; A.num_sel = d->num_sel; A.idx64 = d->idx_is_int64;
+  A.window = d->window; A.sel_block = d->sel_block; A.num_sel = d->num_sel; A.idx64 = d->idx_is_int64; A.per_block = d->sel_block / 16;
   A.idx = idx; A.fmask = fmask; A.scale = d->scale; A.part = (float*)ws; A.out = out;
-  const long units = (long)d->batch * A.units;
+  A.batch = d->batch;
   hipStream_t st = (hipStream_t)stream;
   if (d->dim_head == 64)
-    return d->dtype == 0 ? attend8_launch<__bf16, 64>(A, units, st) : d->dtype == 1 ? attend8_launch<_Float16, 64>(A, units, st) : attend8_launch<float, 64>(A, units, st);
-  return d->dtype == 0 ? attend8_launch<__bf16, 128>(A, units, st) : d->dtype == 1 ? attend8_launch<_Float16, 128>(A, units, st) : attend8_launch<float, 128>(A, units, st);
+    return d->dtype == 0 ? attend8_launch<__bf16, 64>(A, st) : d->dtype == 1 ? attend8_launch<_Float16, 64>(A, st) : attend8_launch<float, 64>(A, st);
+  return d->dtype == 0 ? attend8_launch<__bf16, 128>(A, st) : d->dtype == 1 ? attend8_launch<_Float16, 128>(A, st) : attend8_launch<float, 128>(A, st);
 }
