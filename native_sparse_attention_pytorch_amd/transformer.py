@@ -176,7 +176,7 @@ class Transformer(nn.Module):
                 kk = math.ceil((1 - filter_thres) * logits.shape[-1])
                 val, ind = logits.topk(kk, dim=-1)
                 logits = torch.full_like(logits, float('-inf')).scatter_(-1, ind, val)
-                noise = -torch.log(-torch.log(torch.rand_like(logits).clamp_min(1e-20)).clamp_min(1e-20))
+                noise = -torch.log((-torch.log(torch.rand_like(logits).clamp_min(1e-20))).clamp_min(1e-20))
                 tok = (logits / max(temperature, 1e-10) + noise).argmax(dim=-1, keepdim=True)
             out = torch.cat((out, tok), dim=-1)
         return out[..., prompt.shape[-1]:]
