@@ -594,6 +594,16 @@ int nsa_cache8_attend(const nsa_cache8_desc* d, const void* q, const void* keys,
                       const float* value_scales, const int32_t* lengths, const void* idx, const uint8_t* fmask, void* ws, size_t ws_bytes, void* out,
                       void* stream);
 
+/* nsa_decode_step_dyn over an 8-bit cache (its keys and values; the compressed caches are bf16 as there): the new token's key and value go into row state[0] as by
+ * nsa_cache8_append, before anything attends them.  `cache`: dtype 0, batch, kv_heads, dim_head and group as `capacity` has them; window, sel_block and the lengths
+ * are not read.  ws: 256-byte aligned. */
+int nsa_decode_step8_workspace_bytes(const nsa_decode_step_desc* capacity, const nsa_cache8_desc* cache, size_t* bytes);
+int nsa_decode_step8_dyn(const nsa_decode_step_desc* capacity, const nsa_cache8_desc* cache, int32_t* state, const void* q, const void* k, const void* v,
+                         const float* freqs, void* keys, void* values, float* key_scales, float* value_scales, const void* ck_cache, const void* cv_cache,
+                         const void* mem_k, const void* mem_v, void* k_run, void* v_run, int64_t krun_row_stride, int64_t vrun_row_stride, int32_t run_ring,
+                         const void* gate_logits, int64_t gate_row_stride, const void* gate_bias, void* ws, size_t ws_bytes, void* out, int32_t advance,
+                         void* stream);
+
 /* What is done to the logits x [rows, vocab] of `dtype` (rows row_stride elements apart) before a token is drawn (transformer.py:240-247 draws from plain
  * ones); out: fp32 [rows, vocab] contiguous.  With c = how often entry i is among the first history_lengths[r] (NULL: all) of the
  * `history` tokens of row r ([rows, history] contiguous, int32 or int64, those outside [0, vocab) are passed over):

@@ -194,6 +194,9 @@ def lib():
         L.nsa_cache8_workspace_bytes.argtypes = [vp, C.POINTER(sz)]
         L.nsa_cache8_attend.argtypes = [vp] * 9 + [vp, sz, vp, vp]
         L.nsa_adjust_logits.argtypes = [vp] * 12
+        L.nsa_decode_step8_workspace_bytes.argtypes = [ds, vp, C.POINTER(sz)]
+        L.nsa_decode_step8_dyn.argtypes = [ds, vp] + [vp] * 15 + [i64, i64, i32, vp, i64, vp, vp, sz, vp, i32, vp]
+        L.nsa_decode_step8_workspace_bytes.restype = L.nsa_decode_step8_dyn.restype = C.c_int
         for name in ("nsa_cache8_append", "nsa_cache8_workspace_bytes", "nsa_cache8_attend", "nsa_adjust_logits"):
             getattr(L, name).restype = C.c_int
         for name in ("nsa_loss_workspace_bytes", "nsa_loss_fwd", "nsa_loss_bwd", "nsa_newton_workspace_bytes", "nsa_newton_schulz"):

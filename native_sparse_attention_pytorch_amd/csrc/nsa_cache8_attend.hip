@@ -31,6 +31,9 @@ struct Attend8Args {
   int most;                            // tiles of a unit at most
   float* part;                         // shared: two records for each work-group, [gc][D] sums, [gc] maxima, [gc] weights, rec floats each
   int groups;                          // work-groups of the first launch
+  int parts, per, records;             // else: of a unit, tiles of each; records: leave one for each part
+  const int* compressed;               // keys cached so far, of which num_sel is not more than ... / per_compressed, where they are known to the device
+  int per_compressed, most_compressed;
   int rec, table;                      // table: where in LDS the sequences' first tiles are, in bytes
   void* out;
 };
@@ -71,12 +74,13 @@ __device__ __forceinline__ Keys8 keys_of(const Attend8Args& A, int len) {
 }
 __device__ __forceinline__ int tiles_of(const Attend8Args& A, int b) { return (keys_of(A, cache8_length(A.c, b)).places + kTile - 1) / kTile; }
 // the row of a place of a selection; without one ~ of the newest key's, which is attended: what is there may be read in its place
-__device__ __forceinline__ int selected_row(const Attend8Args& A, const Keys8& K, long unit, int place) {
+__device__ __forceinline__ int selected_row(const Attend8Args& A, const Keys8& K, long unit, int place, int filled) {
   const int none = ~max(K.len - 1, 0);
   if (place >= K.places) return none;
   const int slot = place / A.sel_block, own = (K.len - 1) / A.sel_block;
   long blk = own;
   if (slot < A.num_sel) {
+    if (slot >= filled) return none;
     const long e = unit * A.num_sel + slot;
     const uint8_t live = A.fmask[e];
     blk = A.idx64 ? reinterpret_cast<const long*>(A.idx)[e] : (long)reinterpret_cast<const int*>(A.idx)[e];
@@ -158,6 +162,11 @@ struct Shares {
   }
 };
 
+// slots of a selection that are filled
+__device__ __forceinline__ int filled_slots(const Attend8Args& A) {
+  return A.compressed == nullptr ? A.num_sel : min(A.num_sel, min(max(A.compressed[0], 0), A.most_compressed) / A.per_compressed);
+}
+
 // a value that is the same in all lanes, for the compiler too
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ long uniform(long x) { return (long)((unsigned long)(unsigned)uniform((int)(x >> 32)) << 32 | (unsigned)uniform((int)x)); }
@@ -191,31 +200,31 @@ __device__ __forceinline__ void first_tiles(const Attend8Args& A, long* first) {
 // all sequences have as many tiles
 __device__ __forceinline__ bool alike(const Attend8Args& A) { return A.sel_block > 0 || A.c.lengths == nullptr || A.c.length_stride == 0; }
 
-template <class T, int D, int MODE, int kWaves>
-__global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend8Args A) {
+// A work-group: SHARED, its share of all units' tiles; else the unit, or the part of one, that is its own.
+template <class T, int D, int MODE, int kWaves, bool SHARED>
+__device__ __forceinline__ void attend8_body(const Attend8Args& A, const int group_id, const int groups_all, char* lds) {
   constexpr int QP = Parts8<T>::Q, PP = Parts8<T>::P, KS = D / 32, DT = D / 16;
-  extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, q4 = lane >> 4;
   // (the length of a sequence without keys counts for a selection: no tile of it has any)
   long pos = 0, end = 0, each = 0;
   Shares all;
   const long* first = reinterpret_cast<const long*>(lds + A.table);
-  if (A.shared) {
+  if constexpr (SHARED) {
     if (alike(A)) {
       each = uniform(length_on_line(A.sel_block > 0 ? A.most : tiles_of(A, 0)));
-      all.set(each * A.batch * A.units, gridDim.x);
+      all.set(each * A.batch * A.units, groups_all);
     } else {
       first_tiles<64 * kWaves>(A, const_cast<long*>(first));
-      all.set(uniform(first[A.batch]) * A.units, gridDim.x);
+      all.set(uniform(first[A.batch]) * A.units, groups_all);
     }
-    pos = blockIdx.x * all.share;
+    pos = group_id * all.share;
     end = min(all.total, pos + all.share);
     if (pos >= end) return;
   }
   int seq = -1;
   do {
   int b, u, t0, t1, tiles;
-  if (A.shared) {
+  if constexpr (SHARED) {
     long at, length = each;            // of the unit that `pos` lies in: where it begins, how long it is
     if (each > 0) {
       const long unit = quotient(pos, each);
@@ -246,10 +255,12 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend
     pos = at + length;
     if (t0 >= t1) continue;            // (its tiles are all in the next share)
   } else {
-    b = blockIdx.x / A.units;
-    u = blockIdx.x - b * A.units;
-    t0 = 0;
-    t1 = tiles = A.most;
+    const int own = group_id / A.parts;
+    b = own / A.units;
+    u = own - b * A.units;
+    t0 = (group_id - own * A.parts) * A.per;
+    t1 = min(A.most, t0 + A.per);
+    tiles = A.records ? -1 : A.most;
   }
   const bool whole_unit = t0 == 0 && t1 == tiles;
   const long unit = (long)b * A.units + u;
@@ -294,6 +305,7 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend
 #pragma unroll
   for (int c = 0; c < DT; ++c) O[c] = floatx4{0.f, 0.f, 0.f, 0.f};
 
+  const int filled = MODE == kRange ? 0 : filled_slots(A);
   // tiles c0 .. c1 - 1 at a time: as many as there are lanes, or room in LDS, for where their rows are
   const int chunk = MODE == kBlocks ? 32 * nw : MODE == kPacked ? kListed : t1 - t0;
   int c0 = t0, lane_row = -1;
@@ -439,7 +451,7 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend
       // lane 2 r + i: keys 16 i .. 16 i + 15 of tile c0 + w0 + r nw
       const int at = 2 * (c0 + w0 + (lane >> 1) * nw) + (lane & 1), slot = at / A.per_block;
       long blk = -1;
-      if (slot < A.num_sel) {
+      if (slot < filled) {
         const long e = unit * A.num_sel + slot;
         const uint8_t live = A.fmask[e];
         blk = A.idx64 ? reinterpret_cast<const long*>(A.idx)[e] : (long)reinterpret_cast<const int*>(A.idx)[e];
@@ -452,7 +464,7 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend
     } else if constexpr (MODE == kPacked) {
       if (c0 > t0) __syncthreads();
       for (int i = tid; i < (c1 - c0) * kTile; i += 64 * kWaves) {
-        const int r = selected_row(A, K, unit, c0 * kTile + i), at = (r ^ (r >> 31)) >> A.block_shift;
+        const int r = selected_row(A, K, unit, c0 * kTile + i, filled), at = (r ^ (r >> 31)) >> A.block_shift;
         row_s[i] = r;
         ks_s[i] = kz[at];
         vs_s[i] = vz[at];
@@ -527,7 +539,7 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend
         *reinterpret_cast<vec*>(reinterpret_cast<T*>(A.out) + ((long)b * A.c.hk * A.g + head0 + g) * D + f) =
             L == 0.f ? vec{(T)0.f, (T)0.f, (T)0.f, (T)0.f} : vec{(T)(o[0] / L), (T)(o[1] / L), (T)(o[2] / L), (T)(o[3] / L)};
       } else {
-        float* rec = A.part + (2L * blockIdx.x + (t0 == 0)) * A.rec;
+        float* rec = A.part + (SHARED ? 2L * group_id + (t0 == 0) : group_id) * A.rec;
         *reinterpret_cast<floatx4*>(rec + g * D + f) = o;
         if (f == 0) {
           float Mg = -INFINITY;
@@ -541,6 +553,20 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_attend_kernel(const Attend
   }
   if (pos < end) __syncthreads();      // (LDS is used again)
   } while (pos < end);
+}
+
+template <class T, int D, int MODE, int W, bool SHARED>
+__global__ __launch_bounds__(64 * W) void cache8_attend_kernel(const Attend8Args A) {
+  extern __shared__ __align__(16) char lds[];
+  attend8_body<T, D, MODE, W, SHARED>(A, blockIdx.x, gridDim.x, lds);
+}
+
+// The sliding window and the selected blocks of a step in one launch: neither waits for the other.
+template <int D, int MODE>
+__global__ __launch_bounds__(512) void cache8_step_kernel(const Attend8Args S, const Attend8Args F, const int groups) {
+  extern __shared__ __align__(16) char lds[];
+  if ((int)blockIdx.x < groups) attend8_body<__bf16, D, kRange, 8, false>(S, blockIdx.x, groups, lds);
+  else attend8_body<__bf16, D, MODE, 8, false>(F, blockIdx.x - groups, gridDim.x - groups, lds);
 }
 
 // the parts of a head, weighted by their maxima
@@ -647,20 +673,26 @@ static int attend8_plan(const nsa_cache8_desc* d, Attend8Args& A, size_t& bytes)
   return 0;
 }
 
-template <class T, int D, int MODE, int W>
+// bytes of LDS besides the table of first tiles
+template <int D>
+static int attend8_lds(const Attend8Args& A, int waves, bool lists) {
+  const int cols = A.gc < 16 ? A.gc : 16, merge = (waves * 32 + waves * cols * (D / 2 + 4)) * 4, rows = lists ? kListed * kTile * 12 : 0;
+  return ((merge > rows ? merge : rows) + 15) / 16 * 16;
+}
+
+template <class T, int D, int MODE, int W, bool SHARED>
 static void attend8_mode(const Attend8Args& A, hipStream_t st) {
-  const int cols = A.gc < 16 ? A.gc : 16;
-  const size_t merge = (W * 32 + (size_t)W * cols * (D / 2 + 4)) * 4, lists = MODE == kPacked ? (size_t)kListed * kTile * 12 : 0;
   Attend8Args B = A;
-  B.table = (int)((merge > lists ? merge : lists) + 15) / 16 * 16;
-  const size_t table = A.shared && A.sel_block == 0 && A.c.lengths && A.c.length_stride ? (size_t)(A.batch + 1) * 8 : 0;
-  const dim3 grid((unsigned)(A.shared ? A.groups : A.batch * A.units));
-  hipLaunchKernelGGL((cache8_attend_kernel<T, D, MODE, W>), grid, dim3(64 * W), (unsigned)(B.table + table), st, B);
-  if (!A.shared) return;
+  B.table = attend8_lds<D>(A, W, MODE == kPacked);
+  B.parts = 1; B.per = A.most;
+  const int table = SHARED && A.sel_block == 0 && A.c.lengths && A.c.length_stride ? (A.batch + 1) * 8 : 0;
+  const dim3 grid((unsigned)(SHARED ? A.groups : A.batch * A.units));
+  hipLaunchKernelGGL((cache8_attend_kernel<T, D, MODE, W, SHARED>), grid, dim3(64 * W), B.table + table, st, B);
+  if (!SHARED) return;
   // few heads have many parts each; of many heads, most are finished, and a work-group finds out no more than that
   const unsigned heads = (unsigned)(A.batch * A.c.hk * A.g);
-  if (heads <= 128) hipLaunchKernelGGL((cache8_merge_kernel<T, D, 512>), dim3(heads), dim3(512), (unsigned)table, st, B);
-  else hipLaunchKernelGGL((cache8_merge_kernel<T, D, 128>), dim3(heads), dim3(128), (unsigned)table, st, B);
+  if (heads <= 128) hipLaunchKernelGGL((cache8_merge_kernel<T, D, 512>), dim3(heads), dim3(512), table, st, B);
+  else hipLaunchKernelGGL((cache8_merge_kernel<T, D, 128>), dim3(heads), dim3(128), table, st, B);
 }
 
 template <class T, int D>
@@ -676,13 +708,73 @@ static int attend8_launch(const Attend8Args& A, hipStream_t st) {
     const long rows = (long)b * A.units * A.num_sel;
     if (A.idx) B.idx = A.idx64 ? (const void*)(reinterpret_cast<const long*>(A.idx) + rows) : (const void*)(reinterpret_cast<const int*>(A.idx) + rows);
     if (A.fmask) B.fmask += rows;
-    if (A.sel_block == 0) A.shared ? attend8_mode<T, D, kRange, 4>(B, st) : attend8_mode<T, D, kRange, 8>(B, st);
-    else if (A.sel_block % 16 == 0) A.shared ? attend8_mode<T, D, kBlocks, 4>(B, st) : attend8_mode<T, D, kBlocks, 8>(B, st);
-    else attend8_mode<T, D, kPacked, 8>(B, st);
+    if (A.sel_block == 0) A.shared ? attend8_mode<T, D, kRange, 4, true>(B, st) : attend8_mode<T, D, kRange, 8, false>(B, st);
+    else if (A.sel_block % 16 == 0) A.shared ? attend8_mode<T, D, kBlocks, 4, true>(B, st) : attend8_mode<T, D, kBlocks, 8, false>(B, st);
+    else A.shared ? attend8_mode<T, D, kPacked, 8, true>(B, st) : attend8_mode<T, D, kPacked, 8, false>(B, st);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
   }
   return 0;
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// The window and the blocks of a step, as records: parts of eight tiles, one for each wave, while the chip has room for them.
+static void step8_branches(const Step8& s, Attend8Args& S, Attend8Args& F) {
+  const nsa_cache8_desc* d = s.d;
+  auto branch = [&](Attend8Args& A, bool per_head, long places) {
+    A.batch = d->batch; A.g = d->group;
+    A.units = per_head ? d->kv_heads * d->group : d->kv_heads;
+    A.gc = per_head ? 1 : d->group;
+    A.rec = A.gc * d->dim_head + ((2 * A.gc + 3) & ~3);
+    A.most = (int)((places + kTile - 1) / kTile);
+    const long units = (long)d->batch * A.units;
+    int per = 8;
+    while (per < A.most && (A.most + per - 1) / per * units > 512) per += 8;
+    while ((A.most + per - 1) / per > 128) per += 8;      // (records that the merge takes)
+    A.per = per; A.parts = (A.most + per - 1) / per; A.records = 1;
+    A.block_shift = __builtin_ctz(d->block);
+    A.scale = d->scale;
+  };
+  const long window = (long)s.window + 15 < d->capacity ? s.window + 15L : d->capacity;
+  branch(S, false, window);
+  S.window = s.window;
+  branch(F, s.per_head, ((long)s.num_sel + 1) * s.sel_block);
+  F.sel_block = s.sel_block; F.num_sel = s.num_sel; F.per_block = s.sel_block / 16;
+}
+
+void cache8_step_parts(const Step8& s, int parts[2], int rec[2]) {
+  Attend8Args S{}, F{};
+  step8_branches(s, S, F);
+  parts[0] = S.parts; parts[1] = F.parts; rec[0] = S.rec; rec[1] = F.rec;
+}
+
+template <int D>
+static void step8_launch(const Attend8Args& S, const Attend8Args& F, hipStream_t st) {
+  const int a = attend8_lds<D>(S, 8, false), b = attend8_lds<D>(F, 8, F.sel_block % 16 != 0);
+  const int groups = S.batch * S.units * S.parts, all = groups + F.batch * F.units * F.parts;
+  if (F.sel_block % 16 == 0) hipLaunchKernelGGL((cache8_step_kernel<D, kBlocks>), dim3((unsigned)all), dim3(512), a > b ? a : b, st, S, F, groups);
+  else hipLaunchKernelGGL((cache8_step_kernel<D, kPacked>), dim3((unsigned)all), dim3(512), a > b ? a : b, st, S, F, groups);
+}
+
+int cache8_step_attend(const Step8& s, const void* rq, const int32_t* idx, const uint8_t* fmask, float* window_records, float* block_records, void* stream) {
+  const nsa_cache8_desc* d = s.d;
+  Attend8Args S{}, F{};
+  step8_branches(s, S, F);
+  for (Attend8Args* A : {&S, &F}) {
+    A->c = cache8_args(d, s.keys, s.values, s.key_scales, s.value_scales, s.state);
+    A->c.length = 1;                   // the new token is in the cache
+    A->c.length_stride = 0;
+    A->c.cap = s.rows;
+    A->q = rq; A->q0 = (long)d->kv_heads * d->group * d->dim_head; A->q1 = d->dim_head;
+  }
+  S.part = window_records;
+  F.part = block_records;
+  F.idx = idx; F.fmask = fmask;
+  F.compressed = s.state + 1; F.per_compressed = s.per_block; F.most_compressed = s.compressed;
+  if (d->dim_head == 64) step8_launch<64>(S, F, (hipStream_t)stream);
+  else step8_launch<128>(S, F, (hipStream_t)stream);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : (int)e;
 }
 
 }  // namespace nsa

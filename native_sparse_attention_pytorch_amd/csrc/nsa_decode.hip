@@ -14,6 +14,7 @@
 // query heads as (zero-padded) columns: a lane then owns one head, the softmax statistics are
 // per-lane scalars and the rescaling of O^T = V^T P needs no cross-lane traffic.
 #include "nsa_common.hpp"
+#include "nsa_cache8.hpp"
 #include "../../include/nsa_hip.h"
 
 namespace nsa {
@@ -1087,4 +1088,112 @@ extern "C" int nsa_decode_step_dyn(const nsa_decode_step_desc* cap, int32_t* sta
   if (!state || ((k_run || v_run) && run_ring <= 0)) return NSA_E_ARG;
   return nsa::run_decode_step(cap, state, q, k, v, freqs, 0, k_cache, v_cache, ck_cache, cv_cache, mem_k, mem_v, k_run, v_run, krun_row_stride, vrun_row_stride,
                        run_ring, gate_logits, gate_row_stride, gate_bias, ws, ws_bytes, out, advance != 0, stream);
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// The step over an 8-bit cache: five launches - the new token's queries, key and value; the compressed branch, whose logits are left in memory; their
+// top-k; window and selected blocks; merge and gate.  (A block's scale may grow with its newest row, and with it what is held of the others: the
+// row goes into the cache before anything attends it, where a bf16 row goes in beside the window's attention.)
+namespace nsa {
+
+struct Step8Layout {
+  StepLayout L;
+  Step8 s;
+  DecodePlan Pf, Ps;                   // of the merge: parts and records
+  size_t off_rf, off_rs, off_logits, off_idx, off_vals, off_fm, total;
+};
+
+static int make_step8_layout(const nsa_decode_step_desc* d, const nsa_cache8_desc* cache, Step8Layout& X) {
+  if (int e = make_step_layout(d, X.L)) return e;
+  if (!cache8_check(cache) || cache->dtype != 0 || cache->batch != d->batch || cache->kv_heads != d->kv_heads || cache->dim_head != d->dim_head ||
+      (long)cache->group * cache->kv_heads != d->heads || d->pos >= cache->capacity)
+    return NSA_E_ARG;
+  const int g = cache->group;
+  if (!cache8_supported(cache) || g > 32 || cache->kv_stride[2] >= 1L << 31 || (long)d->batch * d->heads >= 1L << 16) return NSA_E_UNSUPPORTED;
+  const bool has_c = d->num_compressed > 0;
+  if (X.L.k > 0 && (X.L.nb > 64 * 32 || X.L.k > 64)) return NSA_E_UNSUPPORTED;
+  Step8& s = X.s;
+  s = Step8{};
+  s.d = cache; s.rows = d->pos + 1;
+  s.window = d->window < cache->capacity ? d->window + 1 : cache->capacity; s.sel_block = d->block; s.num_sel = X.L.k; s.per_block = d->per_block; s.compressed = d->num_compressed;
+  s.per_head = !d->share && g > 1;
+  int parts[2], rec[2];
+  cache8_step_parts(s, parts, rec);
+  const int units[2] = {d->kv_heads, s.per_head ? d->heads : d->kv_heads};
+  for (int i = 0; i < 2; ++i) {
+    DecodePlan& P = i ? X.Pf : X.Ps;
+    P = DecodePlan{};
+    P.b = d->batch; P.hk = d->kv_heads; P.g = g; P.d = d->dim_head;
+    P.units = units[i]; P.gc = i && s.per_head ? 1 : g;
+    P.nparts = parts[i]; P.rec = rec[i];
+  }
+  size_t o = 0;
+  o = up256(o + (size_t)d->batch * d->heads * d->dim_head * 2);          // the rotated queries, then the compressed branch's partials
+  X.L.off_rq = 0; X.L.off_wsc = o;
+  o = up256(o + X.L.wsc);
+  X.off_rf = o;     o = up256(o + (size_t)d->batch * units[1] * parts[1] * rec[1] * 4);
+  X.off_rs = o;     o = up256(o + (size_t)d->batch * units[0] * parts[0] * rec[0] * 4);
+  X.off_logits = o; o = up256(o + (size_t)d->batch * d->heads * (has_c ? d->num_compressed : 1) * 4);
+  const size_t sel = (size_t)d->batch * X.L.sel_units * (X.L.k > 0 ? X.L.k : 1);
+  X.off_idx = o;    o = up256(o + sel * 4);
+  X.off_vals = o;   o = up256(o + sel * 4);
+  X.off_fm = o;     o = up256(o + sel);
+  X.total = o;
+  return 0;
+}
+
+}  // namespace nsa
+
+extern "C" int nsa_decode_step8_workspace_bytes(const nsa_decode_step_desc* capacity, const nsa_cache8_desc* cache, size_t* bytes) {
+  nsa::Step8Layout X;
+  if (!bytes) return NSA_E_ARG;
+  if (int e = nsa::make_step8_layout(capacity, cache, X)) return e;
+  *bytes = X.total;
+  return 0;
+}
+
+extern "C" int nsa_decode_step8_dyn(const nsa_decode_step_desc* d, const nsa_cache8_desc* cache, int32_t* state, const void* q, const void* k, const void* v,
+                                    const float* freqs, void* keys, void* values, float* key_scales, float* value_scales, const void* ck_cache,
+                                    const void* cv_cache, const void* mem_k, const void* mem_v, void* k_run, void* v_run, int64_t krun_row, int64_t vrun_row,
+                                    int32_t ring, const void* gate_logits, int64_t gate_row, const void* gate_bias, void* ws, size_t ws_bytes, void* out,
+                                    int32_t advance, void* stream) {
+  using namespace nsa;
+  Step8Layout X;
+  if (int e = make_step8_layout(d, cache, X)) return e;
+  if (!state || !q || !k || !v || !freqs || !keys || !values || !key_scales || !value_scales || !gate_logits || !ws || !out || (uintptr_t)ws % 256) return NSA_E_ARG;
+  if (ws_bytes < X.total) return NSA_E_WORKSPACE;
+  const bool has_c = d->num_compressed > 0;
+  if (has_c && (!ck_cache || !cv_cache)) return NSA_E_ARG;
+  if (((uintptr_t)keys | (uintptr_t)values | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16) return NSA_E_ARG;
+  if ((d->q_stride[0] | d->q_stride[1] | d->k_stride[0] | d->k_stride[1] | d->v_stride[0] | d->v_stride[1]) & 7) return NSA_E_ARG;
+  if (!k_run != !v_run || (k_run && (ring <= 0 || ((krun_row | vrun_row) & 7) || ((d->krun_stride[0] | d->krun_stride[1] | d->vrun_stride[0] | d->vrun_stride[1]) & 7))))
+    return NSA_E_ARG;
+  char* w = (char*)ws;
+  void* rq = w;
+  X.s.keys = keys; X.s.values = values; X.s.key_scales = key_scales; X.s.value_scales = value_scales; X.s.state = state;
+  nsa_cache8_desc own = *cache;
+  own.scale = d->scale;
+  X.s.d = &own;
+  if (int e = cache8_step_prep(X.s, q, d->q_stride, k, d->k_stride, v, d->v_stride, freqs, rq, k_run, d->krun_stride, krun_row, v_run, d->vrun_stride, vrun_row,
+                               ring, stream))
+    return e;
+  DecodePlan Pc{};
+  int32_t* idx = (int32_t*)(w + X.off_idx);
+  uint8_t* fm = (uint8_t*)(w + X.off_fm);
+  if (has_c) {
+    if (int e = make_decode_plan(&X.L.c, Pc, true, X.L.tiles_s)) return e;
+    Pc.dyn = state; Pc.dyn_kind = 1; Pc.window = d->window; Pc.per_block = d->per_block; Pc.smax = X.L.k;
+    Pc.cap_len = d->pos + 1; Pc.cap_nc = d->num_compressed; Pc.lstride = d->num_compressed;
+    float* logits = (float*)(w + X.off_logits);
+    const AttendArgs C = attend_args(Pc, q, ck_cache, cv_cache, mem_k, mem_v, nullptr, nullptr, w + X.L.off_wsc, X.L.k > 0 ? logits : nullptr);
+    if (int e = launch_attend_role<kPlain>(C, X.L.wsc, stream)) return e;
+    if (X.L.k > 0)
+      if (int e = decode_topk_launch(logits, d->batch, d->kv_heads, d->heads / d->kv_heads, d->num_compressed, d->per_block, d->share, X.L.k, idx,
+                                     (float*)(w + X.off_vals), fm, state, stream))
+        return e;
+  }
+  if (int e = cache8_step_attend(X.s, rq, idx, fm, (float*)(w + X.off_rs), (float*)(w + X.off_rf), stream)) return e;
+  const DecodePlan* pp[3] = {&Pc, &X.Pf, &X.Ps};
+  const void* wsp[3] = {has_c ? w + X.L.off_wsc : nullptr, w + X.off_rf, w + X.off_rs};
+  return launch_combine(pp, wsp, gate_logits, gate_row, gate_bias, out, advance ? state : nullptr, stream);
 }

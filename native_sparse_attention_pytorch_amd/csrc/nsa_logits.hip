@@ -30,7 +30,7 @@ struct LogitsArgs {
   float* out;
 };
 
-constexpr int kLogitsThreads = 512, kSweeps = 2;         // kSweeps: of a slice, at most
+constexpr int kLogitsThreads = 512, kRun = 8, kSweeps = 2;         // kRun: entries of a thread at a time; kSweeps: of a slice, at most
 
 // n consecutive values of any alignment (that of the type at least)
 template <class T, int N>
@@ -39,7 +39,7 @@ struct __attribute__((packed, aligned(sizeof(T)))) Run { T v[N]; };
 template <class T, class I>
 __global__ __launch_bounds__(kLogitsThreads) void adjust_logits_kernel(const LogitsArgs A) {
   extern __shared__ __align__(16) int count_s[];
-  constexpr int V = 8;
+  constexpr int V = kRun;
   const int tid = threadIdx.x;
   const long r = blockIdx.x / A.slices;
   const int v0 = (int)(blockIdx.x - r * A.slices) * A.slice, v1 = min(A.vocab, v0 + A.slice);
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(kLogitsThreads) void adjust_logits_kernel(const Log
 #pragma unroll
   for (int k = 0; k < kSweeps; ++k) {
     const int i = v0 + (k * kLogitsThreads + tid) * V;
-    ok[k] = 0xff;
+    ok[k] = ~0u;
     if (i + V > v1) continue;
     a[k] = *reinterpret_cast<const Run<T, V>*>(x + i);
     if (A.allowed_kind == 1) {
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kLogitsThreads) void adjust_logits_kernel(const Log
       v = v - pres;
     }
     if (bias) v = v + b;
-    v = v / temp;
+    if (temp != 1.f) v = v / temp;
     return ok ? v : -INFINITY;
   };
 #pragma unroll
@@ -153,7 +153,7 @@ extern "C" int nsa_adjust_logits(const nsa_logits_desc* d, const void* x, const 
   if (!x || !out || (d->history > 0 && !history) || (d->allowed_kind != 0 && !allowed)) return NSA_E_ARG;
   if (d->rows > 1L << 30 || d->vocab > 1 << 30) return NSA_E_UNSUPPORTED;
   // A slice: work-groups enough for the chip several times over, whole sweeps of the threads, two of them where there are rows enough
-  const int sweep = kLogitsThreads * 8;
+  const int sweep = kLogitsThreads * kRun;
   long slice = ((long)d->rows * d->vocab / 1024 + sweep - 1) / sweep * sweep;
   slice = std::max<long>(sweep, std::min<long>(slice, kSweeps * sweep));
   const long slices = (d->vocab + slice - 1) / slice;

@@ -17,6 +17,9 @@ indexed from the device-side position), compresses it and appends the compressed
         y = session.step(x)
     cache = session.cache()                                  # back to the module's cache format
 
+With `cache_dtype=torch.float8_e4m3fn` the session holds keys and values in 8 bits (ops.Cache8: a power-of-two scale for each 32 tokens of a kv head),
+half of a bf16 cache's memory: the new token's row is rounded before anything attends it, the compressed keys and values stay bf16.
+
 The reference has no counterpart; results equal `forward_inference` up to the order in which split
 partial results are merged (the split is sized for the capacity rather than the current length).
 """
@@ -27,7 +30,8 @@ import ctypes as C
 import torch
 
 from . import _lib
-from .ops import _kernel_dim, _pad_dim, rms_norm_supported, skinny_linear, skinny_linear_supported
+from .ops import (_CACHE8_DESC, _kernel_dim, _pad_dim, cache8_append, make_cache8, rms_norm_supported, skinny_linear,
+                  skinny_linear_supported)
 
 _BF16 = torch.bfloat16
 
@@ -40,7 +44,9 @@ def ring_rows(first, count_range: torch.Tensor, ring: int) -> torch.Tensor:
 
 
 class DecodeSession:
-    def __init__(self, module, cache, max_len: int, capture: bool = True):
+    def __init__(self, module, cache, max_len: int, capture: bool = True, cache_dtype: torch.dtype | None = None):
+        if cache_dtype not in (None, _BF16, torch.float8_e4m3fn):
+            raise ValueError(f"DecodeSession: cache_dtype {cache_dtype}, expected bfloat16 or float8_e4m3fn")
         m = self.module = module
         assert m.causal, 'inference only relevant for autoregressive'
         (cache_k, cache_v), ((cache_ck, cache_cv), (run_k, run_v)) = cache
@@ -69,7 +75,14 @@ class DecodeSession:
             buf = torch.zeros((b, hk, rows, d), dtype=_BF16, device=dev)
             buf[:, :, :src.shape[-2], :src.shape[-1]].copy_(src)      # the module's own decode steps hand back padded rows
             return buf
-        self.K, self.V = grown(cache_k, self.max_len), grown(cache_v, self.max_len)
+        self.cache8 = None
+        if cache_dtype == torch.float8_e4m3fn:
+            self.cache8 = make_cache8(b, hk, self.max_len, d0, device=dev)
+            with torch.no_grad():
+                cache8_append(self.cache8, cache_k[..., :d0], cache_v[..., :d0])
+            self.K, self.V = self.cache8[:2]
+        else:
+            self.K, self.V = grown(cache_k, self.max_len), grown(cache_v, self.max_len)
         # one spare row: the capture warm-up and the recording of the window-completing graph write row `nc` of the compressed
         # caches whatever nc is, also when the prefill already filled all max_nc rows (the real steps never do: completes_window)
         self.CK, self.CV = grown(cache_ck, self.max_nc + 1), grown(cache_cv, self.max_nc + 1)
@@ -188,8 +201,14 @@ class DecodeSession:
         for name in ("q_stride", "k_stride", "v_stride"):
             getattr(dsc, name)[:] = (width, self.d)
         nbytes = C.c_size_t()
-        _lib.check(_lib.lib().nsa_decode_step_workspace_bytes(C.byref(dsc), C.byref(nbytes), None, None, None),
-                   "nsa_decode_step_workspace_bytes")
+        if self.cache8 is None:
+            _lib.check(_lib.lib().nsa_decode_step_workspace_bytes(C.byref(dsc), C.byref(nbytes), None, None, None),
+                       "nsa_decode_step_workspace_bytes")
+        else:
+            keys, _, scales, _ = self.cache8
+            self._desc8 = _CACHE8_DESC.pack(self.b, self.hk, self.hq // self.hk, self.d, self.cache8.block, keys.shape[2], 0, 0, 0, 0, 0, 0, 0, 0, dsc.scale, 0,
+                                            *keys.stride()[:3], *scales.stride()[:2], 0, 0)
+            _lib.check(_lib.lib().nsa_decode_step8_workspace_bytes(C.byref(dsc), self._desc8, C.byref(nbytes)), "nsa_decode_step8_workspace_bytes")
         return dsc, torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
 
     def layer_step(self, x_in: torch.Tensor, advance: int):
@@ -204,8 +223,7 @@ class DecodeSession:
             qkvg = torch.nn.functional.linear(x, self.w_cat)         # 'b 1 ((hq + 2 hk) d + 3 hq)', contiguous
         merged = torch.empty((self.b, 1, hq * d), dtype=_BF16, device=qkvg.device)
         gl = qkvg if self.fused_gate else m.to_strategy_combine[0](x).to(_BF16).contiguous()
-        _lib.check(_lib.lib().nsa_decode_step_dyn(*self._step_args(qkvg, gl, merged, advance),
-                                                  torch.cuda.current_stream(qkvg.device).cuda_stream), "nsa_decode_step_dyn")
+        _lib.check(self._step_fn()(*self._step_args(qkvg, gl, merged, advance), torch.cuda.current_stream(qkvg.device).cuda_stream), "decode step")
         w_out = self.w_out if self.w_out is not None else m.combine_heads.weight
         if self.own_out:
             return skinny_linear(merged, w_out, m.combine_heads.bias)
@@ -215,13 +233,17 @@ class DecodeSession:
         eps = self.module.norm.eps
         return torch.finfo(torch.float32).eps if eps is None else eps      # as the library's kernel takes it for a bf16 input
 
+    def _step_fn(self):
+        return _lib.lib().nsa_decode_step_dyn if self.cache8 is None else _lib.lib().nsa_decode_step8_dyn
+
     def _step_args(self, qkvg, gl, merged, advance):
-        """Arguments of nsa_decode_step_dyn up to the stream; `gl`: the gate logits' tensor (qkvg itself: its last columns)."""
+        """Arguments of `_step_fn` up to the stream; `gl`: the gate logits' tensor (qkvg itself: its last columns)."""
         hq, hk, d = self.hq, self.hk, self.d
         p = qkvg.data_ptr()
         gate_ptr, gate_row = (p + 2 * (hq + 2 * hk) * d, qkvg.shape[-1]) if gl is qkvg else (gl.data_ptr(), 0)
-        return (C.byref(self._desc), self.state.data_ptr(), p, p + 2 * hq * d, p + 2 * (hq + hk) * d, self.freqs.data_ptr(),
-                self.K.data_ptr(), self.V.data_ptr(), self.CK.data_ptr(), self.CV.data_ptr(), self.mem_k.data_ptr(), self.mem_v.data_ptr(),
+        caches = (self.K, self.V) if self.cache8 is None else self.cache8
+        return (C.byref(self._desc), *(() if self.cache8 is None else (self._desc8,)), self.state.data_ptr(), p, p + 2 * hq * d, p + 2 * (hq + hk) * d,
+                self.freqs.data_ptr(), *(t.data_ptr() for t in caches), self.CK.data_ptr(), self.CV.data_ptr(), self.mem_k.data_ptr(), self.mem_v.data_ptr(),
                 self.ring_k.data_ptr(), self.ring_v.data_ptr(), self.ring_k.stride(2), self.ring_v.stride(2), self.ring,
                 gate_ptr, gate_row, self.gate_bias.data_ptr() if self.gate_bias is not None else None,
                 self._ws.data_ptr(), self._ws.numel(), merged.data_ptr(), int(advance))
@@ -236,7 +258,7 @@ class DecodeSession:
         qkvg = torch.empty((self.b, 1, self.w_cat.shape[0]), dtype=_BF16, device=merged.device)
         rstd = torch.empty((self.b,), dtype=torch.float32, device=merged.device)
         self._direct_bufs = (qkvg, merged, rstd)
-        fn = _lib.lib().nsa_decode_step_dyn
+        fn = self._step_fn()
         self._direct_args = tuple(a if not isinstance(a, (int, type(None))) else t(a) for a, t in zip(self._step_args(qkvg, qkvg, merged, 1), fn.argtypes))
 
     def _step_direct(self, x: torch.Tensor) -> torch.Tensor:
@@ -253,7 +275,7 @@ class DecodeSession:
         else:
             rc = L.nsa_rmsnorm_fwd(b, dim, x.data_ptr(), dim, norm_weight.data_ptr(), eps, self.x_buf.data_ptr(), rstd.data_ptr(), st)
             torch.mm(self.x_buf.view(b, dim), self.w_cat.t(), out=qkvg.view(b, -1))
-        rc = rc or L.nsa_decode_step_dyn(*self._direct_args, st)
+        rc = rc or self._step_fn()(*self._direct_args, st)
         if self.own_out:
             y = torch.empty_like(x)
             rc = rc or L.nsa_skinny_linear(b, merged.shape[-1], dim, merged.data_ptr(), merged.shape[-1], None, 0.0, w_out.data_ptr(),
@@ -313,7 +335,8 @@ class DecodeSession:
         return self.outs[event].clone()
 
     def cache(self):
-        """The caches in the module's format `((k, v), ((ck, cv), (run_k, run_v)))` (copies of the filled parts)."""
+        """The caches in the module's format `((k, v), ((ck, cv), (run_k, run_v)))` (copies of the filled parts; of an
+        8-bit cache what its codes stand for, which bf16 holds exactly)."""
         t, st, cbs = self.pos, self.st, self.cbs
         first = (t // st) * st - (cbs - st)                          # first position of the open window
         rows = ring_rows(first, torch.arange(t - first, device=self.K.device), self.ring)
@@ -322,20 +345,21 @@ class DecodeSession:
         if first < 0:                                                # positions before the sequence start read as zero
             run_k[:, :, :-first] = 0
             run_v[:, :, :-first] = 0
-        return ((self.K[:, :, :t].clone(), self.V[:, :, :t].clone()),
+        keys, vals = (self.K[:, :, :t].clone(), self.V[:, :, :t].clone()) if self.cache8 is None else self.cache8.rows(0, t)
+        return ((keys, vals),
                 ((self.CK[:, :, :self.nc, :d0].clone(), self.CV[:, :, :self.nc, :d0].clone()), (run_k, run_v)))
 
 
 class TransformerDecodeSession:
     """Token-by-token decoding of a `Transformer` (transformer.py:213-252 with use_cache_kv) as one graph replay per
     token: embedding, every layer's attention step and feed-forward, final norm and logits.  `caches` is what
-    `model(prompt, return_cache=True)` returned; `max_len` the longest sequence to decode to."""
+    `model(prompt, return_cache=True)` returned; `max_len` the longest sequence to decode to; `cache_dtype` as in `DecodeSession`."""
 
-    def __init__(self, model, caches, max_len: int):
+    def __init__(self, model, caches, max_len: int, cache_dtype: torch.dtype | None = None):
         self.model = model
         dev = caches[0][0][0].device
         b = caches[0][0][0].shape[0]
-        self.layers = [DecodeSession(attn, cache, max_len, capture=False) for (attn, _), cache in zip(model.layers, caches)]
+        self.layers = [DecodeSession(attn, cache, max_len, capture=False, cache_dtype=cache_dtype) for (attn, _), cache in zip(model.layers, caches)]
         self.tok = torch.zeros((b, 1), dtype=torch.long, device=dev)
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))

@@ -152,12 +152,21 @@ class Transformer(nn.Module):
 
 
     @torch.no_grad()
-    def sample(self, prompt, seq_len, temperature=1., filter_thres=0.9, use_cache_kv=False, use_graph=False):
+    def sample(self, prompt, seq_len, temperature=1., filter_thres=0.9, use_cache_kv=False, use_graph=False, cache_dtype=None, repetition_penalty=1.,
+               frequency_penalty=0., presence_penalty=0., logit_bias=None, allowed=None):
         """Extend `prompt` to seq_len tokens and return the new ones (transformer.py:213-252).
         temperature <= 0 is greedy; otherwise gumbel sampling over the top (1 - filter_thres)
         share of the vocabulary.  With use_cache_kv every step after the first is a decode step;
         use_graph (with use_cache_kv, bf16 models) replays those steps from a captured HIP graph
-        (decode_session.TransformerDecodeSession) instead of launching them one by one."""
+        (decode_session.TransformerDecodeSession) instead of launching them one by one, with the keys and
+        values held in 8 bits where cache_dtype is torch.float8_e4m3fn.  The penalties for tokens that the
+        sequence holds (the prompt's among them), logit_bias and allowed change the logits before a token is
+        drawn as ops.adjust_logits does; allowed may be a function of the tokens so far 'b n' that returns one."""
+        if cache_dtype is not None and not (use_cache_kv and use_graph):
+            raise ValueError("sample: cache_dtype is that of a session's caches: use_cache_kv and use_graph")
+        from . import ops
+        adjusted = logit_bias is not None or allowed is not None or any(
+            isinstance(p, torch.Tensor) or p != neutral for p, neutral in ((repetition_penalty, 1.), (frequency_penalty, 0.), (presence_penalty, 0.)))
         out, cache, session = prompt.clone(), None, None
         for _ in range(max(0, seq_len - prompt.shape[-1])):
             if session is not None:
@@ -168,8 +177,12 @@ class Transformer(nn.Module):
                     cache = next_cache
                     if use_graph:
                         from .decode_session import TransformerDecodeSession
-                        session = TransformerDecodeSession(self, cache, max_len=seq_len)
-            logits = logits[:, -1].float()
+                        session = TransformerDecodeSession(self, cache, max_len=seq_len, cache_dtype=cache_dtype)
+            logits = logits[:, -1]
+            if adjusted:
+                logits = ops.adjust_logits(logits, out, repetition_penalty=repetition_penalty, frequency_penalty=frequency_penalty,
+                                           presence_penalty=presence_penalty, bias=logit_bias, allowed=allowed(out) if callable(allowed) else allowed)
+            logits = logits.float()
             if temperature <= 0.:
                 tok = logits.argmax(dim=-1, keepdim=True)
             else:
