@@ -106,12 +106,89 @@ struct Step8 {
   int window, sel_block, num_sel, per_block, compressed;      // per_block: compressed keys of a selected block; compressed: that the caches may hold
   bool per_head;
 };
-// the new token: its queries rotated to rq, its key and value into the cache, both unrotated into the ring
-int cache8_step_prep(const Step8& s, const void* q, const int64_t* q_stride, const void* k, const int64_t* k_stride, const void* v, const int64_t* v_stride,
+// The new token: its queries rotated to rq, its key and value into the cache, both unrotated into the ring.
+struct StepPrepArgs {
+  Cache8Args c;
+  int rows, g, ring;
+  const __bf16 *q, *k, *v;
+  long q0, q1, k0, k1, v0, v1;
+  const float* freqs;
+  __bf16 *rq, *krun, *vrun;
+  long ku0, ku1, ku_row, vu0, vu1, vu_row;
+};
+
+// A work-group of two waves for each sequence and kv head, `unit`: the group's queries by both, then the key by one and the value by the other.  A lane
+// has a pair of features.
+template <int D>
+__device__ __forceinline__ void step8_prep(const StepPrepArgs& A, const int unit) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = unit / A.c.hk, h = unit - b * A.c.hk, pos = A.c.lengths[0];
+  if (lane >= D / 2) return;
+  float sn, cs;
+  sincosf((float)pos * A.freqs[lane], &sn, &cs);
+  // (rounded to bf16 as the rotation by itself does)
+  auto rotated = [&](bf16x2 x) {
+    const float a = (float)x[0], c = (float)x[1];
+    return bf16x2{(__bf16)(a * cs - c * sn), (__bf16)(c * cs + a * sn)};
+  };
+  for (int i = wave; i < A.g; i += 2) {
+    const int head = h * A.g + i;
+    const bf16x2 y = *reinterpret_cast<const bf16x2*>(A.q + b * A.q0 + head * A.q1 + 2 * lane);
+    *reinterpret_cast<bf16x2*>(A.rq + ((long)b * A.c.hk * A.g + head) * D + 2 * lane) = rotated(y);
+  }
+  if (pos < 0 || pos >= A.rows) return;
+  const bool is_v = wave == 1;
+  bf16x2 x = *reinterpret_cast<const bf16x2*>((is_v ? A.v + b * A.v0 + h * A.v1 : A.k + b * A.k0 + h * A.k1) + 2 * lane);
+  __bf16* run = is_v ? A.vrun : A.krun;
+  if (run != nullptr) {
+    const long at = pos % A.ring;
+    *reinterpret_cast<bf16x2*>(run + (is_v ? b * A.vu0 + h * A.vu1 + at * A.vu_row : b * A.ku0 + h * A.ku1 + at * A.ku_row) + 2 * lane) = x;
+  }
+  if (!is_v) x = rotated(x);
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float m = fabsf((float)x[e]);
+    top = fmaxf(top, m < INFINITY ? m : 0.f);
+  }
+  // (of the lanes that have features: half a wave with 64)
+#pragma unroll
+  for (int o = 1; o < D / 2; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  const int held = pos % A.c.block;
+  uint8_t* codes = (is_v ? A.c.values : A.c.keys) + b * A.c.s0 + h * A.c.s1 + (long)(pos - held) * A.c.s2;
+  float* scale = (is_v ? A.c.value_scales : A.c.key_scales) + b * A.c.z0 + h * A.c.z1 + pos / A.c.block;
+  const float s_old = held > 0 ? *scale : 0.f, s_new = fmaxf(power_of_two(scale_exponent(bits_of(top))), s_old), inv = 1.0f / s_new;
+  if (held > 0 && s_new != s_old) {
+    for (int i = lane; i < held * (D / 8); i += D / 2) {
+      uintx2* at = reinterpret_cast<uintx2*>(codes + (i / (D / 8)) * A.c.s2 + i % (D / 8) * 8);
+      *at = codes_of(values_of(*at), s_old * inv);
+    }
+  }
+  if (lane == 0) *scale = s_new;
+  const uintx2 both = codes_of(floatx8{(float)x[0], (float)x[1], 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, inv);
+  *reinterpret_cast<uint16_t*>(codes + held * A.c.s2 + 2 * lane) = (uint16_t)both[0];
+}
+
+inline StepPrepArgs step8_prep_args(const Step8& s, const void* q, const int64_t* q_stride, const void* k, const int64_t* k_stride, const void* v, const int64_t* v_stride,
                      const float* freqs, void* rq, void* krun, const int64_t* krun_stride, int64_t krun_row, void* vrun, const int64_t* vrun_stride,
-                     int64_t vrun_row, int ring, void* stream);
+                     int64_t vrun_row, int ring) {
+  const nsa_cache8_desc* d = s.d;
+  StepPrepArgs A{};
+  A.c = cache8_args(d, s.keys, s.values, s.key_scales, s.value_scales, s.state);
+  A.rows = s.rows; A.g = d->group; A.ring = ring;
+  A.q = (const __bf16*)q; A.k = (const __bf16*)k; A.v = (const __bf16*)v;
+  A.q0 = q_stride[0]; A.q1 = q_stride[1]; A.k0 = k_stride[0]; A.k1 = k_stride[1]; A.v0 = v_stride[0]; A.v1 = v_stride[1];
+  A.freqs = freqs; A.rq = (__bf16*)rq; A.krun = (__bf16*)krun; A.vrun = (__bf16*)vrun;
+  if (krun) {
+    A.ku0 = krun_stride[0]; A.ku1 = krun_stride[1]; A.ku_row = krun_row; A.vu0 = vrun_stride[0]; A.vu1 = vrun_stride[1]; A.vu_row = vrun_row;
+  }
+  return A;
+}
+int cache8_step_prep(const Step8& s, const StepPrepArgs& A, void* stream);
 // Parts and floats of a record of each unit, {sliding window, selected blocks}: records [gc][D] sums, [gc] maxima, [gc] weights, as nsa_decode_combine takes them.
 void cache8_step_parts(const Step8& s, int parts[2], int rec[2]);
-int cache8_step_attend(const Step8& s, const void* rq, const int32_t* idx, const uint8_t* fmask, float* window_records, float* block_records, void* stream);
+// The blocks are idx where fmask is set, or the ones that the work-groups choose themselves from `pooled` [batch, rows of the selection, pooled_stride].
+int cache8_step_attend(const Step8& s, const void* rq, const int32_t* idx, const uint8_t* fmask, const float* pooled, long pooled_stride,
+                       float* window_records, float* block_records, void* stream);
 
 }  // namespace nsa

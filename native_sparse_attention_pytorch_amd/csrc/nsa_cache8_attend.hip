@@ -13,6 +13,7 @@
 // parts (one of bf16, two of fp16, three of fp32: exact), probabilities of two (three for fp32 results): 2^-17 (2^-24) of each.  At 16 columns
 // the matrix cores have the time for it.
 #include "nsa_cache8.hpp"
+#include "nsa_decode_topk.hpp"
 
 namespace nsa {
 
@@ -34,6 +35,8 @@ struct Attend8Args {
   int parts, per, records;             // else: of a unit, tiles of each; records: leave one for each part
   const int* compressed;               // keys cached so far, of which num_sel is not more than ... / per_compressed, where they are known to the device
   int per_compressed, most_compressed;
+  const float* pooled;                 // logits of the blocks, from which the work-group makes its unit's selection itself
+  long pooled_stride;
   int rec, table;                      // table: where in LDS the sequences' first tiles are, in bytes
   void* out;
 };
@@ -74,17 +77,22 @@ __device__ __forceinline__ Keys8 keys_of(const Attend8Args& A, int len) {
 }
 __device__ __forceinline__ int tiles_of(const Attend8Args& A, int b) { return (keys_of(A, cache8_length(A.c, b)).places + kTile - 1) / kTile; }
 // the row of a place of a selection; without one ~ of the newest key's, which is attended: what is there may be read in its place
-__device__ __forceinline__ int selected_row(const Attend8Args& A, const Keys8& K, long unit, int place, int filled) {
+__device__ __forceinline__ int selected_row(const Attend8Args& A, const Keys8& K, long unit, int place, int filled, const int* sel) {
   const int none = ~max(K.len - 1, 0);
   if (place >= K.places) return none;
   const int slot = place / A.sel_block, own = (K.len - 1) / A.sel_block;
   long blk = own;
   if (slot < A.num_sel) {
     if (slot >= filled) return none;
-    const long e = unit * A.num_sel + slot;
-    const uint8_t live = A.fmask[e];
-    blk = A.idx64 ? reinterpret_cast<const long*>(A.idx)[e] : (long)reinterpret_cast<const int*>(A.idx)[e];
-    if (live == 0 || blk < 0 || blk > own) return none;
+    if (sel != nullptr) {
+      blk = sel[slot];
+    } else {
+      const long e = unit * A.num_sel + slot;
+      const uint8_t live = A.fmask[e];
+      blk = A.idx64 ? reinterpret_cast<const long*>(A.idx)[e] : (long)reinterpret_cast<const int*>(A.idx)[e];
+      blk = live != 0 ? blk : -1;
+    }
+    if (blk < 0 || blk > own) return none;
   }
   const long row = blk * A.sel_block + (place - slot * A.sel_block);
   return row < K.len ? (int)row : none;
@@ -200,9 +208,10 @@ __device__ __forceinline__ void first_tiles(const Attend8Args& A, long* first) {
 // all sequences have as many tiles
 __device__ __forceinline__ bool alike(const Attend8Args& A) { return A.sel_block > 0 || A.c.lengths == nullptr || A.c.length_stride == 0; }
 
-// A work-group: SHARED, its share of all units' tiles; else the unit, or the part of one, that is its own.
-template <class T, int D, int MODE, int kWaves, bool SHARED>
-__device__ __forceinline__ void attend8_body(const Attend8Args& A, const int group_id, const int groups_all, char* lds) {
+// A work-group: SHARED, its share of all units' tiles; else the unit, or the part of one, that is its own.  CHOOSE: it selects the blocks itself, into sel_s (64
+// of them, and 128 words besides).
+template <class T, int D, int MODE, int kWaves, bool SHARED, bool CHOOSE = false>
+__device__ __forceinline__ void attend8_body(const Attend8Args& A, const int group_id, const int groups_all, char* lds, int* sel_s = nullptr) {
   constexpr int QP = Parts8<T>::Q, PP = Parts8<T>::P, KS = D / 32, DT = D / 16;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, q4 = lane >> 4;
   // (the length of a sequence without keys counts for a selection: no tile of it has any)
@@ -306,6 +315,13 @@ __device__ __forceinline__ void attend8_body(const Attend8Args& A, const int gro
   for (int c = 0; c < DT; ++c) O[c] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   const int filled = MODE == kRange ? 0 : filled_slots(A);
+  if constexpr (CHOOSE) {
+    if (filled > 0) {                  // (at most 64)
+      const int blocks = min(max(A.compressed[0], 0), A.most_compressed) / A.per_compressed;
+      if (wave == 0) wave_topk(A.pooled + unit * A.pooled_stride, blocks, filled, lane, reinterpret_cast<float*>(sel_s + 64), sel_s + 128, sel_s, nullptr, nullptr);
+      __syncthreads();
+    }
+  }
   // tiles c0 .. c1 - 1 at a time: as many as there are lanes, or room in LDS, for where their rows are
   const int chunk = MODE == kBlocks ? 32 * nw : MODE == kPacked ? kListed : t1 - t0;
   int c0 = t0, lane_row = -1;
@@ -452,10 +468,14 @@ __device__ __forceinline__ void attend8_body(const Attend8Args& A, const int gro
       const int at = 2 * (c0 + w0 + (lane >> 1) * nw) + (lane & 1), slot = at / A.per_block;
       long blk = -1;
       if (slot < filled) {
-        const long e = unit * A.num_sel + slot;
-        const uint8_t live = A.fmask[e];
-        blk = A.idx64 ? reinterpret_cast<const long*>(A.idx)[e] : (long)reinterpret_cast<const int*>(A.idx)[e];
-        blk = live != 0 && blk >= 0 && blk < 1L << 30 ? blk : -1;
+        if constexpr (CHOOSE) {
+          blk = sel_s[slot];
+        } else {
+          const long e = unit * A.num_sel + slot;
+          const uint8_t live = A.fmask[e];
+          blk = A.idx64 ? reinterpret_cast<const long*>(A.idx)[e] : (long)reinterpret_cast<const int*>(A.idx)[e];
+          blk = live != 0 && blk >= 0 && blk < 1L << 30 ? blk : -1;
+        }
       } else if (slot == A.num_sel && last >= 0) {
         blk = last / A.sel_block;      // the newest key's
       }
@@ -464,7 +484,7 @@ __device__ __forceinline__ void attend8_body(const Attend8Args& A, const int gro
     } else if constexpr (MODE == kPacked) {
       if (c0 > t0) __syncthreads();
       for (int i = tid; i < (c1 - c0) * kTile; i += 64 * kWaves) {
-        const int r = selected_row(A, K, unit, c0 * kTile + i, filled), at = (r ^ (r >> 31)) >> A.block_shift;
+        const int r = selected_row(A, K, unit, c0 * kTile + i, filled, CHOOSE ? sel_s : nullptr), at = (r ^ (r >> 31)) >> A.block_shift;
         row_s[i] = r;
         ks_s[i] = kz[at];
         vs_s[i] = vz[at];
@@ -562,11 +582,14 @@ __global__ __launch_bounds__(64 * W) void cache8_attend_kernel(const Attend8Args
 }
 
 // The sliding window and the selected blocks of a step in one launch: neither waits for the other.
-template <int D, int MODE>
+template <int D, int MODE, bool CHOOSE>
 __global__ __launch_bounds__(512) void cache8_step_kernel(const Attend8Args S, const Attend8Args F, const int groups) {
   extern __shared__ __align__(16) char lds[];
-  if ((int)blockIdx.x < groups) attend8_body<__bf16, D, kRange, 8, false>(S, blockIdx.x, groups, lds);
-  else attend8_body<__bf16, D, MODE, 8, false>(F, blockIdx.x - groups, gridDim.x - groups, lds);
+  __shared__ int sel_s[192];
+  // (the blocks' work-groups first: choosing comes before their attention)
+  const int later = gridDim.x - groups;
+  if ((int)blockIdx.x < later) attend8_body<__bf16, D, MODE, 8, false, CHOOSE>(F, blockIdx.x, later, lds, sel_s);
+  else attend8_body<__bf16, D, kRange, 8, false>(S, blockIdx.x - later, groups, lds);
 }
 
 // the parts of a head, weighted by their maxima
@@ -752,11 +775,17 @@ template <int D>
 static void step8_launch(const Attend8Args& S, const Attend8Args& F, hipStream_t st) {
   const int a = attend8_lds<D>(S, 8, false), b = attend8_lds<D>(F, 8, F.sel_block % 16 != 0);
   const int groups = S.batch * S.units * S.parts, all = groups + F.batch * F.units * F.parts;
-  if (F.sel_block % 16 == 0) hipLaunchKernelGGL((cache8_step_kernel<D, kBlocks>), dim3((unsigned)all), dim3(512), a > b ? a : b, st, S, F, groups);
-  else hipLaunchKernelGGL((cache8_step_kernel<D, kPacked>), dim3((unsigned)all), dim3(512), a > b ? a : b, st, S, F, groups);
+  const unsigned bytes = a > b ? a : b;
+  const dim3 grid((unsigned)all), block(512);
+  const bool blocks = F.sel_block % 16 == 0;
+  if (blocks && F.pooled) hipLaunchKernelGGL((cache8_step_kernel<D, kBlocks, true>), grid, block, bytes, st, S, F, groups);
+  else if (blocks) hipLaunchKernelGGL((cache8_step_kernel<D, kBlocks, false>), grid, block, bytes, st, S, F, groups);
+  else if (F.pooled) hipLaunchKernelGGL((cache8_step_kernel<D, kPacked, true>), grid, block, bytes, st, S, F, groups);
+  else hipLaunchKernelGGL((cache8_step_kernel<D, kPacked, false>), grid, block, bytes, st, S, F, groups);
 }
 
-int cache8_step_attend(const Step8& s, const void* rq, const int32_t* idx, const uint8_t* fmask, float* window_records, float* block_records, void* stream) {
+int cache8_step_attend(const Step8& s, const void* rq, const int32_t* idx, const uint8_t* fmask, const float* pooled, long pooled_stride,
+                       float* window_records, float* block_records, void* stream) {
   const nsa_cache8_desc* d = s.d;
   Attend8Args S{}, F{};
   step8_branches(s, S, F);
@@ -769,7 +798,7 @@ int cache8_step_attend(const Step8& s, const void* rq, const int32_t* idx, const
   }
   S.part = window_records;
   F.part = block_records;
-  F.idx = idx; F.fmask = fmask;
+  F.idx = idx; F.fmask = fmask; F.pooled = pooled; F.pooled_stride = pooled_stride;
   F.compressed = s.state + 1; F.per_compressed = s.per_block; F.most_compressed = s.compressed;
   if (d->dim_head == 64) step8_launch<64>(S, F, (hipStream_t)stream);
   else step8_launch<128>(S, F, (hipStream_t)stream);

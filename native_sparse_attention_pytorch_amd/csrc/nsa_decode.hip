@@ -15,6 +15,7 @@
 // per-lane scalars and the rescaling of O^T = V^T P needs no cross-lane traffic.
 #include "nsa_common.hpp"
 #include "nsa_cache8.hpp"
+#include "nsa_decode_topk.hpp"
 #include "../../include/nsa_hip.h"
 
 namespace nsa {
@@ -156,120 +157,6 @@ struct AttendArgs {
   NewToken nt;
   TopkIn topk;
 };
-
-__device__ __forceinline__ float wave_reduce_max(float v) {
-#pragma unroll
-  for (int o = 1; o <= 32; o <<= 1) v = fmaxf(v, o == 1 ? dpp_quad_xor1(v) : o == 2 ? dpp_quad_xor2(v) : __shfl_xor(v, o, 64));
-  return v;
-}
-__device__ __forceinline__ float wave_reduce_sum(float v) {
-#pragma unroll
-  for (int o = 1; o <= 32; o <<= 1) v += o == 1 ? dpp_quad_xor1(v) : o == 2 ? dpp_quad_xor2(v) : __shfl_xor(v, o, 64);
-  return v;
-}
-
-// Block selection of one row by one wave (NSA.py:693-713, 721: softmax with the extra -1e3 column, the k largest in descending
-// order, equal ones lower index first; a slot is live when its probability exceeds 1e-10).  nb <= 2048, k <= min(64, nb).
-// Lane l holds entries l, l + 64, ...  The k-th largest of the 64 lanes' maxima (a bitwise search with ballots: 31 steps) is a
-// lower bound of the k-th largest entry that only a few entries beyond the k reach; those are listed in LDS, a lane takes
-// one and counts the listed ones that come before it: its slot.  (Extracting maxima one by one, k dependent rounds of a wave
-// maximum and a re-scan: 16 us for 8 rows of 512 with k = 16.)  sel[slot] = block, or -1 for a dead slot.
-__device__ __forceinline__ void wave_topk(const float* __restrict__ row, int nb, int k, int lane, float* __restrict__ cand_p, int* __restrict__ cand_j,
-                                          int* __restrict__ sel, int* __restrict__ idx_out, unsigned char* __restrict__ fm_out) {
-  const int vpl = (nb + 63) >> 6;
-  float x[32];
-  float mx = -1e3f;
-#pragma unroll
-  for (int c = 0; c < 32; c += 8) {
-    if (c >= vpl) continue;                               // wave-uniform
-#pragma unroll
-    for (int r = c; r < c + 8; ++r) x[r] = r * 64 + lane < nb ? row[r * 64 + lane] : -INFINITY;
-  }
-#pragma unroll
-  for (int c = 0; c < 32; c += 8) {
-    if (c >= vpl) continue;
-#pragma unroll
-    for (int r = c; r < c + 8; ++r) mx = fmaxf(mx, x[r]);
-  }
-  mx = wave_reduce_max(mx);
-  float sum = 0.f;
-#pragma unroll
-  for (int c = 0; c < 32; c += 8) {
-    if (c >= vpl) continue;
-#pragma unroll
-    for (int r = c; r < c + 8; ++r) { x[r] = __expf(x[r] - mx); sum += x[r]; }
-  }
-  sum = wave_reduce_sum(sum) + __expf(-1e3f - mx);
-  const float inv = 1.0f / sum;
-  int top = 0;                                             // probabilities as integers: same order, padding negative
-#pragma unroll
-  for (int c = 0; c < 32; c += 8) {
-    if (c >= vpl) continue;
-#pragma unroll
-    for (int r = c; r < c + 8; ++r) {
-      float p = x[r] * inv;
-      p = (p == p) ? p : INFINITY;                         // NaN (a diverged row): ordered first, like torch.topk
-      p = r * 64 + lane < nb ? p : -1.0f;
-      x[r] = p;
-      top = max(top, __builtin_bit_cast(int, p));
-    }
-  }
-  int T = 0;
-  for (int bit = 30; bit >= 0; --bit) {
-    const int c = T | (1 << bit);
-    if ((int)__popcll(__ballot(top >= c)) >= k) T = c;
-  }
-  auto count = [&](int v) {                                // entries >= v
-    int n = 0;
-#pragma unroll
-    for (int c = 0; c < 32; c += 8) {
-      if (c >= vpl) continue;
-#pragma unroll
-      for (int r = c; r < c + 8; ++r) n += (int)__popcll(__ballot(__builtin_bit_cast(int, x[r]) >= v));
-    }
-    return n;
-  };
-  int ties = 64;                                           // entries equal to T that are listed
-  if (count(T) > 64) {                                     // (many equal entries, or the k largest in few lanes: the exact k-th largest)
-    T = 0;
-    for (int bit = 30; bit >= 0; --bit) {
-      const int c = T | (1 << bit);
-      if (count(c) >= k) T = c;
-    }
-    ties = k - count(T + 1);
-  }
-  int listed = 0;
-  const unsigned long long below = (1ull << lane) - 1;
-#pragma unroll
-  for (int c = 0; c < 32; c += 8) {
-    if (c >= vpl) continue;
-#pragma unroll
-    for (int r = c; r < c + 8; ++r) {
-      const int v = __builtin_bit_cast(int, x[r]);
-      const unsigned long long eq = __ballot(v == T);
-      const bool keep = v > T || (v == T && (int)__popcll(eq & below) < ties);
-      const unsigned long long kept = __ballot(keep);
-      const int at = listed + (int)__popcll(kept & below);
-      if (keep && at < 64) { cand_p[at] = x[r]; cand_j[at] = r * 64 + lane; }
-      listed += (int)__popcll(kept);
-      ties -= (int)__popcll(eq);
-    }
-  }
-  __builtin_amdgcn_wave_barrier();                         // LDS operations of one wave execute in order
-  listed = min(listed, 64);
-  const float p = lane < listed ? cand_p[lane] : -1.0f;
-  const int j = lane < listed ? cand_j[lane] : 0;
-  int rank = 0;
-  for (int i = 0; i < listed; ++i) {
-    const float pi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), i));
-    rank += (pi > p) | ((pi == p) & (i < lane));           // the list is in index order
-  }
-  if (lane < listed && rank < k) {
-    const bool live = p < INFINITY && p > 1e-10f;
-    sel[rank] = live ? j : -1;
-    if (idx_out != nullptr) { idx_out[rank] = j; fm_out[rank] = live ? 1 : 0; }
-  }
-}
 
 // Pooled importance logits of one 32-key tile (NSA.py:448-476: mean over a block's npf keys and, if shared, the group's heads):
 // key 8 (i / 4) + 4 h + i % 4 of the tile is register i, head n_ the lane.
@@ -1091,10 +978,29 @@ extern "C" int nsa_decode_step_dyn(const nsa_decode_step_desc* cap, int32_t* sta
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// The step over an 8-bit cache: five launches - the new token's queries, key and value; the compressed branch, whose logits are left in memory; their
-// top-k; window and selected blocks; merge and gate.  (A block's scale may grow with its newest row, and with it what is held of the others: the
-// row goes into the cache before anything attends it, where a bf16 row goes in beside the window's attention.)
+// The step over an 8-bit cache: three launches - the compressed branch, and beside it the new token's queries, key and value; window and selected blocks, whose
+// work-groups make the selection; merge and gate.  (A block's scale may grow with its newest row, and with it what is held of the others: the row goes into the
+// cache before anything attends it, where a bf16 row goes in beside the window's attention.  Blocks of other than 1, 2, 4 .. 32 compressed keys: as in
+// the bf16 step a launch more, for their top-k.)
 namespace nsa {
+
+template <int D, int ROLE>
+__global__ __launch_bounds__(64 * kDecodeWaves) __attribute__((amdgpu_waves_per_eu(2))) void decode_attend_prep_kernel(const AttendArgs A, const StepPrepArgs P) {
+  static_assert(kDecodeWaves == 2, "step8_prep has work for two waves");
+  __shared__ DecodeShared<D> sh;
+  if ((int)blockIdx.x < A.P.nsplit) decode_attend_body<D, ROLE>(A, blockIdx.x, sh);
+  else step8_prep<D>(P, blockIdx.y);
+}
+
+template <int ROLE>
+static int launch_attend_prep(const AttendArgs& A, size_t ws_bytes, const StepPrepArgs& P, void* stream) {
+  if (int e = check_attend(A.P, A.q, A.k, A.v, A.mem_k, A.mem_v, A.idx, A.fmask, A.part, ws_bytes)) return e;
+  const dim3 grid(A.P.nsplit + 1, A.P.b * A.P.units), block(64 * kDecodeWaves);      // (units: the kv heads)
+  if (A.P.d == 64) hipLaunchKernelGGL((decode_attend_prep_kernel<64, ROLE>), grid, block, 0, (hipStream_t)stream, A, P);
+  else hipLaunchKernelGGL((decode_attend_prep_kernel<128, ROLE>), grid, block, 0, (hipStream_t)stream, A, P);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : (int)e;
+}
 
 struct Step8Layout {
   StepLayout L;
@@ -1133,7 +1039,7 @@ static int make_step8_layout(const nsa_decode_step_desc* d, const nsa_cache8_des
   o = up256(o + X.L.wsc);
   X.off_rf = o;     o = up256(o + (size_t)d->batch * units[1] * parts[1] * rec[1] * 4);
   X.off_rs = o;     o = up256(o + (size_t)d->batch * units[0] * parts[0] * rec[0] * 4);
-  X.off_logits = o; o = up256(o + (size_t)d->batch * d->heads * (has_c ? d->num_compressed : 1) * 4);
+  X.off_logits = o; o = up256(o + (size_t)d->batch * d->heads * (has_c ? d->num_compressed : 1) * 4);      // (pooled ones are fewer)
   const size_t sel = (size_t)d->batch * X.L.sel_units * (X.L.k > 0 ? X.L.k : 1);
   X.off_idx = o;    o = up256(o + sel * 4);
   X.off_vals = o;   o = up256(o + sel * 4);
@@ -1174,25 +1080,29 @@ extern "C" int nsa_decode_step8_dyn(const nsa_decode_step_desc* d, const nsa_cac
   nsa_cache8_desc own = *cache;
   own.scale = d->scale;
   X.s.d = &own;
-  if (int e = cache8_step_prep(X.s, q, d->q_stride, k, d->k_stride, v, d->v_stride, freqs, rq, k_run, d->krun_stride, krun_row, v_run, d->vrun_stride, vrun_row,
-                               ring, stream))
-    return e;
+  const StepPrepArgs prep = step8_prep_args(X.s, q, d->q_stride, k, d->k_stride, v, d->v_stride, freqs, rq, k_run, d->krun_stride, krun_row, v_run, d->vrun_stride,
+                                            vrun_row, ring);
   DecodePlan Pc{};
   int32_t* idx = (int32_t*)(w + X.off_idx);
   uint8_t* fm = (uint8_t*)(w + X.off_fm);
-  if (has_c) {
+  float* logits = (float*)(w + X.off_logits);
+  const long nb = X.L.nb > 0 ? X.L.nb : 1;
+  const bool choose = has_c && X.L.k > 0 && X.L.pooled;
+  if (!has_c) {
+    if (int e = cache8_step_prep(X.s, prep, stream)) return e;
+  } else {
     if (int e = make_decode_plan(&X.L.c, Pc, true, X.L.tiles_s)) return e;
     Pc.dyn = state; Pc.dyn_kind = 1; Pc.window = d->window; Pc.per_block = d->per_block; Pc.smax = X.L.k;
     Pc.cap_len = d->pos + 1; Pc.cap_nc = d->num_compressed; Pc.lstride = d->num_compressed;
-    float* logits = (float*)(w + X.off_logits);
-    const AttendArgs C = attend_args(Pc, q, ck_cache, cv_cache, mem_k, mem_v, nullptr, nullptr, w + X.L.off_wsc, X.L.k > 0 ? logits : nullptr);
-    if (int e = launch_attend_role<kPlain>(C, X.L.wsc, stream)) return e;
-    if (X.L.k > 0)
+    AttendArgs C = attend_args(Pc, q, ck_cache, cv_cache, mem_k, mem_v, nullptr, nullptr, w + X.L.off_wsc, X.L.k > 0 && !choose ? logits : nullptr);
+    C.pool = PoolOut{logits, nb, d->per_block, d->share ? 1 : 0};
+    if (int e = choose ? launch_attend_prep<kPooled>(C, X.L.wsc, prep, stream) : launch_attend_prep<kPlain>(C, X.L.wsc, prep, stream)) return e;
+    if (X.L.k > 0 && !choose)
       if (int e = decode_topk_launch(logits, d->batch, d->kv_heads, d->heads / d->kv_heads, d->num_compressed, d->per_block, d->share, X.L.k, idx,
                                      (float*)(w + X.off_vals), fm, state, stream))
         return e;
   }
-  if (int e = cache8_step_attend(X.s, rq, idx, fm, (float*)(w + X.off_rs), (float*)(w + X.off_rf), stream)) return e;
+  if (int e = cache8_step_attend(X.s, rq, idx, fm, choose ? logits : nullptr, nb, (float*)(w + X.off_rs), (float*)(w + X.off_rf), stream)) return e;
   const DecodePlan* pp[3] = {&Pc, &X.Pf, &X.Ps};
   const void* wsp[3] = {has_c ? w + X.L.off_wsc : nullptr, w + X.off_rf, w + X.off_rs};
   return launch_combine(pp, wsp, gate_logits, gate_row, gate_bias, out, advance ? state : nullptr, stream);
