@@ -44,7 +44,9 @@ struct Attend8Args {
 typedef __attribute__((__vector_size__(2 * sizeof(float)))) float floatx2;
 
 constexpr int kTile = 32, kTable = 2048, kListed = 64;      // kTable: sequences of a launch; kListed: tiles whose rows are in LDS
-constexpr int kUnit = 8, kShare = 16, kAlone = 40;            // see Shares; kAlone: tiles of a unit up to which it has a work-group of eight waves for itself
+// see Shares.  kAlone: tiles of a unit up to which it has a work-group for itself and no merge follows (34 tiles of 8 units 13 us, shared 19); kAloneMany: where
+// there are units for all CUs (79 tiles of 256 units 37 us, shared 47; of lengths from 10 to 2500, 512 units 29 and 28)
+constexpr int kUnit = 8, kShare = 16, kAlone = 40, kAloneMany = 96;
 
 __device__ __forceinline__ floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -688,7 +690,7 @@ static int attend8_plan(const nsa_cache8_desc* d, Attend8Args& A, size_t& bytes)
   const long tiles = (places + kTile - 1) / kTile;
   if ((long)d->batch * d->kv_heads * d->group >= 1L << 23) return NSA_E_UNSUPPORTED;
   A.most = (int)tiles;
-  A.shared = tiles > kAlone;
+  A.shared = tiles > (units >= 256 ? kAloneMany : kAlone);
   const int resident = d->dtype == 2 ? (d->dim_head == 64 ? 4 : 2) : d->dim_head == 64 ? 4 : 2;
   const long most = ((tiles + kUnit) * (units < 1L << 20 ? units : 1L << 20) + kShare - 1) / kShare;
   A.groups = A.shared ? (int)(most < 256 * resident ? most : 256 * resident) : 0;
@@ -731,9 +733,22 @@ static int attend8_launch(const Attend8Args& A, hipStream_t st) {
     const long rows = (long)b * A.units * A.num_sel;
     if (A.idx) B.idx = A.idx64 ? (const void*)(reinterpret_cast<const long*>(A.idx) + rows) : (const void*)(reinterpret_cast<const int*>(A.idx) + rows);
     if (A.fmask) B.fmask += rows;
-    if (A.sel_block == 0) A.shared ? attend8_mode<T, D, kRange, 4, true>(B, st) : attend8_mode<T, D, kRange, 8, false>(B, st);
-    else if (A.sel_block % 16 == 0) A.shared ? attend8_mode<T, D, kBlocks, 4, true>(B, st) : attend8_mode<T, D, kBlocks, 8, false>(B, st);
-    else A.shared ? attend8_mode<T, D, kPacked, 8, true>(B, st) : attend8_mode<T, D, kPacked, 8, false>(B, st);
+    // Work-groups of two waves where a unit has not tiles enough for eight, or the chip not room: it holds one of eight on a CU with 128 features, two with 64.
+    // us with eight / two: 3 tiles of 800 units 18.6 / 8.7, 10 of 320 14.9 / 12.8, 10 of 640 21.4 / 13.7, 32 of 640 44 / 41; 43 of 296 17 / 28, 79 of 256 37 / 63.
+    const int units = B.batch * A.units, slots = D == 64 ? 512 : 256;
+    const bool few = A.most <= 4 || (units > slots && A.most <= 12) || units > 2 * slots;
+    if (A.sel_block == 0) {
+      if (A.shared) attend8_mode<T, D, kRange, 4, true>(B, st);
+      else if (few) attend8_mode<T, D, kRange, 2, false>(B, st);
+      else attend8_mode<T, D, kRange, 8, false>(B, st);
+    } else if (A.sel_block % 16 == 0) {
+      if (A.shared) attend8_mode<T, D, kBlocks, 4, true>(B, st);
+      else if (few) attend8_mode<T, D, kBlocks, 2, false>(B, st);
+      else attend8_mode<T, D, kBlocks, 8, false>(B, st);
+    } else {
+      if (A.shared) attend8_mode<T, D, kPacked, 8, true>(B, st);
+      else attend8_mode<T, D, kPacked, 8, false>(B, st);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
   }
