@@ -573,9 +573,9 @@ int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_t* cols, co
  * `window` of its keys (0: all), or with sel_block > 0 the blocks idx of sel_block keys (of each kv head, or of each head where per_head_sel:
  * [batch, kv_heads or heads, num_sel] contiguous, int32 or int64) whose fmask byte is not 0, as far as the sequence has them, and the keys of the block
  * that its newest key is in.  A block named twice counts twice.  No key: zeros.  out: [batch, heads, dim_head] contiguous, of `dtype`.  group <= 32;
- * num_sel <= 2^20, (num_sel + 1) * sel_block and kv_stride below 2^30, q 16-byte aligned with strides of multiples of 8.
+ * num_sel <= 2^20, (num_sel + 1) * sel_block below 2^30, the row stride below 2^31, batch * heads below 2^23, q 16-byte aligned with strides of multiples of 8.
  * Sums in fp32, q and the probabilities as sums of bf16 parts (q exactly; probabilities to 16 bits, of fp32 queries to 24), results rounded once.
- * Only rows that are attended are read, in tiles of 16 that may begin before the first and end behind the last of them, in the cache. */
+ * Only rows that are attended are read.  ws: aligned to 16 bytes, and not needed where its size is 0. */
 typedef struct nsa_cache8_desc {
   int32_t batch, kv_heads, group, dim_head;
   int32_t block, capacity;
@@ -611,7 +611,8 @@ int nsa_decode_step8_dyn(const nsa_decode_step_desc* capacity, const nsa_cache8_
  *   x <- (x + bias[i]) / temperature[r];  entries that are not allowed: -inf.
  * repetition, frequency, presence, temperature: fp32 values of the rows at stride 0 or 1, NULL: the descriptor's for all rows.  bias: fp32, rows bias_stride apart (0: one for all).  allowed: bytes
  * [.., vocab] (allowed_kind 1) or int32 words of 32 entries each, lowest bit first (allowed_kind 2), rows allowed_stride elements apart (0: one
- * for all); kind 0: none.  Every step is rounded to fp32 by itself.  rows and vocab up to 2^30, 4 rows vocab / 1024 below 2^31. */
+ * for all); kind 0: none.  Every step is rounded to fp32 by itself.  rows and vocab up to 2^30, rows times
+ * vocab / 4096 (rounded up) below 2^23. */
 typedef struct nsa_logits_desc {
   int64_t rows, row_stride;
   int32_t vocab, dtype;

@@ -2925,6 +2925,12 @@ def _counts_ok(t, batch: int) -> bool:
     return dtype in (torch.int32, torch.int64) and len(shape) <= 1 and shape.numel() in (1, batch)
 
 
+def _overlaps(shape, stride) -> bool:
+    """Whether two places of a tensor may be one in memory."""
+    axes = sorted((at, n) for n, at in zip(shape, stride) if n > 1)
+    return any(at < step for (at, _), step in zip(axes, [1, *(at * n for at, n in axes)]))
+
+
 def _int32(t: Tensor) -> Tensor:
     return t if t.dtype == torch.int32 else t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
 
@@ -2941,6 +2947,8 @@ def _append_plan(cache, k, v, starts, counts):
     block = _cache8_plan(name, *cache)
     shape, stride, sstride = cache[0], cache[1], cache[7]
     batch, hk, capacity, d = shape
+    if _overlaps(shape, stride) or _overlaps(cache[6], sstride):
+        raise RuntimeError(f"{name}: cache strides {stride}, {sstride}: sequences or heads share memory (expanded?)")
     if k[2] not in _LOSS_TYPES or v[2] != k[2]:
         raise RuntimeError(f"{name}: k {k[2]}, v {v[2]}: expected both bf16, both fp16 or both fp32")
     if len(k[0]) != 4 or v[0] != k[0] or k[0][:2] != (batch, hk) or not 0 < k[0][3] <= d or _kernel_dim(k[0][3]) != d:

@@ -95,6 +95,19 @@ def test_rows(library, what):
     assert not library.calls
 
 
+@pytest.mark.parametrize("shared", [GOOD._replace(keys=codes(1, 2, 64, 64).expand(2, 2, 64, 64), values=codes(1, 2, 64, 64).expand(2, 2, 64, 64)),
+                                    GOOD._replace(key_scales=torch.ones(2, 1, 4).expand(2, 2, 4), value_scales=torch.ones(2, 1, 4).expand(2, 2, 4))])
+def test_a_cache_whose_sequences_share_memory_is_read_only(library, shared):
+    from native_sparse_attention_pytorch_amd import ops
+    ops.cache8_attend(Q, shared, 5)
+    assert len(library.calls) == 1
+    with pytest.raises(RuntimeError, match="share memory"):
+        ops.cache8_append(shared, K, K)
+    rows_first = GOOD._replace(keys=codes(2, 64, 2, 64).transpose(1, 2), values=codes(2, 64, 2, 64).transpose(1, 2))
+    ops.cache8_append(rows_first, K, K)
+    assert len(library.calls) == 2
+
+
 BAD_QUERIES = {
     "doubles": dict(q=Q.double()), "two tokens": dict(q=torch.randn(2, 6, 2, 64)), "three axes": dict(q=Q[:, :, 0]), "other sequences": dict(q=Q[:1]),
     "uneven heads": dict(q=Q[:, :5]), "too many heads": dict(q=torch.randn(2, 66, 1, 64)), "no heads": dict(q=Q[:, :0]), "too wide": dict(q=torch.randn(2, 6, 1, 100)),
