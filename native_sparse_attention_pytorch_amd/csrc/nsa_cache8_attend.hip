@@ -152,18 +152,22 @@ struct Tile8 {                         // what a lane holds of 32 keys
   float ks[2], vs[2];                  // ks: of key n.  vs: one for all 16 keys (kPacked reads them from LDS where it needs them)
 };
 
-// Shared tiles.  A sequence's tiles are as many as its length has, known to the device only.  All units lie one after the other on a line, each as long as its
-// tiles and kUnit more (what a unit costs besides them), and the line is cut into equal shares, one for each work-group, whatever the lengths are.  A unit whose
-// tiles lie in one share is finished there; of the others each share leaves a record, and the merge finds them by the same arithmetic.  (Parts of a fixed
-// size for each unit, sized for the capacity: 48 sequences of 1 to 16384 keys took 105 us where these take __; most work-groups had nothing to do,
-// and a few too much.)
-// n / d of n below 2^50: by the division of doubles, put right where that is rounded up (one of 64-bit integers takes 150 instructions)
+// a value that is the same in all lanes, for the compiler too
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long uniform(long x) { return (long)((unsigned long)(unsigned)uniform((int)(x >> 32)) << 32 | (unsigned)uniform((int)x)); }
+
+// n / d of n below 2^50, the same in all lanes: by the division of doubles, put right where that is rounded up (one of 64-bit integers takes 150 instructions)
 __device__ __forceinline__ long quotient(long n, long d) {
   long q = (long)((double)n / (double)d);
   q -= q * d > n;
-  return q + (n - q * d >= d);
+  return uniform(q + (n - q * d >= d));
 }
 
+// Shared tiles.  A sequence's tiles are as many as its length has, known to the device only.  All units lie one after the other on a line, each as long as its
+// tiles and kUnit more (what a unit costs besides them), and the line is cut into equal shares, one for each work-group, whatever the lengths are.  A unit whose
+// tiles lie in one share is finished there; of the others each share leaves a record, and the merge finds them by the same arithmetic.  (Parts of a fixed
+// size for each unit, sized for the capacity: 48 sequences of 1 to 16384 keys took 105 us where these take 50; most work-groups had nothing to do,
+// and a few too much.)
 struct Shares {
   long total, share;                   // the line's length, a work-group's part of it
   __device__ __forceinline__ void set(long all, int groups) {
@@ -176,10 +180,6 @@ struct Shares {
 __device__ __forceinline__ int filled_slots(const Attend8Args& A) {
   return A.compressed == nullptr ? A.num_sel : min(A.num_sel, min(max(A.compressed[0], 0), A.most_compressed) / A.per_compressed);
 }
-
-// a value that is the same in all lanes, for the compiler too
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ long uniform(long x) { return (long)((unsigned long)(unsigned)uniform((int)(x >> 32)) << 32 | (unsigned)uniform((int)x)); }
 
 __device__ __forceinline__ long length_on_line(long tiles) { return tiles > 0 ? tiles + kUnit : 0; }
 
