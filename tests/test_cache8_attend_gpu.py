@@ -203,3 +203,26 @@ def test_calls_on_streams_in_graphs_and_again():
         for c, got in zip(calls, outs):
             assert torch.equal(got, c())
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("what", ["all", "window", "blocks", "packed blocks"])
+def test_more_sequences_than_a_launch_takes(what):
+    """2050 sequences over one cache (expanded, as a prompt that all share): a launch takes 2048."""
+    from native_sparse_attention_pytorch_amd import ops
+    b, n, at = 2050, 3264, [0, 1, 1024, 2046, 2047, 2048, 2049]
+    _, cache = made(1, 1, 1, n, 64, 64, "bf16")
+    gen = torch.Generator().manual_seed(5)
+    q = torch.randn(b, 2, 1, 64, generator=gen).bfloat16()
+    lengths = torch.randint(0, n + 1, (b,), generator=gen, dtype=torch.int32)
+    lengths[2048] = n
+    many = ops.Cache8(*(t.to(DEV).expand(b, *t.shape[1:]) for t in cache))
+    few = tuple(t.expand(len(at), *t.shape[1:]) for t in cache)
+    args = {"all": {}, "window": {"window": 40}, "blocks": {"size": 32}, "packed blocks": {"size": 24}}[what]
+    if "size" in args:
+        args["idx"] = torch.randint(0, n // args["size"], (b, 1, 1, 4), generator=gen)
+        args["fmask"] = torch.rand(b, 1, 1, 4, generator=gen) < 0.8
+        got = ops.cache8_select_attend(q.to(DEV), many, lengths.to(DEV), args["size"], args["idx"].to(DEV), args["fmask"].to(DEV))
+        args["idx"], args["fmask"] = args["idx"][at], args["fmask"][at]
+    else:
+        got = ops.cache8_attend(q.to(DEV), many, lengths.to(DEV), **args)
+    close(got[at], *R.attend(q[at], few, lengths[at].tolist(), **args), keys=n)
