@@ -2863,7 +2863,8 @@ _CACHE8_DESC, _LOGITS_DESC = struct.Struct("@14ifi7q"), struct.Struct("@2q2iq2i2
 
 class Cache8(NamedTuple):
     """Keys and values in 8 bits: e4m3 codes 'b hk n d' (d 64 or 128) and fp32 scales 'b hk n/block', a power of two for each `block` tokens of a kv head
-    (16, 32, 64 or 128); a row stands for its codes times its block's scale.  Made by `make_cache8`, filled by `cache8_append`."""
+    (16, 32, 64 or 128); a row stands for its codes times its block's scale.  Made by `make_cache8`, filled by `cache8_append`; scales of other origin have to be
+    powers of two from 2^-110 to 2^119 too, the kernels read no more of them than the exponent."""
     keys: Tensor
     values: Tensor
     key_scales: Tensor
