@@ -573,7 +573,7 @@ int nsa_newton_schulz(int32_t many, const int32_t* rows, const int32_t* cols, co
  * `window` of its keys (0: all), or with sel_block > 0 the blocks idx of sel_block keys (of each kv head, or of each head where per_head_sel:
  * [batch, kv_heads or heads, num_sel] contiguous, int32 or int64) whose fmask byte is not 0, as far as the sequence has them, and the keys of the block
  * that its newest key is in.  A block named twice counts twice.  No key: zeros.  out: [batch, heads, dim_head] contiguous, of `dtype`.  group <= 32;
- * num_sel <= 2^20, (num_sel + 1) * sel_block below 2^30, the row stride below 2^31, batch * heads below 2^23, q 16-byte aligned with strides of multiples of 8.
+ * num_sel <= 2^20, (num_sel + 1) * sel_block below 2^30, the row stride below 2^28, batch * heads below 2^23, q 16-byte aligned with strides of multiples of 8.
  * Sums in fp32, q and the probabilities as sums of bf16 parts (q exactly; probabilities to 16 bits, of fp32 queries to 24), results rounded once.
  * Only rows that are attended are read.  ws: aligned to 16 bytes, and not needed where its size is 0. */
 typedef struct nsa_cache8_desc {

@@ -152,10 +152,16 @@ __device__ __forceinline__ void transpose_bytes(const uint32_t (&d)[4], uint32_t
 // Where a unit's keys are: a range of rows; selected blocks of a multiple of 16 keys; selected blocks of any size.
 enum { kRange = 0, kBlocks = 1, kPacked = 2 };
 
+// a float at an address that is the same in all lanes, through the scalar cache: it waits for no other load
+__device__ __forceinline__ float of_all(const float* p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) float*>(reinterpret_cast<uintptr_t>(p));
+}
+
 template <int D>
 struct Tile8 {                         // what a lane holds of 32 keys
   uintx4 k[2][D / 64];                 // key n of each 16: 16 codes
-  uint32_t v[2][4][D / 64];            // keys 4 q + e: D / 16 codes
+  typedef __attribute__((__vector_size__(D / 16))) uint32_t words;
+  words v[2][4];                       // keys 4 q + e: D / 16 codes
   float ks[2], vs[2];                  // ks: of key n.  vs: one for all 16 keys (kPacked reads them from LDS where it needs them)
 };
 
@@ -340,57 +346,51 @@ __device__ __forceinline__ void attend8_body(const Attend8Args& A, const int gro
     const int x = K.base + (c0 + w0 + r * nw) * kTile + 16 * i;
     return x <= last ? x : -1;
   };
-  // the rows of 16 keys that begin with r0 where they may not all be there: without one ~ of the newest, which is attended and read instead
-  auto row = [&](int r0, int x) { return (r0 >= 0) & (x >= K.first) & (x <= last) ? x : ~last; };
+  auto there = [&](int r0, int x) { return (r0 >= 0) & (x >= K.first) & (x <= last); };
   auto whole = [&](int r0) { return r0 >= K.first && r0 + 15 <= last; };
+  // Of 16 keys that begin with row r0 and may not all be there: key x is read where it is or, in its place, the nearest that is (the newest where none is).
+  // Addresses are one for the wave and 32 bits of a lane's own.
+  auto beyond = [&](int r0, int x) { return r0 < 0 ? 0u : (uint32_t)((min(max(r0 + x, K.first), last) - r0) * s2); };
+  using words = typename Tile8<D>::words;
   auto load_k = [&](int r, Tile8<D>& X) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint8_t* p;
       if constexpr (MODE == kPacked) {
         const int at = (w0 + r * nw) * kTile + 16 * i + n, x = row_s[at];
         X.ks[i] = ks_s[at];
-        p = kb + (long)(x ^ (x >> 31)) * s2 + k_lane;
-      } else {
-        const int r0 = row0(r, i);
-        X.ks[i] = kz[(r0 < 0 ? last : r0) >> A.block_shift];
-        if (whole(r0)) {
-          p = kb + r0 * s2 + (n * s2 + k_lane);
-        } else {
-          const int x = row(r0, r0 + n);
-          p = kb + (x ^ (x >> 31)) * s2 + k_lane;
-        }
-      }
+        const uint8_t* p = kb + (long)(x ^ (x >> 31)) * s2 + k_lane;
 #pragma unroll
-      for (int j = 0; j < D / 64; ++j) X.k[i][j] = *reinterpret_cast<const uintx4*>(p + 64 * j);
+        for (int j = 0; j < D / 64; ++j) X.k[i][j] = *reinterpret_cast<const uintx4*>(p + 64 * j);
+      } else {
+        const int r0 = row0(r, i), rb = r0 < 0 ? last : r0;
+        X.ks[i] = of_all(kz + (rb >> A.block_shift));
+        const uint8_t* p = kb + rb * s2;
+        const uint32_t off = (whole(r0) ? n * (uint32_t)s2 : beyond(r0, n)) + k_lane;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) X.k[i][j] = *reinterpret_cast<const uintx4*>(p + 64 * j + off);
+      }
     }
   };
   auto load_v = [&](int r, Tile8<D>& X) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint8_t* p[4];
       if constexpr (MODE == kPacked) {
         const intx4 rv = *reinterpret_cast<const intx4*>(row_s + (w0 + r * nw) * kTile + 16 * i + 4 * q4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = vb + (long)(rv[e] ^ (rv[e] >> 31)) * s2 + v_lane;
+        for (int e = 0; e < 4; ++e) X.v[i][e] = *reinterpret_cast<const words*>(vb + (long)(rv[e] ^ (rv[e] >> 31)) * s2 + v_lane);
       } else {
-        const int r0 = row0(r, i);
-        X.vs[i] = vz[(r0 < 0 ? last : r0) >> A.block_shift];
+        const int r0 = row0(r, i), rb = r0 < 0 ? last : r0;
+        X.vs[i] = of_all(vz + (rb >> A.block_shift));
+        const uint8_t* p = vb + rb * s2;
         if (whole(r0)) {
+          const uint32_t off = 4 * q4 * (uint32_t)s2 + v_lane;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = vb + r0 * s2 + (4 * q4 * s2 + v_lane) + e * s2;
+          for (int e = 0; e < 4; ++e) X.v[i][e] = *reinterpret_cast<const words*>(p + e * s2 + off);
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int x = row(r0, r0 + 4 * q4 + e);
-            p[e] = vb + (x ^ (x >> 31)) * s2 + v_lane;
-          }
+          for (int e = 0; e < 4; ++e) X.v[i][e] = *reinterpret_cast<const words*>(p + (beyond(r0, 4 * q4 + e) + v_lane));
         }
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) X.v[i][e][j] = reinterpret_cast<const uint32_t*>(p[e])[j];
     }
   };
 
@@ -418,7 +418,7 @@ __device__ __forceinline__ void attend8_body(const Attend8Args& A, const int gro
         const int r0 = row0(r, i);
         if (!whole(r0)) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[4 * i + e] = row(r0, r0 + 4 * q4 + e) >= 0 ? s[4 * i + e] : -INFINITY;
+          for (int e = 0; e < 4; ++e) s[4 * i + e] = there(r0, r0 + 4 * q4 + e) ? s[4 * i + e] : -INFINITY;
         }
       }
     }
@@ -509,17 +509,23 @@ __device__ __forceinline__ void attend8_body(const Attend8Args& A, const int gro
       return r;
     };
     Tile8<D> X;
+    bf16x8 P[PP];
     int r = next(0);
-    if (r < rounds) { load_k(r, X); load_v(r, X); }
-    while (r < rounds) {
-      const int rn = next(r + 1);
+    if (r < rounds) {
+      load_k(r, X);
+      load_v(r, X);
+      // (the last tile by itself: a load that may be there or not is one that the compiler can only wait for together with all others)
+      for (int rn = next(r + 1); rn < rounds; rn = next(r + 1)) {
+        scores(r, X);
+        load_k(rn, X);
+        probabilities(r, X, P);
+        products(X, P);
+        load_v(rn, X);
+        r = rn;
+      }
       scores(r, X);
-      if (rn < rounds) load_k(rn, X);
-      bf16x8 P[PP];
       probabilities(r, X, P);
       products(X, P);
-      if (rn < rounds) load_v(rn, X);
-      r = rn;
     }
   }
   l = quarters_sum(l);
@@ -683,7 +689,7 @@ __global__ __launch_bounds__(kMerge) void cache8_merge_kernel(const Attend8Args 
 // units, parts and records of a call
 static int attend8_plan(const nsa_cache8_desc* d, Attend8Args& A, size_t& bytes) {
   if (!cache8_check(d) || d->group <= 0 || d->window < 0 || d->sel_block < 0 || d->num_sel < 0) return NSA_E_ARG;
-  if (!cache8_supported(d) || d->group > 32 || d->num_sel > 1 << 20 || ((long)d->num_sel + 1) * d->sel_block >= 1L << 30 || d->kv_stride[2] >= 1L << 31)
+  if (!cache8_supported(d) || d->group > 32 || d->num_sel > 1 << 20 || ((long)d->num_sel + 1) * d->sel_block >= 1L << 30 || d->kv_stride[2] >= 1L << 28)
     return NSA_E_UNSUPPORTED;
   const bool per_head = d->sel_block > 0 && d->per_head_sel;
   A.g = d->group;

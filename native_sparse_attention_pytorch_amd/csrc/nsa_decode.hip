@@ -1017,7 +1017,7 @@ static int make_step8_layout(const nsa_decode_step_desc* d, const nsa_cache8_des
       (long)cache->group * cache->kv_heads != d->heads || d->pos >= cache->capacity)
     return NSA_E_ARG;
   const int g = cache->group;
-  if (!cache8_supported(cache) || g > 32 || cache->kv_stride[2] >= 1L << 31 || (long)d->batch * d->heads >= 1L << 16) return NSA_E_UNSUPPORTED;
+  if (!cache8_supported(cache) || g > 32 || cache->kv_stride[2] >= 1L << 28 || (long)d->batch * d->heads >= 1L << 16) return NSA_E_UNSUPPORTED;
   const bool has_c = d->num_compressed > 0;
   if (X.L.k > 0 && (X.L.nb > 64 * 32 || X.L.k > 64)) return NSA_E_UNSUPPORTED;
   Step8& s = X.s;
