@@ -469,7 +469,8 @@ __device__ __forceinline__ void attend8_body(const Attend8Args& A, const int gro
   };
 
   // the wave's tiles; those of a selection whose blocks are not there are passed over.  The next tile's keys are asked for as soon as this one's
-  // are operands, its values likewise: one set of registers, two waves more on a SIMD than with two sets
+  // are operands, its values likewise: one set of registers (with two, and loads a tile further ahead, 32768 keys take 21.9 us instead of 20.8, 524287 72
+  // instead of 67, 17 blocks of 64 12.9 instead of 12.1)
   for (; c0 < t1; c0 += chunk) {
     const int c1 = min(t1, c0 + chunk), rounds = c0 + w0 < c1 ? (c1 - c0 - w0 + nw - 1) / nw : 0;
     if constexpr (MODE == kBlocks) {
@@ -704,7 +705,8 @@ static int attend8_plan(const nsa_cache8_desc* d, Attend8Args& A, size_t& bytes)
   if ((long)d->batch * d->kv_heads * d->group >= 1L << 23) return NSA_E_UNSUPPORTED;
   A.most = (int)tiles;
   A.shared = tiles > (units >= 256 ? kAloneMany : kAlone);
-  const int resident = d->dtype == 2 ? (d->dim_head == 64 ? 4 : 2) : d->dim_head == 64 ? 4 : 2;
+  // (work-groups of a CU: with three of 128 features 32768 keys take 22.8 us instead of 20.8, 48 ragged sequences 49.5 instead of 48; five of 64 the same)
+  const int resident = d->dim_head == 64 ? 4 : 2;
   const long most = ((tiles + kUnit) * (units < 1L << 20 ? units : 1L << 20) + kShare - 1) / kShare;
   A.groups = A.shared ? (int)(most < 256 * resident ? most : 256 * resident) : 0;
   bytes = A.shared ? 2 * (size_t)A.groups * A.rec * sizeof(float) : 0;
