@@ -6,8 +6,9 @@
 // block's new rows are held in registers in between, 32 values a lane, by one wave up to 2048 values and by up to eight for 128 rows of 128.  A
 // block that holds rows already is read too, and its rows are written again only where the scale grows.
 //
-// Measured: a prompt of 30011 tokens, 4 heads of 64 bf16 features, 12.7 us (46 MB: 3.6 TB/s; a copy of as much takes 10); six chunks of 1021 tokens, 5
-// heads of 128 fp32 features, 9.4 us (31 MB); one token for each of 64 sequences, 8 heads, 4.6 us, most of it the launch.
+// Measured: a prompt of 30011 tokens, 4 heads of 64 bf16 features, 11.4 us (46 MB: 4.1 TB/s; a copy of as much takes 10); six chunks of 1021 tokens, 5
+// heads of 128 fp32 features, 8.7 us (31 MB); one token for each of 64 sequences, 8 heads, 4.3 us, most of it the launch.  Blocks that are new as a whole have
+// loads without a branch between them (with the test of each row 12.7 and 9.4 us; with rows outside read as their neighbours in all blocks 12.1, 8.6 and 4.6).
 #include "nsa_cache8.hpp"
 
 namespace nsa {
@@ -54,29 +55,43 @@ __global__ __launch_bounds__((AppendShape<D, B>::THREADS)) void cache8_append_ke
   constexpr int RPW = 64 / LPR, STEP = RPW * S::WAVES;
   const int mine = part * RPW + lane / LPR, f = lane % LPR * 8;
 
-  floatx8 x[S::PER];
+  // All loads before the first value is looked at; of the rows of a load that are not there the nearest that is is read
+  typedef __attribute__((__vector_size__(8 * sizeof(T)))) T vec;
+  vec x[S::PER];
   uintx2 old[S::PER];
   float top = 0.f, s_old = 0.f;
   const bool held = first > 0;
-  if (any) {
-    if (held) s_old = *scale;
-    const T* from = src + (long)(mine - first) * s_row + f;
+  const bool all_new = !held && last >= B;       // no row is asked about
+  auto fresh = [&](int row) { return row >= first && row < last; };
+  auto some = [&](int c) { return part * RPW + c * STEP < last && part * RPW + c * STEP + RPW > first; };      // of a load's rows
+  auto largest = [&](int c, bool in) {
+    const floatx8 y = __builtin_convertvector(x[c], floatx8);
 #pragma unroll
-    for (int c = 0; c < S::PER; ++c) {
-      const int row = mine + c * STEP;
-      if (row >= first && row < last) x[c] = load_values(from + (long)(c * STEP) * s_row);
-      else if (row < first) old[c] = *reinterpret_cast<const uintx2*>(dst + row * A.c.s2 + f);
+    for (int e = 0; e < 8; ++e) {
+      const float m = fabsf(y[e]);
+      top = fmaxf(top, in && m < INFINITY ? m : 0.f);
     }
+  };
+  if (any) {
+    const T* from = src + f;
+    if (all_new) {
 #pragma unroll
-    for (int c = 0; c < S::PER; ++c) {
-      const int row = mine + c * STEP;
-      if (row >= first && row < last) {
+      for (int c = 0; c < S::PER; ++c) x[c] = *reinterpret_cast<const vec*>(from + (long)(mine + c * STEP - first) * s_row);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float m = fabsf(x[c][e]);
-          top = fmaxf(top, m < INFINITY ? m : 0.f);
-        }
+      for (int c = 0; c < S::PER; ++c) largest(c, true);
+    } else {
+#pragma unroll
+      for (int c = 0; c < S::PER; ++c)
+        if (some(c)) x[c] = *reinterpret_cast<const vec*>(from + (long)(min(max(mine + c * STEP, first), last - 1) - first) * s_row);
+      if (held) {
+        s_old = *scale;
+#pragma unroll
+        for (int c = 0; c < S::PER; ++c)
+          if (part * RPW + c * STEP < first) old[c] = *reinterpret_cast<const uintx2*>(dst + min(mine + c * STEP, first - 1) * A.c.s2 + f);
       }
+#pragma unroll
+      for (int c = 0; c < S::PER; ++c)
+        if (some(c)) largest(c, fresh(mine + c * STEP));
     }
     top = wave_max(top);
   }
@@ -95,7 +110,7 @@ __global__ __launch_bounds__((AppendShape<D, B>::THREADS)) void cache8_append_ke
   for (int c = 0; c < S::PER; ++c) {
     const int row = mine + c * STEP;
     uintx2* to = reinterpret_cast<uintx2*>(dst + row * A.c.s2 + f);
-    if (row >= first && row < last) *to = codes_of(x[c], inv);
+    if (all_new || fresh(row)) *to = codes_of(__builtin_convertvector(x[c], floatx8), inv);
     else if (row < first && s_new != s_old) *to = codes_of(values_of(old[c]), s_old * inv);
   }
 }
