@@ -14,11 +14,11 @@
 // the matrix cores have the time for it: they are busy for 5 to 12 % of the times below.
 //
 // Measured (this kernel, then the merge of the shares; a copy reaches 4.7 TB/s): one sequence of 524287 keys, 16 heads on 2 of 128 features, 52 us
-// (5.1 TB/s) and 6; of 32768 keys, 32 heads on 8, 17 us (3.9 TB/s) and 4; 48 sequences of 1 to 16384 keys, 44 us (3.8 TB/s) and 5; 16 blocks of 64 keys
-// and the newest of 32 sequences, 16 heads on 4 of 64 features, 12 us, and of one sequence, 32 heads on 8 of 128, 13 us - loads that wait for each
+// (5.2 TB/s) and 6; of 32768 keys, 32 heads on 8, 17 us (3.9 TB/s) and 4; 48 sequences of 1 to 16384 keys, 40 us (4.3 TB/s) and 5; 16 blocks of 64 keys
+// and the newest of 32 sequences, 16 heads on 4 of 64 features, 11 us, and of one sequence, 32 heads on 8 of 128, 12 us - loads that wait for each
 // other: the length, the blocks' numbers, the rows, five tiles one after the other in each wave.
-// More than 16 query heads of a kv head are two groups of columns, each converted for by waves of its own: 128 heads on 4, 26 sequences of 3 to 9339 keys,
-// take 32 us where 34 MB are 7.
+// More than 16 query heads of a kv head are two groups of columns, each converted for by waves of its own: 26 sequences of 3 to 9339 keys, 4 kv heads, take
+// 30 us with 32 query heads each and 23 with 16.
 #include "nsa_cache8.hpp"
 #include "nsa_decode_topk.hpp"
 
@@ -179,7 +179,7 @@ __device__ __forceinline__ long quotient(long n, long d) {
 // Shared tiles.  A sequence's tiles are as many as its length has, known to the device only.  All units lie one after the other on a line, each as long as its
 // tiles and kUnit more (what a unit costs besides them), and the line is cut into equal shares, one for each work-group, whatever the lengths are.  A unit whose
 // tiles lie in one share is finished there; of the others each share leaves a record, and the merge finds them by the same arithmetic.  (Parts of a fixed
-// size for each unit, sized for the capacity: 48 sequences of 1 to 16384 keys took 105 us where these take 50; most work-groups had nothing to do,
+// size for each unit, sized for the capacity: 48 sequences of 1 to 16384 keys took 105 us where these take 48; most work-groups had nothing to do,
 // and a few too much.)
 struct Shares {
   long total, share;                   // the line's length, a work-group's part of it
