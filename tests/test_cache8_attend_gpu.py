@@ -226,3 +226,26 @@ def test_more_sequences_than_a_launch_takes(what):
     else:
         got = ops.cache8_attend(q.to(DEV), many, lengths.to(DEV), **args)
     close(got[at], *R.attend(q[at], few, lengths[at].tolist(), **args), keys=n)
+
+
+def test_rows_far_apart():
+    """Rows of the largest distance that is taken, where 32 bits just hold the offsets of sixteen; beyond it the call is refused."""
+    from native_sparse_attention_pytorch_amd import ops
+    step = (1 << 28) - 16
+    far = [torch.empty(31 * step + 64, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn).as_strided((1, 1, 32, 64), (64, 64, step, 1)) for _ in range(2)]
+    near = ops.make_cache8(1, 1, 32, 64, block=16)
+    cache = ops.Cache8(*far, near.key_scales.clone(), near.value_scales.clone())
+    k, v = (torch.randn(1, 1, 29, 64, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    q = torch.randn(1, 4, 1, 64, device=DEV, dtype=torch.bfloat16)
+    idx, one = torch.zeros(1, 1, 1, 1, dtype=torch.int64, device=DEV), torch.ones(1, 1, 1, 1, dtype=torch.bool, device=DEV)
+    for c in (cache, near):
+        ops.cache8_append(c, k, v)
+    assert torch.equal(cache.keys[:, :, :29].view(torch.uint8), near.keys[:, :, :29].view(torch.uint8))
+    for n in (29, 16, 5):
+        for window in (None, 7):
+            assert torch.equal(ops.cache8_attend(q, cache, n, window=window), ops.cache8_attend(q, near, n, window=window))
+        for size in (16, 8):
+            assert torch.equal(ops.cache8_select_attend(q, cache, n, size, idx, one), ops.cache8_select_attend(q, near, n, size, idx, one))
+    beyond = [t.as_strided((1, 1, 16, 64), (64, 64, step + 16, 1)) for t in far]
+    with pytest.raises(RuntimeError, match="nsa_cache8_workspace_bytes"):
+        ops.cache8_attend(q, ops.Cache8(*beyond, near.key_scales[:, :, :1], near.value_scales[:, :, :1]), 5)
