@@ -19,6 +19,8 @@
 // other: the length, the blocks' numbers, the rows, five tiles one after the other in each wave.
 // More than 16 query heads of a kv head are two groups of columns, each converted for by waves of its own: 26 sequences of 3 to 9339 keys, 4 kv heads, take
 // 30 us with 32 query heads each and 23 with 16.
+#include <type_traits>
+
 #include "nsa_cache8.hpp"
 #include "nsa_decode_topk.hpp"
 
@@ -531,62 +533,66 @@ __device__ __forceinline__ void attend8_body(const Attend8Args& A, const int gro
   }
   l = quarters_sum(l);
 
-  // the waves' results as one
-  __syncthreads();                               // (the lists of rows are read no more)
-  constexpr int H = D / 2, RO = H + 4;           // half of the features at a time
+  // The waves' results as one, weighted by their maxima, by whoever sums them: all of a head's are asked for at once.  NW: waves of a group of columns; X: of four
+  // quarters of a lane's features, how many go through LDS at a time.
+  if constexpr (MODE == kPacked) __syncthreads();          // (the lists of rows are read no more)
   float* m_s = reinterpret_cast<float*>(lds);
   float* l_s = m_s + kWaves * 16;
   float* o_s = l_s + kWaves * 16;                // [wave][cols of a group][RO]
   const int most = min(16, A.gc);
-  if (q4 == 0) m_s[wave * 16 + n] = m;
-  __syncthreads();
-  float M = -INFINITY;
+  if (q4 == 0) { m_s[wave * 16 + n] = m; l_s[wave * 16 + n] = l; }
+  auto merge = [&](auto nw_, auto x_) {
+    constexpr int NW = decltype(nw_)::value, X = decltype(x_)::value, H = D * X / 4, RO = H + 4;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w)
-    if (w < nw) M = fmaxf(M, m_s[(group * nw + w) * 16 + n]);
-  const float by = m == -INFINITY ? 0.f : fast_exp2(m - M);
-  if (q4 == 0) l_s[wave * 16 + n] = m == -INFINITY ? l : by * l;      // (a NaN that raised no maximum)
+    for (int part = 0; part < 4 / X; ++part) {
+      // (place f of a part: feature DT (4 (f / X DT) + X part) + f % X DT)
+      if (n < cols) {
+        float* o = o_s + (wave * most + n) * RO + X * DT * q4;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    // (place f of the half: feature DT (4 (f / 2 DT) + 2 half) + f % 2 DT)
-    if (n < cols) {
-      float* o = o_s + (wave * most + n) * RO + 2 * DT * q4;
+        for (int i = 0; i < X; ++i)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+          for (int c = 0; c < DT; c += 4) {
+            const int x = X * part + i;
+            *reinterpret_cast<floatx4*>(o + DT * i + c) = floatx4{O[c][x], O[c + 1][x], O[c + 2][x], O[c + 3][x]};
+          }
+      }
+      __syncthreads();
+      for (int i = tid; i < A.gc * (H / 4); i += 64 * kWaves) {
+        const int g = i / (H / 4), at = i % (H / 4) * 4, w0 = (g >> 4) * NW, c = g & 15, f = DT * (4 * (at / (X * DT)) + X * part) + at % (X * DT);
+        float mw[NW], lw[NW], M = -INFINITY, L = 0.f;
+        floatx4 ow[NW], o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < DT; c += 4) {
-          const int x = 2 * half + i;
-          *reinterpret_cast<floatx4*>(o + DT * i + c) = floatx4{O[c][x] * by, O[c + 1][x] * by, O[c + 2][x] * by, O[c + 3][x] * by};
+        for (int w = 0; w < NW; ++w) {
+          mw[w] = m_s[(w0 + w) * 16 + c];
+          lw[w] = l_s[(w0 + w) * 16 + c];
+          ow[w] = *reinterpret_cast<const floatx4*>(o_s + ((w0 + w) * most + c) * RO + at);
+          M = fmaxf(M, mw[w]);
         }
-    }
-    __syncthreads();
-    for (int i = tid; i < A.gc * (H / 4); i += 64 * kWaves) {
-      const int g = i / (H / 4), at = i % (H / 4) * 4, gr = g >> 4, c = g & 15, f = DT * (4 * (at / (2 * DT)) + 2 * half) + at % (2 * DT);
-      floatx4 o = {0.f, 0.f, 0.f, 0.f};
-      float L = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w)
-        if (w < nw) {
-          L += l_s[(gr * nw + w) * 16 + c];
-          o += *reinterpret_cast<const floatx4*>(o_s + ((gr * nw + w) * most + c) * RO + at);
+        for (int w = 0; w < NW; ++w) {
+          const float by = mw[w] == -INFINITY ? 0.f : fast_exp2(mw[w] - M);
+          L += mw[w] == -INFINITY ? lw[w] : by * lw[w];    // (a NaN that raised no maximum)
+          o += ow[w] * by;
         }
-      if (whole_unit) {
-        typedef __attribute__((__vector_size__(4 * sizeof(T)))) T vec;
-        *reinterpret_cast<vec*>(reinterpret_cast<T*>(A.out) + ((long)b * A.c.hk * A.g + head0 + g) * D + f) =
-            L == 0.f ? vec{(T)0.f, (T)0.f, (T)0.f, (T)0.f} : vec{(T)(o[0] / L), (T)(o[1] / L), (T)(o[2] / L), (T)(o[3] / L)};
-      } else {
-        float* rec = A.part + (SHARED ? 2L * group_id + (t0 == 0) : group_id) * A.rec;
-        *reinterpret_cast<floatx4*>(rec + g * D + f) = o;
-        if (f == 0) {
-          float Mg = -INFINITY;
-          for (int w = 0; w < nw; ++w) Mg = fmaxf(Mg, m_s[(gr * nw + w) * 16 + c]);
-          rec[A.gc * D + g] = Mg;
-          rec[A.gc * D + A.gc + g] = L;
+        if (whole_unit) {
+          typedef __attribute__((__vector_size__(4 * sizeof(T)))) T vec;
+          *reinterpret_cast<vec*>(reinterpret_cast<T*>(A.out) + ((long)b * A.c.hk * A.g + head0 + g) * D + f) =
+              L == 0.f ? vec{(T)0.f, (T)0.f, (T)0.f, (T)0.f} : vec{(T)(o[0] / L), (T)(o[1] / L), (T)(o[2] / L), (T)(o[3] / L)};
+        } else {
+          float* rec = A.part + (SHARED ? 2L * group_id + (t0 == 0) : group_id) * A.rec;
+          *reinterpret_cast<floatx4*>(rec + g * D + f) = o;
+          if (f == 0) {
+            rec[A.gc * D + g] = M;
+            rec[A.gc * D + A.gc + g] = L;
+          }
         }
       }
+      if (part + 1 < 4 / X) __syncthreads();
     }
-    if (half == 0) __syncthreads();
-  }
+  };
+  if (groups == 1 && A.gc <= 8) merge(std::integral_constant<int, kWaves>{}, std::integral_constant<int, 4>{});
+  else if (groups == 1) merge(std::integral_constant<int, kWaves>{}, std::integral_constant<int, 2>{});
+  else merge(std::integral_constant<int, kWaves / 2>{}, std::integral_constant<int, 2>{});
   if (pos < end) __syncthreads();      // (LDS is used again)
   } while (pos < end);
 }
@@ -716,7 +722,7 @@ static int attend8_plan(const nsa_cache8_desc* d, Attend8Args& A, size_t& bytes)
 // bytes of LDS besides the table of first tiles
 template <int D>
 static int attend8_lds(const Attend8Args& A, int waves, bool lists) {
-  const int cols = A.gc < 16 ? A.gc : 16, merge = (waves * 32 + waves * cols * (D / 2 + 4)) * 4, rows = lists ? kListed * kTile * 12 : 0;
+  const int cols = A.gc < 16 ? A.gc : 16, merge = (waves * 32 + waves * cols * ((cols <= 8 ? D : D / 2) + 4)) * 4, rows = lists ? kListed * kTile * 12 : 0;
   return ((merge > rows ? merge : rows) + 15) / 16 * 16;
 }
 
