@@ -597,8 +597,9 @@ __device__ __forceinline__ void attend8_body(const Attend8Args& A, const int gro
   } while (pos < end);
 }
 
+// (shared tiles of 64 features: registers for the four work-groups of a CU that are launched; fp32, 20000 keys of 8 sequences 28.4 -> 26.7 us)
 template <class T, int D, int MODE, int W, bool SHARED>
-__global__ __launch_bounds__(64 * W) void cache8_attend_kernel(const Attend8Args A) {
+__global__ __launch_bounds__(64 * W, SHARED && D == 64 && W == 4 ? 4 : 1) void cache8_attend_kernel(const Attend8Args A) {
   extern __shared__ __align__(16) char lds[];
   attend8_body<T, D, MODE, W, SHARED>(A, blockIdx.x, gridDim.x, lds);
 }
