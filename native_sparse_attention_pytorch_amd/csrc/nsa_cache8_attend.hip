@@ -53,9 +53,10 @@ struct Attend8Args {
 typedef __attribute__((__vector_size__(2 * sizeof(float)))) float floatx2;
 
 constexpr int kTile = 32, kTable = 2048, kListed = 64;      // kTable: sequences of a launch; kListed: tiles whose rows are in LDS
-// see Shares.  kAlone: tiles of a unit up to which it has a work-group for itself and no merge follows (34 tiles of 8 units 13 us, shared 19); kAloneMany: where
-// there are units for all CUs (79 tiles of 256 units 37 us, shared 47; of lengths from 10 to 2500, 512 units 29 and 28)
-constexpr int kUnit = 8, kShare = 16, kAlone = 40, kAloneMany = 96;
+// see Shares.  kAlone: tiles of a unit up to which it has a work-group for itself and no merge follows (us alone / shared: 51 tiles of 8 units 12.7 / 12.9, of 64
+// units 14.0 / 16.7; 65 of 8 units 15.2 / 12.0, of 64 units 17.2 / 18.4, or 16.8 / 14.8 where lengths are from 10 keys on); kAloneMany: where there are units for all
+// CUs (51 to 104 tiles of 512 units 47 / 54 to 93 / 98; lengths from 10 to 2560 keys 22 / 25, to 4300 33 / 29)
+constexpr int kUnit = 8, kShare = 16, kAlone = 52, kAloneMany = 96;
 
 __device__ __forceinline__ floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 

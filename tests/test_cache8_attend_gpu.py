@@ -249,3 +249,21 @@ def test_rows_far_apart():
     beyond = [t.as_strided((1, 1, 16, 64), (64, 64, step + 16, 1)) for t in far]
     with pytest.raises(RuntimeError, match="nsa_cache8_workspace_bytes"):
         ops.cache8_attend(q, ops.Cache8(*beyond, near.key_scales[:, :, :1], near.value_scales[:, :, :1]), 5)
+
+
+@pytest.mark.parametrize("size, chosen", [(64, 40), (16, 150), (40, 60), (7, 300)])
+@pytest.mark.parametrize("dtype, d, block, g, per_head", [("bf16", 64, 32, 4, False), ("bf16", 128, 16, 20, False), ("fp16", 128, 64, 3, True), ("fp32", 64, 128, 8, False), ("fp32", 128, 32, 2, True)])
+def test_many_selected_blocks(dtype, d, block, g, per_head, size, chosen):
+    """So many that work-groups share them."""
+    from native_sparse_attention_pytorch_amd import ops
+    lengths = [2, 700, 2816, 0]
+    b, hk = len(lengths), 2
+    q, cache = made(b, hk, g, 2816, d, block, dtype, seed=chosen)
+    cache = spoil(cache, lengths)
+    gen = torch.Generator().manual_seed(size)
+    units = hk * g if per_head else hk
+    idx = torch.randint(-1, 2816 // size + 2, (b, units, 1, chosen), generator=gen, dtype=torch.int32)
+    fmask = torch.rand(b, units, 1, chosen, generator=gen) < 0.8
+    got = ops.cache8_select_attend(q.to(DEV), on_device(cache), torch.tensor(lengths, device=DEV, dtype=torch.int32), size, idx.to(DEV), fmask.to(DEV))
+    close(got, *R.attend(q, cache, lengths, size=size, idx=idx, fmask=fmask), keys=size * (chosen + 1))
+    assert not got[3].any()
