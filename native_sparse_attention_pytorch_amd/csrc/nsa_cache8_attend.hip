@@ -13,10 +13,10 @@
 // parts (one of bf16, two of fp16, three of fp32: exact), probabilities of two (three for fp32 results): 2^-17 (2^-24) of each.  At 16 columns
 // the matrix cores have the time for it: they are busy for 5 to 12 % of the times below.
 //
-// Measured (this kernel, then the merge of the shares; a copy reaches 4.7 TB/s): one sequence of 524287 keys, 16 heads on 2 of 128 features, 52 us
-// (5.2 TB/s) and 6; of 32768 keys, 32 heads on 8, 17 us (3.9 TB/s) and 4; 48 sequences of 1 to 16384 keys, 40 us (4.3 TB/s) and 5; 16 blocks of 64 keys
-// and the newest of 32 sequences, 16 heads on 4 of 64 features, 11 us, and of one sequence, 32 heads on 8 of 128, 12 us - loads that wait for each
-// other: the length, the blocks' numbers, the rows, five tiles one after the other in each wave.
+// Measured (this kernel, then the merge of the shares; a copy reaches 4.7 TB/s): one sequence of 524287 keys, 16 heads on 2 of 128 features, 51 us
+// (5.3 TB/s) and 6; of 32768 keys, 32 heads on 8, 16 us (4.1 TB/s) and 4; 48 sequences of 1 to 16384 keys, 38 us (4.5 TB/s) and 5; 16 blocks of 64 keys
+// and the newest of 32 sequences, 16 heads on 4 of 64 features, 10 us, and of one sequence, 32 heads on 8 of 128, 11 us: a few CUs have it all, and one
+// takes 64 KB in 1.4 us, by eight waves or by sixteen (11.2 us).
 // More than 16 query heads of a kv head are two groups of columns, each converted for by waves of its own: 26 sequences of 3 to 9339 keys, 4 kv heads, take
 // 30 us with 32 query heads each and 23 with 16.
 #include <type_traits>
