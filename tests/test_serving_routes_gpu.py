@@ -98,3 +98,33 @@ def test_a_conversation(dtype):
             # half a step of a value, or of the scale's smallest code: the scale is below 2^-7 of the largest of 32 rows of these
             for rows, x in ((rows_k, k), (rows_v, v)):
                 assert ((rows[0] - x[0].float()).abs() <= x[0].float().abs() * 2 ** -4 + 2 ** -10 * 2 ** -4).all()
+
+
+def test_calls_at_once_on_two_streams():
+    """Each call has its own workspace: what runs beside it changes nothing."""
+    from native_sparse_attention_pytorch_amd import ops
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    rand = lambda *shape: torch.randn(*shape, device=DEV, generator=gen).bfloat16()
+    work = []
+    for rows in (9000, 12000):
+        cache = ops.make_cache8(3, 4, rows, 128, block=64)
+        ops.cache8_append(cache, rand(3, 4, rows, 128), rand(3, 4, rows, 128))
+        lengths = torch.tensor([rows, rows // 3, 1], dtype=torch.int32, device=DEV)
+        history = torch.randint(0, 50000, (40, 700), device=DEV, generator=gen)
+        work.append((rand(3, 16, 1, 128), cache, lengths, rand(40, 50000), history))
+
+    def step(q, cache, lengths, logits, history):
+        return ops.cache8_attend(q, cache, lengths), ops.cache8_attend(q, cache, lengths, window=3000), ops.adjust_logits(logits, history, repetition_penalty=1.3)
+    want = [step(*w) for w in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for s, w, to in zip(streams, work, got):
+            with torch.cuda.stream(s):
+                to.append(step(*w))
+    torch.cuda.synchronize()
+    for to, here in zip(got, want):
+        for results in to:
+            for a, b in zip(results, here):
+                assert torch.equal(a, b)
