@@ -267,3 +267,12 @@ def test_many_selected_blocks(dtype, d, block, g, per_head, size, chosen):
     got = ops.cache8_select_attend(q.to(DEV), on_device(cache), torch.tensor(lengths, device=DEV, dtype=torch.int32), size, idx.to(DEV), fmask.to(DEV))
     close(got, *R.attend(q, cache, lengths, size=size, idx=idx, fmask=fmask), keys=size * (chosen + 1))
     assert not got[3].any()
+
+
+@pytest.mark.parametrize("lengths", [[40000], [40000, 3, 0, 39999]])
+@pytest.mark.parametrize("dtype, g", [("bf16", 4), ("fp32", 1), ("bf16", 20)])
+def test_few_units_of_many_tiles(dtype, g, lengths):
+    from native_sparse_attention_pytorch_amd import ops
+    q, cache = made(len(lengths), 1, g, 40000, 64, 64, dtype, seed=g)
+    got = ops.cache8_attend(q.to(DEV), on_device(spoil(cache, lengths)), torch.tensor(lengths, device=DEV, dtype=torch.int32))
+    close(got, *R.attend(q, cache, lengths), keys=40000)
