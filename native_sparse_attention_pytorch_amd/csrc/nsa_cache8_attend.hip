@@ -56,10 +56,10 @@ constexpr int kTile = 32, kTable = 2048, kListed = 64;      // kTable: sequences
 // see Shares.  kUnit: of 4, 48 ragged sequences take 55 us instead of 47; of 12, 48.  kShare: of 16, 57 to 125 tiles of 8 units take 12.0 to 13.6 us instead of
 // 10.1 to 10.5
 constexpr int kUnit = 8, kShare = 4;
-// Tiles of a unit up to which it has a work-group for itself and no merge follows.  us alone / shared: of 128 features, 26 tiles of 8 units 10.2 / 10.1, 34 tiles
-// 11.5 / 10.3, 25 of 16 units 8.8 / 11.4 to 12.8, 40 tiles 11.1 / 11.5; of 64 features, 40 tiles of 4 units 9.1 / 9.0, 34 of 16 9.3 / 9.7; 42 of 64 units 14.1 / 14.5, 50 tiles
-// 15.7 / 15.3; 41 of 512 units of lengths from 10 keys on 14 / 21, 91 tiles 23 / 25, 125 tiles 31 / 28
-__host__ inline int alone_up_to(long units, int dim) { return units >= 256 ? 96 : units >= 64 ? 50 : dim == 64 ? 40 : 30; }
+// Tiles of a unit up to which it has a work-group for itself and no merge follows.  us alone / shared: of 128 features, 34 tiles of 8 units 11.5 / 10.3, 50 tiles 14.3 /
+// 10.4, 42 of 64 units 14.1 / 14.5, 50 tiles 15.7 / 15.3; of 64 features, 50 of 16 units 10.4 / 11.3; 41 of 512 units of lengths from 10 keys on 14 / 21, 91 tiles
+// 23 / 25, 125 tiles 31 / 28.  These are calls replayed from a graph; by itself a call is the host's, and a second launch and a workspace take it from 11 to 15.5.
+__host__ inline int alone_up_to(long units) { return units >= 256 ? 96 : 50; }
 
 __device__ __forceinline__ floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -715,7 +715,7 @@ static int attend8_plan(const nsa_cache8_desc* d, Attend8Args& A, size_t& bytes)
   const long tiles = (places + kTile - 1) / kTile;
   if ((long)d->batch * d->kv_heads * d->group >= 1L << 23) return NSA_E_UNSUPPORTED;
   A.most = (int)tiles;
-  A.shared = tiles > alone_up_to(units, d->dim_head);
+  A.shared = tiles > alone_up_to(units);
   // (work-groups of a CU: with three of 128 features 32768 keys take 22.8 us instead of 20.8, 48 ragged sequences 49.5 instead of 48; five of 64 the same)
   const int resident = d->dim_head == 64 ? 4 : 2;
   // (and of a unit 256, whose records are merged: with 512, 131072 keys of one kv head take 21.0 us instead of 18.3)
