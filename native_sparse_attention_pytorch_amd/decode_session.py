@@ -25,6 +25,7 @@ partial results are merged (the split is sized for the capacity rather than the 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -145,11 +146,11 @@ class DecodeSession:
             (self.own_in and self.own_out) or self.w_cat.numel() * 2 >= 32 << 20)
         self._graphs = None
         if capture:
-            # the libraries initialise themselves on first use (outside the capture); the warm-up steps write row `pos` of
-            # the caches and row `nc` of the compressed caches, which the first real steps overwrite, and leave both counters alone
+            # the libraries initialise themselves on first use (outside the capture); the warm-up steps write row `pos` of bf16
+            # caches and row `nc` of the compressed caches, which the first real steps overwrite, and leave both counters alone
             side = torch.cuda.Stream(device=dev)
             side.wait_stream(torch.cuda.current_stream(dev))
-            with torch.cuda.stream(side), torch.no_grad():
+            with torch.cuda.stream(side), torch.no_grad(), self.warming_up():
                 for _ in range(2):
                     self.layer_step(self.x_buf, advance=0)
                     self.compress_window(count=False)
@@ -164,6 +165,21 @@ class DecodeSession:
                 self._prepare_direct(merged)
 
     # ---------------------------------------------------------------------------------------
+
+    @contextlib.contextmanager
+    def warming_up(self):
+        """Around steps with advance=0 on the current stream: an 8-bit cache is afterwards what it was.  Their row `pos` is the next token's, but it may have raised the
+        scale of its block, and the block's other rows are then rounded for a token that the sequence does not have."""
+        if self.cache8 is None:
+            yield
+            return
+        block = self.cache8.block
+        at = self.pos // block
+        parts = [t[:, :, at * block:(at + 1) * block] for t in self.cache8[:2]] + [t[:, :, at] for t in self.cache8[2:]]
+        held = [t.clone() for t in parts]
+        yield
+        for t, before in zip(parts, held):
+            t.copy_(before)
 
     def _record(self, event: bool, step: bool):
         self._graphs[event] = g = torch.cuda.CUDAGraph()
@@ -363,7 +379,9 @@ class TransformerDecodeSession:
         self.tok = torch.zeros((b, 1), dtype=torch.long, device=dev)
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(side), torch.no_grad():
+        with torch.cuda.stream(side), torch.no_grad(), contextlib.ExitStack() as warm:
+            for layer in self.layers:
+                warm.enter_context(layer.warming_up())
             for _ in range(2):
                 self._body(advance=0, event=True, count=False)
         torch.cuda.current_stream(dev).wait_stream(side)
