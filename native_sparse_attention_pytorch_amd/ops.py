@@ -3159,9 +3159,11 @@ def _logits_plan(logits, history, history_lengths, bias, allowed, numbers, value
         if width is None or allowed[0] not in ((width,), (*lead, width)):
             raise RuntimeError(f"{name}: allowed {allowed[2]} {tuple(allowed[0])}: expected bool 'v' or '... v', or int32 words of 32 entries, for logits {tuple(shape)}")
         kind = 2 if allowed[2] == torch.int32 else 1
+    axes = lambda size: [n for n in size if n != 1]
     for what, t in zip(("repetition_penalty", "frequency_penalty", "presence_penalty", "temperature"), numbers):
-        if t is not None and (not t[2].is_floating_point or t[0].numel() not in (1, rows) or len(t[0]) > max(len(lead), 1)):
-            raise RuntimeError(f"{name}: {what} {t[2]} {tuple(t[0])}: expected a number, or floating, one or one for each of {rows} rows")
+        # (the rows' shape, or one axis: as many values in another shape may be in another order)
+        if t is not None and (not t[2].is_floating_point or axes(t[0]) not in ([], [rows], axes(lead)) or len(t[0]) > max(len(lead), 1)):
+            raise RuntimeError(f"{name}: {what} {t[2]} {tuple(t[0])}: expected a number, or floating, one or one for each row, for logits {tuple(shape)}")
     if not (0 < values[0] < math.inf and abs(values[1]) < math.inf and abs(values[2]) < math.inf and 0 < values[3] < math.inf):
         raise ValueError(f"{name}: repetition_penalty {values[0]}, frequency_penalty {values[1]}, presence_penalty {values[2]}, temperature {values[3]}: "
                          "expected finite numbers, the first and the last above 0")
@@ -3250,7 +3252,7 @@ def adjust_logits(logits: Tensor, history: Tensor | None = None, history_lengths
         c > 0:  x <- (x / repetition_penalty where x > 0, else x repetition_penalty) - frequency_penalty c - presence_penalty
         x <- (x + bias) / temperature;   -inf where not `allowed`
 
-    The four numbers are Python's, or floating tensors of one value or one for each row (above 0 where a number has to be: not checked).  bias: 'v' or '... v';
+    The four numbers are Python's, or floating tensors of one value or one for each row, '...' or all along one axis (above 0 where a number has to be: not checked).  bias: 'v' or '... v';
     allowed: bool 'v' or '... v', or int32 words of 32 entries each, the lowest bit the first, 'v/32' rounded up.  A row may have nothing allowed.
     No gradients."""
     numbers, tensors = [], []
