@@ -3139,7 +3139,8 @@ def cache8_select_attend(q: Tensor, cache: Cache8, lengths, block: int, idx: Ten
 
 @functools.lru_cache(maxsize=256)
 def _logits_plan(logits, history, history_lengths, bias, allowed, numbers, values):
-    """(descriptor, which of the operands have to be laid out first) of these layouts; `numbers`: of the four tensors that may stand for values."""
+    """(descriptor up to `history` and behind it, which of the operands have to be laid out first) of these layouts; `history`: (shape up to its tokens, type,
+    whether it is contiguous), since a sequence has one more of them at each step; `numbers`: of the four tensors that may stand for values."""
     name = "adjust_logits"
     shape, stride, dtype = logits
     if dtype not in _LOSS_TYPES or len(shape) < 1 or shape[-1] == 0:
@@ -3147,8 +3148,8 @@ def _logits_plan(logits, history, history_lengths, bias, allowed, numbers, value
     lead, vocab = shape[:-1], shape[-1]
     rows = lead.numel()
     whole = torch.int32, torch.int64
-    if history is not None and (history[2] not in whole or len(history[0]) < 1 or history[0][:-1] != lead):
-        raise RuntimeError(f"{name}: history {history[2]} {tuple(history[0])}: expected int32 or int64 '... t' for logits {tuple(shape)}")
+    if history is not None and (history[1] not in whole or history[0] != lead):
+        raise RuntimeError(f"{name}: history {history[1]} of rows {None if history[0] is None else tuple(history[0])}: expected int32 or int64 '... t' for logits {tuple(shape)}")
     if history_lengths is not None and (history is None or history_lengths[2] not in whole or history_lengths[0] != lead):
         raise RuntimeError(f"{name}: history_lengths {history_lengths[2]} {tuple(history_lengths[0])}: expected int32 or int64, one for each row of a history")
     if bias is not None and (not bias[2].is_floating_point or bias[0] not in ((vocab,), shape)):
@@ -3188,17 +3189,16 @@ def _logits_plan(logits, history, history_lengths, bias, allowed, numbers, value
 
     contiguous = lambda t: all(n == 1 or at == w for n, at, w in zip(t[0], t[1], _strides_of(t[0])))
     x_step, bias_step, allowed_step = row_step(logits, vocab), row_step(bias, vocab), row_step(allowed, None if allowed is None else allowed[0][-1])
-    fixes = (x_step is None, history is not None and not contiguous(history), history_lengths is not None and not (history_lengths[2] == torch.int32 and contiguous(history_lengths)),
+    fixes = (x_step is None, history is not None and not history[2], history_lengths is not None and not (history_lengths[2] == torch.int32 and contiguous(history_lengths)),
              bias is not None and (bias[2] != torch.float32 or bias_step is None), allowed is not None and allowed_step is None,
              tuple(t is not None and not (t[2] == torch.float32 and contiguous(t)) for t in numbers))
     if fixes[3]:
         bias_step = 0 if len(bias[0]) == 1 and len(lead) else vocab
     if fixes[4]:
         allowed_step = 0 if len(allowed[0]) == 1 and len(lead) else allowed[0][-1]
-    desc = _LOGITS_DESC.pack(rows, vocab if x_step is None else x_step, vocab, _LOSS_TYPES[dtype], 0 if history is None else history[0][-1],
-                             history is not None and history[2] == torch.int64, kind, bias_step, allowed_step,
-                             *(int(t is not None and t[0].numel() > 1) for t in numbers), *values)
-    return desc, fixes, any(fixes[:5]) or any(fixes[5])
+    desc = _LOGITS_DESC.pack(rows, vocab if x_step is None else x_step, vocab, _LOSS_TYPES[dtype], 0, history is not None and history[1] == torch.int64, kind,
+                             bias_step, allowed_step, *(int(t is not None and t[0].numel() > 1) for t in numbers), *values)
+    return desc[:24], desc[32:], fixes, any(fixes[:5]) or any(fixes[5])
 
 
 def _strides_of(shape):
@@ -3214,8 +3214,12 @@ def _adjust_logits(logits, history, history_lengths, bias, allowed, repetition, 
     given = history, history_lengths, bias, allowed, repetition, frequency, presence, temperature
     if device < 0 or any([t is not None and t.get_device() != device for t in given]):
         raise RuntimeError("adjust_logits: needs tensors on one GPU (HIP kernels, no CPU fallback)")
-    desc, fixes, any_fix = _logits_plan(_layout(logits), _layout(history), _layout(history_lengths), _layout(bias), _layout(allowed),
-                                        (_layout(repetition), _layout(frequency), _layout(presence), _layout(temperature)), tuple(values))
+    tokens, past = 0, None
+    if history is not None:
+        past = history.shape[:-1] if history.dim() else None, history.dtype, history.is_contiguous()
+        tokens = history.shape[-1] if history.dim() else 0
+    head, tail, fixes, any_fix = _logits_plan(_layout(logits), past, _layout(history_lengths), _layout(bias), _layout(allowed),
+                                              (_layout(repetition), _layout(frequency), _layout(presence), _layout(temperature)), tuple(values))
     out = torch.empty_like(logits, dtype=torch.float32, memory_format=torch.contiguous_format)
     if not out.numel():
         return out
@@ -3227,8 +3231,8 @@ def _adjust_logits(logits, history, history_lengths, bias, allowed, repetition, 
         history_lengths = _int32(history_lengths).contiguous() if fixes[2] else history_lengths
         bias, allowed = bias.float().contiguous() if fixes[3] else bias, allowed.contiguous() if fixes[4] else allowed
         repetition, frequency, presence, temperature = (t.float().contiguous() if fix else t for t, fix in zip(given[4:], fixes[5]))
-    _lib.check(_lib.lib().nsa_adjust_logits(desc, logits.data_ptr(), _ptr(history), _ptr(history_lengths), _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(bias),
-                                            _ptr(allowed), _ptr(temperature), out.data_ptr(), _stream()), "nsa_adjust_logits")
+    _lib.check(_lib.lib().nsa_adjust_logits(head + tokens.to_bytes(8, "little") + tail, logits.data_ptr(), _ptr(history), _ptr(history_lengths), _ptr(repetition),
+                                            _ptr(frequency), _ptr(presence), _ptr(bias), _ptr(allowed), _ptr(temperature), out.data_ptr(), _stream()), "nsa_adjust_logits")
     return out
 
 
