@@ -596,7 +596,7 @@ int nsa_cache8_attend(const nsa_cache8_desc* d, const void* q, const void* keys,
 
 /* nsa_decode_step_dyn over an 8-bit cache (its keys and values; the compressed caches are bf16 as there): the new token's key and value go into row state[0] as by
  * nsa_cache8_append, before anything attends them.  `cache`: dtype 0, batch, kv_heads, dim_head and group as `capacity` has them; window, sel_block and the lengths
- * are not read.  ws: 256-byte aligned. */
+ * are not read.  capacity->num_compressed: 1 or more (state[1] may be 0).  ws: 256-byte aligned. */
 int nsa_decode_step8_workspace_bytes(const nsa_decode_step_desc* capacity, const nsa_cache8_desc* cache, size_t* bytes);
 int nsa_decode_step8_dyn(const nsa_decode_step_desc* capacity, const nsa_cache8_desc* cache, int32_t* state, const void* q, const void* k, const void* v,
                          const float* freqs, void* keys, void* values, float* key_scales, float* value_scales, const void* ck_cache, const void* cv_cache,

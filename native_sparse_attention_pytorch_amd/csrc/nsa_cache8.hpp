@@ -184,7 +184,6 @@ inline StepPrepArgs step8_prep_args(const Step8& s, const void* q, const int64_t
   }
   return A;
 }
-int cache8_step_prep(const Step8& s, const StepPrepArgs& A, void* stream);
 // Parts and floats of a record of each unit, {sliding window, selected blocks}: records [gc][D] sums, [gc] maxima, [gc] weights, as nsa_decode_combine takes them.
 void cache8_step_parts(const Step8& s, int parts[2], int rec[2]);
 // The blocks are idx where fmask is set, or the ones that the work-groups choose themselves from `pooled` [batch, rows of the selection, pooled_stride].

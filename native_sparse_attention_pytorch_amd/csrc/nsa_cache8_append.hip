@@ -164,20 +164,3 @@ extern "C" int nsa_cache8_append(const nsa_cache8_desc* d, int32_t rows, const v
   hipStream_t st = (hipStream_t)stream;
   return d->dtype == 0 ? append_dim<__bf16>(A, d->dim_head, st) : d->dtype == 1 ? append_dim<_Float16>(A, d->dim_head, st) : append_dim<float>(A, d->dim_head, st);
 }
-
-// ------------------------------------------------------------------------------------------------------------
-namespace nsa {
-
-template <int D>
-__global__ __launch_bounds__(128) void cache8_step_prep_kernel(const StepPrepArgs A) { step8_prep<D>(A, blockIdx.x); }
-
-int cache8_step_prep(const Step8& s, const StepPrepArgs& A, void* stream) {
-  const nsa_cache8_desc* d = s.d;
-  const dim3 grid((unsigned)(d->batch * d->kv_heads));
-  if (d->dim_head == 64) hipLaunchKernelGGL((cache8_step_prep_kernel<64>), grid, dim3(128), 0, (hipStream_t)stream, A);
-  else hipLaunchKernelGGL((cache8_step_prep_kernel<128>), grid, dim3(128), 0, (hipStream_t)stream, A);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? 0 : (int)e;
-}
-
-}  // namespace nsa

@@ -1017,7 +1017,7 @@ static int make_step8_layout(const nsa_decode_step_desc* d, const nsa_cache8_des
     return NSA_E_ARG;
   const int g = cache->group;
   if (!cache8_supported(cache) || g > 32 || cache->kv_stride[2] >= 1L << 28 || (long)d->batch * d->heads >= 1L << 16) return NSA_E_UNSUPPORTED;
-  const bool has_c = d->num_compressed > 0;
+  if (d->num_compressed == 0) return NSA_E_UNSUPPORTED;      // (the new token goes into the cache beside the compressed branch)
   if (X.L.k > 0 && (X.L.nb > 64 * 32 || X.L.k > 64)) return NSA_E_UNSUPPORTED;
   Step8& s = X.s;
   s = Step8{};
@@ -1040,7 +1040,7 @@ static int make_step8_layout(const nsa_decode_step_desc* d, const nsa_cache8_des
   o = up256(o + X.L.wsc);
   X.off_rf = o;     o = up256(o + (size_t)d->batch * units[1] * parts[1] * rec[1] * 4);
   X.off_rs = o;     o = up256(o + (size_t)d->batch * units[0] * parts[0] * rec[0] * 4);
-  X.off_logits = o; o = up256(o + (size_t)d->batch * d->heads * (has_c ? d->num_compressed : 1) * 4);      // (pooled ones are fewer)
+  X.off_logits = o; o = up256(o + (size_t)d->batch * d->heads * d->num_compressed * 4);      // (pooled ones are fewer)
   const size_t sel = (size_t)d->batch * X.L.sel_units * (X.L.k > 0 ? X.L.k : 1);
   X.off_idx = o;    o = up256(o + sel * 4);
   X.off_vals = o;   o = up256(o + sel * 4);
@@ -1067,10 +1067,10 @@ extern "C" int nsa_decode_step8_dyn(const nsa_decode_step_desc* d, const nsa_cac
   using namespace nsa;
   Step8Layout X;
   if (int e = make_step8_layout(d, cache, X)) return e;
-  if (!state || !q || !k || !v || !freqs || !keys || !values || !key_scales || !value_scales || !gate_logits || !ws || !out || (uintptr_t)ws % 256) return NSA_E_ARG;
+  if (!state || !q || !k || !v || !freqs || !keys || !values || !key_scales || !value_scales || !ck_cache || !cv_cache || !gate_logits || !ws || !out ||
+      (uintptr_t)ws % 256)
+    return NSA_E_ARG;
   if (ws_bytes < X.total) return NSA_E_WORKSPACE;
-  const bool has_c = d->num_compressed > 0;
-  if (has_c && (!ck_cache || !cv_cache)) return NSA_E_ARG;
   if (((uintptr_t)keys | (uintptr_t)values | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16) return NSA_E_ARG;
   if ((d->q_stride[0] | d->q_stride[1] | d->k_stride[0] | d->k_stride[1] | d->v_stride[0] | d->v_stride[1]) & 7) return NSA_E_ARG;
   if (!k_run != !v_run || (k_run && (ring <= 0 || ((krun_row | vrun_row) & 7) || ((d->krun_stride[0] | d->krun_stride[1] | d->vrun_stride[0] | d->vrun_stride[1]) & 7))))
@@ -1083,28 +1083,24 @@ extern "C" int nsa_decode_step8_dyn(const nsa_decode_step_desc* d, const nsa_cac
   X.s.d = &own;
   const StepPrepArgs prep = step8_prep_args(X.s, q, d->q_stride, k, d->k_stride, v, d->v_stride, freqs, rq, k_run, d->krun_stride, krun_row, v_run, d->vrun_stride,
                                             vrun_row, ring);
-  DecodePlan Pc{};
+  DecodePlan Pc;
   int32_t* idx = (int32_t*)(w + X.off_idx);
   uint8_t* fm = (uint8_t*)(w + X.off_fm);
   float* logits = (float*)(w + X.off_logits);
   const long nb = X.L.nb > 0 ? X.L.nb : 1;
-  const bool choose = has_c && X.L.k > 0 && X.L.pooled;
-  if (!has_c) {
-    if (int e = cache8_step_prep(X.s, prep, stream)) return e;
-  } else {
-    if (int e = make_decode_plan(&X.L.c, Pc, true, X.L.tiles_s)) return e;
-    Pc.dyn = state; Pc.dyn_kind = 1; Pc.window = d->window; Pc.per_block = d->per_block; Pc.smax = X.L.k;
-    Pc.cap_len = d->pos + 1; Pc.cap_nc = d->num_compressed; Pc.lstride = d->num_compressed;
-    AttendArgs C = attend_args(Pc, q, ck_cache, cv_cache, mem_k, mem_v, nullptr, nullptr, w + X.L.off_wsc, X.L.k > 0 && !choose ? logits : nullptr);
-    C.pool = PoolOut{logits, nb, d->per_block, d->share ? 1 : 0};
-    if (int e = choose ? launch_attend_prep<kPooled>(C, X.L.wsc, prep, stream) : launch_attend_prep<kPlain>(C, X.L.wsc, prep, stream)) return e;
-    if (X.L.k > 0 && !choose)
-      if (int e = decode_topk_launch(logits, d->batch, d->kv_heads, d->heads / d->kv_heads, d->num_compressed, d->per_block, d->share, X.L.k, idx,
-                                     (float*)(w + X.off_vals), fm, state, stream))
-        return e;
-  }
+  const bool choose = X.L.k > 0 && X.L.pooled;
+  if (int e = make_decode_plan(&X.L.c, Pc, true, X.L.tiles_s)) return e;
+  Pc.dyn = state; Pc.dyn_kind = 1; Pc.window = d->window; Pc.per_block = d->per_block; Pc.smax = X.L.k;
+  Pc.cap_len = d->pos + 1; Pc.cap_nc = d->num_compressed; Pc.lstride = d->num_compressed;
+  AttendArgs C = attend_args(Pc, q, ck_cache, cv_cache, mem_k, mem_v, nullptr, nullptr, w + X.L.off_wsc, X.L.k > 0 && !choose ? logits : nullptr);
+  C.pool = PoolOut{logits, nb, d->per_block, d->share ? 1 : 0};
+  if (int e = choose ? launch_attend_prep<kPooled>(C, X.L.wsc, prep, stream) : launch_attend_prep<kPlain>(C, X.L.wsc, prep, stream)) return e;
+  if (X.L.k > 0 && !choose)
+    if (int e = decode_topk_launch(logits, d->batch, d->kv_heads, d->heads / d->kv_heads, d->num_compressed, d->per_block, d->share, X.L.k, idx,
+                                   (float*)(w + X.off_vals), fm, state, stream))
+      return e;
   if (int e = cache8_step_attend(X.s, rq, idx, fm, choose ? logits : nullptr, nb, (float*)(w + X.off_rs), (float*)(w + X.off_rf), stream)) return e;
   const DecodePlan* pp[3] = {&Pc, &X.Pf, &X.Ps};
-  const void* wsp[3] = {has_c ? w + X.L.off_wsc : nullptr, w + X.off_rf, w + X.off_rs};
+  const void* wsp[3] = {w + X.L.off_wsc, w + X.off_rf, w + X.off_rs};
   return launch_combine(pp, wsp, gate_logits, gate_row, gate_bias, out, advance ? state : nullptr, stream);
 }
