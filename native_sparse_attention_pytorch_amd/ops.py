@@ -3138,10 +3138,10 @@ def cache8_select_attend(q: Tensor, cache: Cache8, lengths, block: int, idx: Ten
 
 
 @functools.lru_cache(maxsize=256)
-def _logits_plan(logits, history, history_lengths, bias, allowed, numbers, values):
+def _logits_plan(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values):
     """(descriptor up to `history` and behind it, which of the operands have to be laid out first) of these layouts; `history`: (shape up to its tokens, type,
-    whether it is contiguous), since a sequence has one more of them at each step; `numbers`: of the four tensors that may stand for values."""
-    name = "adjust_logits"
+    whether it is contiguous), since a sequence has one more of them at each step; the last four: of the tensors that may stand for values."""
+    name, numbers = "adjust_logits", (repetition, frequency, presence, temperature)
     shape, stride, dtype = logits
     if dtype not in _LOSS_TYPES or len(shape) < 1 or shape[-1] == 0:
         raise RuntimeError(f"{name}: logits {dtype} {tuple(shape)}: expected bf16, fp16 or fp32 '... v'")
@@ -3210,16 +3210,21 @@ def _strides_of(shape):
 
 
 def _adjust_logits(logits, history, history_lengths, bias, allowed, repetition, frequency, presence, temperature, values):
-    device = logits.get_device()
-    given = history, history_lengths, bias, allowed, repetition, frequency, presence, temperature
-    if device < 0 or any([t is not None and t.get_device() != device for t in given]):
-        raise RuntimeError("adjust_logits: needs tensors on one GPU (HIP kernels, no CPU fallback)")
-    tokens, past = 0, None
+    device, elsewhere, layouts = logits.get_device(), False, []
+    for t in (history_lengths, bias, allowed, repetition, frequency, presence, temperature):
+        if t is None:
+            layouts.append(None)
+        else:
+            elsewhere |= t.get_device() != device
+            layouts.append((t.shape, t.stride(), t.dtype))
+    past, tokens = None, 0
     if history is not None:
-        past = history.shape[:-1] if history.dim() else None, history.dtype, history.is_contiguous()
-        tokens = history.shape[-1] if history.dim() else 0
-    head, tail, fixes, any_fix = _logits_plan(_layout(logits), past, _layout(history_lengths), _layout(bias), _layout(allowed),
-                                              (_layout(repetition), _layout(frequency), _layout(presence), _layout(temperature)), tuple(values))
+        elsewhere |= history.get_device() != device
+        size = history.shape
+        past, tokens = (size[:-1] if size else None, history.dtype, history.is_contiguous()), size[-1] if size else 0
+    if device < 0 or elsewhere:
+        raise RuntimeError("adjust_logits: needs tensors on one GPU (HIP kernels, no CPU fallback)")
+    head, tail, fixes, any_fix = _logits_plan((logits.shape, logits.stride(), logits.dtype), past, *layouts, tuple(values))
     out = torch.empty_like(logits, dtype=torch.float32, memory_format=torch.contiguous_format)
     if not out.numel():
         return out
@@ -3230,7 +3235,7 @@ def _adjust_logits(logits, history, history_lengths, bias, allowed, repetition, 
         logits, history = logits.contiguous() if fixes[0] else logits, history.contiguous() if fixes[1] else history
         history_lengths = _int32(history_lengths).contiguous() if fixes[2] else history_lengths
         bias, allowed = bias.float().contiguous() if fixes[3] else bias, allowed.contiguous() if fixes[4] else allowed
-        repetition, frequency, presence, temperature = (t.float().contiguous() if fix else t for t, fix in zip(given[4:], fixes[5]))
+        repetition, frequency, presence, temperature = (t.float().contiguous() if fix else t for t, fix in zip((repetition, frequency, presence, temperature), fixes[5]))
     _lib.check(_lib.lib().nsa_adjust_logits(head + tokens.to_bytes(8, "little") + tail, logits.data_ptr(), _ptr(history), _ptr(history_lengths), _ptr(repetition),
                                             _ptr(frequency), _ptr(presence), _ptr(bias), _ptr(allowed), _ptr(temperature), out.data_ptr(), _stream()), "nsa_adjust_logits")
     return out
