@@ -6,9 +6,10 @@
 // block's new rows are held in registers in between, 32 values a lane, by one wave up to 2048 values and by up to eight for 128 rows of 128.  A
 // block that holds rows already is read too, and its rows are written again only where the scale grows.
 //
-// Measured: a prompt of 30011 tokens, 4 heads of 64 bf16 features, 11.4 us (46 MB: 4.1 TB/s; a copy of as much takes 10); six chunks of 1021 tokens, 5
-// heads of 128 fp32 features, 8.7 us (31 MB); one token for each of 64 sequences, 8 heads, 4.3 us, most of it the launch.  Blocks that are new as a whole have
-// loads without a branch between them (with the test of each row 12.7 and 9.4 us; with rows outside read as their neighbours in all blocks 12.1, 8.6 and 4.6).
+// Measured in a trace: a prompt of 30011 tokens, 4 heads of 64 bf16 features, 11.6 us (46 MB: 4.0 TB/s; a copy of as much takes 10); six chunks of 1021 tokens, 5
+// heads of 128 fp32 features, 8.8 us (31 MB); one token for each of 64 sequences, 8 heads, 4.6 us, most of it the launch.  Blocks that are new as a whole have
+// loads without a branch between them (replayed from a graph 11.4, 8.7 and 4.3 us; with the test of each row 12.7 and 9.4; with rows outside read as their neighbours in
+// all blocks 12.1, 8.6 and 4.6).
 #include "nsa_cache8.hpp"
 
 namespace nsa {

@@ -11,12 +11,13 @@
 //     holds D / 16 consecutive features of those eight keys: bytes are transposed four by four (v_perm) and converted in pairs.
 // Codes become bf16 exactly; a key's scale goes into the conversion, a value's into its probability, both powers of two.  Queries are sums of bf16
 // parts (one of bf16, two of fp16, three of fp32: exact), probabilities of two (three for fp32 results): 2^-17 (2^-24) of each.  At 16 columns
-// the matrix cores have the time for it: they are busy for 5 to 12 % of the times below.
+// the matrix cores have the time for it: they are busy for up to 12 % of the times below.  Two parts for results of 16 bits: of 32768 in bf16 some 47 then round the other
+// way than with exact probabilities, with three some 11, which 17 tiles of 64 features do not get for nothing (10.3 us instead of 9.9; 32768 keys 20.2 instead of 20.0).
 //
-// Measured (this kernel, then the merge of the shares; a copy reaches 4.7 TB/s): one sequence of 524287 keys, 16 heads on 2 of 128 features, 51 us
-// (5.3 TB/s) and 6; of 32768 keys, 32 heads on 8, 16 us (4.1 TB/s) and 4; 48 sequences of 1 to 16384 keys, 38 us (4.5 TB/s) and 5; 16 blocks of 64 keys
-// and the newest of 32 sequences, 16 heads on 4 of 64 features, 10 us, and of one sequence, 32 heads on 8 of 128, 11 us: a few CUs have it all, and one
-// takes 64 KB in 1.4 us, by eight waves or by sixteen (11.2 us).
+// Measured in a trace (this kernel, then the merge of the shares; a copy reaches 4.7 TB/s): one sequence of 524287 keys, 16 heads on 2 of 128 features, 51.1 us
+// (5.3 TB/s) and 5.8; of 32768 keys, 32 heads on 8, 16.5 us (4.1 TB/s) and 4.0; 48 sequences of 1 to 16384 keys, 38.7 us (4.4 TB/s) and 4.8; 16 blocks of 64 keys
+// and the newest of 32 sequences, 16 heads on 4 of 64 features, 10.0 us, and of one sequence, 32 heads on 8 of 128, 11.2 us: a few CUs have it all, and one
+// takes 64 KB in 1.4 us, by eight waves or by sixteen (the same within 0.2 us).
 // More than 16 query heads of a kv head are two groups of columns, each converted for by waves of its own: 26 sequences of 3 to 9339 keys, 4 kv heads, take
 // 30 us with 32 query heads each and 23 with 16.
 #include <type_traits>
@@ -56,9 +57,10 @@ constexpr int kTile = 32, kTable = 2048, kListed = 64;      // kTable: sequences
 // see Shares.  kUnit: of 4, 48 ragged sequences take 55 us instead of 47; of 12, 48.  kShare: of 16, 57 to 125 tiles of 8 units take 12.0 to 13.6 us instead of
 // 10.1 to 10.5
 constexpr int kUnit = 8, kShare = 4;
-// Tiles of a unit up to which it has a work-group for itself and no merge follows.  us alone / shared: of 128 features, 34 tiles of 8 units 11.5 / 10.3, 50 tiles 14.3 /
-// 10.4, 42 of 64 units 14.1 / 14.5, 50 tiles 15.7 / 15.3; of 64 features, 50 of 16 units 10.4 / 11.3; 41 of 512 units of lengths from 10 keys on 14 / 21, 91 tiles
-// 23 / 25, 125 tiles 31 / 28.  These are calls replayed from a graph; by itself a call is the host's, and a second launch and a workspace take it from 11 to 15.5.
+// Tiles of a unit up to which it has a work-group for itself and no merge follows.  us alone / shared, replayed from a graph and, in brackets, as calls: of 128 features
+// and scales of 32 rows, 34 tiles of 8 units 11.5 / 10.4 (11.2 / 15.4), 50 tiles 14.4 / 10.4 (13.7 / 15.1), 42 of 64 units 14.1 / 14.8 (13.1 / 14.8), 50 tiles 15.8 / 15.3
+// (14.7 / 14.9); of 64 features, 50 of 16 units 11.6 / 9.6 (11.1 / 14.9); 41 of 512 units of lengths from 10 keys on 14.3 / 21.4 (13.1 / 20.2), 91 tiles 23.3 / 25.2 (22.1 /
+// 23.8), 125 tiles 30.5 / 28.4 (29.4 / 27.0).  With few units the kernels alone would be shared from 34 tiles on; a call has a second launch and a workspace more then.
 __host__ inline int alone_up_to(long units) { return units >= 256 ? 96 : 50; }
 
 __device__ __forceinline__ floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }

@@ -982,7 +982,7 @@ extern "C" int nsa_decode_step_dyn(const nsa_decode_step_desc* cap, int32_t* sta
 // work-groups make the selection; merge and gate.  (A block's scale may grow with its newest row, and with it what is held of the others: the row goes into the
 // cache before anything attends it, where a bf16 row goes in beside the window's attention.  Blocks of other than 1, 2, 4 .. 32 compressed keys: as in
 // the bf16 step a launch more, for their top-k.)  32 heads of 128 features on 8, 32k tokens of context, us of a whole step of the layer at batch 1, 8 and 32:
-// 52, 73 and 130, over a bf16 cache of twice the size 50, 75 and 136.
+// 51, 73 and 130, over a bf16 cache of twice the size 50, 75 and 136; the three kernels in a trace 8.7, 10.6 and 5.1, 19.0, 13.4 and 6.1, 51.6 (270 MB: 5.2 TB/s), 29.1 and 7.4.
 namespace nsa {
 
 template <int D, int ROLE>

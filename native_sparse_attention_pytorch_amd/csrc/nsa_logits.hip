@@ -4,8 +4,8 @@
 // into LDS - the tokens that fall into the slice, by integer additions, so that their order changes nothing - and then passes over the slice: no
 // counts in memory and one launch, for a history that every slice reads again (from L2).
 //
-// Measured: 64 rows of 128000 bf16 logits, 4096 tokens of history, a bit mask, 16.7 us (52 MB: 3.1 TB/s; 11 without history and mask: all work-groups are on the
-// chip at once and write only when they have counted); 300 rows of 50021 fp32 ones with a bias, 34 us (137 MB: 4.0 TB/s); 8 rows of 256, 4.6 us.
+// Measured in a trace: 64 rows of 128000 bf16 logits, 4096 tokens of history, a bit mask, 16.6 us (52 MB: 3.1 TB/s; 11 without history and mask: all work-groups are on the
+// chip at once and write only when they have counted); 300 rows of 50021 fp32 ones with a bias, 34.2 us (137 MB: 4.0 TB/s); 8 rows of 256, 4.6 us.
 // Slices of 256 threads are up to 2 us faster with a history of some hundred tokens (300 rows of 50021: 24.6 and 25.7) and slower with thousands (256 rows of
 // 32000 with 4096: 20.4 and 16.8).  Asking for the history before the entries changed nothing (17.3 and 33.9 us), and neither did divisions of five instructions by reciprocals (17.3 and
 // 34.4): neither the one wait nor the arithmetic is what it waits for.
